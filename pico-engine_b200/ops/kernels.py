@@ -1887,3 +1887,180 @@ def route_rows(h: torch.Tensor, router: torch.Tensor, n_outputs: int, n_experts:
                                  0 if correction is None else _code(correction, "correction"), top_k, float(factor), out.data_ptr(), _ptr(ids), T,
                                  stream_ptr()), "route_rows")
     return out
+
+
+# ---------------------------------------------------------------------------- several answers to a prompt
+
+SHARED_HEAD_DIMS = (64, 128)
+
+
+def _need_here(t: torch.Tensor, name: str) -> None:
+    """The launch goes to the current device's stream: its tensors have to lie there."""
+    if t.get_device() != torch.cuda.current_device():
+        raise KernelError(f"{name} lives on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def attention_shared_takes(dtype: torch.dtype, n_heads: int, n_kv_heads: int, head_dim: int, scale: float) -> bool:
+    return dtype == torch.bfloat16 and head_dim in SHARED_HEAD_DIMS and scale > 0 and n_heads // n_kv_heads <= 128
+
+
+def shared_group_rows(members):
+    """``groups`` of ``attention_shared`` for the rows of a step, on the host: ``members`` lists (tokens, shared positions, which of them
+    has the least position) group after group, in the order of the rows; a row on its own is (1, 0, 0)."""
+    rows, at = [], 0
+    for n, shared, lead in members:
+        if n < 1 or shared < 0 or shared % PAGE or not 0 <= lead < n:
+            raise KernelError(f"a group of {n} tokens that share {shared} positions, led by its token {lead}: shared positions are whole pages of {PAGE}")
+        rows.extend([(at, n, shared, at + lead)] * n)
+        at += n
+    return rows
+
+
+def shared_groups(members, device) -> torch.Tensor:
+    """``shared_group_rows`` as int32 [T, 4] on ``device``."""
+    return torch.tensor(shared_group_rows(members), dtype=torch.int32).view(-1, 4).to(device, non_blocking=True)
+
+
+def attention_shared(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int, head_dim: int, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                     block_table: torch.Tensor, table_stride: int, tok_pos: torch.Tensor, tok_row: torch.Tensor, groups: torch.Tensor,
+                     window: Optional[int], scale: float, max_context: int, out: Optional[torch.Tensor] = None, keep_first: int = 0,
+                     slopes: Optional[torch.Tensor] = None, sinks: Optional[torch.Tensor] = None, early_pages: bool = True) -> torch.Tensor:
+    """``attention_decode`` for single tokens of which several share the first pages of their sequences: those pages are read once for
+    all rows of a group.  ``groups`` int32 [T, 4], a row a token (``shared_groups``): the first token of its group, how many consecutive tokens the
+    group has, how many positions they share (whole pages, no more than the least position of the group; 0: none), and which token has
+    the least position: its row of the page table names the shared pages.  Head sizes 64 and 128 (``attention_shared_takes``); results are
+    those of ``attention_decode`` up to the order of float32 sums."""
+    from .library import for_head_dim
+    T = tok_pos.shape[0]
+    _need(q, "q", torch.bfloat16); _need(k_pool, "k_pool", torch.bfloat16); _need(v_pool, "v_pool", torch.bfloat16, k_pool.shape)
+    if not attention_shared_takes(q.dtype, n_heads, n_kv_heads, head_dim, scale) or n_heads % n_kv_heads:
+        raise KernelError(f"attention_shared takes head sizes {SHARED_HEAD_DIMS}, a positive scale and at most 128 query heads a key head, not "
+                          f"{n_heads} / {n_kv_heads} heads of {head_dim}, scale {scale}")
+    if k_pool.dim() != 4 or tuple(k_pool.shape[1:]) != (n_kv_heads, PAGE, head_dim):
+        raise KernelError(f"cache pool must be [pages, {n_kv_heads}, {PAGE}, {head_dim}], not {tuple(k_pool.shape)}")
+    _need(block_table, "block_table", torch.int32)
+    _need(tok_pos, "tok_pos", torch.int32, (T,)); _need(tok_row, "tok_row", torch.int32, (T,)); _need(groups, "groups", torch.int32, (T, 4))
+    if q_stride % 8 or q_stride < n_heads * head_dim or (T and q.numel() < (T - 1) * q_stride + n_heads * head_dim):
+        raise KernelError(f"q must hold {T} rows of {n_heads * head_dim} numbers, {q_stride} (a multiple of 8) apart")
+    if max_context < 1 or keep_first < 0 or (window is not None and window < 0) or groups.data_ptr() % 16:
+        raise KernelError("max_context must be positive, window and keep_first not negative, and groups start on a 16-byte boundary")
+    if slopes is not None:
+        _need(slopes, "slopes", torch.float32, (n_heads,))
+    if sinks is not None:
+        _need(sinks, "sinks", torch.float32, (n_heads,))
+    if out is None:
+        out = torch.empty(T, n_heads * head_dim, dtype=torch.bfloat16, device=q.device)
+    _need(out, "out", torch.bfloat16, (T, n_heads * head_dim))
+    _need_here(q, "q")
+    lib = for_head_dim(head_dim)
+    check(lib.pe_attention_shared(q.data_ptr(), q_stride, out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_pool.shape[0], block_table.data_ptr(),
+                                  table_stride, tok_pos.data_ptr(), tok_row.data_ptr(), groups.data_ptr(), T, n_heads, n_kv_heads, head_dim, window or 0,
+                                  keep_first if window else 0, scale, max_context, _ptr(slopes), _ptr(sinks), 1 if early_pages else 0, None,
+                                  status_ptr(q.device), stream_ptr()), "attention_shared")
+    return out
+
+
+def adjust_logits(logits: torch.Tensor, slots: Optional[torch.Tensor] = None, history: Optional[torch.Tensor] = None,
+                  penalties: Optional[torch.Tensor] = None, bias_range: Optional[torch.Tensor] = None, bias_ids: Optional[torch.Tensor] = None,
+                  bias_values: Optional[torch.Tensor] = None, masks: Optional[torch.Tensor] = None, mask_rows: Optional[torch.Tensor] = None,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The rules on what may be chosen next, on float32 logits [B, V]; returns ``out`` (a new tensor, or ``logits`` itself to change them in place).
+
+    ``history`` int16 [n, V] with ``slots`` int32 [B] (its row of each batch row) and ``penalties`` float32 [B, 3] (repetition, presence, frequency):
+    the sign bit of an entry says that the token stands in the prompt, the other 15 bits how often it has been generated (``note_tokens``).
+    Seen tokens' logits are divided by the repetition penalty where positive and multiplied by it elsewhere; generated ones lose
+    presence + count * frequency.  ``bias_range`` int32 [B, 2]: from where to where row b's biases lie in ``bias_ids`` (int32) and ``bias_values``
+    (float32); a token that stands there twice gets both.  ``masks`` int32 [M, ceil(V / 32)] with ``mask_rows`` int32 [B]: where bit v % 32 of word
+    v / 32 of row b's mask is 0, the logit becomes -inf, whatever it was; -1: no mask.  A row that its mask leaves nothing is -inf everywhere."""
+    if logits.dim() != 2:
+        raise KernelError(f"logits must be [rows, vocabulary], not {tuple(logits.shape)}")
+    B, V = logits.shape
+    _need(logits, "logits", torch.float32)
+    n = n_bias = n_masks = 0
+    if (history is None) != (penalties is None) or (history is not None and slots is None):
+        raise KernelError("history, slots and penalties go together")
+    if history is not None:
+        n = history.shape[0]
+        _need(history, "history", torch.int16, (n, V)); _need(slots, "slots", torch.int32, (B,)); _need(penalties, "penalties", torch.float32, (B, 3))
+    if (bias_range is None) != (bias_ids is None) or (bias_ids is None) != (bias_values is None):
+        raise KernelError("bias_range, bias_ids and bias_values go together")
+    if bias_ids is not None:
+        n_bias = bias_ids.shape[0]
+        _need(bias_ids, "bias_ids", torch.int32, (n_bias,)); _need(bias_values, "bias_values", torch.float32, (n_bias,))
+        _need(bias_range, "bias_range", torch.int32, (B, 2))
+        if bias_range.data_ptr() % 8:
+            raise KernelError("bias_range must start on an 8-byte boundary")
+    if (masks is None) != (mask_rows is None):
+        raise KernelError("masks and mask_rows go together")
+    if masks is not None:
+        n_masks = masks.shape[0]
+        _need(masks, "masks", torch.int32, (n_masks, (V + 31) // 32)); _need(mask_rows, "mask_rows", torch.int32, (B,))
+    if out is None:
+        out = torch.empty_like(logits)
+    _need(out, "out", torch.float32, (B, V))
+    if B == 0 or V == 0:
+        return out
+    if B > 65535:
+        raise KernelError(f"adjust_logits takes at most 65,535 rows, not {B}")
+    _need_here(logits, "logits")
+    from .library import answers
+    check(answers().pe_adjust_logits(logits.data_ptr(), out.data_ptr(), B, V, _ptr(slots), _ptr(history), n, _ptr(penalties), _ptr(bias_range),
+                                     _ptr(bias_ids) if n_bias else None, _ptr(bias_values), n_bias, _ptr(masks) if n_masks else None, n_masks,
+                                     _ptr(mask_rows), stream_ptr()), "adjust_logits")
+    return out
+
+
+def note_tokens(history: Optional[torch.Tensor], slots: torch.Tensor, tokens: torch.Tensor, prompt: bool = False,
+                states: Optional[torch.Tensor] = None, transitions: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Tokens (int32 [N]) of the sequences ``slots`` (int32 [N]) into ``history`` (int16 [n, V], in place): ``prompt`` marks them as the prompt's, else
+    their counts go up by one (and stay at 32,767).  ``states`` int32 [n] with ``transitions`` int32 [S, V]: the state of each sequence's token
+    automaton follows its tokens, in their order; -1 stays -1, and is what a token leads to that the state does not allow.  Slots and tokens that
+    are outside the tables change nothing (a token outside the automaton's leads to -1)."""
+    if tokens.dim() != 1:
+        raise KernelError(f"tokens must be one row, not {tuple(tokens.shape)}")
+    N = tokens.shape[0]
+    _need(tokens, "tokens", torch.int32); _need(slots, "slots", torch.int32, (N,))
+    if (states is None) != (transitions is None) or (history is None and states is None):
+        raise KernelError("note_tokens needs a history, or states with their transitions, or both")
+    n = history.shape[0] if history is not None else states.shape[0]
+    V = history.shape[-1] if history is not None else transitions.shape[-1]
+    if history is not None:
+        _need(history, "history", torch.int16, (n, V))
+    n_states = 0
+    if states is not None:
+        n_states = transitions.shape[0]
+        _need(states, "states", torch.int32, (n,)); _need(transitions, "transitions", torch.int32, (n_states, V))
+    if N == 0 or n == 0:
+        return history
+    _need_here(tokens, "tokens")
+    from .library import answers
+    check(answers().pe_note_tokens(_ptr(history), n, V, slots.data_ptr(), tokens.data_ptr(), N, 1 if prompt else 0, _ptr(states), _ptr(transitions), n_states,
+                                   stream_ptr()), "note_tokens")
+    return history
+
+
+def step_tables(slots: torch.Tensor, starts: torch.Tensor, lens: torch.Tensor, held: torch.Tensor, pages: torch.Tensor, resident: torch.Tensor,
+                tok_pos: torch.Tensor, tok_row: torch.Tensor, row_first: torch.Tensor, places: torch.Tensor, tables: torch.Tensor):
+    """The layout of a step from the lengths of its requests (all int32).  Row b brings ``lens[b]`` tokens of the sequence with row ``slots[b]``
+    of the ``resident`` page table [n, R], from position ``starts[b]`` on; the first ``held[b]`` entries of that row are known, and the ones missing
+    for the row's new length are the next numbers of ``pages`` (rows in their order; they are written into ``resident``).  Fills ``tok_pos``, ``tok_row`` and
+    ``places`` (page * 64 + position % 64) [T] for every token, ``row_first`` [B + 1] and ``tables`` [B, W] (-1 behind a row's last page, and for
+    pages that are not there); entries of the first three behind the last token stay as they are.  Returns those five.  Rows of one call that name
+    the same slot must bring no new pages."""
+    if tables.dim() != 2 or resident.dim() != 2:
+        raise KernelError("resident and tables must be page tables, a row a sequence")
+    B, T = slots.shape[0], tok_pos.shape[0]
+    for t, name in ((slots, "slots"), (starts, "starts"), (lens, "lens"), (held, "held")):
+        _need(t, name, torch.int32, (B,))
+    _need(pages, "pages", torch.int32, (pages.numel(),)); _need(resident, "resident", torch.int32)
+    for t, name in ((tok_pos, "tok_pos"), (tok_row, "tok_row"), (places, "places")):
+        _need(t, name, torch.int32, (T,))
+    _need(row_first, "row_first", torch.int32, (B + 1,)); _need(tables, "tables", torch.int32, (B, tables.shape[1]))
+    if B == 0:
+        raise KernelError("a step needs at least one row")
+    _need_here(slots, "slots")
+    from .library import answers
+    check(answers().pe_step_tables(slots.data_ptr(), starts.data_ptr(), lens.data_ptr(), held.data_ptr(), pages.data_ptr(), pages.shape[0],
+                                   resident.data_ptr(), resident.shape[0], resident.shape[1], B, tok_pos.data_ptr(), tok_row.data_ptr(),
+                                   row_first.data_ptr(), places.data_ptr(), T, tables.data_ptr(), tables.shape[1], stream_ptr()), "step_tables")
+    return tok_pos, tok_row, row_first, places, tables

@@ -31,7 +31,9 @@ STATE_SOURCES = ("state_space.cu", "state_space_tiles.cu", "state_space_tcgen05.
 # The kernels of sublayers that read the same rows and share their first and last product, of heads with several maps, and of routers
 # that read normed rows.
 JOINED_SOURCES = ("joined_ops.cu", "attention_diff.cu", "attention_diff_tcgen05.cu")
-HEAD_DIM_SOURCES = ("attention_decode.cu", "attention_prefill.cu", "attention_prefill_tcgen05.cu")      # compiled per head size
+# The kernels of several answers to a prompt and of rules on what may be chosen: logits under penalties, biases and masks, and the tables of a step.
+ANSWER_SOURCES = ("logit_rules.cu", "step_tables.cu")
+HEAD_DIM_SOURCES = ("attention_decode.cu", "attention_prefill.cu", "attention_prefill_tcgen05.cu", "attention_shared.cu")      # compiled per head size
 
 _SIGNATURES = {
     "pe_embed": [P, I, P, P, I, I, I, F, P],
@@ -132,7 +134,14 @@ _EXTRA_SIGNATURES = {
     "pe_batch_norm_qkv_rope_store": [P, P, I, F, P, P, I, P, I, I, I, I, I, P, P, P, P, P, P, P, I, I, P, P],
 }
 
+_ANSWER_SIGNATURES = {
+    "pe_adjust_logits": [P, P, I, I, P, P, I, P, P, P, P, I, P, I, P, P],
+    "pe_note_tokens": [P, I, I, P, P, I, I, P, P, I, P],
+    "pe_step_tables": [P, P, P, P, P, I, P, I, I, I, P, P, P, P, I, P, I, P],
+}
+
 _HEAD_DIM_SIGNATURES = {
+    "pe_attention_shared": [P, I, P, P, P, LL, P, I, P, P, P, I, I, I, I, I, I, F, I, P, P, I, P, P, P],
     "pe_attention_decode": [P, I, P, P, P, P, I, P, P, I, I, I, I, I, F, I, I, P, P, I, P, P],
     "pe_attention_decode_splits": [I, I, I, I, P],
     "pe_attention_prefill": [P, I, P, P, P, P, I, P, P, P, I, I, I, I, I, F, P],
@@ -258,6 +267,20 @@ def joined() -> ctypes.CDLL:
         lib.pe_set_pdl(0 if os.environ.get("PICO_ENGINE_PDL", "1") == "0" else 1)
         _joined = lib
     return _joined
+
+
+_answers = None
+
+
+def answers() -> ctypes.CDLL:
+    """The library of the kernels of several answers to a prompt and of rules on what may be chosen; compiled at the first call."""
+    global _answers
+    if _answers is None:
+        lib = build.load("answers", ANSWER_SOURCES)
+        declare(lib, _ANSWER_SIGNATURES)
+        lib.pe_set_pdl(0 if os.environ.get("PICO_ENGINE_PDL", "1") == "0" else 1)
+        _answers = lib
+    return _answers
 
 
 _extras = None
