@@ -29,7 +29,7 @@
 #ifndef PE_HEAD_DIM
 #error "compile with -DPE_HEAD_DIM=<head size>"
 #endif
-#include "common.cuh"
+#include "attention_shared.cuh"
 #include <map>
 #include <mutex>
 #include <utility>
@@ -221,12 +221,50 @@ __device__ __forceinline__ void ad_consume(float (&acc)[AD_NCHUNK][4][4], float 
     }
 }
 
-template <int AD_WARPS>
+// What the joined form (OWN) has to know: the groups of the step's tokens and where attention_shared.cu has left its partial results.
+struct AdGroups { const int4* groups; AsScratch scratch; int T, grid; };
+
+// The results of the group's positions for row `row` (query head of the key head) and column `col`, joined to (m, l, o).
+struct AdJoin {
+    int c0, c1;                                     // the CTAs that had steps of this token's tile: c0 .. c1 - 1
+    size_t row0;
+    __device__ AdJoin(const AdGroups& p, const int4& g, int tok, int shared, int pos, int window, int keep_first, int nh, int nkv, int kvh) : c0(0), c1(0), row0(0) {
+        if (shared == 0) return;
+        const int R = nh / nkv, per_tile = AS_QTILE / R, i = tok - g.x, tiles = (g.y + per_tile - 1) / per_tile;
+        const int n_steps = (as_pages(shared, pos, window, keep_first).n + 1) / 2;
+        if (n_steps == 0) return;
+        const long long steps = p.scratch.before[p.T], first = p.scratch.before[g.x] + ((long long)kvh * tiles + i / per_tile) * n_steps;
+        const int ctas = as_ctas(steps, p.grid);
+        c0 = as_cta_of(first, steps, ctas);
+        c1 = as_cta_of(first + n_steps - 1, steps, ctas) + 1;
+        row0 = as_row(0, g, nh, nkv, kvh, i * R);
+    }
+    __device__ void join(const AdGroups& p, int row, int col, float& m, float& l, float& o) const {
+        float top = m;
+        for (int c = c0; c < c1; ++c) {
+            const float4 e = p.scratch.ends[row0 + row + (size_t)c * AS_QTILE];
+            top = fmaxf(top, fmaxf(e.x, e.z));
+        }
+        if (top == -INFINITY) return;
+        const auto weight = [&](float at) { return at == -INFINITY ? 0.f : exp2f(at - top); };
+        const float own = weight(m);
+        l *= own; o *= own; m = top;
+        for (int c = c0; c < c1; ++c) {
+            const size_t at = row0 + row + (size_t)c * AS_QTILE;
+            const float4 e = p.scratch.ends[at];
+            l = fmaf(e.y, weight(e.x), fmaf(e.w, weight(e.z), l));
+            o = fmaf(p.scratch.sums[at * AD_HD + col], weight(fmaxf(e.x, e.z)), o);
+        }
+    }
+};
+
+// OWN: a token reads the positions behind those that it shares with its group (everything below counts from there), and joins the group's results.
+template <int AD_WARPS, bool OWN>
 __global__ void __launch_bounds__(32 * (AD_WARPS + 1), AD_CTAS(AD_WARPS)) attention_decode_kernel(
     const bf16* q, int q_stride, const bf16* k_pool, const bf16* v_pool,
     const int* block_table, int table_stride, const int* tok_pos,
     const int* tok_row, int nh, int nkv, int window, float scale_log2e, int n_splits, int stages,
-    int* status, bf16* out, int keep_first, const float* slopes, const float* sinks) {
+    int* status, bf16* out, int keep_first, const float* slopes, const float* sinks, const AdGroups grouped) {
     constexpr int AD_GROUPS = AD_WARPS / 4, AD_THREADS = 32 * (AD_WARPS + 1);
     extern __shared__ __align__(128) unsigned char ad_smem[];   // result rows, then the ring (later: the warps' partial results)
     __shared__ __align__(8) unsigned long long bars[2 * AD_MAX_STAGES + 1];
@@ -240,8 +278,19 @@ __global__ void __launch_bounds__(32 * (AD_WARPS + 1), AD_CTAS(AD_WARPS)) attent
     const int G = nh / nkv, head_tiles = (G + 15) / 16;
     const int kvh = blockIdx.y / head_tiles, ht = blockIdx.y % head_tiles;
     // positions and page tables were uploaded before the step began: they may be read before the wait
-    const int pos = tok_pos[tok];
+    int pos = tok_pos[tok];
     const int* table = block_table + (size_t)tok_row[tok] * table_stride;
+    int4 group = make_int4(0, 0, 0, 0);
+    int shared = 0;
+    const int kept_keys = keep_first;
+    if constexpr (OWN) {
+        group = grouped.groups[tok];
+        shared = as_shared(group, tok, grouped.T, table_stride);
+        const int skip = min(shared, pos / PE_PAGE * PE_PAGE);
+        pos -= skip;
+        table += skip / PE_PAGE;
+        keep_first = max(keep_first - skip, 0);
+    }
     const int lo = (window > 0 && pos - window + 1 > 0) ? pos - window + 1 : 0;
     // The pages a token reads, in the order they are visited: those of the sequence's first keep_first keys where the window
     // has left them behind, then the window's.  Entry v of that list is page v (v < kept_pages) or first_page + v - kept_pages.
@@ -420,6 +469,14 @@ __global__ void __launch_bounds__(32 * (AD_WARPS + 1), AD_CTAS(AD_WARPS)) attent
     }
     __syncthreads();
     if (n_splits > 1) ad_cluster_wait();                     // every CTA of the cluster has set up its barrier
+    const auto joined = [&] {
+        if constexpr (OWN) {
+            pdl_wait();                                      // (the producer has not waited for the kernel in front)
+            return AdJoin(grouped, group, tok, shared, window > 0 && shared ? tok_pos[group.w] : 0, window, kept_keys, nh, nkv, kvh);
+        } else {
+            return 0;
+        }
+    }();
     for (int idx = threadIdx.x; idx < rows * AD_HD; idx += AD_THREADS) {
         const int row = idx / AD_HD, col = idx % AD_HD;
         const float m = row_max[row];
@@ -430,8 +487,10 @@ __global__ void __launch_bounds__(32 * (AD_WARPS + 1), AD_CTAS(AD_WARPS)) attent
             l += w_sum[w * 16 + row];
         }
         if (n_splits == 1) {
+            float m_all = m;
+            if constexpr (OWN) joined.join(grouped, ht * 16 + row, col, m_all, l, o);
             // sinks [nh] (or null): one more place of that score joins the head's denominator and carries no value
-            if (sinks) l += exp2f(fmaf(sinks[kvh * G + ht * 16 + row], 1.4426950408889634f, -m));
+            if (sinks) l += exp2f(fmaf(sinks[kvh * G + ht * 16 + row], 1.4426950408889634f, -m_all));
             out[((size_t)tok * nh + kvh * G + ht * 16 + row) * AD_HD + col] = __float2bfloat16_rn(l > 0.f ? o / l : 0.f);
             continue;
         }
@@ -470,6 +529,7 @@ __global__ void __launch_bounds__(32 * (AD_WARPS + 1), AD_CTAS(AD_WARPS)) attent
             o = fmaf(src[j], wgt, o);
             l = fmaf(src[slice + 1], wgt, l);
         }
+        if constexpr (OWN) joined.join(grouped, ht * 16 + row, split * slice + j, m, l, o);
         if (sinks) l += exp2f(fmaf(sinks[kvh * G + ht * 16 + row], 1.4426950408889634f, -m));
         out[((size_t)tok * nh + kvh * G + ht * 16 + row) * AD_HD + split * slice + j] = __float2bfloat16_rn(l > 0.f ? o / l : 0.f);
     }
@@ -482,7 +542,7 @@ extern "C" void pe_set_pdl(int on) { pe_pdl_enabled() = on ? 1 : 0; }
 // live in one process, and the function-local statics of a template with external linkage would be one
 // object for all of them (the dynamic linker makes such symbols unique across libraries).
 namespace {
-template <int WARPS>
+template <int WARPS, bool OWN = false>
 struct AdVariant {
     static constexpr int threads = 32 * (WARPS + 1), groups = WARPS / 4, ctas_per_sm = AD_CTAS(WARPS);
 
@@ -497,16 +557,16 @@ struct AdVariant {
         static bool wide = false;
         if (!allowed) {
             cudaFuncAttributes own;
-            PE_TRY(cudaFuncGetAttributes(&own, attention_decode_kernel<WARPS>));
+            PE_TRY(cudaFuncGetAttributes(&own, attention_decode_kernel<WARPS, OWN>));
             allowed = 48 * 1024 - own.sharedSizeBytes;
         }
         if (!wide) {                                         // clusters of more than 8 CTAs are an opt-in; if it is refused,
-            cudaFuncSetAttribute(attention_decode_kernel<WARPS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);   // the
+            cudaFuncSetAttribute(attention_decode_kernel<WARPS, OWN>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);   // the
             cudaGetLastError();                              // occupancy query below answers 0 for them and fewer ranges are used
             wide = true;
         }
         if (smem > allowed) {
-            PE_TRY(cudaFuncSetAttribute(attention_decode_kernel<WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+            PE_TRY(cudaFuncSetAttribute(attention_decode_kernel<WARPS, OWN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
             allowed = smem;
         }
         return 0;
@@ -531,7 +591,7 @@ struct AdVariant {
             attr[0].val.clusterDim.x = splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
             cfg.attrs = attr;
             cfg.numAttrs = 1;
-            if (cudaOccupancyMaxActiveClusters(&n, attention_decode_kernel<WARPS>, &cfg) != cudaSuccess) { cudaGetLastError(); n = 0; }
+            if (cudaOccupancyMaxActiveClusters(&n, attention_decode_kernel<WARPS, OWN>, &cfg) != cudaSuccess) { cudaGetLastError(); n = 0; }
         }
         known[{splits, smem}] = n;
         return n;
@@ -564,7 +624,7 @@ struct AdVariant {
     static int launch(dim3 grid, int n_splits, int stages, cudaStream_t stream, const bf16* q, int q_stride, const bf16* k_pool,
                       const bf16* v_pool, const int* block_table, int table_stride, const int* tok_pos, const int* tok_row,
                       int nh, int nkv, int window, float scale_log2e, int* status, bf16* out, bool early, int keep_first,
-                      const float* slopes, const float* sinks) {
+                      const float* slopes, const float* sinks, const AdGroups& grouped) {
         const size_t smem = smem_bytes(stages);
         { const int e = allow_smem(smem); if (e) return e; }
         cudaLaunchConfig_t cfg = {};
@@ -586,8 +646,8 @@ struct AdVariant {
         }
         cfg.attrs = attr;
         cfg.numAttrs = n_attr;
-        PE_TRY(cudaLaunchKernelEx(&cfg, attention_decode_kernel<WARPS>, q, q_stride, k_pool, v_pool, block_table, table_stride,
-                                  tok_pos, tok_row, nh, nkv, window, scale_log2e, n_splits, stages, status, out, keep_first, slopes, sinks));
+        PE_TRY(cudaLaunchKernelEx(&cfg, attention_decode_kernel<WARPS, OWN>, q, q_stride, k_pool, v_pool, block_table, table_stride,
+                                  tok_pos, tok_row, nh, nkv, window, scale_log2e, n_splits, stages, status, out, keep_first, slopes, sinks, grouped));
         PE_LAUNCH_CHECK();
         return 0;
     }
@@ -642,6 +702,28 @@ extern "C" int pe_attention_decode_splits(int T, int nh, int nkv, int max_contex
     return c.splits;
 }
 
+namespace {
+template <bool OWN>
+int ad_run(const void* q, int q_stride, void* out, const void* k_pool, const void* v_pool, const int* block_table, int table_stride, const int* tok_pos,
+           const int* tok_row, int T, int nh, int nkv, int window, float scale, int max_context, int early_pages, int* status, void* stream, int keep_first,
+           const float* slopes, const float* sinks, const AdGroups& grouped) {
+    const int G = nh / nkv;
+    if ((long long)nkv * ((G + 15) / 16) > 65535) return PE_ERR_UNSUPPORTED;
+    const AdShape c = ad_choose(T, nh, nkv, max_context);
+    if (c.stages < 1) return PE_ERR_UNSUPPORTED;
+    const dim3 grid(c.splits, nkv * ((G + 15) / 16), T);
+    const float scale_log2e = scale * 1.4426950408889634f;
+    const auto go = [&](auto variant) {
+        return decltype(variant)::launch(grid, c.splits, c.stages, (cudaStream_t)stream, (const bf16*)q, q_stride, (const bf16*)k_pool,
+                                         (const bf16*)v_pool, block_table, table_stride, tok_pos, tok_row, nh, nkv, window, scale_log2e,
+                                         status, (bf16*)out, early_pages != 0, keep_first, slopes, sinks, grouped);
+    };
+    if constexpr (AD_HD <= 64) { if (c.warps == 16) return go(AdVariant<16, OWN>()); }
+    if constexpr (AD_HD <= 128) { if (c.warps == 4) return go(AdVariant<4, OWN>()); }
+    return go(AdVariant<8, OWN>());
+}
+}  // namespace
+
 extern "C" int pe_attention_decode(const void* q, int q_stride, void* out, const void* k_pool, const void* v_pool,
                                    const int* block_table, int table_stride, const int* tok_pos, const int* tok_row,
                                    int T, int nh, int nkv, int hd, int window, float scale, int max_context,
@@ -656,18 +738,17 @@ extern "C" int pe_attention_decode(const void* q, int q_stride, void* out, const
     if (hd != AD_HD || nkv <= 0 || nh % nkv || max_context <= 0 || q_stride % 8 || T > 65535 || !status) return PE_ERR_UNSUPPORTED;
     if (keep_first < 0 || (slopes && !(scale > 0.f))) return PE_ERR_UNSUPPORTED;
     if (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15) return PE_ERR_UNSUPPORTED;
-    const int G = nh / nkv;
-    if ((long long)nkv * ((G + 15) / 16) > 65535) return PE_ERR_UNSUPPORTED;
-    const AdShape c = ad_choose(T, nh, nkv, max_context);
-    if (c.stages < 1) return PE_ERR_UNSUPPORTED;
-    const dim3 grid(c.splits, nkv * ((G + 15) / 16), T);
-    const float scale_log2e = scale * 1.4426950408889634f;
-    const auto go = [&](auto variant) {
-        return decltype(variant)::launch(grid, c.splits, c.stages, (cudaStream_t)stream, (const bf16*)q, q_stride, (const bf16*)k_pool,
-                                         (const bf16*)v_pool, block_table, table_stride, tok_pos, tok_row, nh, nkv, window, scale_log2e,
-                                         status, (bf16*)out, early_pages != 0, keep_first, slopes, sinks);
-    };
-    if constexpr (AD_HD <= 64) { if (c.warps == 16) return go(AdVariant<16>()); }
-    if constexpr (AD_HD <= 128) { if (c.warps == 4) return go(AdVariant<4>()); }
-    return go(AdVariant<8>());
+    return ad_run<false>(q, q_stride, out, k_pool, v_pool, block_table, table_stride, tok_pos, tok_row, T, nh, nkv, window, scale, max_context, early_pages,
+                         status, stream, keep_first, slopes, sinks, AdGroups{});
 }
+
+#if AD_HD == 64 || AD_HD == 128
+// The rows' own positions, and the sum of both parts: attention_shared.cu calls it behind its own kernel.
+int pe_attention_decode_own(const void* q, int q_stride, void* out, const void* k_pool, const void* v_pool, const int* block_table, int table_stride,
+                            const int* tok_pos, const int* tok_row, int T, int nh, int nkv, int window, float scale, int max_context, int early_pages,
+                            int* status, void* stream, int keep_first, const float* slopes, const float* sinks, const void* groups, const AsScratch& scratch) {
+    if (max_context <= 0 || T > 65535) return PE_ERR_UNSUPPORTED;
+    return ad_run<true>(q, q_stride, out, k_pool, v_pool, block_table, table_stride, tok_pos, tok_row, T, nh, nkv, window, scale, max_context, early_pages,
+                        status, stream, keep_first, slopes, sinks, AdGroups{(const int4*)groups, scratch, T, pe_sm_count()});
+}
+#endif

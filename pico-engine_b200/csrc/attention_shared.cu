@@ -3,66 +3,487 @@
 //
 //   o = sum_j w_j v_j / (sum_j w_j + e^sink),   w_j = exp(scale q.k_j - slope (pos - j)),   j <= pos, j > pos - window or j < keep_first
 //
-// A warp a row and query head, a key at a time.
+// This kernel reads the shared positions, once for all rows of a group: rows (tokens x query heads of a key head) fill the 128 rows of a
+// tensor-core tile, where attention_decode.cu has the 16 of one token.  Its partial results (sums, maximum, weight of a row, in float32) go to
+// scratch, and the kernel of attention_decode.cu, which follows and reads each row's own positions, joins them:
+// m = max m_i, l = sum l_i 2^(m_i - m), o = sum o_i 2^(m_i - m).
+//
+//   a persistent CTA an SM takes an equal share of all steps (attention_shared.cuh), tile after tile
+//   warp 0      loader: the tile's queries as one box [tokens][heads of the key head][64 columns], and two pages of keys and values a step
+//   warp 1      issues S = Q.K^T three steps ahead of O += P.V, across the border of tiles
+//   warps 2-9   softmax, two warpgroups that take the steps in turn (as in attention_prefill_tcgen05.cu); at the end of a tile both write their half of O
+//
+// All keys of a step are visible to all rows but for windows, pages that are not there and the half step behind an odd number of pages, so
+// the masks are a variant of their own (MASKED).  Every wait is bounded; one that runs out sets *status to 7 and the roles leave their loops.
 #ifndef PE_HEAD_DIM
 #error "compile with -DPE_HEAD_DIM=<head size>"
 #endif
-#include "common.cuh"
+#include "tcgen05_attention.cuh"
+#include "attention_shared.cuh"
 
 #if PE_HEAD_DIM == 64 || PE_HEAD_DIM == 128
 
 #define AS_HD PE_HEAD_DIM
-#define AS_PER (AS_HD / 32)
+#define AS_KTILE (2 * PE_PAGE)                     // keys of a step
+#define AS_PANELS (AS_HD / 64)
+#define AS_STAGES (AS_HD == 64 ? 5 : 3)
+#define AS_AHEAD 3
+#define AS_THREADS 320
+#define AS_Q_BYTES (AS_QTILE * AS_HD * 2)
+#define AS_HALF_BYTES (AS_KTILE * AS_HD * 2)       // keys (or values) of a step
+#define AS_STAGE_BYTES (2 * AS_HALF_BYTES)
+#define AS_TILE_BYTES (AS_Q_BYTES + AS_STAGES * AS_STAGE_BYTES)
+#define AS_BUFFERS 3
+#define AS_BARS (4 + 3 * AS_BUFFERS + 4 * AS_STAGES + 8)
+#define AS_SMEM_BYTES (AS_TILE_BYTES + 8 * AS_BARS + 2 * AS_QTILE * 4)
+#define AS_O_COL (AS_BUFFERS * AS_KTILE)
+#define AS_LAZY 8.0f
 
-__global__ void __launch_bounds__(128) attention_shared_kernel(const bf16* q, int q_stride, bf16* out, const bf16* k_pool, const bf16* v_pool,
-                                                               const int* block_table, int table_stride, const int* tok_pos, const int* tok_row,
-                                                               int T, int nh, int nkv, int window, int keep_first, float scale,
-                                                               const float* slopes, const float* sinks) {
-    pdl_launch_dependents();
-    pdl_wait();
-    const int lane = threadIdx.x & 31, item = blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (item >= T * nh) return;
-    const int tok = item / nh, h = item % nh, kvh = h / (nh / nkv), pos = tok_pos[tok];
-    const int* table = block_table + (size_t)tok_row[tok] * table_stride;
-    float qf[AS_PER], o[AS_PER], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int i = 0; i < AS_PER; ++i) { qf[i] = to_f(q[(size_t)tok * q_stride + h * AS_HD + lane * AS_PER + i]) * scale; o[i] = 0.f; }
-    const float slope = slopes ? slopes[h] : 0.f;
-    const int lo = window > 0 ? max(0, pos - window + 1) : 0;
-    for (int j = 0; j <= pos; ++j) {
-        if (j < lo && j >= keep_first) { j = lo - 1; continue; }
-        const int page = table[j / PE_PAGE];
-        if (page < 0) continue;
-        const size_t at = (((size_t)page * nkv + kvh) * PE_PAGE + j % PE_PAGE) * AS_HD + lane * AS_PER;
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < AS_PER; ++i) s = fmaf(qf[i], to_f(k_pool[at + i]), s);
-        s = warp_sum(s) - slope * (float)(pos - j);
-        const float m_new = fmaxf(m, s), a = expf(m - m_new), w = expf(s - m_new);
-        l = fmaf(l, a, w);
-        m = m_new;
-#pragma unroll
-        for (int i = 0; i < AS_PER; ++i) o[i] = fmaf(o[i], a, w * to_f(v_pool[at + i]));
+struct AsArgs {
+    const int4* groups; const int* block_table; int table_stride; const int* tok_pos; const int* tok_row;
+    int T, nh, nkv, window, keep_first; float scale_log2e; const float* slopes; float inv_scale;
+    int pool_rows; AsScratch scratch;
+};
+
+// One tile's share of a CTA's steps, and how to come to the next.  Every role walks its own copy.
+struct AsWalk {
+    const AsArgs& p;
+    long long x, end, before, in_group;            // the next step; the CTA's last; steps in front of the group and in it
+    int t;                                         // the group's first token
+    int4 g; AsPages pages; int n_steps, tiles;
+    int kvh, tile, first, count;                   // the tile, and its steps here
+    __device__ AsWalk(const AsArgs& args) : p(args), in_group(0) {}
+    // the group that starts with token t: its steps, 0 if none starts there
+    __device__ static long long group(const AsArgs& p, int t, int4& g, AsPages& pages, int& n_steps, int& tiles) {
+        g = p.groups[t];
+        const int shared = g.x == t ? as_shared(g, t, p.T, p.table_stride) : 0;
+        if (shared == 0) return 0;
+        pages = as_pages(shared, p.window > 0 ? p.tok_pos[g.w] : 0, p.window, p.keep_first);
+        const int per_tile = AS_QTILE / (p.nh / p.nkv);
+        n_steps = (pages.n + 1) / 2;
+        tiles = (g.y + per_tile - 1) / per_tile;
+        return (long long)n_steps * tiles * p.nkv;
     }
-    if (sinks) l += expf(sinks[h] - m);
+    __device__ void start(long long from, long long to, int at, long long in_front) {
+        x = from; end = to; t = at; before = in_front;
+        in_group = group(p, t, g, pages, n_steps, tiles);
+        count = 0;
+    }
+    __device__ bool next() {
+        x += count;
+        if (x >= end) return false;
+        while (x >= before + in_group) {
+            before += in_group;
+            t += in_group > 0 ? g.y : 1;
+            in_group = group(p, t, g, pages, n_steps, tiles);
+        }
+        const long long o = x - before, seg = o / n_steps;
+        first = (int)(o - seg * n_steps);
+        kvh = (int)(seg / tiles); tile = (int)(seg - (long long)kvh * tiles);
+        count = (int)min((long long)(n_steps - first), end - x);
+        return true;
+    }
+};
+
+template <bool MASKED>
+__global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                                                                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AsArgs p, int* status) {
+    extern __shared__ __align__(1024) unsigned char as_mem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned q_s = at_smem(as_mem), kv_s = q_s + AS_Q_BYTES;
+    unsigned long long* bars = reinterpret_cast<unsigned long long*>(as_mem + AS_TILE_BYTES);
+    unsigned& tmem_base_s = *reinterpret_cast<unsigned*>(bars);
+    unsigned long long *q_full = bars + 1, *q_empty = bars + 2, *o_empty = bars + 3;
+    unsigned long long *s_full = bars + 4, *p_full = s_full + AS_BUFFERS, *pv_done = p_full + AS_BUFFERS;
+    unsigned long long *k_full = pv_done + AS_BUFFERS, *v_full = k_full + AS_STAGES, *k_empty = v_full + AS_STAGES, *v_empty = k_empty + AS_STAGES;
+    unsigned long long* told = v_empty + AS_STAGES;                 // [warpgroup][32 rows]: a step's reference points are there
+    float* refs = reinterpret_cast<float*>(bars + AS_BARS);         // [warpgroup][row]: reference point of the group's last step
+    __shared__ long long scan[AS_THREADS / 32], from_before;
+    __shared__ int from_t;
+    if (q_s & 1023u) {                                              // every thread alike: nothing is allocated yet
+        if (threadIdx.x == 0) atomicExch(status, 6);
+        return;
+    }
+    pdl_wait();
+
+    // ---- this CTA's share of the steps: a scan over the groups (a token a thread; the second time round only where there are more tokens)
+    const int grid = gridDim.x;
+    long long total = 0, begin = 0, end = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+        long long run = 0;
+        for (int base = 0; base < p.T; base += AS_THREADS) {
+            const int t = base + threadIdx.x;
+            long long mine = 0;
+            if (t < p.T) { int4 g; AsPages pages; int n_steps, tiles; mine = AsWalk::group(p, t, g, pages, n_steps, tiles); }
+            long long sum = mine;
 #pragma unroll
-    for (int i = 0; i < AS_PER; ++i) out[((size_t)tok * nh + h) * AS_HD + lane * AS_PER + i] = __float2bfloat16_rn(l > 0.f ? o[i] / l : 0.f);
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long up = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += up;
+            }
+            __syncthreads();
+            if (lane == 31) scan[warp] = sum;
+            __syncthreads();
+            long long in_front = run + sum - mine;
+#pragma unroll
+            for (int w = 0; w < AS_THREADS / 32; ++w) {
+                if (w < warp) in_front += scan[w];
+                run += scan[w];
+            }
+            if (pass == 0 && blockIdx.x == 0 && t < p.T) p.scratch.before[t] = in_front;
+            if (pass == 0 && p.T <= AS_THREADS) {                   // all groups are in hand
+                total = run;
+                const int ctas = as_ctas(total, grid);
+                if ((int)blockIdx.x < ctas) { begin = total * blockIdx.x / ctas; end = total * (blockIdx.x + 1) / ctas; }
+            }
+            if ((pass == 1 || p.T <= AS_THREADS) && mine > 0 && begin < end && begin >= in_front && begin < in_front + mine) { from_t = t; from_before = in_front; }
+        }
+        if (pass == 0) {
+            total = run;
+            const int ctas = as_ctas(total, grid);
+            if ((int)blockIdx.x < ctas) { begin = total * blockIdx.x / ctas; end = total * (blockIdx.x + 1) / ctas; }
+            if (blockIdx.x == 0 && threadIdx.x == 0) p.scratch.before[p.T] = total;
+            if (p.T <= AS_THREADS) break;
+        }
+    }
+    if (begin >= end) { pdl_launch_dependents(); return; }          // (the whole block)
+
+    if (threadIdx.x == 0) {
+        auto init = [](unsigned long long* bar, unsigned count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(at_smem(bar)), "r"(count) : "memory"); };
+        init(q_full, 1); init(q_empty, 1); init(o_empty, 8);
+        for (int s = 0; s < AS_STAGES; ++s) { init(&k_full[s], 1); init(&v_full[s], 1); init(&k_empty[s], 1); init(&v_empty[s], 1); }
+        for (int b = 0; b < AS_BUFFERS; ++b) { init(&s_full[b], 1); init(&p_full[b], 4); init(&pv_done[b], 1); }
+        for (int w = 0; w < 8; ++w) init(&told[w], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(at_smem(&tmem_base_s)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const unsigned tmem = tmem_base_s;
+    pdl_launch_dependents();                                        // (behind the allocation, see attention_prefill_tcgen05.cu)
+
+    const int R = p.nh / p.nkv, per_tile = AS_QTILE / R;
+    AsWalk w(p);
+    w.start(begin, end, from_t, from_before);
+    if (warp == 0) {
+        if (lane == 0) {                                            // ---------------- loader
+            bool ok = true;
+            int it = 0, seg = 0, asked_k = 0, asked_v = 0;
+            for (; ok && w.next(); ++seg) {
+                const int* table = p.block_table + (size_t)p.tok_row[w.g.w] * p.table_stride;
+                if (seg > 0 && !at_wait(at_smem(q_empty), (unsigned)(seg - 1) & 1u)) { ok = false; break; }
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(at_smem(q_full)), "r"((unsigned)(per_tile * R * AS_HD * 2)) : "memory");
+#pragma unroll
+                for (int c = 0; c < AS_PANELS; ++c)
+                    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                                 ::"r"(q_s + c * (AS_QTILE * 128)), "l"(&map_q), "r"(at_smem(q_full)), "r"(64 * c), "r"(w.kvh * R), "r"(w.g.x + w.tile * per_tile) : "memory");
+                auto row_of = [&](int j) {                          // a page that is not there is read from beyond the pool's end, which gives zeros
+                    const int page = j < w.pages.n ? table[w.pages.at(j)] : -1;
+                    return page >= 0 && page < p.pool_rows / (p.nkv * PE_PAGE) ? (page * p.nkv + w.kvh) * PE_PAGE : p.pool_rows;
+                };
+                int y[2] = {row_of(2 * w.first), row_of(2 * w.first + 1)};
+                for (int i = 0; i < w.count; ++i, ++it) {
+                    const int s = it % AS_STAGES, j = 2 * (w.first + i);
+                    const unsigned k_dst = kv_s + s * AS_STAGE_BYTES, v_dst = k_dst + AS_HALF_BYTES, round = (unsigned)(it / AS_STAGES - 1) & 1u;
+                    int next[2] = {p.pool_rows, p.pool_rows};       // the next step's entries travel during the waits
+                    if (i + 1 < w.count) { next[0] = row_of(j + 2); next[1] = row_of(j + 3); }
+                    auto bring = [&](const CUtensorMap* map, unsigned dst, unsigned long long* bar) {
+                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(at_smem(bar)), "r"((unsigned)AS_HALF_BYTES) : "memory");
+#pragma unroll
+                        for (int x = 0; x < 2; ++x)
+#pragma unroll
+                            for (int c = 0; c < AS_PANELS; ++c) at_tma_2d(dst + c * (AS_KTILE * 128) + x * (PE_PAGE * 128), map, 64 * c, y[x], at_smem(bar));
+                    };
+                    if (it >= AS_STAGES && !at_wait(at_smem(&k_empty[s]), round)) { ok = false; break; }
+                    bring(&map_k, k_dst, &k_full[s]);
+                    asked_k = it + 1;
+                    if (it >= AS_STAGES && !at_wait(at_smem(&v_empty[s]), round)) { ok = false; break; }
+                    bring(&map_v, v_dst, &v_full[s]);
+                    asked_v = it + 1;
+                    y[0] = next[0]; y[1] = next[1];
+                }
+            }
+            if (!ok) {                                              // what has been asked for lands before the block ends
+                atomicExch(status, 7);
+                at_wait(at_smem(q_full), (unsigned)(seg > 0 ? seg - 1 : 0) & 1u);
+                for (int n = max(0, asked_k - AS_STAGES); n < asked_k; ++n) at_wait(at_smem(&k_full[n % AS_STAGES]), (unsigned)(n / AS_STAGES) & 1u);
+                for (int n = max(0, asked_v - AS_STAGES); n < asked_v; ++n) at_wait(at_smem(&v_full[n % AS_STAGES]), (unsigned)(n / AS_STAGES) & 1u);
+            }
+        }
+    } else if (warp == 1) {                                         // ---------------- MMA issuer: the warp waits, one thread issues
+        const unsigned elected = pe_elect();
+        const unsigned idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(AS_KTILE >> 3) << 17) | ((unsigned)(AS_QTILE >> 4) << 24);
+        const unsigned idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((unsigned)(AS_HD >> 3) << 17) | ((unsigned)(AS_QTILE >> 4) << 24);
+        const unsigned long long dq = at_desc(q_s, 0, 1024), dk = at_desc(kv_s, 0, 1024), dv = at_desc(kv_s + AS_HALF_BYTES, AS_KTILE * 128, 1024);
+        const int steps = (int)(end - begin);
+        AsWalk ahead(p);                                            // the tile that S has come to
+        ahead.start(begin, end, from_t, from_before);
+        int a_left = 0, a_seg = -1;
+        bool ok = true;
+        auto issue_s = [&](int it) -> bool {
+            const int s = it % AS_STAGES, b = it % AS_BUFFERS;
+            if (a_left == 0) {                                      // the next tile's queries
+                ahead.next();
+                a_left = ahead.count;
+                ++a_seg;
+                if (!at_wait_warp(at_smem(q_full), (unsigned)a_seg & 1u)) return false;
+            }
+            if (it >= AS_BUFFERS && !at_wait_warp(at_smem(&pv_done[b]), (unsigned)(it / AS_BUFFERS - 1) & 1u)) return false;
+            if (!at_wait_warp(at_smem(&k_full[s]), (unsigned)(it / AS_STAGES) & 1u)) return false;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const unsigned long long dks = dk + (unsigned long long)(s * (AS_STAGE_BYTES >> 4));
+#pragma unroll
+            for (int kk = 0; kk < AS_HD / 16; ++kk) {
+                const unsigned off_q = ((kk / 4) * (AS_QTILE * 128) + (kk % 4) * 32) >> 4, off_k = ((kk / 4) * (AS_KTILE * 128) + (kk % 4) * 32) >> 4;
+                at_mma(elected, tmem + b * AS_KTILE, dq + off_q, dks + off_k, idesc_s, kk > 0 ? 1u : 0u);
+            }
+            at_commit_by(elected, at_smem(&k_empty[s]));
+            at_commit_by(elected, at_smem(&s_full[b]));
+            if (--a_left == 0) at_commit_by(elected, at_smem(q_empty));      // the tile's queries have been read
+            return true;
+        };
+        for (int it = 0; it < min(AS_AHEAD, steps) && ok; ++it) ok = issue_s(it);
+        int it = 0;
+        for (int seg = 0; ok && w.next(); ++seg) {
+            for (int i = 0; i < w.count; ++i, ++it) {
+                const int s = it % AS_STAGES, b = it % AS_BUFFERS;
+                if (!at_wait_warp(at_smem(&v_full[s]), (unsigned)(it / AS_STAGES) & 1u)) { ok = false; break; }
+                if (!at_wait_warp(at_smem(&p_full[b]), (unsigned)(it / AS_BUFFERS) & 1u)) { ok = false; break; }
+                if (i == 0 && seg > 0 && !at_wait_warp(at_smem(o_empty), (unsigned)(seg - 1) & 1u)) { ok = false; break; }     // the tile before has left O
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const unsigned long long dvs = dv + (unsigned long long)(s * (AS_STAGE_BYTES >> 4));
+#pragma unroll
+                for (int kk = 0; kk < AS_KTILE / 16; ++kk)
+                    at_mma_ts(elected, tmem + AS_O_COL, tmem + b * AS_KTILE + kk * 8, dvs + ((kk * 16 * 128) >> 4), idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
+                at_commit_by(elected, at_smem(&v_empty[s]));
+                at_commit_by(elected, at_smem(&pv_done[b]));
+                if (it + AS_AHEAD < steps && !issue_s(it + AS_AHEAD)) { ok = false; break; }
+            }
+        }
+        if (!ok) atomicExch(status, 7);
+    } else {                                                        // ---------------- softmax, warps 2..9
+        const int quarter = warp & 3;                               // the 32 lanes of tensor memory this warp may touch
+        const int g = (warp - 2) >> 2;                              // the warpgroup: steps g, g + 2, ..
+        const int r = quarter * 32 + lane;                          // this thread's row of the tile
+        const unsigned lane_addr = tmem + ((unsigned)(quarter * 32) << 16);
+        const unsigned long long scale2 = at_two(p.scale_log2e, p.scale_log2e);
+        bool ok = true;
+        int it0 = 0;                                                // the CTA's steps before this tile
+        for (int seg = 0; ok && w.next(); ++seg, it0 += w.count) {
+            const int* table = p.block_table + (size_t)p.tok_row[w.g.w] * p.table_stride;
+            const int tok_i = w.tile * per_tile + r / R;            // the row's token in its group
+            const int rows = min(per_tile, w.g.y - w.tile * per_tile) * R;
+            const bool live = r < rows;
+            const int h = w.kvh * R + r % R;
+            int pos = 0;
+            float slope = 0.f;
+            if (MASKED && live) {
+                pos = p.tok_pos[w.g.x + tok_i];
+                if (p.slopes) slope = p.slopes[h] * p.inv_scale;
+            }
+            const int pool_pages = p.pool_rows / (p.nkv * PE_PAGE);
+            auto there_at = [&](int j) { if (j >= w.pages.n) return false; const int page = table[w.pages.at(j)]; return page >= 0 && page < pool_pages; };
+            float m_mine = -INFINITY, l_mine = 0.f;
+            const int i0 = (g ^ it0) & 1;                           // the group's first step of this tile
+            bool there[2] = {true, true};
+#pragma unroll
+            for (int x = 0; x < 2; ++x) there[x] = i0 < w.count && there_at(2 * (w.first + i0) + x);
+            for (int i = i0; i < w.count; i += 2) {
+                const int it = it0 + i, b = it % AS_BUFFERS;
+                const unsigned s_addr = lane_addr + b * AS_KTILE;
+                bool after[2] = {true, true};
+#pragma unroll
+                for (int x = 0; x < 2; ++x) after[x] = i + 2 < w.count && there_at(2 * (w.first + i + 2) + x);
+                if (!at_wait_warp(at_smem(&s_full[b]), (unsigned)(it / AS_BUFFERS) & 1u)) { ok = false; break; }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                unsigned raw[AS_KTILE];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) at_ld32_start(s_addr + 32 * c, raw + 32 * c);
+                at_ld_wait();
+#pragma unroll
+                for (int c = 0; c < 4; ++c) at_pin32(raw + 32 * c);
+                float s[AS_KTILE], base[2] = {0.f, 0.f}, mx[8];
+#pragma unroll
+                for (int c = 0; c < AS_KTILE; ++c) s[c] = __uint_as_float(raw[c]);
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    float* sx = s + x * PE_PAGE;
+                    if (!there[x] || !live) {
+                        at_mask_behind<PE_PAGE>(sx, -1);
+                    } else if (MASKED) {
+                        const int key0 = w.pages.at(2 * (w.first + i) + x) * PE_PAGE;
+                        if (p.window > 0 && key0 <= pos - p.window && key0 + PE_PAGE - 1 >= p.keep_first) {
+                            const int lo = pos - p.window + 1 - key0, kept_here = p.keep_first - key0;
+#pragma unroll
+                            for (int c = 0; c < PE_PAGE; ++c)
+                                if (c < lo && c >= kept_here) sx[c] = -INFINITY;
+                        }
+                        if (p.slopes) {                             // the distance's share: what grows along the page here, the page's own part in `base`
+                            base[x] = slope * (float)(key0 - pos);
+#pragma unroll
+                            for (int c = 0; c < PE_PAGE; ++c) sx[c] = fmaf(slope, (float)c, sx[c]);
+                        }
+                    }
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) mx[4 * x + c] = fmaxf(fmaxf(sx[c], sx[c + 4]), sx[c + 8]);
+#pragma unroll
+                    for (int c = 12; c < PE_PAGE - 4; c += 8) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) mx[4 * x + k] = fmaxf(fmaxf(mx[4 * x + k], sx[c + k]), sx[c + 4 + k]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mx[4 * x + k] = fmaxf(mx[4 * x + k], sx[PE_PAGE - 4 + k]);
+                }
+                const float m_step = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) + base[0], fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])) + base[1]);
+                // the row's reference point up to the step before, from the other warpgroup (asked for at a tile's first step too: a wait by
+                // parity has to see every phase)
+                float m_run = -INFINITY;
+                if (it > 0) {
+                    if (!at_wait_warp(at_smem(&told[4 * (g ^ 1) + quarter]), (unsigned)((it - 1) >> 1) & 1u)) { ok = false; break; }
+                    if (i > 0) m_run = refs[(g ^ 1) * AS_QTILE + r];
+                }
+                const float m_tile = m_step * p.scale_log2e;
+                const float m_new = (m_run != -INFINITY && m_tile <= m_run + AS_LAZY) ? m_run : fmaxf(m_run, m_tile);
+                refs[g * AS_QTILE + r] = m_new;
+                __syncwarp();
+                if (lane == 0) at_arrive(at_smem(&told[4 * g + quarter]));
+                const float m_use = m_new == -INFINITY ? 0.f : m_new;
+                const float alpha = m_run == -INFINITY ? 1.0f : at_exp2(m_run - m_use);
+                l_mine *= m_mine == -INFINITY ? 1.0f : at_exp2(m_mine - m_use);
+                m_mine = m_new;
+                unsigned long long sum[2] = {0ull, 0ull};
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    float packed[PE_PAGE / 2];
+                    const float off = fmaf(base[x], p.scale_log2e, -m_use);
+#pragma unroll
+                    for (int c = 0; c < PE_PAGE; c += 2) packed[c >> 1] = __uint_as_float(at_exp2_pair(s[x * PE_PAGE + c], s[x * PE_PAGE + c + 1], scale2, at_two(off, off), sum[(c >> 1) & 1]));
+                    at_st32(s_addr + x * (PE_PAGE / 2), packed);
+                }
+                l_mine += at_sum_four(sum[0], sum[1]);
+                if (i > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+                    if (!at_wait_warp(at_smem(&pv_done[(it - 1) % AS_BUFFERS]), (unsigned)((it - 1) / AS_BUFFERS) & 1u)) { ok = false; break; }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+                    for (int c = 0; c < AS_HD; c += 32) {
+                        float o[32];
+                        at_ld32(lane_addr + AS_O_COL + c, o);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) o[k] *= alpha;
+                        at_st32(lane_addr + AS_O_COL + c, o);
+                    }
+                }
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) at_arrive(at_smem(&p_full[b]));
+                there[0] = after[0]; there[1] = after[1];
+            }
+            if (!ok) break;
+            // ---- the tile's end: both groups write their half of O, and the reference point and sum of their own steps.  (Reference points only grow, and
+            // the last step's is what O goes by: the larger of the two.)
+            const int last = it0 + w.count - 1;
+            if (!at_wait_warp(at_smem(&pv_done[last % AS_BUFFERS]), (unsigned)(last / AS_BUFFERS) & 1u)) { ok = false; break; }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            float o[AS_HD / 2];
+#pragma unroll
+            for (int c = 0; c < AS_HD / 2; c += 32) at_ld32(lane_addr + AS_O_COL + g * (AS_HD / 2) + c, o + c);
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) at_arrive(at_smem(o_empty));
+            if (live) {
+                const size_t row = as_row(blockIdx.x, w.g, p.nh, p.nkv, w.kvh, w.tile * per_tile * R + r);
+                reinterpret_cast<float2*>(p.scratch.ends + row)[g] = make_float2(m_mine, l_mine);
+                float4* to = reinterpret_cast<float4*>(p.scratch.sums + row * AS_HD + g * (AS_HD / 2));
+#pragma unroll
+                for (int c = 0; c < AS_HD / 8; ++c) to[c] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+            }
+        }
+        if (!ok) atomicExch(status, 7);
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
 }
+
+namespace {
+
+// queries of `tokens` rows, `stride` elements apart, as boxes of [box_tokens][box_heads][64 columns]
+int as_query_map(CUtensorMap* map, const void* q, long long tokens, int heads, long long stride, int box_heads, int box_tokens) {
+    at_encode_fn enc = at_encoder();
+    if (!enc) return PE_ERR_UNSUPPORTED;
+    const cuuint64_t dims[3] = {(cuuint64_t)AS_HD, (cuuint64_t)heads, (cuuint64_t)tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)AS_HD * 2, (cuuint64_t)stride * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens}, elem[3] = {1, 1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : 20000 + (int)r;
+}
+
+template <bool MASKED>
+int as_launch(int grid, cudaStream_t stream, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const AsArgs& p, int* status) {
+    static bool wide = false;
+    if (!wide) {
+        PE_TRY(cudaFuncSetAttribute(attention_shared_kernel<MASKED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)AS_SMEM_BYTES));
+        wide = true;
+    }
+    PE_TRY(pe_launch(attention_shared_kernel<MASKED>, dim3(grid), AS_THREADS, AS_SMEM_BYTES, stream, mq, mk, mv, p, status));
+    PE_LAUNCH_CHECK();
+    return 0;
+}
+
+long long as_before_bytes(int T) { return ((long long)(T + 1) * 8 + 255) / 256 * 256; }
+long long as_rows(int T, int nh) { return (long long)pe_sm_count() * AS_QTILE + (long long)T * nh; }
+
+}  // namespace
+
+extern "C" long long pe_attention_shared_scratch(int T, int nh) { return as_before_bytes(T) + as_rows(T, nh) * (AS_HD * 4 + 16); }
+
+// the kernel of attention_decode.cu for the rows' own positions
+int pe_attention_decode_own(const void* q, int q_stride, void* out, const void* k_pool, const void* v_pool, const int* block_table, int table_stride,
+                            const int* tok_pos, const int* tok_row, int T, int nh, int nkv, int window, float scale, int max_context, int early_pages,
+                            int* status, void* stream, int keep_first, const float* slopes, const float* sinks, const void* groups, const AsScratch& scratch);
 
 extern "C" int pe_attention_shared(const void* q, int q_stride, void* out, const void* k_pool, const void* v_pool, long long pool_pages,
                                    const int* block_table, int table_stride, const int* tok_pos, const int* tok_row, const void* groups, int T,
                                    int nh, int nkv, int hd, int window, int keep_first, float scale, int max_context, const float* slopes,
                                    const float* sinks, int early_pages, void* scratch, int* status, void* stream) {
     if (T <= 0) return 0;
-    if (hd != AS_HD || nkv <= 0 || nh % nkv || q_stride % 8 || !(scale > 0.f) || (long long)T * nh > 0x7fffffff) return PE_ERR_UNSUPPORTED;
-    PE_TRY(pe_launch(attention_shared_kernel, (T * nh + 3) / 4, 128, 0, (cudaStream_t)stream, (const bf16*)q, q_stride, (bf16*)out, (const bf16*)k_pool,
-                     (const bf16*)v_pool, block_table, table_stride, tok_pos, tok_row, T, nh, nkv, window, window > 0 ? keep_first : 0, scale, slopes, sinks));
-    PE_LAUNCH_CHECK();
-    return 0;
+    if (hd != AS_HD || nkv <= 0 || nh % nkv || nh / nkv > AS_QTILE || q_stride % 8 || !(scale > 0.f) || !status || !scratch || keep_first < 0) return PE_ERR_UNSUPPORTED;
+    if (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)groups | (uintptr_t)scratch) & 15) return PE_ERR_UNSUPPORTED;
+    if (pool_pages * nkv * PE_PAGE > 0x7fffff00ll) return PE_ERR_UNSUPPORTED;       // TMA coordinates are 32-bit
+    const int R = nh / nkv;
+    CUtensorMap mq, mk, mv;
+    int rc = as_query_map(&mq, q, T, nh, q_stride, R, AS_QTILE / R);
+    if (rc) return rc;
+    rc = at_make_map(&mk, k_pool, pool_pages * nkv * PE_PAGE, hd, hd, PE_PAGE);
+    if (rc) return rc;
+    rc = at_make_map(&mv, v_pool, pool_pages * nkv * PE_PAGE, hd, hd, PE_PAGE);
+    if (rc) return rc;
+    AsArgs p = {};
+    p.groups = (const int4*)groups; p.block_table = block_table; p.table_stride = table_stride; p.tok_pos = tok_pos; p.tok_row = tok_row;
+    p.T = T; p.nh = nh; p.nkv = nkv; p.window = window; p.keep_first = window > 0 ? keep_first : 0; p.scale_log2e = scale * 1.4426950408889634f;
+    p.slopes = slopes; p.inv_scale = 1.0f / scale; p.pool_rows = (int)(pool_pages * nkv * PE_PAGE);
+    p.scratch.before = (long long*)scratch;
+    p.scratch.sums = (float*)((char*)scratch + as_before_bytes(T));
+    p.scratch.ends = (float4*)(p.scratch.sums + as_rows(T, nh) * AS_HD);
+    rc = window > 0 || slopes ? as_launch<true>(pe_sm_count(), (cudaStream_t)stream, mq, mk, mv, p, status)
+                              : as_launch<false>(pe_sm_count(), (cudaStream_t)stream, mq, mk, mv, p, status);
+    if (rc) return rc;
+    return pe_attention_decode_own(q, q_stride, out, k_pool, v_pool, block_table, table_stride, tok_pos, tok_row, T, nh, nkv, window, scale, max_context,
+                                   early_pages, status, stream, p.keep_first, slopes, sinks, groups, p.scratch);
 }
 
 #else   // other head sizes: the rows of a group are read one by one (attention_decode.cu)
 
+extern "C" long long pe_attention_shared_scratch(int, int) { return 0; }
 extern "C" int pe_attention_shared(const void*, int, void*, const void*, const void*, long long, const int*, int, const int*, const int*, const void*,
                                    int, int, int, int, int, int, float, int, const float*, const float*, int, void*, int*, void*) {
     return PE_ERR_UNSUPPORTED;

@@ -1952,11 +1952,14 @@ def attention_shared(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: i
         out = torch.empty(T, n_heads * head_dim, dtype=torch.bfloat16, device=q.device)
     _need(out, "out", torch.bfloat16, (T, n_heads * head_dim))
     _need_here(q, "q")
+    if T == 0:
+        return out
     lib = for_head_dim(head_dim)
+    scratch = torch.empty(lib.pe_attention_shared_scratch(T, n_heads), dtype=torch.uint8, device=q.device)      # (of the call: graphs and streams share none)
     check(lib.pe_attention_shared(q.data_ptr(), q_stride, out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_pool.shape[0], block_table.data_ptr(),
                                   table_stride, tok_pos.data_ptr(), tok_row.data_ptr(), groups.data_ptr(), T, n_heads, n_kv_heads, head_dim, window or 0,
-                                  keep_first if window else 0, scale, max_context, _ptr(slopes), _ptr(sinks), 1 if early_pages else 0, None,
-                                  status_ptr(q.device), stream_ptr()), "attention_shared")
+                                  keep_first if window else 0, scale, max_context, _ptr(slopes), _ptr(sinks), 1 if early_pages else 0, scratch.data_ptr(),
+                                  status_ptr(q.device), stream_ptr()), "attention_shared", 2)
     return out
 
 
