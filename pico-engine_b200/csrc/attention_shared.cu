@@ -28,7 +28,7 @@
 #define AS_PANELS (AS_HD / 64)
 #define AS_STAGES (AS_HD == 64 ? 5 : 3)
 #define AS_AHEAD 3
-#define AS_THREADS 320
+#define AS_THREADS AS_COUNTED
 #define AS_Q_BYTES (AS_QTILE * AS_HD * 2)
 #define AS_HALF_BYTES (AS_KTILE * AS_HD * 2)       // keys (or values) of a step
 #define AS_STAGE_BYTES (2 * AS_HALF_BYTES)
@@ -42,46 +42,38 @@
 struct AsArgs {
     const int4* groups; const int* block_table; int table_stride; const int* tok_pos; const int* tok_row;
     int T, nh, nkv, window, keep_first; float scale_log2e; const float* slopes; float inv_scale;
-    int pool_rows; AsScratch scratch;
+    int pool_rows, early; AsScratch scratch;
 };
 
-// One tile's share of a CTA's steps, and how to come to the next.  Every role walks its own copy.
+// A CTA's tiles one after the other.  Every warp walks its own copy, in shared memory: one lane takes the step, all of them read.
 struct AsWalk {
-    const AsArgs& p;
-    long long x, end, before, in_group;            // the next step; the CTA's last; steps in front of the group and in it
-    int t;                                         // the group's first token
-    int4 g; AsPages pages; int n_steps, tiles;
+    AsGroup now;
+    int x, end;                                    // the next step, and where the CTA's end
     int kvh, tile, first, count;                   // the tile, and its steps here
-    __device__ AsWalk(const AsArgs& args) : p(args), in_group(0) {}
-    // the group that starts with token t: its steps, 0 if none starts there
-    __device__ static long long group(const AsArgs& p, int t, int4& g, AsPages& pages, int& n_steps, int& tiles) {
-        g = p.groups[t];
-        const int shared = g.x == t ? as_shared(g, t, p.T, p.table_stride) : 0;
-        if (shared == 0) return 0;
-        pages = as_pages(shared, p.window > 0 ? p.tok_pos[g.w] : 0, p.window, p.keep_first);
-        const int per_tile = AS_QTILE / (p.nh / p.nkv);
-        n_steps = (pages.n + 1) / 2;
-        tiles = (g.y + per_tile - 1) / per_tile;
-        return (long long)n_steps * tiles * p.nkv;
-    }
-    __device__ void start(long long from, long long to, int at, long long in_front) {
-        x = from; end = to; t = at; before = in_front;
-        in_group = group(p, t, g, pages, n_steps, tiles);
-        count = 0;
-    }
-    __device__ bool next() {
+    const int* table;                              // the page table's row that names the shared pages
+    __device__ __forceinline__ bool step(const AsArgs& p) {
         x += count;
         if (x >= end) return false;
-        while (x >= before + in_group) {
-            before += in_group;
-            t += in_group > 0 ? g.y : 1;
-            in_group = group(p, t, g, pages, n_steps, tiles);
+        bool moved = count == 0;
+        while (x >= now.before + now.steps) {
+            const int before = now.before + now.steps;
+            now.load(p.groups, p.tok_pos, now.t + (now.steps > 0 ? now.g.y : 1), p.T, p.table_stride, p.nh, p.nkv, p.window, p.keep_first);
+            now.before = before;
+            moved = true;
         }
-        const long long o = x - before, seg = o / n_steps;
-        first = (int)(o - seg * n_steps);
-        kvh = (int)(seg / tiles); tile = (int)(seg - (long long)kvh * tiles);
-        count = (int)min((long long)(n_steps - first), end - x);
+        if (moved) table = p.block_table + (size_t)p.tok_row[now.g.w] * p.table_stride;
+        const int o = x - now.before, n = as_tile_steps(now.pages), tiles = as_tiles(now.g, p.nh, p.nkv), seg = o / n;
+        first = o - seg * n;
+        kvh = seg / tiles; tile = seg - kvh * tiles;
+        count = min(n - first, end - x);
         return true;
+    }
+    __device__ __forceinline__ bool next(const AsArgs& p, int lane) {        // the whole warp
+        bool more = false;
+        __syncwarp();
+        if (lane == 0) more = step(p);
+        __syncwarp();
+        return __shfl_sync(0xffffffffu, more, 0);
     }
 };
 
@@ -98,63 +90,76 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
     unsigned long long *k_full = pv_done + AS_BUFFERS, *v_full = k_full + AS_STAGES, *k_empty = v_full + AS_STAGES, *v_empty = k_empty + AS_STAGES;
     unsigned long long* told = v_empty + AS_STAGES;                 // [warpgroup][32 rows]: a step's reference points are there
     float* refs = reinterpret_cast<float*>(bars + AS_BARS);         // [warpgroup][row]: reference point of the group's last step
-    __shared__ long long scan[AS_THREADS / 32], from_before;
-    __shared__ int from_t;
+    __shared__ int scan[AS_THREADS / 32];
+    __shared__ AsWalk walks[AS_THREADS / 32 + 2];                   // the first tile; a warp's each; the second one of the issuer
     if (q_s & 1023u) {                                              // every thread alike: nothing is allocated yet
         if (threadIdx.x == 0) atomicExch(status, 6);
         return;
     }
-    pdl_wait();
+    // The description of the step was there before the kernels in front began, or (early == 0) they have ended: p.early says which.  So have the
+    // shared pages.  Queries, and the scratch that the call before may still be reading, wait.
+    if (!p.early) pdl_wait();
 
     // ---- this CTA's share of the steps: a scan over the groups (a token a thread; the second time round only where there are more tokens)
-    const int grid = gridDim.x;
-    long long total = 0, begin = 0, end = 0;
-    for (int pass = 0; pass < 2; ++pass) {
-        long long run = 0;
-        for (int base = 0; base < p.T; base += AS_THREADS) {
-            const int t = base + threadIdx.x;
-            long long mine = 0;
-            if (t < p.T) { int4 g; AsPages pages; int n_steps, tiles; mine = AsWalk::group(p, t, g, pages, n_steps, tiles); }
-            long long sum = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long up = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= o) sum += up;
-            }
-            __syncthreads();
-            if (lane == 31) scan[warp] = sum;
-            __syncthreads();
-            long long in_front = run + sum - mine;
-#pragma unroll
-            for (int w = 0; w < AS_THREADS / 32; ++w) {
-                if (w < warp) in_front += scan[w];
-                run += scan[w];
-            }
-            if (pass == 0 && blockIdx.x == 0 && t < p.T) p.scratch.before[t] = in_front;
-            if (pass == 0 && p.T <= AS_THREADS) {                   // all groups are in hand
-                total = run;
-                const int ctas = as_ctas(total, grid);
-                if ((int)blockIdx.x < ctas) { begin = total * blockIdx.x / ctas; end = total * (blockIdx.x + 1) / ctas; }
-            }
-            if ((pass == 1 || p.T <= AS_THREADS) && mine > 0 && begin < end && begin >= in_front && begin < in_front + mine) { from_t = t; from_before = in_front; }
-        }
-        if (pass == 0) {
-            total = run;
-            const int ctas = as_ctas(total, grid);
-            if ((int)blockIdx.x < ctas) { begin = total * blockIdx.x / ctas; end = total * (blockIdx.x + 1) / ctas; }
-            if (blockIdx.x == 0 && threadIdx.x == 0) p.scratch.before[p.T] = total;
-            if (p.T <= AS_THREADS) break;
-        }
-    }
-    if (begin >= end) { pdl_launch_dependents(); return; }          // (the whole block)
-
-    if (threadIdx.x == 0) {
+    AsGroup mine;
+    mine.steps = 0;
+    auto load = [&](int t) { mine.load(p.groups, p.tok_pos, t, p.T, p.table_stride, p.nh, p.nkv, p.window, p.keep_first); };
+    if ((int)threadIdx.x < p.T) load(threadIdx.x);
+    if (threadIdx.x == 32) {
         auto init = [](unsigned long long* bar, unsigned count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(at_smem(bar)), "r"(count) : "memory"); };
         init(q_full, 1); init(q_empty, 1); init(o_empty, 8);
         for (int s = 0; s < AS_STAGES; ++s) { init(&k_full[s], 1); init(&v_full[s], 1); init(&k_empty[s], 1); init(&v_empty[s], 1); }
         for (int b = 0; b < AS_BUFFERS; ++b) { init(&s_full[b], 1); init(&p_full[b], 4); init(&pv_done[b], 1); }
         for (int w = 0; w < 8; ++w) init(&told[w], 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
+    }
+    int begin = 0, end = 0, total = 0;
+    auto deal = [&] {
+        const AsDeal d(total, gridDim.x);
+        if ((int)blockIdx.x < d.ctas) { begin = d.begin(blockIdx.x); end = d.begin(blockIdx.x + 1); }
+    };
+    for (int pass = 0; pass < 2; ++pass) {
+        int run = 0;
+        for (int base = 0; base < p.T; base += AS_THREADS) {
+            const int t = base + threadIdx.x;
+            if (p.T > AS_COUNTED && (base > 0 || pass > 0)) {
+                mine.steps = 0;
+                if (t < p.T) load(t);
+            }
+            int sum = mine.steps;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += up;
+            }
+            __syncthreads();
+            if (lane == 31) scan[warp] = sum;
+            __syncthreads();
+            mine.before = run + sum - mine.steps;
+#pragma unroll
+            for (int w = 0; w < AS_THREADS / 32; ++w) {
+                if (w < warp) mine.before += scan[w];
+                run += scan[w];
+            }
+            if (pass == 0 && p.T > AS_COUNTED && blockIdx.x == 0 && t < p.T) { pdl_wait(); p.scratch.before[t] = mine.before; }
+            if (pass == 0 && p.T <= AS_COUNTED) { total = run; deal(); }         // all groups are in hand
+            if ((pass == 1 || p.T <= AS_COUNTED) && begin < end && begin >= mine.before && begin < mine.before + mine.steps) {
+                walks[0].now = mine;
+                walks[0].x = begin; walks[0].end = end; walks[0].count = 0;
+                walks[0].step(p);                                   // the first tile
+            }
+        }
+        if (pass == 0) {
+            if (p.T <= AS_COUNTED) break;
+            total = run;
+            deal();
+            if (blockIdx.x == 0 && threadIdx.x == 0) { pdl_wait(); p.scratch.before[p.T] = total; }
+        }
+    }
+    if (begin >= end) {                                             // (the whole block)
+        pdl_wait();
+        pdl_launch_dependents();
+        return;
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(at_smem(&tmem_base_s)), "r"(512u) : "memory");
@@ -164,33 +169,42 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned tmem = tmem_base_s;
-    pdl_launch_dependents();                                        // (behind the allocation, see attention_prefill_tcgen05.cu)
+    const int R = p.nh / p.nkv, per_tile = AS_QTILE / R, pool_pages = p.pool_rows / (p.nkv * PE_PAGE);
+    // (the first tile has been found; a warp's own copy goes on from there)
+    AsWalk& w = walks[warp + 1];
+    if (lane == 0) { w = walks[0]; if (warp == 1) walks[AS_THREADS / 32 + 1] = walks[0]; }
+    __syncwarp();
+    auto advance = [&](int seg) { return seg == 0 ? true : w.next(p, lane); };
 
-    const int R = p.nh / p.nkv, per_tile = AS_QTILE / R;
-    AsWalk w(p);
-    w.start(begin, end, from_t, from_before);
-    if (warp == 0) {
-        if (lane == 0) {                                            // ---------------- loader
-            bool ok = true;
-            int it = 0, seg = 0, asked_k = 0, asked_v = 0;
-            for (; ok && w.next(); ++seg) {
-                const int* table = p.block_table + (size_t)p.tok_row[w.g.w] * p.table_stride;
-                if (seg > 0 && !at_wait(at_smem(q_empty), (unsigned)(seg - 1) & 1u)) { ok = false; break; }
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(at_smem(q_full)), "r"((unsigned)(per_tile * R * AS_HD * 2)) : "memory");
+    if (warp == 0) {                                                // ---------------- loader: one lane asks, the others wait for the walk
+        bool ok = true;
+        int it = 0, seg = 0, asked_k = 0, asked_v = 0, asked_q = 0;
+        for (; ok && advance(seg); ++seg) {
+            if (lane == 0) {
+                const int count = w.count, first = w.first, kvh = w.kvh, n = w.now.pages.n;
+                const int* table = w.table;
+                const AsPages pages = w.now.pages;
+                auto page_of = [&](int j) { return j < n ? table[pages.at(j)] : -1; };
+                auto ask_q = [&] {
+                    if (seg > 0 && !at_wait(at_smem(q_empty), (unsigned)(seg - 1) & 1u)) return false;
+                    pdl_wait();
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(at_smem(q_full)), "r"((unsigned)(per_tile * R * AS_HD * 2)) : "memory");
 #pragma unroll
-                for (int c = 0; c < AS_PANELS; ++c)
-                    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-                                 ::"r"(q_s + c * (AS_QTILE * 128)), "l"(&map_q), "r"(at_smem(q_full)), "r"(64 * c), "r"(w.kvh * R), "r"(w.g.x + w.tile * per_tile) : "memory");
-                auto row_of = [&](int j) {                          // a page that is not there is read from beyond the pool's end, which gives zeros
-                    const int page = j < w.pages.n ? table[w.pages.at(j)] : -1;
-                    return page >= 0 && page < p.pool_rows / (p.nkv * PE_PAGE) ? (page * p.nkv + w.kvh) * PE_PAGE : p.pool_rows;
+                    for (int c = 0; c < AS_PANELS; ++c)
+                        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                                     ::"r"(q_s + c * (AS_QTILE * 128)), "l"(&map_q), "r"(at_smem(q_full)), "r"(64 * c), "r"(kvh * R), "r"(w.now.g.x + w.tile * per_tile) : "memory");
+                    ++asked_q;
+                    return true;
                 };
-                int y[2] = {row_of(2 * w.first), row_of(2 * w.first + 1)};
-                for (int i = 0; i < w.count; ++i, ++it) {
-                    const int s = it % AS_STAGES, j = 2 * (w.first + i);
+                int page[2] = {page_of(2 * first), page_of(2 * first + 1)};
+                if (seg > 0) ok = ask_q();                          // (the first tile's behind its first step: keys and values need not wait for the kernel in front)
+                for (int i = 0; ok && i < count; ++i, ++it) {
+                    const int s = it % AS_STAGES, j = 2 * (first + i);
                     const unsigned k_dst = kv_s + s * AS_STAGE_BYTES, v_dst = k_dst + AS_HALF_BYTES, round = (unsigned)(it / AS_STAGES - 1) & 1u;
-                    int next[2] = {p.pool_rows, p.pool_rows};       // the next step's entries travel during the waits
-                    if (i + 1 < w.count) { next[0] = row_of(j + 2); next[1] = row_of(j + 3); }
+                    // a page that is not there is read from beyond the pool's end, which gives zeros
+                    const int y[2] = {(unsigned)page[0] < (unsigned)pool_pages ? (page[0] * p.nkv + kvh) * PE_PAGE : p.pool_rows,
+                                      (unsigned)page[1] < (unsigned)pool_pages ? (page[1] * p.nkv + kvh) * PE_PAGE : p.pool_rows};
+                    if (i + 1 < count) { page[0] = page_of(j + 2); page[1] = page_of(j + 3); }       // travel during the waits
                     auto bring = [&](const CUtensorMap* map, unsigned dst, unsigned long long* bar) {
                         asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(at_smem(bar)), "r"((unsigned)AS_HALF_BYTES) : "memory");
 #pragma unroll
@@ -204,30 +218,33 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
                     if (it >= AS_STAGES && !at_wait(at_smem(&v_empty[s]), round)) { ok = false; break; }
                     bring(&map_v, v_dst, &v_full[s]);
                     asked_v = it + 1;
-                    y[0] = next[0]; y[1] = next[1];
+                    if (seg == 0 && i == 0) ok = ask_q();
+                }
+                if (!ok) {                                          // what has been asked for lands before the block ends
+                    atomicExch(status, 7);
+                    if (asked_q > 0) at_wait(at_smem(q_full), (unsigned)(asked_q - 1) & 1u);
+                    for (int n = max(0, asked_k - AS_STAGES); n < asked_k; ++n) at_wait(at_smem(&k_full[n % AS_STAGES]), (unsigned)(n / AS_STAGES) & 1u);
+                    for (int n = max(0, asked_v - AS_STAGES); n < asked_v; ++n) at_wait(at_smem(&v_full[n % AS_STAGES]), (unsigned)(n / AS_STAGES) & 1u);
                 }
             }
-            if (!ok) {                                              // what has been asked for lands before the block ends
-                atomicExch(status, 7);
-                at_wait(at_smem(q_full), (unsigned)(seg > 0 ? seg - 1 : 0) & 1u);
-                for (int n = max(0, asked_k - AS_STAGES); n < asked_k; ++n) at_wait(at_smem(&k_full[n % AS_STAGES]), (unsigned)(n / AS_STAGES) & 1u);
-                for (int n = max(0, asked_v - AS_STAGES); n < asked_v; ++n) at_wait(at_smem(&v_full[n % AS_STAGES]), (unsigned)(n / AS_STAGES) & 1u);
-            }
+            ok = __shfl_sync(0xffffffffu, ok, 0);
         }
     } else if (warp == 1) {                                         // ---------------- MMA issuer: the warp waits, one thread issues
+        // Behind the allocation, and behind the end of the kernel in front: the next kernel counts on both (it reads queries and keys without a wait)
+        pdl_wait();
+        pdl_launch_dependents();
         const unsigned elected = pe_elect();
         const unsigned idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(AS_KTILE >> 3) << 17) | ((unsigned)(AS_QTILE >> 4) << 24);
         const unsigned idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((unsigned)(AS_HD >> 3) << 17) | ((unsigned)(AS_QTILE >> 4) << 24);
         const unsigned long long dq = at_desc(q_s, 0, 1024), dk = at_desc(kv_s, 0, 1024), dv = at_desc(kv_s + AS_HALF_BYTES, AS_KTILE * 128, 1024);
-        const int steps = (int)(end - begin);
-        AsWalk ahead(p);                                            // the tile that S has come to
-        ahead.start(begin, end, from_t, from_before);
-        int a_left = 0, a_seg = -1;
-        bool ok = true;
+        const int steps = end - begin;
+        AsWalk& ahead = walks[AS_THREADS / 32 + 1];                 // the tile that S has come to
+        int a_left = ahead.count, a_seg = 0;
+        bool ok = at_wait_warp(at_smem(q_full), 0u);
         auto issue_s = [&](int it) -> bool {
             const int s = it % AS_STAGES, b = it % AS_BUFFERS;
             if (a_left == 0) {                                      // the next tile's queries
-                ahead.next();
+                ahead.next(p, lane);
                 a_left = ahead.count;
                 ++a_seg;
                 if (!at_wait_warp(at_smem(q_full), (unsigned)a_seg & 1u)) return false;
@@ -248,8 +265,9 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
         };
         for (int it = 0; it < min(AS_AHEAD, steps) && ok; ++it) ok = issue_s(it);
         int it = 0;
-        for (int seg = 0; ok && w.next(); ++seg) {
-            for (int i = 0; i < w.count; ++i, ++it) {
+        for (int seg = 0; ok && advance(seg); ++seg) {
+            const int count = w.count;
+            for (int i = 0; i < count; ++i, ++it) {
                 const int s = it % AS_STAGES, b = it % AS_BUFFERS;
                 if (!at_wait_warp(at_smem(&v_full[s]), (unsigned)(it / AS_STAGES) & 1u)) { ok = false; break; }
                 if (!at_wait_warp(at_smem(&p_full[b]), (unsigned)(it / AS_BUFFERS) & 1u)) { ok = false; break; }
@@ -271,33 +289,34 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
         const int r = quarter * 32 + lane;                          // this thread's row of the tile
         const unsigned lane_addr = tmem + ((unsigned)(quarter * 32) << 16);
         const unsigned long long scale2 = at_two(p.scale_log2e, p.scale_log2e);
+        pdl_wait();                                                 // (scratch is written)
         bool ok = true;
         int it0 = 0;                                                // the CTA's steps before this tile
-        for (int seg = 0; ok && w.next(); ++seg, it0 += w.count) {
-            const int* table = p.block_table + (size_t)p.tok_row[w.g.w] * p.table_stride;
-            const int tok_i = w.tile * per_tile + r / R;            // the row's token in its group
-            const int rows = min(per_tile, w.g.y - w.tile * per_tile) * R;
+        for (int seg = 0; ok && advance(seg); ++seg) {
+            const int count = w.count, first = w.first;
+            const int odd_end = w.now.pages.n & 1 ? w.now.pages.n / 2 - first : -1;       // the step whose second page is not there
+            const int rows = min(per_tile, w.now.g.y - w.tile * per_tile) * R;
             const bool live = r < rows;
-            const int h = w.kvh * R + r % R;
             int pos = 0;
             float slope = 0.f;
             if (MASKED && live) {
-                pos = p.tok_pos[w.g.x + tok_i];
-                if (p.slopes) slope = p.slopes[h] * p.inv_scale;
+                pos = p.tok_pos[w.now.g.x + w.tile * per_tile + r / R];
+                if (p.slopes) slope = p.slopes[w.kvh * R + r % R] * p.inv_scale;
             }
-            const int pool_pages = p.pool_rows / (p.nkv * PE_PAGE);
-            auto there_at = [&](int j) { if (j >= w.pages.n) return false; const int page = table[w.pages.at(j)]; return page >= 0 && page < pool_pages; };
             float m_mine = -INFINITY, l_mine = 0.f;
             const int i0 = (g ^ it0) & 1;                           // the group's first step of this tile
-            bool there[2] = {true, true};
-#pragma unroll
-            for (int x = 0; x < 2; ++x) there[x] = i0 < w.count && there_at(2 * (w.first + i0) + x);
-            for (int i = i0; i < w.count; i += 2) {
+            auto page_of = [&](int j) { return j < w.now.pages.n ? w.table[w.now.pages.at(j)] : -1; };
+            int page[2] = {0, 0};                                   // (masked: entries of the page table, asked for a step ahead)
+            if (MASKED && i0 < count) { page[0] = page_of(2 * (first + i0)); page[1] = page_of(2 * (first + i0) + 1); }
+            for (int i = i0; i < count; i += 2) {
                 const int it = it0 + i, b = it % AS_BUFFERS;
                 const unsigned s_addr = lane_addr + b * AS_KTILE;
-                bool after[2] = {true, true};
+                bool there[2] = {live, live && i != odd_end};
+                if (MASKED) {
 #pragma unroll
-                for (int x = 0; x < 2; ++x) after[x] = i + 2 < w.count && there_at(2 * (w.first + i + 2) + x);
+                    for (int x = 0; x < 2; ++x) there[x] = live && (unsigned)page[x] < (unsigned)pool_pages;
+                    if (i + 2 < count) { page[0] = page_of(2 * (first + i + 2)); page[1] = page_of(2 * (first + i + 2) + 1); }
+                }
                 if (!at_wait_warp(at_smem(&s_full[b]), (unsigned)(it / AS_BUFFERS) & 1u)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 unsigned raw[AS_KTILE];
@@ -312,10 +331,10 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     float* sx = s + x * PE_PAGE;
-                    if (!there[x] || !live) {
+                    if (!there[x]) {
                         at_mask_behind<PE_PAGE>(sx, -1);
                     } else if (MASKED) {
-                        const int key0 = w.pages.at(2 * (w.first + i) + x) * PE_PAGE;
+                        const int key0 = w.now.pages.at(2 * (first + i) + x) * PE_PAGE;
                         if (p.window > 0 && key0 <= pos - p.window && key0 + PE_PAGE - 1 >= p.keep_first) {
                             const int lo = pos - p.window + 1 - key0, kept_here = p.keep_first - key0;
 #pragma unroll
@@ -381,26 +400,30 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) at_arrive(at_smem(&p_full[b]));
-                there[0] = after[0]; there[1] = after[1];
             }
             if (!ok) break;
             // ---- the tile's end: both groups write their half of O, and the reference point and sum of their own steps.  (Reference points only grow, and
             // the last step's is what O goes by: the larger of the two.)
-            const int last = it0 + w.count - 1;
+            const int last = it0 + count - 1;
+            it0 += count;
             if (!at_wait_warp(at_smem(&pv_done[last % AS_BUFFERS]), (unsigned)(last / AS_BUFFERS) & 1u)) { ok = false; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            float o[AS_HD / 2];
+            const size_t block = as_block(blockIdx.x, w.now.g, p.nh, p.nkv, w.kvh, w.tile);
+            if (live) reinterpret_cast<float2*>(p.scratch.ends + block + r)[g] = make_float2(m_mine, l_mine);
+            float* to = p.scratch.sums + block * AS_HD + r;
 #pragma unroll
-            for (int c = 0; c < AS_HD / 2; c += 32) at_ld32(lane_addr + AS_O_COL + g * (AS_HD / 2) + c, o + c);
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) at_arrive(at_smem(o_empty));
-            if (live) {
-                const size_t row = as_row(blockIdx.x, w.g, p.nh, p.nkv, w.kvh, w.tile * per_tile * R + r);
-                reinterpret_cast<float2*>(p.scratch.ends + row)[g] = make_float2(m_mine, l_mine);
-                float4* to = reinterpret_cast<float4*>(p.scratch.sums + row * AS_HD + g * (AS_HD / 2));
+            for (int c = 0; c < AS_HD / 2; c += 32) {
+                float o[32];
+                at_ld32(lane_addr + AS_O_COL + g * (AS_HD / 2) + c, o);
+                if (c + 32 == AS_HD / 2) {
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) at_arrive(at_smem(o_empty));
+                }
+                if (live) {                                         // a column at a time: the warp's rows lie side by side
 #pragma unroll
-                for (int c = 0; c < AS_HD / 8; ++c) to[c] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+                    for (int k = 0; k < 32; ++k) to[(size_t)(g * (AS_HD / 2) + c + k) * rows] = o[k];
+                }
             }
         }
         if (!ok) atomicExch(status, 7);
@@ -439,8 +462,9 @@ int as_launch(int grid, cudaStream_t stream, const CUtensorMap& mq, const CUtens
     return 0;
 }
 
-long long as_before_bytes(int T) { return ((long long)(T + 1) * 8 + 255) / 256 * 256; }
-long long as_rows(int T, int nh) { return (long long)pe_sm_count() * AS_QTILE + (long long)T * nh; }
+long long as_before_bytes(int T) { return ((long long)(T + 1) * 4 + 255) / 256 * 256; }
+int as_grid() { return pe_sm_count() < AS_MAX_CTAS ? pe_sm_count() : AS_MAX_CTAS; }
+long long as_rows(int T, int nh) { return (long long)as_grid() * AS_QTILE + (long long)T * nh; }
 
 }  // namespace
 
@@ -449,7 +473,7 @@ extern "C" long long pe_attention_shared_scratch(int T, int nh) { return as_befo
 // the kernel of attention_decode.cu for the rows' own positions
 int pe_attention_decode_own(const void* q, int q_stride, void* out, const void* k_pool, const void* v_pool, const int* block_table, int table_stride,
                             const int* tok_pos, const int* tok_row, int T, int nh, int nkv, int window, float scale, int max_context, int early_pages,
-                            int* status, void* stream, int keep_first, const float* slopes, const float* sinks, const void* groups, const AsScratch& scratch);
+                            int* status, void* stream, int keep_first, const float* slopes, const float* sinks, const void* groups, const AsScratch& scratch, int grid);
 
 extern "C" int pe_attention_shared(const void* q, int q_stride, void* out, const void* k_pool, const void* v_pool, long long pool_pages,
                                    const int* block_table, int table_stride, const int* tok_pos, const int* tok_row, const void* groups, int T,
@@ -459,6 +483,7 @@ extern "C" int pe_attention_shared(const void* q, int q_stride, void* out, const
     if (hd != AS_HD || nkv <= 0 || nh % nkv || nh / nkv > AS_QTILE || q_stride % 8 || !(scale > 0.f) || !status || !scratch || keep_first < 0) return PE_ERR_UNSUPPORTED;
     if (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)groups | (uintptr_t)scratch) & 15) return PE_ERR_UNSUPPORTED;
     if (pool_pages * nkv * PE_PAGE > 0x7fffff00ll) return PE_ERR_UNSUPPORTED;       // TMA coordinates are 32-bit
+    if ((long long)T * nkv * (table_stride / 2 + 1) > 0x7fffffffll) return PE_ERR_UNSUPPORTED;      // steps are counted in 32 bits
     const int R = nh / nkv;
     CUtensorMap mq, mk, mv;
     int rc = as_query_map(&mq, q, T, nh, q_stride, R, AS_QTILE / R);
@@ -471,14 +496,15 @@ extern "C" int pe_attention_shared(const void* q, int q_stride, void* out, const
     p.groups = (const int4*)groups; p.block_table = block_table; p.table_stride = table_stride; p.tok_pos = tok_pos; p.tok_row = tok_row;
     p.T = T; p.nh = nh; p.nkv = nkv; p.window = window; p.keep_first = window > 0 ? keep_first : 0; p.scale_log2e = scale * 1.4426950408889634f;
     p.slopes = slopes; p.inv_scale = 1.0f / scale; p.pool_rows = (int)(pool_pages * nkv * PE_PAGE);
-    p.scratch.before = (long long*)scratch;
+    p.early = early_pages != 0;
+    p.scratch.before = (int*)scratch;
     p.scratch.sums = (float*)((char*)scratch + as_before_bytes(T));
     p.scratch.ends = (float4*)(p.scratch.sums + as_rows(T, nh) * AS_HD);
-    rc = window > 0 || slopes ? as_launch<true>(pe_sm_count(), (cudaStream_t)stream, mq, mk, mv, p, status)
-                              : as_launch<false>(pe_sm_count(), (cudaStream_t)stream, mq, mk, mv, p, status);
+    rc = window > 0 || slopes ? as_launch<true>(as_grid(), (cudaStream_t)stream, mq, mk, mv, p, status)
+                              : as_launch<false>(as_grid(), (cudaStream_t)stream, mq, mk, mv, p, status);
     if (rc) return rc;
     return pe_attention_decode_own(q, q_stride, out, k_pool, v_pool, block_table, table_stride, tok_pos, tok_row, T, nh, nkv, window, scale, max_context,
-                                   early_pages, status, stream, p.keep_first, slopes, sinks, groups, p.scratch);
+                                   early_pages, status, stream, p.keep_first, slopes, sinks, groups, p.scratch, as_grid());
 }
 
 #else   // other head sizes: the rows of a group are read one by one (attention_decode.cu)
