@@ -233,77 +233,91 @@ struct AdGroups { const int4* groups; AsScratch scratch; int T, grid; };
 // What a token has to join: the CTAs c0 .. c1 - 1 of attention_shared.cu had steps of its tile.  weights[c - c0][row] is what the sums of
 // CTA c count, group_max[row] and group_sum[row] are maximum and weight of all of them (16 rows: query heads of the tile of heads).
 struct AdJoin {
-    int c0, c1, tile_rows, row; size_t block;       // row: of the tile, of the first query head here
+    int c0, c1; size_t row;                         // row: of the first query head here, of CTA 0
     // Before the kernel in front has ended, where the steps can be counted here (a warp, some tokens a lane); else from what it has written.
-    __device__ __forceinline__ void find(const AdGroups& p, const int4& g, int tok, int shared, const int* tok_pos, int table_stride, int window, int keep_first,
-                                         int nh, int nkv, int kvh, int head0, int lane) {
+    __device__ __forceinline__ void find(const AdGroups& p, const int4& g, int tok, int shared, const int* tok_pos, const int* tok_row, int table_stride, int window,
+                                         int keep_first, int nh, int nkv, int kvh, int head0, int lane) {
         c0 = c1 = 0;
-        tile_rows = 1; row = 0; block = 0;
+        row = 0;
         if (shared == 0) return;
-        int before = 0, steps = 0;
-        if (p.T <= AS_COUNTED) {
-            for (int t = lane; t < p.T; t += 32) {
-                AsGroup at;
-                at.load(p.groups, tok_pos, t, p.T, table_stride, nh, nkv, window, keep_first);
-                steps += at.steps;
-                before += t < g.x ? at.steps : 0;
-            }
+        int steps = 0, tiles = 0, before = 0;
+        AsGroup at;
+        const auto load = [&](int t) { at.tiles = 0; if (t < p.T) at.load(p.groups, tok_pos, tok_row, t, p.T, table_stride, nh, nkv, window, keep_first); };
+        const bool counted = p.T <= AS_COUNTED;
+        if (counted) {
+            for (int t = lane; t < p.T; t += 32) { load(t); steps += at.steps(); tiles += at.tiles; }
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) { steps += __shfl_xor_sync(0xffffffffu, steps, o); before += __shfl_xor_sync(0xffffffffu, before, o); }
+            for (int o = 16; o > 0; o >>= 1) { steps += __shfl_xor_sync(0xffffffffu, steps, o); tiles += __shfl_xor_sync(0xffffffffu, tiles, o); }
         } else {
             pdl_wait();
             before = p.scratch.before[g.x];
             steps = p.scratch.before[p.T];
+            tiles = p.scratch.before[p.T + 1];
         }
-        const int R = nh / nkv, per_tile = AS_QTILE / R, i = tok - g.x, tile = i / per_tile, tiles = as_tiles(g, nh, nkv);
-        const int n_steps = as_tile_steps(as_pages(shared, window > 0 ? tok_pos[g.w] : 0, window, keep_first));
-        const int first = before + (kvh * tiles + tile) * n_steps;
-        if (n_steps == 0 || steps <= 0 || first < 0 || first > steps - n_steps) return;      // (nothing to join, or the kernel in front has given up)
-        const AsDeal d(steps, p.grid);
-        c0 = d.cta_of(first);
-        c1 = d.cta_of(first + n_steps - 1) + 1;
-        tile_rows = min(per_tile, g.y - tile * per_tile) * R;
-        row = (i - tile * per_tile) * R + head0;
-        block = as_block(0, g, nh, nkv, kvh, tile);
+        if (steps <= 0 || tiles <= 0) return;
+        const AsDeal d(steps, tiles, p.grid);
+        if (counted) {
+            if (p.T > 32) {
+                for (int t = lane; t < g.x; t += 32) { load(t); before += at.units(d); }
+            } else {
+                before = lane < g.x ? at.units(d) : 0;       // (in hand)
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+        }
+        const int R = nh / nkv, per_tile = AS_QTILE / R, i = tok - g.x, tile = i / per_tile;
+        const int n = as_tile_steps(as_pages(shared, window > 0 ? tok_pos[g.w] : 0, window, keep_first));
+        const int first = before + (kvh * as_tiles(g, nh, nkv) + tile) * d.units(n);
+        if (n == 0 || first < 0 || first > steps - 1) return;     // (nothing to join, or the kernel in front has given up)
+        const int2 c = d.ctas_of(first, n);
+        c0 = min(max(c.x, 0), p.grid);
+        c1 = min(c.y, p.grid);
+        row = as_block(0, g, nh, nkv, kvh, tile) + (size_t)((i - tile * per_tile) * R + head0);
     }
     // a warp for every row: the lanes take the CTAs in turn
     __device__ __forceinline__ void weigh(const AdGroups& p, int j, int lane, float* weights, float* top_of, float* weight_of) const {
-        const float4* ends = p.scratch.ends + block + row + j;
-        float top = -INFINITY, sum = 0.f;
-        for (int c = c0 + lane; c < c1; c += 32) {
-            const float4 e = ends[(size_t)c * AS_QTILE];
-            top = fmaxf(top, fmaxf(e.x, e.z));
-        }
+        const float4* ends = p.scratch.ends + row + j;
+        const auto end_of = [&](int c) { return c < c1 ? ends[(size_t)c * AS_QTILE] : make_float4(-INFINITY, 0.f, -INFINITY, 0.f); };
+        const float4 mine = end_of(c0 + lane);
+        float top = fmaxf(mine.x, mine.z), sum = 0.f;
+        for (int c = c0 + 32 + lane; c < c1; c += 32) { const float4 e = end_of(c); top = fmaxf(top, fmaxf(e.x, e.z)); }
         top = warp_max(top);
         const auto weight = [&](float at) { return at == -INFINITY ? 0.f : ad_ex2(at - top); };
         for (int c = c0 + lane; c < c1; c += 32) {
-            const float4 e = ends[(size_t)c * AS_QTILE];
+            const float4 e = c == c0 + lane ? mine : end_of(c);
             sum = fmaf(e.y, weight(e.x), fmaf(e.w, weight(e.z), sum));
             weights[(c - c0) * 16 + j] = weight(fmaxf(e.x, e.z));
         }
         sum = warp_sum(sum);
         if (lane == 0) { top_of[j] = top; weight_of[j] = sum; }
     }
-    // The sums of the outputs `first`, `first` + `step`, .. (N of them, below `end`; output x is row x % rows, column col0 + x / rows): all loads of a CTA's block
-    // are asked for before the first is used
+    // The sums of the outputs `first`, `first` + `step`, .. (N of them, below `end`; output x is row x / cols, column col0 + x % cols), some CTAs' at a time: all their
+    // loads are asked for before the first is used
     template <int N>
-    __device__ __forceinline__ void sums(const AdGroups& p, int first, int step, int end, int rows, int col0, const float* weights, float (&o)[N]) const {
+    __device__ __forceinline__ void sums(const AdGroups& p, int first, int step, int end, int cols, int col0, const float* weights, float (&o)[N]) const {
+        constexpr int AT_ONCE = N >= 16 ? 1 : 16 / N;
         size_t at[N];
         int j[N];
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const int x = first + k * step < end ? first + k * step : 0;
-            j[k] = x % rows;
-            at[k] = block * AD_HD + (size_t)(col0 + x / rows) * tile_rows + row + j[k];
+            j[k] = x / cols;
+            at[k] = (row + j[k]) * AD_HD + col0 + x % cols;
             o[k] = 0.f;
         }
-#pragma unroll 2
-        for (int c = c0; c < c1; ++c) {
-            float v[N];
+        for (int c = c0; c < c1; c += AT_ONCE) {
+            float v[AT_ONCE][N];
 #pragma unroll
-            for (int k = 0; k < N; ++k) v[k] = p.scratch.sums[at[k] + (size_t)c * (AS_QTILE * AD_HD)];
+            for (int e = 0; e < AT_ONCE; ++e)
 #pragma unroll
-            for (int k = 0; k < N; ++k) o[k] = fmaf(v[k], weights[(c - c0) * 16 + j[k]], o[k]);
+                for (int k = 0; k < N; ++k) v[e][k] = c + e < c1 ? p.scratch.sums[at[k] + (size_t)(c + e) * (AS_QTILE * AD_HD)] : 0.f;
+#pragma unroll
+            for (int e = 0; e < AT_ONCE; ++e)
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    const float w = c + e < c1 ? weights[(c + e - c0) * 16 + j[k]] : 0.f;
+                    o[k] = w == 0.f ? o[k] : fmaf(v[e][k], w, o[k]);
+                }
         }
     }
 };
@@ -424,6 +438,11 @@ __global__ void __launch_bounds__(32 * (AD_WARPS + 1), AD_CTAS(AD_WARPS)) attent
             }
             alive = __shfl_sync(0xffffffffu, alive, 0);
         }
+        if constexpr (OWN) {                                     // which of the group's results to join: found while the others compute
+            AdJoin join;
+            join.find(grouped, group, tok, shared, tok_pos, tok_row, table_stride, window, kept_keys, nh, nkv, kvh, ht * 16, lane);
+            if (lane == 0) join_s[0] = join;
+        }
     } else {
         // ---- the consumers
         const int last_phys = table[last_page];               // the page of the newest token
@@ -492,17 +511,14 @@ __global__ void __launch_bounds__(32 * (AD_WARPS + 1), AD_CTAS(AD_WARPS)) attent
         }
     }
 
-    if constexpr (OWN) {
-        // what the group has left, when it has: found before the kernel in front has ended, read behind it
-        AdJoin join;
-        join.find(grouped, group, tok, shared, tok_pos, table_stride, window, kept_keys, nh, nkv, kvh, ht * 16, lane);
-        pdl_wait();
-        for (int row = warp; row < rows; row += AD_WARPS + 1) join.weigh(grouped, row, lane, weights, group_max, group_sum);
-        if (threadIdx.x == 0) join_s[0] = join;
-    }
     // ---- merge the warps: the ring is free once every warp has left its loop.  Each warp scales its sums
     // to the CTA's max of the row first, so that merging is adding.
     __syncthreads();
+    if constexpr (OWN) {
+        pdl_wait();                                              // the kernel in front has left its results
+        const AdJoin join = join_s[0];
+        for (int row = warp; row < rows; row += AD_WARPS + 1) join.weigh(grouped, row, lane, weights, group_max, group_sum);
+    }
     float* part = reinterpret_cast<float*>(ring);           // [AD_WARPS][16][AD_ROW] sums, then per (warp, row): max, sum
     float* w_max = part + AD_WARPS * 16 * AD_ROW;
     float* w_sum = w_max + AD_WARPS * 16;
@@ -542,24 +558,29 @@ __global__ void __launch_bounds__(32 * (AD_WARPS + 1), AD_CTAS(AD_WARPS)) attent
         m = top;
     };
     if constexpr (OWN) {
-        if (n_splits == 1) {                                 // outputs row by row within a column, as the group's results lie
-            constexpr int N = (16 * AD_HD + AD_THREADS - 1) / AD_THREADS;
-            float theirs[N];
+        if (n_splits == 1) {
+            constexpr int N = (16 * AD_HD + AD_THREADS - 1) / AD_THREADS, HALF = (N + 1) / 2;      // in two turns: up to eight rows, and the others
             const AdJoin join = join_s[0];
-            join.sums(grouped, threadIdx.x, AD_THREADS, rows * AD_HD, rows, 0, weights, theirs);
 #pragma unroll
-            for (int k = 0; k < N; ++k) {
-                const int x = threadIdx.x + k * AD_THREADS, row = x % rows, col = x / rows;
-                if (x >= rows * AD_HD) break;
-                float m = row_max[row], o = 0.f, l = 0.f;
+            for (int x0 = 0; x0 < 2; ++x0) {
+                const int at0 = threadIdx.x + x0 * HALF * AD_THREADS;
+                if (x0 * HALF * AD_THREADS >= rows * AD_HD) break;
+                float theirs[HALF];
+                join.sums(grouped, at0, AD_THREADS, rows * AD_HD, AD_HD, 0, weights, theirs);
 #pragma unroll
-                for (int w = 0; w < AD_WARPS; ++w) {
-                    o += part[((size_t)w * 16 + row) * AD_ROW + col];
-                    l += w_sum[w * 16 + row];
+                for (int k = 0; k < HALF; ++k) {
+                    const int x = at0 + k * AD_THREADS, row = x / AD_HD, col = x % AD_HD;
+                    if (x >= rows * AD_HD) break;
+                    float m = row_max[row], o = 0.f, l = 0.f;
+#pragma unroll
+                    for (int w = 0; w < AD_WARPS; ++w) {
+                        o += part[((size_t)w * 16 + row) * AD_ROW + col];
+                        l += w_sum[w * 16 + row];
+                    }
+                    with_group(row, theirs[k], m, l, o);
+                    if (sinks) l += exp2f(fmaf(sinks[kvh * G + ht * 16 + row], 1.4426950408889634f, -m));
+                    out[((size_t)tok * nh + kvh * G + ht * 16 + row) * AD_HD + col] = __float2bfloat16_rn(l > 0.f ? o / l : 0.f);
                 }
-                with_group(row, theirs[k], m, l, o);
-                if (sinks) l += exp2f(fmaf(sinks[kvh * G + ht * 16 + row], 1.4426950408889634f, -m));
-                out[((size_t)tok * nh + kvh * G + ht * 16 + row) * AD_HD + col] = __float2bfloat16_rn(l > 0.f ? o / l : 0.f);
             }
             return;
         }
@@ -607,11 +628,11 @@ __global__ void __launch_bounds__(32 * (AD_WARPS + 1), AD_CTAS(AD_WARPS)) attent
     float theirs[N_SLICE];
     if constexpr (OWN) {
         const AdJoin join = join_s[0];
-        if (my_cols > 0) join.sums(grouped, threadIdx.x, AD_THREADS, rows * my_cols, rows, split * slice, weights, theirs);
+        if (my_cols > 0) join.sums(grouped, threadIdx.x, AD_THREADS, rows * my_cols, my_cols, split * slice, weights, theirs);
     }
     int turn = 0;
     for (int idx = threadIdx.x; idx < rows * my_cols; idx += AD_THREADS, ++turn) {
-        const int row = OWN ? idx % rows : idx / my_cols, j = OWN ? idx / rows : idx - row * my_cols;
+        const int row = idx / my_cols, j = idx - row * my_cols;
         float m = -INFINITY;
         for (int r = 0; r < n_splits; ++r) m = fmaxf(m, gather[(r * 16 + row) * grow + slice]);
         float o = 0.f, l = 0.f;

@@ -8,9 +8,9 @@
 // scratch, and the kernel of attention_decode.cu, which follows and reads each row's own positions, joins them:
 // m = max m_i, l = sum l_i 2^(m_i - m), o = sum o_i 2^(m_i - m).
 //
-//   a persistent CTA an SM takes an equal share of all steps (attention_shared.cuh), tile after tile
+//   a CTA an SM takes an equal share of all steps (attention_shared.cuh)
 //   warp 0      loader: the tile's queries as one box [tokens][heads of the key head][64 columns], and two pages of keys and values a step
-//   warp 1      issues S = Q.K^T three steps ahead of O += P.V, across the border of tiles
+//   warp 1      issues S = Q.K^T three steps ahead of O += P.V
 //   warps 2-9   softmax, two warpgroups that take the steps in turn (as in attention_prefill_tcgen05.cu); at the end of a tile both write their half of O
 //
 // All keys of a step are visible to all rows but for windows, pages that are not there and the half step behind an odd number of pages, so
@@ -34,8 +34,9 @@
 #define AS_STAGE_BYTES (2 * AS_HALF_BYTES)
 #define AS_TILE_BYTES (AS_Q_BYTES + AS_STAGES * AS_STAGE_BYTES)
 #define AS_BUFFERS 3
-#define AS_BARS (4 + 3 * AS_BUFFERS + 4 * AS_STAGES + 8)
-#define AS_SMEM_BYTES (AS_TILE_BYTES + 8 * AS_BARS + 2 * AS_QTILE * 4)
+#define AS_BARS ((4 + 3 * AS_BUFFERS + 4 * AS_STAGES + 8 + 1) / 2 * 2)      // (what follows them lies on 16 bytes)
+#define AS_WALKS (AS_THREADS / 32 + 1)             // the first tile; a warp's each
+#define AS_SMEM_BYTES (AS_TILE_BYTES + 8 * AS_BARS + 2 * AS_QTILE * 4 + AS_WALKS * (int)sizeof(AsWalk) + 2 * (AS_THREADS / 32) * 4)
 #define AS_O_COL (AS_BUFFERS * AS_KTILE)
 #define AS_LAZY 8.0f
 
@@ -48,30 +49,32 @@ struct AsArgs {
 // A CTA's tiles one after the other.  Every warp walks its own copy, in shared memory: one lane takes the step, all of them read.
 struct AsWalk {
     AsGroup now;
-    int x, end;                                    // the next step, and where the CTA's end
+    int x, end;                                    // the next unit, and where the CTA's end
     int kvh, tile, first, count;                   // the tile, and its steps here
     const int* table;                              // the page table's row that names the shared pages
-    __device__ __forceinline__ bool step(const AsArgs& p) {
-        x += count;
-        if (x >= end) return false;
-        bool moved = count == 0;
-        while (x >= now.before + now.steps) {
-            const int before = now.before + now.steps;
-            now.load(p.groups, p.tok_pos, now.t + (now.steps > 0 ? now.g.y : 1), p.T, p.table_stride, p.nh, p.nkv, p.window, p.keep_first);
-            now.before = before;
-            moved = true;
-        }
-        if (moved) table = p.block_table + (size_t)p.tok_row[now.g.w] * p.table_stride;
-        const int o = x - now.before, n = as_tile_steps(now.pages), tiles = as_tiles(now.g, p.nh, p.nkv), seg = o / n;
-        first = o - seg * n;
+    __device__ __forceinline__ void load(const AsArgs& p, int t) { now.load(p.groups, p.tok_pos, p.tok_row, t, p.T, p.table_stride, p.nh, p.nkv, p.window, p.keep_first); }
+    __device__ __forceinline__ void place(const AsArgs& p, const AsDeal& d) {
+        table = p.block_table + (size_t)now.row * p.table_stride;
+        const int n = as_tile_steps(now.pages), units = d.units(n), tiles = as_tiles(now.g, p.nh, p.nkv), o = x - now.before, seg = o / units, j = o - seg * units;
         kvh = seg / tiles; tile = seg - kvh * tiles;
-        count = min(n - first, end - x);
+        first = d.chunk ? (int)((long long)n * j / units) : j;
+        count = d.chunk ? (int)((long long)n * (j + 1) / units) - first : min(n - first, end - x);
+    }
+    __device__ __forceinline__ bool step(const AsArgs& p, const AsDeal& d) {
+        x += d.chunk ? 1 : count;
+        if (x >= end) return false;
+        while (x >= now.before + now.units(d)) {
+            const int before = now.before + now.units(d);
+            load(p, now.t + (now.tiles > 0 ? now.g.y : 1));
+            now.before = before;
+        }
+        place(p, d);
         return true;
     }
-    __device__ __forceinline__ bool next(const AsArgs& p, int lane) {        // the whole warp
+    __device__ __forceinline__ bool next(const AsArgs& p, const AsDeal& d, int lane) {        // the whole warp
         bool more = false;
         __syncwarp();
-        if (lane == 0) more = step(p);
+        if (lane == 0) more = step(p, d);
         __syncwarp();
         return __shfl_sync(0xffffffffu, more, 0);
     }
@@ -90,8 +93,9 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
     unsigned long long *k_full = pv_done + AS_BUFFERS, *v_full = k_full + AS_STAGES, *k_empty = v_full + AS_STAGES, *v_empty = k_empty + AS_STAGES;
     unsigned long long* told = v_empty + AS_STAGES;                 // [warpgroup][32 rows]: a step's reference points are there
     float* refs = reinterpret_cast<float*>(bars + AS_BARS);         // [warpgroup][row]: reference point of the group's last step
-    __shared__ int scan[AS_THREADS / 32];
-    __shared__ AsWalk walks[AS_THREADS / 32 + 2];                   // the first tile; a warp's each; the second one of the issuer
+    AsWalk* walks = reinterpret_cast<AsWalk*>(refs + 2 * AS_QTILE);
+    static_assert((AS_TILE_BYTES + 8 * AS_BARS + 2 * AS_QTILE * 4) % alignof(AsWalk) == 0, "the walks' place");
+    int (*scan)[AS_THREADS / 32] = reinterpret_cast<int (*)[AS_THREADS / 32]>(walks + AS_WALKS);
     if (q_s & 1023u) {                                              // every thread alike: nothing is allocated yet
         if (threadIdx.x == 0) atomicExch(status, 6);
         return;
@@ -100,62 +104,65 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
     // shared pages.  Queries, and the scratch that the call before may still be reading, wait.
     if (!p.early) pdl_wait();
 
-    // ---- this CTA's share of the steps: a scan over the groups (a token a thread; the second time round only where there are more tokens)
+    // ---- this CTA's share of the steps: all steps and tiles, then a scan over the groups' units (a token a thread; tokens beyond are read again)
     AsGroup mine;
-    mine.steps = 0;
-    auto load = [&](int t) { mine.load(p.groups, p.tok_pos, t, p.T, p.table_stride, p.nh, p.nkv, p.window, p.keep_first); };
-    if ((int)threadIdx.x < p.T) load(threadIdx.x);
+    auto load = [&](int t) {
+        mine.tiles = 0;
+        if (t < p.T) mine.load(p.groups, p.tok_pos, p.tok_row, t, p.T, p.table_stride, p.nh, p.nkv, p.window, p.keep_first);
+    };
+    load(threadIdx.x);
     if (threadIdx.x == 32) {
         auto init = [](unsigned long long* bar, unsigned count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(at_smem(bar)), "r"(count) : "memory"); };
-        init(q_full, 1); init(q_empty, 1); init(o_empty, 8);
+        init(q_full, 1); init(q_empty, 8); init(o_empty, 8);         // q_empty: the eight warps that write the tile's results through the queries' place
         for (int s = 0; s < AS_STAGES; ++s) { init(&k_full[s], 1); init(&v_full[s], 1); init(&k_empty[s], 1); init(&v_empty[s], 1); }
         for (int b = 0; b < AS_BUFFERS; ++b) { init(&s_full[b], 1); init(&p_full[b], 4); init(&pv_done[b], 1); }
         for (int w = 0; w < 8; ++w) init(&told[w], 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
     }
-    int begin = 0, end = 0, total = 0;
-    auto deal = [&] {
-        const AsDeal d(total, gridDim.x);
-        if ((int)blockIdx.x < d.ctas) { begin = d.begin(blockIdx.x); end = d.begin(blockIdx.x + 1); }
-    };
-    for (int pass = 0; pass < 2; ++pass) {
-        int run = 0;
-        for (int base = 0; base < p.T; base += AS_THREADS) {
-            const int t = base + threadIdx.x;
-            if (p.T > AS_COUNTED && (base > 0 || pass > 0)) {
-                mine.steps = 0;
-                if (t < p.T) load(t);
-            }
-            int sum = mine.steps;
+    int steps = 0, tiles = 0;
+    for (int base = AS_THREADS; base < p.T; base += AS_THREADS) { steps += mine.steps(); tiles += mine.tiles; load(base + threadIdx.x); }
+    steps += mine.steps(); tiles += mine.tiles;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int up = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= o) sum += up;
-            }
-            __syncthreads();
-            if (lane == 31) scan[warp] = sum;
-            __syncthreads();
-            mine.before = run + sum - mine.steps;
+    for (int o = 16; o > 0; o >>= 1) { steps += __shfl_xor_sync(0xffffffffu, steps, o); tiles += __shfl_xor_sync(0xffffffffu, tiles, o); }
+    if (lane == 0) { scan[0][warp] = steps; scan[1][warp] = tiles; }
+    __syncthreads();
+    steps = tiles = 0;
 #pragma unroll
-            for (int w = 0; w < AS_THREADS / 32; ++w) {
-                if (w < warp) mine.before += scan[w];
-                run += scan[w];
-            }
-            if (pass == 0 && p.T > AS_COUNTED && blockIdx.x == 0 && t < p.T) { pdl_wait(); p.scratch.before[t] = mine.before; }
-            if (pass == 0 && p.T <= AS_COUNTED) { total = run; deal(); }         // all groups are in hand
-            if ((pass == 1 || p.T <= AS_COUNTED) && begin < end && begin >= mine.before && begin < mine.before + mine.steps) {
-                walks[0].now = mine;
-                walks[0].x = begin; walks[0].end = end; walks[0].count = 0;
-                walks[0].step(p);                                   // the first tile
-            }
+    for (int w = 0; w < AS_THREADS / 32; ++w) { steps += scan[0][w]; tiles += scan[1][w]; }
+    const AsDeal deal(steps, tiles, gridDim.x);
+    if (p.T > AS_THREADS) {
+        load(threadIdx.x);
+        if (blockIdx.x == 0 && threadIdx.x == 0) { pdl_wait(); p.scratch.before[p.T] = steps; p.scratch.before[p.T + 1] = tiles; }
+    }
+    int begin = 0, end = 0, units = 0;                              // this CTA's units, and all so far
+    if (!deal.chunk && (int)blockIdx.x < deal.ctas) { begin = deal.begin(blockIdx.x); end = deal.begin(blockIdx.x + 1); }
+    if (deal.chunk) { begin = blockIdx.x; end = begin + 1; }
+    for (int base = 0; base < p.T; base += AS_THREADS) {
+        if (base > 0) load(base + threadIdx.x);
+        const int own = mine.units(deal);
+        int sum = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += up;
         }
-        if (pass == 0) {
-            if (p.T <= AS_COUNTED) break;
-            total = run;
-            deal();
-            if (blockIdx.x == 0 && threadIdx.x == 0) { pdl_wait(); p.scratch.before[p.T] = total; }
+        __syncthreads();
+        if (lane == 31) scan[0][warp] = sum;
+        __syncthreads();
+        mine.before = units + sum - own;
+#pragma unroll
+        for (int w = 0; w < AS_THREADS / 32; ++w) {
+            if (w < warp) mine.before += scan[0][w];
+            units += scan[0][w];
+        }
+        if (p.T > AS_COUNTED && blockIdx.x == 0 && base + (int)threadIdx.x < p.T) { pdl_wait(); p.scratch.before[base + threadIdx.x] = mine.before; }
+        if (begin < end && begin >= mine.before && begin < mine.before + own) {
+            AsWalk& w = walks[0];
+            w.now = mine; w.x = begin; w.end = end;
+            w.place(p, deal);                                       // the first tile
         }
     }
+    if (begin >= units) end = begin;
     if (begin >= end) {                                             // (the whole block)
         pdl_wait();
         pdl_launch_dependents();
@@ -172,9 +179,9 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
     const int R = p.nh / p.nkv, per_tile = AS_QTILE / R, pool_pages = p.pool_rows / (p.nkv * PE_PAGE);
     // (the first tile has been found; a warp's own copy goes on from there)
     AsWalk& w = walks[warp + 1];
-    if (lane == 0) { w = walks[0]; if (warp == 1) walks[AS_THREADS / 32 + 1] = walks[0]; }
+    if (lane == 0) w = walks[0];
     __syncwarp();
-    auto advance = [&](int seg) { return seg == 0 ? true : w.next(p, lane); };
+    auto advance = [&](int seg) { return seg == 0 ? true : w.next(p, deal, lane); };
 
     if (warp == 0) {                                                // ---------------- loader: one lane asks, the others wait for the walk
         bool ok = true;
@@ -237,18 +244,9 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
         const unsigned idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(AS_KTILE >> 3) << 17) | ((unsigned)(AS_QTILE >> 4) << 24);
         const unsigned idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((unsigned)(AS_HD >> 3) << 17) | ((unsigned)(AS_QTILE >> 4) << 24);
         const unsigned long long dq = at_desc(q_s, 0, 1024), dk = at_desc(kv_s, 0, 1024), dv = at_desc(kv_s + AS_HALF_BYTES, AS_KTILE * 128, 1024);
-        const int steps = end - begin;
-        AsWalk& ahead = walks[AS_THREADS / 32 + 1];                 // the tile that S has come to
-        int a_left = ahead.count, a_seg = 0;
-        bool ok = at_wait_warp(at_smem(q_full), 0u);
+        bool ok = true;
         auto issue_s = [&](int it) -> bool {
             const int s = it % AS_STAGES, b = it % AS_BUFFERS;
-            if (a_left == 0) {                                      // the next tile's queries
-                ahead.next(p, lane);
-                a_left = ahead.count;
-                ++a_seg;
-                if (!at_wait_warp(at_smem(q_full), (unsigned)a_seg & 1u)) return false;
-            }
             if (it >= AS_BUFFERS && !at_wait_warp(at_smem(&pv_done[b]), (unsigned)(it / AS_BUFFERS - 1) & 1u)) return false;
             if (!at_wait_warp(at_smem(&k_full[s]), (unsigned)(it / AS_STAGES) & 1u)) return false;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -260,14 +258,14 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
             }
             at_commit_by(elected, at_smem(&k_empty[s]));
             at_commit_by(elected, at_smem(&s_full[b]));
-            if (--a_left == 0) at_commit_by(elected, at_smem(q_empty));      // the tile's queries have been read
             return true;
         };
-        for (int it = 0; it < min(AS_AHEAD, steps) && ok; ++it) ok = issue_s(it);
         int it = 0;
-        for (int seg = 0; ok && advance(seg); ++seg) {
+        for (int seg = 0; ok && advance(seg); ++seg) {              // S never runs into the next tile: its queries come when this one's results have left their place
             const int count = w.count;
-            for (int i = 0; i < count; ++i, ++it) {
+            ok = at_wait_warp(at_smem(q_full), (unsigned)seg & 1u);
+            for (int i = 0; ok && i < min(AS_AHEAD, count); ++i) ok = issue_s(it + i);
+            for (int i = 0; ok && i < count; ++i, ++it) {
                 const int s = it % AS_STAGES, b = it % AS_BUFFERS;
                 if (!at_wait_warp(at_smem(&v_full[s]), (unsigned)(it / AS_STAGES) & 1u)) { ok = false; break; }
                 if (!at_wait_warp(at_smem(&p_full[b]), (unsigned)(it / AS_BUFFERS) & 1u)) { ok = false; break; }
@@ -279,7 +277,7 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
                     at_mma_ts(elected, tmem + AS_O_COL, tmem + b * AS_KTILE + kk * 8, dvs + ((kk * 16 * 128) >> 4), idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
                 at_commit_by(elected, at_smem(&v_empty[s]));
                 at_commit_by(elected, at_smem(&pv_done[b]));
-                if (it + AS_AHEAD < steps && !issue_s(it + AS_AHEAD)) { ok = false; break; }
+                if (i + AS_AHEAD < count && !issue_s(it + AS_AHEAD)) { ok = false; break; }
             }
         }
         if (!ok) atomicExch(status, 7);
@@ -410,7 +408,10 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const size_t block = as_block(blockIdx.x, w.now.g, p.nh, p.nkv, w.kvh, w.tile);
             if (live) reinterpret_cast<float2*>(p.scratch.ends + block + r)[g] = make_float2(m_mine, l_mine);
-            float* to = p.scratch.sums + block * AS_HD + r;
+            // through the queries' place (the last S has read them), 16 columns of the warp's 32 rows at a time, 16-byte pieces exchanged by the row inside
+            // a run of four: a lane storing its own row would touch 32 lines an instruction
+            const unsigned stage = q_s + (warp - 2) * 2048;
+            float* to = p.scratch.sums + block * AS_HD + g * (AS_HD / 2);
 #pragma unroll
             for (int c = 0; c < AS_HD / 2; c += 32) {
                 float o[32];
@@ -420,11 +421,26 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
                     __syncwarp();
                     if (lane == 0) at_arrive(at_smem(o_empty));
                 }
-                if (live) {                                         // a column at a time: the warp's rows lie side by side
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) to[(size_t)(g * (AS_HD / 2) + c + k) * rows] = o[k];
+                for (int half = 0; half < 2; ++half) {
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(stage + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)), "f"(o[16 * half + 4 * k]), "f"(o[16 * half + 4 * k + 1]),
+                                     "f"(o[16 * half + 4 * k + 2]), "f"(o[16 * half + 4 * k + 3]) : "memory");
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {                   // eight rows an instruction
+                        const int x = 8 * k + (lane >> 2), row = quarter * 32 + x;
+                        float4 v;
+                        asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(stage + x * 64 + (((lane & 3) ^ ((x >> 1) & 3)) << 4)) : "memory");
+                        if (row < rows) *reinterpret_cast<float4*>(to + (size_t)row * AS_HD + c + 16 * half + 4 * (lane & 3)) = v;
+                    }
                 }
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // (the next tile's queries come by another proxy)
+            __syncwarp();
+            if (lane == 0) at_arrive(at_smem(q_empty));
         }
         if (!ok) atomicExch(status, 7);
     }
@@ -462,7 +478,7 @@ int as_launch(int grid, cudaStream_t stream, const CUtensorMap& mq, const CUtens
     return 0;
 }
 
-long long as_before_bytes(int T) { return ((long long)(T + 1) * 4 + 255) / 256 * 256; }
+long long as_before_bytes(int T) { return ((long long)(T + 2) * 4 + 255) / 256 * 256; }
 int as_grid() { return pe_sm_count() < AS_MAX_CTAS ? pe_sm_count() : AS_MAX_CTAS; }
 long long as_rows(int T, int nh) { return (long long)as_grid() * AS_QTILE + (long long)T * nh; }
 
