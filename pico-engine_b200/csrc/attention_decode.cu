@@ -29,7 +29,7 @@
 #ifndef PE_HEAD_DIM
 #error "compile with -DPE_HEAD_DIM=<head size>"
 #endif
-#include "attention_shared.cuh"
+#include "common.cuh"
 #include <map>
 #include <mutex>
 #include <utility>
@@ -111,12 +111,6 @@ __device__ __forceinline__ uint4 ad_ld16(const bf16* p) {
     asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
     return v;
 }
-// the same past the first-level cache, for a kernel that reads them without having waited itself
-__device__ __forceinline__ uint4 ad_ld16_l2(const bf16* p) {
-    uint4 v;
-    asm volatile("ld.global.cg.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
-    return v;
-}
 __device__ __forceinline__ void ad_mma(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
                                        unsigned b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -127,11 +121,6 @@ __device__ __forceinline__ unsigned ad_transpose(unsigned a) {
     unsigned d;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
-}
-__device__ __forceinline__ float ad_ex2(float x) {          // 2^x; 2^-inf = 0
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 __device__ __forceinline__ unsigned ad_pack(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
@@ -144,6 +133,11 @@ __device__ __forceinline__ unsigned ad_pack(float lo, float hi) {
 // qf[c][0/1] (rows g / g + 8) and the 16-byte loads of key rows hold columns c*32 + t*8 .. +8,
 // so both operands of S = Q.K^T see the head dimension in the same permuted order.
 
+__device__ __forceinline__ float ad_ex2(float x) {          // 2^x; 2^-inf = 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 // One tile of 16 keys against the warp's 16 query rows.  kt, vt: shared-memory addresses of the
 // tile's first key and value row; key0: position of that key.  At least one key of the tile is
@@ -227,109 +221,12 @@ __device__ __forceinline__ void ad_consume(float (&acc)[AD_NCHUNK][4][4], float 
     }
 }
 
-// What the joined form (OWN) has to know: the groups of the step's tokens and where attention_shared.cu has left its partial results.
-struct AdGroups { const int4* groups; AsScratch scratch; int T, grid; };
-
-// What a token has to join: the CTAs c0 .. c1 - 1 of attention_shared.cu had steps of its tile.  weights[c - c0][row] is what the sums of
-// CTA c count, group_max[row] and group_sum[row] are maximum and weight of all of them (16 rows: query heads of the tile of heads).
-struct AdJoin {
-    int c0, c1; size_t row;                         // row: of the first query head here, of CTA 0
-    // Before the kernel in front has ended, where the steps can be counted here (a warp, some tokens a lane); else from what it has written.
-    __device__ __forceinline__ void find(const AdGroups& p, const int4& g, int tok, int shared, const int* tok_pos, const int* tok_row, int table_stride, int window,
-                                         int keep_first, int nh, int nkv, int kvh, int head0, int lane) {
-        c0 = c1 = 0;
-        row = 0;
-        if (shared == 0) return;
-        int steps = 0, tiles = 0, before = 0;
-        AsGroup at;
-        const auto load = [&](int t) { at.tiles = 0; if (t < p.T) at.load(p.groups, tok_pos, tok_row, t, p.T, table_stride, nh, nkv, window, keep_first); };
-        const bool counted = p.T <= AS_COUNTED;
-        if (counted) {
-            for (int t = lane; t < p.T; t += 32) { load(t); steps += at.steps(); tiles += at.tiles; }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) { steps += __shfl_xor_sync(0xffffffffu, steps, o); tiles += __shfl_xor_sync(0xffffffffu, tiles, o); }
-        } else {
-            pdl_wait();
-            before = p.scratch.before[g.x];
-            steps = p.scratch.before[p.T];
-            tiles = p.scratch.before[p.T + 1];
-        }
-        if (steps <= 0 || tiles <= 0) return;
-        const AsDeal d(steps, tiles, p.grid);
-        if (counted) {
-            if (p.T > 32) {
-                for (int t = lane; t < g.x; t += 32) { load(t); before += at.units(d); }
-            } else {
-                before = lane < g.x ? at.units(d) : 0;       // (in hand)
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-        }
-        const int R = nh / nkv, per_tile = AS_QTILE / R, i = tok - g.x, tile = i / per_tile;
-        const int n = as_tile_steps(as_pages(shared, window > 0 ? tok_pos[g.w] : 0, window, keep_first));
-        const int first = before + (kvh * as_tiles(g, nh, nkv) + tile) * d.units(n);
-        if (n == 0 || first < 0 || first > steps - 1) return;     // (nothing to join, or the kernel in front has given up)
-        const int2 c = d.ctas_of(first, n);
-        c0 = min(max(c.x, 0), p.grid);
-        c1 = min(c.y, p.grid);
-        row = as_block(0, g, nh, nkv, kvh, tile) + (size_t)((i - tile * per_tile) * R + head0);
-    }
-    // a warp for every row: the lanes take the CTAs in turn
-    __device__ __forceinline__ void weigh(const AdGroups& p, int j, int lane, float* weights, float* top_of, float* weight_of) const {
-        const float4* ends = p.scratch.ends + row + j;
-        const auto end_of = [&](int c) { return c < c1 ? ends[(size_t)c * AS_QTILE] : make_float4(-INFINITY, 0.f, -INFINITY, 0.f); };
-        const float4 mine = end_of(c0 + lane);
-        float top = fmaxf(mine.x, mine.z), sum = 0.f;
-        for (int c = c0 + 32 + lane; c < c1; c += 32) { const float4 e = end_of(c); top = fmaxf(top, fmaxf(e.x, e.z)); }
-        top = warp_max(top);
-        const auto weight = [&](float at) { return at == -INFINITY ? 0.f : ad_ex2(at - top); };
-        for (int c = c0 + lane; c < c1; c += 32) {
-            const float4 e = c == c0 + lane ? mine : end_of(c);
-            sum = fmaf(e.y, weight(e.x), fmaf(e.w, weight(e.z), sum));
-            weights[(c - c0) * 16 + j] = weight(fmaxf(e.x, e.z));
-        }
-        sum = warp_sum(sum);
-        if (lane == 0) { top_of[j] = top; weight_of[j] = sum; }
-    }
-    // The sums of the outputs `first`, `first` + `step`, .. (N of them, below `end`; output x is row x / cols, column col0 + x % cols), some CTAs' at a time: all their
-    // loads are asked for before the first is used
-    template <int N>
-    __device__ __forceinline__ void sums(const AdGroups& p, int first, int step, int end, int cols, int col0, const float* weights, float (&o)[N]) const {
-        constexpr int AT_ONCE = N >= 16 ? 1 : 16 / N;
-        size_t at[N];
-        int j[N];
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            const int x = first + k * step < end ? first + k * step : 0;
-            j[k] = x / cols;
-            at[k] = (row + j[k]) * AD_HD + col0 + x % cols;
-            o[k] = 0.f;
-        }
-        for (int c = c0; c < c1; c += AT_ONCE) {
-            float v[AT_ONCE][N];
-#pragma unroll
-            for (int e = 0; e < AT_ONCE; ++e)
-#pragma unroll
-                for (int k = 0; k < N; ++k) v[e][k] = c + e < c1 ? p.scratch.sums[at[k] + (size_t)(c + e) * (AS_QTILE * AD_HD)] : 0.f;
-#pragma unroll
-            for (int e = 0; e < AT_ONCE; ++e)
-#pragma unroll
-                for (int k = 0; k < N; ++k) {
-                    const float w = c + e < c1 ? weights[(c + e - c0) * 16 + j[k]] : 0.f;
-                    o[k] = w == 0.f ? o[k] : fmaf(v[e][k], w, o[k]);
-                }
-        }
-    }
-};
-#define AD_JOIN_BYTES ((AS_MAX_CTAS + 2) * 16 * 4)             // weights, maxima and weights of all
-
-// OWN: a token reads the positions behind those that it shares with its group (everything below counts from there), and joins the group's results.
-template <int AD_WARPS, bool OWN>
+template <int AD_WARPS>
 __global__ void __launch_bounds__(32 * (AD_WARPS + 1), AD_CTAS(AD_WARPS)) attention_decode_kernel(
     const bf16* q, int q_stride, const bf16* k_pool, const bf16* v_pool,
     const int* block_table, int table_stride, const int* tok_pos,
     const int* tok_row, int nh, int nkv, int window, float scale_log2e, int n_splits, int stages,
-    int* status, bf16* out, int keep_first, const float* slopes, const float* sinks, const AdGroups grouped) {
+    int* status, bf16* out, int keep_first, const float* slopes, const float* sinks) {
     constexpr int AD_GROUPS = AD_WARPS / 4, AD_THREADS = 32 * (AD_WARPS + 1);
     extern __shared__ __align__(128) unsigned char ad_smem[];   // result rows, then the ring (later: the warps' partial results)
     __shared__ __align__(8) unsigned long long bars[2 * AD_MAX_STAGES + 1];
@@ -343,19 +240,8 @@ __global__ void __launch_bounds__(32 * (AD_WARPS + 1), AD_CTAS(AD_WARPS)) attent
     const int G = nh / nkv, head_tiles = (G + 15) / 16;
     const int kvh = blockIdx.y / head_tiles, ht = blockIdx.y % head_tiles;
     // positions and page tables were uploaded before the step began: they may be read before the wait
-    int pos = tok_pos[tok];
+    const int pos = tok_pos[tok];
     const int* table = block_table + (size_t)tok_row[tok] * table_stride;
-    int4 group = make_int4(0, 0, 0, 0);
-    int shared = 0;
-    const int kept_keys = keep_first;
-    if constexpr (OWN) {
-        group = grouped.groups[tok];
-        shared = as_shared(group, tok, grouped.T, table_stride);
-        const int skip = min(shared, pos / PE_PAGE * PE_PAGE);
-        pos -= skip;
-        table += skip / PE_PAGE;
-        keep_first = max(keep_first - skip, 0);
-    }
     const int lo = (window > 0 && pos - window + 1 > 0) ? pos - window + 1 : 0;
     // The pages a token reads, in the order they are visited: those of the sequence's first keep_first keys where the window
     // has left them behind, then the window's.  Entry v of that list is page v (v < kept_pages) or first_page + v - kept_pages.
@@ -375,9 +261,7 @@ __global__ void __launch_bounds__(32 * (AD_WARPS + 1), AD_CTAS(AD_WARPS)) attent
     // columns.  gather[range][row][0..slice) holds that range's sums for this CTA's columns, [slice] the
     // row's max and [slice + 1] its sum; the other CTAs write theirs with st.async, which counts bytes on gbar.
     float* gather = reinterpret_cast<float*>(ad_smem);
-    unsigned char* ring = ad_smem + AD_RES_BYTES + (OWN ? AD_JOIN_BYTES : 0);
-    float* weights = reinterpret_cast<float*>(ad_smem + AD_RES_BYTES);       // of the group's results (OWN)
-    float *group_max = weights + AS_MAX_CTAS * 16, *group_sum = group_max + 16;
+    unsigned char* ring = ad_smem + AD_RES_BYTES;
     const unsigned ring0 = ad_smem_addr(ring), full0 = ad_smem_addr(bars), empty0 = full0 + 8u * AD_MAX_STAGES;
     const unsigned gather0 = ad_smem_addr(gather), gbar = empty0 + 8u * AD_MAX_STAGES;
     const int rows = min(16, G - ht * 16);
@@ -397,7 +281,6 @@ __global__ void __launch_bounds__(32 * (AD_WARPS + 1), AD_CTAS(AD_WARPS)) attent
     __syncthreads();
     if (n_splits > 1) ad_cluster_arrive();                   // waited for just before the first write to another CTA
 
-    __shared__ AdJoin join_s[1];
     float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
     float acc[AD_NCHUNK][4][4];
 #pragma unroll
@@ -438,17 +321,10 @@ __global__ void __launch_bounds__(32 * (AD_WARPS + 1), AD_CTAS(AD_WARPS)) attent
             }
             alive = __shfl_sync(0xffffffffu, alive, 0);
         }
-        if constexpr (OWN) {                                     // which of the group's results to join: found while the others compute
-            AdJoin join;
-            join.find(grouped, group, tok, shared, tok_pos, tok_row, table_stride, window, kept_keys, nh, nkv, kvh, ht * 16, lane);
-            if (lane == 0) join_s[0] = join;
-        }
     } else {
         // ---- the consumers
         const int last_phys = table[last_page];               // the page of the newest token
-        // OWN: the kernel in front lets this one begin when everything before it has ended: queries and the newest rows are there, its own results are not
-        if constexpr (!OWN) pdl_wait();
-        const auto fresh = [](const bf16* at) { return OWN ? ad_ld16_l2(at) : ad_ld16(at); };
+        pdl_wait();
         const int r_lo = ht * 16 + g, r_hi = r_lo + 8;        // this lane's two query heads within the group
         const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
         uint4 qf[AD_NCHUNK][2];
@@ -457,8 +333,8 @@ __global__ void __launch_bounds__(32 * (AD_WARPS + 1), AD_CTAS(AD_WARPS)) attent
             const int col = c * 32 + t * 8;
             const bool cin = col + 8 <= AD_HD;
             const bf16* qp = q + (size_t)tok * q_stride + col;
-            qf[c][0] = (cin && r_lo < G) ? fresh(qp + (size_t)(kvh * G + r_lo) * AD_HD) : zero;
-            qf[c][1] = (cin && r_hi < G) ? fresh(qp + (size_t)(kvh * G + r_hi) * AD_HD) : zero;
+            qf[c][0] = (cin && r_lo < G) ? ad_ld16(qp + (size_t)(kvh * G + r_lo) * AD_HD) : zero;
+            qf[c][1] = (cin && r_hi < G) ? ad_ld16(qp + (size_t)(kvh * G + r_hi) * AD_HD) : zero;
         }
         const int grp = warp >> 2, first_key = (warp & 3) * 16;
         const bool biased = slopes != nullptr;
@@ -485,7 +361,7 @@ __global__ void __launch_bounds__(32 * (AD_WARPS + 1), AD_CTAS(AD_WARPS)) attent
                     const size_t off = (((size_t)last_phys * nkv + kvh) * PE_PAGE + (pos % PE_PAGE)) * AD_HD;
                     const unsigned at = (unsigned)(((pos - key0) * AD_HD + lane * 8) * 2);
                     if (lane * 8 < AD_HD) {
-                        const uint4 kr = fresh(k_pool + off + lane * 8), vr = fresh(v_pool + off + lane * 8);
+                        const uint4 kr = ad_ld16(k_pool + off + lane * 8), vr = ad_ld16(v_pool + off + lane * 8);
                         asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(kt + at), "r"(kr.x), "r"(kr.y), "r"(kr.z), "r"(kr.w) : "memory");
                         asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(vt + at), "r"(vr.x), "r"(vr.y), "r"(vr.z), "r"(vr.w) : "memory");
                     }
@@ -514,11 +390,6 @@ __global__ void __launch_bounds__(32 * (AD_WARPS + 1), AD_CTAS(AD_WARPS)) attent
     // ---- merge the warps: the ring is free once every warp has left its loop.  Each warp scales its sums
     // to the CTA's max of the row first, so that merging is adding.
     __syncthreads();
-    if constexpr (OWN) {
-        pdl_wait();                                              // the kernel in front has left its results
-        const AdJoin join = join_s[0];
-        for (int row = warp; row < rows; row += AD_WARPS + 1) join.weigh(grouped, row, lane, weights, group_max, group_sum);
-    }
     float* part = reinterpret_cast<float*>(ring);           // [AD_WARPS][16][AD_ROW] sums, then per (warp, row): max, sum
     float* w_max = part + AD_WARPS * 16 * AD_ROW;
     float* w_sum = w_max + AD_WARPS * 16;
@@ -549,42 +420,6 @@ __global__ void __launch_bounds__(32 * (AD_WARPS + 1), AD_CTAS(AD_WARPS)) attent
     }
     __syncthreads();
     if (n_splits > 1) ad_cluster_wait();                     // every CTA of the cluster has set up its barrier
-    // the group's results of (row, col) joined to a row's maximum, weight and sum
-    const auto with_group = [&](int row, float sum, float& m, float& l, float& o) {
-        const float top = fmaxf(m, group_max[row]);
-        const float own = m == -INFINITY ? 0.f : ad_ex2(m - top), theirs = group_max[row] == -INFINITY ? 0.f : ad_ex2(group_max[row] - top);
-        l = fmaf(group_sum[row], theirs, l * own);
-        o = fmaf(sum, theirs, o * own);
-        m = top;
-    };
-    if constexpr (OWN) {
-        if (n_splits == 1) {
-            constexpr int N = (16 * AD_HD + AD_THREADS - 1) / AD_THREADS, HALF = (N + 1) / 2;      // in two turns: up to eight rows, and the others
-            const AdJoin join = join_s[0];
-#pragma unroll
-            for (int x0 = 0; x0 < 2; ++x0) {
-                const int at0 = threadIdx.x + x0 * HALF * AD_THREADS;
-                if (x0 * HALF * AD_THREADS >= rows * AD_HD) break;
-                float theirs[HALF];
-                join.sums(grouped, at0, AD_THREADS, rows * AD_HD, AD_HD, 0, weights, theirs);
-#pragma unroll
-                for (int k = 0; k < HALF; ++k) {
-                    const int x = at0 + k * AD_THREADS, row = x / AD_HD, col = x % AD_HD;
-                    if (x >= rows * AD_HD) break;
-                    float m = row_max[row], o = 0.f, l = 0.f;
-#pragma unroll
-                    for (int w = 0; w < AD_WARPS; ++w) {
-                        o += part[((size_t)w * 16 + row) * AD_ROW + col];
-                        l += w_sum[w * 16 + row];
-                    }
-                    with_group(row, theirs[k], m, l, o);
-                    if (sinks) l += exp2f(fmaf(sinks[kvh * G + ht * 16 + row], 1.4426950408889634f, -m));
-                    out[((size_t)tok * nh + kvh * G + ht * 16 + row) * AD_HD + col] = __float2bfloat16_rn(l > 0.f ? o / l : 0.f);
-                }
-            }
-            return;
-        }
-    }
     for (int idx = threadIdx.x; idx < rows * AD_HD; idx += AD_THREADS) {
         const int row = idx / AD_HD, col = idx % AD_HD;
         const float m = row_max[row];
@@ -624,14 +459,7 @@ __global__ void __launch_bounds__(32 * (AD_WARPS + 1), AD_CTAS(AD_WARPS)) attent
         if (threadIdx.x == 0) atomicExch(status, 4);
         return;
     }
-    constexpr int N_SLICE = OWN ? (16 * ((AD_HD + 1) / 2) + AD_THREADS - 1) / AD_THREADS : 1;
-    float theirs[N_SLICE];
-    if constexpr (OWN) {
-        const AdJoin join = join_s[0];
-        if (my_cols > 0) join.sums(grouped, threadIdx.x, AD_THREADS, rows * my_cols, my_cols, split * slice, weights, theirs);
-    }
-    int turn = 0;
-    for (int idx = threadIdx.x; idx < rows * my_cols; idx += AD_THREADS, ++turn) {
+    for (int idx = threadIdx.x; idx < rows * my_cols; idx += AD_THREADS) {
         const int row = idx / my_cols, j = idx - row * my_cols;
         float m = -INFINITY;
         for (int r = 0; r < n_splits; ++r) m = fmaxf(m, gather[(r * 16 + row) * grow + slice]);
@@ -642,7 +470,6 @@ __global__ void __launch_bounds__(32 * (AD_WARPS + 1), AD_CTAS(AD_WARPS)) attent
             o = fmaf(src[j], wgt, o);
             l = fmaf(src[slice + 1], wgt, l);
         }
-        if constexpr (OWN) with_group(row, theirs[turn], m, l, o);
         if (sinks) l += exp2f(fmaf(sinks[kvh * G + ht * 16 + row], 1.4426950408889634f, -m));
         out[((size_t)tok * nh + kvh * G + ht * 16 + row) * AD_HD + split * slice + j] = __float2bfloat16_rn(l > 0.f ? o / l : 0.f);
     }
@@ -655,14 +482,14 @@ extern "C" void pe_set_pdl(int on) { pe_pdl_enabled() = on ? 1 : 0; }
 // live in one process, and the function-local statics of a template with external linkage would be one
 // object for all of them (the dynamic linker makes such symbols unique across libraries).
 namespace {
-template <int WARPS, bool OWN = false>
+template <int WARPS>
 struct AdVariant {
     static constexpr int threads = 32 * (WARPS + 1), groups = WARPS / 4, ctas_per_sm = AD_CTAS(WARPS);
 
     static size_t smem_bytes(int stages) {
         size_t body = (size_t)stages * AD_STAGE_BYTES;
         if (body < (size_t)AD_SCRATCH_BYTES(WARPS)) body = AD_SCRATCH_BYTES(WARPS);
-        return AD_RES_BYTES + (OWN ? AD_JOIN_BYTES : 0) + body;
+        return AD_RES_BYTES + body;
     }
 
     static int allow_smem(size_t smem) {
@@ -670,16 +497,16 @@ struct AdVariant {
         static bool wide = false;
         if (!allowed) {
             cudaFuncAttributes own;
-            PE_TRY(cudaFuncGetAttributes(&own, attention_decode_kernel<WARPS, OWN>));
+            PE_TRY(cudaFuncGetAttributes(&own, attention_decode_kernel<WARPS>));
             allowed = 48 * 1024 - own.sharedSizeBytes;
         }
         if (!wide) {                                         // clusters of more than 8 CTAs are an opt-in; if it is refused,
-            cudaFuncSetAttribute(attention_decode_kernel<WARPS, OWN>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);   // the
+            cudaFuncSetAttribute(attention_decode_kernel<WARPS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);   // the
             cudaGetLastError();                              // occupancy query below answers 0 for them and fewer ranges are used
             wide = true;
         }
         if (smem > allowed) {
-            PE_TRY(cudaFuncSetAttribute(attention_decode_kernel<WARPS, OWN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+            PE_TRY(cudaFuncSetAttribute(attention_decode_kernel<WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
             allowed = smem;
         }
         return 0;
@@ -704,7 +531,7 @@ struct AdVariant {
             attr[0].val.clusterDim.x = splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
             cfg.attrs = attr;
             cfg.numAttrs = 1;
-            if (cudaOccupancyMaxActiveClusters(&n, attention_decode_kernel<WARPS, OWN>, &cfg) != cudaSuccess) { cudaGetLastError(); n = 0; }
+            if (cudaOccupancyMaxActiveClusters(&n, attention_decode_kernel<WARPS>, &cfg) != cudaSuccess) { cudaGetLastError(); n = 0; }
         }
         known[{splits, smem}] = n;
         return n;
@@ -714,7 +541,7 @@ struct AdVariant {
     // page ranges a sequence is cut into and how many pages a CTA keeps in flight.  As many ranges as fill the
     // GPU once, and no more than let all clusters be resident at the same time.
     static int shape(int ctas, int pages, int limit, int* stages_out) {
-        const int fit = (AD_SMEM_BUDGET(WARPS) - AD_RES_BYTES - (OWN ? AD_JOIN_BYTES : 0)) / AD_STAGE_BYTES;
+        const int fit = (AD_SMEM_BUDGET(WARPS) - AD_RES_BYTES) / AD_STAGE_BYTES;
         int splits = 148 * ctas_per_sm / ctas;
         if (splits > limit) splits = limit;
         if (splits > pages) splits = pages;
@@ -728,11 +555,6 @@ struct AdVariant {
             // A ring that is used more than once has a multiple of `groups` stages: a stage then always serves
             // the same warps, which therefore see every phase of its barriers (see the kernel).
             if (stages < most) stages -= stages % groups;
-            if (OWN) {                                       // (a row's own part may be longer than `pages`, which is a guess)
-                stages = fit < AD_MAX_STAGES ? fit : AD_MAX_STAGES;
-                if (stages > 2 * most + 2) stages = 2 * most + 2;
-                stages -= stages % groups;
-            }
             if (splits == 1 || stages < 1 || clusters_at_once(splits, smem_bytes(stages)) >= ctas) break;
         }
         *stages_out = stages;
@@ -742,7 +564,7 @@ struct AdVariant {
     static int launch(dim3 grid, int n_splits, int stages, cudaStream_t stream, const bf16* q, int q_stride, const bf16* k_pool,
                       const bf16* v_pool, const int* block_table, int table_stride, const int* tok_pos, const int* tok_row,
                       int nh, int nkv, int window, float scale_log2e, int* status, bf16* out, bool early, int keep_first,
-                      const float* slopes, const float* sinks, const AdGroups& grouped) {
+                      const float* slopes, const float* sinks) {
         const size_t smem = smem_bytes(stages);
         { const int e = allow_smem(smem); if (e) return e; }
         cudaLaunchConfig_t cfg = {};
@@ -764,8 +586,8 @@ struct AdVariant {
         }
         cfg.attrs = attr;
         cfg.numAttrs = n_attr;
-        PE_TRY(cudaLaunchKernelEx(&cfg, attention_decode_kernel<WARPS, OWN>, q, q_stride, k_pool, v_pool, block_table, table_stride,
-                                  tok_pos, tok_row, nh, nkv, window, scale_log2e, n_splits, stages, status, out, keep_first, slopes, sinks, grouped));
+        PE_TRY(cudaLaunchKernelEx(&cfg, attention_decode_kernel<WARPS>, q, q_stride, k_pool, v_pool, block_table, table_stride,
+                                  tok_pos, tok_row, nh, nkv, window, scale_log2e, n_splits, stages, status, out, keep_first, slopes, sinks));
         PE_LAUNCH_CHECK();
         return 0;
     }
@@ -791,23 +613,22 @@ extern "C" void pe_attention_decode_set_max_splits(int n) { ad_split_limit() = n
 //                  where all triples of short sequences then run in one turn instead of two (64 sequences of 500 tokens 15.4
 //                  against 12.3 us, 48 of 800 17.9 against 16.9, 40 of 500 12.0 against 11.6; 40 of 800 would take 15.2 against 16.4)
 struct AdShape { int warps, splits, stages; };
-template <bool OWN>
 static AdShape ad_choose(int T, int nh, int nkv, int max_context) {
     const int G = nh / nkv, ctas = T * nkv * ((G + 15) / 16), limit = ad_split_limit();
     const int pages = (max_context + PE_PAGE - 1) / PE_PAGE;
     const auto range = [&](int splits) { return (pages + splits - 1) / splits; };
     AdShape c = {8, 1, 1};
-    c.splits = AdVariant<8, OWN>::shape(ctas, pages, limit, &c.stages);
+    c.splits = AdVariant<8>::shape(ctas, pages, limit, &c.stages);
     if constexpr (AD_HD <= 64) {                             // larger heads need the registers
         if (ctas <= 32) {
             AdShape w = {16, 1, 1};
-            w.splits = AdVariant<16, OWN>::shape(ctas, pages, limit, &w.stages);
+            w.splits = AdVariant<16>::shape(ctas, pages, limit, &w.stages);
             if (range(w.splits) >= 8) return w;
         }
     }
     if constexpr (AD_HD <= 128) {                            // larger heads leave room for one page only
         AdShape n = {4, 1, 1};
-        n.splits = AdVariant<4, OWN>::shape(ctas, pages, limit, &n.stages);
+        n.splits = AdVariant<4>::shape(ctas, pages, limit, &n.stages);
         if (AD_HD <= 64 ? range(n.splits) == 1 ? n.splits != 2 || 2 * ctas > 222 : range(n.splits) == 2 && n.splits * ctas > (n.splits == 1 ? 2 : 1) * 148
                         : (c.splits == 1 && n.splits >= 3 && pages >= 16) || (ctas > 148 && ctas <= 2 * 148 && pages <= (ctas < 192 ? 8 : 12)))
             return n;
@@ -816,33 +637,10 @@ static AdShape ad_choose(int T, int nh, int nkv, int max_context) {
 }
 
 extern "C" int pe_attention_decode_splits(int T, int nh, int nkv, int max_context, int* stages_out) {
-    const AdShape c = ad_choose<false>(T, nh, nkv, max_context);
+    const AdShape c = ad_choose(T, nh, nkv, max_context);
     if (stages_out) *stages_out = c.stages;
     return c.splits;
 }
-
-namespace {
-constexpr int AD_OWN_PAGES = 8;
-template <bool OWN>
-int ad_run(const void* q, int q_stride, void* out, const void* k_pool, const void* v_pool, const int* block_table, int table_stride, const int* tok_pos,
-           const int* tok_row, int T, int nh, int nkv, int window, float scale, int max_context, int early_pages, int* status, void* stream, int keep_first,
-           const float* slopes, const float* sinks, const AdGroups& grouped) {
-    const int G = nh / nkv;
-    if ((long long)nkv * ((G + 15) / 16) > 65535) return PE_ERR_UNSUPPORTED;
-    const AdShape c = ad_choose<OWN>(T, nh, nkv, OWN && max_context > AD_OWN_PAGES * PE_PAGE ? AD_OWN_PAGES * PE_PAGE : max_context);
-    if (c.stages < 1) return PE_ERR_UNSUPPORTED;
-    const dim3 grid(c.splits, nkv * ((G + 15) / 16), T);
-    const float scale_log2e = scale * 1.4426950408889634f;
-    const auto go = [&](auto variant) {
-        return decltype(variant)::launch(grid, c.splits, c.stages, (cudaStream_t)stream, (const bf16*)q, q_stride, (const bf16*)k_pool,
-                                         (const bf16*)v_pool, block_table, table_stride, tok_pos, tok_row, nh, nkv, window, scale_log2e,
-                                         status, (bf16*)out, early_pages != 0, keep_first, slopes, sinks, grouped);
-    };
-    if constexpr (AD_HD <= 64) { if (c.warps == 16) return go(AdVariant<16, OWN>()); }
-    if constexpr (AD_HD <= 128) { if (c.warps == 4) return go(AdVariant<4, OWN>()); }
-    return go(AdVariant<8, OWN>());
-}
-}  // namespace
 
 extern "C" int pe_attention_decode(const void* q, int q_stride, void* out, const void* k_pool, const void* v_pool,
                                    const int* block_table, int table_stride, const int* tok_pos, const int* tok_row,
@@ -858,17 +656,18 @@ extern "C" int pe_attention_decode(const void* q, int q_stride, void* out, const
     if (hd != AD_HD || nkv <= 0 || nh % nkv || max_context <= 0 || q_stride % 8 || T > 65535 || !status) return PE_ERR_UNSUPPORTED;
     if (keep_first < 0 || (slopes && !(scale > 0.f))) return PE_ERR_UNSUPPORTED;
     if (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15) return PE_ERR_UNSUPPORTED;
-    return ad_run<false>(q, q_stride, out, k_pool, v_pool, block_table, table_stride, tok_pos, tok_row, T, nh, nkv, window, scale, max_context, early_pages,
-                         status, stream, keep_first, slopes, sinks, AdGroups{});
+    const int G = nh / nkv;
+    if ((long long)nkv * ((G + 15) / 16) > 65535) return PE_ERR_UNSUPPORTED;
+    const AdShape c = ad_choose(T, nh, nkv, max_context);
+    if (c.stages < 1) return PE_ERR_UNSUPPORTED;
+    const dim3 grid(c.splits, nkv * ((G + 15) / 16), T);
+    const float scale_log2e = scale * 1.4426950408889634f;
+    const auto go = [&](auto variant) {
+        return decltype(variant)::launch(grid, c.splits, c.stages, (cudaStream_t)stream, (const bf16*)q, q_stride, (const bf16*)k_pool,
+                                         (const bf16*)v_pool, block_table, table_stride, tok_pos, tok_row, nh, nkv, window, scale_log2e,
+                                         status, (bf16*)out, early_pages != 0, keep_first, slopes, sinks);
+    };
+    if constexpr (AD_HD <= 64) { if (c.warps == 16) return go(AdVariant<16>()); }
+    if constexpr (AD_HD <= 128) { if (c.warps == 4) return go(AdVariant<4>()); }
+    return go(AdVariant<8>());
 }
-
-#if AD_HD == 64 || AD_HD == 128
-// The rows' own positions, and the sum of both parts: attention_shared.cu calls it behind its own kernel.
-int pe_attention_decode_own(const void* q, int q_stride, void* out, const void* k_pool, const void* v_pool, const int* block_table, int table_stride,
-                            const int* tok_pos, const int* tok_row, int T, int nh, int nkv, int window, float scale, int max_context, int early_pages,
-                            int* status, void* stream, int keep_first, const float* slopes, const float* sinks, const void* groups, const AsScratch& scratch, int grid) {
-    if (max_context <= 0 || T > 65535) return PE_ERR_UNSUPPORTED;
-    return ad_run<true>(q, q_stride, out, k_pool, v_pool, block_table, table_stride, tok_pos, tok_row, T, nh, nkv, window, scale, max_context, early_pages,
-                        status, stream, keep_first, slopes, sinks, AdGroups{(const int4*)groups, scratch, T, grid});
-}
-#endif

@@ -107,6 +107,8 @@ SHARED = [  # nh, nkv, hd, [(shared positions, own tokens)]
     (128, 1, 64, [(128, [1, 66])]),                                             # one row a tile
     (5, 1, 128, [(20032, [9, 1, 1500])]),                                       # long
     (2, 2, 64, [(64 * (1 + i % 4), [1 + i % 3] * (1 + i % 5)) for i in range(70)]),      # many small groups
+    (2, 1, 128, [(64 * (i % 4), [1 + i % 70] * (2 + i % 5)) for i in range(110)]),       # more than 320 rows
+    (4, 4, 64, [(64, [3] * 300), (0, [40]), (192, [65] * 29)]),
 ]
 
 
