@@ -54,14 +54,14 @@ static_assert(AS_QAREA_BYTES % 1024 == 0 && 2 * AS_STAGES >= AS_WORKERS, "own pa
 #define AS_O_COL (AS_BUFFERS * AS_KTILE)
 #define AS_LAZY 8.0f
 #define AS_MIN_STEPS 2                             // steps of a chunk or run at least, where there are as many
+#define AS_MAX_TOKENS 1024                         // whose places in the two lines fit where results leave otherwise
 #define AS_MAX_CTAS 160
+static_assert(2 * AS_MAX_TOKENS * 4 <= AS_OUT_BYTES, "the tokens' places");
 #define AS_MOST_OWN 256                            // runs that a row's own part may lie with, and two more at its ends
-#define AS_COUNTED 320                             // up to so many tokens the join counts the steps itself while the first kernel runs; with more it takes them from there
 #define AS_JOIN_THREADS 256
 
 struct AsScratch {
-    int *shared_before, *own_before;                // T > AS_COUNTED: units in front of the group that starts with token t, of token t; [T] of the first: steps,
-                                                    //                 tiles, [T] of the second: pages of all
+    int4* plan;                                     // [T][own tiles of all key heads]: where the join finds a row's parts (AsPart)
     float* sums;                                    // [rows][head size]
     float4* ends;                                   // [rows]: reference point (a maximum, in powers of two) and weight of either warpgroup's steps; sums
                                                     //         are relative to the larger of the two
@@ -123,12 +123,15 @@ struct AsDeal {
     __device__ __forceinline__ int2 ctas_of(int before, int n) const { return chunk ? make_int2(before, before + units(n)) : make_int2(runs.cta_of(before), runs.cta_of(before + n - 1) + 1); }
 };
 
-// How many of the CTAs take shared steps: a step costs a CTA 1,650 cycles, an own page (its warps together) 600, with heads of 128 1,000.
-__device__ __forceinline__ int as_split(int steps, int pages, int grid) {
+// How many of the CTAs take shared steps.  Measured (cycles of a CTA, on top of what both kinds need): a step 1,490, an own page 440 (its warps together), and a
+// CTA of shared steps needs the time of three more; with heads of 128 1,930, 1,270 and five.  Both kinds end together where
+// step (steps / s + more) = page pages / (grid - s).
+__device__ __forceinline__ int as_split(int steps, int tiles, int pages, int grid) {
+    constexpr float step = AS_HD == 64 ? 1490.f : 1930.f, page = AS_HD == 64 ? 440.f : 1270.f, more = AS_HD == 64 ? 3.f : 5.f;
     if (steps == 0) return 0;
-    // (each operation rounds by itself: both kernels have to come to the same number)
-    const float shared = __fmul_rn(1650.f, (float)steps), all = __fadd_rn(shared, __fmul_rn(AS_HD == 64 ? 600.f : 1000.f, (float)pages));
-    return min(max(__float2int_rn(__fmul_rn((float)grid, __fdiv_rn(shared, all))), 1), grid - 1);
+    const float b = more * step * grid - step * steps - page * pages, a2 = 2.f * more * step;
+    const int s = __float2int_rn((b + sqrtf(b * b + 2.f * a2 * step * steps * grid)) / a2);
+    return min(max(min(s, steps / AS_MIN_STEPS + tiles), 1), grid - 1);
 }
 
 __device__ __forceinline__ int as_tiles(const int4& g, const AsArgs& p) { return (g.y + p.per_tile - 1) / p.per_tile; }
@@ -173,8 +176,8 @@ struct AsWalk {
         table = p.block_table + (size_t)now.row * p.table_stride;
         const int n = now.pages.steps(), units = d.units(n), tiles = as_tiles(now.g, p), o = x - now.before, seg = o / units, j = o - seg * units;
         kvh = seg / tiles; tile = seg - kvh * tiles;
-        first = d.chunk ? (int)((long long)n * j / units) : j;
-        count = d.chunk ? (int)((long long)n * (j + 1) / units) - first : min(n - first, end - x);
+        first = d.chunk ? (int)((unsigned)n * j / units) : j;        // (n: half a table row at most, units: the CTAs)
+        count = d.chunk ? (int)((unsigned)n * (j + 1) / units) - first : min(n - first, end - x);
     }
     __device__ __forceinline__ bool step(const AsArgs& p, const AsDeal& d) {
         x += d.chunk ? 1 : count;
@@ -260,6 +263,7 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
     AsWalk* walks = reinterpret_cast<AsWalk*>(refs + 2 * AS_QTILE);
     static_assert((AS_TILE_BYTES + 8 * AS_BARS + 2 * AS_QTILE * 4) % alignof(AsWalk) == 0 && sizeof(AsWalk) % alignof(AsOwnWalk) == 0, "the walks' places");
     AsOwnWalk* own_walk = reinterpret_cast<AsOwnWalk*>(walks + AS_WALKS);        // each worker's first own tile
+    int *shared_at = reinterpret_cast<int*>(as_mem), *own_at = shared_at + AS_MAX_TOKENS;       // of a CTA with own pages: units in front of a group, pages in front of a token
     int (*scan)[AS_THREADS / 32] = reinterpret_cast<int (*)[AS_THREADS / 32]>(own_walk + AS_WORKERS);
     if (q_s & 1023u) {                                              // every thread alike: nothing is allocated yet
         if (threadIdx.x == 0) atomicExch(status, 6);
@@ -313,7 +317,7 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
         if (w < warp) own.before += scan[2][w];
         total[0] += scan[0][w]; total[1] += scan[1][w]; total[2] += scan[2][w];
     }
-    const int cta = blockIdx.x, split = as_split(total[0], total[2], p.grid), own_cta = cta - split, own_ctas = p.grid - split;
+    const int cta = blockIdx.x, split = as_split(total[0], total[1], total[2], p.grid), own_cta = cta - split, own_ctas = p.grid - split;
     const AsDeal deal(total[0], total[1], split);
     const AsRuns own_runs(total[2], p.least_own, AS_WORKERS * own_ctas);
     int begin = cta, end = cta + 1, units = 0, own_units = 0;       // this CTA's units of the first line; all so far
@@ -338,7 +342,7 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
             }
         }
         const int t = base + (int)threadIdx.x;
-        if (p.T > AS_COUNTED && cta == 0 && t < p.T) { pdl_wait(); p.scratch.shared_before[t] = group.before; p.scratch.own_before[t] = own.before; }
+        if (own_cta >= 0 && t < p.T) { shared_at[t] = group.before; own_at[t] = own.before; }
         if (begin < end && begin >= group.before && begin < group.before + mine) {
             AsWalk& w = walks[0];
             w.now = group; w.x = begin; w.end = end;
@@ -359,7 +363,6 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
             z.step(p, deal);
         }
     }
-    if (p.T > AS_COUNTED && cta == 0 && threadIdx.x == 0) { p.scratch.shared_before[p.T] = total[0]; p.scratch.shared_before[p.T + 1] = total[1]; p.scratch.own_before[p.T] = total[2]; }
     const bool has_shared = begin < min(end, units), has_own = own_cta >= 0 && own_cta < own_runs.ctas;       // (the first worker's run comes first)
     if (!has_shared && !has_own) {                                  // (the whole block)
         pdl_wait();
@@ -398,7 +401,30 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
     AsOwnWalk& ow = *reinterpret_cast<AsOwnWalk*>(&w);
     static_assert(sizeof(AsOwnWalk) <= sizeof(AsWalk) && alignof(AsWalk) >= alignof(AsOwnWalk), "the own walk takes the other's place");
 
-    if (warp == 0) {                                                // ---------------- loader: one lane asks, the others wait for the walk
+    if (warp == 0 && has_own) {                                     // ---------------- the plan of the join, while the workers read
+        pdl_wait();                                                 // (scratch is written)
+        const int all = p.T * p.nkv * p.own_tiles, ctas = min(own_ctas, own_runs.ctas);
+        for (int e = own_cta * 32 + lane; e < all; e += ctas * 32) {
+            const int tok = e / (p.nkv * p.own_tiles), of = e - tok * (p.nkv * p.own_tiles), kvh = of / p.own_tiles, tile = of - kvh * p.own_tiles;
+            const int4 g = p.groups[tok];
+            AsOwn row;
+            row.set(p, tok, g);
+            const int first = own_at[tok] + of * row.pages.n, o0 = own_runs.cta_of(first);
+            const int on = min(own_runs.cta_of(first + row.pages.n - 1) + 1 - o0, AS_MOST_OWN + 2);       // (more only for positions behind max_context)
+            int c0 = 0, n = 0, at = 0;
+            const int shared = as_shared(g, tok, p.T, p.table_stride);
+            AsPages pages = {0, 0, 0};
+            if (shared > 0) pages.set(shared / PE_PAGE, p.window > 0 ? p.tok_pos[g.w] : 0, p.window, p.keep_first);
+            if (pages.n > 0) {
+                const int i = tok - g.x, group_tile = i / per_tile;
+                const int2 c = deal.ctas_of(shared_at[g.x] + (kvh * as_tiles(g, p) + group_tile) * deal.units(pages.steps()), pages.steps());
+                c0 = c.x;
+                n = c.y - c.x;
+                at = (int)as_block(c0, g, p, kvh, group_tile) + (i - group_tile * per_tile) * R + tile * AS_OTILE;
+            }
+            p.scratch.plan[e] = make_int4(n, on, at, (int)as_own_block(o0, tok, p, kvh, tile));
+        }
+    } else if (warp == 0) {                                                // ---------------- loader: one lane asks, the others wait for the walk
         bool ok = true;
         int it = 0, asked_k = 0, asked_v = 0, asked_q = 0;
                 // keys and values of two pages (rows y of the pools) into the stage of step `it`
@@ -825,94 +851,20 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
     }
 }
 
-// The join: a block a token and (16 heads of a) key head.  What it reads of the step's description may be older than the kernel in front, its results are not:
-// it counts the steps of up to AS_COUNTED tokens itself while that kernel runs.
+// The join: a block a token and (16 heads of a) key head.
 __global__ void __launch_bounds__(AS_JOIN_THREADS) attention_join_kernel(const __grid_constant__ AsArgs p, bf16* out, const float* sinks) {
     __shared__ float weights[AS_MAX_CTAS + AS_MOST_OWN + 2][AS_OTILE], weight_of[AS_OTILE];
-    __shared__ int counts[4][AS_JOIN_THREADS / 32];
     pdl_launch_dependents();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tok = blockIdx.y, tiles = p.own_tiles, R = p.R;
-    const int kvh = blockIdx.x / tiles, tile = blockIdx.x - kvh * tiles, head0 = tile * AS_OTILE, heads = min(AS_OTILE, R - head0);
-    if (!p.early) pdl_wait();
-    const bool counted = p.T <= AS_COUNTED;
-    const int4 g = p.groups[tok];
-    AsOwn own;
-    own.set(p, tok, g);
-    const int shared = as_shared(g, tok, p.T, p.table_stride), per_tile = p.per_tile, i = tok - g.x;
-    AsPages pages = {0, 0, 0};
-    if (shared > 0) pages.set(shared / PE_PAGE, p.window > 0 ? p.tok_pos[g.w] : 0, p.window, p.keep_first);
-    // all steps and tiles, the units in front of the group; the pages of all tokens and in front of this one
-    AsGroup at;
-    int sum[4] = {0, 0, 0, 0}, before = 0;
-    auto load = [&](int t) {
-        at.tiles = 0;
-        if (t >= p.T) return 0;
-        at.load(p, t);
-        AsOwn o;
-        o.set(p, t, at.g);
-        return o.steps;
-    };
-    auto add_up = [&](int& a, int& b, int& c, int& d) {             // over the block
-        int v[4] = {a, b, c, d};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
-        }
-        __syncthreads();
-        if (lane == 0) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) counts[k][warp] = v[k];
-        }
-        __syncthreads();
-        a = b = c = d = 0;
-#pragma unroll
-        for (int w = 0; w < AS_JOIN_THREADS / 32; ++w) { a += counts[0][w]; b += counts[1][w]; c += counts[2][w]; d += counts[3][w]; }
-    };
-    if (counted) {
-        for (int t = threadIdx.x; t < AS_COUNTED && t - (int)threadIdx.x < p.T; t += AS_JOIN_THREADS) {
-            const int pages_of = load(t);
-            sum[0] += at.steps(); sum[1] += at.tiles; sum[2] += pages_of; sum[3] += t < tok ? pages_of : 0;
-        }
-        add_up(sum[0], sum[1], sum[2], sum[3]);
-    } else {
-        pdl_wait();
-        sum[0] = p.scratch.shared_before[p.T]; sum[1] = p.scratch.shared_before[p.T + 1]; sum[2] = p.scratch.own_before[p.T]; sum[3] = p.scratch.own_before[tok];
-        before = shared > 0 ? p.scratch.shared_before[g.x] : 0;
-    }
-    const int split = as_split(sum[0], sum[2], p.grid);
-    const AsDeal deal(sum[0], sum[1], split);
-    if (counted) {
-        int none = 0, none2 = 0, none3 = 0;
-        for (int t = threadIdx.x; t < AS_COUNTED && t - (int)threadIdx.x < p.T; t += AS_JOIN_THREADS) {
-            if (p.T > AS_JOIN_THREADS) load(t);                     // (else it is in hand)
-            before += t < g.x ? at.units(deal) : 0;
-        }
-        add_up(before, none, none2, none3);
-    }
-    // the runs that had pages of this row: o0 .. o0 + on; the CTAs that had steps of it: c0 .. c0 + n
-    int c0 = 0, n = 0, o0 = 0, on = 0;
-    size_t block = 0;
-    {
-        const AsRuns runs(sum[2], p.least_own, AS_WORKERS * (p.grid - split));
-        const int first = sum[3] + (kvh * tiles + tile) * own.pages.n, last = first + own.pages.n - 1;
-        if (first >= 0 && last < sum[2]) {
-            o0 = runs.cta_of(first);
-            on = min(runs.cta_of(last) + 1 - o0, AS_MOST_OWN + 2);       // (more only for positions behind max_context)
-        }
-    }
-    if (pages.n > 0 && sum[0] > 0) {
-        const int of = i / per_tile, first = before + (kvh * as_tiles(g, p) + of) * deal.units(pages.steps());
-        const int2 c = deal.ctas_of(first, pages.steps());
-        if (first >= 0 && c.x >= 0 && c.y <= p.grid) { c0 = c.x; n = c.y - c.x; }       // (else the kernel in front has given up)
-        block = as_block(c0, g, p, kvh, of);
-    }
-    const int row = (i % per_tile) * R + head0;                     // of the shared tile
-    const size_t own_block = as_own_block(o0, tok, p, kvh, tile);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tok = blockIdx.y, R = p.R;
+    const int kvh = blockIdx.x / p.own_tiles, tile = blockIdx.x - kvh * p.own_tiles, head0 = tile * AS_OTILE, heads = min(AS_OTILE, R - head0);
+    pdl_wait();
+    const int4 plan = p.scratch.plan[tok * gridDim.x + blockIdx.x];
+    const int n = min(max(plan.x, 0), AS_MAX_CTAS), on = min(max(plan.y, 0), AS_MOST_OWN + 2);       // results of shared steps, and of own pages
+    const size_t row = plan.z, own_row = plan.w;
     // ---- sums: thread x has output x % AS_HD of head x / AS_HD.  The first AT_ONCE of them are asked for before the weights are known
     constexpr int N = (AS_OTILE * AS_HD / 2 + AS_JOIN_THREADS - 1) / AS_JOIN_THREADS, AT_ONCE = 32 / N;     // N: outputs of a thread, up to 8 heads; twice round with more
-    const float* from = p.scratch.sums + (block + row) * AS_HD;
-    const float* own_from = p.scratch.own_sums + own_block * AS_HD;
+    const float* from = p.scratch.sums + row * AS_HD;
+    const float* own_from = p.scratch.own_sums + own_row * AS_HD;
     float v[AT_ONCE][N];
     auto ask = [&](int x0, int e0) {
 #pragma unroll
@@ -923,13 +875,12 @@ __global__ void __launch_bounds__(AS_JOIN_THREADS) attention_join_kernel(const _
             for (int k = 0; k < N; ++k) v[e][k] = of < n + on && x0 + k * AS_JOIN_THREADS < heads * AS_HD ? at[x0 + k * AS_JOIN_THREADS] : 0.f;
         }
     };
-    pdl_wait();
     ask(threadIdx.x, 0);
     // ---- weights, a warp a head, a partial result a lane
     for (int h = warp; h < heads; h += AS_JOIN_THREADS / 32) {
         auto end_of = [&](int e) {                                  // reference points and weights; sums go by the larger one
-            if (e < n) return p.scratch.ends[block + row + h + (size_t)e * AS_QTILE];
-            const float2 o = p.scratch.own_ends[own_block + h + (size_t)(e - n) * AS_OTILE];
+            if (e < n) return p.scratch.ends[row + h + (size_t)e * AS_QTILE];
+            const float2 o = p.scratch.own_ends[own_row + h + (size_t)(e - n) * AS_OTILE];
             return make_float4(o.x, o.y, -INFINITY, 0.f);
         };
         float4 mine = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
@@ -994,15 +945,15 @@ int as_launch(int grid, cudaStream_t stream, const CUtensorMap& mq, const CUtens
     return 0;
 }
 
-long long as_before_bytes(int T) { return (2ll * (T + 2) * 4 + 255) / 256 * 256; }
+long long as_plan_bytes(int T, int nh, int nkv) { return ((long long)T * nkv * ((nh / nkv + AS_OTILE - 1) / AS_OTILE) * 16 + 255) / 256 * 256; }
 int as_grid() { return pe_sm_count() < AS_MAX_CTAS ? pe_sm_count() : AS_MAX_CTAS; }
 long long as_rows(int T, int nh) { return (long long)as_grid() * AS_QTILE + (long long)T * nh; }
 long long as_own_rows(int T, int nh) { return (long long)AS_WORKERS * as_grid() * AS_OTILE + (long long)T * nh; }
 
 }  // namespace
 
-extern "C" long long pe_attention_shared_scratch(int T, int nh) {
-    return as_before_bytes(T) + as_rows(T, nh) * (AS_HD * 4 + 16) + as_own_rows(T, nh) * (AS_HD * 4 + 8);
+extern "C" long long pe_attention_shared_scratch(int T, int nh, int nkv) {
+    return as_plan_bytes(T, nh, nkv) + as_rows(T, nh) * (AS_HD * 4 + 16) + as_own_rows(T, nh) * (AS_HD * 4 + 8);
 }
 
 extern "C" int pe_attention_shared(const void* q, int q_stride, void* out, const void* k_pool, const void* v_pool, long long pool_pages,
@@ -1014,7 +965,7 @@ extern "C" int pe_attention_shared(const void* q, int q_stride, void* out, const
     if (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)groups | (uintptr_t)scratch) & 15) return PE_ERR_UNSUPPORTED;
     if (pool_pages * nkv * PE_PAGE > 0x7fffff00ll) return PE_ERR_UNSUPPORTED;       // TMA coordinates are 32-bit
     const int R = nh / nkv;
-    if (T > 65535 || (long long)T * nkv * ((R + AS_OTILE - 1) / AS_OTILE) * (table_stride + 1ll) > 0x7fffffffll) return PE_ERR_UNSUPPORTED;      // steps are counted in 32 bits
+    if (T > AS_MAX_TOKENS || as_rows(T, nh) > 0x7fffffff || (long long)T * nkv * ((R + AS_OTILE - 1) / AS_OTILE) * (table_stride + 1ll) > 0x7fffffffll) return PE_ERR_UNSUPPORTED;      // steps are counted in 32 bits
     CUtensorMap mq, mk, mv;
     int rc = as_query_map(&mq, q, T, nh, q_stride, R, AS_QTILE / R);
     if (rc) return rc;
@@ -1031,8 +982,7 @@ extern "C" int pe_attention_shared(const void* q, int q_stride, void* out, const
     p.least_own = ((max_context + PE_PAGE - 1) / PE_PAGE + AS_MOST_OWN - 1) / AS_MOST_OWN;       // a row's own part lies with AS_MOST_OWN runs at most
     p.q = (const bf16*)q; p.q_stride = q_stride;
     char* at = (char*)scratch;
-    p.scratch.shared_before = (int*)at; p.scratch.own_before = (int*)at + T + 2;
-    at += as_before_bytes(T);
+    p.scratch.plan = (int4*)at; at += as_plan_bytes(T, nh, nkv);
     p.scratch.ends = (float4*)at; at += as_rows(T, nh) * 16;
     p.scratch.sums = (float*)at; at += as_rows(T, nh) * AS_HD * 4;
     p.scratch.own_sums = (float*)at; at += as_own_rows(T, nh) * AS_HD * 4;
@@ -1046,7 +996,7 @@ extern "C" int pe_attention_shared(const void* q, int q_stride, void* out, const
 
 #else   // other head sizes: the rows of a group are read one by one (attention_decode.cu)
 
-extern "C" long long pe_attention_shared_scratch(int, int) { return 0; }
+extern "C" long long pe_attention_shared_scratch(int, int, int) { return 0; }
 extern "C" int pe_attention_shared(const void*, int, void*, const void*, const void*, long long, const int*, int, const int*, const int*, const void*,
                                    int, int, int, int, int, int, float, int, const float*, const float*, int, void*, int*, void*) {
     return PE_ERR_UNSUPPORTED;

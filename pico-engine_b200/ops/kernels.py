@@ -1892,6 +1892,7 @@ def route_rows(h: torch.Tensor, router: torch.Tensor, n_outputs: int, n_experts:
 # ---------------------------------------------------------------------------- several answers to a prompt
 
 SHARED_HEAD_DIMS = (64, 128)
+SHARED_MAX_ROWS = 1024        # AS_MAX_TOKENS of csrc/attention_shared.cu
 
 
 def _need_here(t: torch.Tensor, name: str) -> None:
@@ -1900,8 +1901,9 @@ def _need_here(t: torch.Tensor, name: str) -> None:
         raise KernelError(f"{name} lives on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
 
 
-def attention_shared_takes(dtype: torch.dtype, n_heads: int, n_kv_heads: int, head_dim: int, scale: float) -> bool:
-    return dtype == torch.bfloat16 and head_dim in SHARED_HEAD_DIMS and scale > 0 and n_heads // n_kv_heads <= 128
+def attention_shared_takes(dtype: torch.dtype, rows: int, n_heads: int, n_kv_heads: int, head_dim: int, scale: float) -> bool:
+    return (dtype == torch.bfloat16 and rows <= SHARED_MAX_ROWS and head_dim in SHARED_HEAD_DIMS and scale > 0 and n_heads % n_kv_heads == 0
+            and n_heads // n_kv_heads <= 128)
 
 
 def shared_group_rows(members):
@@ -1933,9 +1935,9 @@ def attention_shared(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: i
     from .library import for_head_dim
     T = tok_pos.shape[0]
     _need(q, "q", torch.bfloat16); _need(k_pool, "k_pool", torch.bfloat16); _need(v_pool, "v_pool", torch.bfloat16, k_pool.shape)
-    if not attention_shared_takes(q.dtype, n_heads, n_kv_heads, head_dim, scale) or n_heads % n_kv_heads:
-        raise KernelError(f"attention_shared takes head sizes {SHARED_HEAD_DIMS}, a positive scale and at most 128 query heads a key head, not "
-                          f"{n_heads} / {n_kv_heads} heads of {head_dim}, scale {scale}")
+    if not attention_shared_takes(q.dtype, T, n_heads, n_kv_heads, head_dim, scale):
+        raise KernelError(f"attention_shared takes at most {SHARED_MAX_ROWS} rows, head sizes {SHARED_HEAD_DIMS}, a positive scale and at most 128 query heads a key "
+                          f"head, not {T} rows, {n_heads} / {n_kv_heads} heads of {head_dim}, scale {scale}")
     if k_pool.dim() != 4 or tuple(k_pool.shape[1:]) != (n_kv_heads, PAGE, head_dim):
         raise KernelError(f"cache pool must be [pages, {n_kv_heads}, {PAGE}, {head_dim}], not {tuple(k_pool.shape)}")
     _need(block_table, "block_table", torch.int32)
@@ -1955,7 +1957,7 @@ def attention_shared(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: i
     if T == 0:
         return out
     lib = for_head_dim(head_dim)
-    scratch = torch.empty(lib.pe_attention_shared_scratch(T, n_heads), dtype=torch.uint8, device=q.device)      # (of the call: graphs and streams share none)
+    scratch = torch.empty(lib.pe_attention_shared_scratch(T, n_heads, n_kv_heads), dtype=torch.uint8, device=q.device)      # (of the call: graphs and streams share none)
     check(lib.pe_attention_shared(q.data_ptr(), q_stride, out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_pool.shape[0], block_table.data_ptr(),
                                   table_stride, tok_pos.data_ptr(), tok_row.data_ptr(), groups.data_ptr(), T, n_heads, n_kv_heads, head_dim, window or 0,
                                   keep_first if window else 0, scale, max_context, _ptr(slopes), _ptr(sinks), 1 if early_pages else 0, scratch.data_ptr(),

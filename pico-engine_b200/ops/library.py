@@ -312,7 +312,7 @@ def for_head_dim(head_dim: int) -> ctypes.CDLL:
     if lib is None:
         lib = build.load(f"attention_hd{head_dim}", HEAD_DIM_SOURCES, {"PE_HEAD_DIM": str(head_dim)})
         declare(lib, _HEAD_DIM_SIGNATURES)
-        lib.pe_attention_shared_scratch.argtypes = [I, I]
+        lib.pe_attention_shared_scratch.argtypes = [I, I, I]
         lib.pe_attention_shared_scratch.restype = c_longlong
         lib.pe_set_pdl(0 if os.environ.get("PICO_ENGINE_PDL", "1") == "0" else 1)
         _by_head_dim[head_dim] = lib
