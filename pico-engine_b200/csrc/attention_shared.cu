@@ -58,7 +58,7 @@ static_assert(AS_QAREA_BYTES % 1024 == 0 && 2 * AS_STAGES >= AS_WORKERS, "own pa
 #define AS_MAX_CTAS 160
 static_assert(2 * AS_MAX_TOKENS * 4 <= AS_OUT_BYTES, "the tokens' places");
 #define AS_MOST_OWN 256                            // runs that a row's own part may lie with, and two more at its ends
-#define AS_JOIN_THREADS 256
+#define AS_JOIN_THREADS 512
 
 struct AsScratch {
     int4* plan;                                     // [T][own tiles of all key heads]: where the join finds a row's parts (AsPart)
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
     load(threadIdx.x);
     if (threadIdx.x == 32) {
         auto init = [](unsigned long long* bar, unsigned count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(at_smem(bar)), "r"(count) : "memory"); };
-        init(q_full, 1); init(q_empty, 8); init(o_empty, 8);         // q_empty: the eight warps that write the tile's results through the queries' place
+        init(q_full, 1); init(q_empty, 8); init(o_empty, 8);         // q_empty: the eight warps that write the tile's results
         for (int s = 0; s < AS_STAGES; ++s) { init(&k_full[s], 1); init(&v_full[s], 1); init(&k_empty[s], 1); init(&v_empty[s], 1); }
         for (int b = 0; b < AS_BUFFERS; ++b) { init(&s_full[b], 1); init(&p_full[b], 4); init(&pv_done[b], 1); }
         for (int w = 0; w < 8; ++w) init(&told[w], 1);
@@ -652,9 +652,9 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const size_t block = as_block(cta, w.now.g, p, w.kvh, w.tile);
             if (live) reinterpret_cast<float2*>(p.scratch.ends + block + r)[g] = make_float2(m_mine, l_mine);
-            // through the start of the queries' place (the last S has read them), eight columns of the warp's 32 rows at a time, 16-byte pieces exchanged by the
-            // row inside a run of eight: a lane storing its own row would touch 32 lines an instruction
-            const unsigned stage = q_s + (warp - 2) * 1024;
+            // through the stages (the tile's products have read them, the next tile's come when this is done), 32 columns of the warp's 32 rows at a time, 16-byte
+            // pieces exchanged by the row inside a run of eight: a lane storing its own row would touch 32 lines an instruction
+            const unsigned stage = kv_s + (warp - 2) * 4096;
             float* to = p.scratch.sums + block * AS_HD + g * (AS_HD / 2);
 #pragma unroll
             for (int c = 0; c < AS_HD / 2; c += 32) {
@@ -665,24 +665,20 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
                     __syncwarp();
                     if (lane == 0) at_arrive(at_smem(o_empty));
                 }
+                __syncwarp();
 #pragma unroll
-                for (int part = 0; part < 4; ++part) {
-                    __syncwarp();
+                for (int k = 0; k < 8; ++k)
+                    asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(stage + lane * 128 + ((k ^ (lane & 7)) << 4)), "f"(o[4 * k]), "f"(o[4 * k + 1]), "f"(o[4 * k + 2]), "f"(o[4 * k + 3]) : "memory");
+                __syncwarp();
 #pragma unroll
-                    for (int k = 0; k < 2; ++k)
-                        asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(stage + lane * 32 + ((k ^ ((lane >> 2) & 1)) << 4)), "f"(o[8 * part + 4 * k]), "f"(o[8 * part + 4 * k + 1]),
-                                     "f"(o[8 * part + 4 * k + 2]), "f"(o[8 * part + 4 * k + 3]) : "memory");
-                    __syncwarp();
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {                   // sixteen rows an instruction
-                        const int x = 16 * k + (lane >> 1), row = quarter * 32 + x;
-                        float4 v;
-                        asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(stage + x * 32 + (((lane & 1) ^ ((x >> 2) & 1)) << 4)) : "memory");
-                        if (row < rows) *reinterpret_cast<float4*>(to + (size_t)row * AS_HD + c + 8 * part + 4 * (lane & 1)) = v;
-                    }
+                for (int k = 0; k < 8; ++k) {                       // four rows an instruction
+                    const int x = 4 * k + (lane >> 3), row = quarter * 32 + x;
+                    float4 v;
+                    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(stage + x * 128 + (((lane & 7) ^ (x & 7)) << 4)) : "memory");
+                    if (row < rows) *reinterpret_cast<float4*>(to + (size_t)row * AS_HD + c + 4 * (lane & 7)) = v;
                 }
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // (the next tile's queries come by another proxy)
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // (what comes next there comes by another proxy)
             __syncwarp();
             if (lane == 0) at_arrive(at_smem(q_empty));
         }
@@ -740,14 +736,16 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
 #pragma unroll
                 for (int x = 0; x < 8; ++x) sc[x][0] = sc[x][1] = sc[x][2] = sc[x][3] = 0.f;
 #pragma unroll
-                for (int c = 0; c < AS_HD / 16; ++c)
+                for (int c = 0; c < AS_HD / 16; ++c) {              // four fetches in front of the products that wait for them
+                    unsigned kf[4][4];                              // keys 0-7 and 8-15 of 16, columns 0-7 and 8-15
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) as_matrices(kf[x], as_at(keys, x * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * c + ((lane >> 3) & 1)));
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                        unsigned kf[4];                             // keys 0-7 and 8-15 of 16, columns 0-7 and 8-15
-                        as_matrices(kf, as_at(keys, x * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * c + ((lane >> 3) & 1)));
-                        as_mma(sc[2 * x], qf[c], kf[0], kf[1]);
-                        as_mma(sc[2 * x + 1], qf[c], kf[2], kf[3]);
+                        as_mma(sc[2 * x], qf[c], kf[x][0], kf[x][1]);
+                        as_mma(sc[2 * x + 1], qf[c], kf[x][2], kf[x][3]);
                     }
+                }
                 __syncwarp();
                 if (y_next >= 0) y_next = rows_of(entry, kvh_next);
                 if (lane == 0 && y_next >= 0) {                     // the keys have been read: the next ones, and behind the tile's last page the next tile's queries
@@ -806,14 +804,16 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
                     __syncwarp();
                 }
 #pragma unroll
-                for (int x = 0; x < 4; ++x)
+                for (int c = 0; c < AS_HD / 8; c += 2) {            // sixteen columns of four times 16 keys
+                    unsigned vf[4][4];
 #pragma unroll
-                    for (int c = 0; c < AS_HD / 8; c += 2) {        // 16 keys of sixteen columns
-                        unsigned vf[4];
-                        as_matrices_turned(vf, as_at(values, x * 16 + (lane & 15), c + (lane >> 4)));
-                        as_mma(acc[c], pf[x], vf[0], vf[1]);
-                        as_mma(acc[c + 1], pf[x], vf[2], vf[3]);
+                    for (int x = 0; x < 4; ++x) as_matrices_turned(vf[x], as_at(values, x * 16 + (lane & 15), c + (lane >> 4)));
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        as_mma(acc[c], pf[x], vf[x][0], vf[x][1]);
+                        as_mma(acc[c + 1], pf[x], vf[x][2], vf[x][3]);
                     }
+                }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0 && y_next >= 0) { own_page(&map_v, k, 1, y_next, &own_v[k]); ++asked_v; }
@@ -861,21 +861,18 @@ __global__ void __launch_bounds__(AS_JOIN_THREADS) attention_join_kernel(const _
     const int4 plan = p.scratch.plan[tok * gridDim.x + blockIdx.x];
     const int n = min(max(plan.x, 0), AS_MAX_CTAS), on = min(max(plan.y, 0), AS_MOST_OWN + 2);       // results of shared steps, and of own pages
     const size_t row = plan.z, own_row = plan.w;
-    // ---- sums: thread x has output x % AS_HD of head x / AS_HD.  The first AT_ONCE of them are asked for before the weights are known
-    constexpr int N = (AS_OTILE * AS_HD / 2 + AS_JOIN_THREADS - 1) / AS_JOIN_THREADS, AT_ONCE = 32 / N;     // N: outputs of a thread, up to 8 heads; twice round with more
-    const float* from = p.scratch.sums + row * AS_HD;
-    const float* own_from = p.scratch.own_sums + own_row * AS_HD;
-    float v[AT_ONCE][N];
-    auto ask = [&](int x0, int e0) {
+    // thread x has output x % AS_HD of head x / AS_HD.  The first results of either kind are asked for at once, beside what the weights are made of: a fetch of what
+    // another SM has just written takes 1,200 cycles or more, and rows seldom have more results than these
+    constexpr int FIRST = 16, FIRST_OWN = 2;
+    const float *from = p.scratch.sums + row * AS_HD, *own_from = p.scratch.own_sums + own_row * AS_HD;
+    float v[FIRST], u[FIRST_OWN];
+    auto ask = [&](int x) {
 #pragma unroll
-        for (int e = 0; e < AT_ONCE; ++e) {
-            const int of = e0 + e;
-            const float* at = of < n ? from + (size_t)of * (AS_QTILE * AS_HD) : own_from + (size_t)(of - n) * (AS_OTILE * AS_HD);
+        for (int e = 0; e < FIRST; ++e) v[e] = e < n && x < heads * AS_HD ? from[x + e * (AS_QTILE * AS_HD)] : 0.f;
 #pragma unroll
-            for (int k = 0; k < N; ++k) v[e][k] = of < n + on && x0 + k * AS_JOIN_THREADS < heads * AS_HD ? at[x0 + k * AS_JOIN_THREADS] : 0.f;
-        }
+        for (int e = 0; e < FIRST_OWN; ++e) u[e] = e < on && x < heads * AS_HD ? own_from[x + e * (AS_OTILE * AS_HD)] : 0.f;
     };
-    ask(threadIdx.x, 0);
+    ask(threadIdx.x);
     // ---- weights, a warp a head, a partial result a lane
     for (int h = warp; h < heads; h += AS_JOIN_THREADS / 32) {
         auto end_of = [&](int e) {                                  // reference points and weights; sums go by the larger one
@@ -886,9 +883,11 @@ __global__ void __launch_bounds__(AS_JOIN_THREADS) attention_join_kernel(const _
         float4 mine = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
         if (lane < n + on) mine = end_of(lane);
         float top = fmaxf(mine.x, mine.z), sum = 0.f;
+#pragma unroll 1
         for (int e = lane + 32; e < n + on; e += 32) { const float4 at = end_of(e); top = fmaxf(top, fmaxf(at.x, at.z)); }
         top = warp_max(top);
         const auto weight = [&](float at) { return at == -INFINITY ? 0.f : at_exp2(at - top); };
+#pragma unroll 1
         for (int e = lane; e < n + on; e += 32) {
             const float4 at = e == lane ? mine : end_of(e);
             sum = fmaf(at.y, weight(at.x), fmaf(at.w, weight(at.z), sum));
@@ -899,23 +898,22 @@ __global__ void __launch_bounds__(AS_JOIN_THREADS) attention_join_kernel(const _
         if (lane == 0) weight_of[h] = sum > 0.f ? 1.f / sum : 0.f;
     }
     __syncthreads();
-    for (int x0 = threadIdx.x; x0 < heads * AS_HD; x0 += N * AS_JOIN_THREADS) {
-        float o[N];
+    // ---- sums
+#pragma unroll 1
+    for (int x = threadIdx.x; x < heads * AS_HD; x += AS_JOIN_THREADS) {
+        const int h = x / AS_HD;
+        if (x >= AS_JOIN_THREADS) ask(x);
+        float o = 0.f;
+        auto add = [&](float value, int e) { const float at = weights[e][h]; o = at == 0.f ? o : fmaf(value, at, o); };
 #pragma unroll
-        for (int k = 0; k < N; ++k) o[k] = 0.f;
-        for (int e0 = 0; e0 < n + on; e0 += AT_ONCE) {
-            if (e0 > 0 || x0 >= N * AS_JOIN_THREADS) ask(x0, e0);
+        for (int e = 0; e < FIRST; ++e) if (e < n) add(v[e], e);
+#pragma unroll 4
+        for (int e = FIRST; e < n; ++e) add(from[x + (size_t)e * (AS_QTILE * AS_HD)], e);
 #pragma unroll
-            for (int e = 0; e < AT_ONCE; ++e) {
-                if (e0 + e >= n + on) break;
-#pragma unroll
-                for (int k = 0; k < N; ++k) { const float at = weights[e0 + e][min((x0 + k * AS_JOIN_THREADS) / AS_HD, AS_OTILE - 1)]; o[k] = at == 0.f ? o[k] : fmaf(v[e][k], at, o[k]); }
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (x0 + k * AS_JOIN_THREADS < heads * AS_HD)
-                out[((size_t)tok * p.nh + kvh * R + head0) * AS_HD + x0 + k * AS_JOIN_THREADS] = __float2bfloat16_rn(o[k] * weight_of[(x0 + k * AS_JOIN_THREADS) / AS_HD]);
+        for (int e = 0; e < FIRST_OWN; ++e) if (e < on) add(u[e], n + e);
+#pragma unroll 4
+        for (int e = FIRST_OWN; e < on; ++e) add(own_from[x + e * (AS_OTILE * AS_HD)], n + e);
+        out[((size_t)tok * p.nh + kvh * R + head0) * AS_HD + x] = __float2bfloat16_rn(o * weight_of[h]);
     }
 }
 
