@@ -5,12 +5,20 @@
 //     z = logits[b][v]
 //     h != 0:   z = z > 0 ? z / repetition : z * repetition
 //     count c:  z -= presence + c * frequency                     (c > 0)
-//     z += the row's biases of v (a list of ids and values; an id that stands there twice counts twice, in the list's order)
+//     z += the row's biases of v (a list of ids and values; those of an id that stands there twice are added up first, in the list's order)
 //     v is not in the row's mask: z = -inf                        (whatever z was)
+//
+// What bounds it: bytes.  A block takes some thousand tokens of a row, eight a thread, all of a thread's loads under way at once; what the result does not
+// hang on is not read: where the mask leaves nothing of a warp's 128 tokens, neither logits nor history (run by run, those of 2 in 100 tokens
+// spread at random came to so many single sectors that all of them are read faster), and where the row is changed in place, logits of tokens that have not
+// been seen, which are not written either.  Biases are few and lie anywhere: a second kernel adds them to the result, an entry a thread
+// (picked out of the list and added up in shared memory by every block of the first one they cost as much as all the rest: 64 rows of 151,936 under
+// all rules 33 us, 24.6 this way; penalties alone 19.2 us, 5.1 TB/s, a mask alone 13.4).
 #include "common.cuh"
 
 #define LR_THREADS 256
-#define LR_CHUNK 2048
+#define LR_CHUNK (LR_THREADS * 8)                   // tokens of a block: eight a thread (with sixteen, and so fewer blocks an SM, 64 rows with penalties took 23 us instead of 19)
+#define LR_LIST 512                                 // entries of a list of biases that a block looks at in one turn
 
 struct LrArgs {
     const float* logits; float* out; int rows, vocab;
@@ -20,31 +28,141 @@ struct LrArgs {
     const unsigned* masks; int n_masks, mask_words; const int* mask_rows;
 };
 
-__global__ void __launch_bounds__(LR_THREADS) adjust_logits_kernel(const LrArgs p) {
+// Four tokens at a time: those that lie on 16 bytes of the row (a vocabulary need not be a multiple of four), and what is left at the row's ends one by one.
+// ALIGNED: logits and out start on 16 bytes; else every load and store takes one number.
+template <bool ALIGNED, bool IN_PLACE>
+__global__ void __launch_bounds__(LR_THREADS, 8) adjust_logits_kernel(const LrArgs p) {
+    constexpr int TURNS = LR_CHUNK / 4 / LR_THREADS;                // runs of a thread
     pdl_launch_dependents();
     pdl_wait();
-    const int b = blockIdx.y, begin = blockIdx.x * LR_CHUNK, end = min(p.vocab, begin + LR_CHUNK);
-    const float* row = p.logits + (size_t)b * p.vocab;
-    float* out = p.out + (size_t)b * p.vocab;
-    const int slot = p.history ? p.slots[b] : -1;
-    const short* seen = p.history && slot >= 0 && slot < p.n_slots ? p.history + (size_t)slot * p.vocab : nullptr;
-    const float repetition = seen ? p.penalties[3 * b] : 1.f, presence = seen ? p.penalties[3 * b + 1] : 0.f, frequency = seen ? p.penalties[3 * b + 2] : 0.f;
-    const int2 list = p.bias_ids ? p.bias_range[b] : make_int2(0, 0);
-    const int m = p.masks ? p.mask_rows[b] : -1;
-    const unsigned* mask = p.masks && m >= 0 && m < p.n_masks ? p.masks + (size_t)m * p.mask_words : nullptr;
-    for (int v = begin + threadIdx.x; v < end; v += LR_THREADS) {
-        float z = row[v];
-        if (seen) {
-            const int h = seen[v], count = h & 0x7fff;
-            if (h != 0) z = z > 0.f ? z / repetition : z * repetition;
-            if (count > 0) z -= fmaf((float)count, frequency, presence);
+    const int b = blockIdx.y, V = p.vocab;
+    const size_t at0 = (size_t)b * V;
+    const float* row = p.logits + at0;
+    float* out = p.out + at0;
+    const int slot = p.history ? p.slots[b] : -1, m = p.masks ? p.mask_rows[b] : -1;
+    const bool known = slot >= 0 && slot < p.n_slots;
+    const short* seen = p.history + (known ? (size_t)slot * V : 0);
+    const unsigned* mask = m >= 0 && m < p.n_masks ? p.masks + (size_t)m * p.mask_words : nullptr;
+    float repetition = 1.f, inverse = 1.f, presence = 0.f, frequency = 0.f;
+    if (known) { repetition = p.penalties[3 * b]; presence = p.penalties[3 * b + 1]; frequency = p.penalties[3 * b + 2]; inverse = 1.f / repetition; }      // (its rounding joins the product's: a step of float32 where a quotient has half of one)
+    // the chunk's tokens begin .. end - 1: runs of four from `base` on, before and behind them (first and last chunk) a few single ones
+    const int head = min((int)(-at0 & 3), V), base = head + blockIdx.x * LR_CHUNK, stop = min(base + LR_CHUNK, V), runs = (stop - base) >> 2;
+    if (blockIdx.x > 0 && base >= V) return;                        // (the single tokens at the row's start have moved the chunks)
+    const bool eight = ((size_t)(known ? seen - p.history : 0) + base) % 4 == 0 && !((uintptr_t)p.history & 7);      // the history's runs lie on 8 bytes
+    auto bits_of = [&](int v) {                                     // which of the tokens v .. v + 3 are allowed
+        if (!mask) return 15u;
+        const int word = v >> 5;
+        const unsigned lo = mask[word];
+        return ((v & 31) > 28 ? __funnelshift_r(lo, word + 1 < p.mask_words ? mask[word + 1] : 0u, v & 31) : lo >> (v & 31)) & 15u;
+    };
+    unsigned allowed[TURNS];
+    short4 h[TURNS];
+    float4 z[TURNS];
+#pragma unroll
+    for (int k = 0; k < TURNS; ++k) {
+        const int r = k * LR_THREADS + threadIdx.x;
+        allowed[k] = r < runs ? bits_of(base + 4 * r) : 0u;
+    }
+#pragma unroll
+    for (int k = 0; k < TURNS; ++k) {
+        const int v = base + 4 * (k * LR_THREADS + (int)threadIdx.x);
+        h[k] = make_short4(0, 0, 0, 0);
+        const bool some = __any_sync(0xffffffffu, allowed[k] != 0u) && k * LR_THREADS + (int)threadIdx.x < runs;
+        if (known && some) h[k] = eight ? *reinterpret_cast<const short4*>(seen + v) : make_short4(seen[v], seen[v + 1], seen[v + 2], seen[v + 3]);
+        if (!IN_PLACE && some) z[k] = ALIGNED ? *reinterpret_cast<const float4*>(row + v) : make_float4(row[v], row[v + 1], row[v + 2], row[v + 3]);
+    }
+    auto rule = [&](float x, short h_v) {
+        const int count = h_v & 0x7fff;
+        if (h_v != 0) x *= x > 0.f ? inverse : repetition;
+        return count > 0 ? x - fmaf((float)count, frequency, presence) : x;
+    };
+    // one token by itself
+    auto single = [&](int v, bool is_allowed, short h_v) {
+        if (!is_allowed) out[v] = -INFINITY;
+        else if (!IN_PLACE || h_v != 0) out[v] = rule(row[v], h_v);
+    };
+#pragma unroll
+    for (int k = 0; k < TURNS; ++k) {
+        const int r = k * LR_THREADS + (int)threadIdx.x, v = base + 4 * r;
+        if (r >= runs) continue;
+        const short4 t = h[k];
+        if constexpr (IN_PLACE) {                                   // only runs in which something changes are read and written
+            if (allowed[k] == 15u && t.x == 0 && t.y == 0 && t.z == 0 && t.w == 0) continue;
+            if (allowed[k]) z[k] = ALIGNED ? *reinterpret_cast<const float4*>(row + v) : make_float4(row[v], row[v + 1], row[v + 2], row[v + 3]);
         }
-        float bias = 0.f;
-        for (int e = max(list.x, 0); e < min(list.y, p.n_bias); ++e)
-            if (p.bias_ids[e] == v) bias += p.bias_values[e];
-        z += bias;
-        if (mask && !((mask[v >> 5] >> (v & 31)) & 1u)) z = -INFINITY;
-        out[v] = z;
+        float4 x = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (allowed[k] & 1u) x.x = rule(z[k].x, t.x);
+        if (allowed[k] & 2u) x.y = rule(z[k].y, t.y);
+        if (allowed[k] & 4u) x.z = rule(z[k].z, t.z);
+        if (allowed[k] & 8u) x.w = rule(z[k].w, t.w);
+        if constexpr (ALIGNED) *reinterpret_cast<float4*>(out + v) = x;
+        else { out[v] = x.x; out[v + 1] = x.y; out[v + 2] = x.z; out[v + 3] = x.w; }
+    }
+    // what is left: up to three tokens in front of the first run and behind the last
+    const int before = blockIdx.x == 0 ? head : 0, left = before + (stop - base - 4 * runs);
+    if ((int)threadIdx.x < left) {
+        const int v = (int)threadIdx.x < before ? (int)threadIdx.x : base + 4 * runs + (int)threadIdx.x - before;
+        single(v, bits_of(v) & 1u, known ? seen[v] : (short)0);
+    }
+}
+
+// out += the row's biases, where the mask allows the token: a block a row, LR_LIST entries of its list a turn.  The first entry of a token adds all of the turn's, in
+// the list's order, so that no sum depends on which thread comes first.  A table in shared memory tells which entry is a token's first and whether
+// there are others; only then is the turn's list read through (by every entry it took 11 us for 64 lists of 300).
+__global__ void __launch_bounds__(LR_THREADS) add_biases_kernel(const LrArgs p) {
+    constexpr int PER = LR_LIST / LR_THREADS, PLACES = 4 * LR_LIST;      // entries of a thread; places of the table, most of them empty
+    __shared__ int ids[LR_LIST], token[PLACES], first_of[PLACES], count[PLACES];
+    __shared__ float values[LR_LIST];
+    pdl_launch_dependents();
+    for (int i = threadIdx.x; i < PLACES; i += LR_THREADS) { token[i] = -1; first_of[i] = LR_LIST; count[i] = 0; }
+    pdl_wait();
+    const int b = blockIdx.x, m = p.masks ? p.mask_rows[b] : -1;
+    const int2 list = p.bias_range[b];
+    const int first = max(list.x, 0), last = min(list.y, p.n_bias);
+    const unsigned* mask = m >= 0 && m < p.n_masks ? p.masks + (size_t)m * p.mask_words : nullptr;
+    float* out = p.out + (size_t)b * p.vocab;
+    for (int base = first; base < last; base += LR_LIST) {
+        int id[PER], place[PER];
+        float now[PER];
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int e = k * LR_THREADS + threadIdx.x;
+            id[k] = base + e < last ? p.bias_ids[base + e] : -1;
+            values[e] = base + e < last ? p.bias_values[base + e] : 0.f;
+            if (id[k] >= p.vocab) id[k] = -1;
+            ids[e] = id[k];
+        }
+        __syncthreads();                                            // (the table is empty, and the turn before has written)
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            now[k] = 0.f;
+            if (id[k] < 0) continue;
+            if (mask && !((mask[id[k] >> 5] >> (id[k] & 31)) & 1u)) { id[k] = -1; continue; }
+            now[k] = out[id[k]];
+            unsigned at = ((unsigned)id[k] * 2654435761u) >> 20 & (PLACES - 1);
+            for (;;) {
+                const int there = atomicCAS(&token[at], -1, id[k]);
+                if (there == -1 || there == id[k]) break;
+                at = (at + 1) & (PLACES - 1);
+            }
+            place[k] = at;
+            atomicMin(&first_of[at], k * LR_THREADS + (int)threadIdx.x);
+            atomicAdd(&count[at], 1);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int e = k * LR_THREADS + threadIdx.x;
+            if (id[k] < 0 || first_of[place[k]] != e) continue;
+            float sum = values[e];
+            for (int i = e + 1, left = count[place[k]] - 1; left > 0; ++i)
+                if (ids[i] == id[k]) { sum += values[i]; --left; }
+            out[id[k]] = now[k] + sum;
+        }
+        if (base + LR_LIST < last) {                                // empty the table for the next turn
+            __syncthreads();
+            for (int i = threadIdx.x; i < PLACES; i += LR_THREADS) { token[i] = -1; first_of[i] = LR_LIST; count[i] = 0; }
+        }
     }
 }
 
@@ -94,8 +212,15 @@ extern "C" int pe_adjust_logits(const float* logits, float* out, int rows, int v
         return PE_ERR_UNSUPPORTED;
     const LrArgs p = {logits, out, rows, vocab, slots, (const short*)history, n_slots, penalties, (const int2*)bias_range, bias_ids, bias_values, n_bias,
                       (const unsigned*)masks, n_masks, (vocab + 31) / 32, mask_rows};
-    PE_TRY(pe_launch(adjust_logits_kernel, dim3((vocab + LR_CHUNK - 1) / LR_CHUNK, rows), LR_THREADS, 0, (cudaStream_t)stream, p));
+    const bool aligned = !(((uintptr_t)logits | (uintptr_t)out) & 15), in_place = logits == out;
+    const auto kernel = aligned ? (in_place ? adjust_logits_kernel<true, true> : adjust_logits_kernel<true, false>)
+                                : (in_place ? adjust_logits_kernel<false, true> : adjust_logits_kernel<false, false>);
+    PE_TRY(pe_launch(kernel, dim3((vocab + LR_CHUNK - 1) / LR_CHUNK, rows), LR_THREADS, 0, (cudaStream_t)stream, p));
     PE_LAUNCH_CHECK();
+    if (bias_ids) {
+        PE_TRY(pe_launch(add_biases_kernel, rows, LR_THREADS, 0, (cudaStream_t)stream, p));
+        PE_LAUNCH_CHECK();
+    }
     return 0;
 }
 

@@ -11,7 +11,7 @@ from typing import Optional
 
 import torch
 
-from .library import DTYPE_CODE, KernelError, check, core, extras, gated, mixers, stream_ptr
+from .library import DTYPE_CODE, KernelError, answers, check, core, extras, for_head_dim, gated, mixers, stream_ptr
 
 PAGE = 64     # tokens per cache page; PE_PAGE in csrc/common.cuh
 
@@ -1932,18 +1932,18 @@ def attention_shared(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: i
     group has, how many positions they share (whole pages, no more than the least position of the group; 0: none), and which token has
     the least position: its row of the page table names the shared pages.  Head sizes 64 and 128 (``attention_shared_takes``); results are
     those of ``attention_decode`` up to the order of float32 sums."""
-    from .library import for_head_dim
-    T = tok_pos.shape[0]
-    _need(q, "q", torch.bfloat16); _need(k_pool, "k_pool", torch.bfloat16); _need(v_pool, "v_pool", torch.bfloat16, k_pool.shape)
-    if not attention_shared_takes(q.dtype, T, n_heads, n_kv_heads, head_dim, scale):
+    T, pool = tok_pos.shape[0], k_pool.shape
+    _need(q, "q", torch.bfloat16); _need(k_pool, "k_pool", torch.bfloat16); _need(v_pool, "v_pool", torch.bfloat16, pool)
+    if not attention_shared_takes(torch.bfloat16, T, n_heads, n_kv_heads, head_dim, scale):
         raise KernelError(f"attention_shared takes at most {SHARED_MAX_ROWS} rows, head sizes {SHARED_HEAD_DIMS}, a positive scale and at most 128 query heads a key "
                           f"head, not {T} rows, {n_heads} / {n_kv_heads} heads of {head_dim}, scale {scale}")
-    if k_pool.dim() != 4 or tuple(k_pool.shape[1:]) != (n_kv_heads, PAGE, head_dim):
-        raise KernelError(f"cache pool must be [pages, {n_kv_heads}, {PAGE}, {head_dim}], not {tuple(k_pool.shape)}")
+    if len(pool) != 4 or pool[1:] != (n_kv_heads, PAGE, head_dim):
+        raise KernelError(f"cache pool must be [pages, {n_kv_heads}, {PAGE}, {head_dim}], not {tuple(pool)}")
     _need(block_table, "block_table", torch.int32)
     _need(tok_pos, "tok_pos", torch.int32, (T,)); _need(tok_row, "tok_row", torch.int32, (T,)); _need(groups, "groups", torch.int32, (T, 4))
-    if q_stride % 8 or q_stride < n_heads * head_dim or (T and q.numel() < (T - 1) * q_stride + n_heads * head_dim):
-        raise KernelError(f"q must hold {T} rows of {n_heads * head_dim} numbers, {q_stride} (a multiple of 8) apart")
+    width = n_heads * head_dim
+    if q_stride % 8 or q_stride < width or (T and q.numel() < (T - 1) * q_stride + width):
+        raise KernelError(f"q must hold {T} rows of {width} numbers, {q_stride} (a multiple of 8) apart")
     if max_context < 1 or keep_first < 0 or (window is not None and window < 0) or groups.data_ptr() % 16:
         raise KernelError("max_context must be positive, window and keep_first not negative, and groups start on a 16-byte boundary")
     if slopes is not None:
@@ -1951,15 +1951,17 @@ def attention_shared(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: i
     if sinks is not None:
         _need(sinks, "sinks", torch.float32, (n_heads,))
     if out is None:
-        out = torch.empty(T, n_heads * head_dim, dtype=torch.bfloat16, device=q.device)
-    _need(out, "out", torch.bfloat16, (T, n_heads * head_dim))
+        out = torch.empty(T, width, dtype=torch.bfloat16, device=q.device)
+    else:
+        _need(out, "out", torch.bfloat16, (T, width))
     _need_here(q, "q")
     if T == 0:
         return out
     lib = for_head_dim(head_dim)
-    scratch = torch.empty(lib.pe_attention_shared_scratch(T, n_heads, n_kv_heads), dtype=torch.uint8, device=q.device)      # (of the call: graphs and streams share none)
-    check(lib.pe_attention_shared(q.data_ptr(), q_stride, out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_pool.shape[0], block_table.data_ptr(),
-                                  table_stride, tok_pos.data_ptr(), tok_row.data_ptr(), groups.data_ptr(), T, n_heads, n_kv_heads, head_dim, window or 0,
+    # (the scratch is the call's own: calls on two streams and captured graphs share none)
+    scratch = torch.empty(lib.pe_attention_shared_scratch(T, n_heads, n_kv_heads), dtype=torch.uint8, device=q.device)
+    check(lib.pe_attention_shared(q.data_ptr(), q_stride, out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), pool[0], block_table.data_ptr(), table_stride,
+                                  tok_pos.data_ptr(), tok_row.data_ptr(), groups.data_ptr(), T, n_heads, n_kv_heads, head_dim, window or 0,
                                   keep_first if window else 0, scale, max_context, _ptr(slopes), _ptr(sinks), 1 if early_pages else 0, scratch.data_ptr(),
                                   status_ptr(q.device), stream_ptr()), "attention_shared", 2)
     return out
@@ -2002,16 +2004,16 @@ def adjust_logits(logits: torch.Tensor, slots: Optional[torch.Tensor] = None, hi
         _need(masks, "masks", torch.int32, (n_masks, (V + 31) // 32)); _need(mask_rows, "mask_rows", torch.int32, (B,))
     if out is None:
         out = torch.empty_like(logits)
-    _need(out, "out", torch.float32, (B, V))
+    elif out is not logits:
+        _need(out, "out", torch.float32, (B, V))
     if B == 0 or V == 0:
         return out
     if B > 65535:
         raise KernelError(f"adjust_logits takes at most 65,535 rows, not {B}")
     _need_here(logits, "logits")
-    from .library import answers
     check(answers().pe_adjust_logits(logits.data_ptr(), out.data_ptr(), B, V, _ptr(slots), _ptr(history), n, _ptr(penalties), _ptr(bias_range),
                                      _ptr(bias_ids) if n_bias else None, _ptr(bias_values), n_bias, _ptr(masks) if n_masks else None, n_masks,
-                                     _ptr(mask_rows), stream_ptr()), "adjust_logits")
+                                     _ptr(mask_rows), stream_ptr()), "adjust_logits", 2 if n_bias else 1)
     return out
 
 
@@ -2038,7 +2040,6 @@ def note_tokens(history: Optional[torch.Tensor], slots: torch.Tensor, tokens: to
     if N == 0 or n == 0:
         return history
     _need_here(tokens, "tokens")
-    from .library import answers
     check(answers().pe_note_tokens(_ptr(history), n, V, slots.data_ptr(), tokens.data_ptr(), N, 1 if prompt else 0, _ptr(states), _ptr(transitions), n_states,
                                    stream_ptr()), "note_tokens")
     return history
@@ -2055,17 +2056,15 @@ def step_tables(slots: torch.Tensor, starts: torch.Tensor, lens: torch.Tensor, h
     if tables.dim() != 2 or resident.dim() != 2:
         raise KernelError("resident and tables must be page tables, a row a sequence")
     B, T = slots.shape[0], tok_pos.shape[0]
-    for t, name in ((slots, "slots"), (starts, "starts"), (lens, "lens"), (held, "held")):
-        _need(t, name, torch.int32, (B,))
+    row, res, table = (B,), resident.shape, tables.shape
+    _need(slots, "slots", torch.int32, row); _need(starts, "starts", torch.int32, row); _need(lens, "lens", torch.int32, row); _need(held, "held", torch.int32, row)
     _need(pages, "pages", torch.int32, (pages.numel(),)); _need(resident, "resident", torch.int32)
-    for t, name in ((tok_pos, "tok_pos"), (tok_row, "tok_row"), (places, "places")):
-        _need(t, name, torch.int32, (T,))
-    _need(row_first, "row_first", torch.int32, (B + 1,)); _need(tables, "tables", torch.int32, (B, tables.shape[1]))
+    _need(tok_pos, "tok_pos", torch.int32); _need(tok_row, "tok_row", torch.int32, (T,)); _need(places, "places", torch.int32, (T,))
+    _need(row_first, "row_first", torch.int32, (B + 1,)); _need(tables, "tables", torch.int32, (B, table[1]))
     if B == 0:
         raise KernelError("a step needs at least one row")
     _need_here(slots, "slots")
-    from .library import answers
     check(answers().pe_step_tables(slots.data_ptr(), starts.data_ptr(), lens.data_ptr(), held.data_ptr(), pages.data_ptr(), pages.shape[0],
-                                   resident.data_ptr(), resident.shape[0], resident.shape[1], B, tok_pos.data_ptr(), tok_row.data_ptr(),
-                                   row_first.data_ptr(), places.data_ptr(), T, tables.data_ptr(), tables.shape[1], stream_ptr()), "step_tables")
+                                   resident.data_ptr(), res[0], res[1], B, tok_pos.data_ptr(), tok_row.data_ptr(),
+                                   row_first.data_ptr(), places.data_ptr(), T, tables.data_ptr(), table[1], stream_ptr()), "step_tables")
     return tok_pos, tok_row, row_first, places, tables

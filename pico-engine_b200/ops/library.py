@@ -306,10 +306,10 @@ def head_dim_sizes() -> range:
 
 def for_head_dim(head_dim: int) -> ctypes.CDLL:
     """The tensor-core attention kernels compiled for one head size; compiled at the first call."""
-    if head_dim not in head_dim_sizes():
-        raise KernelError(f"head size {head_dim} is not taken: multiples of 16 from 16 to 256 are")
     lib = _by_head_dim.get(head_dim)
     if lib is None:
+        if head_dim not in head_dim_sizes():
+            raise KernelError(f"head size {head_dim} is not taken: multiples of 16 from 16 to 256 are")
         lib = build.load(f"attention_hd{head_dim}", HEAD_DIM_SOURCES, {"PE_HEAD_DIM": str(head_dim)})
         declare(lib, _HEAD_DIM_SIGNATURES)
         lib.pe_attention_shared_scratch.argtypes = [I, I, I]
