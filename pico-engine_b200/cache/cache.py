@@ -18,6 +18,8 @@ sequence.
 * Values may have another head size and another number of heads than keys (``KVNeed.v_head_dim``, ``v_heads``): the
   pools are then shaped accordingly (this library's attention kernels take equal shapes; a mixer that asks for
   others brings the kernel that reads them).
+* A sequence may be *forked* (``fork``): the new ones begin with its positions.  Whole pages are shared, a page that is not full yet is copied (each
+  sequence goes on in its own), and so is the state.  A shared page is free again when its last sequence has given it back.
 * Beside what sequences hold there is one *idle* slot with one page in every group (``idle_slot``,
   ``idle_page``: the index after the last real one): a step that is padded to a fixed number of rows
   (a captured decode step of a bucket of rows) lets its idle rows read and write there, so that
@@ -72,6 +74,9 @@ class Cache:
         self.max_seqs = max_seqs
         self.slots = FreeList(max_seqs, "sequence slot")
         self.lengths: Dict[int, int] = {}
+        self.births: Dict[int, int] = {}          # slot -> a number of its own for each sequence that has held it
+        self.prefix: Dict[int, tuple] = {}        # slot -> (family, positions): forked sequences of a family share so many positions, in whole pages
+        self._born = self._families = 0
         self.groups: List[KVGroup] = []
         self.group_of: Dict[int, int] = {}        # schedule entry -> group
         self.index_in_group: Dict[int, int] = {}
@@ -107,6 +112,8 @@ class Cache:
         """A slot for a new, empty sequence."""
         (slot,) = self.slots.take(1)
         self.lengths[slot] = 0
+        self._born += 1
+        self.births[slot] = self._born
         for g in self.groups:
             g.table[slot] = []
         for t in self.state.values():
@@ -119,8 +126,38 @@ class Cache:
             raise CacheStateError(f"sequence slot {slot} is closed but is not open")
         for g in self.groups:
             g.pages.give(p for p in g.table.pop(slot) if p >= 0)
-        del self.lengths[slot]
+        del self.lengths[slot], self.births[slot]
+        self.prefix.pop(slot, None)
         self.slots.give([slot])
+
+    def fork(self, slot: int, n: int = 1) -> List[int]:
+        """``n`` new sequences that begin with the positions of ``slot`` (which goes on as one of the family)."""
+        if slot not in self.lengths:
+            raise CacheStateError(f"sequence slot {slot} is forked but is not open")
+        length = self.lengths[slot]
+        whole, part = length // PAGE, length % PAGE != 0
+        if self.slots.free_count < n or any(part and g.pages.free_count < n for g in self.groups):
+            raise CacheFull(f"{n} sequences wanted from slot {slot}: {self.slots.free_count} slots are free, and "
+                            f"{[g.pages.free_count for g in self.groups]} pages")
+        new = [self.open() for _ in range(n)]
+        for g in self.groups:
+            row = g.table[slot]
+            own = g.pages.take(n) if part and row[whole] >= 0 else [-1] * n
+            for s, page in zip(new, own):
+                g.pages.share(p for p in row[:whole] if p >= 0)
+                g.table[s] = row[:whole] + ([page] if part else [])
+            if g.k is not None and part and row[whole] >= 0 and n:
+                for pool in (g.k, g.v):
+                    pool[:, own] = pool[:, row[whole]:row[whole] + 1].clone()
+        for t in self.state.values():
+            t[new] = t[slot:slot + 1].clone()
+        if self.prefix.get(slot, (0, -1))[1] != whole * PAGE:
+            self._families += 1
+            self.prefix[slot] = (self._families, whole * PAGE)
+        for s in new:
+            self.lengths[s] = length
+            self.prefix[s] = self.prefix[slot]
+        return new
 
     def length(self, slot: int) -> int:
         return 0 if slot == self.idle_slot else self.lengths[slot]
@@ -199,8 +236,13 @@ class Cache:
             raise CacheStateError("open sequences and held slots differ")
         for g in self.groups:
             g.pages.check()
-            held = [p for row in g.table.values() for p in row if p >= 0]
-            if len(held) != len(set(held)):
-                raise CacheStateError("a page belongs to two sequences")
+            held: Dict[int, int] = {}
+            for row in g.table.values():
+                for p in row:
+                    if p >= 0:
+                        held[p] = held.get(p, 0) + 1
+            for p, times in held.items():
+                if times != g.pages.times_held(p):
+                    raise CacheStateError("a page belongs to two sequences" if times > g.pages.times_held(p) else f"page {p} is held more often than sequences own it")
             if len(held) != g.pages.held_count:
                 raise CacheStateError("pages are held that no sequence owns")

@@ -16,12 +16,13 @@ class CacheStateError(RuntimeError):
 
 class FreeList:
     """Integers 0..n-1, taken and given back.  The lowest free ones are taken first, so a
-    batch that follows another uses the same ones again."""
+    batch that follows another uses the same ones again.  What is held may be shared: it is free again when
+    it has been given back once for being taken and once for every time it was shared."""
 
     def __init__(self, n: int, what: str):
         self.n, self.what = n, what
         self._free: List[int] = list(range(n - 1, -1, -1))     # pop() yields the lowest
-        self._held = [False] * n
+        self._held = [0] * n                                   # how often each is held
 
     @property
     def free_count(self) -> int:
@@ -36,16 +37,30 @@ class FreeList:
             raise CacheFull(f"{count} {self.what}(s) wanted, {len(self._free)} of {self.n} free")
         got = [self._free.pop() for _ in range(count)]
         for i in got:
-            self._held[i] = True
+            self._held[i] = 1
         return got
 
-    def give(self, items) -> None:
+    def share(self, items) -> None:
+        """Hold what is held already once more."""
         items = list(items)
         for i in items:
             if not (0 <= i < self.n) or not self._held[i]:
+                raise CacheStateError(f"{self.what} {i} is shared but is not held")
+        for i in items:
+            self._held[i] += 1
+
+    def times_held(self, item: int) -> int:
+        return self._held[item]
+
+    def give(self, items) -> None:
+        free = []
+        for i in items:
+            if not (0 <= i < self.n) or not self._held[i]:
                 raise CacheStateError(f"{self.what} {i} is given back but is not held")
-            self._held[i] = False
-        self._free.extend(items)
+            self._held[i] -= 1
+            if not self._held[i]:
+                free.append(i)
+        self._free.extend(free)
         self._free.sort(reverse=True)
 
     def check(self) -> None:
@@ -53,5 +68,5 @@ class FreeList:
         if len(set(self._free)) != len(self._free):
             raise CacheStateError(f"a {self.what} is in the free list twice")
         for i in range(self.n):
-            if self._held[i] == (i in set(self._free)):
+            if bool(self._held[i]) == (i in set(self._free)):
                 raise CacheStateError(f"{self.what} {i} is {'both held and free' if self._held[i] else 'lost'}")

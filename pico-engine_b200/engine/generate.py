@@ -24,6 +24,7 @@ class Request:
     max_new_tokens: int
     output: List[int] = field(default_factory=list)
     finish_reason: str = ""         # "stop", "length" or "empty"
+    family: int = -1                # requests of one family (0, 1, ..) follow one another and have the same prompt; -1: a family of its own
 
 
 class Backend(Protocol):
@@ -37,6 +38,10 @@ class Backend(Protocol):
     #   decode_end(handle) -> List[int]
     # where sources[j] >= 0 names the row of the step begun just before whose chosen token is
     # row j's input (tokens[j] is then ignored), and optionally decode_idle().
+    # A backend that is given several answers to a prompt has
+    #   prefill_answers(slots, prompts, requests: list of lists) -> (list of lists of further slots, List[int])
+    # which runs each prompt once, in its slot, and opens a slot for every further request of the prompt's list that
+    # goes on from there; the tokens come request after request.
 
 
 class GenerationError(ValueError):
@@ -129,10 +134,22 @@ def run_batch(backend: Backend, batch: Sequence[Request], stop_token_ids: Iterab
             r.finish_reason = "length"
     if not active:
         return
-    slot_of = {r.index: backend.open() for r in active}
+    prompts: List[List[Request]] = []          # the requests of every prompt that is run
+    for r in active:
+        if prompts and r.family >= 0 and r.family == prompts[-1][0].family:
+            prompts[-1].append(r)
+        else:
+            prompts.append([r])
+    slot_of = {p[0].index: backend.open() for p in prompts}
     try:
-        chosen = backend.prefill([slot_of[r.index] for r in active], [r.prompt for r in active],
-                                 [r.index for r in active])
+        if len(prompts) == len(active):
+            chosen = backend.prefill([slot_of[r.index] for r in active], [r.prompt for r in active],
+                                     [r.index for r in active])
+        else:
+            further, chosen = backend.prefill_answers([slot_of[p[0].index] for p in prompts], [p[0].prompt for p in prompts],
+                                                      [[r.index for r in p] for p in prompts])
+            for p, slots in zip(prompts, further):
+                slot_of.update((r.index, slot) for r, slot in zip(p[1:], slots))
         if getattr(backend, "pipelined", False):
             _decode_ahead(backend, active, chosen, slot_of, stop)
             return
@@ -196,16 +213,22 @@ def _decode_ahead(backend, rows: List[Request], chosen: Sequence[int], slot_of: 
 
 
 def generate(backend: Backend, prompts: Sequence[Sequence[int]], max_new_tokens, stop_token_ids: Iterable[int],
-             max_batch: int, max_tokens: int) -> List[Request]:
+             max_batch: int, max_tokens: int, answers: int = 1) -> List[Request]:
     """``max_new_tokens`` is one number or one per prompt.  An empty prompt yields nothing
-    (pico-engine returns ("", []) for it, src/pico_engine/engine.py:313-314)."""
+    (pico-engine returns ("", []) for it, src/pico_engine/engine.py:313-314).  ``answers``: so many requests for every prompt, one
+    after the other; those of a batch run their prompt once and go on from its cache."""
+    if answers < 1:
+        raise GenerationError("a prompt needs at least one answer")
     if isinstance(max_new_tokens, int):
         max_new_tokens = [max_new_tokens] * len(prompts)
     if len(max_new_tokens) != len(prompts):
         raise GenerationError("max_new_tokens must be one number or one per prompt")
     if any(m < 0 for m in max_new_tokens):
         raise GenerationError("max_new_tokens must be non-negative")
-    requests = [Request(i, [int(t) for t in p], int(m)) for i, (p, m) in enumerate(zip(prompts, max_new_tokens))]
+    requests = []
+    for i, (p, m) in enumerate(zip(prompts, max_new_tokens)):
+        ids = [int(t) for t in p]
+        requests += [Request(i * answers + j, ids, int(m), family=i if answers > 1 else -1) for j in range(answers)]
     runnable = []
     for r in requests:
         if not r.prompt:

@@ -161,3 +161,80 @@ def test_values_and_state_may_be_shaped_otherwise():
     assert c.bytes() == 4 * (2 * 3 * PAGE * (2 * 16 + 2 * 24) + 3 * PAGE * 40) + 3 * 6 * 2 + 3 * 3 * 4
     with pytest.raises(ValueError, match="state_dtype"):
         Cache([CacheNeeds(state_elems=2, state_dtype="int8")], 64, 1, torch.float32, "cpu")
+
+
+def test_a_held_item_may_be_shared():
+    f = FreeList(3, "page")
+    a, b = f.take(2)
+    f.share([a, a])
+    assert f.times_held(a) == 3 and f.free_count == 1
+    f.give([a, b]); f.check()
+    assert f.free_count == 2 and f.times_held(a) == 2
+    f.give([a, a]); f.check()
+    assert f.free_count == 3
+    for bad in (a, 2, 3, -1):
+        with pytest.raises(CacheStateError):
+            f.share([bad])
+    f.check()
+
+
+@pytest.mark.parametrize("length", [1, 63, 64, 65, 200])
+def test_fork_shares_whole_pages_and_copies_the_last_one(length):
+    c = Cache(needs(window=None, state=4), max_tokens=2048, max_seqs=6, dtype=torch.float32, device="cpu")
+    a = c.open()
+    c.reserve(a, length); c.advance(a, length)
+    for g in c.groups:
+        g.k.uniform_(); g.v.uniform_()
+    for t in c.state.values():
+        t[a].uniform_()
+    before = [g.pages.held_count for g in c.groups]
+    b, d = c.fork(a, 2)
+    c.check()
+    whole = length // PAGE
+    for g, n in zip(c.groups, before):
+        for s in (b, d):
+            assert g.table[s][:whole] == g.table[a][:whole] and len(g.table[s]) == len(g.table[a])
+        last = {g.table[s][-1] for s in (a, b, d)}
+        assert g.pages.held_count == n + (2 if length % PAGE else 0) and len(last) == (3 if length % PAGE else 1)
+        for s in (b, d):
+            assert torch.equal(g.k[:, g.table[s]], g.k[:, g.table[a]]) and torch.equal(g.v[:, g.table[s]], g.v[:, g.table[a]])
+    for t in c.state.values():
+        assert torch.equal(t[b], t[a]) and torch.equal(t[d], t[a])
+    assert c.prefix[a] == c.prefix[b] == c.prefix[d] and c.prefix[a][1] == whole * PAGE and c.length(b) == length
+    c.reserve(a, 70); c.advance(a, 70)                      # each goes on in pages of its own
+    c.close(a); c.check()
+    assert torch.equal(c.groups[0].k[:, c.groups[0].table[b]], c.groups[0].k[:, c.groups[0].table[d]]) or length % PAGE
+    c.close(b); c.check(); c.close(d); c.check()
+    assert all(g.pages.free_count == g.pages.n for g in c.groups) and not c.prefix and not c.births
+
+
+def test_fork_of_windowed_sequences_and_of_forks():
+    c = Cache(needs(window=100), max_tokens=4096, max_seqs=8, dtype=torch.float32, device="cpu")
+    a = c.open()
+    c.reserve(a, 300); c.advance(a, 300)
+    (b,) = c.fork(a)
+    assert c.groups[1].table[b][:3] == c.groups[1].table[a][:3] and c.groups[1].table[b][0] == -1
+    c.reserve(b, 200); c.advance(b, 200)                    # b's window leaves what a still holds
+    c.check()
+    assert c.groups[1].table[a][3] >= 0 and c.groups[1].table[b][3] == -1
+    family = c.prefix[a]
+    (d,) = c.fork(a)                                         # the same positions: the same family
+    assert c.prefix[a] == c.prefix[d] == family
+    (e,) = c.fork(b)                                         # more of them: a family of its own
+    assert c.prefix[e] == c.prefix[b] != family and c.prefix[b][1] == 448
+    for s in (a, b, d, e):
+        c.close(s); c.check()
+
+
+def test_fork_refuses_what_it_cannot_hold():
+    c = Cache(needs(), max_tokens=256, max_seqs=3, dtype=torch.float32, device="cpu")
+    a = c.open()
+    c.reserve(a, 130); c.advance(a, 130)
+    for n, closed in ((3, False), (2, False)):               # too many slots; too few pages for two copies
+        with pytest.raises(CacheFull):
+            c.fork(a, n)
+        c.check()
+        assert list(c.lengths) == [a]
+    assert c.fork(a, 0) == []
+    with pytest.raises(CacheStateError):
+        c.fork(1)

@@ -197,3 +197,51 @@ def test_prompts_are_cut_into_steps_of_a_token_budget():
         assert [seen[r][0] for r in range(len(lengths))] == lengths
     with pytest.raises(GenerationError):
         cut_prompts([3], 0)
+
+
+class Family(Scripted):
+    """A backend that goes on from a prompt's cache for its further requests."""
+
+    def prefill_answers(self, slots, prompts, requests):
+        self.calls.append(("answers", [list(r) for r in requests], [len(p) for p in prompts]))
+        further = [[self.open() for _ in r[1:]] for r in requests]
+        for s, more, p in zip(slots, further, prompts):
+            for x in [s] + more:
+                self.open_slots[x] += len(p)
+        return further, [self.script[i][0] for r in requests for i in r]
+
+
+def test_answers_to_a_prompt_run_it_once():
+    script = {0: [1, 2, 3], 1: [9], 2: [4, 9], 3: [5, 6, 7], 4: [9], 5: [8, 8, 8]}
+    be = Family(script)
+    reqs = generate(be, [[1, 2, 3], [4]], [3, 2], stop_token_ids=[9], max_batch=8, max_tokens=4096, answers=3)
+    assert [r.index for r in reqs] == list(range(6)) and [r.family for r in reqs] == [0, 0, 0, 1, 1, 1]
+    assert [r.output for r in reqs] == [[1, 2, 3], [], [4], [5, 6], [], [8, 8]]
+    assert be.calls[0] == ("answers", [[0, 1, 2], [3, 4, 5]], [3, 1])
+    assert be.calls[1][:2] == ("decode", [0, 2, 3, 5])
+    assert not be.open_slots and be.free == list(range(8))
+
+
+def test_answers_that_do_not_fit_one_batch_run_their_prompt_again():
+    script = {i: [i + 1, i + 1] for i in range(6)}
+    be = Family(script, slots=4)
+    reqs = generate(be, [[1, 2], [3]], 2, stop_token_ids=[], max_batch=4, max_tokens=4096, answers=3)
+    assert [r.output for r in reqs] == [[i + 1] * 2 for i in range(6)]
+    assert [c[:2] for c in be.calls if c[0] != "decode"] == [("answers", [[0, 1, 2], [3]]), ("answers", [[4, 5]])]
+    # one answer each, and a prompt that is empty or may not be answered: the plain way
+    be = Family({i: [i] for i in range(6)})
+    reqs = generate(be, [[], [7], [8]], [3, 0, 1], stop_token_ids=[], max_batch=1, max_tokens=4096, answers=2)
+    assert [r.finish_reason for r in reqs] == ["empty", "empty", "length", "length", "length", "length"]
+    assert all(c[0] != "answers" for c in be.calls)
+    with pytest.raises(GenerationError):
+        generate(be, [[1]], 1, [], 1, 4096, answers=0)
+
+
+def test_an_error_among_answers_gives_all_slots_back():
+    class Broken(Family):
+        def decode(self, *a):
+            raise RuntimeError("no")
+    be = Broken({i: [1, 1] for i in range(3)})
+    with pytest.raises(RuntimeError):
+        generate(be, [[1, 2]], 2, [], 8, 4096, answers=3)
+    assert not be.open_slots and be.free == list(range(8))
