@@ -25,8 +25,13 @@ struct LrArgs {
     const int* slots; const short* history; int n_slots;
     const float* penalties;
     const int2* bias_range; const int* bias_ids; const float* bias_values; int n_bias;
-    const unsigned* masks; int n_masks, mask_words; const int* mask_rows;
+    const unsigned* masks; int n_masks, mask_words; const int* mask_rows; int by_slot;      // by_slot: mask_rows has an entry a slot, not a row
 };
+// the mask of row b, or -1
+__device__ __forceinline__ int lr_mask(const LrArgs& p, int b, int slot) {
+    if (!p.masks || (p.by_slot && (slot < 0 || slot >= p.n_slots))) return -1;
+    return p.mask_rows[p.by_slot ? slot : b];
+}
 
 // Four tokens at a time: those that lie on 16 bytes of the row (a vocabulary need not be a multiple of four), and what is left at the row's ends one by one.
 // ALIGNED: logits and out start on 16 bytes; else every load and store takes one number.
@@ -39,8 +44,8 @@ __global__ void __launch_bounds__(LR_THREADS, 8) adjust_logits_kernel(const LrAr
     const size_t at0 = (size_t)b * V;
     const float* row = p.logits + at0;
     float* out = p.out + at0;
-    const int slot = p.history ? p.slots[b] : -1, m = p.masks ? p.mask_rows[b] : -1;
-    const bool known = slot >= 0 && slot < p.n_slots;
+    const int slot = p.slots ? p.slots[b] : -1, m = lr_mask(p, b, slot);
+    const bool known = p.history && slot >= 0 && slot < p.n_slots;
     const short* seen = p.history + (known ? (size_t)slot * V : 0);
     const unsigned* mask = m >= 0 && m < p.n_masks ? p.masks + (size_t)m * p.mask_words : nullptr;
     float repetition = 1.f, inverse = 1.f, presence = 0.f, frequency = 0.f;
@@ -116,7 +121,7 @@ __global__ void __launch_bounds__(LR_THREADS) add_biases_kernel(const LrArgs p) 
     pdl_launch_dependents();
     for (int i = threadIdx.x; i < PLACES; i += LR_THREADS) { token[i] = -1; first_of[i] = LR_LIST; count[i] = 0; }
     pdl_wait();
-    const int b = blockIdx.x, m = p.masks ? p.mask_rows[b] : -1;
+    const int b = blockIdx.x, m = lr_mask(p, b, p.by_slot ? p.slots[b] : -1);
     const int2 list = p.bias_range[b];
     const int first = max(list.x, 0), last = min(list.y, p.n_bias);
     const unsigned* mask = m >= 0 && m < p.n_masks ? p.masks + (size_t)m * p.mask_words : nullptr;
@@ -205,13 +210,13 @@ extern "C" void pe_set_pdl(int on) { pe_pdl_enabled() = on ? 1 : 0; }     // (th
 
 extern "C" int pe_adjust_logits(const float* logits, float* out, int rows, int vocab, const int* slots, const void* history, int n_slots,
                                 const float* penalties, const void* bias_range, const int* bias_ids, const float* bias_values, int n_bias,
-                                const void* masks, int n_masks, const int* mask_rows, void* stream) {
+                                const void* masks, int n_masks, const int* mask_rows, int by_slot, void* stream) {
     if (rows <= 0) return 0;
-    if (vocab <= 0 || rows > 65535 || (history && (!slots || !penalties)) || (bias_ids && (!bias_range || !bias_values)) || (masks && !mask_rows) ||
+    if (vocab <= 0 || rows > 65535 || (history && (!slots || !penalties)) || (bias_ids && (!bias_range || !bias_values)) || (masks && !mask_rows) || (by_slot && !slots) ||
         ((uintptr_t)bias_range & 7))
         return PE_ERR_UNSUPPORTED;
     const LrArgs p = {logits, out, rows, vocab, slots, (const short*)history, n_slots, penalties, (const int2*)bias_range, bias_ids, bias_values, n_bias,
-                      (const unsigned*)masks, n_masks, (vocab + 31) / 32, mask_rows};
+                      (const unsigned*)masks, n_masks, (vocab + 31) / 32, mask_rows, by_slot};
     const bool aligned = !(((uintptr_t)logits | (uintptr_t)out) & 15), in_place = logits == out;
     const auto kernel = aligned ? (in_place ? adjust_logits_kernel<true, true> : adjust_logits_kernel<true, false>)
                                 : (in_place ? adjust_logits_kernel<false, true> : adjust_logits_kernel<false, false>);

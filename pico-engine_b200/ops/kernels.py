@@ -416,6 +416,10 @@ def attention(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int, hea
     but each token's own (see ``attention_decode``); a caller that cannot promise this passes False."""
     if q.dtype == torch.bfloat16:
         if ctx.one_token_each:
+            groups = ctx.scratch.get("shared_groups")        # rows of the step that share pages, where reading those once pays
+            if groups is not None and attention_shared_takes(q.dtype, tok_pos.shape[0], n_heads, n_kv_heads, head_dim, scale):
+                return attention_shared(q, q_stride, n_heads, n_kv_heads, head_dim, k_pool, v_pool, block_table, table_stride, tok_pos, tok_row, groups,
+                                        window, scale, ctx.max_context, early_pages=own_rows_only, together=True)
             return attention_decode(q, q_stride, n_heads, n_kv_heads, head_dim, k_pool, v_pool, block_table,
                                     table_stride, tok_pos, tok_row, window, scale, ctx.max_context,
                                     early_pages=own_rows_only)
@@ -1048,6 +1052,10 @@ def attention_headmix(q: torch.Tensor, q_stride: int, n_heads: int, n_kv: int, h
             and HEADMIX_TENSOR_CORES == "1"):
         # single tokens at the same sizes: the decode kernel of the plain attention, which knows both as well (the kernels before
         # it in the stream write no cache row but each token's own)
+        groups = ctx.scratch.get("shared_groups")
+        if groups is not None and attention_shared_takes(q.dtype, tok_pos.shape[0], n_heads, n_kv, head_dim, scale):
+            return attention_shared(q, q_stride, n_heads, n_kv, head_dim, k_pool, v_pool, block_table, table_stride, tok_pos, tok_row, groups, window, scale,
+                                    ctx.max_context, keep_first=keep_first, slopes=slopes, sinks=sink, together=True)
         return attention_decode(q, q_stride, n_heads, n_kv, head_dim, k_pool, v_pool, block_table, table_stride, tok_pos, tok_row,
                                 window, scale, ctx.max_context, keep_first=keep_first, slopes=slopes, sinks=sink)
     lib = mixers()
@@ -1906,6 +1914,18 @@ def attention_shared_takes(dtype: torch.dtype, rows: int, n_heads: int, n_kv_hea
             and n_heads // n_kv_heads <= 128)
 
 
+# Bytes of keys and values that a layer does not read again before reading shared pages together pays.  Read row by row they come from L2 at 8 to 13 TB/s; what
+# the second way costs is a longer start and its join.  Measured on a B200, one by one against together: 14 heads of 64, 16 rows on 2,048
+# positions (16 MB) 8.2 us against 9.6, on 8,192 (63 MB) 16.4, 12.9, 64 on 8,192 (264 MB) 35.8, 16.4; 28 heads of 128, 8 rows on 4,096 (59 MB) 14.3,
+# 15.6, 16 on 2,048 (63 MB) 15.1, 14.8, 64 on 8,192 (1,057 MB) 144, 30.5.
+SHARING_PAYS_BYTES = 64_000_000
+
+
+def sharing_pays(saved_bytes: int) -> bool:
+    """Whether reading shared pages together saves time, for so many bytes of keys and values that are not read again."""
+    return saved_bytes >= SHARING_PAYS_BYTES
+
+
 def shared_group_rows(members):
     """``groups`` of ``attention_shared`` for the rows of a step, on the host: ``members`` lists (tokens, shared positions, which of them
     has the least position) group after group, in the order of the rows; a row on its own is (1, 0, 0)."""
@@ -1926,9 +1946,10 @@ def shared_groups(members, device) -> torch.Tensor:
 def attention_shared(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int, head_dim: int, k_pool: torch.Tensor, v_pool: torch.Tensor,
                      block_table: torch.Tensor, table_stride: int, tok_pos: torch.Tensor, tok_row: torch.Tensor, groups: torch.Tensor,
                      window: Optional[int], scale: float, max_context: int, out: Optional[torch.Tensor] = None, keep_first: int = 0,
-                     slopes: Optional[torch.Tensor] = None, sinks: Optional[torch.Tensor] = None, early_pages: bool = True) -> torch.Tensor:
+                     slopes: Optional[torch.Tensor] = None, sinks: Optional[torch.Tensor] = None, early_pages: bool = True,
+                     together: Optional[bool] = None) -> torch.Tensor:
     """``attention_decode`` for single tokens of which several share the first pages of their sequences: those pages are read once for
-    all rows of a group.  ``groups`` int32 [T, 4], a row a token (``shared_groups``): the first token of its group, how many consecutive tokens the
+    all rows of a group (``together`` False: by every row; None: where ``sharing_pays`` for what the rows can share at most).  ``groups`` int32 [T, 4], a row a token (``shared_groups``): the first token of its group, how many consecutive tokens the
     group has, how many positions they share (whole pages, no more than the least position of the group; 0: none), and which token has
     the least position: its row of the page table names the shared pages.  Head sizes 64 and 128 (``attention_shared_takes``); results are
     those of ``attention_decode`` up to the order of float32 sums."""
@@ -1958,6 +1979,12 @@ def attention_shared(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: i
     if T == 0:
         return out
     lib = for_head_dim(head_dim)
+    if not (sharing_pays(4 * T * max_context * n_kv_heads * head_dim) if together is None else together):
+        check(lib.pe_attention_decode(q.data_ptr(), q_stride, out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(), table_stride,
+                                      tok_pos.data_ptr(), tok_row.data_ptr(), T, n_heads, n_kv_heads, head_dim, window or 0, scale, max_context,
+                                      1 if early_pages else 0, status_ptr(q.device), stream_ptr(), keep_first if window else 0, _ptr(slopes), _ptr(sinks)),
+              "attention_shared")
+        return out
     # (the scratch is the call's own: calls on two streams and captured graphs share none)
     scratch = torch.empty(lib.pe_attention_shared_scratch(T, n_heads, n_kv_heads), dtype=torch.uint8, device=q.device)
     check(lib.pe_attention_shared(q.data_ptr(), q_stride, out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), pool[0], block_table.data_ptr(), table_stride,
@@ -1970,7 +1997,7 @@ def attention_shared(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: i
 def adjust_logits(logits: torch.Tensor, slots: Optional[torch.Tensor] = None, history: Optional[torch.Tensor] = None,
                   penalties: Optional[torch.Tensor] = None, bias_range: Optional[torch.Tensor] = None, bias_ids: Optional[torch.Tensor] = None,
                   bias_values: Optional[torch.Tensor] = None, masks: Optional[torch.Tensor] = None, mask_rows: Optional[torch.Tensor] = None,
-                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                  out: Optional[torch.Tensor] = None, states: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The rules on what may be chosen next, on float32 logits [B, V]; returns ``out`` (a new tensor, or ``logits`` itself to change them in place).
 
     ``history`` int16 [n, V] with ``slots`` int32 [B] (its row of each batch row) and ``penalties`` float32 [B, 3] (repetition, presence, frequency):
@@ -1978,7 +2005,9 @@ def adjust_logits(logits: torch.Tensor, slots: Optional[torch.Tensor] = None, hi
     Seen tokens' logits are divided by the repetition penalty where positive and multiplied by it elsewhere; generated ones lose
     presence + count * frequency.  ``bias_range`` int32 [B, 2]: from where to where row b's biases lie in ``bias_ids`` (int32) and ``bias_values``
     (float32); a token that stands there twice gets both.  ``masks`` int32 [M, ceil(V / 32)] with ``mask_rows`` int32 [B]: where bit v % 32 of word
-    v / 32 of row b's mask is 0, the logit becomes -inf, whatever it was; -1: no mask.  A row that its mask leaves nothing is -inf everywhere."""
+    v / 32 of row b's mask is 0, the logit becomes -inf, whatever it was; -1: no mask.  A row that its mask leaves nothing is -inf everywhere.
+    ``states`` int32 [n] stands in the place of ``mask_rows`` where the masks are those of an automaton's states (``note_tokens``): row b's mask is
+    that of ``states[slots[b]]``."""
     if logits.dim() != 2:
         raise KernelError(f"logits must be [rows, vocabulary], not {tuple(logits.shape)}")
     B, V = logits.shape
@@ -1986,9 +2015,11 @@ def adjust_logits(logits: torch.Tensor, slots: Optional[torch.Tensor] = None, hi
     n = n_bias = n_masks = 0
     if (history is None) != (penalties is None) or (history is not None and slots is None):
         raise KernelError("history, slots and penalties go together")
+    if slots is not None:
+        _need(slots, "slots", torch.int32, (B,))
     if history is not None:
         n = history.shape[0]
-        _need(history, "history", torch.int16, (n, V)); _need(slots, "slots", torch.int32, (B,)); _need(penalties, "penalties", torch.float32, (B, 3))
+        _need(history, "history", torch.int16, (n, V)); _need(penalties, "penalties", torch.float32, (B, 3))
     if (bias_range is None) != (bias_ids is None) or (bias_ids is None) != (bias_values is None):
         raise KernelError("bias_range, bias_ids and bias_values go together")
     if bias_ids is not None:
@@ -1997,11 +2028,18 @@ def adjust_logits(logits: torch.Tensor, slots: Optional[torch.Tensor] = None, hi
         _need(bias_range, "bias_range", torch.int32, (B, 2))
         if bias_range.data_ptr() % 8:
             raise KernelError("bias_range must start on an 8-byte boundary")
-    if (masks is None) != (mask_rows is None):
-        raise KernelError("masks and mask_rows go together")
+    if (masks is None) != (mask_rows is None and states is None) or (mask_rows is not None and states is not None) or (states is not None and slots is None):
+        raise KernelError("masks and mask_rows go together, or masks, slots and states")
     if masks is not None:
         n_masks = masks.shape[0]
-        _need(masks, "masks", torch.int32, (n_masks, (V + 31) // 32)); _need(mask_rows, "mask_rows", torch.int32, (B,))
+        _need(masks, "masks", torch.int32, (n_masks, (V + 31) // 32))
+        if states is None:
+            _need(mask_rows, "mask_rows", torch.int32, (B,))
+        else:
+            n = states.shape[0]
+            _need(states, "states", torch.int32, (n,))
+            if history is not None and history.shape[0] != n:
+                raise KernelError(f"history and states must have a row a slot each, not {history.shape[0]} and {n}")
     if out is None:
         out = torch.empty_like(logits)
     elif out is not logits:
@@ -2013,7 +2051,7 @@ def adjust_logits(logits: torch.Tensor, slots: Optional[torch.Tensor] = None, hi
     _need_here(logits, "logits")
     check(answers().pe_adjust_logits(logits.data_ptr(), out.data_ptr(), B, V, _ptr(slots), _ptr(history), n, _ptr(penalties), _ptr(bias_range),
                                      _ptr(bias_ids) if n_bias else None, _ptr(bias_values), n_bias, _ptr(masks) if n_masks else None, n_masks,
-                                     _ptr(mask_rows), stream_ptr()), "adjust_logits", 2 if n_bias else 1)
+                                     _ptr(mask_rows if states is None else states), 0 if states is None else 1, stream_ptr()), "adjust_logits", 2 if n_bias else 1)
     return out
 
 

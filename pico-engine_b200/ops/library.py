@@ -135,7 +135,7 @@ _EXTRA_SIGNATURES = {
 }
 
 _ANSWER_SIGNATURES = {
-    "pe_adjust_logits": [P, P, I, I, P, P, I, P, P, P, P, I, P, I, P, P],
+    "pe_adjust_logits": [P, P, I, I, P, P, I, P, P, P, P, I, P, I, P, I, P],
     "pe_note_tokens": [P, I, I, P, P, I, I, P, P, I, P],
     "pe_step_tables": [P, P, P, P, P, I, P, I, I, I, P, P, P, P, I, P, I, P],
 }

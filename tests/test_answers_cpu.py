@@ -76,7 +76,9 @@ def rules(**change):
     (dict(history=i32(6, 100)), "history must be torch.int16"), (dict(history=there(torch.zeros(6, 99, dtype=torch.int16))), "history must have shape"),
     (dict(penalties=f32(4, 2)), "penalties must have shape"), (dict(bias_range=None), "go together"), (dict(bias_values=f32(8)), "bias_values must have shape"),
     (dict(bias_range=i32(5, 2)), "bias_range must have shape"), (dict(masks=None), "go together"), (dict(masks=i32(2, 3)), "masks must have shape"),
-    (dict(mask_rows=i32(3)), "mask_rows must have shape"), (dict(out=f32(4, 99)), "out must have shape"),
+    (dict(mask_rows=i32(3)), "mask_rows must have shape"), (dict(states=i32(6)), "go together"), (dict(mask_rows=None), "go together"),
+    (dict(mask_rows=None, states=i32(5)), "a row a slot each"), (dict(mask_rows=None, states=i32(6, 1)), "states must have shape"),
+    (dict(slots=i32(3)), "slots must have shape"), (dict(slots=None, history=None, penalties=None, mask_rows=None, states=i32(6)), "go together"), (dict(out=f32(4, 99)), "out must have shape"),
     (dict(logits=there(torch.zeros(100, 4).T)), "logits must be contiguous"),
 ])
 def test_adjust_logits_refuses(change, what):

@@ -63,11 +63,11 @@ class Answers:
         self.rows = randn(self.T, nh * hd + extra, seed=seed + 1, scale=1.5).bfloat16()      # queries inside wider rows
         self.sinks, self.slopes = randn(nh, seed=seed + 2), torch.exp2(-8.0 * torch.arange(1, nh + 1, device="cuda") / nh)
 
-    def run(self, K, window=None, keep=0, sinks=False, slopes=False, groups=None, out=None, bound=None):
+    def run(self, K, window=None, keep=0, sinks=False, slopes=False, groups=None, out=None, bound=None, together=True):
         return K.attention_shared(self.rows, self.rows.shape[1], self.nh, self.nkv, self.hd, self.k, self.v, self.table, self.width, ints(self.pos),
                                   torch.arange(self.T, dtype=torch.int32, device="cuda"), K.shared_groups(self.members, "cuda") if groups is None else groups,
                                   window, self.hd ** -0.5, bound or max(self.pos) + 1, out=out, keep_first=keep,
-                                  slopes=self.slopes if slopes else None, sinks=self.sinks if sinks else None)
+                                  slopes=self.slopes if slopes else None, sinks=self.sinks if sinks else None, together=together)
 
     def want(self, window=None, keep=0, sinks=False, slopes=False):
         """(result, sum p |v|) in 64 bits."""
@@ -167,6 +167,8 @@ def test_attention_shared_equals_each_row_alone(K):
     first = a.run(K)
     for _ in range(3):
         assert torch.equal(a.run(K), first)
+    agree(a.run(K, together=False), *want)                               # (the decode kernel, every row by itself)
+    assert torch.equal(a.run(K, together=None), a.run(K, together=False))      # what little rows share here does not pay
     assert torch.equal(a.run(K, bound=30000), a.run(K, bound=30000))
     K.check_status("cuda")
 
@@ -180,7 +182,7 @@ def test_attention_shared_in_two_captured_graphs(K):
         fixed = dict(groups=K.shared_groups(x.members, "cuda"))
         pos, row = ints(x.pos), torch.arange(x.T, dtype=torch.int32, device="cuda")
         call = lambda x=x, f=fixed, pos=pos, row=row: K.attention_shared(x.rows, x.rows.shape[1], x.nh, x.nkv, x.hd, x.k, x.v, x.table, x.width, pos, row,
-                                                                       f["groups"], None, x.hd ** -0.5, max(x.pos) + 1)
+                                                                       f["groups"], None, x.hd ** -0.5, max(x.pos) + 1, together=True)
         args.append(call)
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
@@ -344,6 +346,22 @@ def test_adjust_logits_of_a_view(K):
         logits.copy_(c["logits"])
         c["logits"] = logits
         rules_agree(adjust(K, c, out=out), want, size)
+
+
+def test_adjust_logits_by_an_automatons_states(K):
+    """The mask of a slot's state in the place of one named by the row: the same results; states and slots outside the tables have no mask."""
+    c = rules_case(9, 1234, seed=2, biases=20)
+    states = ints([-1, 3, 0, 2, 5, 1, 4, 2, 0, 1, -7, 3])
+    c["slots"] = ints([11, 0, 12, -1, 4, 7, 6, 10, 2])
+    n = len(states)
+    c["history"] = c["history"][:n] if c["history"].shape[0] >= n else None
+    assert c["history"] is not None
+    named = ints([int(states[s]) if 0 <= s < n else -1 for s in c["slots"].tolist()])
+    want = K.adjust_logits(c["logits"], c["slots"], c["history"], c["penalties"], c["bias_range"], c["bias_ids"], c["bias_values"], c["masks"], named)
+    got = K.adjust_logits(c["logits"], c["slots"], c["history"], c["penalties"], c["bias_range"], c["bias_ids"], c["bias_values"], c["masks"], states=states)
+    assert torch.equal(got, want)
+    alone = K.adjust_logits(c["logits"], c["slots"], masks=c["masks"], states=states)
+    assert torch.equal(alone, K.adjust_logits(c["logits"], masks=c["masks"], mask_rows=named))
 
 
 def test_rules_then_the_choice(K):
