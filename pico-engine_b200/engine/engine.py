@@ -17,7 +17,7 @@ from ..cache import Cache, PAGE
 from ..config.registry import architecture, read_config
 from ..ops import kernels
 from ..ops.library import core, require_cuda
-from ..sampling import Sampler, SamplingParams
+from ..sampling import RuleMemory, Sampler, SamplingParams, TokenAutomaton
 from ..weights import load_folder, load_into, random_tensor
 from .generate import Request, cut_prompts, generate as run_generation, held_tokens
 from .graph import GraphedDecode, TokenLoop, bucket_rows
@@ -70,6 +70,7 @@ class Engine:
         self.stepper: Optional[Stepper] = None
         self._graphs = {}
         self._token_loop: Optional[TokenLoop] = None
+        self._memory: Optional[RuleMemory] = None
         self.last_timing = {}                     # host-clock seconds of the last generate call, by phase
 
     @classmethod
@@ -95,40 +96,56 @@ class Engine:
             max_tokens = max(max_tokens, c.n_pages * PAGE)
             max_context = max(max_context, self.stepper.max_context)
             max_seqs = max(max_seqs, c.max_seqs)
-        self.cache = self.stepper = None
+        self.cache = self.stepper = self._memory = None
         self._graphs.clear()
         self.cache = Cache(self.model.cache_needs(), max_tokens, max_seqs, self.dtype, self.device)
         self.model.prepare(max_context)
         self.stepper = Stepper(self.model, self.cache, max_context)
 
+    def rule_memory(self) -> RuleMemory:
+        """What the sequences of the cache's slots have seen, for sampling under rules."""
+        if self._memory is None:
+            self._memory = RuleMemory(self.cache.max_seqs, self.model.plan.vocab_size, self.device)
+        return self._memory
+
     # ------------------------------------------------------------------ generation
     @torch.inference_mode()
     def generate(self, prompt: Union[Sequence[int], Sequence[Sequence[int]]], max_tokens: Union[int, Sequence[int]] = 64,
                  temperature: float = 0.7, top_k: int = 0, top_p: float = 0.9, use_graph: bool = True,
-                 seed: int = 0, stop_token_ids: Optional[Iterable[int]] = None):
+                 seed: int = 0, stop_token_ids: Optional[Iterable[int]] = None, n: int = 1, repetition_penalty: float = 1.0,
+                 presence_penalty: float = 0.0, frequency_penalty: float = 0.0, logit_bias=(), grammar: Optional[TokenAutomaton] = None):
         """Generated token ids: a list for one prompt (a list of ints), a list of lists for a
         batch of prompts.  ``stop_token_ids`` defaults to the configuration's eos ids; a stop
-        token ends its sequence and is not returned."""
+        token ends its sequence and is not returned.  ``n``: answers to each prompt, each with a stream of draws of its own; a prompt's answers then
+        stand in a list in its place.  The prompt is run once and its cache read once for all of them where that pays.
+        ``repetition_penalty``, ``presence_penalty``, ``frequency_penalty``, ``logit_bias`` (a dict or pairs of token and value) and ``grammar``: rules on what
+        may be chosen (``SamplingParams``)."""
         single = len(prompt) > 0 and isinstance(prompt[0], int) or len(prompt) == 0
         prompts = [list(prompt)] if single else [list(p) for p in prompt]
-        requests = self.generate_requests(prompts, max_tokens, SamplingParams(temperature, top_k, top_p, seed),
-                                          use_graph, stop_token_ids)
+        params = SamplingParams(temperature, top_k, top_p, seed, repetition_penalty, presence_penalty, frequency_penalty, logit_bias, grammar)
+        requests = self.generate_requests(prompts, max_tokens, params, use_graph, stop_token_ids, n)
         outs = [r.output for r in requests]
+        if n > 1:
+            outs = [outs[i: i + n] for i in range(0, len(outs), n)]
         return outs[0] if single else outs
 
     def generate_requests(self, prompts, max_tokens, params: SamplingParams, use_graph: bool = True,
-                          stop_token_ids: Optional[Iterable[int]] = None) -> List[Request]:
+                          stop_token_ids: Optional[Iterable[int]] = None, answers: int = 1) -> List[Request]:
+        """One request per prompt, or ``answers`` of them, one after the other."""
+        if answers < 1:
+            raise ValueError("a prompt needs at least one answer")
+        params.check_vocab(self.model.plan.vocab_size)
         stop = tuple(self.model.plan.stop_token_ids) if stop_token_ids is None else tuple(stop_token_ids)
         mnt = [max_tokens] * len(prompts) if isinstance(max_tokens, int) else list(max_tokens)
         probe = [Request(i, list(p), m) for i, (p, m) in enumerate(zip(prompts, mnt)) if len(p)]
         if probe:
-            need = [held_tokens(r) for r in probe]
+            need = [held_tokens(r) for r in probe for _ in range(answers)]
             budget = self._want_tokens or sum(sorted(need, reverse=True)[:self.max_batch])
             self.ensure_cache(max(budget, max(need)), max(len(r.prompt) + max(r.max_new_tokens - 1, 0) for r in probe))
         self.last_timing = {"prefill_s": 0.0, "decode_s": 0.0, "decode_steps": 0, "h2d_bytes": 0}
         backend = EngineBackend(self, Sampler(params), use_graph)
         budget = self.cache.n_pages * PAGE if self.cache is not None else PAGE
-        requests = run_generation(backend, prompts, mnt, stop, self.max_batch, budget)
+        requests = run_generation(backend, prompts, mnt, stop, self.max_batch, budget, answers)
         kernels.check_status(self.device)
         return requests
 
@@ -150,15 +167,52 @@ class EngineBackend:
     def _int32(self, values) -> torch.Tensor:
         return torch.tensor(list(values), dtype=torch.int32).to(self.e.device, non_blocking=True)
 
+    def _rules(self, slots):
+        """The rules of a step's rows (None without any)."""
+        return self.e.rule_memory().rules(self.sampler.params, self._int32(slots)) if self.sampler.params.ruled else None
+
     def prefill(self, slots, prompts, requests) -> List[int]:
-        """The prompts of a batch: in one step, or, where they have more tokens than ``Engine.prefill_tokens_per_step``,
+        """The prompts of a batch, and the first token of each."""
+        t0 = time.perf_counter()
+        logits = self._prompts(slots, prompts)
+        if self.sampler.params.ruled:
+            self.e.rule_memory().begin(self.sampler.params, slots, prompts)
+        chosen = self.sampler.choose(logits, self._int32(requests), self._int32([0] * len(slots)), rules=self._rules(slots)).tolist()
+        self.e.last_timing["prefill_s"] += time.perf_counter() - t0
+        return chosen
+
+    def prefill_answers(self, slots, prompts, requests):
+        """Several answers to a prompt: the prompt runs in its slot, the sequences of the other answers are forked from it, and each chooses its
+        first token from the prompt's logits."""
+        t0 = time.perf_counter()
+        logits = self._prompts(slots, prompts)
+        further = []
+        try:
+            for s, r in zip(slots, requests):
+                further.append(self.e.cache.fork(s, len(r) - 1))
+            if self.sampler.params.ruled:
+                self.e.rule_memory().begin(self.sampler.params, slots, prompts, further)
+            rows = [i for i, r in enumerate(requests) for _ in r]
+            everyone = [x for s, more in zip(slots, further) for x in [s] + more]
+            logits = logits[torch.tensor(rows, device=logits.device)]
+            chosen = self.sampler.choose(logits, self._int32(i for r in requests for i in r), self._int32([0] * len(rows)),
+                                         rules=self._rules(everyone)).tolist()
+        except Exception:
+            for more in further:
+                for s in more:
+                    self.e.cache.close(s)
+            raise
+        self.e.last_timing["prefill_s"] += time.perf_counter() - t0
+        return further, chosen
+
+    def _prompts(self, slots, prompts) -> torch.Tensor:
+        """The logits behind the prompts of a batch: in one step, or, where they have more tokens than ``Engine.prefill_tokens_per_step``,
         in several (the activations of a step grow with its tokens: the cache may hold a batch whose prompts in one
         step would not fit beside it).  A prompt's later pieces start inside its sequence; the logits that choose a
         request's first token are those of its last piece's last token."""
-        t0 = time.perf_counter()
         budget = self.e.prefill_tokens_per_step
         if sum(len(p) for p in prompts) <= budget:
-            logits = self.e.stepper.step(slots, prompts, use_graph=self.use_graph)
+            return self.e.stepper.step(slots, prompts, use_graph=self.use_graph)
         else:
             rows = [None] * len(slots)
             for pieces in cut_prompts([len(p) for p in prompts], budget):
@@ -167,23 +221,22 @@ class EngineBackend:
                                           [[n - 1] if end else [] for (_, _, n), end in zip(pieces, ends)])
                 for k, r in enumerate(r for (r, _, _), end in zip(pieces, ends) if end):
                     rows[r] = out[k]
-            logits = torch.stack(rows)
-        chosen = self.sampler.choose(logits, self._int32(requests), self._int32([0] * len(slots))).tolist()
-        self.e.last_timing["prefill_s"] += time.perf_counter() - t0
-        return chosen
+            return torch.stack(rows)
 
     MAX_GRAPHS = 24      # captured decode steps an engine keeps (each holds its buffers); the least recently used goes
 
-    def _graph(self, rows: int) -> GraphedDecode:
-        """The captured step for ``rows`` rows: one per bucket of rows and kind of sampling.  Temperature,
-        top-k, top-p and seed are numbers the graph reads at run time, so calls that vary them share it."""
-        key = (bucket_rows(rows), self.sampler.kind(self.e.model.plan.vocab_size))
+    def _graph(self, slots) -> GraphedDecode:
+        """The captured step for so many rows: one per bucket of rows, kind of sampling and of rules, and whether shared pages are read once.
+        Temperature, top-k, top-p, seed, penalties and biases are numbers the graph reads at run time, so calls that vary them share it."""
+        shared = self.e.stepper.sharing_pays(slots)
+        key = (bucket_rows(len(slots)), self.sampler.kind(self.e.model.plan.vocab_size), self.sampler.rule_kind(), shared)
         graphs = self.e._graphs
         g = graphs.pop(key, None)
         if g is None:
             if self.e._token_loop is None:
                 self.e._token_loop = TokenLoop(self.e.device)
-            g = GraphedDecode(self.e.stepper, self.sampler, key[0], self.e._token_loop)
+            g = GraphedDecode(self.e.stepper, self.sampler, key[0], self.e._token_loop, shared,
+                              self.e.rule_memory() if self.sampler.params.ruled else None)
             while len(graphs) >= self.MAX_GRAPHS:
                 graphs.pop(next(iter(graphs)))
         graphs[key] = g                                  # most recently used last
@@ -194,10 +247,10 @@ class EngineBackend:
         step's description is copied from pinned memory, the result is read back."""
         t0, sent = time.perf_counter(), self.e.stepper.h2d_bytes
         if self.use_graph:
-            chosen = self._graph(len(slots)).launch(slots, tokens, requests, steps, sampler=self.sampler).tokens()
+            chosen = self._graph(slots).launch(slots, tokens, requests, steps, sampler=self.sampler).tokens()
         else:
             logits = self.e.stepper.step(slots, [[t] for t in tokens])
-            chosen = self.sampler.choose(logits, self._int32(requests), self._int32(steps)).tolist()
+            chosen = self.sampler.choose(logits, self._int32(requests), self._int32(steps), rules=self._rules(slots)).tolist()
         t = self.e.last_timing
         t["decode_s"] += time.perf_counter() - t0
         t["decode_steps"] += 1
@@ -216,7 +269,7 @@ class EngineBackend:
         now, sent = time.perf_counter(), self.e.stepper.h2d_bytes
         if self._mark is None:
             self._mark = now
-        flight = self._graph(len(slots)).launch(slots, [0 if s >= 0 else t for t, s in zip(tokens, sources)],
+        flight = self._graph(slots).launch(slots, [0 if s >= 0 else t for t, s in zip(tokens, sources)],
                                                 requests, steps, sources, sampler=self.sampler)
         t = self.e.last_timing
         t["decode_steps"] += 1

@@ -181,26 +181,58 @@ def bucket_rows(rows: int) -> int:
     return b
 
 
+# Page tables of a step that the host would have to write and send, in entries of its rows' sequences, from which on the device keeps them and lays the
+# step out itself (``ResidentTables``).
+RESIDENT_ENTRIES = 2048
+
+
 class GraphedDecode:
     """``B`` is the number of rows of the captured step; a launch may bring fewer.  ``sampler`` says how tokens
     are chosen (greedy, or which cuts a draw makes: that fixes the kernels of the graph); its temperature,
     top-k, top-p and seed are read from the device buffer at run time, so one graph serves every setting
-    of the same kind (``launch(..., sampler=)``)."""
+    of the same kind (``launch(..., sampler=)``).  ``shared``: rows of a family of forked sequences read its pages once for
+    all.  A sampler with rules needs ``memory`` (``RuleMemory``), what its sequences have seen; their numbers are read from the buffer too."""
 
-    def __init__(self, stepper: Stepper, sampler, B: int, loop: Optional[TokenLoop] = None):
-        self.stepper, self.sampler, self.B = stepper, sampler, B
+    def __init__(self, stepper: Stepper, sampler, B: int, loop: Optional[TokenLoop] = None, shared: bool = False, memory=None):
+        self.stepper, self.sampler, self.B, self.shared = stepper, sampler, B, shared
         cache = stepper.cache
         self.loop = loop or TokenLoop(stepper.device)
         if B > TokenLoop.ROWS:
             raise ValueError(f"a decode step of {B} rows is more than the {TokenLoop.ROWS} the token buffer holds")
         self.widths = [pages_for(stepper.max_context)] * len(cache.groups)
-        self.layout = StepLayout(B, B, B, self.widths)
-        n = self.layout.total
-        self.extra = n                                   # request ids [B], step counters [B], token sources [B], settings [6]
+        # request ids [B], step counters [B], token sources [B], settings [6]; then the rules' penalties [B, 3], places of the biases [B, 2], their
+        # tokens and values; then what the device needs to lay out the step: positions, entries known and new pages a group, each [B]
         self.pad = (B + 3) & ~3
-        self.settings_at = n + 3 * self.pad              # a multiple of 4 words: the 64-bit seed is aligned
-        self.dev = torch.zeros(self.settings_at + 8, dtype=torch.int32, device=stepper.device)
-        self.host = np.zeros(self.dev.numel(), dtype=np.int32)
+        penalized, bias_room, grammar = sampler.rule_kind()
+        at = 3 * self.pad + 8                            # (a multiple of 4 words: the 64-bit seed is aligned)
+        self.rule_at = at
+        at += 5 * self.pad + 2 * bias_room
+        self.place_at = at
+        at += (1 + 2 * len(cache.groups)) * self.pad
+        self.layout = StepLayout(B, B, B, self.widths, shared=shared, room=at)
+        n = self.layout.total
+        self.extra = self.layout.extra
+        self.settings_at, self.rule_at, self.place_at = self.extra + 3 * self.pad, self.extra + self.rule_at, self.extra + self.place_at
+        self.dev = torch.zeros(n, dtype=torch.int32, device=stepper.device)
+        self.host = np.zeros(n, dtype=np.int32)
+        self.places = torch.zeros(B, dtype=torch.int32, device=stepper.device)
+        self.rules = None
+        if penalized or bias_room or grammar is not None:
+            from ..sampling.rules import StepRules
+            if memory is None:
+                raise ValueError("a sampler with rules needs the memory of its sequences")
+            lay, r = self.layout, self.rule_at
+            self.rules = StepRules(memory, self.dev[lay.slots: lay.slots + B], grammar=grammar)
+            if penalized:
+                memory.history                           # (made now: not while a graph is being captured)
+                self.rules.penalties = self.dev[r: r + 3 * B].view(torch.float32).view(B, 3)
+            if bias_room:
+                self.rules.bias_range = self.dev[r + 3 * self.pad: r + 3 * self.pad + 2 * B].view(B, 2)
+                self.rules.bias_ids = self.dev[r + 5 * self.pad: r + 5 * self.pad + bias_room]
+                self.rules.bias_values = self.dev[r + 5 * self.pad + bias_room: r + 5 * self.pad + 2 * bias_room].view(torch.float32)
+            if grammar is not None:
+                grammar.on(stepper.device)
+        self.bias_room = bias_room
         self.tokens_out = self.loop.chosen[:B]
         self.logits: Optional[torch.Tensor] = None
         self.graph: Optional[torch.cuda.CUDAGraph] = None
@@ -213,10 +245,21 @@ class GraphedDecode:
         lay, B, pad, n = self.layout, self.B, self.pad, len(slots)
         if n > B:
             raise ValueError(f"a step of {n} rows does not fit a graph of {B}")
+        if (sampler or self.sampler).kind(self.stepper.vocab) != self.sampler.kind(self.stepper.vocab) or \
+                (sampler or self.sampler).rule_kind() != self.sampler.rule_kind():
+            raise ValueError("this graph was captured for another kind of sampling")
         idle = [self.stepper.cache.idle_slot] * (B - n)
-        _, fresh, starts = self.stepper.describe(list(slots) + idle, [1] * B, None, [[t] for t in tokens] + [[0]] * (B - n),
-                                                 self.widths)
-        self.host[:lay.total] = fresh
+        st, every = self.stepper, list(slots) + idle
+        entries = sum(pages_for(st.cache.length(s) + 1) for s in slots) * len(self.widths)
+        tables = st.resident_tables() if entries >= RESIDENT_ENTRIES else None
+        self._new_pages = None
+        if tables is None:
+            _, fresh, starts = st.describe(every, [1] * B, None, [[t] for t in tokens] + [[0]] * (B - n), self.widths, shared=self.shared, room=lay.room)
+            self.host[:lay.total] = fresh
+            self.used = lay.total
+        else:
+            starts = st.describe_tokens(every, list(tokens) + [0] * (B - n), lay, self.host)
+            self.used = lay.tables[0]
         self.host[self.extra: self.extra + B] = 0
         self.host[self.extra: self.extra + n] = np.asarray(requests, dtype=np.int32)
         self.host[self.extra + pad: self.extra + pad + B] = 0
@@ -225,11 +268,41 @@ class GraphedDecode:
         if sources is not None:
             self.host[self.extra + 2 * pad: self.extra + 2 * pad + n] = np.asarray(sources, dtype=np.int32)
         p = (sampler or self.sampler).params
-        if (sampler or self.sampler).kind(self.stepper.vocab) != self.sampler.kind(self.stepper.vocab):
-            raise ValueError("this graph was captured for another kind of sampling")
+        if self.rules is not None:
+            r = self.rule_at
+            if self.rules.penalties is not None:
+                self.host[r: r + 3 * B].view(np.float32)[:] = np.tile(np.asarray(p.penalties, dtype=np.float32), B)
+            if self.bias_room:
+                many = len(p.logit_bias)
+                self.host[r + 3 * pad: r + 3 * pad + 2 * B] = np.tile(np.asarray([0, many], dtype=np.int32), B)
+                ids = r + 5 * pad
+                self.host[ids: ids + many] = [t for t, _ in p.logit_bias]
+                self.host[ids + self.bias_room: ids + self.bias_room + many].view(np.float32)[:] = [v for _, v in p.logit_bias]
         self.host[self.settings_at: self.settings_at + 6] = kernels.sample_settings_words(
             p.temperature if p.temperature > 0 else 1.0, p.top_k, p.top_p, p.seed)
-        self._starts, self._slots = starts, list(slots) + idle
+        if tables is not None:                           # (last: from here on the device is taken to know these pages)
+            at = self.place_at
+            self.host[at: at + B] = starts
+            self._new_pages = []
+            for g in range(len(self.widths)):
+                at = self.place_at + (1 + 2 * g) * pad
+                held, pages = tables.fresh(g, every)
+                self.host[at: at + B] = held
+                if len(pages) <= pad:                    # (more only when sequences are new here: those go by a copy of their own)
+                    self.host[at + pad: at + pad + len(pages)] = pages
+                self._new_pages.append(pages)
+        self._starts, self._slots = starts, every
+
+    def _lay_out(self) -> None:
+        """Positions, rows and page tables of the step, worked out on the device."""
+        st, lay, B, pad = self.stepper, self.layout, self.B, self.pad
+        dev, tables = self.dev, st.resident_tables()
+        part = lambda at, n: dev[at: at + n]             # noqa: E731
+        for g, pages in enumerate(self._new_pages):
+            at = self.place_at + (1 + 2 * g) * pad
+            fresh = part(at + pad, len(pages)) if len(pages) <= pad else st.upload(np.asarray(pages, dtype=np.int32))
+            tables.lay_out(g, part(lay.slots, B), part(self.place_at, B), part(lay.lens, B), part(at, B), fresh, part(lay.pos, B), part(lay.row, B),
+                           part(lay.first, B + 1), self.places, part(lay.tables[g], B * lay.widths[g]).view(B, lay.widths[g]))
 
     def _forward(self) -> None:
         lay, B, pad = self.layout, self.B, self.pad
@@ -242,7 +315,7 @@ class GraphedDecode:
         self.logits = self.stepper.model.forward(ids, ctx, self.dev[lay.want: lay.want + B])
         self.sampler.choose(self.logits, self.dev[self.extra: self.extra + B],
                             self.dev[self.extra + pad: self.extra + pad + B], self.tokens_out,
-                            settings=self.dev[self.settings_at: self.settings_at + 6])
+                            settings=self.dev[self.settings_at: self.settings_at + 6], rules=self.rules)
 
     def _capture(self) -> None:
         # The warm-up runs and the capture write the shared token buffer; what the step before chose
@@ -250,7 +323,9 @@ class GraphedDecode:
         # rewritten with the same numbers by every run, but per-sequence state (a mixer's running sums) would
         # be advanced once per run: it is put back after the warm-up, so that only the replay counts.
         keep = self.loop.chosen.clone()
+        # So would what the rules remember.
         state = self.stepper.cache.snapshot_state()
+        seen = self.rules.memory.snapshot(self._slots) if self.rules is not None else None
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
@@ -258,6 +333,8 @@ class GraphedDecode:
                 self.loop.chosen.copy_(keep)
                 self._forward()
             self.stepper.cache.restore_state(state)
+            if seen is not None:
+                self.rules.memory.restore(seen)
         torch.cuda.current_stream().wait_stream(side)
         self.loop.chosen.copy_(keep)
         graph = torch.cuda.CUDAGraph()
@@ -275,7 +352,9 @@ class GraphedDecode:
         launched before this one chose (``tokens[j]`` is then any valid id).  ``sampler``: the settings of
         this step's draws (of the kind the graph was captured for); default: the sampler of the capture."""
         self._fill(slots, tokens, requests, steps, sources, sampler)
-        self.stepper.upload(self.host, self.dev)
+        self.stepper.upload(self.host[:self.used], self.dev)
+        if self._new_pages is not None:
+            self._lay_out()
         if self.graph is None and not self.failed:
             stream = torch.cuda.current_stream()
             try:

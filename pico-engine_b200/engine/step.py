@@ -39,6 +39,8 @@ class StepLayout:
     W: int
     widths: List[int]
     n_tiles: tuple = (0, 0)          # attention runs of at most 64 and of at most 128 tokens (0, 0: every row brings one token)
+    shared: bool = False             # whether the rows that share pages are named (``kernels.shared_groups``)
+    room: int = 0                    # words in front of the page tables that a captured step uses for itself
     ids: int = 0
     pos: int = 0
     row: int = 0
@@ -48,6 +50,8 @@ class StepLayout:
     want: int = 0
     tiles: Optional[List[int]] = None
     tables: Optional[List[int]] = None
+    groups: int = 0
+    extra: int = 0
     total: int = 0
 
     def __post_init__(self):
@@ -62,6 +66,10 @@ class StepLayout:
         self.tiles = []
         for n in self.n_tiles:
             self.tiles.append(o); o += 4 * n
+        self.groups = o
+        if self.shared:
+            o += 4 * self.B
+        self.extra = o; o += _pad4(self.room)
         self.tables = []
         for w in self.widths:
             self.tables.append(o); o += _pad4(self.B * w)
@@ -80,6 +88,37 @@ class Stepper:
         self.h2d_bytes = 0                        # bytes of step descriptions copied to the device so far
         self._prompt_graphs: dict = {}            # (rows, tokens) -> GraphedPrompt, the most recently used last
         self._prompt_pool = None
+        self._resident = None
+
+    # ------------------------------------------------------------------ rows that share pages
+    def families(self, slots: Sequence[int]):
+        """``members`` of ``kernels.shared_group_rows`` for a step of one token a row: consecutive rows of a family of forked
+        sequences share its pages; the others are on their own."""
+        cache, out, at = self.cache, [], 0
+        while at < len(slots):
+            family = cache.prefix.get(slots[at])
+            n = 1
+            while family is not None and at + n < len(slots) and cache.prefix.get(slots[at + n]) == family:
+                n += 1
+            if n == 1 or family[1] == 0:
+                out.extend([(1, 0, 0)] * n)
+            else:
+                starts = [cache.length(s) for s in slots[at:at + n]]
+                out.append((n, family[1], starts.index(min(starts))))
+            at += n
+        return out
+
+    def sharing_pays(self, slots: Sequence[int]) -> bool:
+        """Whether a step of one token for each of these sequences should read the pages that some of them share once for all."""
+        members = self.families(slots) if self.cache.prefix else ()
+        if not any(n > 1 for n, _, _ in members) or len(slots) > kernels.SHARED_MAX_ROWS or self.cache.dtype != torch.bfloat16:
+            return False
+        most = 0                                 # of a layer: the bytes of shared keys and values that rows after the first do not read again
+        for g in self.cache.groups:
+            heads, dim = g.need.value_shape
+            a_position = 2 * (g.need.n_kv_heads * g.need.head_dim + heads * dim)
+            most = max(most, sum((n - 1) * min(shared, g.need.window or shared) * a_position for n, shared, _ in members))
+        return kernels.sharing_pays(most)
 
     # ------------------------------------------------------------------ building a step
     def _stage(self, host: np.ndarray):
@@ -97,13 +136,14 @@ class Stepper:
 
     def describe(self, slots: Sequence[int], lens: Sequence[int], want: Optional[Sequence[Sequence[int]]],
                  token_ids: Optional[Sequence[Sequence[int]]], widths: Optional[List[int]] = None,
-                 n_tiles: Optional[tuple] = None):
+                 n_tiles: Optional[tuple] = None, shared: bool = False, room: int = 0):
         """Check the step, reserve its pages and lay its arrays out on the host.
 
         Returns ``(layout, host int32 array, starts)``.  ``want[b]`` are places among row b's
         tokens of this step; None asks for each row's last token.  ``n_tiles``: how many attention runs
         (of at most 64 and at most 128 tokens) the layout holds, for a step of fixed sizes; where the
         rows make fewer, the last row's first token is listed again (the same result written twice).
+        ``shared``: name the rows that share pages (a step of one token a row).
         """
         cache = self.cache
         B = len(slots)
@@ -145,7 +185,9 @@ class Stepper:
                     if len(rows) > n:
                         raise StepError(f"the step has {len(rows)} attention runs, its layout holds {n}")
                     rows.extend([filler] * (n - len(rows)))
-        lay = StepLayout(T, B, W, widths, tuple(len(r) for r in tile_rows))
+        if shared and any(n != 1 for n in lens):
+            raise StepError("rows read shared pages together in steps of one token a row")
+        lay = StepLayout(T, B, W, widths, tuple(len(r) for r in tile_rows), shared, room)
         host = np.zeros(lay.total, dtype=np.int32)
         for off, rows in zip(lay.tiles, tile_rows):
             if rows:
@@ -172,9 +214,43 @@ class Stepper:
                     raise StepError(f"row {b}: wanted place {p} is none of its {lens[b]} tokens")
                 host[w_at] = cu[b] + p
                 w_at += 1
+        if shared:
+            host[lay.groups: lay.groups + 4 * B] = np.asarray(kernels.shared_group_rows(self.families(slots)), dtype=np.int32).reshape(-1)
         for g, off in enumerate(lay.tables):
             host[off: off + B * widths[g]] = cache.page_table(g, slots, widths[g]).reshape(-1)
         return lay, host, starts
+
+    def resident_tables(self):
+        """The page tables on the device, or None where the cache's are not kept there."""
+        from .tables import ResidentTables
+        if self._resident is None and ResidentTables.takes(self.cache):
+            self._resident = ResidentTables(self.cache, self.max_context)
+        return self._resident
+
+    def describe_tokens(self, slots: Sequence[int], tokens: Sequence[int], lay: StepLayout, host: np.ndarray) -> List[int]:
+        """``describe`` for a step of one token a row whose positions, rows and page tables the device works out itself: the checks, the reserved pages,
+        and in ``host`` the token ids, slots, lengths, wanted rows and shared pages.  Returns the positions."""
+        cache, B = self.cache, len(slots)
+        live = [s for s in slots if s != cache.idle_slot]
+        if len(set(live)) != len(live):
+            raise StepError("a sequence appears twice in one step")
+        starts = [cache.length(s) for s in slots]
+        if max(starts) + 1 > self.max_context:
+            raise StepError(f"row {starts.index(max(starts))} would reach {max(starts) + 1} tokens; the engine was set up for sequences of at most {self.max_context}")
+        ids = np.asarray(tokens, dtype=np.int64)
+        if ids.shape != (B,):
+            raise StepError(f"{ids.shape} tokens given for {B} rows")
+        if ids.min() < 0 or ids.max() >= self.vocab:
+            raise StepError(f"row {int(((ids < 0) | (ids >= self.vocab)).argmax())} has a token outside the vocabulary of {self.vocab}")
+        for s in live:
+            cache.reserve(s, 1)
+        host[lay.ids: lay.ids + B] = ids
+        host[lay.slots: lay.slots + B] = slots
+        host[lay.lens: lay.lens + B] = 1
+        host[lay.want: lay.want + B] = np.arange(B, dtype=np.int32)
+        if lay.shared:
+            host[lay.groups: lay.groups + 4 * B] = np.asarray(kernels.shared_group_rows(self.families(slots)), dtype=np.int32).reshape(-1)
+        return starts
 
     def context(self, lay: StepLayout, dev: torch.Tensor, lens: List[int], starts: List[int],
                 slot_ids: Sequence[int] = ()) -> StepContext:
@@ -182,6 +258,8 @@ class Stepper:
                   for g, off in enumerate(lay.tables)}
         scratch = {name: dev[off: off + 4 * n].view(n, 4)
                    for name, off, n in zip(("prefill_tiles", "prefill_tiles_128"), lay.tiles, lay.n_tiles) if n}
+        if lay.shared:
+            scratch["shared_groups"] = dev[lay.groups: lay.groups + 4 * lay.B].view(lay.B, 4)
         return StepContext(scratch=scratch,
             T=lay.T, B=lay.B, dtype=self.model.dtype, device=self.device,
             tok_pos=dev[lay.pos: lay.pos + lay.T], tok_row=dev[lay.row: lay.row + lay.T],
@@ -239,10 +317,10 @@ class Stepper:
                 return g.launch(slots, token_ids)
         if device_tokens is not None:
             lens = [1] * len(slots)
-            lay, host, starts = self.describe(slots, lens, want, None)
+            lay, host, starts = self.describe(slots, lens, want, None, shared=self.sharing_pays(slots))
         else:
             lens = [len(t) for t in token_ids]
-            lay, host, starts = self.describe(slots, lens, want, token_ids)
+            lay, host, starts = self.describe(slots, lens, want, token_ids, shared=all(n == 1 for n in lens) and self.sharing_pays(slots))
         dev = self.upload(host)
         ctx = self.context(lay, dev, lens, starts, slots)
         ids = device_tokens if device_tokens is not None else dev[lay.ids: lay.ids + lay.T]

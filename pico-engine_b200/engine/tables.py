@@ -1,0 +1,51 @@
+"""The cache's page tables on the device, brought up to date by the pages that a step takes."""
+from __future__ import annotations
+
+from typing import Dict, List, Sequence, Tuple
+
+import numpy as np
+import torch
+
+from ..cache import Cache, pages_for
+from ..ops import kernels
+
+
+class ResidentTables:
+    """A page table row for every sequence slot in every group of the cache.  A step of one token a row sends four numbers a row and the pages that
+    are not there yet, and ``kernels.step_tables`` lays the step out; without them the host writes and sends rows x pages of the longest sequence, every step.
+    Rows are known by the sequence that holds the slot (``Cache.births``), so a slot that is closed and opened again starts anew."""
+
+    def __init__(self, cache: Cache, max_context: int):
+        self.cache, self.width = cache, pages_for(max_context)
+        self.tables = [torch.full((cache.max_seqs + 1, self.width), -1, dtype=torch.int32, device=cache.device) for _ in cache.groups]
+        for t in self.tables:
+            t[cache.idle_slot, 0] = cache.idle_page
+        self.known: List[Dict[int, Tuple[int, int]]] = [{} for _ in cache.groups]       # slot -> (birth, entries on the device)
+
+    @staticmethod
+    def takes(cache: Cache) -> bool:
+        """Whether tables only ever grow: a group with a window takes entries back, which the rows on the device do not learn."""
+        return len(cache.groups) > 0 and all(g.need.window is None for g in cache.groups)
+
+    def fresh(self, group: int, slots: Sequence[int]):
+        """(entries on the device of each row, the pages behind them in the rows' order) of a step whose pages have been reserved; they count as known
+        from now on."""
+        cache, table, known = self.cache, self.cache.groups[group].table, self.known[group]
+        held, pages = np.empty(len(slots), dtype=np.int32), []
+        for b, s in enumerate(slots):
+            if s == cache.idle_slot:
+                held[b] = 1
+                continue
+            birth, n = known.get(s, (0, 0))
+            row = table[s]
+            if birth != cache.births[s]:
+                n = 0
+            held[b] = n
+            if n < len(row):
+                pages.extend(row[n:])
+            known[s] = (cache.births[s], len(row))
+        return held, pages
+
+    def lay_out(self, group: int, slots: torch.Tensor, starts: torch.Tensor, lens: torch.Tensor, held: torch.Tensor, pages: torch.Tensor, tok_pos: torch.Tensor,
+                tok_row: torch.Tensor, row_first: torch.Tensor, places: torch.Tensor, table: torch.Tensor) -> None:
+        kernels.step_tables(slots, starts, lens, held, pages, self.tables[group], tok_pos, tok_row, row_first, places, table)
