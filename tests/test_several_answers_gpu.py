@@ -223,13 +223,14 @@ def test_tables_on_the_device_change_no_token(models, monkeypatch, name, dtype):
     monkeypatch.setattr(graph_module.GraphedDecode, "launch", launch)
     old, eng.max_batch = eng.max_batch, 4
     try:
+        monkeypatch.setattr(graph_module, "RESIDENT_ROWS", 1000)
         want = [eng.generate(prompts, budgets, n=n, **kw) for n in (1, 3)]
         assert not seen
-        monkeypatch.setattr(graph_module, "RESIDENT_ENTRIES", 1)
+        monkeypatch.setattr(graph_module, "RESIDENT_ROWS", 1)
         assert [eng.generate(prompts, budgets, n=n, **kw) for n in (1, 3)] == want
         rows = len(seen)
         assert rows > 20 and sum(seen) > 20 and 0 in seen
-        monkeypatch.setattr(graph_module, "RESIDENT_ENTRIES", 3)                # some steps this way, some that
+        monkeypatch.setattr(graph_module, "RESIDENT_ROWS", 3)                # some steps this way, some that
         assert [eng.generate(prompts, budgets, n=n, **kw) for n in (1, 3)] == want
         assert rows < len(seen) < 2 * rows
     finally:
@@ -246,7 +247,7 @@ def test_windowed_caches_keep_their_tables_on_the_host(models):
 def test_everything_together(models, together, monkeypatch):
     """Answers that share pages, under penalties, biases and a grammar, with their tables on the device: what is chosen is (nearly) the best of the plain
     logits under the rules, and allowed.  The logits' tolerance of 4e-2 grows by the repetition penalty of 1.3 at most (it multiplies negative ones)."""
-    monkeypatch.setattr(graph_module, "RESIDENT_ENTRIES", 1)
+    monkeypatch.setattr(graph_module, "RESIDENT_ROWS", 1)
     cfg = dict(TINY["C"], use_sliding_window=False)
     from pico_engine.engine.engine import Engine
     import tempfile
