@@ -4,7 +4,8 @@ Options are pico-engine's (src/pico_engine/__main__.py:23-39) with their names, 
 meanings: ``--prompt``, ``--max-tokens 64``, ``--temperature 0.7`` (0 is greedy), ``--top-p 0.9``,
 ``--top-k 0``, ``--no-graph``.  There is no tokenizer in this library, so ``--prompt`` takes token
 ids ("5,17,3"; repeat the option for a batch) and the output is token ids; ``--seed``,
-``--dtype`` and ``--stop-token-ids`` are additions.  Without a model folder, ``--random-config NAME``
+``--dtype``, ``--stop-token-ids``, ``--n`` and the rules on what may be said (``--repetition-penalty``, ``--presence-penalty``, ``--frequency-penalty``,
+``--logit-bias``) are additions.  Without a model folder, ``--random-config NAME``
 draws the weights of a named shape from ``--seed`` and ``--random-prompt LEN[,LEN...]`` draws
 prompts, so that random weights become tokens in one line.  ``--n-gpu-layers`` (offload of
 another architecture) is not taken.
@@ -22,6 +23,11 @@ def parse_ids(text: str) -> list[int]:
     if text.startswith("["):
         return [int(t) for t in json.loads(text)]
     return [int(t) for t in text.replace(",", " ").split()]
+
+
+def parse_bias(text: str) -> list[tuple[int, float]]:
+    """"17:-2.5,4:1": pairs of token id and value."""
+    return [(int(t), float(v)) for t, _, v in (pair.partition(":") for pair in text.replace(",", " ").split())]
 
 
 def random_prompts(lengths, vocab: int, seed: int) -> list[list[int]]:
@@ -49,6 +55,11 @@ def main(argv=None) -> None:
     p.add_argument("--top-p", type=float, default=0.9)
     p.add_argument("--top-k", type=int, default=0)
     p.add_argument("--seed", type=int, default=0, help="names the stream of random draws")
+    p.add_argument("--n", type=int, default=1, metavar="ANSWERS", help="answers to every prompt, which is run and kept once for all of them")
+    p.add_argument("--repetition-penalty", type=float, default=1.0, help="divides (multiplies, below 0) logits of tokens seen so far, the prompt's included")
+    p.add_argument("--presence-penalty", type=float, default=0.0, help="taken off logits of tokens in the answer so far")
+    p.add_argument("--frequency-penalty", type=float, default=0.0, help="the same times how often they are there")
+    p.add_argument("--logit-bias", type=parse_bias, default=[], metavar="ID:VALUE[,ID:VALUE...]", help="added to logits")
     p.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
     p.add_argument("--no-graph", action="store_true", help="disable CUDA-graph decode and launch every kernel")
     args = p.parse_args(argv)
@@ -73,6 +84,8 @@ def main(argv=None) -> None:
         p.error("--layers goes with --random-config")
     elif not (args.model / "config.json").is_file():
         p.error(f"model folder has no config.json: {args.model}")
+    if args.n < 1:
+        p.error("--n must be at least 1")
     if args.max_tokens < 0:
         p.error("--max-tokens must be non-negative")
     prompts = [parse_ids(t) for t in (args.prompt or [])]
@@ -104,8 +117,11 @@ def main(argv=None) -> None:
     load_s = time.perf_counter() - t0
     t0 = time.perf_counter()
     outs = eng.generate(prompts, args.max_tokens, args.temperature, args.top_k, args.top_p,
-                        use_graph=not args.no_graph, seed=args.seed, stop_token_ids=stop)
+                        use_graph=not args.no_graph, seed=args.seed, stop_token_ids=stop, n=args.n, repetition_penalty=args.repetition_penalty,
+                        presence_penalty=args.presence_penalty, frequency_penalty=args.frequency_penalty, logit_bias=args.logit_bias)
     gen_s = time.perf_counter() - t0
+    if args.n > 1:                                       # a line an answer
+        prompts, outs = [q for q in prompts for _ in range(args.n)], [o for answers in outs for o in answers]
     n = sum(len(o) for o in outs)
     print(f"\n[engine] loaded in {load_s:.1f}s; generated {n} tokens in {gen_s:.2f}s ({n / max(gen_s, 1e-9):.1f} tok/s)")
     print("=" * 60)

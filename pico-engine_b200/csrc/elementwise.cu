@@ -90,7 +90,8 @@ __global__ void select_tokens_kernel(int* ids, const int* prev, const int* src, 
 
 extern "C" int pe_select_tokens(int* ids, const int* prev, const int* src, int n, void* stream) {
     if (n <= 0) return 0;
-    PE_TRY(pe_launch(select_tokens_kernel, (n + 127) / 128, 128, 0, (cudaStream_t)stream, ids, prev, src, n));
+    // An ordinary launch: what the launches before it wrote (a step's tables) is there for every kernel behind it, those that read ahead of their wait included.
+    select_tokens_kernel<<<(n + 127) / 128, 128, 0, (cudaStream_t)stream>>>(ids, prev, src, n);
     PE_LAUNCH_CHECK();
     return 0;
 }

@@ -181,9 +181,9 @@ def bucket_rows(rows: int) -> int:
     return b
 
 
-# Rows of a step from which on the page tables stay on the device and the device lays the step out (``ResidentTables``).  Wall time of a step of a two-layer
-# model with 14 heads of 64, tables from the host against on the device, us: 2 rows 117 / 122; 4 rows of 100 tokens 124 / 122, of 16,000 144 / 137; 8 rows of
-# 100 138 / 124, of 8,000 163 / 138; 64 rows of 500 465 / 187; 256 rows of 2,000 1,800 / 345; 512 rows of 4,000 4,030 / 675.
+# Rows of a captured step from which on the page tables stay on the device and the step lays itself out there (``ResidentTables``).  Wall time of a step of a
+# two-layer model with 14 heads of 64, tables from the host against on the device, us: 1 row 114 / 115; 2 rows of 100 tokens 118 / 118, of 16,000 134 / 129;
+# 4 rows of 100 123 / 118; 8 rows of 100 139 / 120, of 8,000 165 / 133; 64 rows of 500 440 / 183; 256 rows of 2,000 1,700 / 343; 512 rows of 4,000 3,790 / 670.
 RESIDENT_ROWS = 4
 
 
@@ -216,6 +216,7 @@ class GraphedDecode:
         self.settings_at, self.rule_at, self.place_at = self.extra + 3 * self.pad, self.extra + self.rule_at, self.extra + self.place_at
         self.dev = torch.zeros(n, dtype=torch.int32, device=stepper.device)
         self.host = np.zeros(n, dtype=np.int32)
+        self.tables = stepper.resident_tables() if B >= RESIDENT_ROWS else None
         self.places = torch.zeros(B, dtype=torch.int32, device=stepper.device)
         self.rules = None
         if penalized or bias_room or grammar is not None:
@@ -251,9 +252,7 @@ class GraphedDecode:
             raise ValueError("this graph was captured for another kind of sampling")
         idle = [self.stepper.cache.idle_slot] * (B - n)
         st, every = self.stepper, list(slots) + idle
-        tables = st.resident_tables() if n >= RESIDENT_ROWS else None
-        self._new_pages = None
-        if tables is None:
+        if self.tables is None:
             _, fresh, starts = st.describe(every, [1] * B, None, [[t] for t in tokens] + [[0]] * (B - n), self.widths, shared=self.shared, room=lay.room)
             self.host[:lay.total] = fresh
             self.used = lay.total
@@ -280,29 +279,27 @@ class GraphedDecode:
                 self.host[ids + self.bias_room: ids + self.bias_room + many].view(np.float32)[:] = [v for _, v in p.logit_bias]
         self.host[self.settings_at: self.settings_at + 6] = kernels.sample_settings_words(
             p.temperature if p.temperature > 0 else 1.0, p.top_k, p.top_p, p.seed)
-        if tables is not None:                           # (last: from here on the device is taken to know these pages)
+        self._many = []
+        if self.tables is not None:                      # (last: from here on the device is taken to know these pages)
             at = self.place_at
             self.host[at: at + B] = starts
-            self._new_pages = []
             for g in range(len(self.widths)):
                 at = self.place_at + (1 + 2 * g) * pad
-                held, pages = tables.fresh(g, every)
+                held, pages = self.tables.fresh(g, every)
+                if len(pages) > pad:                     # only when sequences are new here: those go by a launch of their own, before the step's
+                    self._many.append((g, np.concatenate([held, np.asarray(pages, dtype=np.int32)])))
+                    held = [1 if s == st.cache.idle_slot else len(st.cache.groups[g].table[s]) for s in every]
+                    pages = []
                 self.host[at: at + B] = held
-                if len(pages) <= pad:                    # (more only when sequences are new here: those go by a copy of their own)
-                    self.host[at + pad: at + pad + len(pages)] = pages
-                self._new_pages.append(pages)
+                self.host[at + pad: at + pad + len(pages)] = pages
         self._starts, self._slots = starts, every
 
-    def _lay_out(self) -> None:
-        """Positions, rows and page tables of the step, worked out on the device."""
-        st, lay, B, pad = self.stepper, self.layout, self.B, self.pad
-        dev, tables = self.dev, st.resident_tables()
-        part = lambda at, n: dev[at: at + n]             # noqa: E731
-        for g, pages in enumerate(self._new_pages):
-            at = self.place_at + (1 + 2 * g) * pad
-            fresh = part(at + pad, len(pages)) if len(pages) <= pad else st.upload(np.asarray(pages, dtype=np.int32))
-            tables.lay_out(g, part(lay.slots, B), part(self.place_at, B), part(lay.lens, B), part(at, B), fresh, part(lay.pos, B), part(lay.row, B),
-                           part(lay.first, B + 1), self.places, part(lay.tables[g], B * lay.widths[g]).view(B, lay.widths[g]))
+    def _lay_out(self, g: int, held: torch.Tensor, pages: torch.Tensor) -> None:
+        """Positions, rows and the page tables of group ``g``, worked out on the device."""
+        lay, B = self.layout, self.B
+        part = lambda at, n: self.dev[at: at + n]        # noqa: E731
+        kernels.step_tables(part(lay.slots, B), part(self.place_at, B), part(lay.lens, B), held, pages, self.tables.tables[g], part(lay.pos, B),
+                            part(lay.row, B), part(lay.first, B + 1), self.places, part(lay.tables[g], B * lay.widths[g]).view(B, lay.widths[g]))
 
     def _forward(self) -> None:
         lay, B, pad = self.layout, self.B, self.pad
@@ -310,6 +307,10 @@ class GraphedDecode:
         ctx.max_context = self.stepper.max_context       # launch shapes must not depend on the step
         ctx.starts = [self.stepper.max_context - 1] * B
         ids = self.dev[lay.ids: lay.ids + B]
+        if self.tables is not None:
+            for g in range(len(self.widths)):
+                at = self.place_at + (1 + 2 * g) * pad
+                self._lay_out(g, self.dev[at: at + B], self.dev[at + pad: at + 2 * pad])
         # rows whose token the host has not seen take it from the step before, on the device
         kernels.select_tokens(ids, self.loop.chosen, self.dev[self.extra + 2 * pad: self.extra + 2 * pad + B])
         self.logits = self.stepper.model.forward(ids, ctx, self.dev[lay.want: lay.want + B])
@@ -353,8 +354,9 @@ class GraphedDecode:
         this step's draws (of the kind the graph was captured for); default: the sampler of the capture."""
         self._fill(slots, tokens, requests, steps, sources, sampler)
         self.stepper.upload(self.host[:self.used], self.dev)
-        if self._new_pages is not None:
-            self._lay_out()
+        for g, numbers in self._many:
+            sent = self.stepper.upload(numbers)
+            self._lay_out(g, sent[:self.B], sent[self.B:])
         if self.graph is None and not self.failed:
             stream = torch.cuda.current_stream()
             try:

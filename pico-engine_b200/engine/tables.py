@@ -7,7 +7,6 @@ import numpy as np
 import torch
 
 from ..cache import Cache, pages_for
-from ..ops import kernels
 
 
 class ResidentTables:
@@ -45,7 +44,3 @@ class ResidentTables:
                 pages.extend(row[n:])
             known[s] = (cache.births[s], len(row))
         return held, pages
-
-    def lay_out(self, group: int, slots: torch.Tensor, starts: torch.Tensor, lens: torch.Tensor, held: torch.Tensor, pages: torch.Tensor, tok_pos: torch.Tensor,
-                tok_row: torch.Tensor, row_first: torch.Tensor, places: torch.Tensor, table: torch.Tensor) -> None:
-        kernels.step_tables(slots, starts, lens, held, pages, self.tables[group], tok_pos, tok_row, row_first, places, table)

@@ -211,8 +211,8 @@ def test_tables_on_the_device_change_no_token(models, monkeypatch, name, dtype):
 
     def launch(self, slots, *a, **k):
         flight = plainly(self, slots, *a, **k)
-        if self._new_pages is not None:
-            seen.append(sum(len(p) for p in self._new_pages))
+        if self.tables is not None:
+            seen.append(len(self._many))
             lay, cache = self.layout, eng.cache
             for g, w in enumerate(lay.widths):
                 table = self.dev[lay.tables[g]: lay.tables[g] + self.B * w].view(self.B, w).cpu().numpy()
@@ -224,17 +224,21 @@ def test_tables_on_the_device_change_no_token(models, monkeypatch, name, dtype):
     old, eng.max_batch = eng.max_batch, 4
     try:
         monkeypatch.setattr(graph_module, "RESIDENT_ROWS", 1000)
+        eng._graphs.clear()
         want = [eng.generate(prompts, budgets, n=n, **kw) for n in (1, 3)]
         assert not seen
         monkeypatch.setattr(graph_module, "RESIDENT_ROWS", 1)
+        eng._graphs.clear()
         assert [eng.generate(prompts, budgets, n=n, **kw) for n in (1, 3)] == want
         rows = len(seen)
-        assert rows > 20 and sum(seen) > 20 and 0 in seen
+        assert rows > 20 and sum(seen) > 0 and 0 in seen
         monkeypatch.setattr(graph_module, "RESIDENT_ROWS", 3)                # some steps this way, some that
+        eng._graphs.clear()
         assert [eng.generate(prompts, budgets, n=n, **kw) for n in (1, 3)] == want
         assert rows < len(seen) < 2 * rows
     finally:
         eng.max_batch = old
+        eng._graphs.clear()
     nothing_held(eng)
 
 
@@ -260,7 +264,7 @@ def test_everything_together(models, together, monkeypatch):
     prompts = prompts_of(cfg, [130, 20, 300, 64])
     greedy = eng.generate(prompts, 16, temperature=0, n=6, stop_token_ids=(), grammar=grammar, **params)
     drawn = eng.generate(prompts, 16, temperature=0.9, n=6, seed=4, stop_token_ids=(13,), grammar=grammar, **params)
-    assert len(together) > 0 and any(g.shared and g._new_pages is not None and g.graph is not None for g in eng._graphs.values())
+    assert len(together) > 0 and any(g.shared and g.tables is not None and g.graph is not None for g in eng._graphs.values())
     for p, answers in zip(prompts, greedy):
         for out in answers:
             assert grammar.walk(out) >= 0 and len(out) == 16
