@@ -170,3 +170,47 @@ def test_benchmark_command_line_writes_its_record(tmp_path):
         s = rec["decode"][b]["tokens_per_s"]
         assert s["n"] == 2 and 0 < s["p10"] <= s["median"] <= s["p90"]
     assert "decode batch 3" in r.stdout
+
+
+def test_rules_and_answers_on_the_command_line(tmp_path):
+    from pico_engine.__main__ import parse_bias
+    assert parse_bias("17:-2.5, 4:1") == [(17, -2.5), (4, 1.0)] and parse_bias("3:-inf") == [(3, float("-inf"))] and parse_bias("") == []
+    for bad in ("17", "a:1", "3:x"):
+        with pytest.raises(ValueError):
+            parse_bias(bad)
+    (tmp_path / "config.json").write_text("{}")
+    for args, what in ((("--n", "0"), "at least 1"), (("--logit-bias", "17"), "--logit-bias")):
+        r = subprocess.run([sys.executable, "-m", "pico_engine", str(tmp_path), "--prompt", "1,2", *args], cwd=ROOT, capture_output=True, text=True)
+        assert r.returncode != 0 and what in r.stderr
+
+
+def test_rules_on_the_next_token_are_checked():
+    import torch
+    from pico_engine.sampling import Sampler, SamplingParams, TokenAutomaton
+    from pico_engine.sampling.automaton import pack_mask
+    p = SamplingParams()
+    assert not p.ruled and not p.penalized and Sampler(p).rule_kind() == (False, 0, None)
+    p = SamplingParams(logit_bias={5: 1, 3: -float("inf")}, repetition_penalty=1.1)
+    assert p.ruled and p.logit_bias == ((5, 1.0), (3, -float("inf"))) and Sampler(p).rule_kind() == (True, 64, None)
+    assert Sampler(SamplingParams(logit_bias=[(i, 0.5) for i in range(65)])).rule_kind() == (False, 128, None)
+    nan, inf = float("nan"), float("inf")
+    for bad in (dict(repetition_penalty=0.0), dict(repetition_penalty=-1.0), dict(repetition_penalty=inf), dict(repetition_penalty=nan), dict(presence_penalty=nan),
+                dict(frequency_penalty=inf), dict(logit_bias={-1: 0.0}), dict(logit_bias=[(3, 1.0), (3, 2.0)]), dict(logit_bias={3: nan}), dict(logit_bias={3: inf}),
+                dict(grammar=torch.zeros(2, 2))):
+        with pytest.raises(ValueError):
+            SamplingParams(**bad)
+    for bad in (SamplingParams(logit_bias={50: 1.0}), SamplingParams(grammar=TokenAutomaton([[0] * 49]))):
+        with pytest.raises(ValueError, match="vocabulary"):
+            bad.check_vocab(50)
+    for bad in ([], [[]], [0, 1], [[0.0, 1.0]], [[True, False]], [[0, 2], [1, 1]], [[-2, 0]], [[-1, -1]]):
+        with pytest.raises(ValueError):
+            TokenAutomaton(bad)
+    for start in (-1, 2):
+        with pytest.raises(ValueError, match="start"):
+            TokenAutomaton([[0, 1], [1, -1]], start)
+    a = TokenAutomaton([[1, -1, 0], [-1, 0, -1]])
+    assert a.vocab == 3 and a.walk([2, 2, 0]) == 1 and a.walk([0, 1, 0]) == 1 and a.walk([0, 0]) == -1 and a.walk([1, 2]) == -1 and a.walk([], 1) == 1
+    allowed = torch.rand(3, 70, generator=torch.Generator().manual_seed(1)) < 0.5
+    words = pack_mask(allowed).long() & 0xffffffff
+    assert words.shape == (3, 3) and pack_mask(allowed).dtype == torch.int32
+    assert torch.equal((words[:, torch.arange(70) // 32] >> (torch.arange(70) % 32)) & 1, allowed.long()) and int((words[:, 2] >> 6).max()) == 0
