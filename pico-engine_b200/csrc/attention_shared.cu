@@ -11,7 +11,7 @@
 // one tile, or (more tiles than half the CTAs) a run of several (AsDeal).  Own: the pages of the tiles of 16 heads, token after token, in each the key
 // heads; every one of a CTA's AS_WORKERS warps takes a run of them, and runs differ by one page at most, whatever the rows' lengths.  There is a CTA an SM, and
 // each works on one line; how many take which goes by what their steps and pages cost (as_split).  (CTAs that took some of both went through two starts
-// and two ends: 64 answers of 28 heads of 128 took 33 us.)  Each CTA and each worker leaves sums, maxima and weights of its tiles' rows in scratch
+// and two ends: 64 answers of 28 heads of 128 on five prompts took 33 us instead of 29.)  Each CTA and each worker leaves sums, maxima and weights of its tiles' rows in scratch
 // (float32).  The second kernel joins them, a block a token and key head: m = max m_i, l = sum l_i 2^(m_i - m), o = sum o_i 2^(m_i - m).
 //
 //   warp 0      loader: a tile's queries as one box [tokens][heads of the key head][64 columns], and two pages of keys and values a step
@@ -41,7 +41,7 @@
 #define AS_OQ_BYTES (AS_OTILE * AS_HD * 2)         // queries of an own tile
 #define AS_PAGE_BYTES (PE_PAGE * AS_HD * 2)        // keys (or values) of a page
 #define AS_Q_BYTES (AS_QTILE * AS_HD * 2)
-#define AS_OUT_BYTES (8 * 1024)                    // through which results leave: the start of the queries' place
+#define AS_OUT_BYTES (8 * 1024)                    // in front of the own tiles' queries: the tokens' places in the two lines
 #define AS_QAREA_BYTES (AS_Q_BYTES > AS_OUT_BYTES + AS_WORKERS * AS_OQ_BYTES ? AS_Q_BYTES : AS_OUT_BYTES + AS_WORKERS * AS_OQ_BYTES)
 #define AS_HALF_BYTES (AS_KTILE * AS_HD * 2)       // keys (or values) of a step
 #define AS_STAGE_BYTES (2 * AS_HALF_BYTES)
@@ -282,6 +282,10 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
         if (t < p.T) { group.load(p, t); own.set(p, t, group.g); }
     };
     load(threadIdx.x);
+    if (warp == 1) {                                                // (while that travels; behind the shares it cost answers in a window 1.0 of 26.3 us)
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(at_smem(&tmem_base_s)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
     if (threadIdx.x == 32) {
         auto init = [](unsigned long long* bar, unsigned count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(at_smem(bar)), "r"(count) : "memory"); };
         init(q_full, 1); init(q_empty, 8); init(o_empty, 8);         // q_empty: the eight warps that write the tile's results
@@ -364,14 +368,11 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
         }
     }
     const bool has_shared = begin < min(end, units), has_own = own_cta >= 0 && own_cta < own_runs.ctas;       // (the first worker's run comes first)
+    if (!has_shared && warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base_s), "r"(512u) : "memory");
     if (!has_shared && !has_own) {                                  // (the whole block)
         pdl_wait();
         pdl_launch_dependents();
         return;
-    }
-    if (warp == 1 && has_shared) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(at_smem(&tmem_base_s)), "r"(512u) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
