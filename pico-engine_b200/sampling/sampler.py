@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import math
+import operator
 from dataclasses import dataclass
 from typing import Optional, Tuple
 
@@ -9,6 +10,8 @@ import torch
 
 from ..ops import kernels
 from .automaton import TokenAutomaton
+
+FLOAT32_TINY, FLOAT32_MAX = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max       # what the kernels take
 
 
 @dataclass(frozen=True)
@@ -22,7 +25,7 @@ class SamplingParams:
     Rules on what may be chosen, which the project does not have, change the logits before all that: ``repetition_penalty`` divides the
     positive and multiplies the negative ones of tokens in the prompt or the output; ``presence_penalty`` and ``frequency_penalty`` (times
     the number of times) are taken off those of tokens in the output; ``logit_bias`` ((token, value), ..) is added; ``grammar`` allows what its
-    state for the sequence allows."""
+    state for the sequence allows (where biases of -inf leave none of that, the choice is no longer the grammar's)."""
     temperature: float = 0.7
     top_k: int = 0
     top_p: float = 0.9
@@ -34,13 +37,16 @@ class SamplingParams:
     grammar: Optional[TokenAutomaton] = None
 
     def __post_init__(self):
-        if not (self.repetition_penalty > 0 and math.isfinite(self.repetition_penalty)):
+        if not FLOAT32_TINY <= self.repetition_penalty <= FLOAT32_MAX:
             raise ValueError("repetition_penalty must be positive")
-        if not (math.isfinite(self.presence_penalty) and math.isfinite(self.frequency_penalty)):
+        if not (abs(self.presence_penalty) <= FLOAT32_MAX and abs(self.frequency_penalty) <= FLOAT32_MAX):
             raise ValueError("presence_penalty and frequency_penalty must be numbers")
         bias = self.logit_bias.items() if isinstance(self.logit_bias, dict) else self.logit_bias
-        bias = tuple((int(t), float(v)) for t, v in bias)
-        if any(t < 0 or math.isnan(v) or v == math.inf for t, v in bias) or len({t for t, _ in bias}) != len(bias):
+        try:
+            bias = tuple((operator.index(t), float(v)) for t, v in bias)
+        except TypeError:
+            raise ValueError("logit_bias must be pairs of a token and a number") from None
+        if any(t < 0 or not (abs(v) <= FLOAT32_MAX or v == -math.inf) for t, v in bias) or len({t for t, _ in bias}) != len(bias):
             raise ValueError("logit_bias names tokens, each once, with a number (or -inf) each")
         object.__setattr__(self, "logit_bias", bias)
         if self.grammar is not None and not isinstance(self.grammar, TokenAutomaton):

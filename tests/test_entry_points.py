@@ -196,6 +196,7 @@ def test_rules_on_the_next_token_are_checked():
     nan, inf = float("nan"), float("inf")
     for bad in (dict(repetition_penalty=0.0), dict(repetition_penalty=-1.0), dict(repetition_penalty=inf), dict(repetition_penalty=nan), dict(presence_penalty=nan),
                 dict(frequency_penalty=inf), dict(logit_bias={-1: 0.0}), dict(logit_bias=[(3, 1.0), (3, 2.0)]), dict(logit_bias={3: nan}), dict(logit_bias={3: inf}),
+                dict(logit_bias={3: 1e39}), dict(logit_bias={3.5: 1.0}), dict(logit_bias=[3, 4]), dict(frequency_penalty=-1e39), dict(repetition_penalty=1e-39),
                 dict(grammar=torch.zeros(2, 2))):
         with pytest.raises(ValueError):
             SamplingParams(**bad)
