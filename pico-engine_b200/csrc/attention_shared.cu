@@ -16,7 +16,7 @@
 //
 //   warp 0      loader: a tile's queries as one box [tokens][heads of the key head][64 columns], and two pages of keys and values a step
 //   warp 1      issues S = Q.K^T three steps ahead of O += P.V
-//   warps 2-9   shared: softmax, two warpgroups that take the steps in turn (as in attention_prefill_tcgen05.cu); at the end of a tile both write
+//   warps 4-11  shared: softmax, two warpgroups that take the steps in turn (as in attention_prefill_tcgen05.cu); at the end of a tile both write
 //               their half of O.  Own: every warp goes its own way through its run, a page at a time with mma.sync; it asks for the next page itself when
 //               it has read the one before.  (Two warpgroups that shared a page and met at two barriers took 2,000 cycles for it.)
 //
@@ -35,7 +35,9 @@
 #define AS_PANELS (AS_HD / 64)
 #define AS_STAGES (AS_HD == 64 ? 5 : 3)
 #define AS_AHEAD 3
-#define AS_THREADS 320
+#define AS_THREADS 384                             // three warpgroups: loader, issuer and two warps without work; two that compute
+#define AS_REGS_SERVE 88
+#define AS_REGS_COMPUTE 208                        // of a thread: 128 x 88 + 256 x 208 = 384 x 168, what the block is launched with (as_launch looks)
 #define AS_WORKERS (AS_HD == 64 ? 8 : 6)           // warps that read own pages: each has half a stage, a page of keys and values
 #define AS_OTILE 16                                // rows of an own tile
 #define AS_OQ_BYTES (AS_OTILE * AS_HD * 2)         // queries of an own tile
@@ -49,7 +51,7 @@
 static_assert(AS_QAREA_BYTES % 1024 == 0 && 2 * AS_STAGES >= AS_WORKERS, "own pages use the places of the shared ones");
 #define AS_BUFFERS 3
 #define AS_BARS ((4 + 3 * AS_BUFFERS + 4 * AS_STAGES + 8 + 3 * AS_WORKERS + 1) / 2 * 2)      // (what follows them lies on 16 bytes)
-#define AS_WALKS (AS_THREADS / 32 + 1)             // the first tile; a warp's each
+#define AS_WALKS 11                                // the first tile; a working warp's each
 #define AS_SMEM_BYTES (AS_TILE_BYTES + 8 * AS_BARS + 2 * AS_QTILE * 4 + AS_WALKS * (int)sizeof(AsWalk) + AS_WORKERS * (int)sizeof(AsOwnWalk) + 4 * (AS_THREADS / 32) * 4)
 #define AS_O_COL (AS_BUFFERS * AS_KTILE)
 #define AS_LAZY 8.0f
@@ -394,14 +396,16 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
                      ::"r"(q_s + AS_OUT_BYTES + k * AS_OQ_BYTES), "l"(p.q + (size_t)z.now.t * p.q_stride + (size_t)(z.kvh * R + z.tile * AS_OTILE) * AS_HD), "r"(bytes), "r"(at_smem(&own_q[k])) : "memory");
     };
     // (the first tile has been found; a warp's own copy goes on from there)
-    AsWalk& w = walks[warp + 1];
-    if (lane == 0 && has_shared) w = walks[0];
+    AsWalk& w = walks[warp < 2 ? warp + 1 : warp < 4 ? 0 : warp - 1];
+    if (lane == 0 && has_shared && (warp < 2 || warp >= 4)) w = walks[0];
     __syncwarp();
     auto advance = [&](int seg) { return seg == 0 ? has_shared : as_next(w, p, deal, lane); };
     // the same of own tiles, in the same place when the others are done
     AsOwnWalk& ow = *reinterpret_cast<AsOwnWalk*>(&w);
     static_assert(sizeof(AsOwnWalk) <= sizeof(AsWalk) && alignof(AsWalk) >= alignof(AsOwnWalk), "the own walk takes the other's place");
 
+    if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AS_REGS_SERVE));
     if (warp == 0 && has_own) {                                     // ---------------- the plan of the join, while the workers read
         pdl_wait();                                                 // (scratch is written)
         const int all = p.T * p.nkv * p.own_tiles, ctas = min(own_ctas, own_runs.ctas);
@@ -526,9 +530,11 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
             }
         }
         if (!ok) atomicExch(status, 7);
-    } else {                                                        // ---------------- softmax, warps 2..9
+    }
+    } else {                                                        // ---------------- softmax, warps 4..11
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(AS_REGS_COMPUTE));
         const int quarter = warp & 3;                               // the 32 lanes of tensor memory this warp may touch
-        const int g = (warp - 2) >> 2;                              // the warpgroup: steps g, g + 2, ..
+        const int g = (warp - 4) >> 2;                              // the warpgroup: steps g, g + 2, ..
         const int r = quarter * 32 + lane;                          // this thread's row of the tile
         const unsigned lane_addr = tmem + ((unsigned)(quarter * 32) << 16);
         const unsigned long long scale2 = at_two(p.scale_log2e, p.scale_log2e);
@@ -655,7 +661,7 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
             if (live) reinterpret_cast<float2*>(p.scratch.ends + block + r)[g] = make_float2(m_mine, l_mine);
             // through the stages (the tile's products have read them, the next tile's come when this is done), 32 columns of the warp's 32 rows at a time, 16-byte
             // pieces exchanged by the row inside a run of eight: a lane storing its own row would touch 32 lines an instruction
-            const unsigned stage = kv_s + (warp - 2) * 4096;
+            const unsigned stage = kv_s + (warp - 4) * 4096;
             float* to = p.scratch.sums + block * AS_HD + g * (AS_HD / 2);
 #pragma unroll
             for (int c = 0; c < AS_HD / 2; c += 32) {
@@ -684,7 +690,7 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
             if (lane == 0) at_arrive(at_smem(q_empty));
         }
         // ---------------- own pages (of a CTA that has no shared steps): worker k's run
-        const int k = warp - 2, gr = lane >> 2, tq = lane & 3;      // fragment row and column of the lane
+        const int k = warp - 4, gr = lane >> 2, tq = lane & 3;      // fragment row and column of the lane
         bool more = has_own && k < AS_WORKERS && own_cta + k * own_ctas < own_runs.ctas;
         __syncwarp();
         if (lane == 0 && more) ow = own_walk[k];
@@ -932,11 +938,16 @@ int as_query_map(CUtensorMap* map, const void* q, long long tokens, int heads, l
     return r == CUDA_SUCCESS ? 0 : 20000 + (int)r;
 }
 
+static_assert(AS_SMEM_BYTES <= 227 * 1024, "shared memory of a block");
+
 template <bool MASKED>
 int as_launch(int grid, cudaStream_t stream, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const AsArgs& p, int* status) {
     static bool wide = false;
     if (!wide) {
         PE_TRY(cudaFuncSetAttribute(attention_shared_kernel<MASKED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)AS_SMEM_BYTES));
+        cudaFuncAttributes made;
+        PE_TRY(cudaFuncGetAttributes(&made, attention_shared_kernel<MASKED>));
+        if (made.numRegs * AS_THREADS < 128 * AS_REGS_SERVE + 256 * AS_REGS_COMPUTE) return PE_ERR_UNSUPPORTED;      // the computing warps would wait for registers for good
         wide = true;
     }
     PE_TRY(pe_launch(attention_shared_kernel<MASKED>, dim3(grid), AS_THREADS, AS_SMEM_BYTES, stream, mq, mk, mv, p, status));
