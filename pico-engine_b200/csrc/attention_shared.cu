@@ -20,6 +20,12 @@
 //               their half of O.  Own: every warp goes its own way through its run, a page at a time with mma.sync; it asks for the next page itself when
 //               it has read the one before.  (Two warpgroups that shared a page and met at two barriers took 2,000 cycles for it.)
 //
+// What bounds it (64 answers of 14 heads on 31,744 positions, 25.6 us; cycles of a CTA of shared steps): its share of the work 6,300, the first step's keys 5,100, 16
+// steps of 1,365 each (their exponentials alone are 1,024; a polynomial on the multiply-add units in the place of a quarter of them made a step longer, since a
+// warp's instructions then are what it waits for), the end 4,000; the join's three fetches that depend on one another 4.3 us.  With few shared positions the own
+// pages are fetched at 3.8 TB/s once they have begun.  The computing warps keep a row's 128 scores in registers: with 168 a thread the masked variant spilled 500
+// bytes, and answers in a window took 25.2 us instead of 21.2.
+//
 // All keys of a shared step are visible to all rows but for windows, pages that are not there and the half step behind an odd number of pages,
 // so the masks are a variant of their own (MASKED).  Every wait is bounded; one that runs out sets *status to 7, and the roles leave their loops.
 #ifndef PE_HEAD_DIM
@@ -36,8 +42,8 @@
 #define AS_STAGES (AS_HD == 64 ? 5 : 3)
 #define AS_AHEAD 3
 #define AS_THREADS 384                             // three warpgroups: loader, issuer and two warps without work; two that compute
-#define AS_REGS_SERVE 88
-#define AS_REGS_COMPUTE 208                        // of a thread: 128 x 88 + 256 x 208 = 384 x 168, what the block is launched with (as_launch looks)
+#define AS_REGS_SERVE 72
+#define AS_REGS_COMPUTE 216                        // of a thread: 128 x 72 + 256 x 216 = 384 x 168, what the block is launched with (as_launch looks)
 #define AS_WORKERS (AS_HD == 64 ? 8 : 6)           // warps that read own pages: each has half a stage, a page of keys and values
 #define AS_OTILE 16                                // rows of an own tile
 #define AS_OQ_BYTES (AS_OTILE * AS_HD * 2)         // queries of an own tile
@@ -126,7 +132,7 @@ struct AsDeal {
 };
 
 // How many of the CTAs take shared steps.  Measured (cycles of a CTA, on top of what both kinds need): a step 1,490, an own page 440 (its warps together), and a
-// CTA of shared steps needs the time of three more; with heads of 128 1,930, 1,270 and five.  Both kinds end together where
+// CTA of shared steps needs the time of three more; with heads of 128 1,930, 1,270 and five (a fifth less or more of a step's cost takes 2 to 10 % longer).  Both kinds end together where
 // step (steps / s + more) = page pages / (grid - s).
 __device__ __forceinline__ int as_split(int steps, int tiles, int pages, int grid) {
     constexpr float step = AS_HD == 64 ? 1490.f : 1930.f, page = AS_HD == 64 ? 440.f : 1270.f, more = AS_HD == 64 ? 3.f : 5.f;
