@@ -13,8 +13,9 @@
 // spread at random came to so many single sectors that all of them are read faster), and where the row is changed in place, logits of tokens that have not
 // been seen, which are not written either.  Biases are few and lie anywhere: a second kernel adds them to the result, an entry a thread
 // (picked out of the list and added up in shared memory by every block of the first one they cost as much as all the rest: 64 rows of 151,936 under
-// all rules 33 us, 24.6 this way; penalties alone 19.2 us, 5.1 TB/s, a mask alone 13.4).
+// all rules 33 us, 23.8 this way, its lists read while the first one works; penalties alone 19.2 us, 5.1 TB/s, a mask alone 13.4).
 #include "common.cuh"
+#include <type_traits>
 
 #define LR_THREADS 256
 #define LR_CHUNK (LR_THREADS * 8)                   // tokens of a block: eight a thread (with sixteen, and so fewer blocks an SM, 64 rows with penalties took 23 us instead of 19)
@@ -27,24 +28,22 @@ struct LrArgs {
     const int2* bias_range; const int* bias_ids; const float* bias_values; int n_bias;
     const unsigned* masks; int n_masks, mask_words; const int* mask_rows; int by_slot;      // by_slot: mask_rows has an entry a slot, not a row
 };
-// the mask of row b, or -1
-__device__ __forceinline__ int lr_mask(const LrArgs& p, int b, int slot) {
-    if (!p.masks || (p.by_slot && (slot < 0 || slot >= p.n_slots))) return -1;
-    return p.mask_rows[p.by_slot ? slot : b];
-}
+// the mask of the row whose entry is number `at`, or -1
+__device__ __forceinline__ int lr_mask(const LrArgs& p, int at, int entries) { return p.masks && at >= 0 && at < entries ? p.mask_rows[at] : -1; }
 
 // Four tokens at a time: those that lie on 16 bytes of the row (a vocabulary need not be a multiple of four), and what is left at the row's ends one by one.
-// ALIGNED: logits and out start on 16 bytes; else every load and store takes one number.
-template <bool ALIGNED, bool IN_PLACE>
+// ALIGNED: logits and out start on 16 bytes; else every load and store takes one number.  BY_SLOT: p.by_slot (a choice at run time made the mask of a row
+// wait for its slot either way: 200 rows of 50,257 under masks 17.5 us instead of 16.2).
+template <bool ALIGNED, bool IN_PLACE, bool BY_SLOT>
 __global__ void __launch_bounds__(LR_THREADS, 8) adjust_logits_kernel(const LrArgs p) {
     constexpr int TURNS = LR_CHUNK / 4 / LR_THREADS;                // runs of a thread
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();                                        // (behind the wait: the second kernel reads its lists before this one has ended)
     const int b = blockIdx.y, V = p.vocab;
     const size_t at0 = (size_t)b * V;
     const float* row = p.logits + at0;
     float* out = p.out + at0;
-    const int slot = p.slots ? p.slots[b] : -1, m = lr_mask(p, b, slot);
+    const int slot = BY_SLOT || p.history ? p.slots[b] : -1, m = BY_SLOT ? lr_mask(p, slot, p.n_slots) : lr_mask(p, b, p.rows);
     const bool known = p.history && slot >= 0 && slot < p.n_slots;
     const short* seen = p.history + (known ? (size_t)slot * V : 0);
     const unsigned* mask = m >= 0 && m < p.n_masks ? p.masks + (size_t)m * p.mask_words : nullptr;
@@ -120,8 +119,8 @@ __global__ void __launch_bounds__(LR_THREADS) add_biases_kernel(const LrArgs p) 
     __shared__ float values[LR_LIST];
     pdl_launch_dependents();
     for (int i = threadIdx.x; i < PLACES; i += LR_THREADS) { token[i] = -1; first_of[i] = LR_LIST; count[i] = 0; }
-    pdl_wait();
-    const int b = blockIdx.x, m = lr_mask(p, b, p.by_slot ? p.slots[b] : -1);
+    // Lists and masks were there before the first kernel began to work; the wait is for its results.
+    const int b = blockIdx.x, m = p.by_slot ? lr_mask(p, p.slots[b], p.n_slots) : lr_mask(p, b, p.rows);
     const int2 list = p.bias_range[b];
     const int first = max(list.x, 0), last = min(list.y, p.n_bias);
     const unsigned* mask = m >= 0 && m < p.n_masks ? p.masks + (size_t)m * p.mask_words : nullptr;
@@ -140,10 +139,8 @@ __global__ void __launch_bounds__(LR_THREADS) add_biases_kernel(const LrArgs p) 
         __syncthreads();                                            // (the table is empty, and the turn before has written)
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
-            now[k] = 0.f;
             if (id[k] < 0) continue;
             if (mask && !((mask[id[k] >> 5] >> (id[k] & 31)) & 1u)) { id[k] = -1; continue; }
-            now[k] = out[id[k]];
             unsigned at = ((unsigned)id[k] * 2654435761u) >> 20 & (PLACES - 1);
             for (;;) {
                 const int there = atomicCAS(&token[at], -1, id[k]);
@@ -154,6 +151,9 @@ __global__ void __launch_bounds__(LR_THREADS) add_biases_kernel(const LrArgs p) 
             atomicMin(&first_of[at], k * LR_THREADS + (int)threadIdx.x);
             atomicAdd(&count[at], 1);
         }
+        if (base == first) pdl_wait();
+#pragma unroll
+        for (int k = 0; k < PER; ++k) now[k] = id[k] >= 0 ? out[id[k]] : 0.f;
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
@@ -169,6 +169,7 @@ __global__ void __launch_bounds__(LR_THREADS) add_biases_kernel(const LrArgs p) 
             for (int i = threadIdx.x; i < PLACES; i += LR_THREADS) { token[i] = -1; first_of[i] = LR_LIST; count[i] = 0; }
         }
     }
+    if (first >= last) pdl_wait();                                  // (the kernel behind this one counts on the first one's end as well)
 }
 
 // Tokens into the table of what a sequence has seen.  prompt: their sign bits are set; else their counts go up by one, to 32,767 at most.
@@ -218,8 +219,12 @@ extern "C" int pe_adjust_logits(const float* logits, float* out, int rows, int v
     const LrArgs p = {logits, out, rows, vocab, slots, (const short*)history, n_slots, penalties, (const int2*)bias_range, bias_ids, bias_values, n_bias,
                       (const unsigned*)masks, n_masks, (vocab + 31) / 32, mask_rows, by_slot};
     const bool aligned = !(((uintptr_t)logits | (uintptr_t)out) & 15), in_place = logits == out;
-    const auto kernel = aligned ? (in_place ? adjust_logits_kernel<true, true> : adjust_logits_kernel<true, false>)
-                                : (in_place ? adjust_logits_kernel<false, true> : adjust_logits_kernel<false, false>);
+    const auto pick = [&](auto by) {
+        constexpr bool BY_SLOT = decltype(by)::value;
+        return aligned ? (in_place ? adjust_logits_kernel<true, true, BY_SLOT> : adjust_logits_kernel<true, false, BY_SLOT>)
+                       : (in_place ? adjust_logits_kernel<false, true, BY_SLOT> : adjust_logits_kernel<false, false, BY_SLOT>);
+    };
+    const auto kernel = by_slot ? pick(std::true_type()) : pick(std::false_type());
     PE_TRY(pe_launch(kernel, dim3((vocab + LR_CHUNK - 1) / LR_CHUNK, rows), LR_THREADS, 0, (cudaStream_t)stream, p));
     PE_LAUNCH_CHECK();
     if (bias_ids) {
