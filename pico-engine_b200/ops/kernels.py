@@ -1903,10 +1903,12 @@ SHARED_HEAD_DIMS = (64, 128)
 SHARED_MAX_ROWS = 1024        # AS_MAX_TOKENS of csrc/attention_shared.cu
 
 
-def _need_here(t: torch.Tensor, name: str) -> None:
-    """The launch goes to the current device's stream: its tensors have to lie there."""
-    if t.get_device() != torch.cuda.current_device():
-        raise KernelError(f"{name} lives on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+def _stream_here(t: torch.Tensor, name: str) -> int:
+    """The handle of the current device's stream, to which the launch goes: its tensors have to lie there."""
+    device = torch._C._cuda_getDevice()
+    if t.get_device() != device:
+        raise KernelError(f"{name} lives on {t.device}, the current device is cuda:{device}")
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def attention_shared_takes(dtype: torch.dtype, rows: int, n_heads: int, n_kv_heads: int, head_dim: int, scale: float) -> bool:
@@ -1958,7 +1960,7 @@ def attention_shared(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: i
     if not attention_shared_takes(torch.bfloat16, T, n_heads, n_kv_heads, head_dim, scale):
         raise KernelError(f"attention_shared takes at most {SHARED_MAX_ROWS} rows, head sizes {SHARED_HEAD_DIMS}, a positive scale and at most 128 query heads a key "
                           f"head, not {T} rows, {n_heads} / {n_kv_heads} heads of {head_dim}, scale {scale}")
-    if len(pool) != 4 or pool[1:] != (n_kv_heads, PAGE, head_dim):
+    if len(pool) != 4 or pool != (pool[0], n_kv_heads, PAGE, head_dim):
         raise KernelError(f"cache pool must be [pages, {n_kv_heads}, {PAGE}, {head_dim}], not {tuple(pool)}")
     _need(block_table, "block_table", torch.int32)
     _need(tok_pos, "tok_pos", torch.int32, (T,)); _need(tok_row, "tok_row", torch.int32, (T,)); _need(groups, "groups", torch.int32, (T, 4))
@@ -1975,14 +1977,14 @@ def attention_shared(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: i
         out = torch.empty(T, width, dtype=torch.bfloat16, device=q.device)
     else:
         _need(out, "out", torch.bfloat16, (T, width))
-    _need_here(q, "q")
+    stream = _stream_here(q, "q")
     if T == 0:
         return out
     lib = for_head_dim(head_dim)
     if not (sharing_pays(4 * T * max_context * n_kv_heads * head_dim) if together is None else together):
         check(lib.pe_attention_decode(q.data_ptr(), q_stride, out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(), table_stride,
                                       tok_pos.data_ptr(), tok_row.data_ptr(), T, n_heads, n_kv_heads, head_dim, window or 0, scale, max_context,
-                                      1 if early_pages else 0, status_ptr(q.device), stream_ptr(), keep_first if window else 0, _ptr(slopes), _ptr(sinks)),
+                                      1 if early_pages else 0, status_ptr(q.device), stream, keep_first if window else 0, _ptr(slopes), _ptr(sinks)),
               "attention_shared")
         return out
     # (the scratch is the call's own: calls on two streams and captured graphs share none)
@@ -1990,7 +1992,7 @@ def attention_shared(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: i
     check(lib.pe_attention_shared(q.data_ptr(), q_stride, out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), pool[0], block_table.data_ptr(), table_stride,
                                   tok_pos.data_ptr(), tok_row.data_ptr(), groups.data_ptr(), T, n_heads, n_kv_heads, head_dim, window or 0,
                                   keep_first if window else 0, scale, max_context, _ptr(slopes), _ptr(sinks), 1 if early_pages else 0, scratch.data_ptr(),
-                                  status_ptr(q.device), stream_ptr()), "attention_shared", 2)
+                                  status_ptr(q.device), stream), "attention_shared", 2)
     return out
 
 
@@ -2048,10 +2050,10 @@ def adjust_logits(logits: torch.Tensor, slots: Optional[torch.Tensor] = None, hi
         return out
     if B > 65535:
         raise KernelError(f"adjust_logits takes at most 65,535 rows, not {B}")
-    _need_here(logits, "logits")
+    stream = _stream_here(logits, "logits")
     check(answers().pe_adjust_logits(logits.data_ptr(), out.data_ptr(), B, V, _ptr(slots), _ptr(history), n, _ptr(penalties), _ptr(bias_range),
                                      _ptr(bias_ids) if n_bias else None, _ptr(bias_values), n_bias, _ptr(masks) if n_masks else None, n_masks,
-                                     _ptr(mask_rows if states is None else states), 0 if states is None else 1, stream_ptr()), "adjust_logits", 2 if n_bias else 1)
+                                     _ptr(mask_rows if states is None else states), 0 if states is None else 1, stream), "adjust_logits", 2 if n_bias else 1)
     return out
 
 
@@ -2077,9 +2079,9 @@ def note_tokens(history: Optional[torch.Tensor], slots: torch.Tensor, tokens: to
         _need(states, "states", torch.int32, (n,)); _need(transitions, "transitions", torch.int32, (n_states, V))
     if N == 0 or n == 0:
         return history
-    _need_here(tokens, "tokens")
+    stream = _stream_here(tokens, "tokens")
     check(answers().pe_note_tokens(_ptr(history), n, V, slots.data_ptr(), tokens.data_ptr(), N, 1 if prompt else 0, _ptr(states), _ptr(transitions), n_states,
-                                   stream_ptr()), "note_tokens")
+                                   stream), "note_tokens")
     return history
 
 
@@ -2101,8 +2103,8 @@ def step_tables(slots: torch.Tensor, starts: torch.Tensor, lens: torch.Tensor, h
     _need(row_first, "row_first", torch.int32, (B + 1,)); _need(tables, "tables", torch.int32, (B, table[1]))
     if B == 0:
         raise KernelError("a step needs at least one row")
-    _need_here(slots, "slots")
+    stream = _stream_here(slots, "slots")
     check(answers().pe_step_tables(slots.data_ptr(), starts.data_ptr(), lens.data_ptr(), held.data_ptr(), pages.data_ptr(), pages.shape[0],
                                    resident.data_ptr(), res[0], res[1], B, tok_pos.data_ptr(), tok_row.data_ptr(),
-                                   row_first.data_ptr(), places.data_ptr(), T, tables.data_ptr(), table[1], stream_ptr()), "step_tables")
+                                   row_first.data_ptr(), places.data_ptr(), T, tables.data_ptr(), table[1], stream), "step_tables")
     return tok_pos, tok_row, row_first, places, tables
