@@ -44,6 +44,7 @@ def attention(**change):
     (dict(v_pool=there(torch.zeros(8, 2, 64, 64, dtype=torch.bfloat16))), "v_pool must have shape"),
     (dict(head_dim=32), "head sizes"), (dict(scale=0.0), "positive scale"), (dict(n_heads=13), "query heads"), (dict(n_heads=258, q_stride=258 * 64), "at most 128 query heads"),
     (dict(q_stride=900), "multiple of 8"), (dict(q_stride=888), "rows of 896"), (dict(q_stride=2000), "rows of 896"),
+    (dict(tok_pos=i32(1025)), "at most 1024 rows"), (dict(k_pool=there(torch.zeros(0, dtype=torch.bfloat16)), v_pool=there(torch.zeros(0, dtype=torch.bfloat16))), "cache pool must be"),
     (dict(tok_row=i32(2)), "tok_row must have shape"), (dict(groups=i32(2, 4)), "groups must have shape"),
     (dict(max_context=0), "max_context"), (dict(keep_first=-1), "not negative"), (dict(window=-4), "not negative"),
     (dict(sinks=f32(2)), "sinks must have shape"), (dict(slopes=f32(2)), "slopes must have shape"),

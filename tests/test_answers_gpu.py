@@ -173,6 +173,39 @@ def test_attention_shared_equals_each_row_alone(K):
     K.check_status("cuda")
 
 
+@pytest.mark.parametrize("nh,nkv,hd", [(2, 1, 64), (4, 2, 128)])
+def test_attention_shared_of_as_many_rows_as_it_takes(K, nh, nkv, hd):
+    groups = [(64 * (1 + i % 3), [1 + (i + j) % 66 for j in range(16)]) for i in range(32)] + [(128, [1 + j % 5 for j in range(512)])]
+    a = Answers(nh, nkv, hd, groups, seed=hd)
+    assert a.T == K.SHARED_MAX_ROWS
+    agree(a.run(K), *a.want())
+    agree(a.run(K, window=90, keep=3), *a.want(window=90, keep=3))
+    K.check_status("cuda")
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_attention_shared_of_what_is_no_number(K, hd, value):
+    """A key that is no number in a group's prompt reaches all of its rows' heads of that key head, one in a row's own part that row's, a value its column;
+    nothing else moves by a bit."""
+    a = Answers(6, 2, hd, [(640, [3, 70, 130]), (192, [5, 9])], seed=hd)
+    agree(a.run(K), *a.want())
+    before = a.run(K).view(5, 2, 3, hd).clone()
+    for pool, page, rows in ((a.k, a.table[0, 4], [0, 1, 2]), (a.k, a.table[1, 10], [1]), (a.v, a.table[3, 1], [3, 4]), (a.v, a.table[2, 12], [2])):
+        keep = pool[page, 1].clone()
+        pool[page, 1, 1] = value if pool is a.k else pool[page, 1, 1].index_fill(0, torch.tensor([5], device="cuda"), value)
+        got = a.run(K).view(5, 2, 3, hd)
+        pool[page, 1] = keep
+        touched = torch.zeros(5, 2, 3, hd, dtype=torch.bool, device="cuda")
+        touched[rows, 1] = True
+        if pool is a.v:
+            touched[..., :5] = touched[..., 6:] = False
+        assert torch.equal(got[~touched], before[~touched])
+        assert not torch.isfinite(got[touched]).any() if value != value or pool is a.v else True
+    agree(a.run(K), *a.want())
+    K.check_status("cuda")
+
+
 def test_attention_shared_in_two_captured_graphs(K):
     """Two graphs captured one after the other and replayed in turn, on two streams at once, beside eager calls: each has scratch of its own."""
     a, b = (Answers(14, 2, 64, [(64 * n, [1 + 5 * i for i in range(m)])], seed=n) for n, m in ((30, 20), (100, 9)))

@@ -307,3 +307,20 @@ def test_steps_with_and_without_shared_pages(models, together, tmp_path, name):
     for a, b in zip(*logits.values()):
         assert float((a - b).abs().max()) <= 8e-2 * float(a.abs().max())
         assert not torch.equal(a[1], a[2])
+
+
+def test_command_line(models, tmp_path):
+    import json
+    import os
+    import subprocess
+    import sys
+    eng, cfg, w = models[("A", "float32")]
+    folder = write_model(tmp_path / "m", dict(TINY["A"]), w)
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-m", "pico_engine", str(folder), "--prompt", "5,17,3", "--prompt", "9,9", "--max-tokens", "6", "--temperature", "0.8",
+                        "--dtype", "float32", "--n", "2", "--repetition-penalty", "1.3", "--frequency-penalty", "0.5", "--logit-bias", "3:2.5,17:-1"],
+                       cwd=root, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-2000:]
+    lines = [json.loads(line) for line in r.stdout.splitlines() if line.startswith("{")]
+    want = eng.generate([[5, 17, 3], [9, 9]], 6, 0.8, n=2, repetition_penalty=1.3, frequency_penalty=0.5, logit_bias={3: 2.5, 17: -1.0})
+    assert [(q["prompt"], q["output"]) for q in lines] == [(p, o) for p, answers in zip(([5, 17, 3], [9, 9]), want) for o in answers]
