@@ -19,7 +19,7 @@ from ..ops import kernels
 from ..ops.library import core, require_cuda
 from ..sampling import RuleMemory, Sampler, SamplingParams, TokenAutomaton
 from ..weights import load_folder, load_into, random_tensor
-from .generate import Request, cut_prompts, generate as run_generation, held_tokens
+from .generate import Request, cut_prompts, generate as run_generation, forked_tokens, held_tokens
 from .graph import GraphedDecode, TokenLoop, bucket_rows
 from .step import Stepper
 
@@ -139,7 +139,7 @@ class Engine:
         mnt = [max_tokens] * len(prompts) if isinstance(max_tokens, int) else list(max_tokens)
         probe = [Request(i, list(p), m) for i, (p, m) in enumerate(zip(prompts, mnt)) if len(p)]
         if probe:
-            need = [held_tokens(r) for r in probe for _ in range(answers)]
+            need = [forked_tokens(r) if j else held_tokens(r) for r in probe for j in range(answers)]
             budget = self._want_tokens or sum(sorted(need, reverse=True)[:self.max_batch])
             self.ensure_cache(max(budget, max(need)), max(len(r.prompt) + max(r.max_new_tokens - 1, 0) for r in probe))
         self.last_timing = {"prefill_s": 0.0, "decode_s": 0.0, "decode_steps": 0, "h2d_bytes": 0}

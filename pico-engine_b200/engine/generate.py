@@ -54,9 +54,14 @@ def held_tokens(r: Request) -> int:
     return (n + PAGE - 1) // PAGE * PAGE
 
 
+def forked_tokens(r: Request) -> int:
+    """The same for a request that goes on from the prompt of another of its family: the prompt's whole pages are the other's."""
+    return held_tokens(r) - len(r.prompt) // PAGE * PAGE
+
+
 def plan_batches(requests: Sequence[Request], max_batch: int, max_tokens: int) -> List[List[Request]]:
     """Requests in their order, cut into batches of at most ``max_batch`` sequences whose
-    largest possible cache holdings fit ``max_tokens`` together."""
+    largest possible cache holdings fit ``max_tokens`` together (a prompt's whole pages count once for its family)."""
     if max_batch < 1:
         raise GenerationError("max_batch must be at least 1")
     batches: List[List[Request]] = []
@@ -66,11 +71,12 @@ def plan_batches(requests: Sequence[Request], max_batch: int, max_tokens: int) -
         need = held_tokens(r)
         if need > max_tokens:
             raise GenerationError(f"request {r.index} can hold {need} tokens, the cache has room for {max_tokens}")
-        if cur and (len(cur) == max_batch or held + need > max_tokens):
+        more = forked_tokens(r) if cur and r.family >= 0 and r.family == cur[-1].family else need
+        if cur and (len(cur) == max_batch or held + more > max_tokens):
             batches.append(cur)
-            cur, held = [], 0
+            cur, held, more = [], 0, need
         cur.append(r)
-        held += need
+        held += more
     if cur:
         batches.append(cur)
     return batches

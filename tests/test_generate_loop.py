@@ -237,6 +237,18 @@ def test_answers_that_do_not_fit_one_batch_run_their_prompt_again():
         generate(be, [[1]], 1, [], 1, 4096, answers=0)
 
 
+def test_a_familys_prompt_counts_once_a_batch():
+    from pico_engine.engine.generate import Request, forked_tokens, held_tokens, plan_batches
+    r = [Request(i, [1] * 130, 60, family=0) for i in range(5)] + [Request(5, [1] * 64, 1, family=1), Request(6, [1] * 64, 1, family=1), Request(7, [1] * 64, 1)]
+    assert (held_tokens(r[0]), forked_tokens(r[0])) == (192, 64) and (held_tokens(r[5]), forked_tokens(r[5])) == (64, 0)
+    assert forked_tokens(Request(0, [1] * 63, 1)) == 64 and forked_tokens(Request(0, [1] * 64, 2)) == 64
+    cut = lambda *a: [[q.index for q in b] for b in plan_batches(r, *a)]         # noqa: E731
+    assert cut(8, 192 + 4 * 64 + 2 * 64) == [[0, 1, 2, 3, 4, 5, 6, 7]]
+    assert cut(8, 192 + 4 * 64) == [[0, 1, 2, 3, 4], [5, 6, 7]]
+    assert cut(8, 192 + 64) == [[0, 1], [2, 3], [4, 5, 6], [7]] and cut(3, 10 ** 6) == [[0, 1, 2], [3, 4, 5], [6, 7]]
+    assert cut(8, 192) == [[0], [1], [2], [3], [4], [5, 6, 7]]
+
+
 def test_an_error_among_answers_gives_all_slots_back():
     class Broken(Family):
         def decode(self, *a):

@@ -92,6 +92,23 @@ def test_answers_of_one_prompt_of_none_and_over_several_batches(models):
     nothing_held(eng)
 
 
+@pytest.mark.parametrize("name", ["C", "P4"])
+def test_a_cache_that_holds_a_familys_prompt_once(tmp_path, name):
+    """No more pages than the prompt's and what the answers add: every batch runs, with the answers of a cache that is large enough for all."""
+    from pico_engine.engine.engine import Engine
+    cfg = TINY["C"] if name == "C" else OTHERS[name][0]
+    weights = make_weights(cfg, 2, sharp=True) if name == "C" else OTHERS[name][1](cfg)
+    folder = write_model(tmp_path / "m", dict(cfg), weights)
+    prompts = prompts_of(cfg, [300, 40])
+    kw = dict(max_tokens=20, temperature=0.9, top_p=1.0, seed=1, stop_token_ids=())
+    want = Engine(folder, dtype="float32").generate([p for p in prompts for _ in range(6)], **kw)
+    for tokens in (320 + 5 * 64 + 6 * 64, 320 + 5 * 64, 320 + 64, 320):          # all together; a family a batch; two answers; one
+        eng = Engine(folder, dtype="float32", max_tokens_in_cache=tokens)
+        assert eng.generate(prompts, n=6, **kw) == [want[:6], want[6:]]
+        assert eng.cache.n_pages * 64 == tokens
+        nothing_held(eng)
+
+
 @pytest.mark.parametrize("name", ["A", "B", "C"])
 def test_a_prompt_in_portions(models, name):
     eng, cfg, _ = models[(name, "float32")]
