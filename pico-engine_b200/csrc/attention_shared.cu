@@ -86,7 +86,7 @@ struct AsArgs {
 // The positions that token t reads with its group; 0: it reads all by itself (alone in its group, or not a group of this step)
 __device__ __forceinline__ int as_shared(const int4& g, int t, int T, int table_stride) {
     if (g.y < 2 || g.x < 0 || t < g.x || g.y > T - g.x || t >= g.x + g.y || g.w < g.x || g.w >= g.x + g.y) return 0;
-    return max(0, min(g.z / PE_PAGE, table_stride)) * PE_PAGE;
+    return max(0, min(g.z / PE_PAGE, table_stride - 1)) * PE_PAGE;
 }
 // Pages in the order they are read: page j is j < kept ? j : page_lo + j - kept.
 struct AsPages {
@@ -169,7 +169,7 @@ struct AsOwn {
         const int at = max(p.tok_pos[t], 0);
         skip = min(as_shared(g, t, p.T, p.table_stride), at / PE_PAGE * PE_PAGE);
         pos = at - skip;
-        pages.set(pos / PE_PAGE + 1, pos, p.window, max(p.keep_first - skip, 0));
+        pages.set(min(pos / PE_PAGE + 1, p.table_stride - skip / PE_PAGE), pos, p.window, max(p.keep_first - skip, 0));      // (no further than the table)
         steps = pages.n * p.nkv * p.own_tiles;
     }
     __device__ __forceinline__ void load(const AsArgs& p, int token) { set(p, token, p.groups[token]); }
@@ -977,7 +977,7 @@ extern "C" int pe_attention_shared(const void* q, int q_stride, void* out, const
                                    int nh, int nkv, int hd, int window, int keep_first, float scale, int max_context, const float* slopes,
                                    const float* sinks, int early_pages, void* scratch, int* status, void* stream) {
     if (T <= 0) return 0;
-    if (hd != AS_HD || nkv <= 0 || nh % nkv || nh / nkv > AS_QTILE || q_stride % 8 || !(scale > 0.f) || !status || !scratch || keep_first < 0) return PE_ERR_UNSUPPORTED;
+    if (hd != AS_HD || nkv <= 0 || nh % nkv || nh / nkv > AS_QTILE || q_stride % 8 || !(scale > 0.f) || !status || !scratch || keep_first < 0 || table_stride < 1) return PE_ERR_UNSUPPORTED;
     if (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)groups | (uintptr_t)scratch) & 15) return PE_ERR_UNSUPPORTED;
     if (pool_pages * nkv * PE_PAGE > 0x7fffff00ll) return PE_ERR_UNSUPPORTED;       // TMA coordinates are 32-bit
     const int R = nh / nkv;

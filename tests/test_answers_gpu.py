@@ -173,6 +173,21 @@ def test_attention_shared_equals_each_row_alone(K):
     K.check_status("cuda")
 
 
+def test_attention_shared_reads_no_further_than_the_table(K):
+    """Positions and shared pages beyond a row of the table: what the row names is read."""
+    a = Answers(14, 2, 64, [(192, [64, 128]), (128, [64])], seed=8)
+    want = a.want()
+    a.table = a.table[:, :5].contiguous()                                # (the second row's pages fill it)
+    a.width = 5
+    a.pos[1] += 64 * 40
+    a.pos[2] += 64 * 2 + 5
+    agree(a.run(K), *want)
+    groups = K.shared_groups(a.members, "cuda")
+    groups[:2, 2] = 64 * 100                                             # the first group's rows name two pages of their own behind the three: those are not shared
+    a.run(K, groups=groups)
+    K.check_status("cuda")
+
+
 @pytest.mark.parametrize("nh,nkv,hd", [(2, 1, 64), (4, 2, 128)])
 def test_attention_shared_of_as_many_rows_as_it_takes(K, nh, nkv, hd):
     groups = [(64 * (1 + i % 3), [1 + (i + j) % 66 for j in range(16)]) for i in range(32)] + [(128, [1 + j % 5 for j in range(512)])]
