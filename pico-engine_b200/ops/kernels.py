@@ -1917,10 +1917,10 @@ def attention_shared_takes(dtype: torch.dtype, rows: int, n_heads: int, n_kv_hea
 
 
 # Bytes of keys and values that a layer does not read again before reading shared pages together pays.  Read row by row they come from L2 at 8 to 13 TB/s; what
-# the second way costs is a longer start and its join.  Measured on a B200, one by one against together: 14 heads of 64, 16 rows on 2,048
-# positions (16 MB) 8.2 us against 9.6, on 8,192 (63 MB) 16.4, 12.9, 64 on 8,192 (264 MB) 35.8, 16.4; 28 heads of 128, 8 rows on 4,096 (59 MB) 14.3,
-# 15.6, 16 on 2,048 (63 MB) 15.1, 14.8, 64 on 8,192 (1,057 MB) 144, 30.5.
-SHARING_PAYS_BYTES = 64_000_000
+# the second way costs is a longer start and its join.  Measured on a B200, one by one against together, us: 14 heads of 64, 16 rows on 2,048 positions
+# (16 MB) 8.0 and 9.4, on 4,032 (31 MB) 10.7 and 10.1, on 6,016 (46 MB) 13.2 and 11.5, 64 rows on 4,096 (132 MB) 20.9 and 16.3; 28 heads of 128, 8 rows on 3,200 (46 MB)
+# 12.4 and 14.0, on 4,096 (59 MB) 14.3 and 14.3, on 6,016 (86 MB) 18.5 and 16.2, 64 on 8,192 (1,057 MB) 144 and 28.4.
+SHARING_PAYS_BYTES = 50_000_000
 
 
 def sharing_pays(saved_bytes: int) -> bool:
