@@ -56,7 +56,7 @@
 #define AS_TILE_BYTES (AS_QAREA_BYTES + AS_STAGES * AS_STAGE_BYTES)
 static_assert(AS_QAREA_BYTES % 1024 == 0 && 2 * AS_STAGES >= AS_WORKERS, "own pages use the places of the shared ones");
 #define AS_BUFFERS 3
-#define AS_BARS ((4 + 3 * AS_BUFFERS + 4 * AS_STAGES + 8 + 3 * AS_WORKERS + 1) / 2 * 2)      // (what follows them lies on 16 bytes)
+#define AS_BARS ((5 + 3 * AS_BUFFERS + 4 * AS_STAGES + 8 + 3 * AS_WORKERS + 1) / 2 * 2)      // (what follows them lies on 16 bytes)
 #define AS_WALKS 11                                // the first tile; a working warp's each
 #define AS_SMEM_BYTES (AS_TILE_BYTES + 8 * AS_BARS + 2 * AS_QTILE * 4 + AS_WALKS * (int)sizeof(AsWalk) + AS_WORKERS * (int)sizeof(AsOwnWalk) + 4 * (AS_THREADS / 32) * 4)
 #define AS_O_COL (AS_BUFFERS * AS_KTILE)
@@ -262,8 +262,8 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
     const unsigned q_s = at_smem(as_mem), kv_s = q_s + AS_QAREA_BYTES;
     unsigned long long* bars = reinterpret_cast<unsigned long long*>(as_mem + AS_TILE_BYTES);
     unsigned& tmem_base_s = *reinterpret_cast<unsigned*>(bars);
-    unsigned long long *q_full = bars + 1, *q_empty = bars + 2, *o_empty = bars + 3;
-    unsigned long long *s_full = bars + 4, *p_full = s_full + AS_BUFFERS, *pv_done = p_full + AS_BUFFERS;
+    unsigned long long *q_full = bars + 1, *q_empty = bars + 2, *o_empty = bars + 3, *o_full = bars + 4;
+    unsigned long long *s_full = bars + 5, *p_full = s_full + AS_BUFFERS, *pv_done = p_full + AS_BUFFERS;
     unsigned long long *k_full = pv_done + AS_BUFFERS, *v_full = k_full + AS_STAGES, *k_empty = v_full + AS_STAGES, *v_empty = k_empty + AS_STAGES;
     unsigned long long* told = v_empty + AS_STAGES;                 // [warpgroup][32 rows]: a step's reference points are there
     unsigned long long *own_q = told + 8, *own_k = own_q + AS_WORKERS, *own_v = own_k + AS_WORKERS;      // [worker]: what it has asked for is there
@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
     }
     if (threadIdx.x == 32) {
         auto init = [](unsigned long long* bar, unsigned count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(at_smem(bar)), "r"(count) : "memory"); };
-        init(q_full, 1); init(q_empty, 8); init(o_empty, 8);         // q_empty: the eight warps that write the tile's results
+        init(q_full, 1); init(q_empty, 8); init(o_empty, 8); init(o_full, 1);         // q_empty: the eight warps that write the tile's results
         for (int s = 0; s < AS_STAGES; ++s) { init(&k_full[s], 1); init(&v_full[s], 1); init(&k_empty[s], 1); init(&v_empty[s], 1); }
         for (int b = 0; b < AS_BUFFERS; ++b) { init(&s_full[b], 1); init(&p_full[b], 4); init(&pv_done[b], 1); }
         for (int w = 0; w < 8; ++w) init(&told[w], 1);
@@ -532,6 +532,7 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
                     at_mma_ts(elected, tmem + AS_O_COL, tmem + b * AS_KTILE + kk * 8, dvs + ((kk * 16 * 128) >> 4), idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
                 at_commit_by(elected, at_smem(&v_empty[s]));
                 at_commit_by(elected, at_smem(&pv_done[b]));
+                if (i + 1 == count) at_commit_by(elected, at_smem(o_full));
                 if (i + AS_AHEAD < count && !issue_s(it + AS_AHEAD)) { ok = false; break; }
             }
         }
@@ -659,9 +660,10 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
             if (!ok) break;
             // ---- the tile's end: both groups write their half of O, and the reference point and sum of their own steps.  (Reference points only grow, and
             // the last step's is what O goes by: the larger of the two.)
-            const int last = it0 + count - 1;
             it0 += count;
-            if (!at_wait_warp(at_smem(&pv_done[last % AS_BUFFERS]), (unsigned)(last / AS_BUFFERS) & 1u)) { ok = false; break; }
+            // (A barrier of the tile's, of which every warp sees every phase.  pv_done[last % 3] would not do: where values come late, the group that took the step before
+            // the last can be here before the products of last - 3 are done, and a wait by parity takes the phase before those for the last one.)
+            if (!at_wait_warp(at_smem(o_full), (unsigned)seg & 1u)) { ok = false; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const size_t block = as_block(cta, w.now.g, p, w.kvh, w.tile);
             if (live) reinterpret_cast<float2*>(p.scratch.ends + block + r)[g] = make_float2(m_mine, l_mine);

@@ -173,6 +173,24 @@ def test_attention_shared_equals_each_row_alone(K):
     K.check_status("cuda")
 
 
+@pytest.mark.parametrize("window,keep", [(2000, 4), (None, 0)])
+def test_attention_shared_when_memory_is_slow(K, window, keep):
+    """Keys and values that come from DRAM, late and in any order, call after call without a pause: the same bits every time.  (Such calls once
+    had results of a tile that were taken before its last products were done.)"""
+    a = Answers(32, 8, 128, [(2496, [1 + 61 * i % 1500 for i in range(24)]), (960, [1 + 97 * i % 700 for i in range(8)])], seed=6)
+    want = a.want(window=window, keep=keep, sinks=True)
+    flush = torch.empty(2 ** 28, dtype=torch.uint8, device="cuda")       # more than L2 holds
+    first = a.run(K, window, keep, sinks=True)
+    agree(first, *want)
+    wrong = torch.zeros((), device="cuda")
+    for _ in range(400):
+        flush.zero_()
+        for _ in range(2):
+            wrong += (a.run(K, window, keep, sinks=True) != first).any()
+    assert int(wrong) == 0
+    K.check_status("cuda")
+
+
 def test_attention_shared_reads_no_further_than_the_table(K):
     """Positions and shared pages beyond a row of the table: what the row names is read."""
     a = Answers(14, 2, 64, [(192, [64, 128]), (128, [64])], seed=8)
