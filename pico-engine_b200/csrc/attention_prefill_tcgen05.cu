@@ -54,7 +54,7 @@
 #define AT_STAGE_BYTES (2 * 2 * AT_KTILE * AT_HD * 2)   // keys, then values, of two pages and one head
 #define AT_TILE_BYTES (AT_Q_BYTES + AT_STAGES * AT_STAGE_BYTES)
 #define AT_BUFFERS 3                               // S buffers
-#define AT_BAR_WORDS (2 + 3 * AT_BUFFERS + 4 * AT_STAGES + 12)
+#define AT_BAR_WORDS (2 + 3 * AT_BUFFERS + 4 * AT_STAGES + 13)
 #define AT_SMEM_BYTES (AT_TILE_BYTES + 8 * AT_BAR_WORDS + 2 * 2 * AT_QTILE * 4)
 #define AT_TMEM_COLS 512                           // S buffers (then P) at columns 0, 128 and 256, O from column 384
 #define AT_O_COL (AT_BUFFERS * 2 * AT_KTILE)
@@ -86,6 +86,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
     unsigned long long *k_full = pv_done + AT_BUFFERS, *v_full = k_full + AT_STAGES, *k_empty = v_full + AT_STAGES, *v_empty = k_empty + AT_STAGES;
     unsigned long long* told = v_empty + AT_STAGES;                 // [warpgroup][32 rows]: a step's reference points are there
     unsigned long long* met = told + 8;                             // [32 rows]: both warpgroups have come to the end
+    unsigned long long* o_full = met + 4;                           // and so have the products
     float* refs = reinterpret_cast<float*>(bars + AT_BAR_WORDS);    // [warpgroup][row]: reference point of the group's last step
     float* sums = refs + 2 * AT_QTILE;                              // [warpgroup][row]: at the end, the group's share of the row's sum
     if (q_s & 1023u) {                                              // every thread alike: nothing is allocated yet
@@ -128,6 +129,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
         for (int b = 0; b < AT_BUFFERS; ++b) { init(&s_full[b], 1); init(&p_full[b], 4); init(&pv_done[b], 1); }     // p_full: a warpgroup's four warps
         for (int w = 0; w < 8; ++w) init(&told[w], 1);
         for (int q = 0; q < 4; ++q) init(&met[q], 2);
+        init(o_full, 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
         // the queries and the first step are asked for before the block meets
         const int y[2] = {rows_of(table[page_at(0)]), rows_of(1 < n_pages ? table[page_at(1)] : -1)};
@@ -204,6 +206,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
                     at_mma_ts(elected, tmem + AT_O_COL, tmem + b * (2 * AT_KTILE) + kk * 8, dvs + ((kk * 16 * 128) >> 4), idesc_o, (it > 0 || kk > 0) ? 1u : 0u);
                 at_commit_by(elected, at_smem(&v_empty[s]));   // the stage's values have been read
                 at_commit_by(elected, at_smem(&pv_done[b]));   // and O holds this step's share
+                if (it + 1 == n_steps) at_commit_by(elected, at_smem(o_full));
                 if (it + AT_AHEAD < n_steps && !issue_s(it + AT_AHEAD)) ok = false;
             }
             if (!ok) atomicExch(status, 5);
@@ -328,7 +331,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
         if (lane == 0) at_arrive(at_smem(&met[quarter]));
         const int last = n_steps - 1;
         if (ok && !at_wait_warp(at_smem(&met[quarter]), 0u)) ok = false;
-        if (ok && !at_wait_warp(at_smem(&pv_done[last % AT_BUFFERS]), (unsigned)(last / AT_BUFFERS) & 1u)) ok = false;
+        // (not pv_done[last % 3]: the group that took the step before the last may be here before the products of last - 3, which have the same barrier, are done,
+        // and a wait by parity takes the phase before those for the last one)
+        if (ok && !at_wait_warp(at_smem(o_full), 0u)) ok = false;
         if (ok) {
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const float m_run = refs[(last & 1) * AT_QTILE + r];

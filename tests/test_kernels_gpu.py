@@ -520,6 +520,27 @@ def test_attention_prefill_tcgen05(K, nh, nkv, hd, lens, window, cached):
     assert float(err.max()) < PREFILL_ATTENTION_BOUND, (float(err.max()), int(err.argmax()), tok_row[int(err.argmax())], tok_pos[int(err.argmax())])
 
 
+@pytest.mark.parametrize("nh,nkv,hd", [(14, 2, 64), (16, 8, 128)])
+def test_attention_prefill_tcgen05_when_memory_is_slow(K, nh, nkv, hd):
+    """Cached prompts whose keys and values come from DRAM, call after call: the same bits every time."""
+    lens, g = [3000, 1100, 129, 4000] * 3, torch.Generator(device="cuda").manual_seed(hd)
+    pages = [(n + 63) // 64 for n in lens]
+    kp, vp = (torch.randn(sum(pages), nkv, 64, hd, generator=g, device="cuda").bfloat16() for _ in range(2))
+    order = torch.randperm(sum(pages), generator=g, device="cuda").tolist()
+    table = torch.tensor([[order.pop() for _ in range(n)] + [-1] * (max(pages) - n) for n in pages], dtype=torch.int32, device="cuda")
+    new = [min(100, n) for n in lens]
+    tiles = K.prefill_tiles(new, [n - m for n, m in zip(lens, new)], "cuda", K.PREFILL_TILE_TCGEN05)
+    q = torch.randn(sum(new), nh * hd, generator=g, device="cuda").bfloat16()
+    run = lambda: K.attention_prefill_tcgen05(q, nh * hd, nh, nkv, hd, kp, vp, table, table.shape[1], tiles, sum(new), None, hd ** -0.5)     # noqa: E731
+    flush, wrong, first = torch.empty(2 ** 28, dtype=torch.uint8, device="cuda"), torch.zeros((), device="cuda"), run()
+    assert torch.isfinite(first).all()
+    for _ in range(300):
+        flush.zero_()
+        wrong += (run() != first).any()
+    assert int(wrong) == 0
+    K.check_status("cuda")
+
+
 @pytest.mark.parametrize("kernel", ["generic_f32", "generic_bf16", "decode", "prefill", "prefill_tcgen05"])
 def test_attention_finds_a_far_key_and_respects_the_windows_edge(K, kernel):
     """One key among hundreds is made to dominate.  Without a window the output must be its
