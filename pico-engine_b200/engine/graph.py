@@ -288,7 +288,7 @@ class GraphedDecode:
                 held, pages = self.tables.fresh(g, every)
                 if len(pages) > pad:                     # only when sequences are new here: those go by a launch of their own, before the step's
                     self._many.append((g, np.concatenate([held, np.asarray(pages, dtype=np.int32)])))
-                    held = [1 if s == st.cache.idle_slot else len(st.cache.groups[g].table[s]) for s in every]
+                    held = [pages_for(start + 1) for start in starts]
                     pages = []
                 self.host[at: at + B] = held
                 self.host[at + pad: at + pad + len(pages)] = pages

@@ -27,8 +27,9 @@ class ResidentTables:
         return len(cache.groups) > 0 and all(g.need.window is None for g in cache.groups)
 
     def fresh(self, group: int, slots: Sequence[int]):
-        """(entries on the device of each row, the pages behind them in the rows' order) of a step whose pages have been reserved; they count as known
-        from now on."""
+        """(entries on the device of each row, the pages behind them in the rows' order) of a step of one token a row whose pages have been reserved; they
+        count as known from now on.  A row's entries go as far as the step's token: what the sequence holds beyond it (reserved ahead) is sent when
+        its positions reach there."""
         cache, table, known = self.cache, self.cache.groups[group].table, self.known[group]
         held, pages = np.empty(len(slots), dtype=np.int32), []
         for b, s in enumerate(slots):
@@ -40,7 +41,7 @@ class ResidentTables:
             if birth != cache.births[s]:
                 n = 0
             held[b] = n
-            if n < len(row):
-                pages.extend(row[n:])
-            known[s] = (cache.births[s], len(row))
+            need = pages_for(cache.lengths[s] + 1)
+            pages.extend(row[n:need])
+            known[s] = (cache.births[s], need)
         return held, pages
