@@ -171,8 +171,6 @@ class Stepper:
             empty_rows = 0
         T = sum(lens)
         W = sum(len(w) for w in want) + empty_rows
-        for s, n in zip(live, (n for s, n in zip(slots, lens) if s != cache.idle_slot)):
-            cache.reserve(s, n)
         if widths is None:
             widths = [max(pages_for(st + n) for st, n in zip(starts, lens))] * len(cache.groups)
         tile_rows = ([], [])
@@ -216,6 +214,8 @@ class Stepper:
                 w_at += 1
         if shared:
             host[lay.groups: lay.groups + 4 * B] = np.asarray(kernels.shared_group_rows(self.families(slots)), dtype=np.int32).reshape(-1)
+        for s, n in zip(live, (n for s, n in zip(slots, lens) if s != cache.idle_slot)):       # (behind every check: a refused step takes no pages)
+            cache.reserve(s, n)
         for g, off in enumerate(lay.tables):
             host[off: off + B * widths[g]] = cache.page_table(g, slots, widths[g]).reshape(-1)
         return lay, host, starts
