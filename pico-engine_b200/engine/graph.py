@@ -279,13 +279,14 @@ class GraphedDecode:
                 self.host[ids + self.bias_room: ids + self.bias_room + many].view(np.float32)[:] = [v for _, v in p.logit_bias]
         self.host[self.settings_at: self.settings_at + 6] = kernels.sample_settings_words(
             p.temperature if p.temperature > 0 else 1.0, p.top_k, p.top_p, p.seed)
-        self._many = []
-        if self.tables is not None:                      # (last: from here on the device is taken to know these pages)
+        self._many, self._learned = [], []
+        if self.tables is not None:
             at = self.place_at
             self.host[at: at + B] = starts
             for g in range(len(self.widths)):
                 at = self.place_at + (1 + 2 * g) * pad
-                held, pages = self.tables.fresh(g, every)
+                held, pages, learned = self.tables.fresh(g, every)
+                self._learned.append((g, learned))
                 if len(pages) > pad:                     # only when sequences are new here: those go by a launch of their own, before the step's
                     self._many.append((g, np.concatenate([held, np.asarray(pages, dtype=np.int32)])))
                     held = [pages_for(start + 1) for start in starts]
@@ -369,6 +370,8 @@ class GraphedDecode:
             self.graph.replay()
         else:
             self._forward()
+        for g, learned in self._learned:
+            self.tables.learn(g, learned)
         for s in slots:
             self.stepper.cache.advance(s, 1)
         return self.loop.read_back(len(slots))

@@ -27,11 +27,11 @@ class ResidentTables:
         return len(cache.groups) > 0 and all(g.need.window is None for g in cache.groups)
 
     def fresh(self, group: int, slots: Sequence[int]):
-        """(entries on the device of each row, the pages behind them in the rows' order) of a step of one token a row whose pages have been reserved; they
-        count as known from now on.  A row's entries go as far as the step's token: what the sequence holds beyond it (reserved ahead) is sent when
-        its positions reach there."""
+        """(entries on the device of each row, the pages behind them in the rows' order, what the device knows when they are there: for ``learn``) of a step of
+        one token a row whose pages have been reserved.  A row's entries go as far as the step's token: what the sequence holds beyond it (reserved ahead) is
+        sent when its positions reach there."""
         cache, table, known = self.cache, self.cache.groups[group].table, self.known[group]
-        held, pages = np.empty(len(slots), dtype=np.int32), []
+        held, pages, learned = np.empty(len(slots), dtype=np.int32), [], {}
         for b, s in enumerate(slots):
             if s == cache.idle_slot:
                 held[b] = 1
@@ -42,6 +42,11 @@ class ResidentTables:
                 n = 0
             held[b] = n
             need = pages_for(cache.lengths[s] + 1)
-            pages.extend(row[n:need])
-            known[s] = (cache.births[s], need)
-        return held, pages
+            if n < need:
+                pages.extend(row[n:need])
+                learned[s] = (cache.births[s], need)
+        return held, pages, learned
+
+    def learn(self, group: int, learned: Dict[int, Tuple[int, int]]) -> None:
+        """The step that ``fresh`` described has been launched: its pages need not be sent again.  (One that failed before is described anew.)"""
+        self.known[group].update(learned)

@@ -1,8 +1,6 @@
 """The page tables that stay on the device (CPU): what a step sends for them, laid out as the kernel does it, is what the cache holds."""
 import random
-import types
 
-import pytest
 import torch
 
 from pico_engine.cache import Cache, CacheNeeds, KVNeed, PAGE, pages_for
@@ -32,9 +30,10 @@ def step(tables, cache, slots):
     for s in slots:
         cache.reserve(s, 1)
     for g in range(len(cache.groups)):
-        held, pages = tables.fresh(g, slots)
+        held, pages, learned = tables.fresh(g, slots)
         got = lay_out(tables.tables[g], slots, [cache.length(s) for s in slots], held, pages)
         assert got == [cache.groups[g].table[s][:pages_for(cache.length(s) + 1)] for s in slots]
+        tables.learn(g, learned)
     for s in slots:
         cache.advance(s, 1)
 
@@ -54,6 +53,20 @@ def test_a_sequence_that_holds_more_pages_than_a_step_needs():
     b = cache.open()
     cache.reserve(b, 130)
     step(tables, cache, [b, a, c])
+
+
+def test_a_step_that_is_not_launched_teaches_the_device_nothing():
+    """Until its step has been launched, a page is sent again."""
+    cache = cache_of()
+    tables = ResidentTables(cache, 512)
+    a, b = cache.open(), cache.open()
+    step(tables, cache, [b])
+    cache.reserve(a, 1)
+    first = tables.fresh(0, [a, b, cache.idle_slot])
+    again = tables.fresh(0, [a, b, cache.idle_slot])
+    assert first[0].tolist() == again[0].tolist() == [0, 1, 1] and first[1] == again[1] == cache.groups[0].table[a] and first[2] == again[2]
+    tables.learn(0, first[2])
+    assert tables.fresh(0, [a, b])[1] == []
 
 
 def test_sequences_that_come_go_fork_and_reserve_ahead():

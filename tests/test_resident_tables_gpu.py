@@ -58,3 +58,33 @@ def test_steps_of_sequences_with_pages_reserved_ahead(eng, monkeypatch):
     want = answers(eng, False)
     monkeypatch.setattr(graph_module, "RESIDENT_ROWS", 4)
     assert answers(eng, True) == want
+
+
+@torch.inference_mode()
+def test_a_launch_that_fails_can_be_made_again(eng, monkeypatch):
+    """The description of a step does not reach the device: the next launch sends its pages again."""
+    eng.ensure_cache(4096, 480, 8)
+    cache, st = eng.cache, eng.stepper
+    prompts = [[7] * 70, [8] * 3, [9] * 64, [5]]
+    g = graph_module.GraphedDecode(st, Sampler(SamplingParams(temperature=0.0)), 4)
+    plainly, got = st.upload, []
+    for fails in (False, True):
+        slots = [cache.open() for _ in prompts]
+        try:
+            st.step(slots, prompts)
+            tokens, seen = [1, 2, 3, 4], []
+            for i in range(66):
+                if fails and i in (0, 5, 58, 60, 63):
+                    def broken(host, dev=None):
+                        raise MemoryError
+                    monkeypatch.setattr(st, "upload", broken)
+                    with pytest.raises(MemoryError):
+                        g.launch(slots, tokens, [0] * 4, [0] * 4)
+                    monkeypatch.setattr(st, "upload", plainly)
+                tokens = g.launch(slots, tokens, [0] * 4, [0] * 4).tokens()
+                seen.append(list(tokens))
+            got.append(seen)
+        finally:
+            for s in slots:
+                cache.close(s)
+    assert got[0] == got[1]
