@@ -375,7 +375,8 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
             z.step(p, deal);
         }
     }
-    const bool has_shared = begin < min(end, units), has_own = own_cta >= 0 && own_cta < own_runs.ctas;       // (the first worker's run comes first)
+    // (the first worker's run comes first; where no row has an own page, the first of these CTAs is there for the plan)
+    const bool has_shared = begin < min(end, units), has_own = own_cta >= 0 && own_cta < max(own_runs.ctas, 1);
     if (!has_shared && warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base_s), "r"(512u) : "memory");
     if (!has_shared && !has_own) {                                  // (the whole block)
         pdl_wait();
@@ -414,14 +415,18 @@ __global__ void __launch_bounds__(AS_THREADS, 1) attention_shared_kernel(const _
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(AS_REGS_SERVE));
     if (warp == 0 && has_own) {                                     // ---------------- the plan of the join, while the workers read
         pdl_wait();                                                 // (scratch is written)
-        const int all = p.T * p.nkv * p.own_tiles, ctas = min(own_ctas, own_runs.ctas);
+        const int all = p.T * p.nkv * p.own_tiles, ctas = min(own_ctas, max(own_runs.ctas, 1));
         for (int e = own_cta * 32 + lane; e < all; e += ctas * 32) {
             const int tok = e / (p.nkv * p.own_tiles), of = e - tok * (p.nkv * p.own_tiles), kvh = of / p.own_tiles, tile = of - kvh * p.own_tiles;
             const int4 g = p.groups[tok];
             AsOwn row;
             row.set(p, tok, g);
-            const int first = own_at[tok] + of * row.pages.n, o0 = own_runs.cta_of(first);
-            const int on = min(own_runs.cta_of(first + row.pages.n - 1) + 1 - o0, AS_MOST_OWN + 2);       // (more only for positions behind max_context)
+            int o0 = 0, on = 0;
+            if (row.pages.n > 0) {                                  // (none: the window of a position beyond the table has left all of its pages behind)
+                const int first = own_at[tok] + of * row.pages.n;
+                o0 = own_runs.cta_of(first);
+                on = min(own_runs.cta_of(first + row.pages.n - 1) + 1 - o0, AS_MOST_OWN + 2);      // (more only for positions behind max_context)
+            }
             int c0 = 0, n = 0, at = 0;
             const int shared = as_shared(g, tok, p.T, p.table_stride);
             AsPages pages = {0, 0, 0};
