@@ -19,7 +19,7 @@
 
 #define LR_THREADS 256
 #define LR_CHUNK (LR_THREADS * 8)                   // tokens of a block: eight a thread (with sixteen, and so fewer blocks an SM, 64 rows with penalties took 23 us instead of 19)
-#define LR_LIST 512                                 // entries of a list of biases that a block looks at in one turn
+#define LR_LIST 512                                 // entries of a list of biases that a block takes in one turn
 
 struct LrArgs {
     const float* logits; float* out; int rows, vocab;
@@ -110,66 +110,200 @@ __global__ void __launch_bounds__(LR_THREADS, 8) adjust_logits_kernel(const LrAr
     }
 }
 
-// out += the row's biases, where the mask allows the token: a block a row, LR_LIST entries of its list a turn.  The first entry of a token adds all of the turn's, in
-// the list's order, so that no sum depends on which thread comes first.  A table in shared memory tells which entry is a token's first and whether
-// there are others; only then is the turn's list read through (by every entry it took 11 us for 64 lists of 300).
+// out += the row's biases, where the mask allows the token: a block a row.  Biases of a token that stands in the list several times are added up first: by its
+// first entry, in the list's order, so that no sum depends on which thread comes first.  How those are found goes by the length of the row's list:
+//   up to LR_LIST entries   a table in shared memory tells which entry is a token's first and whether there are others; only then is the list read through
+//                           (by every entry it took 11 us for 64 lists of 300)
+//   more                    lr_long_list
+// LONG: lists may be longer than LR_LIST (the second way takes more shared memory).
+#define LR_BITS (1 << 17)
+
+__device__ __forceinline__ bool lr_allows(const unsigned* mask, int id) { return !mask || ((mask[id >> 5] >> (id & 31)) & 1u); }
+
+// A list of any length.  A bit a token (of LR_BITS at a time) tells which ones come twice.  The others add what they have.  Those go, LR_LIST entries a turn, into a
+// table; each turn behind adds to their sums what it has of them, and a token whose sum is complete loses its bit, so that its other entries are passed over.
+// 64 lists, of 151,936 tokens: 600 each 16 us, 4,096 each 55 us, 119 us where every token comes twice, half a list apart.  (Turn by turn onto the logit, which lost
+// what cancels between turns, 15, 56 and 53 us; inlined, since with a call the kernel took 0.5 us longer for short lists too.)
+__device__ __forceinline__ void lr_long_list(const LrArgs& p, int first, int last, const unsigned* mask, float* out, int* table, int* ids, float* values, unsigned* twice) {
+    constexpr int PER = LR_LIST / LR_THREADS, PLACES = 2 * LR_LIST;
+    static_assert(4 * PLACES == LR_BITS / 32, "the first of a token's two bits lies where the table comes");
+    unsigned* once = reinterpret_cast<unsigned*>(table);
+    int *token = table, *owner = table + PLACES, *lead = table + 2 * PLACES, *count = table + 3 * PLACES;
+    constexpr int NONE = 0x7fffffff;
+    for (int id0 = 0; id0 < p.vocab; id0 += LR_BITS) {
+        const unsigned here = min(LR_BITS, p.vocab - id0);
+        auto entry = [&](int e) {                                   // the token of entry e, or -1
+            const int id = e < last ? p.bias_ids[e] : -1;
+            return id >= id0 && (unsigned)(id - id0) < here ? id : -1;
+        };
+        auto comes_twice = [&](int id) { return ((twice[(id - id0) >> 5] >> (id & 31)) & 1u) != 0u; };
+        __syncthreads();
+        for (int i = threadIdx.x; i < LR_BITS / 32; i += LR_THREADS) once[i] = twice[i] = 0u;
+        __syncthreads();
+        bool some = false;
+#pragma unroll 4
+        for (int e = first + (int)threadIdx.x; e < last; e += LR_THREADS) {
+            const int id = entry(e);
+            if (id < 0) continue;
+            const unsigned bit = 1u << (id & 31);
+            if (atomicOr(&once[(id - id0) >> 5], bit) & bit) { atomicOr(&twice[(id - id0) >> 5], bit); some = true; }
+        }
+        some = __syncthreads_or(some);
+        if (id0 == 0) pdl_wait();
+#pragma unroll 4
+        for (int e = first + (int)threadIdx.x; e < last; e += LR_THREADS) {
+            const int id = entry(e);
+            if (id >= 0 && !comes_twice(id) && lr_allows(mask, id)) out[id] += p.bias_values[e];
+        }
+        if (!some) continue;
+        for (int turn = first; turn < last; turn += LR_LIST) {
+            // ---- the turn's tokens that are not done, and what the turn itself has of them: values[i] becomes the sum of the token whose first entry is i
+            int id[PER], place[PER];
+            bool mine = false, is_first[PER];
+            __syncthreads();                                        // (the turn before has taken its tokens' bits)
+            for (int i = threadIdx.x; i < PLACES; i += LR_THREADS) { token[i] = -1; owner[i] = lead[i] = NONE; count[i] = 0; }
+#pragma unroll
+            for (int k = 0; k < PER; ++k) {
+                const int i = k * LR_THREADS + threadIdx.x;
+                id[k] = i < last - turn ? entry(turn + i) : -1;
+                if (id[k] >= 0 && !(comes_twice(id[k]) && lr_allows(mask, id[k]))) id[k] = -1;
+                ids[i] = id[k];
+                values[i] = id[k] >= 0 ? p.bias_values[turn + i] : 0.f;
+                mine |= id[k] >= 0;
+            }
+            if (!__syncthreads_or(mine)) continue;
+            auto home = [](int x) { return ((unsigned)x * 2654435761u) >> 20 & (PLACES - 1); };
+#pragma unroll
+            for (int k = 0; k < PER; ++k) {
+                if (id[k] < 0) continue;
+                unsigned at = home(id[k]);
+                for (;;) {
+                    const int there = atomicCAS(&token[at], -1, id[k]);
+                    if (there == -1 || there == id[k]) break;
+                    at = (at + 1) & (PLACES - 1);
+                }
+                place[k] = at;
+                atomicMin(&owner[at], k * LR_THREADS + (int)threadIdx.x);
+                atomicAdd(&count[at], 1);
+            }
+            __syncthreads();
+            float sum[PER];
+#pragma unroll
+            for (int k = 0; k < PER; ++k) {
+                const int i = k * LR_THREADS + threadIdx.x;
+                is_first[k] = id[k] >= 0 && owner[place[k]] == i;
+                if (!is_first[k]) continue;
+                sum[k] = values[i];
+                for (int j = i + 1, left = count[place[k]] - 1; left > 0; ++j)
+                    if (ids[j] == id[k]) { sum[k] += values[j]; --left; }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < PER; ++k)
+                if (is_first[k]) { values[k * LR_THREADS + threadIdx.x] = sum[k]; count[place[k]] = 0; }
+            // ---- the turns behind, one after the other
+            for (int then = turn + LR_LIST; then < last; then += LR_LIST) {
+                int found[PER];
+                bool any = false;
+                __syncthreads();
+#pragma unroll
+                for (int k = 0; k < PER; ++k) {
+                    const int e = then + k * LR_THREADS + (int)threadIdx.x, x = entry(e);
+                    found[k] = -1;
+                    if (x < 0 || !comes_twice(x)) continue;
+                    for (unsigned at = home(x); token[at] != -1; at = (at + 1) & (PLACES - 1))
+                        if (token[at] == x) { found[k] = at; break; }
+                    if (found[k] < 0) continue;
+                    any = true;
+                    atomicMin(&lead[found[k]], e);
+                    atomicAdd(&count[found[k]], 1);
+                }
+                if (!__syncthreads_or(any)) continue;
+#pragma unroll
+                for (int k = 0; k < PER; ++k) {                     // the token's first entry of this turn adds all of them
+                    const int e = then + k * LR_THREADS + (int)threadIdx.x;
+                    if (found[k] < 0 || lead[found[k]] != e) { found[k] = -1; continue; }
+                    const int x = token[found[k]];
+                    float add = values[owner[found[k]]] + p.bias_values[e];
+                    for (int j = e + 1, left = count[found[k]] - 1; left > 0; ++j)
+                        if (p.bias_ids[j] == x) { add += p.bias_values[j]; --left; }
+                    values[owner[found[k]]] = add;
+                }
+                __syncthreads();
+#pragma unroll
+                for (int k = 0; k < PER; ++k)
+                    if (found[k] >= 0) { lead[found[k]] = NONE; count[found[k]] = 0; }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < PER; ++k) {
+                if (!is_first[k]) continue;
+                out[id[k]] += values[k * LR_THREADS + threadIdx.x];
+                atomicAnd(&twice[(id[k] - id0) >> 5], ~(1u << (id[k] & 31)));
+            }
+        }
+    }
+}
+
+template <bool LONG>
 __global__ void __launch_bounds__(LR_THREADS) add_biases_kernel(const LrArgs p) {
     constexpr int PER = LR_LIST / LR_THREADS, PLACES = 4 * LR_LIST;      // entries of a thread; places of the table, most of them empty
-    __shared__ int ids[LR_LIST], token[PLACES], first_of[PLACES], count[PLACES];
+    __shared__ int ids[LR_LIST], table[3 * PLACES];
     __shared__ float values[LR_LIST];
+    int *token = table, *first_of = table + PLACES, *count = table + 2 * PLACES;
     pdl_launch_dependents();
-    for (int i = threadIdx.x; i < PLACES; i += LR_THREADS) { token[i] = -1; first_of[i] = LR_LIST; count[i] = 0; }
     // Lists and masks were there before the first kernel began to work; the wait is for its results.
     const int b = blockIdx.x, m = p.by_slot ? lr_mask(p, p.slots[b], p.n_slots) : lr_mask(p, b, p.rows);
     const int2 list = p.bias_range[b];
-    const int first = max(list.x, 0), last = min(list.y, p.n_bias);
+    const int last = max(min(list.y, p.n_bias), 0), first = min(max(list.x, 0), last);
     const unsigned* mask = m >= 0 && m < p.n_masks ? p.masks + (size_t)m * p.mask_words : nullptr;
     float* out = p.out + (size_t)b * p.vocab;
-    for (int base = first; base < last; base += LR_LIST) {
-        int id[PER], place[PER];
-        float now[PER];
-#pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            const int e = k * LR_THREADS + threadIdx.x;
-            id[k] = base + e < last ? p.bias_ids[base + e] : -1;
-            values[e] = base + e < last ? p.bias_values[base + e] : 0.f;
-            if (id[k] >= p.vocab) id[k] = -1;
-            ids[e] = id[k];
-        }
-        __syncthreads();                                            // (the table is empty, and the turn before has written)
-#pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            if (id[k] < 0) continue;
-            if (mask && !((mask[id[k] >> 5] >> (id[k] & 31)) & 1u)) { id[k] = -1; continue; }
-            unsigned at = ((unsigned)id[k] * 2654435761u) >> 20 & (PLACES - 1);
-            for (;;) {
-                const int there = atomicCAS(&token[at], -1, id[k]);
-                if (there == -1 || there == id[k]) break;
-                at = (at + 1) & (PLACES - 1);
-            }
-            place[k] = at;
-            atomicMin(&first_of[at], k * LR_THREADS + (int)threadIdx.x);
-            atomicAdd(&count[at], 1);
-        }
-        if (base == first) pdl_wait();
-#pragma unroll
-        for (int k = 0; k < PER; ++k) now[k] = id[k] >= 0 ? out[id[k]] : 0.f;
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            const int e = k * LR_THREADS + threadIdx.x;
-            if (id[k] < 0 || first_of[place[k]] != e) continue;
-            float sum = values[e];
-            for (int i = e + 1, left = count[place[k]] - 1; left > 0; ++i)
-                if (ids[i] == id[k]) { sum += values[i]; --left; }
-            out[id[k]] = now[k] + sum;
-        }
-        if (base + LR_LIST < last) {                                // empty the table for the next turn
-            __syncthreads();
-            for (int i = threadIdx.x; i < PLACES; i += LR_THREADS) { token[i] = -1; first_of[i] = LR_LIST; count[i] = 0; }
+    if constexpr (LONG) {
+        __shared__ unsigned twice[LR_BITS / 32];
+        if (last - first > LR_LIST) {                               // (the whole block)
+            lr_long_list(p, first, last, mask, out, table, ids, values, twice);
+            return;
         }
     }
-    if (first >= last) pdl_wait();                                  // (the kernel behind this one counts on the first one's end as well)
+    for (int i = threadIdx.x; i < PLACES; i += LR_THREADS) { token[i] = -1; first_of[i] = LR_LIST; count[i] = 0; }
+    int id[PER], place[PER];
+    float now[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int e = k * LR_THREADS + threadIdx.x;
+        id[k] = e < last - first ? p.bias_ids[first + e] : -1;
+        values[e] = e < last - first ? p.bias_values[first + e] : 0.f;
+        if (id[k] >= p.vocab) id[k] = -1;
+        ids[e] = id[k];
+    }
+    __syncthreads();                                                // (the table is empty)
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        if (id[k] < 0) continue;
+        if (!lr_allows(mask, id[k])) { id[k] = -1; continue; }
+        unsigned at = ((unsigned)id[k] * 2654435761u) >> 20 & (PLACES - 1);
+        for (;;) {
+            const int there = atomicCAS(&token[at], -1, id[k]);
+            if (there == -1 || there == id[k]) break;
+            at = (at + 1) & (PLACES - 1);
+        }
+        place[k] = at;
+        atomicMin(&first_of[at], k * LR_THREADS + (int)threadIdx.x);
+        atomicAdd(&count[at], 1);
+    }
+    pdl_wait();                                                     // (also where the list is empty: the kernel behind this one counts on the first one's end)
+#pragma unroll
+    for (int k = 0; k < PER; ++k) now[k] = id[k] >= 0 ? out[id[k]] : 0.f;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int e = k * LR_THREADS + threadIdx.x;
+        if (id[k] < 0 || first_of[place[k]] != e) continue;
+        float sum = values[e];
+        for (int i = e + 1, left = count[place[k]] - 1; left > 0; ++i)
+            if (ids[i] == id[k]) { sum += values[i]; --left; }
+        out[id[k]] = now[k] + sum;
+    }
 }
 
 // Tokens into the table of what a sequence has seen.  prompt: their sign bits are set; else their counts go up by one, to 32,767 at most.
@@ -228,7 +362,7 @@ extern "C" int pe_adjust_logits(const float* logits, float* out, int rows, int v
     PE_TRY(pe_launch(kernel, dim3((vocab + LR_CHUNK - 1) / LR_CHUNK, rows), LR_THREADS, 0, (cudaStream_t)stream, p));
     PE_LAUNCH_CHECK();
     if (bias_ids) {
-        PE_TRY(pe_launch(add_biases_kernel, rows, LR_THREADS, 0, (cudaStream_t)stream, p));
+        PE_TRY(pe_launch(n_bias > LR_LIST ? add_biases_kernel<true> : add_biases_kernel<false>, rows, LR_THREADS, 0, (cudaStream_t)stream, p));
         PE_LAUNCH_CHECK();
     }
     return 0;

@@ -2006,7 +2006,7 @@ def adjust_logits(logits: torch.Tensor, slots: Optional[torch.Tensor] = None, hi
     the sign bit of an entry says that the token stands in the prompt, the other 15 bits how often it has been generated (``note_tokens``).
     Seen tokens' logits are divided by the repetition penalty where positive and multiplied by it elsewhere; generated ones lose
     presence + count * frequency.  ``bias_range`` int32 [B, 2]: from where to where row b's biases lie in ``bias_ids`` (int32) and ``bias_values``
-    (float32); a token that stands there twice gets both.  ``masks`` int32 [M, ceil(V / 32)] with ``mask_rows`` int32 [B]: where bit v % 32 of word
+    (float32); those of a token that stands there several times are added up first, in the list's order.  ``masks`` int32 [M, ceil(V / 32)] with ``mask_rows`` int32 [B]: where bit v % 32 of word
     v / 32 of row b's mask is 0, the logit becomes -inf, whatever it was; -1: no mask.  A row that its mask leaves nothing is -inf everywhere.
     ``states`` int32 [n] stands in the place of ``mask_rows`` where the masks are those of an automaton's states (``note_tokens``): row b's mask is
     that of ``states[slots[b]]``."""

@@ -1,4 +1,4 @@
-"""Attention over shared pages where it can go wrong unseen: beside tests/test_answers_gpu.py, whose cases and oracle these use.
+"""Attention over shared pages and rules on logits where they can go wrong unseen: beside tests/test_answers_gpu.py, whose cases and oracle these use.
 
 Attention over many keys, by rows: an entry's bound of 2^-8 of sum p |v| is far above a result in which random values cancel.  The roundings of the probabilities do
 not hang together: an error sum_j d_j p_j v_j with |d_j| <= 2^-8 (half a step of bfloat16, each its own) has a root mean square of 2^-8 sqrt(sum p^2 v^2) at most, the result's
@@ -7,7 +7,7 @@ the two; uniform roundings come to 0.29 of it, and a page of 64 keys left out to
 import pytest
 import torch
 
-from test_answers_gpu import Answers, K, agree, ints      # noqa: F401  (K: the fixture)
+from test_answers_gpu import Answers, K, adjust, agree, gen, ints, rules_case, rules_want      # noqa: F401  (K: the fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -117,3 +117,33 @@ def test_pages_read_early_or_late_are_the_same(K, hd, window, keep, sinks, slope
         agree(got[1], *a.want(window, keep, sinks, slopes))
         assert torch.equal(*got)
     K.check_status("cuda")
+
+
+# ---------------------------------------------------------------------------- rules
+
+@pytest.mark.parametrize("apart", [1, 100, 511, 512, 513, 1500, 4000])
+def test_biases_of_a_token_are_added_up_before_they_meet_its_logit(K, apart):
+    """Two that cancel leave the logit as it was, and the third alone counts, however far apart they stand in the list; so do masks and rows beside them."""
+    V, n = 140000, apart + 700
+    c = rules_case(3, V, seed=4, history=False, masks=False)
+    ids = torch.randperm(V - 10, generator=gen(1), device="cuda")[:n].int()
+    values = torch.randn(n, generator=gen(2), device="cuda")
+    ids[::7] = (ids[::7].long() % 400 + 131072).int()                    # (tokens that lie 131,072 above others of the list)
+    first = 20
+    ids[[first, first + apart, first + apart + 600]] = V - 3
+    values[first], values[first + apart], values[first + apart + 600] = 1e8, -1e8, 0.25
+    c["bias_ids"], c["bias_values"], c["bias_range"] = ids, values, ints([[0, n], [0, first + apart + 300], [first + 1, n]])
+    c["masks"], c["mask_rows"] = torch.full((1, (V + 31) // 32), -1, dtype=torch.int32, device="cuda"), ints([-1, 0, -1])
+    got = adjust(K, c)
+    x = c["logits"][:, V - 3]
+    assert got[0, V - 3] == x[0] + 0.25 and got[1, V - 3] == x[1] and got[2, V - 3] == x[2] + (torch.tensor(-1e8, device="cuda") + 0.25)
+    c.pop("masks"), c.pop("mask_rows")
+    want, size = rules_want(c)
+    others = torch.ones(V, dtype=torch.bool, device="cuda")
+    others[V - 3] = False
+    # of the others no token stands there more than 20 times
+    times = torch.bincount(ids.long(), minlength=V)
+    assert int(times[others].max()) <= 20
+    assert bool(((got.double() - want).abs() <= 22 * 2.0 ** -24 * size)[:, others].all())
+    for _ in range(3):
+        assert torch.equal(adjust(K, c), got)
