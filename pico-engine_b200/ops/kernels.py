@@ -1928,6 +1928,14 @@ def sharing_pays(saved_bytes: int) -> bool:
     return saved_bytes >= SHARING_PAYS_BYTES
 
 
+def shared_bytes_at_most(rows: int, n_kv_heads: int, head_dim: int, max_context: int, window: Optional[int] = None, keep_first: int = 0) -> int:
+    """The bytes of keys and values that so many rows would not read again if all of them shared all that they see (bfloat16).  One by one against
+    together under a window, 64 rows on 8,192 positions, us: 14 heads of 64, a window of 100 (3 MB) 5.2 and 14.1, of 2,000 (65 MB) 12.5 and 11.3; 28 heads of 128, of 100 (13 MB) 9.3
+    and 17.8, of 400 (52 MB) 15.1 and 16.6, of 1,000 (129 MB) 23.9 and 17.1."""
+    seen = min(max_context, window + keep_first) if window else max_context
+    return 4 * max(rows - 1, 0) * seen * n_kv_heads * head_dim
+
+
 def shared_group_rows(members):
     """``groups`` of ``attention_shared`` for the rows of a step, on the host: ``members`` lists (tokens, shared positions, which of them
     has the least position) group after group, in the order of the rows; a row on its own is (1, 0, 0)."""
@@ -1981,7 +1989,7 @@ def attention_shared(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: i
     if T == 0:
         return out
     lib = for_head_dim(head_dim)
-    if not (sharing_pays(4 * T * max_context * n_kv_heads * head_dim) if together is None else together):
+    if not (sharing_pays(shared_bytes_at_most(T, n_kv_heads, head_dim, max_context, window, keep_first)) if together is None else together):
         check(lib.pe_attention_decode(q.data_ptr(), q_stride, out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(), table_stride,
                                       tok_pos.data_ptr(), tok_row.data_ptr(), T, n_heads, n_kv_heads, head_dim, window or 0, scale, max_context,
                                       1 if early_pages else 0, status_ptr(q.device), stream, keep_first if window else 0, _ptr(slopes), _ptr(sinks)),

@@ -115,3 +115,15 @@ def test_step_tables_refuses(change, what):
              places=i32(7), tables=i32(3, 5))
     a.update(change)
     refused(lambda: K.step_tables(**a), what)
+
+
+# ---------------------------------------------------------------------------- whether rows are read together
+
+def test_shared_bytes_at_most():
+    """What rows do not read again: nothing of one row, of others what the first reads, which a window and its kept keys bound."""
+    assert K.shared_bytes_at_most(1, 2, 64, 10 ** 6) == 0 == K.shared_bytes_at_most(0, 2, 64, 10 ** 6)
+    assert K.shared_bytes_at_most(16, 2, 64, 4096) == 15 * 4096 * 2 * 64 * 4
+    assert K.shared_bytes_at_most(64, 4, 128, 30000, 100) == K.shared_bytes_at_most(64, 4, 128, 100) == 63 * 100 * 4 * 128 * 4
+    assert K.shared_bytes_at_most(64, 4, 128, 30000, 100, 4) == 63 * 104 * 4 * 128 * 4
+    assert K.shared_bytes_at_most(64, 4, 128, 90, 100, 4) == K.shared_bytes_at_most(64, 4, 128, 90) == K.shared_bytes_at_most(64, 4, 128, 90, 0, 4)
+    assert not K.sharing_pays(K.shared_bytes_at_most(64, 4, 128, 30000, 100)) and K.sharing_pays(K.shared_bytes_at_most(64, 4, 128, 30000))

@@ -119,6 +119,19 @@ def test_pages_read_early_or_late_are_the_same(K, hd, window, keep, sinks, slope
     K.check_status("cuda")
 
 
+def test_a_direct_call_chooses_by_what_its_window_lets_rows_share(K):
+    """Left to choose, a call reads rows one by one where a window leaves little to share, however long the context, and where it has one row."""
+    a = Answers(14, 2, 64, [(640, [1, 30, 64, 65, 200]), (64, [5, 6])], seed=3)
+    for window, keep in ((100, 0), (100, 70)):
+        got = a.run(K, window, keep, bound=30000, together=None)
+        assert torch.equal(got, a.run(K, window, keep, bound=30000, together=False))
+        agree(got, *a.want(window, keep))
+    assert torch.equal(a.run(K, bound=30000, together=None), a.run(K, bound=30000))
+    b = Answers(14, 2, 64, [(4096, [9])], seed=4)
+    assert torch.equal(b.run(K, bound=10 ** 6, together=None), b.run(K, bound=10 ** 6, together=False))
+    K.check_status("cuda")
+
+
 # ---------------------------------------------------------------------------- rules
 
 @pytest.mark.parametrize("apart", [1, 100, 511, 512, 513, 1500, 4000])
