@@ -32,7 +32,7 @@ class TokenAutomaton:
         stuck = (t < 0).all(dim=1)
         if bool(stuck.any()):
             raise ValueError(f"state {int(stuck.nonzero()[0])} allows no token")
-        self.transitions, self.start = t.to(torch.int32).contiguous(), int(start)
+        self.transitions, self.start = t.to(torch.int32, copy=True).contiguous(), int(start)      # (its own: the caller may use the array again)
         self._on: Dict[torch.device, Tuple[torch.Tensor, torch.Tensor]] = {}
 
     @property
