@@ -197,7 +197,7 @@ class EngineBackend:
             logits = logits[torch.tensor(rows, device=logits.device)]
             chosen = self.sampler.choose(logits, self._int32(i for r in requests for i in r), self._int32([0] * len(rows)),
                                          rules=self._rules(everyone)).tolist()
-        except Exception:
+        except BaseException:                            # (a call that is broken off as well: the caller knows the first slots only)
             for more in further:
                 for s in more:
                     self.e.cache.close(s)
