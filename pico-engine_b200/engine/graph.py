@@ -330,15 +330,18 @@ class GraphedDecode:
         seen = self.rules.memory.snapshot(self._slots) if self.rules is not None else None
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
-        with torch.cuda.stream(side):
-            for _ in range(3):
-                self.loop.chosen.copy_(keep)
-                self._forward()
-            self.stepper.cache.restore_state(state)
-            if seen is not None:
-                self.rules.memory.restore(seen)
-        torch.cuda.current_stream().wait_stream(side)
-        self.loop.chosen.copy_(keep)
+        try:
+            with torch.cuda.stream(side):
+                for _ in range(3):
+                    self.loop.chosen.copy_(keep)
+                    self._forward()
+        finally:                                         # (also where a trial run fails: the step itself follows, kernel by kernel)
+            with torch.cuda.stream(side):
+                self.stepper.cache.restore_state(state)
+                if seen is not None:
+                    self.rules.memory.restore(seen)
+            torch.cuda.current_stream().wait_stream(side)
+            self.loop.chosen.copy_(keep)
         graph = torch.cuda.CUDAGraph()
         with _collector_paused(), torch.cuda.graph(graph):
             self._forward()
