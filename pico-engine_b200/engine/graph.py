@@ -152,10 +152,13 @@ class GraphedPrompt:
                 state = cache.snapshot_state()            # the trial runs must not advance a mixer's state (see GraphedDecode)
                 side = torch.cuda.Stream()
                 side.wait_stream(torch.cuda.current_stream())
-                with torch.cuda.stream(side):
-                    self._forward(ctx)                    # (the step ran kernel by kernel before: everything lazy is set up)
-                    cache.restore_state(state)
-                torch.cuda.current_stream().wait_stream(side)
+                try:
+                    with torch.cuda.stream(side):
+                        self._forward(ctx)                # (the step ran kernel by kernel before: everything lazy is set up)
+                finally:
+                    with torch.cuda.stream(side):
+                        cache.restore_state(state)
+                    torch.cuda.current_stream().wait_stream(side)
                 graph = torch.cuda.CUDAGraph()
                 with _collector_paused(), torch.cuda.graph(graph, pool=self.pool):
                     self._forward(ctx)

@@ -1,4 +1,4 @@
-"""A captured decode step whose trial runs fail: the step runs kernel by kernel instead, from where it would have started."""
+"""A captured step whose trial runs fail: the step runs kernel by kernel instead, from where it would have started."""
 import warnings
 
 import pytest
@@ -41,3 +41,24 @@ def test_a_trial_run_that_fails_leaves_no_trace(tmp_path, monkeypatch, name, fai
         got = eng.generate(prompts, use_graph=True, **kw)
     assert got == want
     assert any("no room" in str(w.message) for w in said) and all(g.graph is None for g in eng._graphs.values()) and len(runs) >= 3
+
+
+def test_a_prompts_trial_run_that_fails_leaves_no_trace(tmp_path, monkeypatch):
+    from pico_engine.engine.engine import Engine
+    cfg = kevelorn_models.CONFIGS["K1"]
+    eng = Engine(write_model(tmp_path / "m", dict(cfg), kevelorn_models.make_weights(cfg, 40, 8)), dtype="float32")
+    assert eng.model.cache_needs() and any(n is not None and n.state_elems for n in eng.model.cache_needs())
+    prompts = [[5, 6, 7, 8, 9, 10, 11] * 4, [3, 1, 2]]
+    want = eng.generate(prompts, 10, temperature=0, stop_token_ids=())   # (the first prompt step of its sizes runs kernel by kernel)
+    plainly, broken = graph_module.GraphedPrompt._forward, []
+
+    def forward(self, ctx):
+        plainly(self, ctx)
+        if self.launches == 2 and not broken:
+            broken.append(self)
+            raise RuntimeError("no room for a trial run")
+    monkeypatch.setattr(graph_module.GraphedPrompt, "_forward", forward)
+    with pytest.warns(UserWarning, match="no room"):
+        assert eng.generate(prompts, 10, temperature=0, stop_token_ids=()) == want
+    assert broken and broken[0].graph is None
+    assert eng.generate(prompts, 10, temperature=0, stop_token_ids=()) == want
