@@ -24,7 +24,11 @@
 // steps of 1,365 each (their exponentials alone are 1,024; a polynomial on the multiply-add units in the place of a quarter of them made a step longer, since a
 // warp's instructions then are what it waits for), the end 4,000; the join's three fetches that depend on one another 4.3 us.  With few shared positions the own
 // pages are fetched at 3.8 TB/s once they have begun.  The computing warps keep a row's 128 scores in registers: with 168 a thread the masked variant spilled 500
-// bytes, and answers in a window took 25.2 us instead of 21.2.
+// bytes, and answers in a window took 25.2 us instead of 21.2 (40 to 68 bytes are spilled still).
+//
+// P is bfloat16 on both lines, since that is what the tensor cores multiply at their rate; a rounding is 2^-8 of a probability at most, of either sign, and the sums of weights
+// are of the unrounded ones.  With the reference point up to 2^AS_LAZY below the maximum the largest probabilities are rounded as well, where a maximum taken exactly makes them
+// 1: 0.0021 to 0.0023 of the outputs' size from the 64-bit result, row by row 0.0018.  How pages are dealt out goes by all rows of the call, so a row's bits depend on its neighbours.
 //
 // All keys of a shared step are visible to all rows but for windows, pages that are not there and the half step behind an odd number of pages,
 // so the masks are a variant of their own (MASKED).  Every wait is bounded; one that runs out sets *status to 7, and the roles leave their loops.

@@ -1919,7 +1919,8 @@ def attention_shared_takes(dtype: torch.dtype, rows: int, n_heads: int, n_kv_hea
 # Bytes of keys and values that a layer does not read again before reading shared pages together pays.  Read row by row they come from L2 at 8 to 13 TB/s; what
 # the second way costs is a longer start and its join.  Measured on a B200, one by one against together, us: 14 heads of 64, 16 rows on 2,048 positions
 # (16 MB) 8.0 and 9.4, on 4,032 (31 MB) 10.7 and 10.1, on 6,016 (46 MB) 13.2 and 11.5, 64 rows on 4,096 (132 MB) 20.9 and 16.3; 28 heads of 128, 8 rows on 3,200 (46 MB)
-# 12.4 and 14.0, on 4,096 (59 MB) 14.3 and 14.3, on 6,016 (86 MB) 18.5 and 16.2, 64 on 8,192 (1,057 MB) 144 and 28.4.
+# 12.4 and 14.0, on 4,096 (59 MB) 14.3 and 14.3, on 6,016 (86 MB) 18.5 and 16.2, 64 on 8,192 (1,057 MB) 144 and 28.4.  (One limit for both: heads of 64 would gain from
+# about 25 MB on, heads of 128 lose below 59.)
 SHARING_PAYS_BYTES = 50_000_000
 
 
@@ -1959,10 +1960,16 @@ def attention_shared(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: i
                      slopes: Optional[torch.Tensor] = None, sinks: Optional[torch.Tensor] = None, early_pages: bool = True,
                      together: Optional[bool] = None) -> torch.Tensor:
     """``attention_decode`` for single tokens of which several share the first pages of their sequences: those pages are read once for
-    all rows of a group (``together`` False: by every row; None: where ``sharing_pays`` for what the rows can share at most).  ``groups`` int32 [T, 4], a row a token (``shared_groups``): the first token of its group, how many consecutive tokens the
-    group has, how many positions they share (whole pages, no more than the least position of the group; 0: none), and which token has
-    the least position: its row of the page table names the shared pages.  Head sizes 64 and 128 (``attention_shared_takes``); results are
-    those of ``attention_decode`` up to the order of float32 sums."""
+    all rows of a group (``together`` False: by every row, with ``attention_decode``'s kernel; None: where ``sharing_pays`` for what so many rows could share at most,
+    ``shared_bytes_at_most``: what they do share is known on the device only, so a caller that knows says so).  ``groups`` int32 [T, 4], a row a token
+    (``shared_groups``): the first token of its group, how many consecutive tokens the group has, how many positions they share (whole pages, no more than the
+    least position of the group; 0: none), and which token has the least position: its row of the page table names the shared pages.  Head sizes 64 and 128
+    (``attention_shared_takes``).
+
+    Sums, maxima and weights are float32, the probabilities bfloat16 for the product with the values, as in ``attention_decode``, but over the shared pages relative to a
+    reference point up to 2^8 below the row's maximum, and in other partial sums: the two agree within roundings (0.0021 to 0.0023 of the outputs' size from the
+    64-bit result, ``attention_decode`` 0.0018, the result's own rounding 0.0017), and how a row's pages are dealt to partial sums depends on the other rows of the call.  A row
+    whose sum of weights is no number (a score of +inf or NaN) is no number here and zeros in ``attention_decode``."""
     T, pool = tok_pos.shape[0], k_pool.shape
     _need(q, "q", torch.bfloat16); _need(k_pool, "k_pool", torch.bfloat16); _need(v_pool, "v_pool", torch.bfloat16, pool)
     if not attention_shared_takes(torch.bfloat16, T, n_heads, n_kv_heads, head_dim, scale):
