@@ -11,7 +11,7 @@ from typing import Optional
 
 import torch
 
-from .library import DTYPE_CODE, KernelError, answers, check, core, extras, for_head_dim, gated, mixers, stream_ptr
+from .library import DTYPE_CODE, KernelError, answers, check, core, extras, for_head_dim, gated, long_context, mixers, stream_ptr
 
 PAGE = 64     # tokens per cache page; PE_PAGE in csrc/common.cuh
 
@@ -2123,3 +2123,226 @@ def step_tables(slots: torch.Tensor, starts: torch.Tensor, lens: torch.Tensor, h
                                    resident.data_ptr(), res[0], res[1], B, tok_pos.data_ptr(), tok_row.data_ptr(),
                                    row_first.data_ptr(), places.data_ptr(), T, tables.data_ptr(), table[1], stream), "step_tables")
     return tok_pos, tok_row, row_first, places, tables
+
+
+# ---------------------------------------------------------------------------- a long context's cache: 4-bit pages, and pages selected by their keys' bounds
+
+INT4_HEAD_DIMS = (64, 128)
+INT4_GROUP = 32               # channels that share a step and a middle
+
+
+def int4_takes(dtype: torch.dtype, n_heads: int, n_kv_heads: int, head_dim: int) -> bool:
+    """Whether attention of these heads can have its cache in 4 bits."""
+    return dtype == torch.bfloat16 and head_dim in INT4_HEAD_DIMS and n_kv_heads > 0 and n_heads % n_kv_heads == 0
+
+
+def int4_page_bytes(head_dim: int) -> int:
+    """Bytes of one page (64 positions) and key/value head: 4 bits a channel of key and value, and a bfloat16 step and middle for every 32 of them."""
+    return 2 * PAGE * (head_dim // 2 + head_dim // INT4_GROUP * 4)
+
+
+def int4_pool(n_pages: int, n_kv_heads: int, head_dim: int, device) -> torch.Tensor:
+    """An empty cache of 4-bit keys and values: uint8 [pages, heads, bytes of a page and head]; every position holds zeros."""
+    return torch.zeros(n_pages, n_kv_heads, int4_page_bytes(head_dim), dtype=torch.uint8, device=device)
+
+
+def _int4_heads(n_heads: int, n_kv_heads: int, head_dim: int) -> None:
+    if n_kv_heads < 1 or n_heads < 1 or n_heads % n_kv_heads or head_dim not in INT4_HEAD_DIMS:
+        raise KernelError(f"4-bit caches take head sizes {INT4_HEAD_DIMS} and query heads that share the key/value heads evenly, not {n_heads} / {n_kv_heads} heads of {head_dim}")
+
+
+def _int4_pool(pool: torch.Tensor, n_kv_heads: int, head_dim: int) -> None:
+    _need(pool, "pool", torch.uint8)
+    if pool.dim() != 3 or pool.shape[1] != n_kv_heads or pool.shape[2] != int4_page_bytes(head_dim):
+        raise KernelError(f"a 4-bit cache pool must be [pages, {n_kv_heads}, {int4_page_bytes(head_dim)}] bytes, not {tuple(pool.shape)}")
+    if pool.data_ptr() % 16:
+        raise KernelError("a 4-bit cache pool must start on a 16-byte boundary")
+
+
+def _page_table(block_table: torch.Tensor, table_stride: int) -> int:
+    """The number of rows of a page table."""
+    _need(block_table, "block_table", torch.int32)
+    if table_stride < 1 or block_table.numel() % table_stride or block_table.numel() == 0:
+        raise KernelError(f"block_table must have rows of {table_stride} pages, not {tuple(block_table.shape)}")
+    return block_table.numel() // table_stride
+
+
+def _query_rows(q: torch.Tensor, q_stride: int, T: int, width: int) -> None:
+    _need(q, "q", torch.bfloat16)
+    if q_stride % 8 or q_stride < width or (T and q.numel() < (T - 1) * q_stride + width) or q.data_ptr() % 16:
+        raise KernelError(f"q must hold {T} rows of {width} numbers, {q_stride} (a multiple of 8) apart, from a 16-byte boundary on")
+
+
+def store_int4(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], tok_pos: torch.Tensor,
+               tok_row: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, table_stride: int, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The query heads of ``qkv`` [T, (n_q + 2 n_kv) * head_dim] (bfloat16), turned by the tables' angles (``cos`` and ``sin`` None: as they are), as [T, n_q * head_dim];
+    keys, turned too, and values go into the 4-bit cache ``pool`` (``int4_pool``) at their sequences' positions.
+
+    A group of 32 channels of a row is held as 32 codes c of 0 to 15, a step and a middle in bfloat16, mid = (max + min) / 2, step = (max - min) / 15: c = floor((x - mid) / step) + 8
+    within its bounds, and stands for mid + step * (c - 7.5): at most half a step from x, but for the roundings of step and middle.  A group whose numbers are equal is held as it is; one with an
+    infinity or NaN is NaN as a whole.  Keys are turned in float64 and rounded to bfloat16 before they are coded.
+
+    Tokens of a sequence stand behind one another in the call, in the order of their positions, and no position twice; tokens whose page is not there (-1) are not stored."""
+    T = tok_pos.shape[0]
+    _int4_heads(n_q, n_kv, head_dim)
+    _need(qkv, "qkv", torch.bfloat16, (T, (n_q + 2 * n_kv) * head_dim))
+    _need(tok_pos, "tok_pos", torch.int32, (T,)); _need(tok_row, "tok_row", torch.int32, (T,))
+    _int4_pool(pool, n_kv, head_dim)
+    rows = _page_table(block_table, table_stride)
+    if (cos is None) != (sin is None):
+        raise KernelError("cos and sin go together")
+    if cos is not None:
+        _need(cos, "cos", torch.float32); _need(sin, "sin", torch.float32, cos.shape)
+        if cos.dim() != 2 or cos.shape[0] < 1 or cos.shape[1] != head_dim // 2 or cos.data_ptr() % 16 or sin.data_ptr() % 16:
+            raise KernelError(f"cos/sin tables must be [positions, {head_dim // 2}] from a 16-byte boundary on, not {tuple(cos.shape)}")
+    if qkv.data_ptr() % 16:
+        raise KernelError("qkv must start on a 16-byte boundary")
+    if out is None:
+        out = torch.empty(T, n_q * head_dim, dtype=torch.bfloat16, device=qkv.device)
+    else:
+        _need(out, "out", torch.bfloat16, (T, n_q * head_dim))
+        if out.data_ptr() % 16:
+            raise KernelError("out must start on a 16-byte boundary")
+    stream = _stream_here(qkv, "qkv")
+    if T:
+        check(long_context().pe_store_int4(qkv.data_ptr(), T, n_q, n_kv, head_dim, _ptr(cos), _ptr(sin), 0 if cos is None else cos.shape[0], tok_pos.data_ptr(),
+                                           tok_row.data_ptr(), pool.data_ptr(), pool.shape[0], block_table.data_ptr(), table_stride, rows, out.data_ptr(), stream), "store_int4")
+    return out
+
+
+def load_int4(pool: torch.Tensor, n_kv: int, head_dim: int, tok_pos: torch.Tensor, tok_row: torch.Tensor, block_table: torch.Tensor, table_stride: int):
+    """What a 4-bit cache holds at positions ``tok_pos`` of the sequences ``tok_row`` (int32 [T]): keys and values, float32 [T, n_kv, head_dim].  Zeros where no page is."""
+    T = tok_pos.shape[0]
+    _int4_heads(n_kv, n_kv, head_dim)
+    _int4_pool(pool, n_kv, head_dim)
+    _need(tok_pos, "tok_pos", torch.int32, (T,)); _need(tok_row, "tok_row", torch.int32, (T,))
+    rows = _page_table(block_table, table_stride)
+    stream = _stream_here(pool, "pool")
+    keys = torch.empty(T, n_kv, head_dim, dtype=torch.float32, device=pool.device)
+    values = torch.empty_like(keys)
+    if T:
+        check(long_context().pe_load_int4(pool.data_ptr(), pool.shape[0], n_kv, head_dim, tok_pos.data_ptr(), tok_row.data_ptr(), T, block_table.data_ptr(), table_stride, rows,
+                                          keys.data_ptr(), values.data_ptr(), stream), "load_int4")
+    return keys, values
+
+
+def _int4_out(out: Optional[torch.Tensor], T: int, width: int, device) -> torch.Tensor:
+    if out is None:
+        return torch.empty(T, width, dtype=torch.bfloat16, device=device)
+    _need(out, "out", torch.bfloat16, (T, width))
+    return out
+
+
+def attention_int4(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int, head_dim: int, pool: torch.Tensor, block_table: torch.Tensor, table_stride: int,
+                   tok_pos: torch.Tensor, tok_row: torch.Tensor, window: Optional[int], scale: float, max_context: int, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``attention_decode`` over a 4-bit cache: T tokens (bfloat16), each at position ``tok_pos`` of row ``tok_row`` of the page table, see the positions up to their own (the last
+    ``window`` of them).  ``max_context`` bounds every token's position + 1 and fixes the launch shape.
+
+    Scores are sums of exact products of the queries with codes, in float32; steps and middles join in float32.  Weights are rounded to bfloat16 for the product with
+    the values, and once more behind their multiplication by a value's step.  A row that sees nothing is zeros; one that sees a group that is no number is none where that reaches."""
+    T = tok_pos.shape[0]
+    _int4_heads(n_heads, n_kv_heads, head_dim)
+    _int4_pool(pool, n_kv_heads, head_dim)
+    _query_rows(q, q_stride, T, n_heads * head_dim)
+    _need(tok_pos, "tok_pos", torch.int32, (T,)); _need(tok_row, "tok_row", torch.int32, (T,))
+    rows = _page_table(block_table, table_stride)
+    if max_context < 1 or (window is not None and window < 0):
+        raise KernelError("max_context must be positive, and a window not negative")
+    out = _int4_out(out, T, n_heads * head_dim, q.device)
+    stream = _stream_here(q, "q")
+    if T:
+        check(long_context().pe_attention_int4(q.data_ptr(), q_stride, out.data_ptr(), pool.data_ptr(), pool.shape[0] * n_kv_heads, block_table.data_ptr(), table_stride, rows,
+                                               tok_pos.data_ptr(), tok_row.data_ptr(), T, n_heads, n_kv_heads, head_dim, window or 0, float(scale), int(max_context), 0,
+                                               status_ptr(q.device), stream), "attention_int4")
+    return out
+
+
+def attention_int4_prompt(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int, head_dim: int, pool: torch.Tensor, block_table: torch.Tensor, table_stride: int,
+                          tiles: torch.Tensor, n_tokens: int, window: Optional[int], scale: float, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The same for runs of at most 128 tokens of a sequence, ``tiles`` int32 [n, 4] (``prefill_tiles`` with ``PREFILL_TILE_TCGEN05``), whose own keys and values the cache holds already;
+    ``q`` has ``n_tokens`` rows."""
+    _int4_heads(n_heads, n_kv_heads, head_dim)
+    _int4_pool(pool, n_kv_heads, head_dim)
+    _query_rows(q, q_stride, n_tokens, n_heads * head_dim)
+    _need(tiles, "tiles", torch.int32)
+    if tiles.dim() != 2 or tiles.shape[1] != 4 or tiles.data_ptr() % 16:
+        raise KernelError(f"tiles must be [runs, 4] from a 16-byte boundary on, not {tuple(tiles.shape)}")
+    rows = _page_table(block_table, table_stride)
+    if window is not None and window < 0:
+        raise KernelError("a window must not be negative")
+    out = _int4_out(out, n_tokens, n_heads * head_dim, q.device)
+    stream = _stream_here(q, "q")
+    if n_tokens and tiles.shape[0]:
+        check(long_context().pe_attention_int4_prompt(q.data_ptr(), q_stride, out.data_ptr(), pool.data_ptr(), pool.shape[0] * n_kv_heads, block_table.data_ptr(), table_stride, rows,
+                                                      tiles.data_ptr(), tiles.shape[0], n_tokens, n_heads, n_kv_heads, head_dim, window or 0, float(scale), status_ptr(q.device),
+                                                      stream), "attention_int4_prompt")
+    return out
+
+
+def page_bounds(pool: torch.Tensor, n_kv: int, head_dim: int, tok_pos: torch.Tensor, tok_row: torch.Tensor, block_table: torch.Tensor, table_stride: int,
+                bounds: torch.Tensor) -> torch.Tensor:
+    """The least and the greatest key of every channel of the pages that the tokens of a step have filled: where a token is the last of its page, ``bounds`` (bfloat16 [pages, n_kv, 2, head_dim])
+    gets the page's rows, in place; the others stay as they are.  Of the keys that the 4-bit cache stands for, rounded to bfloat16."""
+    T = tok_pos.shape[0]
+    _int4_heads(n_kv, n_kv, head_dim)
+    _int4_pool(pool, n_kv, head_dim)
+    _need(tok_pos, "tok_pos", torch.int32, (T,)); _need(tok_row, "tok_row", torch.int32, (T,))
+    _need(bounds, "bounds", torch.bfloat16, (pool.shape[0], n_kv, 2, head_dim))
+    rows = _page_table(block_table, table_stride)
+    if bounds.data_ptr() % 16:
+        raise KernelError("bounds must start on a 16-byte boundary")
+    stream = _stream_here(pool, "pool")
+    if T:
+        check(long_context().pe_page_bounds(pool.data_ptr(), pool.shape[0], n_kv, head_dim, tok_pos.data_ptr(), tok_row.data_ptr(), T, block_table.data_ptr(), table_stride, rows,
+                                            bounds.data_ptr(), stream), "page_bounds")
+    return bounds
+
+
+@dataclass
+class SelectedPages:
+    """The pages that tokens attend to, one list a token and key/value head: ``table`` int32 [T * heads, keep], page * heads + head of every page in the order of the
+    positions, -1 behind the last one; ``pos`` int32 [T * heads], the token's place in the row of these pages."""
+    table: torch.Tensor
+    pos: torch.Tensor
+
+
+def select_pages(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int, head_dim: int, bounds: torch.Tensor, block_table: torch.Tensor, table_stride: int,
+                 tok_pos: torch.Tensor, tok_row: torch.Tensor, keep: int, max_context: int) -> SelectedPages:
+    """For every token and key/value head the ``keep`` pages to attend to: its own, the sequence's first (where ``keep`` is 2 or more), and those whose keys can score highest by
+    their ``bounds`` (``page_bounds``): the sum over the head's queries and over the channels of max(q * least, q * greatest), in float64; of equal ones the earlier page.  All pages, where a token sees
+    no more than ``keep``.  ``max_context`` bounds every token's position + 1."""
+    T = tok_pos.shape[0]
+    _int4_heads(n_heads, n_kv_heads, head_dim)
+    _query_rows(q, q_stride, T, n_heads * head_dim)
+    _need(bounds, "bounds", torch.bfloat16)
+    if bounds.dim() != 4 or tuple(bounds.shape[1:]) != (n_kv_heads, 2, head_dim) or bounds.data_ptr() % 16:
+        raise KernelError(f"bounds must be [pages, {n_kv_heads}, 2, {head_dim}] from a 16-byte boundary on, not {tuple(bounds.shape)}")
+    _need(tok_pos, "tok_pos", torch.int32, (T,)); _need(tok_row, "tok_row", torch.int32, (T,))
+    rows = _page_table(block_table, table_stride)
+    if keep < 1 or max_context < 1:
+        raise KernelError("keep and max_context must be positive")
+    stream = _stream_here(q, "q")
+    table = torch.empty(T * n_kv_heads, keep, dtype=torch.int32, device=q.device)
+    pos = torch.empty(T * n_kv_heads, dtype=torch.int32, device=q.device)
+    if T:
+        check(long_context().pe_select_pages(q.data_ptr(), q_stride, T, n_heads, n_kv_heads, head_dim, bounds.data_ptr(), bounds.shape[0], block_table.data_ptr(), table_stride, rows,
+                                             tok_pos.data_ptr(), tok_row.data_ptr(), keep, int(max_context), table.data_ptr(), pos.data_ptr(), stream), "select_pages")
+    return SelectedPages(table, pos)
+
+
+def attention_int4_selected(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int, head_dim: int, pool: torch.Tensor, pages: SelectedPages, scale: float,
+                            out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``attention_int4`` over the pages that ``select_pages`` has found."""
+    _int4_heads(n_heads, n_kv_heads, head_dim)
+    _int4_pool(pool, n_kv_heads, head_dim)
+    places = pages.pos.shape[0]
+    T, keep = places // n_kv_heads, pages.table.shape[1]
+    _need(pages.pos, "pages.pos", torch.int32, (T * n_kv_heads,)); _need(pages.table, "pages.table", torch.int32, (T * n_kv_heads, keep))
+    _query_rows(q, q_stride, T, n_heads * head_dim)
+    out = _int4_out(out, T, n_heads * head_dim, q.device)
+    stream = _stream_here(q, "q")
+    if T:
+        check(long_context().pe_attention_int4(q.data_ptr(), q_stride, out.data_ptr(), pool.data_ptr(), pool.shape[0] * n_kv_heads, pages.table.data_ptr(), keep, places,
+                                               pages.pos.data_ptr(), None, T, n_heads, n_kv_heads, head_dim, 0, float(scale), keep * PAGE, 1, status_ptr(q.device), stream),
+              "attention_int4_selected")
+    return out

@@ -33,6 +33,8 @@ STATE_SOURCES = ("state_space.cu", "state_space_tiles.cu", "state_space_tcgen05.
 JOINED_SOURCES = ("joined_ops.cu", "attention_diff.cu", "attention_diff_tcgen05.cu")
 # The kernels of several answers to a prompt and of rules on what may be chosen: logits under penalties, biases and masks, and the tables of a step.
 ANSWER_SOURCES = ("logit_rules.cu", "step_tables.cu")
+# The kernels of a long context's cache: 4-bit pages appended to, read back and attended to, the bounds of their keys, and the choice of pages by them.
+LONG_SOURCES = ("int4_cache.cu", "page_select.cu", "attention_int4.cu")
 HEAD_DIM_SOURCES = ("attention_decode.cu", "attention_prefill.cu", "attention_prefill_tcgen05.cu", "attention_shared.cu")      # compiled per head size
 
 _SIGNATURES = {
@@ -138,6 +140,15 @@ _ANSWER_SIGNATURES = {
     "pe_adjust_logits": [P, P, I, I, P, P, I, P, P, P, P, I, P, I, P, I, P],
     "pe_note_tokens": [P, I, I, P, P, I, I, P, P, I, P],
     "pe_step_tables": [P, P, P, P, P, I, P, I, I, I, P, P, P, P, I, P, I, P],
+}
+
+_LONG_SIGNATURES = {
+    "pe_store_int4": [P, I, I, I, I, P, P, I, P, P, P, LL, P, I, I, P, P],
+    "pe_load_int4": [P, LL, I, I, P, P, I, P, I, I, P, P, P],
+    "pe_page_bounds": [P, LL, I, I, P, P, I, P, I, I, P, P],
+    "pe_select_pages": [P, I, I, I, I, I, P, LL, P, I, I, P, P, I, I, P, P, P],
+    "pe_attention_int4": [P, I, P, P, LL, P, I, I, P, P, I, I, I, I, I, F, I, I, P, P],
+    "pe_attention_int4_prompt": [P, I, P, P, LL, P, I, I, P, I, I, I, I, I, I, F, P, P],
 }
 
 _HEAD_DIM_SIGNATURES = {
@@ -281,6 +292,20 @@ def answers() -> ctypes.CDLL:
         lib.pe_set_pdl(0 if os.environ.get("PICO_ENGINE_PDL", "1") == "0" else 1)
         _answers = lib
     return _answers
+
+
+_long = None
+
+
+def long_context() -> ctypes.CDLL:
+    """The library of the kernels of a long context's cache; compiled at the first call."""
+    global _long
+    if _long is None:
+        lib = build.load("long", LONG_SOURCES)
+        declare(lib, _LONG_SIGNATURES)
+        lib.pe_set_pdl(0 if os.environ.get("PICO_ENGINE_PDL", "1") == "0" else 1)
+        _long = lib
+    return _long
 
 
 _extras = None
