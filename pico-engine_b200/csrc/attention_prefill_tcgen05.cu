@@ -40,6 +40,7 @@
 #error "compile with -DPE_HEAD_DIM=<head size>"
 #endif
 #include "tcgen05_attention.cuh"
+#include <cuda_fp16.h>
 
 #if PE_HEAD_DIM == 64 || PE_HEAD_DIM == 128
 
@@ -54,7 +55,7 @@
 #define AT_STAGE_BYTES (2 * 2 * AT_KTILE * AT_HD * 2)   // keys, then values, of two pages and one head
 #define AT_TILE_BYTES (AT_Q_BYTES + AT_STAGES * AT_STAGE_BYTES)
 #define AT_BUFFERS 3                               // S buffers
-#define AT_BAR_WORDS (2 + 3 * AT_BUFFERS + 4 * AT_STAGES + 13)
+#define AT_BAR_WORDS (2 + 3 * AT_BUFFERS + 4 * AT_STAGES + 14)
 #define AT_SMEM_BYTES (AT_TILE_BYTES + 8 * AT_BAR_WORDS + 2 * 2 * AT_QTILE * 4)
 #define AT_TMEM_COLS 512                           // S buffers (then P) at columns 0, 128 and 256, O from column 384
 #define AT_O_COL (AT_BUFFERS * 2 * AT_KTILE)
@@ -67,9 +68,29 @@ struct AtArgs {
     const float* slopes; float inv_scale;          // [nh] or null: slopes[h] * (query position - key position) is taken off the scaled score
     int pool_rows;                                 // rows of the key (and value) pool seen as a matrix [rows][head size]
     const float* sinks;                            // [nh] or null: one more place of this (scaled) score joins a row's denominator and carries no value
+    const float* factors;                          // of float16 keys: [pages][nkv], what the scores of a page's keys are multiplied by
 };
 
+// 64 columns of a row of queries, in place: bfloat16 to float16, times `up`
+__device__ __forceinline__ void at_to_half(unsigned row, int r, int groups, int group0, float up) {
+    for (int j = group0; j < group0 + groups; ++j) {
+        const unsigned at = row + (unsigned)((j ^ (r & 7)) << 4);   // (the swizzle exchanges the 16-byte groups of a row)
+        unsigned v[4];
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2 h = __floats2half2_rn(__uint_as_float(v[i] << 16) * up, __uint_as_float(v[i] & 0xffff0000u) * up);
+            v[i] = *reinterpret_cast<const unsigned*>(&h);
+        }
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+    }
+}
+
 // tiles[i] = (batch row, first packed token, number of tokens (<= AT_QTILE), position of the first token)
+// HALF_KEYS: the keys are float16, times a power of two of their page and head (expanded from a cache of fewer bits, whose products with queries bfloat16 keys would be off by more than
+// all else).  The softmax warps then take the queries to float16 before the first product, each row times a power of two of its own, and scores are multiplied back in
+// the exponent's multiply-add, which costs nothing.
+template <bool HALF_KEYS>
 __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q,
                                                                                   const __grid_constant__ CUtensorMap map_k,
                                                                                   const __grid_constant__ CUtensorMap map_v,
@@ -87,6 +108,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
     unsigned long long* told = v_empty + AT_STAGES;                 // [warpgroup][32 rows]: a step's reference points are there
     unsigned long long* met = told + 8;                             // [32 rows]: both warpgroups have come to the end
     unsigned long long* o_full = met + 4;                           // and so have the products
+    unsigned long long* q_half = o_full + 1;                        // the queries are float16
     float* refs = reinterpret_cast<float*>(bars + AT_BAR_WORDS);    // [warpgroup][row]: reference point of the group's last step
     float* sums = refs + 2 * AT_QTILE;                              // [warpgroup][row]: at the end, the group's share of the row's sum
     if (q_s & 1023u) {                                              // every thread alike: nothing is allocated yet
@@ -130,6 +152,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
         for (int w = 0; w < 8; ++w) init(&told[w], 1);
         for (int q = 0; q < 4; ++q) init(&met[q], 2);
         init(o_full, 1);
+        init(q_half, 8);
         asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
         // the queries and the first step are asked for before the block meets
         const int y[2] = {rows_of(table[page_at(0)]), rows_of(1 < n_pages ? table[page_at(1)] : -1)};
@@ -173,12 +196,12 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
             const unsigned elected = pe_elect();
             // instruction descriptors: float32 accumulator, bfloat16 operands, M = 128;
             // S: A and B K-major, N = 128 keys;  O: B MN-major (bit 16), N = head size
-            const unsigned idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)((2 * AT_KTILE) >> 3) << 17) | ((unsigned)(AT_QTILE >> 4) << 24);
+            const unsigned idesc_s = (1u << 4) | (HALF_KEYS ? 0u : (1u << 7) | (1u << 10)) | ((unsigned)((2 * AT_KTILE) >> 3) << 17) | ((unsigned)(AT_QTILE >> 4) << 24);
             const unsigned idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((unsigned)(AT_HD >> 3) << 17) | ((unsigned)(AT_QTILE >> 4) << 24);
             // operand descriptors of stage 0; a stage further on adds its offset in 16-byte units
             const unsigned long long dq = at_desc(q_s, 0, 1024), dk = at_desc(kv_s, 0, 1024);
             const unsigned long long dv = at_desc(kv_s + AT_STAGE_BYTES / 2, 2 * AT_KTILE * 128, 1024);
-            bool ok = at_wait_warp(at_smem(&q_full), 0u);
+            bool ok = at_wait_warp(at_smem(HALF_KEYS ? q_half : &q_full), 0u);
             auto issue_s = [&](int it) -> bool {                    // S = Q . K^T of step `it`, when P.V has read the P that lay in its buffer
                 const int s = it % AT_STAGES, b = it % AT_BUFFERS;
                 if (it >= AT_BUFFERS && !at_wait_warp(at_smem(&pv_done[b]), (unsigned)(it / AT_BUFFERS - 1) & 1u)) return false;
@@ -218,16 +241,47 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
         const int p_r = pos0 + r;
         const unsigned lane_addr = tmem + ((unsigned)(quarter * 32) << 16);
         const float slope = p.slopes ? p.slopes[h] * p.inv_scale : 0.f;     // in units of the unscaled score
+        float row_scale = p.scale_log2e;
+        bool ok = true;
+        if constexpr (HALF_KEYS) {
+            // half a row of queries a thread: its largest, then the row's (through the other half's thread), then float16
+            ok = at_wait_warp(at_smem(&q_full), 0u);
+            constexpr int groups = AT_HD / 16;
+            const unsigned row = q_s + (unsigned)(r * 128 + (AT_HD == 128 ? g * (AT_QTILE * 128) : 0));
+            const int group0 = AT_HD == 128 ? 0 : g * groups;
+            float most = 0.f;
+            for (int j = group0; j < group0 + groups; ++j) {
+                unsigned v[4];
+                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(row + (unsigned)((j ^ (r & 7)) << 4)) : "memory");
+#pragma unroll
+                for (int i = 0; i < 4; ++i) most = fmaxf(most, fmaxf(fabsf(__uint_as_float(v[i] << 16)), fabsf(__uint_as_float(v[i] & 0xffff0000u))));
+            }
+            sums[g * AT_QTILE + r] = most;
+            asm volatile("bar.sync 1, 256;" ::: "memory");          // the softmax warps
+            most = fmaxf(most, sums[(g ^ 1) * AT_QTILE + r]);
+            int exponent = 0;
+            if (most > 0.f) frexpf(fminf(most, 3.0e38f), &exponent);
+            const float up = ldexpf(1.f, 14 - max(exponent, -30));
+            row_scale = p.scale_log2e / up;
+            at_to_half(row, r, groups, group0, up);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");        // the products read them through the tensor core's proxy
+            __syncwarp();
+            if (lane == 0) at_arrive(at_smem(q_half));
+        }
         const unsigned long long scale2 = at_two(p.scale_log2e, p.scale_log2e);
         float m_mine = -INFINITY, l_mine = 0.f;                     // the reference point of this group's last step; its share of the row's sum
-        bool ok = true;
         int entry[2];                                               // the page table's entries of the next step of this group
 #pragma unroll
         for (int x = 0; x < 2; ++x) entry[x] = 2 * g + x < n_pages ? table[page_at(2 * g + x)] : -1;
-        for (int it = g; it < n_steps; it += 2) {
+        for (int it = g; it < n_steps && ok; it += 2) {
             const int b = it % AT_BUFFERS;
             const unsigned s_addr = lane_addr + b * (2 * AT_KTILE);
             const bool there[2] = {entry[0] >= 0, entry[1] >= 0};   // (a page that is not there was read as zeros and is masked)
+            float page_scale[2] = {1.f, 1.f};                       // of float16 keys: what takes the page's scores to powers of two
+            if constexpr (HALF_KEYS) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) page_scale[x] = there[x] ? row_scale * p.factors[entry[x] * p.nkv + kvh] : 1.f;
+            }
 #pragma unroll
             for (int x = 0; x < 2; ++x) entry[x] = 2 * it + 4 + x < n_pages ? table[page_at(2 * it + 4 + x)] : -1;
             if (!at_wait_warp(at_smem(&s_full[b]), (unsigned)(it / AT_BUFFERS) & 1u)) { ok = false; break; }
@@ -278,7 +332,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mx[4 * x + i] = fmaxf(mx[4 * x + i], sx[AT_KTILE - 4 + i]);
             }
-            const float m_step = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) + base[0], fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])) + base[1]);
+            const float m_first = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) + base[0], m_second = fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])) + base[1];
             // the row's reference point up to the step before, from the other warpgroup
             float m_run = -INFINITY;
             if (it > 0) {
@@ -288,7 +342,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
             // The reference point of the exponentials follows the row's maximum only when that has grown by more than
             // AT_LAZY (in powers of two): P then holds values up to 2^AT_LAZY, which bfloat16 and the float32 sums take
             // as well as values up to 1, and O is rescaled on few steps instead of on nearly all.
-            const float m_tile = m_step * p.scale_log2e;
+            const float m_tile = HALF_KEYS ? fmaxf(m_first * page_scale[0], m_second * page_scale[1]) : fmaxf(m_first, m_second) * p.scale_log2e;
             const float m_new = (m_run != -INFINITY && m_tile <= m_run + AT_LAZY) ? m_run : fmaxf(m_run, m_tile);
             refs[g * AT_QTILE + r] = m_new;
             __syncwarp();
@@ -301,9 +355,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 float packed[AT_KTILE / 2];
+                const unsigned long long scale_x = HALF_KEYS ? at_two(page_scale[x], page_scale[x]) : scale2;
                 const float off = fmaf(base[x], p.scale_log2e, -m_use);
 #pragma unroll
-                for (int c = 0; c < AT_KTILE; c += 2) packed[c >> 1] = __uint_as_float(at_exp2_pair(s[x * AT_KTILE + c], s[x * AT_KTILE + c + 1], scale2, at_two(off, off), sum[(c >> 1) & 1]));
+                for (int c = 0; c < AT_KTILE; c += 2) packed[c >> 1] = __uint_as_float(at_exp2_pair(s[x * AT_KTILE + c], s[x * AT_KTILE + c + 1], scale_x, at_two(off, off), sum[(c >> 1) & 1]));
                 at_st32(s_addr + x * (AT_KTILE / 2), packed);       // P over the scores, two keys a column
             }
             l_mine += at_sum_four(sum[0], sum[1]);
@@ -374,16 +429,16 @@ extern "C" int pe_attention_prefill_tcgen05_tile() { return AT_QTILE; }
 // how many of the kernel's CTAs an SM holds at once (one: it takes all of tensor memory), or a negative CUDA error
 extern "C" int pe_attention_prefill_tcgen05_ctas_per_sm() {
     int n = 0;
-    if (cudaFuncSetAttribute(attention_prefill_tcgen05_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)AT_SMEM_BYTES) != cudaSuccess) return -1;
-    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attention_prefill_tcgen05_kernel, AT_THREADS, AT_SMEM_BYTES);
+    if (cudaFuncSetAttribute(attention_prefill_tcgen05_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)AT_SMEM_BYTES) != cudaSuccess) return -1;
+    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attention_prefill_tcgen05_kernel<false>, AT_THREADS, AT_SMEM_BYTES);
     return e == cudaSuccess ? n : -(int)e;
 }
 
 // q: [n_tokens][q_stride] with head h at columns h * hd; pools: [pool_pages][nkv][64][hd]
-extern "C" int pe_attention_prefill_tcgen05(const void* q, int q_stride, void* out, const void* k_pool, const void* v_pool,
-                                            long long pool_pages, const int* block_table, int table_stride, const void* tiles,
-                                            int n_tiles, int n_tokens, int nh, int nkv, int hd, int window, float scale,
-                                            int keep_first, const float* slopes, int* status, void* stream, const float* sinks) {
+template <bool HALF_KEYS>
+static int at_launch(const void* q, int q_stride, void* out, const void* k_pool, const void* v_pool, long long pool_pages, const int* block_table, int table_stride, const void* tiles,
+                     int n_tiles, int n_tokens, int nh, int nkv, int hd, int window, float scale, int keep_first, const float* slopes, int* status, void* stream, const float* sinks,
+                     const float* factors) {
     if (n_tiles <= 0) return 0;
     if (hd != AT_HD || nkv <= 0 || nh % nkv || n_tiles > 65535 || q_stride % 8 || !(scale > 0.f) || !status) return PE_ERR_UNSUPPORTED;
     if (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)out | (uintptr_t)tiles) & 15) return PE_ERR_UNSUPPORTED;
@@ -391,7 +446,7 @@ extern "C" int pe_attention_prefill_tcgen05(const void* q, int q_stride, void* o
     CUtensorMap mq, mk, mv;
     int rc = at_make_map(&mq, q, n_tokens, (long long)nh * hd, q_stride, AT_QTILE);
     if (rc) return rc;
-    rc = at_make_map(&mk, k_pool, pool_pages * nkv * AT_KTILE, hd, hd, AT_KTILE);
+    rc = at_make_map(&mk, k_pool, pool_pages * nkv * AT_KTILE, hd, hd, AT_KTILE);     // (float16 keys are 16-bit numbers like any others to a copy)
     if (rc) return rc;
     rc = at_make_map(&mv, v_pool, pool_pages * nkv * AT_KTILE, hd, hd, AT_KTILE);
     if (rc) return rc;
@@ -400,15 +455,32 @@ extern "C" int pe_attention_prefill_tcgen05(const void* q, int q_stride, void* o
     p.nh = nh; p.nkv = nkv; p.window = window; p.scale_log2e = scale * 1.4426950408889634f;
     p.keep_first = window > 0 && keep_first > 0 ? keep_first : 0; p.slopes = slopes; p.inv_scale = 1.0f / scale;
     p.pool_rows = (int)(pool_pages * nkv * AT_KTILE);
-    p.sinks = sinks;
+    p.sinks = sinks; p.factors = factors;
     const size_t smem = AT_SMEM_BYTES;
     static bool attr_set = false;
     if (!attr_set) {
-        PE_TRY(cudaFuncSetAttribute(attention_prefill_tcgen05_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        PE_TRY(cudaFuncSetAttribute(attention_prefill_tcgen05_kernel<HALF_KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         attr_set = true;
     }
-    PE_TRY(pe_launch(attention_prefill_tcgen05_kernel, dim3(nh, n_tiles), AT_THREADS, smem, (cudaStream_t)stream, mq, mk, mv, p, status));
+    PE_TRY(pe_launch(attention_prefill_tcgen05_kernel<HALF_KEYS>, dim3(nh, n_tiles), AT_THREADS, smem, (cudaStream_t)stream, mq, mk, mv, p, status));
     return 0;
+}
+
+extern "C" int pe_attention_prefill_tcgen05(const void* q, int q_stride, void* out, const void* k_pool, const void* v_pool,
+                                            long long pool_pages, const int* block_table, int table_stride, const void* tiles,
+                                            int n_tiles, int n_tokens, int nh, int nkv, int hd, int window, float scale,
+                                            int keep_first, const float* slopes, int* status, void* stream, const float* sinks) {
+    return at_launch<false>(q, q_stride, out, k_pool, v_pool, pool_pages, block_table, table_stride, tiles, n_tiles, n_tokens, nh, nkv, hd, window, scale, keep_first, slopes, status,
+                            stream, sinks, nullptr);
+}
+
+// The same over float16 keys, the scores of a page's keys times factors[page][kv head].
+extern "C" int pe_attention_prefill_half_keys(const void* q, int q_stride, void* out, const void* k_pool, const void* v_pool, const float* factors, long long pool_pages,
+                                              const int* block_table, int table_stride, const void* tiles, int n_tiles, int n_tokens, int nh, int nkv, int hd, int window,
+                                              float scale, int* status, void* stream) {
+    if (!factors) return PE_ERR_UNSUPPORTED;
+    return at_launch<true>(q, q_stride, out, k_pool, v_pool, pool_pages, block_table, table_stride, tiles, n_tiles, n_tokens, nh, nkv, hd, window, scale, 0, nullptr, status, stream,
+                           nullptr, factors);
 }
 
 #else   // other head sizes: the mma.sync kernel of attention_prefill.cu takes them
@@ -417,6 +489,10 @@ extern "C" int pe_attention_prefill_tcgen05_tile() { return 0; }
 extern "C" int pe_attention_prefill_tcgen05_ctas_per_sm() { return 0; }
 extern "C" int pe_attention_prefill_tcgen05(const void*, int, void*, const void*, const void*, long long, const int*, int, const void*,
                                             int, int, int, int, int, int, float, int, const float*, int*, void*, const float*) {
+    return PE_ERR_UNSUPPORTED;
+}
+extern "C" int pe_attention_prefill_half_keys(const void*, int, void*, const void*, const void*, const float*, long long, const int*, int, const void*, int, int, int, int, int, int,
+                                              float, int*, void*) {
     return PE_ERR_UNSUPPORTED;
 }
 

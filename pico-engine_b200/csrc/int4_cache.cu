@@ -1,6 +1,7 @@
 // A paged cache of 4-bit keys and values (int4_pages.cuh): rows appended with the position rotation on the way, rows read back, and the
 // least and greatest key of a page, channel by channel.
 #include "int4_pages.cuh"
+#include <cuda_fp16.h>
 
 // ---------------------------------------------------------------------------- queries turned, keys and values appended
 //
@@ -311,6 +312,129 @@ extern "C" int pe_page_bounds(const void* pool, long long n_pages, int n_kv, int
     auto kernel = hd == 64 ? page_bounds_kernel<64> : page_bounds_kernel<128>;
     PE_TRY(pe_launch(kernel, dim3((unsigned)blocks), dim3(256), 0, (cudaStream_t)stream, (const unsigned char*)pool, n_pages, n_kv, tok_pos, tok_row, T, block_table,
                      table_stride, n_rows, (bf16*)bounds));
+    PE_LAUNCH_CHECK();
+    return 0;
+}
+
+// ---------------------------------------------------------------------------- pages in 16 bits, for prompts
+// What the runs of a prompt read of a 4-bit cache, as operands of tcgen05.mma: values as bfloat16, keys as float16 times a power of two of their page and head (`factors` takes it
+// back), so that a key keeps 11 bits whatever its size: with keys of 8 bits the scores' errors are what the results are off by (0.0055 of their size; 0.0024 so).  Positions behind a
+// row's last run are zeros.  Expanded once a page and head, for all heads and runs that read it: 7.4 MB to 24 MB of a layer for prompts of 7,541 tokens.
+// A block counts the pages of all rows from the runs, then takes every gridDim.x-th of them.
+
+#define XI_MAX_ROWS 1024
+#define XI_THREADS 256
+
+template <int D>
+__global__ void __launch_bounds__(XI_THREADS) expand_int4_kernel(const unsigned char* pool, int n_pages, int n_kv, const int4* tiles, int n_tiles, const int* block_table, int table_stride,
+                                                                 int n_rows, int window, __half* keys, bf16* values, float* factors) {
+    using B = Int4Block<D>;
+    __shared__ int low[XI_MAX_ROWS], behind[XI_MAX_ROWS], before[XI_MAX_ROWS + 1];     // a row's first page, the position behind its last run, the pages of the rows before it
+    __shared__ float largest[XI_THREADS / 32];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int r = threadIdx.x; r < n_rows; r += XI_THREADS) { low[r] = 0x7fffffff; behind[r] = 0; }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n_tiles; i += XI_THREADS) {
+        const int4 run = tiles[i];                             // row, first token, tokens, position
+        if (run.x < 0 || run.x >= n_rows || run.z <= 0 || run.w < 0) continue;
+        atomicMin(&low[run.x], (window > 0 ? max(0, run.w - window + 1) : 0) / PE_PAGE);
+        atomicMax(&behind[run.x], min(run.w + run.z, table_stride * PE_PAGE));
+    }
+    __syncthreads();
+    if (warp == 0) {
+        int sum = 0;
+        for (int base = 0; base < n_rows; base += 32) {
+            const int r = base + lane, n = r < n_rows ? max(0, (behind[r] + PE_PAGE - 1) / PE_PAGE - low[r]) : 0;
+            int upto = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += v; }
+            if (r < n_rows) before[r] = sum + upto - n;
+            sum += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        if (lane == 0) before[n_rows] = sum;
+    }
+    __syncthreads();
+    const long long items = (long long)before[n_rows] * n_kv;
+    for (long long item = blockIdx.x; item < items; item += gridDim.x) {
+        const int kvh = (int)(item % n_kv), x = (int)(item / n_kv);
+        int row = 0, top = n_rows;
+        while (top - row > 1) { const int mid = (row + top) >> 1; if (before[mid] <= x) row = mid; else top = mid; }
+        const int j = low[row] + x - before[row], there = min(PE_PAGE, behind[row] - j * PE_PAGE), page = block_table[(size_t)row * table_stride + j];
+        if (page < 0 || page >= n_pages) continue;             // (the same for the whole block)
+        const size_t at = (size_t)page * n_kv + kvh;
+        const unsigned char* block = pool + at * B::bytes;
+        // the largest key that the page's steps and middles allow
+        float most = 0.f;
+        for (int i = threadIdx.x; i < there * B::groups; i += XI_THREADS) {
+            const bf16* meta = reinterpret_cast<const bf16*>(block + q4_key_step<D>(i / B::groups, i % B::groups));
+            most = fmaxf(most, fmaf(7.5f, fabsf(to_f(meta[0])), fabsf(to_f(meta[B::groups]))));
+        }
+        most = warp_max(most);
+        __syncthreads();                                       // (the last page's maxima have been read)
+        if (lane == 0) largest[warp] = most;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < XI_THREADS / 32; ++w) most = fmaxf(most, largest[w]);
+        int exponent = 0;
+        if (most > 0.f) frexpf(fminf(most, 3.0e38f), &exponent);                          // most <= 2^exponent
+        const float up = ldexpf(1.f, 14 - max(exponent, -30));
+        if (threadIdx.x == 0) factors[at] = 1.f / up;
+        __half* ko = keys + at * PE_PAGE * D;
+        bf16* vo = values + at * PE_PAGE * D;
+#pragma unroll
+        for (int i = threadIdx.x; i < PE_PAGE * B::key_words; i += XI_THREADS) {
+            const int p = i / B::key_words, rest = i % B::key_words, t = rest / B::groups, b = rest % B::groups;
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (p < there) {
+                const unsigned word = *reinterpret_cast<const unsigned*>(block + i * 4);
+                const bf16* meta = reinterpret_cast<const bf16*>(block + q4_key_step<D>(p, b));
+                const float s = to_f(meta[0]) * up, m = to_f(meta[B::groups]) * up;
+                __half2 two[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) two[e] = __floats2half2_rn(fmaf(s, q4_level(word, e, 0), m), fmaf(s, q4_level(word, e, 1), m));
+                v = *reinterpret_cast<uint4*>(two);
+            }
+            *reinterpret_cast<uint4*>(ko + p * D + 32 * b + 8 * t) = v;
+        }
+#pragma unroll
+        for (int i = threadIdx.x; i < 4 * B::halves * 32; i += XI_THREADS) {
+            const int tile = i / (B::halves * 32), h = i / 32 % B::halves, g = (i & 31) >> 2, t = i & 3;
+            const uint4 four = *reinterpret_cast<const uint4*>(block + B::values + i * 16);
+            const unsigned words[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+            for (int f = 0; f < 2; ++f)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int p = 16 * tile + 8 * f + 2 * t + e;
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        uint2 v = make_uint2(0u, 0u);
+                        if (p < there) {
+                            const bf16* meta = reinterpret_cast<const bf16*>(block + q4_value_step<D>(p, 2 * h + b));
+                            const float s = to_f(meta[0]), m = to_f(meta[B::groups * 16]);
+                            __nv_bfloat162 two[2];
+#pragma unroll
+                            for (int w = 0; w < 2; ++w)
+                                two[w] = __floats2bfloat162_rn(fmaf(s, q4_level(words[2 * b + w], 2 * f, e), m), fmaf(s, q4_level(words[2 * b + w], 2 * f + 1, e), m));
+                            v = *reinterpret_cast<uint2*>(two);
+                        }
+                        *reinterpret_cast<uint2*>(vo + p * D + 32 * (2 * h + b) + 4 * g) = v;
+                    }
+                }
+        }
+    }
+}
+
+extern "C" int pe_expand_int4(const void* pool, long long n_pages, int n_kv, int hd, const int* tiles, int n_tiles, const int* block_table, int table_stride, int n_rows, int window,
+                              void* keys, void* values, float* factors, void* stream) {
+    if (n_tiles <= 0) return 0;
+    if ((hd != 64 && hd != 128) || n_kv <= 0 || n_rows < 1 || n_rows > XI_MAX_ROWS || n_pages * n_kv > 0x7fffffffll) return PE_ERR_UNSUPPORTED;
+    if (((uintptr_t)pool | (uintptr_t)keys | (uintptr_t)values | (uintptr_t)tiles) & 15) return PE_ERR_UNSUPPORTED;
+    auto kernel = hd == 64 ? expand_int4_kernel<64> : expand_int4_kernel<128>;
+    PE_TRY(pe_launch(kernel, dim3(pe_sm_count() * 6), dim3(XI_THREADS), 0, (cudaStream_t)stream, (const unsigned char*)pool, (int)n_pages, n_kv, (const int4*)tiles, n_tiles,
+                     block_table, table_stride, n_rows, window, (__half*)keys, (bf16*)values, factors));
     PE_LAUNCH_CHECK();
     return 0;
 }

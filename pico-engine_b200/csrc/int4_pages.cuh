@@ -29,7 +29,11 @@ struct Int4Block {
 #define Q4_HALF 0x00080008u
 
 // elements (i, 0) and (i, 1) of a word as two bfloat16 numbers, in units of 2^-129
-__device__ __forceinline__ unsigned q4_pair(unsigned word, int i) { return (__funnelshift_r(word, word, 4 * i) & Q4_MASK) | Q4_HALF; }
+__device__ __forceinline__ unsigned q4_pair(unsigned word, int i) {
+    unsigned r;                                                // (one instruction; written as operators it becomes two)
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(__funnelshift_r(word, word, 4 * i)), "r"(Q4_MASK), "r"(Q4_HALF));
+    return r;
+}
 // the level + 1/2 of element (i, e)
 __device__ __forceinline__ float q4_level(unsigned word, int i, int e) {
     const unsigned r = __funnelshift_r(word, word, 4 * i) >> (16 * e);

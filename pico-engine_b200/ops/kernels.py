@@ -2234,9 +2234,11 @@ def _int4_out(out: Optional[torch.Tensor], T: int, width: int, device) -> torch.
 
 
 def attention_int4(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int, head_dim: int, pool: torch.Tensor, block_table: torch.Tensor, table_stride: int,
-                   tok_pos: torch.Tensor, tok_row: torch.Tensor, window: Optional[int], scale: float, max_context: int, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                   tok_pos: torch.Tensor, tok_row: torch.Tensor, window: Optional[int], scale: float, max_context: int, out: Optional[torch.Tensor] = None,
+                   early_pages: bool = False) -> torch.Tensor:
     """``attention_decode`` over a 4-bit cache: T tokens (bfloat16), each at position ``tok_pos`` of row ``tok_row`` of the page table, see the positions up to their own (the last
-    ``window`` of them).  ``max_context`` bounds every token's position + 1 and fixes the launch shape.
+    ``window`` of them).  ``max_context`` bounds every token's position + 1 and fixes the launch shape.  With ``early_pages`` the kernel copies pages while the two kernels before it on the
+    stream may still run: they must have written, of the cache, no page but each token's own, and neither positions nor page tables.
 
     Scores are sums of exact products of the queries with codes, in float32; steps and middles join in float32.  Weights are rounded to bfloat16 for the product with
     the values, and once more behind their multiplication by a value's step.  A row that sees nothing is zeros; one that sees a group that is no number is none where that reaches."""
@@ -2246,14 +2248,14 @@ def attention_int4(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int
     _query_rows(q, q_stride, T, n_heads * head_dim)
     _need(tok_pos, "tok_pos", torch.int32, (T,)); _need(tok_row, "tok_row", torch.int32, (T,))
     rows = _page_table(block_table, table_stride)
-    if max_context < 1 or (window is not None and window < 0):
-        raise KernelError("max_context must be positive, and a window not negative")
+    if max_context < 1 or (window is not None and window < 0) or not scale > 0:
+        raise KernelError("max_context and scale must be positive, and a window not negative")
     out = _int4_out(out, T, n_heads * head_dim, q.device)
     stream = _stream_here(q, "q")
     if T:
         check(long_context().pe_attention_int4(q.data_ptr(), q_stride, out.data_ptr(), pool.data_ptr(), pool.shape[0] * n_kv_heads, block_table.data_ptr(), table_stride, rows,
                                                tok_pos.data_ptr(), tok_row.data_ptr(), T, n_heads, n_kv_heads, head_dim, window or 0, float(scale), int(max_context), 0,
-                                               status_ptr(q.device), stream), "attention_int4")
+                                               1 if early_pages else 0, status_ptr(q.device), stream), "attention_int4")
     return out
 
 
@@ -2268,14 +2270,20 @@ def attention_int4_prompt(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_hea
     if tiles.dim() != 2 or tiles.shape[1] != 4 or tiles.data_ptr() % 16:
         raise KernelError(f"tiles must be [runs, 4] from a 16-byte boundary on, not {tuple(tiles.shape)}")
     rows = _page_table(block_table, table_stride)
-    if window is not None and window < 0:
-        raise KernelError("a window must not be negative")
+    if (window is not None and window < 0) or not scale > 0:
+        raise KernelError("scale must be positive, and a window not negative")
     out = _int4_out(out, n_tokens, n_heads * head_dim, q.device)
     stream = _stream_here(q, "q")
     if n_tokens and tiles.shape[0]:
-        check(long_context().pe_attention_int4_prompt(q.data_ptr(), q_stride, out.data_ptr(), pool.data_ptr(), pool.shape[0] * n_kv_heads, block_table.data_ptr(), table_stride, rows,
-                                                      tiles.data_ptr(), tiles.shape[0], n_tokens, n_heads, n_kv_heads, head_dim, window or 0, float(scale), status_ptr(q.device),
-                                                      stream), "attention_int4_prompt")
+        pages = pool.shape[0]
+        keys = torch.empty(pages, n_kv_heads, PAGE, head_dim, dtype=torch.float16, device=q.device)
+        values = torch.empty(pages, n_kv_heads, PAGE, head_dim, dtype=torch.bfloat16, device=q.device)
+        factors = torch.empty(pages, n_kv_heads, dtype=torch.float32, device=q.device)
+        check(long_context().pe_expand_int4(pool.data_ptr(), pages, n_kv_heads, head_dim, tiles.data_ptr(), tiles.shape[0], block_table.data_ptr(), table_stride, rows, window or 0,
+                                            keys.data_ptr(), values.data_ptr(), factors.data_ptr(), stream), "attention_int4_prompt")
+        check(for_head_dim(head_dim).pe_attention_prefill_half_keys(
+            q.data_ptr(), q_stride, out.data_ptr(), keys.data_ptr(), values.data_ptr(), factors.data_ptr(), pages, block_table.data_ptr(), table_stride, tiles.data_ptr(), tiles.shape[0],
+            n_tokens, n_heads, n_kv_heads, head_dim, window or 0, float(scale), status_ptr(q.device), stream), "attention_int4_prompt")
     return out
 
 
@@ -2339,10 +2347,12 @@ def attention_int4_selected(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_h
     T, keep = places // n_kv_heads, pages.table.shape[1]
     _need(pages.pos, "pages.pos", torch.int32, (T * n_kv_heads,)); _need(pages.table, "pages.table", torch.int32, (T * n_kv_heads, keep))
     _query_rows(q, q_stride, T, n_heads * head_dim)
+    if not scale > 0:
+        raise KernelError("scale must be positive")
     out = _int4_out(out, T, n_heads * head_dim, q.device)
     stream = _stream_here(q, "q")
     if T:
         check(long_context().pe_attention_int4(q.data_ptr(), q_stride, out.data_ptr(), pool.data_ptr(), pool.shape[0] * n_kv_heads, pages.table.data_ptr(), keep, places,
-                                               pages.pos.data_ptr(), None, T, n_heads, n_kv_heads, head_dim, 0, float(scale), keep * PAGE, 1, status_ptr(q.device), stream),
+                                               pages.pos.data_ptr(), None, T, n_heads, n_kv_heads, head_dim, 0, float(scale), keep * PAGE, 1, 0, status_ptr(q.device), stream),
               "attention_int4_selected")
     return out

@@ -74,9 +74,9 @@ def unpack(blocks):
     return out[0], out[3], out[4], out[2]
 
 
-def attend(q, kept, seen, scale):
+def attend(q, kept, seen, scale, halves=False):
     """q [H, D] over blocks of one row: ``kept`` [P, G, 80 D], ``seen`` bool [G, 64 P].  (result [H, D], its bound per number in halves of a bfloat16 step,
-    see the tests) in 64 bits."""
+    see the tests) in 64 bits.  ``halves``: for a kernel that takes keys as float16 and values as bfloat16."""
     H, D = q.shape
     P, G, _ = kept.shape
     keys, values, part, mids = (x.view(P, G, 64, D).transpose(0, 1).reshape(G, P * 64, D) for x in unpack(kept.flatten(0, 1)))
@@ -94,6 +94,10 @@ def attend(q, kept, seen, scale):
         # a score's error: the sums of a group's queries in two bfloat16 parts times its middle (2^-16), and float32 sums
         m, sums = mids[g][seen[g]], q[h].view(-1, 32).sum(1).abs().repeat_interleave(32)
         err = scale * (2.0 ** -16 * (m.abs() @ sums) / 32 + (D + 16) * 2.0 ** -23 * ((k.abs() + m.abs()) @ q[h].abs())) + 2.0 ** -20
+        if halves:
+            # half a step of float16, 2^-11, of every key; below 2^-14 of the page's largest times 2^14, a step of 2^-24 of that (page and query row are brought to 2^14 at most)
+            err = scale * (2.0 ** -11 + (D + 16) * 2.0 ** -23) * (k.abs() @ q[h].abs()) + scale * 2.0 ** -37 * D * k.abs().max() * q[h].abs().max() + 2.0 ** -20
+            s = v                                        # values are rounded to bfloat16, and so are weights
         out.append(o)
         # weights rounded (on v), once more behind a step (on the part that the codes carry), the result rounded; what scores are off moves weights by as much
         bound.append(2.0 ** -8 * (w @ (v.abs() + s.abs()) + o.abs()) + 2 * (w * err) @ (v - o).abs() + 2 * (w @ err) * (w @ (v - o).abs()))

@@ -63,7 +63,7 @@ class Paged:
         return K.attention_int4(q, q.shape[1], self.H, self.G, self.D, self.pool, self.table if table is None else table, self.width, ints(pos), ints(row), window,
                                 self.scale, bound or max(max(pos), 0) + 1, out=out)
 
-    def check(self, got, pos, row, q=None, window=None, table=None):
+    def check(self, got, pos, row, q=None, window=None, table=None, halves=False):
         q = self.q if q is None else q
         table = self.table if table is None else table
         for t, (p, r) in enumerate(zip(pos, row)):
@@ -73,7 +73,7 @@ class Paged:
             there = table[r, :n] >= 0
             seen = seen & there.repeat_interleave(PAGE)
             blocks = self.pool[table[r, :n].clamp(min=0).long()]
-            want, bound = plain.attend(q[t, :self.H * self.D].view(self.H, self.D), blocks, seen[None].expand(self.G, -1), self.scale)
+            want, bound = plain.attend(q[t, :self.H * self.D].view(self.H, self.D), blocks, seen[None].expand(self.G, -1), self.scale, halves)
             off = (got[t].double().view(self.H, self.D) - want).abs()
             assert (off <= bound + 1e-30).all(), (t, p, float((off / (bound + 1e-30)).max()))
 
@@ -166,6 +166,7 @@ def test_attention(K, H, G, D, lengths):
     p = Paged(H, G, D, lengths, 7 + H, rubbish=float("nan"))
     pos, row = [n - 1 for n in lengths], list(range(len(lengths)))
     p.check(p.attention(K, pos, row), pos, row)
+    p.check(p.attention(K, pos, row, bound=1 << 20), pos, row)              # a launch for long contexts, whatever they are
 
 
 @pytest.mark.parametrize("H,G,D", [(14, 2, 64), (16, 4, 128)])
@@ -233,7 +234,7 @@ def test_prompts(K, H, G, D, starts, lens, window):
     pos = [s + i for s, n in zip(starts, lens) for i in range(n)]
     row = [b for b, n in enumerate(lens) for _ in range(n)]
     some = sorted(set(list(range(0, T, 37)) + [0, T - 1, min(T - 1, 127), min(T - 1, 128)]))
-    p.check(got[some], [pos[i] for i in some], [row[i] for i in some], q=q[some], window=window)
+    p.check(got[some], [pos[i] for i in some], [row[i] for i in some], q=q[some], window=window, halves=True)
 
 
 def test_runs_that_are_not_listed_stay(K):
@@ -242,7 +243,7 @@ def test_runs_that_are_not_listed_stay(K):
     out = torch.full((400, 256), 7.0, dtype=torch.bfloat16, device="cuda")
     K.attention_int4_prompt(q, 256, 4, 2, 64, p.pool, p.table, p.width, ints([[1, 230, 40, 30]]), 400, None, p.scale, out=out)
     assert (out[:230] == 7).all() and (out[270:] == 7).all()
-    p.check(out[230:270], list(range(30, 70)), [1] * 40, q=q[230:270])
+    p.check(out[230:270], list(range(30, 70)), [1] * 40, q=q[230:270], halves=True)
 
 
 # ---------------------------------------------------------------------------- bounds and selected pages
@@ -350,7 +351,7 @@ def test_a_prompt_then_tokens(K, H, G, D):
     K.page_bounds(p.pool, G, D, ints(pos), ints(row), p.table, p.width, bounds)
     a = K.attention_int4_prompt(q, H * D, H, G, D, p.pool, p.table, p.width, K.prefill_tiles([n], [0], "cuda", K.PREFILL_TILE_TCGEN05), n, None, p.scale)
     some = [0, 100, n - 1]
-    p.check(a[some], some, [0] * 3, q=q[some])
+    p.check(a[some], some, [0] * 3, q=q[some], halves=True)
     for i in range(n, n + more):
         q, _, _ = append(K, p, x[i:i + 1].contiguous(), [i], [1], cos, sin)
         K.page_bounds(p.pool, G, D, ints([i]), ints([0]), p.table, p.width, bounds)
