@@ -5,11 +5,11 @@
 
 // ---------------------------------------------------------------------------- queries turned, keys and values appended
 //
-// A query head is turned as the model's table says, in float32, and rounded once.  A key is turned in float64 and rounded once more to bfloat16, the type in which
+// A query head is turned as the model's table says, in float32, and rounded once.  A key is turned with twice float32's bits and rounded once more to bfloat16, the type in which
 // a 16-bit cache would hold it: what is coded next to the border of two codes then does not depend on the order of two roundings in float32.
-// A word of the values' codes holds four positions, so one warp writes all tokens of a call that fall into the same 16 positions of a sequence: the first of them is its
-// leader, the others have nothing to do.  Positions of the tile that are not in the call keep their bits.
-
+// A block takes sixteen tokens of a key head as they stand behind one another, eight channels of key and value a thread.  A word of the values' codes holds four positions: the first
+// of its tokens in the block gathers those that follow it in their sequence.  A word that the block has in part only (a tile that lies across two blocks, or begins
+// or ends with the call) is changed bit for bit by two atomic operations, so whoever has the others may write them at the same time, and they keep what nobody writes.
 template <int D>
 __device__ __forceinline__ void q4_load8(const bf16* p, float (&x)[8]) {
     const uint4 v = *reinterpret_cast<const uint4*>(p);
@@ -18,31 +18,41 @@ __device__ __forceinline__ void q4_load8(const bf16* p, float (&x)[8]) {
     for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
 }
 
+#define SI_HEADS 4                                             // query heads a thread, which share the angles it reads
+
 template <int D>
 __device__ __forceinline__ void store_queries(const bf16* qkv, int row_width, int n_q, const float* cos_t, const float* sin_t, int angles,
                                               const int* tok_pos, bf16* q_out, long long item) {
     constexpr int half = D / 2, parts = half / 8;
-    const int part = (int)(item % parts), head = (int)(item / parts % n_q), t = (int)(item / parts / n_q), j = part * 8;
-    const bf16* src = qkv + (size_t)t * row_width + head * D;
-    bf16* dst = q_out + ((size_t)t * n_q + head) * D;
-    uint4 lo = *reinterpret_cast<const uint4*>(src + j), hi = *reinterpret_cast<const uint4*>(src + j + half);
+    const int runs = (n_q + SI_HEADS - 1) / SI_HEADS, part = (int)(item % parts), run = (int)(item / parts % runs), t = (int)(item / parts / runs), j = part * 8;
+    const bf16* src = qkv + (size_t)t * row_width + run * SI_HEADS * D + j;
+    bf16* dst = q_out + ((size_t)t * n_q + run * SI_HEADS) * D + j;
+    const int heads = min(SI_HEADS, n_q - run * SI_HEADS);
+    uint4 lo[SI_HEADS], hi[SI_HEADS];
+#pragma unroll
+    for (int h = 0; h < SI_HEADS; ++h)
+        if (h < heads) { lo[h] = *reinterpret_cast<const uint4*>(src + h * D); hi[h] = *reinterpret_cast<const uint4*>(src + h * D + half); }
     if (cos_t) {
         const size_t at = (size_t)min(max(tok_pos[t], 0), angles - 1) * half + j;
         const float4* cp = reinterpret_cast<const float4*>(cos_t + at);
         const float4* sp = reinterpret_cast<const float4*>(sin_t + at);
         const float4 c0 = cp[0], c1 = cp[1], s0 = sp[0], s1 = sp[1];
         const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-        __nv_bfloat162* l2 = reinterpret_cast<__nv_bfloat162*>(&lo);
-        __nv_bfloat162* h2 = reinterpret_cast<__nv_bfloat162*>(&hi);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 a = __bfloat1622float2(l2[e]), b = __bfloat1622float2(h2[e]);
-            l2[e] = __floats2bfloat162_rn(a.x * c[2 * e] - b.x * s[2 * e], a.y * c[2 * e + 1] - b.y * s[2 * e + 1]);
-            h2[e] = __floats2bfloat162_rn(a.x * s[2 * e] + b.x * c[2 * e], a.y * s[2 * e + 1] + b.y * c[2 * e + 1]);
+        for (int h = 0; h < SI_HEADS; ++h) {
+            __nv_bfloat162* l2 = reinterpret_cast<__nv_bfloat162*>(&lo[h]);
+            __nv_bfloat162* h2 = reinterpret_cast<__nv_bfloat162*>(&hi[h]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 a = __bfloat1622float2(l2[e]), b = __bfloat1622float2(h2[e]);
+                l2[e] = __floats2bfloat162_rn(a.x * c[2 * e] - b.x * s[2 * e], a.y * c[2 * e + 1] - b.y * s[2 * e + 1]);
+                h2[e] = __floats2bfloat162_rn(a.x * s[2 * e] + b.x * c[2 * e], a.y * s[2 * e + 1] + b.y * c[2 * e + 1]);
+            }
         }
     }
-    *reinterpret_cast<uint4*>(dst + j) = lo;
-    *reinterpret_cast<uint4*>(dst + j + half) = hi;
+#pragma unroll
+    for (int h = 0; h < SI_HEADS; ++h)
+        if (h < heads) { *reinterpret_cast<uint4*>(dst + h * D) = lo[h]; *reinterpret_cast<uint4*>(dst + h * D + half) = hi[h]; }
 }
 
 // step and mid of the group that four neighbouring lanes hold eight numbers each of, and the levels of the lane's own
@@ -61,121 +71,118 @@ __device__ __forceinline__ void q4_group(const float (&x)[8], int (&level)[8], b
     for (int i = 0; i < 8; ++i) level[i] = q4_quantise(x[i], s, m);
 }
 
-#define SI_WARPS 8
+// a c - b s (or a s + b c) rounded to float32 as if from twice as many bits: products with their errors, and the error of their sum
+__device__ __forceinline__ float q4_turned(float a, float c, float b, float s) {
+    const float h = __fmul_rn(a, c), l = __fmul_rn(b, s), eh = __fmaf_rn(a, c, -h), el = __fmaf_rn(b, s, -l);
+    const float d = __fadd_rn(h, l), v = __fsub_rn(d, h), e = __fadd_rn(__fsub_rn(h, __fsub_rn(d, v)), __fsub_rn(l, v));
+    const float r = __fadd_rn(d, __fadd_rn(e, __fadd_rn(eh, el)));
+    return fabsf(d) < INFINITY ? r : d;
+}
+
+#define SI_THREADS 256
+#define SI_TOKENS 16
 
 template <int D>
-__global__ void __launch_bounds__(32 * SI_WARPS) store_int4_kernel(const bf16* qkv, int T, int n_q, int n_kv, const float* cos_t, const float* sin_t, int angles,
-                                                                  const int* tok_pos, const int* tok_row, unsigned char* pool, long long n_pages,
-                                                                  const int* block_table, int table_stride, int n_rows, bf16* q_out, int q_blocks) {
+__global__ void __launch_bounds__(SI_THREADS) store_int4_kernel(const bf16* qkv, int T, int n_q, int n_kv, const float* cos_t, const float* sin_t, int angles,
+                                                                const int* tok_pos, const int* tok_row, unsigned char* pool, long long n_pages,
+                                                                const int* block_table, int table_stride, int n_rows, bf16* q_out, int kv_blocks) {
     using B = Int4Block<D>;
-    __shared__ __align__(16) unsigned char fields[SI_WARPS][16][D];    // the values' codes of a warp's tile: sign << 3 | magnitude
+    __shared__ __align__(16) unsigned char fields[SI_TOKENS][D];       // the values' codes: sign << 3 | magnitude
+    __shared__ int at_pos[SI_TOKENS], at_row[SI_TOKENS], at_page[SI_TOKENS];    // page -1: the token is not stored
     pdl_launch_dependents();
     pdl_wait();
     const int row_width = (n_q + 2 * n_kv) * D;
-    if ((int)blockIdx.x < q_blocks) {
-        const long long item = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-        if (item < (long long)T * n_q * (D / 16)) store_queries<D>(qkv, row_width, n_q, cos_t, sin_t, angles, tok_pos, q_out, item);
+    if ((int)blockIdx.x >= kv_blocks) {                                 // (behind the keys' blocks, which take longer)
+        const long long item = (long long)(blockIdx.x - kv_blocks) * blockDim.x + threadIdx.x;
+        if (item < (long long)T * ((n_q + SI_HEADS - 1) / SI_HEADS) * (D / 16)) store_queries<D>(qkv, row_width, n_q, cos_t, sin_t, angles, tok_pos, q_out, item);
         return;
     }
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const long long unit = (long long)(blockIdx.x - q_blocks) * SI_WARPS + warp;
-    const int kvh = (int)(unit % n_kv);
-    const long long tok = unit / n_kv;
-    if (tok >= T) return;
-    const int first = (int)tok, pos = tok_pos[first], row = tok_row[first], at = pos & 15;
-    if (pos < 0 || row < 0 || row >= n_rows || pos / PE_PAGE >= table_stride) return;
-    if (at && first > 0 && tok_row[first - 1] == row && tok_pos[first - 1] == pos - 1) return;      // an earlier token leads this tile
-    const bool same = lane < 16 - at && first + lane < T && tok_row[first + lane] == row && tok_pos[first + lane] == pos + lane;
-    const int n = __ffs(~__ballot_sync(0xffffffffu, same)) - 1;                                     // tokens of the tile
-    const int page = block_table[(size_t)row * table_stride + pos / PE_PAGE];
-    if (page < 0 || page >= n_pages) return;
-    unsigned char* block = pool + ((size_t)page * n_kv + kvh) * B::bytes;
-    const int p0 = pos % PE_PAGE;
-
-    constexpr int lanes = D / 8, per_pass = 32 / lanes, half = D / 2;
-    const int w = lane % lanes, b = w >> 2, t = w & 3, ch = w * 8, j = ch % half;
-    for (int i0 = 0; i0 < n; i0 += per_pass) {
-        const int i = i0 + lane / lanes;
-        const bool mine = i < n;
-        const bf16* src = qkv + (size_t)(first + (mine ? i : 0)) * row_width + (size_t)(n_q + kvh) * D;
-        float x[8];
-        q4_load8<D>(src + ch, x);
+    const int kvh = blockIdx.x % n_kv, first = (int)(blockIdx.x / n_kv) * SI_TOKENS;
+    if (threadIdx.x < SI_TOKENS) {
+        const int i = first + threadIdx.x, pos = i < T ? tok_pos[i] : -1, row = i < T ? tok_row[i] : -1;
+        int page = -1;
+        if (pos >= 0 && row >= 0 && row < n_rows && pos / PE_PAGE < table_stride) page = block_table[(size_t)row * table_stride + pos / PE_PAGE];
+        at_pos[threadIdx.x] = pos; at_row[threadIdx.x] = row; at_page[threadIdx.x] = page < n_pages ? page : -1;
+    }
+    constexpr int lanes = D / 8, half = D / 2;
+    const int w = threadIdx.x % lanes, i = threadIdx.x / lanes, b = w >> 2, t = w & 3, ch = w * 8, j = ch % half;
+    float k[8], y[8], v[8];
+    float4 c0, c1, s0, s1;
+    const bool mine = i < SI_TOKENS && first + i < T;                  // (of 128 channels a thread each, of 64 half the threads have none: whole warps)
+    if (mine) {
+        const bf16* src = qkv + (size_t)(first + i) * row_width + (size_t)(n_q + kvh) * D;
+        q4_load8<D>(src + ch, k);
+        q4_load8<D>(src + (size_t)n_kv * D + ch, v);
         if (cos_t) {
-            float y[8];
             q4_load8<D>(src + (ch < half ? ch + half : ch - half), y);
-            const size_t a = (size_t)min(pos + (mine ? i : 0), angles - 1) * half + j;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const double c = cos_t[a + e], s = sin_t[a + e];
-                const double r = ch < half ? (double)x[e] * c - (double)y[e] * s : (double)y[e] * s + (double)x[e] * c;
-                x[e] = __bfloat162float(__float2bfloat16_rn((float)r));
-            }
+            const size_t a = (size_t)min(max(tok_pos[first + i], 0), angles - 1) * half + j;
+            const float4* cp = reinterpret_cast<const float4*>(cos_t + a);
+            const float4* sp = reinterpret_cast<const float4*>(sin_t + a);
+            c0 = cp[0]; c1 = cp[1]; s0 = sp[0]; s1 = sp[1];
         }
+    }
+    __syncthreads();
+    if (i < SI_TOKENS) {                                               // (a warp as one: the groups' shuffles)
+        const int pos = at_pos[i], page = mine ? at_page[i] : -1, p = pos & (PE_PAGE - 1);
+        if (mine && cos_t) {
+            const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) k[e] = __bfloat162float(__float2bfloat16_rn(q4_turned(k[e], c[e], ch < half ? -y[e] : y[e], s[e])));
+        }
+        unsigned char* block = pool + ((size_t)max(page, 0) * n_kv + kvh) * B::bytes;
         int level[8];
         bf16 step, mid;
-        q4_group(x, level, step, mid);
-        unsigned word = 0;
+        q4_group(k, level, step, mid);
+        if (page >= 0) {
+            unsigned word = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) word |= q4_turn(q4_field(level[2 * e]) | q4_field(level[2 * e + 1]) << 16, e);
-        const int p = p0 + i;
-        if (mine) {
+            for (int e = 0; e < 4; ++e) word |= q4_turn(q4_field(level[2 * e]) | q4_field(level[2 * e + 1]) << 16, e);
             *reinterpret_cast<unsigned*>(block + q4_key_word<D>(p, b, t)) = word;
-            if (t == 0) {
-                bf16* meta = reinterpret_cast<bf16*>(block + q4_key_step<D>(p, b));
-                meta[0] = step; meta[B::groups] = mid;
-            }
+            bf16* meta = reinterpret_cast<bf16*>(block + q4_key_step<D>(p, b));
+            if (t == 0) meta[0] = step;
+            if (t == 1) meta[B::groups] = mid;
         }
-        q4_load8<D>(src + (size_t)n_kv * D + ch, x);
-        q4_group(x, level, step, mid);
-        if (mine) {
+        q4_group(v, level, step, mid);
+        if (page >= 0) {
             unsigned f[2] = {0u, 0u};
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e >> 2] |= (unsigned)((level[e] ^ (level[e] >> 31)) | (level[e] < 0 ? 8 : 0)) << (8 * (e & 3));
-            *reinterpret_cast<uint2*>(&fields[warp][at + i][ch]) = make_uint2(f[0], f[1]);
-            if (t == 0) {
-                bf16* meta = reinterpret_cast<bf16*>(block + q4_value_step<D>(p, b));
-                meta[0] = step; meta[B::groups * 16] = mid;
-            }
+            *reinterpret_cast<uint2*>(&fields[i][ch]) = make_uint2(f[0], f[1]);
+            bf16* meta = reinterpret_cast<bf16*>(block + q4_value_step<D>(p, b));
+            if (t == 0) meta[0] = step;
+            if (t == 1) meta[B::groups * 16] = mid;
         }
     }
-    __syncwarp();
-    // the tile's words: four positions (those of the call), two channels
-    const int g = lane >> 2, tt = lane & 3;
-    unsigned own = 0;
+    __syncthreads();
+    // the words of a token's values: token, g, word of the two of a group's four channels
+    constexpr int words = D / 2;
+#pragma unroll 2
+    for (int x = threadIdx.x; x < SI_TOKENS * words; x += SI_THREADS) {
+        const int n = x / words, rest = x % words, m = rest >> 3, g = rest & 7;                     // m: as in the block's layout
+        if (at_page[n] < 0) continue;
+        const int pos = at_pos[n], r = pos & 15, tt = (r & 7) >> 1;
+        // the word's other positions that the block has: they follow this token or stand before it
+        const auto there = [&](int to) {                                // token n + to - r of this tile: position `to` of it
+            const int o = n + to - r;
+            return o >= 0 && o < SI_TOKENS && at_row[o] == at_row[n] && at_pos[o] == pos + to - r && at_page[o] >= 0;
+        };
+        unsigned own = 0, word = 0;
+        bool leads = true;
 #pragma unroll
-    for (int f = 0; f < 2; ++f)
+        for (int f = 0; f < 2; ++f)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int r = 8 * f + 2 * tt + e;
-            if (r >= at && r < at + n) own |= q4_position_bits(f, e);
-        }
-    if (!own) return;
-#pragma unroll
-    for (int h = 0; h < B::halves; ++h) {
-        uint4* dst = reinterpret_cast<uint4*>(block + q4_value_words<D>(p0 >> 4, h, g, tt));
-        unsigned out[4];
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            unsigned word = 0;
-#pragma unroll
-            for (int f = 0; f < 2; ++f)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const unsigned two = *reinterpret_cast<const unsigned short*>(&fields[warp][8 * f + 2 * tt + e][32 * (2 * h + (m >> 1)) + 4 * g + 2 * (m & 1)]);
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const unsigned code = two >> (8 * c);
-                        word |= q4_turn((((code & 8u) << 12) | ((code & 7u) << 4)) << (16 * e), 2 * f + c);
-                    }
-                }
-            out[m] = word;
-        }
-        if (own != ~0u) {
-            const uint4 old = *dst;
-            out[0] = (out[0] & own) | (old.x & ~own); out[1] = (out[1] & own) | (old.y & ~own);
-            out[2] = (out[2] & own) | (old.z & ~own); out[3] = (out[3] & own) | (old.w & ~own);
-        }
-        *dst = make_uint4(out[0], out[1], out[2], out[3]);
+            for (int e = 0; e < 2; ++e) {
+                const int to = 8 * f + 2 * tt + e;
+                if (!there(to)) continue;
+                if (to < r) leads = false;
+                const unsigned two = *reinterpret_cast<const unsigned short*>(&fields[n + to - r][32 * (m >> 1) + 4 * g + 2 * (m & 1)]);
+                own |= q4_position_bits(f, e);
+                word |= q4_turn((((two & 8u) << 12) | ((two & 7u) << 4)) << (16 * e), 2 * f) | q4_turn((((two & 0x800u) << 4) | ((two & 0x700u) >> 4)) << (16 * e), 2 * f + 1);
+            }
+        if (!leads) continue;
+        unsigned* dst = reinterpret_cast<unsigned*>(pool + ((size_t)at_page[n] * n_kv + kvh) * B::bytes + q4_value_words<D>((pos & (PE_PAGE - 1)) >> 4, m >> 2, g, tt)) + (m & 3);
+        if (own == ~0u) *dst = word;
+        else { atomicAnd(dst, ~own); atomicOr(dst, word); }
     }
 }
 
@@ -184,18 +191,18 @@ extern "C" int pe_store_int4(const void* qkv, int T, int n_q, int n_kv, int hd, 
     if (T <= 0) return 0;
     if ((hd != 64 && hd != 128) || n_q <= 0 || n_kv <= 0 || (((uintptr_t)qkv | (uintptr_t)pool | (uintptr_t)q_out) & 15)) return PE_ERR_UNSUPPORTED;
     if (cos_t && (angles <= 0 || (((uintptr_t)cos_t | (uintptr_t)sin_t) & 15))) return PE_ERR_UNSUPPORTED;
-    const long long items = (long long)T * n_q * (hd / 16), units = (long long)T * n_kv, threads = 32 * SI_WARPS;
-    const long long q_blocks = (items + threads - 1) / threads, blocks = q_blocks + (units + SI_WARPS - 1) / SI_WARPS;
+    const long long items = (long long)T * ((n_q + SI_HEADS - 1) / SI_HEADS) * (hd / 16), q_blocks = (items + SI_THREADS - 1) / SI_THREADS;
+    const long long kv_blocks = (long long)((T + SI_TOKENS - 1) / SI_TOKENS) * n_kv, blocks = q_blocks + kv_blocks, threads = SI_THREADS;
     if (blocks > 0x7fffffffll) return PE_ERR_UNSUPPORTED;
     auto kernel = hd == 64 ? store_int4_kernel<64> : store_int4_kernel<128>;
     PE_TRY(pe_launch(kernel, dim3((unsigned)blocks), dim3((unsigned)threads), 0, (cudaStream_t)stream, (const bf16*)qkv, T, n_q, n_kv, cos_t, sin_t, angles, tok_pos,
-                     tok_row, (unsigned char*)pool, n_pages, block_table, table_stride, n_rows, (bf16*)q_out, (int)q_blocks));
+                     tok_row, (unsigned char*)pool, n_pages, block_table, table_stride, n_rows, (bf16*)q_out, (int)kv_blocks));
     PE_LAUNCH_CHECK();
     return 0;
 }
 
 // ---------------------------------------------------------------------------- rows read back
-// A thread reads eight channels of a key and of a value.  Rows whose page is not there are zeros.
+// A thread reads four channels of a key and of a value.  Rows whose page is not there are zeros.
 
 template <int D>
 __global__ void __launch_bounds__(256) load_int4_kernel(const unsigned char* pool, long long n_pages, int n_kv, const int* tok_pos, const int* tok_row, int T,
@@ -204,48 +211,35 @@ __global__ void __launch_bounds__(256) load_int4_kernel(const unsigned char* poo
     pdl_launch_dependents();
     pdl_wait();
     const long long item = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    const int w = (int)(item % (D / 8)), kvh = (int)(item / (D / 8) % n_kv);
-    const long long tok = item / (D / 8) / n_kv;
+    const int part = (int)(item % (D / 4)), kvh = (int)(item / (D / 4) % n_kv), b = part >> 3, g = part & 7;
+    const long long tok = item / (D / 4) / n_kv;
     if (tok >= T) return;
-    const int pos = tok_pos[tok], row = tok_row[tok], b = w >> 2, t = w & 3;
+    const int pos = tok_pos[tok], row = tok_row[tok];
     int page = -1;
     if (pos >= 0 && row >= 0 && row < n_rows && pos / PE_PAGE < table_stride) page = block_table[(size_t)row * table_stride + pos / PE_PAGE];
-    float k[8], v[8];
-    if (page < 0 || page >= n_pages) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) k[e] = v[e] = 0.f;
-    } else {
+    float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+    if (page >= 0 && page < n_pages) {
         const unsigned char* block = pool + ((size_t)page * n_kv + kvh) * B::bytes;
-        const int p = pos % PE_PAGE, r = p & 15, f = r >> 3, tt = (r & 7) >> 1, e1 = r & 1;
-        const unsigned word = *reinterpret_cast<const unsigned*>(block + q4_key_word<D>(p, b, t));
+        const int p = pos % PE_PAGE, r = p & 15, f = r >> 3, e = r & 1, i = (g & 1) * 2;
+        const unsigned word = *reinterpret_cast<const unsigned*>(block + q4_key_word<D>(p, b, g >> 1));
+        const uint2 two = *reinterpret_cast<const uint2*>(block + q4_value_words<D>(p >> 4, b >> 1, g, (r & 7) >> 1) + (b & 1) * 8);
         const bf16* km = reinterpret_cast<const bf16*>(block + q4_key_step<D>(p, b));
         const bf16* vm = reinterpret_cast<const bf16*>(block + q4_value_step<D>(p, b));
         const float ks = to_f(km[0]), kc = to_f(km[B::groups]), vs = to_f(vm[0]), vc = to_f(vm[B::groups * 16]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) k[e] = fmaf(ks, q4_level(word, e >> 1, e & 1), kc);
-#pragma unroll
-        for (int g2 = 0; g2 < 2; ++g2)
-#pragma unroll
-            for (int m2 = 0; m2 < 2; ++m2) {
-                const int m = 2 * b + m2;
-                const unsigned vw = *reinterpret_cast<const unsigned*>(block + q4_value_words<D>(p >> 4, m >> 2, 2 * t + g2, tt) + (m & 3) * 4);
-                v[4 * g2 + 2 * m2] = fmaf(vs, q4_level(vw, 2 * f, e1), vc);
-                v[4 * g2 + 2 * m2 + 1] = fmaf(vs, q4_level(vw, 2 * f + 1, e1), vc);
-            }
+        k = make_float4(fmaf(ks, q4_level(word, i, 0), kc), fmaf(ks, q4_level(word, i, 1), kc), fmaf(ks, q4_level(word, i + 1, 0), kc), fmaf(ks, q4_level(word, i + 1, 1), kc));
+        v = make_float4(fmaf(vs, q4_level(two.x, 2 * f, e), vc), fmaf(vs, q4_level(two.x, 2 * f + 1, e), vc), fmaf(vs, q4_level(two.y, 2 * f, e), vc),
+                        fmaf(vs, q4_level(two.y, 2 * f + 1, e), vc));
     }
-    const size_t to = ((size_t)tok * n_kv + kvh) * D + w * 8;
-#pragma unroll
-    for (int e = 0; e < 8; e += 4) {
-        *reinterpret_cast<float4*>(keys + to + e) = make_float4(k[e], k[e + 1], k[e + 2], k[e + 3]);
-        *reinterpret_cast<float4*>(values + to + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-    }
+    const size_t to = ((size_t)tok * n_kv + kvh) * D + part * 4;
+    *reinterpret_cast<float4*>(keys + to) = k;
+    *reinterpret_cast<float4*>(values + to) = v;
 }
 
 extern "C" int pe_load_int4(const void* pool, long long n_pages, int n_kv, int hd, const int* tok_pos, const int* tok_row, int T, const int* block_table, int table_stride,
                             int n_rows, float* keys, float* values, void* stream) {
     if (T <= 0) return 0;
     if ((hd != 64 && hd != 128) || n_kv <= 0 || (((uintptr_t)pool | (uintptr_t)keys | (uintptr_t)values) & 15)) return PE_ERR_UNSUPPORTED;
-    const long long blocks = ((long long)T * n_kv * (hd / 8) + 255) / 256;
+    const long long blocks = ((long long)T * n_kv * (hd / 4) + 255) / 256;
     if (blocks > 0x7fffffffll) return PE_ERR_UNSUPPORTED;
     auto kernel = hd == 64 ? load_int4_kernel<64> : load_int4_kernel<128>;
     PE_TRY(pe_launch(kernel, dim3((unsigned)blocks), dim3(256), 0, (cudaStream_t)stream, (const unsigned char*)pool, n_pages, n_kv, tok_pos, tok_row, T, block_table,
@@ -255,51 +249,61 @@ extern "C" int pe_load_int4(const void* pool, long long n_pages, int n_kv, int h
 }
 
 // ---------------------------------------------------------------------------- the bounds of a page's keys
-// A warp a token and head: where the token is the last of its page, the least and the greatest of the page's keys, channel by channel, in float32, rounded to bfloat16.
+// A block looks at sixteen tokens of a key head.  Of the page of each that is the last of its page: the least and the greatest key, channel by channel, in float32, rounded to bfloat16.
 
 template <int D>
 __global__ void __launch_bounds__(256) page_bounds_kernel(const unsigned char* pool, long long n_pages, int n_kv, const int* tok_pos, const int* tok_row, int T,
                                                           const int* block_table, int table_stride, int n_rows, bf16* bounds) {
     using B = Int4Block<D>;
+    __shared__ float ends[2][8][D];
     pdl_launch_dependents();
     pdl_wait();
-    const int lane = threadIdx.x & 31;
-    const long long unit = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    const int kvh = (int)(unit % n_kv);
-    const long long tok = unit / n_kv;
-    if (tok >= T) return;
-    const int pos = tok_pos[tok], row = tok_row[tok];
-    if (pos < 0 || pos % PE_PAGE != PE_PAGE - 1 || row < 0 || row >= n_rows || pos / PE_PAGE >= table_stride) return;
-    const int page = block_table[(size_t)row * table_stride + pos / PE_PAGE];
-    if (page < 0 || page >= n_pages) return;
-    const unsigned char* block = pool + ((size_t)page * n_kv + kvh) * B::bytes;
-    constexpr int lanes = D / 8, per_pass = 32 / lanes;
-    const int w = lane % lanes, b = w >> 2, t = w & 3;
-    float lo[8], hi[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) { lo[e] = INFINITY; hi[e] = -INFINITY; }
-#pragma unroll 4
-    for (int p = lane / lanes; p < PE_PAGE; p += per_pass) {
-        const unsigned word = *reinterpret_cast<const unsigned*>(block + q4_key_word<D>(p, b, t));
-        const bf16* km = reinterpret_cast<const bf16*>(block + q4_key_step<D>(p, b));
-        const float s = to_f(km[0]), c = to_f(km[B::groups]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float x = fmaf(s, q4_level(word, e >> 1, e & 1), c);
-            lo[e] = q4_min(lo[e], x); hi[e] = q4_max(hi[e], x);
-        }
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kvh = blockIdx.x % n_kv, first = (int)(blockIdx.x / n_kv) * 16;
+    int page = -1;
+    if (lane < 16 && first + lane < T) {                       // (every warp for itself)
+        const int pos = tok_pos[first + lane], row = tok_row[first + lane];
+        if (pos >= 0 && pos % PE_PAGE == PE_PAGE - 1 && row >= 0 && row < n_rows && pos / PE_PAGE < table_stride) page = block_table[(size_t)row * table_stride + pos / PE_PAGE];
+        if (page >= n_pages) page = -1;
     }
+    constexpr int lanes = D / 8, rows = 256 / lanes;           // threads a key, keys at a time
+    const int w = threadIdx.x % lanes, b = w >> 2, t = w & 3;
+    for (unsigned left = __ballot_sync(0xffffffffu, page >= 0); left; left &= left - 1) {
+        const int its = __shfl_sync(0xffffffffu, page, __ffs(left) - 1);
+        const unsigned char* block = pool + ((size_t)its * n_kv + kvh) * B::bytes;
+        float lo[8], hi[8];
 #pragma unroll
-    for (int o = lanes; o < 32; o <<= 1)
+        for (int e = 0; e < 8; ++e) { lo[e] = INFINITY; hi[e] = -INFINITY; }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            lo[e] = q4_min(lo[e], __shfl_xor_sync(0xffffffffu, lo[e], o));
-            hi[e] = q4_max(hi[e], __shfl_xor_sync(0xffffffffu, hi[e], o));
+        for (int k = 0; k < PE_PAGE / rows; ++k) {
+            const int p = k * rows + threadIdx.x / lanes;
+            const unsigned word = *reinterpret_cast<const unsigned*>(block + q4_key_word<D>(p, b, t));
+            const bf16* km = reinterpret_cast<const bf16*>(block + q4_key_step<D>(p, b));
+            const float s = to_f(km[0]), c = to_f(km[B::groups]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float x = fmaf(s, q4_level(word, e >> 1, e & 1), c);
+                lo[e] = q4_min(lo[e], x); hi[e] = q4_max(hi[e], x);
+            }
         }
-    if (lane < lanes) {
-        bf16* to = bounds + ((size_t)page * n_kv + kvh) * 2 * D + w * 8;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) { to[e] = __float2bfloat16_rn(lo[e]); to[D + e] = __float2bfloat16_rn(hi[e]); }
+        for (int o = lanes; o < 32; o <<= 1)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                lo[e] = q4_min(lo[e], __shfl_xor_sync(0xffffffffu, lo[e], o));
+                hi[e] = q4_max(hi[e], __shfl_xor_sync(0xffffffffu, hi[e], o));
+            }
+        if (lane < lanes)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { ends[0][warp][w * 8 + e] = lo[e]; ends[1][warp][w * 8 + e] = hi[e]; }
+        __syncthreads();
+        if (threadIdx.x < 2 * D) {
+            const int side = threadIdx.x / D, d = threadIdx.x % D;
+            float x = ends[side][0][d];
+#pragma unroll
+            for (int k = 1; k < 8; ++k) x = side ? q4_max(x, ends[1][k][d]) : q4_min(x, ends[0][k][d]);
+            bounds[(((size_t)its * n_kv + kvh) * 2 + side) * D + d] = __float2bfloat16_rn(x);
+        }
+        __syncthreads();
     }
 }
 
@@ -307,7 +311,7 @@ extern "C" int pe_page_bounds(const void* pool, long long n_pages, int n_kv, int
                               int table_stride, int n_rows, void* bounds, void* stream) {
     if (T <= 0) return 0;
     if ((hd != 64 && hd != 128) || n_kv <= 0 || (((uintptr_t)pool | (uintptr_t)bounds) & 15)) return PE_ERR_UNSUPPORTED;
-    const long long blocks = ((long long)T * n_kv + 7) / 8;
+    const long long blocks = (long long)((T + 15) / 16) * n_kv;
     if (blocks > 0x7fffffffll) return PE_ERR_UNSUPPORTED;
     auto kernel = hd == 64 ? page_bounds_kernel<64> : page_bounds_kernel<128>;
     PE_TRY(pe_launch(kernel, dim3((unsigned)blocks), dim3(256), 0, (cudaStream_t)stream, (const unsigned char*)pool, n_pages, n_kv, tok_pos, tok_row, T, block_table,
