@@ -8,8 +8,8 @@
 // A query head is turned as the model's table says, in float32, and rounded once.  A key is turned with twice float32's bits and rounded once more to bfloat16, the type in which
 // a 16-bit cache would hold it: what is coded next to the border of two codes then does not depend on the order of two roundings in float32.
 // A block takes sixteen tokens of a key head as they stand behind one another, eight channels of key and value a thread.  A word of the values' codes holds four positions: the first
-// of its tokens in the block gathers those that follow it in their sequence.  A word that the block has in part only (a tile that lies across two blocks, or begins
-// or ends with the call) is changed bit for bit by two atomic operations, so whoever has the others may write them at the same time, and they keep what nobody writes.
+// of its tokens in the block gathers those that follow it in their sequence.  A word keeps the bits of positions that are not in the call; one of a
+// tile that lies across two blocks is changed bit for bit by two atomic operations, so the other block may change its own at the same time.
 template <int D>
 __device__ __forceinline__ void q4_load8(const bf16* p, float (&x)[8]) {
     const uint4 v = *reinterpret_cast<const uint4*>(p);
@@ -18,19 +18,18 @@ __device__ __forceinline__ void q4_load8(const bf16* p, float (&x)[8]) {
     for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
 }
 
-#define SI_HEADS 4                                             // query heads a thread, which share the angles it reads
-
-template <int D>
+// HEADS query heads a thread, which share the angles it reads
+template <int D, int HEADS>
 __device__ __forceinline__ void store_queries(const bf16* qkv, int row_width, int n_q, const float* cos_t, const float* sin_t, int angles,
                                               const int* tok_pos, bf16* q_out, long long item) {
     constexpr int half = D / 2, parts = half / 8;
-    const int runs = (n_q + SI_HEADS - 1) / SI_HEADS, part = (int)(item % parts), run = (int)(item / parts % runs), t = (int)(item / parts / runs), j = part * 8;
-    const bf16* src = qkv + (size_t)t * row_width + run * SI_HEADS * D + j;
-    bf16* dst = q_out + ((size_t)t * n_q + run * SI_HEADS) * D + j;
-    const int heads = min(SI_HEADS, n_q - run * SI_HEADS);
-    uint4 lo[SI_HEADS], hi[SI_HEADS];
+    const int runs = (n_q + HEADS - 1) / HEADS, part = (int)(item % parts), run = (int)(item / parts % runs), t = (int)(item / parts / runs), j = part * 8;
+    const bf16* src = qkv + (size_t)t * row_width + run * HEADS * D + j;
+    bf16* dst = q_out + ((size_t)t * n_q + run * HEADS) * D + j;
+    const int heads = min(HEADS, n_q - run * HEADS);
+    uint4 lo[HEADS], hi[HEADS];
 #pragma unroll
-    for (int h = 0; h < SI_HEADS; ++h)
+    for (int h = 0; h < HEADS; ++h)
         if (h < heads) { lo[h] = *reinterpret_cast<const uint4*>(src + h * D); hi[h] = *reinterpret_cast<const uint4*>(src + h * D + half); }
     if (cos_t) {
         const size_t at = (size_t)min(max(tok_pos[t], 0), angles - 1) * half + j;
@@ -39,7 +38,7 @@ __device__ __forceinline__ void store_queries(const bf16* qkv, int row_width, in
         const float4 c0 = cp[0], c1 = cp[1], s0 = sp[0], s1 = sp[1];
         const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
 #pragma unroll
-        for (int h = 0; h < SI_HEADS; ++h) {
+        for (int h = 0; h < HEADS; ++h) {
             __nv_bfloat162* l2 = reinterpret_cast<__nv_bfloat162*>(&lo[h]);
             __nv_bfloat162* h2 = reinterpret_cast<__nv_bfloat162*>(&hi[h]);
 #pragma unroll
@@ -51,7 +50,7 @@ __device__ __forceinline__ void store_queries(const bf16* qkv, int row_width, in
         }
     }
 #pragma unroll
-    for (int h = 0; h < SI_HEADS; ++h)
+    for (int h = 0; h < HEADS; ++h)
         if (h < heads) { *reinterpret_cast<uint4*>(dst + h * D) = lo[h]; *reinterpret_cast<uint4*>(dst + h * D + half) = hi[h]; }
 }
 
@@ -66,9 +65,9 @@ __device__ __forceinline__ void q4_group(const float (&x)[8], int (&level)[8], b
         hi = q4_max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
     q4_scale(lo, hi, step, mid);
-    const float s = __bfloat162float(step), m = __bfloat162float(mid);
+    const float s = __bfloat162float(step), m = __bfloat162float(mid), by = s == 0.f ? 0.f : 1.f / s;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) level[i] = q4_quantise(x[i], s, m);
+    for (int i = 0; i < 8; ++i) level[i] = q4_quantise(x[i], s, m, by);
 }
 
 // a c - b s (or a s + b c) rounded to float32 as if from twice as many bits: products with their errors, and the error of their sum
@@ -79,41 +78,49 @@ __device__ __forceinline__ float q4_turned(float a, float c, float b, float s) {
     return fabsf(d) < INFINITY ? r : d;
 }
 
-#define SI_THREADS 256
+#define SI_THREADS 512
 #define SI_TOKENS 16
 
-template <int D>
-__global__ void __launch_bounds__(SI_THREADS) store_int4_kernel(const bf16* qkv, int T, int n_q, int n_kv, const float* cos_t, const float* sin_t, int angles,
+template <int D, int HEADS>
+__global__ void __launch_bounds__(SI_THREADS, 2) store_int4_kernel(const bf16* qkv, int T, int n_q, int n_kv, const float* cos_t, const float* sin_t, int angles,
                                                                 const int* tok_pos, const int* tok_row, unsigned char* pool, long long n_pages,
                                                                 const int* block_table, int table_stride, int n_rows, bf16* q_out, int kv_blocks) {
     using B = Int4Block<D>;
     __shared__ __align__(16) unsigned char fields[SI_TOKENS][D];       // the values' codes: sign << 3 | magnitude
-    __shared__ int at_pos[SI_TOKENS], at_row[SI_TOKENS], at_page[SI_TOKENS];    // page -1: the token is not stored
+    __shared__ int near_pos[3 * SI_TOKENS], near_row[3 * SI_TOKENS], at_page[SI_TOKENS];    // of the tokens before the block's, its own and those behind; page -1: not stored
+    const int* const at_pos = near_pos + SI_TOKENS;
+    const int* const at_row = near_row + SI_TOKENS;
+    __shared__ int leaders[SI_TOKENS], n_leaders, parts[SI_TOKENS];     // first tokens of words; the tokens of a leader's four positions (2 f + e), a byte each, 255: not here
+    __shared__ unsigned owns[SI_TOKENS];                                // the bits of those
+    __shared__ bool alone[SI_TOKENS];                                   // nobody else has a part of them
     pdl_launch_dependents();
     pdl_wait();
     const int row_width = (n_q + 2 * n_kv) * D;
     if ((int)blockIdx.x >= kv_blocks) {                                 // (behind the keys' blocks, which take longer)
         const long long item = (long long)(blockIdx.x - kv_blocks) * blockDim.x + threadIdx.x;
-        if (item < (long long)T * ((n_q + SI_HEADS - 1) / SI_HEADS) * (D / 16)) store_queries<D>(qkv, row_width, n_q, cos_t, sin_t, angles, tok_pos, q_out, item);
+        if (item < (long long)T * ((n_q + HEADS - 1) / HEADS) * (D / 16)) store_queries<D, HEADS>(qkv, row_width, n_q, cos_t, sin_t, angles, tok_pos, q_out, item);
         return;
     }
     const int kvh = blockIdx.x % n_kv, first = (int)(blockIdx.x / n_kv) * SI_TOKENS;
-    if (threadIdx.x < SI_TOKENS) {
-        const int i = first + threadIdx.x, pos = i < T ? tok_pos[i] : -1, row = i < T ? tok_row[i] : -1;
-        int page = -1;
-        if (pos >= 0 && row >= 0 && row < n_rows && pos / PE_PAGE < table_stride) page = block_table[(size_t)row * table_stride + pos / PE_PAGE];
-        at_pos[threadIdx.x] = pos; at_row[threadIdx.x] = row; at_page[threadIdx.x] = page < n_pages ? page : -1;
+    if (threadIdx.x < 3 * SI_TOKENS) {
+        const int n = threadIdx.x - SI_TOKENS, i = first + n, pos = i >= 0 && i < T ? tok_pos[i] : -1, row = i >= 0 && i < T ? tok_row[i] : -1;
+        near_pos[threadIdx.x] = pos; near_row[threadIdx.x] = row;
+        if (n >= 0 && n < SI_TOKENS) {
+            int page = -1;
+            if (pos >= 0 && row >= 0 && row < n_rows && pos / PE_PAGE < table_stride) page = block_table[(size_t)row * table_stride + pos / PE_PAGE];
+            at_page[n] = page < n_pages ? page : -1;
+        }
     }
     constexpr int lanes = D / 8, half = D / 2;
-    const int w = threadIdx.x % lanes, i = threadIdx.x / lanes, b = w >> 2, t = w & 3, ch = w * 8, j = ch % half;
-    float k[8], y[8], v[8];
+    const bool keys = threadIdx.x < SI_THREADS / 2;                     // the first half of the threads keys, the second values
+    const int w = threadIdx.x % lanes, i = threadIdx.x % (SI_THREADS / 2) / lanes, b = w >> 2, t = w & 3, ch = w * 8, j = ch % half;
+    float x[8], y[8];
     float4 c0, c1, s0, s1;
-    const bool mine = i < SI_TOKENS && first + i < T;                  // (of 128 channels a thread each, of 64 half the threads have none: whole warps)
+    const bool mine = i < SI_TOKENS && first + i < T;                  // (of 64 channels half of either have none: whole warps)
     if (mine) {
-        const bf16* src = qkv + (size_t)(first + i) * row_width + (size_t)(n_q + kvh) * D;
-        q4_load8<D>(src + ch, k);
-        q4_load8<D>(src + (size_t)n_kv * D + ch, v);
-        if (cos_t) {
+        const bf16* src = qkv + (size_t)(first + i) * row_width + (size_t)(n_q + (keys ? 0 : n_kv) + kvh) * D;
+        q4_load8<D>(src + ch, x);
+        if (keys && cos_t) {
             q4_load8<D>(src + (ch < half ? ch + half : ch - half), y);
             const size_t a = (size_t)min(max(tok_pos[first + i], 0), angles - 1) * half + j;
             const float4* cp = reinterpret_cast<const float4*>(cos_t + a);
@@ -122,66 +129,76 @@ __global__ void __launch_bounds__(SI_THREADS) store_int4_kernel(const bf16* qkv,
         }
     }
     __syncthreads();
+    if (threadIdx.x < 32) {
+        const int n = threadIdx.x, r = n < SI_TOKENS ? at_pos[n] & 15 : 0;
+        bool leads = n < SI_TOKENS && at_page[n] >= 0;
+        unsigned own = 0, from = ~0u;
+        bool mine = true;
+        if (leads)
+#pragma unroll
+            for (int f = 0; f < 2; ++f)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int to = 8 * f + (r & 6) + e, o = n + to - r;                             // the token of position `to` of the tile
+                    if (at_row[o] != at_row[n] || at_pos[o] != at_pos[n] + to - r) continue;
+                    if (o < 0 || o >= SI_TOKENS) { mine = false; continue; }                        // another block's
+                    if (at_page[o] < 0) continue;
+                    leads &= to >= r;
+                    own |= q4_position_bits(f, e);
+                    from &= ~(255u << (8 * (2 * f + e))) | (unsigned)o << (8 * (2 * f + e));
+                }
+        const unsigned set = __ballot_sync(0xffffffffu, leads);
+        if (leads) { leaders[__popc(set & ((1u << n) - 1u))] = n; owns[n] = own; parts[n] = (int)from; alone[n] = mine; }
+        if (n == 0) n_leaders = __popc(set);
+    }
     if (i < SI_TOKENS) {                                               // (a warp as one: the groups' shuffles)
-        const int pos = at_pos[i], page = mine ? at_page[i] : -1, p = pos & (PE_PAGE - 1);
-        if (mine && cos_t) {
+        const int page = mine ? at_page[i] : -1, p = at_pos[i] & (PE_PAGE - 1);
+        if (mine && keys && cos_t) {
             const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) k[e] = __bfloat162float(__float2bfloat16_rn(q4_turned(k[e], c[e], ch < half ? -y[e] : y[e], s[e])));
+            for (int e = 0; e < 8; ++e) x[e] = __bfloat162float(__float2bfloat16_rn(q4_turned(x[e], c[e], ch < half ? -y[e] : y[e], s[e])));
         }
         unsigned char* block = pool + ((size_t)max(page, 0) * n_kv + kvh) * B::bytes;
         int level[8];
         bf16 step, mid;
-        q4_group(k, level, step, mid);
-        if (page >= 0) {
+        q4_group(x, level, step, mid);
+        if (page >= 0 && keys) {
             unsigned word = 0;
 #pragma unroll
             for (int e = 0; e < 4; ++e) word |= q4_turn(q4_field(level[2 * e]) | q4_field(level[2 * e + 1]) << 16, e);
             *reinterpret_cast<unsigned*>(block + q4_key_word<D>(p, b, t)) = word;
-            bf16* meta = reinterpret_cast<bf16*>(block + q4_key_step<D>(p, b));
-            if (t == 0) meta[0] = step;
-            if (t == 1) meta[B::groups] = mid;
         }
-        q4_group(v, level, step, mid);
-        if (page >= 0) {
+        if (page >= 0 && !keys) {
             unsigned f[2] = {0u, 0u};
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e >> 2] |= (unsigned)((level[e] ^ (level[e] >> 31)) | (level[e] < 0 ? 8 : 0)) << (8 * (e & 3));
             *reinterpret_cast<uint2*>(&fields[i][ch]) = make_uint2(f[0], f[1]);
-            bf16* meta = reinterpret_cast<bf16*>(block + q4_value_step<D>(p, b));
-            if (t == 0) meta[0] = step;
-            if (t == 1) meta[B::groups * 16] = mid;
+        }
+        if (page >= 0 && t < 2) {
+            bf16* meta = reinterpret_cast<bf16*>(block + (keys ? q4_key_step<D>(p, b) : q4_value_step<D>(p, b)));
+            if (t == 0) meta[0] = step; else meta[keys ? B::groups : B::groups * 16] = mid;
         }
     }
     __syncthreads();
-    // the words of a token's values: token, g, word of the two of a group's four channels
+    // the words of the leaders' positions: m and g as in the block's layout
     constexpr int words = D / 2;
-#pragma unroll 2
-    for (int x = threadIdx.x; x < SI_TOKENS * words; x += SI_THREADS) {
-        const int n = x / words, rest = x % words, m = rest >> 3, g = rest & 7;                     // m: as in the block's layout
-        if (at_page[n] < 0) continue;
-        const int pos = at_pos[n], r = pos & 15, tt = (r & 7) >> 1;
-        // the word's other positions that the block has: they follow this token or stand before it
-        const auto there = [&](int to) {                                // token n + to - r of this tile: position `to` of it
-            const int o = n + to - r;
-            return o >= 0 && o < SI_TOKENS && at_row[o] == at_row[n] && at_pos[o] == pos + to - r && at_page[o] >= 0;
-        };
-        unsigned own = 0, word = 0;
-        bool leads = true;
+    for (int x = threadIdx.x; x < n_leaders * words; x += SI_THREADS) {
+        const int n = leaders[x / words], rest = x % words, m = rest & (D / 16 - 1), g = rest / (D / 16), from = parts[n];
+        unsigned word = 0;
 #pragma unroll
         for (int f = 0; f < 2; ++f)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int to = 8 * f + 2 * tt + e;
-                if (!there(to)) continue;
-                if (to < r) leads = false;
-                const unsigned two = *reinterpret_cast<const unsigned short*>(&fields[n + to - r][32 * (m >> 1) + 4 * g + 2 * (m & 1)]);
-                own |= q4_position_bits(f, e);
+                const int o = (from >> (8 * (2 * f + e))) & 255;
+                if (o == 255) continue;
+                const unsigned two = *reinterpret_cast<const unsigned short*>(&fields[o][32 * (m >> 1) + 4 * g + 2 * (m & 1)]);
                 word |= q4_turn((((two & 8u) << 12) | ((two & 7u) << 4)) << (16 * e), 2 * f) | q4_turn((((two & 0x800u) << 4) | ((two & 0x700u) >> 4)) << (16 * e), 2 * f + 1);
             }
-        if (!leads) continue;
-        unsigned* dst = reinterpret_cast<unsigned*>(pool + ((size_t)at_page[n] * n_kv + kvh) * B::bytes + q4_value_words<D>((pos & (PE_PAGE - 1)) >> 4, m >> 2, g, tt)) + (m & 3);
+        const int p = at_pos[n] & (PE_PAGE - 1);
+        unsigned* dst = reinterpret_cast<unsigned*>(pool + ((size_t)at_page[n] * n_kv + kvh) * B::bytes + q4_value_words<D>(p >> 4, m >> 2, g, (p & 7) >> 1)) + (m & 3);
+        const unsigned own = owns[n];
         if (own == ~0u) *dst = word;
+        else if (alone[n]) *dst = (*dst & ~own) | word;
         else { atomicAnd(dst, ~own); atomicOr(dst, word); }
     }
 }
@@ -191,10 +208,13 @@ extern "C" int pe_store_int4(const void* qkv, int T, int n_q, int n_kv, int hd, 
     if (T <= 0) return 0;
     if ((hd != 64 && hd != 128) || n_q <= 0 || n_kv <= 0 || (((uintptr_t)qkv | (uintptr_t)pool | (uintptr_t)q_out) & 15)) return PE_ERR_UNSUPPORTED;
     if (cos_t && (angles <= 0 || (((uintptr_t)cos_t | (uintptr_t)sin_t) & 15))) return PE_ERR_UNSUPPORTED;
-    const long long items = (long long)T * ((n_q + SI_HEADS - 1) / SI_HEADS) * (hd / 16), q_blocks = (items + SI_THREADS - 1) / SI_THREADS;
+    // one head a thread where the queries are few (its chain is what takes time), two where they fill the GPU (angles are read once for them)
+    const bool few = (long long)T * n_q * (hd / 16) <= pe_sm_count() * 2048ll;
+    const int runs = few ? n_q : (n_q + 1) / 2;
+    const long long items = (long long)T * runs * (hd / 16), q_blocks = (items + SI_THREADS - 1) / SI_THREADS;
     const long long kv_blocks = (long long)((T + SI_TOKENS - 1) / SI_TOKENS) * n_kv, blocks = q_blocks + kv_blocks, threads = SI_THREADS;
     if (blocks > 0x7fffffffll) return PE_ERR_UNSUPPORTED;
-    auto kernel = hd == 64 ? store_int4_kernel<64> : store_int4_kernel<128>;
+    auto kernel = hd == 64 ? (few ? store_int4_kernel<64, 1> : store_int4_kernel<64, 2>) : few ? store_int4_kernel<128, 1> : store_int4_kernel<128, 2>;
     PE_TRY(pe_launch(kernel, dim3((unsigned)blocks), dim3((unsigned)threads), 0, (cudaStream_t)stream, (const bf16*)qkv, T, n_q, n_kv, cos_t, sin_t, angles, tok_pos,
                      tok_row, (unsigned char*)pool, n_pages, block_table, table_stride, n_rows, (bf16*)q_out, (int)kv_blocks));
     PE_LAUNCH_CHECK();

@@ -59,9 +59,12 @@ __device__ __forceinline__ void q4_scale(float lo, float hi, bf16& step, bf16& m
     mid = none ? __ushort_as_bfloat16(0x7fffu) : __float2bfloat16_rn(m);
     step = none ? __ushort_as_bfloat16(0x7fffu) : __float2bfloat16_rn(s);
 }
-__device__ __forceinline__ int q4_quantise(float x, float step, float mid) {
-    const float l = floorf((x - mid) / step);
-    return step == 0.f ? 0 : (int)fminf(fmaxf(l, -8.f), 7.f);
+// floor((x - mid) / step) within the levels; `by`: 1 / step (0 for a step of 0).  The quotient is rounded to the nearest integer through its last bits; the rest, exact in sign,
+// says whether that lies above it.
+__device__ __forceinline__ int q4_quantise(float x, float step, float mid, float by) {
+    const float d = x - mid, r = __fmaf_rn(d, by, 12582912.f), n = r - 12582912.f;
+    const int l = __float_as_int(r) - 0x4b400000 - (__fmaf_rn(-n, step, d) < 0.f ? 1 : 0);
+    return min(max(l, -8), 7);
 }
 
 // byte offsets within a block

@@ -2333,8 +2333,11 @@ def select_pages(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int, 
     table = torch.empty(T * n_kv_heads, keep, dtype=torch.int32, device=q.device)
     pos = torch.empty(T * n_kv_heads, dtype=torch.int32, device=q.device)
     if T:
+        most = min((max_context - 1) // PAGE + 1, table_stride)
+        scores = torch.empty(T * n_kv_heads * most, dtype=torch.int64, device=q.device)       # (the call's own: calls on two streams and captured graphs share none)
         check(long_context().pe_select_pages(q.data_ptr(), q_stride, T, n_heads, n_kv_heads, head_dim, bounds.data_ptr(), bounds.shape[0], block_table.data_ptr(), table_stride, rows,
-                                             tok_pos.data_ptr(), tok_row.data_ptr(), keep, int(max_context), table.data_ptr(), pos.data_ptr(), stream), "select_pages")
+                                             tok_pos.data_ptr(), tok_row.data_ptr(), keep, int(max_context), table.data_ptr(), pos.data_ptr(), scores.data_ptr(), stream), "select_pages",
+              2 if most > keep > 2 else 1)
     return SelectedPages(table, pos)
 
 

@@ -146,7 +146,7 @@ _LONG_SIGNATURES = {
     "pe_store_int4": [P, I, I, I, I, P, P, I, P, P, P, LL, P, I, I, P, P],
     "pe_load_int4": [P, LL, I, I, P, P, I, P, I, I, P, P, P],
     "pe_page_bounds": [P, LL, I, I, P, P, I, P, I, I, P, P],
-    "pe_select_pages": [P, I, I, I, I, I, P, LL, P, I, I, P, P, I, I, P, P, P],
+    "pe_select_pages": [P, I, I, I, I, I, P, LL, P, I, I, P, P, I, I, P, P, P, P],
     "pe_attention_int4": [P, I, P, P, LL, P, I, I, P, P, I, I, I, I, I, F, I, I, I, P, P],
     "pe_expand_int4": [P, LL, I, I, P, I, P, I, I, I, P, P, P, P],
 }
