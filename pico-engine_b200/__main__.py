@@ -5,7 +5,7 @@ meanings: ``--prompt``, ``--max-tokens 64``, ``--temperature 0.7`` (0 is greedy)
 ``--top-k 0``, ``--no-graph``.  There is no tokenizer in this library, so ``--prompt`` takes token
 ids ("5,17,3"; repeat the option for a batch) and the output is token ids; ``--seed``,
 ``--dtype``, ``--stop-token-ids``, ``--n`` and the rules on what may be said (``--repetition-penalty``, ``--presence-penalty``, ``--frequency-penalty``,
-``--logit-bias``) are additions.  Without a model folder, ``--random-config NAME``
+``--logit-bias``) are additions, and so are ``--cache int4`` and ``--attend-pages``.  Without a model folder, ``--random-config NAME``
 draws the weights of a named shape from ``--seed`` and ``--random-prompt LEN[,LEN...]`` draws
 prompts, so that random weights become tokens in one line.  ``--n-gpu-layers`` (offload of
 another architecture) is not taken.
@@ -61,6 +61,8 @@ def main(argv=None) -> None:
     p.add_argument("--frequency-penalty", type=float, default=0.0, help="the same times how often they are there")
     p.add_argument("--logit-bias", type=parse_bias, default=[], metavar="ID:VALUE[,ID:VALUE...]", help="added to logits")
     p.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    p.add_argument("--cache", choices=["int4"], help="hold keys and values in 4 bits (bfloat16 grouped attention with heads of 64 or 128)")
+    p.add_argument("--attend-pages", type=int, metavar="N", help="with --cache int4: a decoded token attends to N pages of 64 positions at most")
     p.add_argument("--no-graph", action="store_true", help="disable CUDA-graph decode and launch every kernel")
     args = p.parse_args(argv)
 
@@ -86,6 +88,8 @@ def main(argv=None) -> None:
         p.error(f"model folder has no config.json: {args.model}")
     if args.n < 1:
         p.error("--n must be at least 1")
+    if args.attend_pages is not None and (args.cache is None or args.attend_pages < 1):
+        p.error("--attend-pages must be positive and goes with --cache int4")
     if args.max_tokens < 0:
         p.error("--max-tokens must be non-negative")
     prompts = [parse_ids(t) for t in (args.prompt or [])]
@@ -111,9 +115,9 @@ def main(argv=None) -> None:
     from .engine.engine import Engine
     t0 = time.perf_counter()
     if config is not None:
-        eng = Engine.from_config(config, seed=args.seed, dtype=args.dtype)
+        eng = Engine.from_config(config, seed=args.seed, dtype=args.dtype, cache=args.cache, attend_pages=args.attend_pages)
     else:
-        eng = Engine(args.model, dtype=args.dtype)
+        eng = Engine(args.model, dtype=args.dtype, cache=args.cache, attend_pages=args.attend_pages)
     load_s = time.perf_counter() - t0
     t0 = time.perf_counter()
     outs = eng.generate(prompts, args.max_tokens, args.temperature, args.top_k, args.top_p,

@@ -102,9 +102,17 @@ def kv_bytes_per_token(engine) -> int:
     itemsize = torch.empty(0, dtype=engine.dtype).element_size()
     for need in engine.model.cache_needs():
         if need is not None and need.kv is not None:
-            v_heads, v_dim = need.kv.value_shape
-            total += (need.kv.n_kv_heads * need.kv.head_dim + v_heads * v_dim) * itemsize
+            total += _position_bytes(engine, need.kv, itemsize)
     return total
+
+
+def _position_bytes(engine, kv, itemsize: int) -> float:
+    """Bytes of the keys and values of one position and layer."""
+    if engine.int4 and kv.may_be_int4:
+        from .ops.kernels import PAGE, int4_page_bytes
+        return kv.n_kv_heads * int4_page_bytes(kv.head_dim) / PAGE
+    v_heads, v_dim = kv.value_shape
+    return (kv.n_kv_heads * kv.head_dim + v_heads * v_dim) * itemsize
 
 
 def decode_step_bytes(engine, batch: int, mean_context: float) -> float:
@@ -116,9 +124,11 @@ def decode_step_bytes(engine, batch: int, mean_context: float) -> float:
         if need is None:
             continue
         if need.kv is not None:
-            v_heads, v_dim = need.kv.value_shape
             seen = mean_context if need.kv.window is None else min(mean_context, need.kv.window)
-            total += batch * seen * (need.kv.n_kv_heads * need.kv.head_dim + v_heads * v_dim) * itemsize
+            if engine.attend_pages is not None and need.kv.window is None and need.kv.may_be_int4 and mean_context > 64 * engine.attend_pages:
+                total += batch * mean_context / 64 * need.kv.n_kv_heads * need.kv.head_dim * 4          # the bounds of all pages
+                seen = 64 * engine.attend_pages
+            total += batch * seen * _position_bytes(engine, need.kv, itemsize)
         if need.state_elems:
             total += 2.0 * batch * need.state_elems * (4 if need.state_dtype == "float32" else itemsize)
     return total
@@ -423,6 +433,8 @@ def main(argv=None) -> None:
     p.add_argument("--warmups", type=int, default=2)
     p.add_argument("--repetitions", type=int, default=3)
     p.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    p.add_argument("--cache", choices=["int4"], help="hold keys and values in 4 bits")
+    p.add_argument("--attend-pages", type=int, metavar="N", help="with --cache int4: a decoded token attends to N pages at most")
     p.add_argument("--no-graph", action="store_true", help="decode without CUDA graphs")
     p.add_argument("--output", help="write the JSON record here")
     p.add_argument("--save-choices", metavar="FILE", help="write which implementation each matrix product got (ops.linear.Choice); "
@@ -445,9 +457,9 @@ def main(argv=None) -> None:
         if args.layers:
             from .config.shapes import with_layers
             d = with_layers(d, args.layers)
-        eng = Engine.from_config(config_from_dict(d), seed=args.seed, draw_on="cuda", dtype=args.dtype)
+        eng = Engine.from_config(config_from_dict(d), seed=args.seed, draw_on="cuda", dtype=args.dtype, cache=args.cache, attend_pages=args.attend_pages)
     else:
-        eng = Engine(args.model, dtype=args.dtype)
+        eng = Engine(args.model, dtype=args.dtype, cache=args.cache, attend_pages=args.attend_pages)
     batches = [int(x) for x in args.batch.split(",") if x]
     if batches:
         eng.ensure_cache(max(batches) * ((args.context + 63) // 64) * 64, args.context, max_seqs=max(batches))

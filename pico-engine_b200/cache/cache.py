@@ -18,6 +18,8 @@ sequence.
 * Values may have another head size and another number of heads than keys (``KVNeed.v_head_dim``, ``v_heads``): the
   pools are then shaped accordingly (this library's attention kernels take equal shapes; a mixer that asks for
   others brings the kernel that reads them).
+* A cache made with ``int4`` holds the groups that take it (``KVNeed.may_be_int4``) in 4 bits: one tensor ``k [entry, page, kv head, bytes]`` (``kernels.int4_pool``: a page and head's
+  keys and values in a block) and no ``v``; with ``bounds`` those without a window also have ``bounds [entry, page, kv head, 2, head_dim]``, the least and the greatest key of every full page.
 * A sequence may be *forked* (``fork``): the new ones begin with its positions.  Whole pages are shared, a page that is not full yet is copied (each
   sequence goes on in its own), and so is the state.  A shared page is free again when its last sequence has given it back.
 * Beside what sequences hold there is one *idle* slot with one page in every group (``idle_slot``,
@@ -51,22 +53,28 @@ def pages_for(tokens: int) -> int:
 class KVGroup:
     need: KVNeed
     entries: List[int]                    # schedule entries that own storage here, in order
-    k: Optional[torch.Tensor]             # [len(entries), pages, n_kv_heads, PAGE, head_dim]
+    k: Optional[torch.Tensor]             # [len(entries), pages, n_kv_heads, PAGE, head_dim], or uint8 [.., n_kv_heads, bytes] with the values (int4)
     v: Optional[torch.Tensor]
     pages: FreeList
     table: Dict[int, List[int]]           # slot -> physical page of each logical page (-1: given back)
+    int4: bool = False
+    bounds: Optional[torch.Tensor] = None
+
+    def pools(self) -> List[torch.Tensor]:
+        """What holds the pages: tensors [entry, page, ..]."""
+        return [t for t in (self.k, self.v, self.bounds) if t is not None]
 
     def bytes(self) -> int:
-        return 0 if self.k is None else (self.k.numel() + self.v.numel()) * self.k.element_size()      # with the idle page
+        return sum(t.numel() * t.element_size() for t in self.pools())      # with the idle page
 
 
 class Cache:
     """``needs[e]`` is what schedule entry ``e`` asks for (None for an entry that reads
     another entry's cache or needs nothing).  ``max_tokens`` is the most tokens live sequences
-    hold at any time, each sequence's count rounded up to PAGE."""
+    hold at any time, each sequence's count rounded up to PAGE.  ``int4``: groups that take it are held in 4 bits; ``bounds``: with the bounds of their pages' keys."""
 
     def __init__(self, needs: Sequence[Optional[CacheNeeds]], max_tokens: int, max_seqs: int, dtype: torch.dtype,
-                 device, allocate: bool = True):
+                 device, allocate: bool = True, int4: bool = False, bounds: bool = False):
         if max_tokens <= 0 or max_seqs <= 0:
             raise ValueError("the cache needs room for at least one token and one sequence")
         self.dtype, self.device = dtype, torch.device(device)
@@ -86,7 +94,7 @@ class Cache:
                 continue
             if n.kv not in by_need:
                 by_need[n.kv] = len(self.groups)
-                self.groups.append(KVGroup(n.kv, [], None, None, FreeList(self.n_pages, "page"), {}))
+                self.groups.append(KVGroup(n.kv, [], None, None, FreeList(self.n_pages, "page"), {}, int4 and n.kv.may_be_int4))
             g = by_need[n.kv]
             self.group_of[e] = g
             self.index_in_group[e] = len(self.groups[g].entries)
@@ -97,6 +105,12 @@ class Cache:
         if allocate:
             for g in self.groups:
                 v_heads, v_dim = g.need.value_shape
+                if g.int4:
+                    from ..ops.kernels import int4_page_bytes
+                    g.k = torch.zeros((len(g.entries), self.n_pages + 1, g.need.n_kv_heads, int4_page_bytes(g.need.head_dim)), dtype=torch.uint8, device=self.device)
+                    if bounds and g.need.window is None:
+                        g.bounds = torch.zeros((len(g.entries), self.n_pages + 1, g.need.n_kv_heads, 2, g.need.head_dim), dtype=torch.bfloat16, device=self.device)
+                    continue
                 g.k = torch.zeros((len(g.entries), self.n_pages + 1, g.need.n_kv_heads, PAGE, g.need.head_dim),
                                   dtype=dtype, device=self.device)
                 g.v = torch.zeros((len(g.entries), self.n_pages + 1, v_heads, PAGE, v_dim), dtype=dtype, device=self.device)
@@ -147,7 +161,7 @@ class Cache:
                 g.pages.share(p for p in row[:whole] if p >= 0)
                 g.table[s] = row[:whole] + ([page] if part else [])
             if g.k is not None and part and row[whole] >= 0 and n:
-                for pool in (g.k, g.v):
+                for pool in g.pools():
                     pool[:, own] = pool[:, row[whole]:row[whole] + 1].clone()
         for t in self.state.values():
             t[new] = t[slot:slot + 1].clone()
@@ -217,10 +231,15 @@ class Cache:
 
     # ------------------------------------------------------------------ what a mixer sees
     def pools(self, entry: int):
-        """(k, v) [page, kv head, PAGE, head_dim] of a schedule entry that owns storage."""
+        """(k, v) [page, kv head, PAGE, head_dim] of a schedule entry that owns storage; in 4 bits (k [page, kv head, bytes], None)."""
         g = self.groups[self.group_of[entry]]
         i = self.index_in_group[entry]
-        return g.k[i], g.v[i]
+        return g.k[i], None if g.v is None else g.v[i]
+
+    def bounds_of(self, entry: int) -> Optional[torch.Tensor]:
+        """[page, kv head, 2, head_dim] of a schedule entry whose group has the bounds of its pages' keys, else None."""
+        g = self.groups[self.group_of[entry]]
+        return None if g.bounds is None else g.bounds[self.index_in_group[entry]]
 
     def state_of(self, entry: int) -> Optional[torch.Tensor]:
         """[slot, elems] float32 of an entry with state, else None."""

@@ -11,13 +11,15 @@ class KVNeed:
     of a sequence's first f positions as well.
     ``v_head_dim``: the size of a value head where it is not the keys' (None: the same); ``v_heads``: the
     number of value heads where it is not the keys' (a cache that keeps one compressed row per position
-    asks for one key head and no value head: ``v_heads=0``)."""
+    asks for one key head and no value head: ``v_heads=0``).  ``may_be_int4``: the mixer also takes pages of 4-bit codes, where the
+    cache is made so."""
     n_kv_heads: int
     head_dim: int
     window: Optional[int] = None
     v_head_dim: Optional[int] = None
     v_heads: Optional[int] = None
     keep_first: int = 0
+    may_be_int4: bool = False
 
     @property
     def value_shape(self):

@@ -79,8 +79,8 @@ class StepLayout:
 class Stepper:
     """Owns nothing but scratch: it drives ``model`` over ``cache``."""
 
-    def __init__(self, model, cache: Cache, max_context: int):
-        self.model, self.cache, self.max_context = model, cache, max_context
+    def __init__(self, model, cache: Cache, max_context: int, attend_pages: Optional[int] = None):
+        self.model, self.cache, self.max_context, self.attend_pages = model, cache, max_context, attend_pages
         self.device = cache.device
         self.vocab = model.plan.vocab_size
         self._ring: List[list] = [[None, None] for _ in range(4)]     # pinned staging buffers and their copy events
@@ -115,6 +115,8 @@ class Stepper:
             return False
         most = 0                                 # of a layer: the bytes of shared keys and values that rows after the first do not read again
         for g in self.cache.groups:
+            if g.int4:                           # (read row by row)
+                continue
             heads, dim = g.need.value_shape
             a_position = 2 * (g.need.n_kv_heads * g.need.head_dim + heads * dim)
             most = max(most, sum((n - 1) * min(shared, g.need.window or shared) * a_position for n, shared, _ in members))
@@ -266,7 +268,7 @@ class Stepper:
             slots=dev[lay.slots: lay.slots + lay.B], row_first=dev[lay.first: lay.first + lay.B + 1],
             row_lens=dev[lay.lens: lay.lens + lay.B], slot_ids=list(slot_ids), lens=list(lens), starts=list(starts),
             one_token_each=all(n == 1 for n in lens), cache=self.cache, tables=tables,
-            max_context=max(s + n for s, n in zip(starts, lens)))
+            max_context=max(s + n for s, n in zip(starts, lens)), attend_pages=self.attend_pages)
 
     def upload(self, host: np.ndarray, dev: Optional[torch.Tensor] = None) -> torch.Tensor:
         slot, staged = self._stage(host)

@@ -65,13 +65,40 @@ class GQAAttention(Mixer):
     # ------------------------------------------------------------------ cache and step
     def cache_needs(self):
         s = self.spec
-        return CacheNeeds(kv=KVNeed(s.n_kv_heads, s.head_dim, s.window))
+        from .position import NoPosition, RotaryHalf
+        return CacheNeeds(kv=KVNeed(s.n_kv_heads, s.head_dim, s.window, may_be_int4=type(self.position) in (RotaryHalf, NoPosition) and s.scale > 0 and
+                                    kernels.int4_takes(self.dtype, s.n_heads, s.n_kv_heads, s.head_dim)))
+
+    def _attend_int4(self, qkv, ctx, kv, owns_cache):
+        """The same from the products' rows on, over a cache of 4 bits."""
+        s = self.spec
+        place = (kv.table, kv.stride)
+        if owns_cache:
+            cos, sin = self._tables(ctx)
+            q = kernels.store_int4(qkv, s.n_heads, s.n_kv_heads, s.head_dim, cos, sin, ctx.tok_pos, ctx.tok_row, kv.k, *place)
+            if kv.bounds is not None:
+                kernels.page_bounds(kv.k, s.n_kv_heads, s.head_dim, ctx.tok_pos, ctx.tok_row, *place, kv.bounds)
+        else:
+            self.position.rotate_and_store(qkv, s.n_heads, s.n_kv_heads, s.head_dim, ctx, None)
+            q = qkv
+        heads = (q, q.shape[1], s.n_heads, s.n_kv_heads, s.head_dim)
+        if not ctx.one_token_each:
+            tiles = ctx.scratch.get("prefill_tiles_128")
+            if tiles is None:
+                tiles = ctx.scratch["prefill_tiles_128"] = kernels.prefill_tiles(ctx.lens, ctx.starts, q.device, kernels.PREFILL_TILE_TCGEN05)
+            return kernels.attention_int4_prompt(*heads, kv.k, *place, tiles, ctx.T, s.window, s.scale)
+        if kv.bounds is not None and ctx.attend_pages is not None and ctx.max_context > ctx.attend_pages * kernels.PAGE:
+            pages = kernels.select_pages(*heads, kv.bounds, *place, ctx.tok_pos, ctx.tok_row, ctx.attend_pages, ctx.max_context)
+            return kernels.attention_int4_selected(*heads, kv.k, pages, s.scale)
+        return kernels.attention_int4(*heads, kv.k, *place, ctx.tok_pos, ctx.tok_row, s.window, s.scale, ctx.max_context, early_pages=owns_cache)
 
     def _attend(self, h, ctx, cache_entry, owns_cache):
         from ..ops.linear import qkv_rope_store, qkv_rope_store_takes
         from .position import NoPosition, RotaryHalf
         s = self.spec
         kv = ctx.kv(cache_entry)
+        if kv.v is None:
+            return self._attend_int4(linear(h, self.w_qkv, self.b_qkv, out_dtype=ctx.dtype), ctx, kv, owns_cache)
         if type(self.position) in (RotaryHalf, NoPosition) and qkv_rope_store_takes(h, self.w_qkv, self.b_qkv, s.head_dim):
             # many rows in bfloat16: projection, bias, rotation and cache write can be one tcgen05 kernel
             cos, sin = self._tables(ctx)
@@ -113,6 +140,10 @@ class GQAAttention(Mixer):
             ctx.settle(x)
             s = self.spec
             kv = ctx.kv(cache_entry)
+            if kv.v is None:
+                qkv = kernels.linear_fused(None, self.w_qkv, self.b_qkv, out_dtype=ctx.dtype, norm_of=x, norm_weight=norm.weight, eps=norm.eps)
+                kernels.linear_fused(self._attend_int4(qkv, ctx, kv, owns_cache), self.w_o, accumulate_into=x)
+                return
             cos, sin = self._tables(ctx)
             q = kernels.norm_qkv_rope_store(x, norm.weight, norm.eps, self.w_qkv, self.b_qkv, s.n_heads, s.n_kv_heads,
                                             s.head_dim, cos, sin, ctx.tok_pos, ctx.tok_row,

@@ -44,11 +44,12 @@ from ..weights.loader import ParamSpec
 @dataclass
 class KVView:
     """Keys and values of one schedule entry for the running step."""
-    k: torch.Tensor               # [page, kv head, PAGE, head_dim]
-    v: torch.Tensor
+    k: torch.Tensor               # [page, kv head, PAGE, head_dim]; in 4 bits uint8 [page, kv head, bytes] with the values, and v is None
+    v: Optional[torch.Tensor]
     table: torch.Tensor           # int32 [B, stride]: physical page of each logical page of each batch row
     stride: int
     window: Optional[int]
+    bounds: Optional[torch.Tensor] = None      # [page, kv head, 2, head_dim]: of the keys of full pages, where tokens attend to selected pages
 
 
 @dataclass
@@ -84,6 +85,7 @@ class StepContext:
     pending_norm: Optional["Norm"] = None   # the norm that product passes on its way into the stream (None: it is added as it is)
     pending_streams: Optional["Part"] = None  # how it enters a residual of several streams (a StreamMix)
     pending_rows: Optional[tuple] = None    # (rows [T, hidden], weights [T]): rows times a number a token that are added with the pending product
+    attend_pages: Optional[int] = None    # pages that single tokens attend to in groups with bounds (None: all)
     stream_source: Optional[torch.Tensor] = None  # the one matrix [T, hidden] that all streams still equal, before the first sum into them
 
     # A part whose product comes out of the library may leave the sum into the residual stream pending, so
@@ -156,7 +158,7 @@ class StepContext:
         g = self.cache.group_of[cache_entry]
         k, v = self.cache.pools(cache_entry)
         t = self.tables[g]
-        return KVView(k, v, t, t.shape[1], self.cache.groups[g].need.window)
+        return KVView(k, v, t, t.shape[1], self.cache.groups[g].need.window, self.cache.bounds_of(cache_entry))
 
     def state(self, cache_entry: int) -> Optional[torch.Tensor]:
         """[slot, elems] float32; row ``slots[b]`` is batch row b's state."""
