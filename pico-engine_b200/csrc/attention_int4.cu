@@ -191,8 +191,7 @@ __device__ __forceinline__ void ai_values(AiState<D>& s, const unsigned (&w)[4][
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const unsigned char* vm = block + B::value_meta + j * (4 * NB * 16) + t * 8;
-        uint2 mids = make_uint2(0u, 0u);
-        if (g < NB) mids = *reinterpret_cast<const uint2*>(vm + (NB + g) * 32);
+        const uint2 mids = *reinterpret_cast<const uint2*>(vm + (NB + (g & (NB - 1))) * 32);       // (rows from NB on are sums that nobody reads)
         ai_mma(s.mids, mids.x, 0u, mids.y, 0u, w[j][0], w[j][1]);
 #pragma unroll
         for (int h = 0; h < B::halves; ++h) {
@@ -231,11 +230,16 @@ __device__ __forceinline__ void ai_bar_expect(unsigned bar, unsigned bytes) {
 __device__ __forceinline__ void ai_bulk_copy(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-// true when the phase with this parity has completed; false when the wait ran out
-__device__ __forceinline__ bool ai_bar_wait(unsigned bar, unsigned parity) {
+__device__ __forceinline__ void ai_bar_arrive(unsigned bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// true when the phase with this parity has completed; a wait is false when it runs out
+__device__ __forceinline__ bool ai_bar_test(unsigned bar, unsigned parity) {
     unsigned done;
     asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-    if (done) return true;
+    return done != 0u;
+}
+__device__ __forceinline__ bool ai_bar_wait(unsigned bar, unsigned parity) {
+    unsigned done;
+    if (ai_bar_test(bar, parity)) return true;
     const long long deadline = clock64() + AI_WAIT_CYCLES;
     for (;;) {
         asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
@@ -262,10 +266,10 @@ __device__ __forceinline__ void ai_send4(unsigned to, float4 v, unsigned bar) {
                  "r"(__float_as_uint(v.y)), "r"(__float_as_uint(v.z)), "r"(__float_as_uint(v.w)), "r"(bar) : "memory");
 }
 
-// Warps of a CTA, blocks that a warp has places for, CTAs an SM.
-template <int D>
+// WARPS of a CTA compute and one more fetches.  Blocks that such a warp has places for, CTAs an SM.
+template <int D, int WARPS>
 struct AiShape {
-    static constexpr int warps = 4, stages = 2, ctas = D == 64 ? 4 : 2;
+    static constexpr int warps = WARPS, stages = 2, ctas = D == 64 && WARPS < 8 ? 2 : 1, threads = 32 * (warps + 1);
     static constexpr int row = D + 4;                          // floats of a head's results: D sums, largest score, sum of weights
     static constexpr int blocks = warps * stages * Int4Block<D>::bytes, parts = warps * 8 * row * 4;
     static constexpr int ring = ((blocks > parts ? blocks : parts) + 127) / 128 * 128;    // the warps' results lie in the ring later
@@ -273,103 +277,114 @@ struct AiShape {
     static constexpr int smem = ring + gather;
 };
 
-template <int D>
-__global__ void __launch_bounds__(32 * AiShape<D>::warps, AiShape<D>::ctas) attention_int4_kernel(
+template <int D, int WARPS>
+__global__ void __launch_bounds__(AiShape<D, WARPS>::threads, AiShape<D, WARPS>::ctas) attention_int4_kernel(
     const bf16* q, int q_stride, const unsigned char* pool, int n_blocks, const int* block_table, int table_stride, int n_rows, const int* tok_pos, const int* tok_row,
     int n_heads, int n_kv, int window, float scale_log2e, int selected, int n_splits, int early, int* status, bf16* out) {
-    using S = AiShape<D>;
+    using S = AiShape<D, WARPS>;
     using B = Int4Block<D>;
-    constexpr int WARPS = S::warps;
     extern __shared__ __align__(128) unsigned char ai_ring[];   // [warp][stage] blocks; later the warps' results; behind it what the other CTAs send
-    __shared__ __align__(8) unsigned long long bars[WARPS * S::stages + 1];
+    __shared__ __align__(8) unsigned long long bars[2 * WARPS * S::stages + 1];           // per warp and stage: a block is there; its place is free
+    __shared__ int filled[WARPS * S::stages];                  // whether the stage holds a block (a page may not be there)
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int split = n_splits > 1 ? (int)ai_cluster_rank() : 0, slice = D / n_splits;
     float* gather = reinterpret_cast<float*>(ai_ring + S::ring);                          // [split][8][slice + 4]
-    const unsigned gather0 = ai_smem(gather), gbar = ai_smem(&bars[WARPS * S::stages]);
+    const unsigned gather0 = ai_smem(gather), full0 = ai_smem(bars), empty0 = full0 + 8u * WARPS * S::stages, gbar = empty0 + 8u * WARPS * S::stages;
     const int G = n_heads / n_kv, head_tiles = (G + 7) / 8, kvh = blockIdx.y / head_tiles, h0 = (blockIdx.y % head_tiles) * 8, heads = min(8, G - h0);
-    const unsigned ring0 = ai_smem(ai_ring) + warp * S::stages * Int4Block<D>::bytes, full0 = ai_smem(&bars[warp * S::stages]);
-    if (lane == 0) {
-        for (int i = 0; i < S::stages; ++i) ai_bar_init(full0 + 8u * i, 1u);
-        if (warp == 0) ai_bar_init(gbar, 1u);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        if (warp == 0 && n_splits > 1) ai_bar_expect(gbar, (unsigned)((n_splits - 1) * heads * (slice + 4) * 4));
-    }
-    __syncwarp();
-    if (n_splits > 1) ai_cluster_arrive();                     // waited for before the first number goes to another CTA
+    if (threadIdx.x < 2 * WARPS * S::stages + 1) ai_bar_init(full0 + 8u * threadIdx.x, 1u);
+    if (threadIdx.x == 2 * WARPS * S::stages && n_splits > 1) ai_bar_expect(gbar, (unsigned)((n_splits - 1) * heads * (slice + 4) * 4));
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (!early) pdl_wait();
     const int tok = blockIdx.z, place = selected ? tok * n_kv + kvh : tok, pos = min(tok_pos[place], table_stride * PE_PAGE - 1), row = selected ? place : tok_row[tok];
-    const int lo = window > 0 ? max(0, pos - window + 1) : 0, first = lo / PE_PAGE + split * WARPS + warp, step = n_splits * WARPS;
+    __syncthreads();
+    if (n_splits > 1) ai_cluster_arrive();                     // waited for before the first number goes to another CTA
+    const int lo = window > 0 ? max(0, pos - window + 1) : 0, step = n_splits * WARPS;
     const int last = pos >= 0 && row >= 0 && row < n_rows ? pos / PE_PAGE : -1;
-    const int n = last >= first ? (last - first) / step + 1 : 0;                          // pages of this warp: first, first + step, ..
-    // the entries of the table for this warp's pages base + lane and base + 32 + lane, as blocks (-1: not there)
-    const int n_pages = selected ? n_blocks : n_blocks / n_kv;
-    const int* table = block_table + (size_t)max(0, min(row, n_rows - 1)) * table_stride;
-    const auto entry = [&](int i) {
-        if (i >= n) return -1;
-        const int page = table[first + i * step];
-        if (page < 0 || page >= n_pages) return -1;
-        return selected ? page : page * n_kv + kvh;
-    };
-    int now = entry(lane), next = entry(32 + lane);
-    int base = 0;
-    const auto block_of = [&](int i) { return __shfl_sync(0xffffffffu, i - base < 32 ? now : next, (i - base) & 31); };
-    const auto fetch = [&](int i, int stage) {
-        if (i >= n) return;
-        const int at = block_of(i);
-        if (at >= 0 && lane == 0) ai_fetch<D>(ring0 + stage * B::bytes, pool + (size_t)at * B::bytes, full0 + 8u * stage);
-    };
-    // (early: the page of the newest position is written by the kernel before this one)
-    const int settled = n - (early && n > 0 && first + (n - 1) * step == last);
-    int fetched = 0;
-    for (; fetched < min(settled, S::stages); ++fetched) fetch(fetched, fetched);
-    if (early) {
-        pdl_wait();
-        for (; fetched < min(n, S::stages); ++fetched) fetch(fetched, fetched);
-    }
     AiState<D> s;
     ai_reset(s);
-    AiQuery<D> f;
-    ai_query<D>(f, q + (size_t)tok * q_stride + (size_t)(kvh * G + h0 + g) * D, h0 + g < G, t);
-    const float scale = scale_log2e * ai_pow2(-AI_DOWN);
-    unsigned phases = 0;
-    bool dead = false;
-    for (int i = 0, stage = 0; i < n; ++i) {
-        if (i - base == 32) { base += 32; now = next; next = entry(base + 32 + lane); }
-        if (block_of(i) >= 0) {
-            if (!dead && !__all_sync(0xffffffffu, ai_bar_wait(full0 + 8u * stage, (phases >> stage) & 1u))) {
-                dead = true;
-                if (lane == 0) atomicExch(status, 21);
+    if (warp == WARPS) {
+        // ---- the warp that fetches: a lane for each of the others, whose pages are first, first + step, ..
+        const int first = lo / PE_PAGE + split * WARPS + lane;
+        const int n = lane < WARPS && last >= first ? (last - first) / step + 1 : 0;
+        const int n_pages = selected ? n_blocks : n_blocks / n_kv;
+        const int* table = block_table + (size_t)max(0, min(row, n_rows - 1)) * table_stride + first;
+        // (early: the page of the newest position is written by the kernel before this one)
+        const int settled = n - (n > 0 && first + (n - 1) * step == last);
+        bool waits = early != 0;
+        int page = n > 0 ? table[0] : -1, next = n > 1 ? table[step] : -1, stage = 0, round = 0;
+        long long deadline = 0;
+        for (int i = 0; __any_sync(0xffffffffu, i < n);) {
+            const unsigned at = (unsigned)(lane * S::stages + stage);
+            bool ready = i < n && !(waits && i >= settled);
+            if (ready && round > 0) ready = ai_bar_test(empty0 + 8u * at, (unsigned)(round - 1) & 1u);
+            if (ready) {
+                const bool there = page >= 0 && page < n_pages;
+                filled[at] = there;
+                if (there) ai_fetch<D>(ai_smem(ai_ring) + at * B::bytes, pool + (size_t)(selected ? page : page * n_kv + kvh) * B::bytes, full0 + 8u * at);
+                else ai_bar_arrive(full0 + 8u * at);
+                page = next;
+                if (++i + 1 < n) next = table[(i + 1) * step];
+                if (++stage == S::stages) { stage = 0; ++round; }
+                deadline = 0;
             }
-            phases ^= 1u << stage;
-            const int at = (first + i * step) * PE_PAGE;
-            if (!dead) ai_block<D>(s, f, ai_ring + (warp * S::stages + stage) * B::bytes, lo - at, pos - at, scale, lane);
+            if (!__any_sync(0xffffffffu, ready)) {
+                if (waits) {
+                    pdl_wait();
+                    waits = false;
+                } else if (!deadline) {
+                    deadline = clock64() + AI_WAIT_CYCLES;
+                } else if (clock64() > deadline && i < n) {
+                    atomicExch(status, 21);
+                    i = n;
+                }
+            }
         }
-        __syncwarp();
-        if (!dead) fetch(i + S::stages, stage);
-        if (++stage == S::stages) stage = 0;
+        if (waits) pdl_wait();
+    } else {
+        // ---- the warps that compute
+        if (early) pdl_wait();
+        AiQuery<D> f;
+        ai_query<D>(f, q + (size_t)tok * q_stride + (size_t)(kvh * G + h0 + g) * D, h0 + g < G, t);
+        const float scale = scale_log2e * ai_pow2(-AI_DOWN);
+        const int first = lo / PE_PAGE + split * WARPS + warp;
+        int stage = 0;
+        unsigned phase = 0;
+        for (int j = first; j <= last; j += step) {
+            const int at = warp * S::stages + stage;
+            if (!__all_sync(0xffffffffu, ai_bar_wait(full0 + 8u * at, phase))) {
+                if (lane == 0) atomicExch(status, 22);
+                break;
+            }
+            if (filled[at]) ai_block<D>(s, f, ai_ring + at * B::bytes, lo - j * PE_PAGE, pos - j * PE_PAGE, scale, lane);
+            __syncwarp();
+            if (lane == 0) ai_bar_arrive(empty0 + 8u * at);
+            if (++stage == S::stages) { stage = 0; phase ^= 1u; }
+        }
     }
 
     // ---- the warps' results, joined in shared memory (the ring is free once every warp has left its loop)
     __syncthreads();
     float* part = reinterpret_cast<float*>(ai_ring);           // [warp][8][row]
+    if (warp < WARPS) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) s.sum[h] += __shfl_xor_sync(0xffffffffu, s.sum[h], o);
-        float* to = part + (warp * 8 + 2 * t + h) * S::row;
-        if (g == 0) { to[D] = s.top[h]; to[D + 1] = s.sum[h]; }
+            for (int o = 4; o < 32; o <<= 1) s.sum[h] += __shfl_xor_sync(0xffffffffu, s.sum[h], o);
+            float* to = part + (warp * 8 + 2 * t + h) * S::row;
+            if (g == 0) { to[D] = s.top[h]; to[D + 1] = s.sum[h]; }
 #pragma unroll
-        for (int b = 0; b < B::groups; ++b) {
-            const float mid = __shfl_sync(0xffffffffu, s.mids[h], b * 4 + t) * ai_pow2(-AI_UP);
-            *reinterpret_cast<float4*>(to + 32 * b + 4 * g) =
-                make_float4(fmaf(s.acc[2 * b][h], ai_pow2(-AI_DOWN), mid), fmaf(s.acc[2 * b][2 + h], ai_pow2(-AI_DOWN), mid),
-                            fmaf(s.acc[2 * b + 1][h], ai_pow2(-AI_DOWN), mid), fmaf(s.acc[2 * b + 1][2 + h], ai_pow2(-AI_DOWN), mid));
+            for (int b = 0; b < B::groups; ++b) {
+                const float mid = __shfl_sync(0xffffffffu, s.mids[h], b * 4 + t) * ai_pow2(-AI_UP);
+                *reinterpret_cast<float4*>(to + 32 * b + 4 * g) =
+                    make_float4(fmaf(s.acc[2 * b][h], ai_pow2(-AI_DOWN), mid), fmaf(s.acc[2 * b][2 + h], ai_pow2(-AI_DOWN), mid),
+                                fmaf(s.acc[2 * b + 1][h], ai_pow2(-AI_DOWN), mid), fmaf(s.acc[2 * b + 1][2 + h], ai_pow2(-AI_DOWN), mid));
+            }
         }
     }
     __syncthreads();
     if (n_splits > 1) ai_cluster_wait();
-    for (int i = threadIdx.x; i < heads * (D / 4); i += 32 * WARPS) {
+    for (int i = threadIdx.x; i < heads * (D / 4); i += S::threads) {
         const int h = i / (D / 4), c = (i % (D / 4)) * 4;
         float m = -INFINITY, l = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -407,7 +422,7 @@ __global__ void __launch_bounds__(32 * AiShape<D>::warps, AiShape<D>::ctas) atte
         if (threadIdx.x == 0) atomicExch(status, 22);
         return;
     }
-    for (int i = threadIdx.x; i < heads * (slice / 4); i += 32 * WARPS) {
+    for (int i = threadIdx.x; i < heads * (slice / 4); i += S::threads) {
         const int h = i / (slice / 4), c = (i % (slice / 4)) * 4;
         float m = -INFINITY, l = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -425,19 +440,278 @@ __global__ void __launch_bounds__(32 * AiShape<D>::warps, AiShape<D>::ctas) atte
     }
 }
 
-namespace {
+// ---------------------------------------------------------------------------- many pages: every warp an equal run of them
+//
+// The blocks of all pairs (a place and a tile of eight heads) stand in one row, and each warp takes an equal run of that row, whatever it cuts: rows of unequal lengths keep all
+// SMs busy to the end.  A place is a token with its page table: a token of the step, or, over selected pages, a token's key head.  What a warp finds for a pair that it has alone
+// it writes; of the others (the first and the last of its run at most) it leaves the sums in a place of its own, and a second kernel joins them.
+
+#define AI_LEAST 4                                             // blocks a warp takes at least
+#define AI_MAX_PLACES 1024
+
 template <int D>
+struct AiStream {
+    static constexpr int warps = D == 64 ? 15 : 11, stages = 2, threads = 32 * (warps + 1), row = D + 4, ring = warps * stages * Int4Block<D>::bytes;
+};
+
+struct AiPlaces {
+    const int* tok_pos; const int* tok_row; const int* block_table;
+    int n, table_stride, n_rows, n_pages, n_kv, n_heads, head_tiles, window, selected;
+    __device__ __forceinline__ int pairs() const { return selected ? head_tiles : n_kv * head_tiles; }      // of a place
+    __device__ __forceinline__ int position(int place) const { return min(tok_pos[place], table_stride * PE_PAGE - 1); }
+    __device__ __forceinline__ int first_seen(int pos) const { return window > 0 ? max(0, pos - window + 1) : 0; }
+    // pages of a place; one that sees nothing has a page that is not there
+    __device__ __forceinline__ int pages(int place) const {
+        const int pos = position(place);
+        return pos < 0 ? 1 : pos / PE_PAGE - first_seen(pos) / PE_PAGE + 1;
+    }
+    __device__ __forceinline__ void heads_of(int place, int pair, int& tok, int& kvh, int& h0) const {
+        tok = selected ? place / n_kv : place;
+        kvh = selected ? place % n_kv : pair / head_tiles;
+        h0 = pair % head_tiles * 8;
+    }
+};
+
+// Warps that share so many blocks.
+__device__ __forceinline__ int ai_workers(int blocks, int most) { return min(most, max(1, blocks / AI_LEAST)); }
+// The block that warp w's run begins with.
+__device__ __forceinline__ int ai_begin(int w, int blocks, int workers) { return (int)((long long)w * blocks / workers); }
+
+// The number of pages before every place, prefix[n] that of all, into shared memory.
+template <int THREADS>
+__device__ __forceinline__ void ai_prefix(const AiPlaces& p, int* prefix, int* warp_sums) {
+    const int each = (p.n + THREADS - 1) / THREADS, from = min(p.n, (int)threadIdx.x * each), to = min(p.n, from + each), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int sum = 0;
+    for (int i = from; i < to; ++i) { const int n = p.pages(i); prefix[i] = n; sum += n; }
+    int before = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, before, o); if (lane >= o) before += v; }
+    if (lane == 31) warp_sums[warp] = before;
+    before -= sum;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) if (w < warp) before += warp_sums[w];
+    for (int i = from; i < to; ++i) { const int n = prefix[i]; prefix[i] = before; before += n; }
+    if (from < p.n && to == p.n) prefix[p.n] = before;
+    __syncthreads();
+}
+
+// Where a block of the row lies: the place, the pair of the place, the page among the place's pages.
+struct AiAt { int place, pair, page, pages; };
+__device__ __forceinline__ AiAt ai_find(int x, int pairs, int n, const int* prefix) {
+    const int y = x / pairs;
+    int lo = 0, hi = n;
+    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (prefix[mid] <= y) lo = mid; else hi = mid; }
+    const int pages = prefix[lo + 1] - prefix[lo], rest = x - prefix[lo] * pairs, pair = rest / pages;
+    return {lo, pair, rest - pair * pages, pages};
+}
+// The block behind it (there is one); true where another pair begins.
+__device__ __forceinline__ bool ai_next(AiAt& a, int pairs, const int* prefix) {
+    if (++a.page < a.pages) return false;
+    a.page = 0;
+    if (++a.pair == pairs) { a.pair = 0; ++a.place; a.pages = prefix[a.place + 1] - prefix[a.place]; }
+    return true;
+}
+
+template <int D>
+__global__ void __launch_bounds__(AiStream<D>::threads, 1) attention_int4_stream_kernel(const bf16* q, int q_stride, const unsigned char* pool, const AiPlaces p, float scale_log2e,
+                                                                                        int early, int most, float* partial, int* prefix_out, int* status, bf16* out) {
+    using S = AiStream<D>;
+    using B = Int4Block<D>;
+    constexpr int WARPS = S::warps;
+    extern __shared__ __align__(128) unsigned char ai_ring[];   // [warp][stage] blocks, then the prefix
+    __shared__ __align__(8) unsigned long long bars[2 * WARPS * S::stages];
+    __shared__ int filled[WARPS * S::stages], warp_sums[S::threads / 32];
+    int* prefix = reinterpret_cast<int*>(ai_ring + S::ring);
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const unsigned full0 = ai_smem(bars), empty0 = full0 + 8u * WARPS * S::stages;
+    if (threadIdx.x < 2 * WARPS * S::stages) ai_bar_init(full0 + 8u * threadIdx.x, 1u);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (!early) pdl_wait();
+    ai_prefix<S::threads>(p, prefix, warp_sums);                // (its barriers also make those of the ring known)
+    const int pairs = p.pairs(), total = prefix[p.n] * pairs, workers = ai_workers(total, most);     // (warp w of the run: block w % grid, so that few are spread over all SMs)
+    if ((int)blockIdx.x >= workers) return;                     // (before anything is written: the kernel in front may still run)
+    if (warp == WARPS) {
+        // ---- the warp that fetches: a lane for each of the others
+        const int w = lane * gridDim.x + blockIdx.x, a = lane < WARPS && w < workers ? ai_begin(w, total, workers) : 0, b = lane < WARPS && w < workers ? ai_begin(w + 1, total, workers) : 0;
+        AiAt at = {0, 0, 0, 1};
+        if (a < b) at = ai_find(a, pairs, p.n, prefix);
+        // the block to fetch, and whether the kernel before this one may still write its page
+        bool newest = false;
+        const auto look = [&]() {
+            const int pos = p.position(at.place), row = p.selected ? at.place : p.tok_row[at.place], j = p.first_seen(pos) / PE_PAGE + at.page;
+            newest = pos < 0 || j == pos / PE_PAGE;
+            if (pos < 0 || row < 0 || row >= p.n_rows) return -1;
+            const int page = p.block_table[(size_t)row * p.table_stride + j];
+            if (page < 0 || page >= p.n_pages) return -1;
+            return p.selected ? page : page * p.n_kv + at.pair / p.head_tiles;
+        };
+        int block = a < b ? look() : -1, stage = 0, round = 0;
+        bool waits = early != 0;
+        long long deadline = 0;
+        for (int x = a; __any_sync(0xffffffffu, x < b);) {
+            const unsigned slot = (unsigned)(lane * S::stages + stage);
+            bool ready = x < b && !(waits && newest);
+            if (ready && round > 0) ready = ai_bar_test(empty0 + 8u * slot, (unsigned)(round - 1) & 1u);
+            if (ready) {
+                filled[slot] = block >= 0;
+                if (block >= 0) ai_fetch<D>(ai_smem(ai_ring) + slot * B::bytes, pool + (size_t)block * B::bytes, full0 + 8u * slot);
+                else ai_bar_arrive(full0 + 8u * slot);
+                if (++x < b) { ai_next(at, pairs, prefix); block = look(); }
+                if (++stage == S::stages) { stage = 0; ++round; }
+                deadline = 0;
+            }
+            if (!__any_sync(0xffffffffu, ready)) {
+                if (waits) {
+                    pdl_wait();
+                    waits = false;
+                } else if (!deadline) {
+                    deadline = clock64() + AI_WAIT_CYCLES;
+                } else if (clock64() > deadline && x < b) {
+                    atomicExch(status, 23);
+                    x = b;
+                }
+            }
+        }
+        if (waits) pdl_wait();
+        if (blockIdx.x == 0) for (int i = lane; i <= p.n; i += 32) prefix_out[i] = prefix[i];
+        return;
+    }
+    // ---- the warps that compute
+    const int w = warp * gridDim.x + blockIdx.x;
+    if (w >= workers) return;
+    const int a = ai_begin(w, total, workers), b = ai_begin(w + 1, total, workers);
+    if (a >= b) return;
+    AiAt at = ai_find(a, pairs, p.n, prefix);
+    if (early) pdl_wait();
+    const float scale = scale_log2e * ai_pow2(-AI_DOWN);
+    const int G = p.n_heads / p.n_kv;
+    AiState<D> s;
+    AiQuery<D> f;
+    int tok = 0, kvh = 0, h0 = 0, pos = 0, lo = 0, from = 0, stage = 0;
+    unsigned phase = 0;
+    bool whole_begin = at.page == 0, first_pair = true;
+    const auto enter = [&]() {
+        p.heads_of(at.place, at.pair, tok, kvh, h0);
+        pos = p.position(at.place);
+        lo = p.first_seen(pos);
+        from = lo / PE_PAGE;
+        ai_reset(s);
+        ai_query<D>(f, q + (size_t)tok * q_stride + (size_t)(kvh * G + h0 + g) * D, h0 + g < G, t);
+    };
+    const auto leave = [&](bool whole) {
+        // the pair's sums: to the result where this warp had all of it, else to the warp's first or second place
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) s.sum[h] += __shfl_xor_sync(0xffffffffu, s.sum[h], o);
+            const int head = 2 * t + h;
+            float* to = partial + ((size_t)(w * 2 + (first_pair ? 0 : 1)) * 8 + head) * S::row;
+            const float r = s.sum[h] == 0.f ? 0.f : 1.f / (s.sum[h] * ai_pow2(-AI_UP));
+            if (!whole && g == 0) *reinterpret_cast<float2*>(to + D) = make_float2(s.top[h], s.sum[h]);
+#pragma unroll
+            for (int gr = 0; gr < B::groups; ++gr) {
+                const float mid = __shfl_sync(0xffffffffu, s.mids[h], gr * 4 + t) * ai_pow2(-AI_UP);
+                const float4 v = make_float4(fmaf(s.acc[2 * gr][h], ai_pow2(-AI_DOWN), mid), fmaf(s.acc[2 * gr][2 + h], ai_pow2(-AI_DOWN), mid),
+                                             fmaf(s.acc[2 * gr + 1][h], ai_pow2(-AI_DOWN), mid), fmaf(s.acc[2 * gr + 1][2 + h], ai_pow2(-AI_DOWN), mid));
+                if (!whole) *reinterpret_cast<float4*>(to + 32 * gr + 4 * g) = v;
+                else if (h0 + head < G)
+                    *reinterpret_cast<uint2*>(out + ((size_t)tok * p.n_heads + kvh * G + h0 + head) * D + 32 * gr + 4 * g) = make_uint2(ai_pack(v.x * r, v.y * r), ai_pack(v.z * r, v.w * r));
+            }
+        }
+        first_pair = false;
+    };
+    enter();
+    for (int x = a;;) {
+        const int slot = warp * S::stages + stage;
+        if (!__all_sync(0xffffffffu, ai_bar_wait(full0 + 8u * slot, phase))) {
+            if (lane == 0) atomicExch(status, 24);
+            return;
+        }
+        const int key0 = (from + at.page) * PE_PAGE;
+        if (filled[slot]) ai_block<D>(s, f, ai_ring + slot * B::bytes, lo - key0, pos - key0, scale, lane);
+        __syncwarp();
+        if (lane == 0) ai_bar_arrive(empty0 + 8u * slot);
+        if (++stage == S::stages) { stage = 0; phase ^= 1u; }
+        if (++x == b) break;
+        if (ai_next(at, pairs, prefix)) {
+            leave(whole_begin);
+            whole_begin = true;
+            enter();
+        }
+    }
+    leave(whole_begin && at.page == at.pages - 1);
+}
+
+// 4 COLS columns of a pair's sums, left by the warps that had a part of it.  512 threads: four numbers of a head each, 64 / COLS of the warps' places at a time.  (Few pairs: eight, so that
+// more blocks share the work: 64 pairs of heads of 128 on 16,000 positions 48 -> 40 us; many pairs: all columns of a block, 800 pairs 96 -> 86 us.)
+template <int D, int COLS>
+__global__ void __launch_bounds__(512) attention_int4_join_kernel(const AiPlaces p, const int* prefix, const float* partial, int most, bf16* out) {
+    constexpr int row = AiStream<D>::row, cols = COLS, groups = 512 / (8 * cols);
+    __shared__ float4 sums[groups][8][cols];
+    __shared__ float2 tops[groups][8];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int pairs = p.pairs(), place = blockIdx.x / pairs, pair = blockIdx.x - place * pairs;
+    const int before = prefix[place], pages = prefix[place + 1] - before, total = prefix[p.n] * pairs, begin = before * pairs + pair * pages, end = begin + pages;
+    const int workers = ai_workers(total, most);
+    const auto worker_of = [&](int x) { return (int)(((long long)(x + 1) * workers - 1) / total); };       // the last one that begins at x or before
+    const int w0 = worker_of(begin), w1 = worker_of(end - 1);
+    if (w0 == w1) return;
+    int tok, kvh, h0;
+    p.heads_of(place, pair, tok, kvh, h0);
+    const int G = p.n_heads / p.n_kv, c0 = blockIdx.y * (4 * cols), c = threadIdx.x % cols, h = threadIdx.x / cols % 8, group = threadIdx.x / (8 * cols);
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int w = w0 + group; w <= w1; w += groups) {
+        const float* src = partial + ((size_t)(w * 2 + (ai_begin(w, total, workers) >= begin ? 0 : 1)) * 8 + h) * row;
+        const float2 ml = *reinterpret_cast<const float2*>(src + D);
+        const float4 v = *reinterpret_cast<const float4*>(src + c0 + 4 * c);
+        const float top = fmaxf(m, ml.x), x = l == 0.f ? 0.f : ai_ex2(m - top), y = ml.y == 0.f ? 0.f : ai_ex2(ml.x - top);
+        o.x = fmaf(v.x, y, o.x * x); o.y = fmaf(v.y, y, o.y * x); o.z = fmaf(v.z, y, o.z * x); o.w = fmaf(v.w, y, o.w * x);
+        l = fmaf(ml.y, y, l * x);
+        m = top;
+    }
+    sums[group][h][c] = o;
+    if (c == 0) tops[group][h] = make_float2(m, l);
+    __syncthreads();
+    if (group || h0 + h >= G) return;
+    m = -INFINITY; l = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < groups; ++i) m = fmaxf(m, tops[i][h].x);
+#pragma unroll
+    for (int i = 0; i < groups; ++i) {
+        const float2 ml = tops[i][h];
+        const float x = ml.y == 0.f ? 0.f : ai_ex2(ml.x - m);
+        const float4 v = sums[i][h][c];
+        o.x = fmaf(v.x, x, o.x); o.y = fmaf(v.y, x, o.y); o.z = fmaf(v.z, x, o.z); o.w = fmaf(v.w, x, o.w);
+        l = fmaf(ml.y, x, l);
+    }
+    const float r = l == 0.f ? 0.f : 1.f / (l * ai_pow2(-AI_UP));
+    *reinterpret_cast<uint2*>(out + ((size_t)tok * p.n_heads + kvh * G + h0 + h) * D + c0 + 4 * c) = make_uint2(ai_pack(o.x * r, o.y * r), ai_pack(o.z * r, o.w * r));
+}
+
+namespace {
+// What a kernel needs to be told once a device.
+inline int ai_allow(const void* kernel, int smem, bool (&done)[64], bool wide) {
+    int dev = 0;
+    PE_TRY(cudaGetDevice(&dev));
+    if (dev < 64 && done[dev]) return 0;
+    PE_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (wide && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) cudaGetLastError();
+    if (dev < 64) done[dev] = true;
+    return 0;
+}
+
+template <int D, int WARPS>
 struct AiLaunch {
-    using S = AiShape<D>;
+    using S = AiShape<D, WARPS>;
     static int allow() {
         static bool done[64] = {};
-        int dev = 0;
-        PE_TRY(cudaGetDevice(&dev));
-        if (dev < 64 && done[dev]) return 0;
-        PE_TRY(cudaFuncSetAttribute(attention_int4_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem));
-        if (cudaFuncSetAttribute(attention_int4_kernel<D>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) cudaGetLastError();
-        if (dev < 64) done[dev] = true;
-        return 0;
+        return ai_allow((const void*)attention_int4_kernel<D, WARPS>, S::smem, done, true);
     }
     // clusters of so many CTAs that the GPU holds at once
     static int at_once(int splits) {
@@ -448,57 +722,104 @@ struct AiLaunch {
         if (cudaGetDevice(&dev) != cudaSuccess) return 0;
         auto it = known.find({dev, splits});
         if (it != known.end()) return it->second;
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(splits, 1, 1024);
-        cfg.blockDim = dim3(32 * S::warps);
-        cfg.dynamicSmemBytes = S::smem;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
         int n = 0;
-        if (cudaOccupancyMaxActiveClusters(&n, attention_int4_kernel<D>, &cfg) != cudaSuccess) { cudaGetLastError(); n = 0; }
+        if (allow() == 0) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(splits, 1, 1024);
+            cfg.blockDim = dim3(S::threads);
+            cfg.dynamicSmemBytes = S::smem;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&n, attention_int4_kernel<D, WARPS>, &cfg) != cudaSuccess) { cudaGetLastError(); n = 0; }
+        }
         known[{dev, splits}] = n;
         return n;
     }
-    // CTAs of a (token, key head, tile of heads): as many as run at once, each warp with a page at least
-    static int splits(long long triples, int units) {
+    // CTAs of a (token, key head, tile of heads): as many as run at once, each warp with a page at least.  (Large clusters find room for fewer than the occupancy says while
+    // the next kernel's first CTAs wait on some SMs: 8 rows of 4,096 with 4 CTAs each 6.4 us, with 8 each, just as many as fit, 11.1.)
+    static int splits(long long triples, int pages) {
         int n = 1;
-        while (n < AI_MAX_SPLITS && n * S::warps < units && at_once(2 * n) >= triples) n *= 2;
+        while (n < AI_MAX_SPLITS && n * WARPS < pages && at_once(2 * n) * (n >= 4 ? 4 : 5) >= triples * 5) n *= 2;
         return n;
     }
-    static int go(int n_splits, unsigned tokens, unsigned tiles_y, cudaStream_t stream, const bf16* q, int q_stride, const unsigned char* pool, int n_blocks,
-                  const int* block_table, int table_stride, int n_rows, const int* tok_pos, const int* tok_row, int n_heads, int n_kv, int window, float scale, int selected,
-                  int early, int* status, bf16* out) {
+    static int go(const AiPlaces& p, int T, int pages, const bf16* q, int q_stride, const unsigned char* pool, float scale_log2e, int early, int* status, bf16* out, cudaStream_t stream) {
         { const int e = allow(); if (e) return e; }
-        PE_TRY(pe_launch_cluster(attention_int4_kernel<D>, dim3(n_splits, tiles_y, tokens), dim3(32 * S::warps), S::smem, stream, n_splits, q, q_stride, pool,
-                                 n_blocks, block_table, table_stride, n_rows, tok_pos, tok_row, n_heads, n_kv, window, scale * 1.4426950408889634f, selected, n_splits, early,
-                                 status, out));
+        const int tiles = p.n_kv * p.head_tiles, n = splits((long long)tiles * T, pages);
+        PE_TRY(pe_launch_cluster(attention_int4_kernel<D, WARPS>, dim3(n, tiles, T), dim3(S::threads), S::smem, stream, n, q, q_stride, pool, p.selected ? p.n_pages : p.n_pages * p.n_kv,
+                                 p.block_table, p.table_stride, p.n_rows, p.tok_pos, p.tok_row, p.n_heads, p.n_kv, p.window, scale_log2e, p.selected, n, early, status, out));
+        PE_LAUNCH_CHECK();
+        return 0;
+    }
+};
+
+template <int D>
+struct AiStreamLaunch {
+    using S = AiStream<D>;
+    static int workers() { return pe_sm_count() * S::warps; }
+    static long long scratch(int places) { return (long long)workers() * 2 * 8 * S::row * 4 + (places + 1) * 4ll; }
+    static int go(const AiPlaces& p, const bf16* q, int q_stride, const unsigned char* pool, float scale_log2e, int early, void* scratch, int* status, bf16* out, cudaStream_t stream) {
+        static bool done[64] = {};
+        { const int e = ai_allow((const void*)attention_int4_stream_kernel<D>, S::ring + (AI_MAX_PLACES + 1) * 4, done, false); if (e) return e; }
+        float* partial = (float*)scratch;
+        int* prefix = (int*)(partial + (size_t)workers() * 2 * 8 * S::row);
+        PE_TRY(pe_launch(attention_int4_stream_kernel<D>, dim3(pe_sm_count()), dim3(S::threads), S::ring + (size_t)(p.n + 1) * 4, stream, q, q_stride, pool, p, scale_log2e, early, workers(),
+                         partial, prefix, status, out));
+        PE_LAUNCH_CHECK();
+        const unsigned pairs = (unsigned)(p.n * (p.selected ? p.head_tiles : p.n_kv * p.head_tiles));
+        if (pairs <= 2u * (unsigned)pe_sm_count())
+            PE_TRY(pe_launch(attention_int4_join_kernel<D, 8>, dim3(pairs, D / 32), dim3(512), 0, stream, p, prefix, partial, workers(), out));
+        else
+            PE_TRY(pe_launch(attention_int4_join_kernel<D, D / 4>, dim3(pairs), dim3(512), 0, stream, p, prefix, partial, workers(), out));
         PE_LAUNCH_CHECK();
         return 0;
     }
 };
 }  // namespace
 
+// Whether a call's blocks are dealt to the warps in equal runs: from 35,000 blocks on, the longest sequence's for every row (one CTA or cluster a pair / equal runs, us; 14 heads of 64 on 2: 64 rows of 20,000
+// to 32,700 72 / 65, 200 of up to 6,000 37 / 35, 32 of 4,000 to 8,192 16.6 / 22.7; 28 heads of 128 on 4: 200 of up to 6,000 94 / 86, 64 of 6,000 to 8,000 63.7 / 64.5, 16 of 8,000 to 16,000 37 / 40).
+static bool ai_streams(int T, int n_heads, int n_kv, int hd, int max_context, int selected) {
+    const long long places = selected ? (long long)T * n_kv : T, pairs = (long long)T * n_kv * ((n_heads / n_kv + 7) / 8), pages = (max_context - 1) / PE_PAGE + 1;
+    return places <= AI_MAX_PLACES && pairs * pages >= 35000 && pairs * pages <= 0x7fffffffll;
+}
+
 extern "C" void pe_set_pdl(int on) { pe_pdl_enabled() = on ? 1 : 0; }
+
+// Bytes of scratch that a call needs (0: none).
+extern "C" long long pe_attention_int4_scratch(int T, int n_heads, int n_kv, int hd, int max_context, int selected) {
+    if (T <= 0 || n_kv <= 0 || n_heads % n_kv || (hd != 64 && hd != 128) || !ai_streams(T, n_heads, n_kv, hd, max_context, selected)) return 0;
+    const int places = selected ? T * n_kv : T;
+    return hd == 64 ? AiStreamLaunch<64>::scratch(places) : AiStreamLaunch<128>::scratch(places);
+}
 
 extern "C" int pe_attention_int4(const void* q, int q_stride, void* out, const void* pool, long long n_blocks, const int* block_table, int table_stride, int n_rows,
                                  const int* tok_pos, const int* tok_row, int T, int n_heads, int n_kv, int hd, int window, float scale, int max_context, int selected,
-                                 int early, int* status, void* stream) {
+                                 int early, void* scratch, int* status, void* stream) {
     if (T <= 0) return 0;
-    if ((hd != 64 && hd != 128) || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv || max_context <= 0 || q_stride % 8 || table_stride < 1 || !status || T > 65535 || n_blocks > 0x7fffffffll || !(scale > 0.f)) return PE_ERR_UNSUPPORTED;
-    if ((((uintptr_t)q | (uintptr_t)pool) & 15) || ((uintptr_t)out & 7)) return PE_ERR_UNSUPPORTED;
-    const int head_tiles = (n_heads / n_kv + 7) / 8;
-    const long long tiles = (long long)n_kv * head_tiles;
-    if (tiles > 65535) return PE_ERR_UNSUPPORTED;
+    if ((hd != 64 && hd != 128) || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv || max_context <= 0 || q_stride % 8 || table_stride < 1 || !status || T > 65535 || n_blocks > 0x7fffffffll ||
+        !(scale > 0.f))
+        return PE_ERR_UNSUPPORTED;
+    if ((((uintptr_t)q | (uintptr_t)pool | (uintptr_t)scratch) & 15) || ((uintptr_t)out & 7)) return PE_ERR_UNSUPPORTED;
+    const int head_tiles = (n_heads / n_kv + 7) / 8, pages = (max_context - 1) / PE_PAGE + 1;
+    if ((long long)n_kv * head_tiles > 65535) return PE_ERR_UNSUPPORTED;
     early = early && !selected;
-    const int units = ((max_context - 1) / PE_PAGE + 1);
+    const AiPlaces p = {tok_pos, tok_row, block_table, selected ? T * n_kv : T, table_stride, n_rows, (int)(selected ? n_blocks : n_blocks / n_kv), n_kv, n_heads, head_tiles, window, selected};
+    const float scale_log2e = scale * 1.4426950408889634f;
+    if (scratch && ai_streams(T, n_heads, n_kv, hd, max_context, selected) && (long long)T * n_kv * head_tiles * table_stride <= 0x7fffffffll) {
+        const auto go = [&](auto v) {
+            return decltype(v)::go(p, (const bf16*)q, q_stride, (const unsigned char*)pool, scale_log2e, early, scratch, status, (bf16*)out, (cudaStream_t)stream);
+        };
+        return hd == 64 ? go(AiStreamLaunch<64>()) : go(AiStreamLaunch<128>());
+    }
     const auto go = [&](auto v) {
-        using L = decltype(v);
-        { const int e = L::allow(); if (e) return e; }
-        return L::go(L::splits(tiles * T, units), (unsigned)T, (unsigned)tiles, (cudaStream_t)stream, (const bf16*)q, q_stride, (const unsigned char*)pool, (int)n_blocks, block_table,
-                     table_stride, n_rows, tok_pos, tok_row, n_heads, n_kv, window, scale, selected, early, status, (bf16*)out);
+        return decltype(v)::go(p, T, pages, (const bf16*)q, q_stride, (const unsigned char*)pool, scale_log2e, early, status, (bf16*)out, (cudaStream_t)stream);
     };
-    return hd == 64 ? go(AiLaunch<64>()) : go(AiLaunch<128>());
+    // Seven warps, of which two CTAs share an SM, where pairs are few and each is cut over many CTAs (one row of 14 heads on 4,096 positions 4.5 us, with fifteen 5.6), but not where one
+    // CTA's warps have a page each (500 positions 3.6, with seven 3.9); else as many as the registers allow (64 rows of 1,000 to 2,000 7.3, with seven 8.9).
+    const bool few = (long long)T * n_kv * head_tiles <= 8;
+    if (hd == 64) return few && pages > 15 ? go(AiLaunch<64, 7>()) : go(AiLaunch<64, 15>());
+    return few && pages > 11 ? go(AiLaunch<128, 7>()) : go(AiLaunch<128, 11>());
 }

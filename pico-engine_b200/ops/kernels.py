@@ -2226,6 +2226,12 @@ def load_int4(pool: torch.Tensor, n_kv: int, head_dim: int, tok_pos: torch.Tenso
     return keys, values
 
 
+def _int4_scratch(T: int, n_heads: int, n_kv_heads: int, head_dim: int, max_context: int, selected: int, device) -> Optional[torch.Tensor]:
+    """What a call leaves for its second kernel to join (the call's own: calls on two streams and captured graphs share none), or None."""
+    nbytes = long_context().pe_attention_int4_scratch(T, n_heads, n_kv_heads, head_dim, max_context, selected)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
 def _int4_out(out: Optional[torch.Tensor], T: int, width: int, device) -> torch.Tensor:
     if out is None:
         return torch.empty(T, width, dtype=torch.bfloat16, device=device)
@@ -2253,9 +2259,10 @@ def attention_int4(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int
     out = _int4_out(out, T, n_heads * head_dim, q.device)
     stream = _stream_here(q, "q")
     if T:
+        scratch = _int4_scratch(T, n_heads, n_kv_heads, head_dim, int(max_context), 0, q.device)
         check(long_context().pe_attention_int4(q.data_ptr(), q_stride, out.data_ptr(), pool.data_ptr(), pool.shape[0] * n_kv_heads, block_table.data_ptr(), table_stride, rows,
                                                tok_pos.data_ptr(), tok_row.data_ptr(), T, n_heads, n_kv_heads, head_dim, window or 0, float(scale), int(max_context), 0,
-                                               1 if early_pages else 0, status_ptr(q.device), stream), "attention_int4")
+                                               1 if early_pages else 0, _ptr(scratch), status_ptr(q.device), stream), "attention_int4", 1 if scratch is None else 2)
     return out
 
 
@@ -2355,7 +2362,8 @@ def attention_int4_selected(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_h
     out = _int4_out(out, T, n_heads * head_dim, q.device)
     stream = _stream_here(q, "q")
     if T:
+        scratch = _int4_scratch(T, n_heads, n_kv_heads, head_dim, keep * PAGE, 1, q.device)
         check(long_context().pe_attention_int4(q.data_ptr(), q_stride, out.data_ptr(), pool.data_ptr(), pool.shape[0] * n_kv_heads, pages.table.data_ptr(), keep, places,
-                                               pages.pos.data_ptr(), None, T, n_heads, n_kv_heads, head_dim, 0, float(scale), keep * PAGE, 1, 0, status_ptr(q.device), stream),
-              "attention_int4_selected")
+                                               pages.pos.data_ptr(), None, T, n_heads, n_kv_heads, head_dim, 0, float(scale), keep * PAGE, 1, 0, _ptr(scratch), status_ptr(q.device), stream),
+              "attention_int4_selected", 1 if scratch is None else 2)
     return out

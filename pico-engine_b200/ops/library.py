@@ -147,7 +147,7 @@ _LONG_SIGNATURES = {
     "pe_load_int4": [P, LL, I, I, P, P, I, P, I, I, P, P, P],
     "pe_page_bounds": [P, LL, I, I, P, P, I, P, I, I, P, P],
     "pe_select_pages": [P, I, I, I, I, I, P, LL, P, I, I, P, P, I, I, P, P, P, P],
-    "pe_attention_int4": [P, I, P, P, LL, P, I, I, P, P, I, I, I, I, I, F, I, I, I, P, P],
+    "pe_attention_int4": [P, I, P, P, LL, P, I, I, P, P, I, I, I, I, I, F, I, I, I, P, P, P],
     "pe_expand_int4": [P, LL, I, I, P, I, P, I, I, I, P, P, P, P],
 }
 
@@ -305,6 +305,8 @@ def long_context() -> ctypes.CDLL:
         lib = build.load("long", LONG_SOURCES)
         declare(lib, _LONG_SIGNATURES)
         lib.pe_set_pdl(0 if os.environ.get("PICO_ENGINE_PDL", "1") == "0" else 1)
+        lib.pe_attention_int4_scratch.argtypes = [I, I, I, I, I, I]
+        lib.pe_attention_int4_scratch.restype = c_longlong
         _long = lib
     return _long
 

@@ -166,7 +166,7 @@ def test_attention(K, H, G, D, lengths):
     p = Paged(H, G, D, lengths, 7 + H, rubbish=float("nan"))
     pos, row = [n - 1 for n in lengths], list(range(len(lengths)))
     p.check(p.attention(K, pos, row), pos, row)
-    p.check(p.attention(K, pos, row, bound=1 << 20), pos, row)              # a launch for long contexts, whatever they are
+    p.check(p.attention(K, pos, row, bound=1 << 21), pos, row)              # a launch for long contexts, whatever they are
 
 
 @pytest.mark.parametrize("H,G,D", [(14, 2, 64), (16, 4, 128)])
@@ -185,15 +185,17 @@ def test_attention_under_a_window(K, H, G, D, window):
             p.values[page, :, :first % PAGE] = float("nan")
     p.pool = plain.pack(p.keys.view(-1, 64, D), p.values.view(-1, 64, D)).view(p.n_pages, G, 80 * D)
     pos, row = [n - 1 for n in lengths], list(range(len(lengths)))
-    p.check(p.attention(K, pos, row, window=window, table=table, bound=4000), pos, row, window=window, table=table)
+    for bound in (4000, 1 << 21):
+        p.check(p.attention(K, pos, row, window=window, table=table, bound=bound), pos, row, window=window, table=table)
 
 
 def test_several_tokens_of_a_row_and_rows_in_any_order(K):
     p = Paged(14, 2, 64, [300, 90, 700], 2)
     pos, row = [0, 299, 17, 89, 650, 5, 699], [2, 0, 1, 1, 2, 0, 2]
     q = randn(7, 14 * 64, seed=3).bfloat16()
-    got = p.attention(K, pos, row, q=q)
-    p.check(got, pos, row, q=q)
+    for bound in (700, 1 << 21):
+        got = p.attention(K, pos, row, q=q, bound=bound)
+        p.check(got, pos, row, q=q)
     alone = torch.cat([p.attention(K, [a], [b], q=q[i:i + 1].contiguous(), bound=700) for i, (a, b) in enumerate(zip(pos, row))])
     p.check(alone, pos, row, q=q)
 
@@ -203,6 +205,9 @@ def test_rows_that_see_nothing_and_groups_that_are_none(K):
     table = p.table.clone()
     table[0] = -1
     table[1, 1] = -1
+    long = p.attention(K, [199, 129, 63], [0, 1, 2], table=table, bound=1 << 21)
+    assert (long[0] == 0).all()
+    p.check(long, [199, 129, 63], [0, 1, 2], table=table)
     out = p.attention(K, [199, 129, 63], [0, 1, 2], table=table)
     assert (out[0] == 0).all()
     p.check(out, [199, 129, 63], [0, 1, 2], table=table)
