@@ -7,6 +7,7 @@ from __future__ import annotations
 import ctypes
 import os
 from dataclasses import dataclass
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -2146,31 +2147,48 @@ def int4_pool(n_pages: int, n_kv_heads: int, head_dim: int, device) -> torch.Ten
     return torch.zeros(n_pages, n_kv_heads, int4_page_bytes(head_dim), dtype=torch.uint8, device=device)
 
 
-def _int4_heads(n_heads: int, n_kv_heads: int, head_dim: int) -> None:
-    if n_kv_heads < 1 or n_heads < 1 or n_heads % n_kv_heads or head_dim not in INT4_HEAD_DIMS:
+_INT4_BYTES = {d: int4_page_bytes(d) for d in INT4_HEAD_DIMS}
+
+
+def _int4_heads(n_heads: int, n_kv_heads: int, head_dim: int) -> int:
+    """The bytes of a page and head."""
+    if head_dim not in _INT4_BYTES or n_kv_heads < 1 or n_heads < 1 or n_heads % n_kv_heads:
         raise KernelError(f"4-bit caches take head sizes {INT4_HEAD_DIMS} and query heads that share the key/value heads evenly, not {n_heads} / {n_kv_heads} heads of {head_dim}")
+    return _INT4_BYTES[head_dim]
 
 
-def _int4_pool(pool: torch.Tensor, n_kv_heads: int, head_dim: int) -> None:
-    _need(pool, "pool", torch.uint8)
-    if pool.dim() != 3 or pool.shape[1] != n_kv_heads or pool.shape[2] != int4_page_bytes(head_dim):
-        raise KernelError(f"a 4-bit cache pool must be [pages, {n_kv_heads}, {int4_page_bytes(head_dim)}] bytes, not {tuple(pool.shape)}")
-    if pool.data_ptr() % 16:
-        raise KernelError("a 4-bit cache pool must start on a 16-byte boundary")
+def _device_here(t: torch.Tensor, name: str) -> int:
+    """The index of the current device, on which the tensor has to lie."""
+    device = t.get_device()
+    if device < 0:
+        raise KernelError(f"{name} must live on a CUDA device")
+    if device != torch._C._cuda_getDevice():
+        raise KernelError(f"{name} lives on {t.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+    return device
 
 
-def _page_table(block_table: torch.Tensor, table_stride: int) -> int:
+def _here(device: int, *tensors) -> None:
+    """(tensor, name, dtype, shape or None) of every argument of a call: contiguous, from a 16-byte boundary on, on the call's device."""
+    for t, name, dtype, shape in tensors:
+        if t.dtype is dtype and t.get_device() == device and t.is_contiguous() and (shape is None or t.shape == shape) and t.data_ptr() % 16 == 0:
+            continue
+        _need(t, name, dtype, shape)
+        if t.get_device() != device:
+            raise KernelError(f"{name} lives on {t.device}, the current device is cuda:{device}")
+        raise KernelError(f"{name} must start on a 16-byte boundary")
+
+
+def _page_rows(block_table: torch.Tensor, table_stride: int) -> int:
     """The number of rows of a page table."""
-    _need(block_table, "block_table", torch.int32)
-    if table_stride < 1 or block_table.numel() % table_stride or block_table.numel() == 0:
+    n = block_table.numel()
+    if table_stride < 1 or n == 0 or n % table_stride:
         raise KernelError(f"block_table must have rows of {table_stride} pages, not {tuple(block_table.shape)}")
-    return block_table.numel() // table_stride
+    return n // table_stride
 
 
 def _query_rows(q: torch.Tensor, q_stride: int, T: int, width: int) -> None:
-    _need(q, "q", torch.bfloat16)
-    if q_stride % 8 or q_stride < width or (T and q.numel() < (T - 1) * q_stride + width) or q.data_ptr() % 16:
-        raise KernelError(f"q must hold {T} rows of {width} numbers, {q_stride} (a multiple of 8) apart, from a 16-byte boundary on")
+    if q_stride % 8 or q_stride < width or (T and q.numel() < (T - 1) * q_stride + width):
+        raise KernelError(f"q must hold {T} rows of {width} numbers, {q_stride} (a multiple of 8) apart")
 
 
 def store_int4(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], tok_pos: torch.Tensor,
@@ -2183,60 +2201,54 @@ def store_int4(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, cos: Optio
     infinity or NaN is NaN as a whole.  Keys are turned in float64 and rounded to bfloat16 before they are coded.
 
     Tokens of a sequence stand behind one another in the call, in the order of their positions, and no position twice; tokens whose page is not there (-1) are not stored."""
-    T = tok_pos.shape[0]
-    _int4_heads(n_q, n_kv, head_dim)
-    _need(qkv, "qkv", torch.bfloat16, (T, (n_q + 2 * n_kv) * head_dim))
-    _need(tok_pos, "tok_pos", torch.int32, (T,)); _need(tok_row, "tok_row", torch.int32, (T,))
-    _int4_pool(pool, n_kv, head_dim)
-    rows = _page_table(block_table, table_stride)
+    T, n_bytes, device = tok_pos.shape[0], _int4_heads(n_q, n_kv, head_dim), _device_here(qkv, "qkv")
+    row, width = (T,), n_q * head_dim
+    _here(device, (qkv, "qkv", torch.bfloat16, (T, width + 2 * n_kv * head_dim)), (tok_pos, "tok_pos", torch.int32, row), (tok_row, "tok_row", torch.int32, row),
+          (pool, "pool", torch.uint8, (pool.shape[0], n_kv, n_bytes)), (block_table, "block_table", torch.int32, None))
+    rows = _page_rows(block_table, table_stride)
     if (cos is None) != (sin is None):
         raise KernelError("cos and sin go together")
+    angles = 0
     if cos is not None:
-        _need(cos, "cos", torch.float32); _need(sin, "sin", torch.float32, cos.shape)
-        if cos.dim() != 2 or cos.shape[0] < 1 or cos.shape[1] != head_dim // 2 or cos.data_ptr() % 16 or sin.data_ptr() % 16:
-            raise KernelError(f"cos/sin tables must be [positions, {head_dim // 2}] from a 16-byte boundary on, not {tuple(cos.shape)}")
-    if qkv.data_ptr() % 16:
-        raise KernelError("qkv must start on a 16-byte boundary")
+        angles = cos.shape[0]
+        _here(device, (cos, "cos", torch.float32, (angles, head_dim // 2)), (sin, "sin", torch.float32, (angles, head_dim // 2)))
+        if angles < 1:
+            raise KernelError("cos and sin must hold a position at least")
     if out is None:
-        out = torch.empty(T, n_q * head_dim, dtype=torch.bfloat16, device=qkv.device)
+        out = qkv.new_empty((T, width))
     else:
-        _need(out, "out", torch.bfloat16, (T, n_q * head_dim))
-        if out.data_ptr() % 16:
-            raise KernelError("out must start on a 16-byte boundary")
-    stream = _stream_here(qkv, "qkv")
+        _here(device, (out, "out", torch.bfloat16, (T, width)))
     if T:
-        check(long_context().pe_store_int4(qkv.data_ptr(), T, n_q, n_kv, head_dim, _ptr(cos), _ptr(sin), 0 if cos is None else cos.shape[0], tok_pos.data_ptr(),
-                                           tok_row.data_ptr(), pool.data_ptr(), pool.shape[0], block_table.data_ptr(), table_stride, rows, out.data_ptr(), stream), "store_int4")
+        check(long_context().pe_store_int4(qkv.data_ptr(), T, n_q, n_kv, head_dim, _ptr(cos), _ptr(sin), angles, tok_pos.data_ptr(), tok_row.data_ptr(), pool.data_ptr(), pool.shape[0],
+                                           block_table.data_ptr(), table_stride, rows, out.data_ptr(), torch._C._cuda_getCurrentRawStream(device)), "store_int4")
     return out
 
 
 def load_int4(pool: torch.Tensor, n_kv: int, head_dim: int, tok_pos: torch.Tensor, tok_row: torch.Tensor, block_table: torch.Tensor, table_stride: int):
     """What a 4-bit cache holds at positions ``tok_pos`` of the sequences ``tok_row`` (int32 [T]): keys and values, float32 [T, n_kv, head_dim].  Zeros where no page is."""
-    T = tok_pos.shape[0]
-    _int4_heads(n_kv, n_kv, head_dim)
-    _int4_pool(pool, n_kv, head_dim)
-    _need(tok_pos, "tok_pos", torch.int32, (T,)); _need(tok_row, "tok_row", torch.int32, (T,))
-    rows = _page_table(block_table, table_stride)
-    stream = _stream_here(pool, "pool")
-    keys = torch.empty(T, n_kv, head_dim, dtype=torch.float32, device=pool.device)
-    values = torch.empty_like(keys)
+    T, n_bytes, device = tok_pos.shape[0], _int4_heads(n_kv, n_kv, head_dim), _device_here(pool, "pool")
+    _here(device, (tok_pos, "tok_pos", torch.int32, (T,)), (tok_row, "tok_row", torch.int32, (T,)), (pool, "pool", torch.uint8, (pool.shape[0], n_kv, n_bytes)),
+          (block_table, "block_table", torch.int32, None))
+    rows = _page_rows(block_table, table_stride)
+    keys, values = pool.new_empty((2, T, n_kv, head_dim), dtype=torch.float32).unbind(0)
     if T:
         check(long_context().pe_load_int4(pool.data_ptr(), pool.shape[0], n_kv, head_dim, tok_pos.data_ptr(), tok_row.data_ptr(), T, block_table.data_ptr(), table_stride, rows,
-                                          keys.data_ptr(), values.data_ptr(), stream), "load_int4")
+                                          keys.data_ptr(), values.data_ptr(), torch._C._cuda_getCurrentRawStream(device)), "load_int4")
     return keys, values
 
 
-def _int4_scratch(T: int, n_heads: int, n_kv_heads: int, head_dim: int, max_context: int, selected: int, device) -> Optional[torch.Tensor]:
-    """What a call leaves for its second kernel to join (the call's own: calls on two streams and captured graphs share none), or None."""
-    nbytes = long_context().pe_attention_int4_scratch(T, n_heads, n_kv_heads, head_dim, max_context, selected)
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+@lru_cache(maxsize=4096)
+def _int4_scratch_bytes(T: int, n_heads: int, n_kv_heads: int, head_dim: int, max_context: int, selected: int) -> int:
+    return long_context().pe_attention_int4_scratch(T, n_heads, n_kv_heads, head_dim, max_context, selected)
 
 
-def _int4_out(out: Optional[torch.Tensor], T: int, width: int, device) -> torch.Tensor:
-    if out is None:
-        return torch.empty(T, width, dtype=torch.bfloat16, device=device)
-    _need(out, "out", torch.bfloat16, (T, width))
-    return out
+def _attend_int4(q, q_stride, out, pool, table, table_stride, rows, tok_pos, tok_row, T, n_heads, n_kv_heads, head_dim, window, scale, max_context, selected, early, device, name) -> None:
+    n = _int4_scratch_bytes(T, n_heads, n_kv_heads, head_dim, max_context, selected)
+    # (what a call leaves for its second kernel to join is the call's own: calls on two streams and captured graphs share none)
+    scratch = pool.new_empty(n) if n else None
+    check(long_context().pe_attention_int4(q.data_ptr(), q_stride, out.data_ptr(), pool.data_ptr(), pool.shape[0] * n_kv_heads, table.data_ptr(), table_stride, rows, tok_pos.data_ptr(),
+                                           _ptr(tok_row), T, n_heads, n_kv_heads, head_dim, window, scale, max_context, selected, early, _ptr(scratch), status_ptr(q.device),
+                                           torch._C._cuda_getCurrentRawStream(device)), name, 1 if scratch is None else 2)
 
 
 def attention_int4(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int, head_dim: int, pool: torch.Tensor, block_table: torch.Tensor, table_stride: int,
@@ -2248,21 +2260,20 @@ def attention_int4(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int
 
     Scores are sums of exact products of the queries with codes, in float32; steps and middles join in float32.  Weights are rounded to bfloat16 for the product with
     the values, and once more behind their multiplication by a value's step.  A row that sees nothing is zeros; one that sees a group that is no number is none where that reaches."""
-    T = tok_pos.shape[0]
-    _int4_heads(n_heads, n_kv_heads, head_dim)
-    _int4_pool(pool, n_kv_heads, head_dim)
-    _query_rows(q, q_stride, T, n_heads * head_dim)
-    _need(tok_pos, "tok_pos", torch.int32, (T,)); _need(tok_row, "tok_row", torch.int32, (T,))
-    rows = _page_table(block_table, table_stride)
+    T, n_bytes, device, width = tok_pos.shape[0], _int4_heads(n_heads, n_kv_heads, head_dim), _device_here(q, "q"), n_heads * head_dim
+    _here(device, (q, "q", torch.bfloat16, None), (tok_pos, "tok_pos", torch.int32, (T,)), (tok_row, "tok_row", torch.int32, (T,)),
+          (pool, "pool", torch.uint8, (pool.shape[0], n_kv_heads, n_bytes)), (block_table, "block_table", torch.int32, None))
+    _query_rows(q, q_stride, T, width)
+    rows = _page_rows(block_table, table_stride)
     if max_context < 1 or (window is not None and window < 0) or not scale > 0:
         raise KernelError("max_context and scale must be positive, and a window not negative")
-    out = _int4_out(out, T, n_heads * head_dim, q.device)
-    stream = _stream_here(q, "q")
+    if out is None:
+        out = q.new_empty((T, width))
+    else:
+        _here(device, (out, "out", torch.bfloat16, (T, width)))
     if T:
-        scratch = _int4_scratch(T, n_heads, n_kv_heads, head_dim, int(max_context), 0, q.device)
-        check(long_context().pe_attention_int4(q.data_ptr(), q_stride, out.data_ptr(), pool.data_ptr(), pool.shape[0] * n_kv_heads, block_table.data_ptr(), table_stride, rows,
-                                               tok_pos.data_ptr(), tok_row.data_ptr(), T, n_heads, n_kv_heads, head_dim, window or 0, float(scale), int(max_context), 0,
-                                               1 if early_pages else 0, _ptr(scratch), status_ptr(q.device), stream), "attention_int4", 1 if scratch is None else 2)
+        _attend_int4(q, q_stride, out, pool, block_table, table_stride, rows, tok_pos, tok_row, T, n_heads, n_kv_heads, head_dim, window or 0, scale, max_context, 0,
+                     1 if early_pages else 0, device, "attention_int4")
     return out
 
 
@@ -2270,17 +2281,20 @@ def attention_int4_prompt(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_hea
                           tiles: torch.Tensor, n_tokens: int, window: Optional[int], scale: float, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The same for runs of at most 128 tokens of a sequence, ``tiles`` int32 [n, 4] (``prefill_tiles`` with ``PREFILL_TILE_TCGEN05``), whose own keys and values the cache holds already;
     ``q`` has ``n_tokens`` rows."""
-    _int4_heads(n_heads, n_kv_heads, head_dim)
-    _int4_pool(pool, n_kv_heads, head_dim)
-    _query_rows(q, q_stride, n_tokens, n_heads * head_dim)
-    _need(tiles, "tiles", torch.int32)
-    if tiles.dim() != 2 or tiles.shape[1] != 4 or tiles.data_ptr() % 16:
-        raise KernelError(f"tiles must be [runs, 4] from a 16-byte boundary on, not {tuple(tiles.shape)}")
-    rows = _page_table(block_table, table_stride)
+    n_bytes, device, width = _int4_heads(n_heads, n_kv_heads, head_dim), _device_here(q, "q"), n_heads * head_dim
+    _here(device, (q, "q", torch.bfloat16, None), (tiles, "tiles", torch.int32, (tiles.shape[0], 4)), (pool, "pool", torch.uint8, (pool.shape[0], n_kv_heads, n_bytes)),
+          (block_table, "block_table", torch.int32, None))
+    _query_rows(q, q_stride, n_tokens, width)
+    rows = _page_rows(block_table, table_stride)
     if (window is not None and window < 0) or not scale > 0:
         raise KernelError("scale must be positive, and a window not negative")
-    out = _int4_out(out, n_tokens, n_heads * head_dim, q.device)
-    stream = _stream_here(q, "q")
+    if rows > 1024:
+        raise KernelError(f"prompts over a 4-bit cache take page tables of at most 1,024 rows, not {rows}")
+    if out is None:
+        out = q.new_empty((n_tokens, width))
+    else:
+        _here(device, (out, "out", torch.bfloat16, (n_tokens, width)))
+    stream = torch._C._cuda_getCurrentRawStream(device)
     if n_tokens and tiles.shape[0]:
         pages = pool.shape[0]
         keys = torch.empty(pages, n_kv_heads, PAGE, head_dim, dtype=torch.float16, device=q.device)
@@ -2298,18 +2312,13 @@ def page_bounds(pool: torch.Tensor, n_kv: int, head_dim: int, tok_pos: torch.Ten
                 bounds: torch.Tensor) -> torch.Tensor:
     """The least and the greatest key of every channel of the pages that the tokens of a step have filled: where a token is the last of its page, ``bounds`` (bfloat16 [pages, n_kv, 2, head_dim])
     gets the page's rows, in place; the others stay as they are.  Of the keys that the 4-bit cache stands for, rounded to bfloat16."""
-    T = tok_pos.shape[0]
-    _int4_heads(n_kv, n_kv, head_dim)
-    _int4_pool(pool, n_kv, head_dim)
-    _need(tok_pos, "tok_pos", torch.int32, (T,)); _need(tok_row, "tok_row", torch.int32, (T,))
-    _need(bounds, "bounds", torch.bfloat16, (pool.shape[0], n_kv, 2, head_dim))
-    rows = _page_table(block_table, table_stride)
-    if bounds.data_ptr() % 16:
-        raise KernelError("bounds must start on a 16-byte boundary")
-    stream = _stream_here(pool, "pool")
+    T, n_bytes, device = tok_pos.shape[0], _int4_heads(n_kv, n_kv, head_dim), _device_here(pool, "pool")
+    _here(device, (tok_pos, "tok_pos", torch.int32, (T,)), (tok_row, "tok_row", torch.int32, (T,)), (pool, "pool", torch.uint8, (pool.shape[0], n_kv, n_bytes)),
+          (block_table, "block_table", torch.int32, None), (bounds, "bounds", torch.bfloat16, (pool.shape[0], n_kv, 2, head_dim)))
+    rows = _page_rows(block_table, table_stride)
     if T:
         check(long_context().pe_page_bounds(pool.data_ptr(), pool.shape[0], n_kv, head_dim, tok_pos.data_ptr(), tok_row.data_ptr(), T, block_table.data_ptr(), table_stride, rows,
-                                            bounds.data_ptr(), stream), "page_bounds")
+                                            bounds.data_ptr(), torch._C._cuda_getCurrentRawStream(device)), "page_bounds")
     return bounds
 
 
@@ -2328,42 +2337,38 @@ def select_pages(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int, 
     no more than ``keep``.  ``max_context`` bounds every token's position + 1."""
     T = tok_pos.shape[0]
     _int4_heads(n_heads, n_kv_heads, head_dim)
+    device = _device_here(q, "q")
+    _here(device, (q, "q", torch.bfloat16, None), (tok_pos, "tok_pos", torch.int32, (T,)), (tok_row, "tok_row", torch.int32, (T,)),
+          (bounds, "bounds", torch.bfloat16, (bounds.shape[0], n_kv_heads, 2, head_dim)), (block_table, "block_table", torch.int32, None))
     _query_rows(q, q_stride, T, n_heads * head_dim)
-    _need(bounds, "bounds", torch.bfloat16)
-    if bounds.dim() != 4 or tuple(bounds.shape[1:]) != (n_kv_heads, 2, head_dim) or bounds.data_ptr() % 16:
-        raise KernelError(f"bounds must be [pages, {n_kv_heads}, 2, {head_dim}] from a 16-byte boundary on, not {tuple(bounds.shape)}")
-    _need(tok_pos, "tok_pos", torch.int32, (T,)); _need(tok_row, "tok_row", torch.int32, (T,))
-    rows = _page_table(block_table, table_stride)
-    if keep < 1 or max_context < 1:
-        raise KernelError("keep and max_context must be positive")
-    stream = _stream_here(q, "q")
-    table = torch.empty(T * n_kv_heads, keep, dtype=torch.int32, device=q.device)
-    pos = torch.empty(T * n_kv_heads, dtype=torch.int32, device=q.device)
+    rows = _page_rows(block_table, table_stride)
+    most = min((max_context - 1) // PAGE + 1, table_stride)
+    if keep < 1 or max_context < 1 or most > 10000:
+        raise KernelError("keep and max_context must be positive, and a token's pages at most 10,000")
+    n = T * n_kv_heads
+    table, pos = tok_pos.new_empty((n, keep)), tok_pos.new_empty(n)
     if T:
-        most = min((max_context - 1) // PAGE + 1, table_stride)
-        scores = torch.empty(T * n_kv_heads * most, dtype=torch.int64, device=q.device)       # (the call's own: calls on two streams and captured graphs share none)
+        scores = tok_pos.new_empty(2 * n * most)      # (the call's own: calls on two streams and captured graphs share none)
         check(long_context().pe_select_pages(q.data_ptr(), q_stride, T, n_heads, n_kv_heads, head_dim, bounds.data_ptr(), bounds.shape[0], block_table.data_ptr(), table_stride, rows,
-                                             tok_pos.data_ptr(), tok_row.data_ptr(), keep, int(max_context), table.data_ptr(), pos.data_ptr(), scores.data_ptr(), stream), "select_pages",
-              2 if most > keep > 2 else 1)
+                                             tok_pos.data_ptr(), tok_row.data_ptr(), keep, max_context, table.data_ptr(), pos.data_ptr(), scores.data_ptr(),
+                                             torch._C._cuda_getCurrentRawStream(device)), "select_pages", 2 if most > keep > 2 else 1)
     return SelectedPages(table, pos)
 
 
 def attention_int4_selected(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int, head_dim: int, pool: torch.Tensor, pages: SelectedPages, scale: float,
                             out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``attention_int4`` over the pages that ``select_pages`` has found."""
-    _int4_heads(n_heads, n_kv_heads, head_dim)
-    _int4_pool(pool, n_kv_heads, head_dim)
-    places = pages.pos.shape[0]
+    n_bytes, device, width, places = _int4_heads(n_heads, n_kv_heads, head_dim), _device_here(q, "q"), n_heads * head_dim, pages.pos.shape[0]
     T, keep = places // n_kv_heads, pages.table.shape[1]
-    _need(pages.pos, "pages.pos", torch.int32, (T * n_kv_heads,)); _need(pages.table, "pages.table", torch.int32, (T * n_kv_heads, keep))
-    _query_rows(q, q_stride, T, n_heads * head_dim)
+    _here(device, (q, "q", torch.bfloat16, None), (pool, "pool", torch.uint8, (pool.shape[0], n_kv_heads, n_bytes)), (pages.pos, "pages.pos", torch.int32, (T * n_kv_heads,)),
+          (pages.table, "pages.table", torch.int32, (places, keep)))
+    _query_rows(q, q_stride, T, width)
     if not scale > 0:
         raise KernelError("scale must be positive")
-    out = _int4_out(out, T, n_heads * head_dim, q.device)
-    stream = _stream_here(q, "q")
+    if out is None:
+        out = q.new_empty((T, width))
+    else:
+        _here(device, (out, "out", torch.bfloat16, (T, width)))
     if T:
-        scratch = _int4_scratch(T, n_heads, n_kv_heads, head_dim, keep * PAGE, 1, q.device)
-        check(long_context().pe_attention_int4(q.data_ptr(), q_stride, out.data_ptr(), pool.data_ptr(), pool.shape[0] * n_kv_heads, pages.table.data_ptr(), keep, places,
-                                               pages.pos.data_ptr(), None, T, n_heads, n_kv_heads, head_dim, 0, float(scale), keep * PAGE, 1, 0, _ptr(scratch), status_ptr(q.device), stream),
-              "attention_int4_selected", 1 if scratch is None else 2)
+        _attend_int4(q, q_stride, out, pool, pages.table, keep, places, pages.pos, None, T, n_heads, n_kv_heads, head_dim, 0, scale, keep * PAGE, 1, 0, device, "attention_int4_selected")
     return out
