@@ -69,7 +69,15 @@ struct AtArgs {
     int pool_rows;                                 // rows of the key (and value) pool seen as a matrix [rows][head size]
     const float* sinks;                            // [nh] or null: one more place of this (scaled) score joins a row's denominator and carries no value
     const float* factors;                          // of float16 keys: [pages][nkv], what the scores of a page's keys are multiplied by
+    int n_rows, n_tokens, pool_pages;              // of float16 keys: what runs and page tables may name
+    int splits; float* partial;                    // of float16 keys: CTAs that may share a run and head's steps, and where each leaves its rows' sums
 };
+
+// How many CTAs share the steps of a run (a few steps each at least), and the first step of one of them.
+#define AT_LEAST_STEPS 4
+__device__ __forceinline__ int at_shares(int steps, int splits) { return min(splits, max(1, steps / AT_LEAST_STEPS)); }
+__device__ __forceinline__ int at_share(int z, int steps, int shares) { return z * steps / shares; }
+#define AT_PARTIAL_ROW (AT_HD + 4)                 // of a row: its columns' sums, reference point, sum of weights
 
 // 64 columns of a row of queries, in place: bfloat16 to float16, times `up`
 __device__ __forceinline__ void at_to_half(unsigned row, int r, int groups, int group0, float up) {
@@ -89,8 +97,9 @@ __device__ __forceinline__ void at_to_half(unsigned row, int r, int groups, int 
 // tiles[i] = (batch row, first packed token, number of tokens (<= AT_QTILE), position of the first token)
 // HALF_KEYS: the keys are float16, times a power of two of their page and head (expanded from a cache of fewer bits, whose products with queries bfloat16 keys would be off by more than
 // all else).  The softmax warps then take the queries to float16 before the first product, each row times a power of two of its own, and scores are multiplied back in
-// the exponent's multiply-add, which costs nothing.
-template <bool HALF_KEYS>
+// the exponent's multiply-add, which costs nothing.  SHARED (of those): several CTAs share a run and head's steps (blockIdx.z) and leave the rows' sums to a second kernel; a variant of
+// its own, since what it keeps in registers is spilled in the loop (7,541 tokens, 28 heads of 128: 274 us without, 304 with it).
+template <bool HALF_KEYS, bool SHARED>
 __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q,
                                                                                   const __grid_constant__ CUtensorMap map_k,
                                                                                   const __grid_constant__ CUtensorMap map_v,
@@ -125,12 +134,23 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
     const int first_key = (p.window > 0 && pos0 - p.window + 1 > 0) ? pos0 - p.window + 1 : 0;
     // (with kept first keys: their pages first, then the window's; where the two meet, all pages from the sequence's start)
     int page_lo = first_key / AT_KTILE, kept = 0;
-    const int page_hi = (pos0 + n - 1) / AT_KTILE;
+    const int page_hi = HALF_KEYS ? min((pos0 + n - 1) / AT_KTILE, p.table_stride - 1) : (pos0 + n - 1) / AT_KTILE;
     if (p.window > 0 && p.keep_first > 0) {
         const int keep_pages = (p.keep_first + AT_KTILE - 1) / AT_KTILE;
         if (page_lo <= keep_pages) page_lo = 0; else kept = keep_pages;
     }
-    const int n_pages = kept + page_hi - page_lo + 1, n_steps = (n_pages + 1) / 2;
+    int n_pages = kept + page_hi - page_lo + 1, n_steps = (n_pages + 1) / 2, shares = 1;
+    if constexpr (HALF_KEYS) {
+        if (brow < 0 || brow >= p.n_rows || n <= 0 || n > AT_QTILE || pos0 < 0 || tok0 < 0 || tok0 + n > p.n_tokens || n_pages <= 0) return;      // (no run of this call)
+        if constexpr (SHARED) {                                     // this CTA's share of the steps
+            shares = at_shares(n_steps, p.splits);
+            if ((int)blockIdx.z >= shares) return;                  // (nothing is allocated yet)
+            const int from = at_share(blockIdx.z, n_steps, shares), to = at_share(blockIdx.z + 1, n_steps, shares);
+            page_lo += 2 * from;
+            n_pages = min(2 * to, n_pages) - 2 * from;
+            n_steps = to - from;
+        }
+    }
     auto page_at = [&](int j) { return j < kept ? j : page_lo + j - kept; };     // the j-th page the run reads, j < n_pages
 
     const int* table = p.block_table + (size_t)brow * p.table_stride;
@@ -276,7 +296,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
         for (int it = g; it < n_steps && ok; it += 2) {
             const int b = it % AT_BUFFERS;
             const unsigned s_addr = lane_addr + b * (2 * AT_KTILE);
-            const bool there[2] = {entry[0] >= 0, entry[1] >= 0};   // (a page that is not there was read as zeros and is masked)
+            const bool there[2] = {entry[0] >= 0 && (!HALF_KEYS || entry[0] < p.pool_pages), entry[1] >= 0 && (!HALF_KEYS || entry[1] < p.pool_pages)};   // (a page that is not there was read as zeros and is masked)
             float page_scale[2] = {1.f, 1.f};                       // of float16 keys: what takes the page's scores to powers of two
             if constexpr (HALF_KEYS) {
 #pragma unroll
@@ -285,7 +305,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
 #pragma unroll
             for (int x = 0; x < 2; ++x) entry[x] = 2 * it + 4 + x < n_pages ? table[page_at(2 * it + 4 + x)] : -1;
             if (!at_wait_warp(at_smem(&s_full[b]), (unsigned)(it / AT_BUFFERS) & 1u)) { ok = false; break; }
-            if (it + 1 == n_steps && (pos0 + n) % AT_KTILE) {       // values behind the run's last token, in the second or the first of the step's pages
+            if (!HALF_KEYS && it + 1 == n_steps && (pos0 + n) % AT_KTILE) {       // (expanded pages have zeros there) values behind the run's last token, in the second or the first of the step's pages
                 if (!at_wait_warp(at_smem(&v_full[it % AT_STAGES]), (unsigned)(it / AT_STAGES) & 1u)) { ok = false; break; }
                 at_clear_rows(kv_s + it % AT_STAGES * AT_STAGE_BYTES + AT_STAGE_BYTES / 2, AT_PANELS, 2 * AT_KTILE * 128,
                               (n_pages - 1 - 2 * it) * AT_KTILE + (pos0 + n) % AT_KTILE, (threadIdx.x - 64) & 127, 128);
@@ -399,20 +419,36 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
                 if (m != -INFINITY) l = fmaf(sums[w * AT_QTILE + r], at_exp2(m - m_run), l);
             }
             if (p.sinks) l += at_exp2(fmaf(p.sinks[h], 1.4426950408889634f, -m_run));   // (a row that saw no key: 2^inf, and 1 / l = 0)
-            const float inv = l > 0.f ? 1.0f / l : 0.f;
-            // through the queries' place: the last products have read them
-            const unsigned o_addr = lane_addr + AT_O_COL + g * (AT_HD / 2);
-            constexpr int GROUPS = AT_HD / 16;                      // 16-byte groups of a warpgroup's half of a row
+            if constexpr (SHARED) {
+                if (shares > 1) {                                   // a share of the row's sums, for the kernel that joins them
+                    float* to = p.partial + (((size_t)(blockIdx.y * p.nh + h) * p.splits + blockIdx.z) * AT_QTILE + r) * AT_PARTIAL_ROW;
+                    if (r < n && g == 0) *reinterpret_cast<float2*>(to + AT_HD) = make_float2(m_run, l);
+#pragma unroll 1
+                    for (int c = 0; c < AT_HD / 2; c += 32) {
+                        float o[32];
+                        at_ld32(lane_addr + AT_O_COL + g * (AT_HD / 2) + c, o);                    // (the whole warp)
+                        if (r < n)
 #pragma unroll
-            for (int c = 0; c < AT_HD / 2; c += 32) {
-                float o[32];
-                unsigned packed[16];
-                at_ld32(o_addr + c, o);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) packed[i] = at_pack(o[2 * i] * inv, o[2 * i + 1] * inv);
-                at_put_row<32>(q_s, AT_HD * 2, r, g * GROUPS + c / 8, packed);
+                            for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(to + g * (AT_HD / 2) + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    }
+                }
             }
-            at_store_rows<AT_HD / 2>(q_s, AT_HD * 2, quarter * 32, g * GROUPS, n, p.out + ((size_t)tok0 * p.nh + h) * AT_HD + g * (AT_HD / 2), (size_t)p.nh * AT_HD, lane);
+            const float inv = l > 0.f ? 1.0f / l : 0.f;
+            if (!SHARED || shares == 1) {
+                // through the queries' place: the last products have read them
+                const unsigned o_addr = lane_addr + AT_O_COL + g * (AT_HD / 2);
+                constexpr int GROUPS = AT_HD / 16;                      // 16-byte groups of a warpgroup's half of a row
+#pragma unroll
+                for (int c = 0; c < AT_HD / 2; c += 32) {
+                    float o[32];
+                    unsigned packed[16];
+                    at_ld32(o_addr + c, o);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) packed[i] = at_pack(o[2 * i] * inv, o[2 * i + 1] * inv);
+                    at_put_row<32>(q_s, AT_HD * 2, r, g * GROUPS + c / 8, packed);
+                }
+                at_store_rows<AT_HD / 2>(q_s, AT_HD * 2, quarter * 32, g * GROUPS, n, p.out + ((size_t)tok0 * p.nh + h) * AT_HD + g * (AT_HD / 2), (size_t)p.nh * AT_HD, lane);
+            }
         }
         if (!ok) atomicExch(status, 5);
     }
@@ -424,21 +460,52 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
     }
 }
 
+// The shares of a run and head, joined: a warp a row, in float32.
+__global__ void __launch_bounds__(256) attention_prefill_join_kernel(const AtArgs p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int4 info = p.tiles[blockIdx.y];
+    const int tok0 = info.y, n = info.z, pos0 = info.w, h = blockIdx.x, lane = threadIdx.x & 31;
+    const int first_key = (p.window > 0 && pos0 - p.window + 1 > 0) ? pos0 - p.window + 1 : 0;
+    const int n_pages = min((pos0 + n - 1) / AT_KTILE, p.table_stride - 1) - first_key / AT_KTILE + 1;
+    if (info.x < 0 || info.x >= p.n_rows || n <= 0 || n > AT_QTILE || pos0 < 0 || tok0 < 0 || tok0 + n > p.n_tokens || n_pages <= 0) return;
+    const int shares = at_shares((n_pages + 1) / 2, p.splits);
+    if (shares == 1) return;
+    constexpr int COLS = AT_HD / 32;                                // columns a lane
+    for (int r = blockIdx.z * 8 + (threadIdx.x >> 5); r < n; r += gridDim.z * 8) {
+        const float* from = p.partial + ((size_t)(blockIdx.y * p.nh + h) * p.splits * AT_QTILE + r) * AT_PARTIAL_ROW;
+        float m = -INFINITY, l = 0.f, o[COLS] = {};
+        for (int z = 0; z < shares; ++z) m = fmaxf(m, from[(size_t)z * AT_QTILE * AT_PARTIAL_ROW + AT_HD]);
+        for (int z = 0; z < shares; ++z) {
+            const float* row = from + (size_t)z * AT_QTILE * AT_PARTIAL_ROW;
+            const float2 ml = *reinterpret_cast<const float2*>(row + AT_HD);
+            const float w = ml.x == -INFINITY ? 0.f : at_exp2(ml.x - m);
+            l = fmaf(ml.y, w, l);
+#pragma unroll
+            for (int c = 0; c < COLS; ++c) o[c] = fmaf(row[lane * COLS + c], w, o[c]);
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        bf16* to = p.out + ((size_t)(tok0 + r) * p.nh + h) * AT_HD + lane * COLS;
+#pragma unroll
+        for (int c = 0; c < COLS; c += 2) *reinterpret_cast<unsigned*>(to + c) = at_pack(o[c] * inv, o[c + 1] * inv);
+    }
+}
+
 extern "C" int pe_attention_prefill_tcgen05_tile() { return AT_QTILE; }
 
 // how many of the kernel's CTAs an SM holds at once (one: it takes all of tensor memory), or a negative CUDA error
 extern "C" int pe_attention_prefill_tcgen05_ctas_per_sm() {
     int n = 0;
-    if (cudaFuncSetAttribute(attention_prefill_tcgen05_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)AT_SMEM_BYTES) != cudaSuccess) return -1;
-    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attention_prefill_tcgen05_kernel<false>, AT_THREADS, AT_SMEM_BYTES);
+    if (cudaFuncSetAttribute(attention_prefill_tcgen05_kernel<false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)AT_SMEM_BYTES) != cudaSuccess) return -1;
+    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attention_prefill_tcgen05_kernel<false, false>, AT_THREADS, AT_SMEM_BYTES);
     return e == cudaSuccess ? n : -(int)e;
 }
 
 // q: [n_tokens][q_stride] with head h at columns h * hd; pools: [pool_pages][nkv][64][hd]
-template <bool HALF_KEYS>
+template <bool HALF_KEYS, bool SHARED>
 static int at_launch(const void* q, int q_stride, void* out, const void* k_pool, const void* v_pool, long long pool_pages, const int* block_table, int table_stride, const void* tiles,
                      int n_tiles, int n_tokens, int nh, int nkv, int hd, int window, float scale, int keep_first, const float* slopes, int* status, void* stream, const float* sinks,
-                     const float* factors) {
+                     const float* factors, int splits, float* partial, int n_rows) {
     if (n_tiles <= 0) return 0;
     if (hd != AT_HD || nkv <= 0 || nh % nkv || n_tiles > 65535 || q_stride % 8 || !(scale > 0.f) || !status) return PE_ERR_UNSUPPORTED;
     if (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)out | (uintptr_t)tiles) & 15) return PE_ERR_UNSUPPORTED;
@@ -455,32 +522,55 @@ static int at_launch(const void* q, int q_stride, void* out, const void* k_pool,
     p.nh = nh; p.nkv = nkv; p.window = window; p.scale_log2e = scale * 1.4426950408889634f;
     p.keep_first = window > 0 && keep_first > 0 ? keep_first : 0; p.slopes = slopes; p.inv_scale = 1.0f / scale;
     p.pool_rows = (int)(pool_pages * nkv * AT_KTILE);
-    p.sinks = sinks; p.factors = factors;
+    p.n_rows = n_rows; p.n_tokens = n_tokens; p.pool_pages = (int)pool_pages;
+    p.sinks = sinks; p.factors = factors; p.splits = splits; p.partial = partial;
     const size_t smem = AT_SMEM_BYTES;
     static bool attr_set = false;
     if (!attr_set) {
-        PE_TRY(cudaFuncSetAttribute(attention_prefill_tcgen05_kernel<HALF_KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        PE_TRY(cudaFuncSetAttribute(attention_prefill_tcgen05_kernel<HALF_KEYS, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         attr_set = true;
     }
-    PE_TRY(pe_launch(attention_prefill_tcgen05_kernel<HALF_KEYS>, dim3(nh, n_tiles), AT_THREADS, smem, (cudaStream_t)stream, mq, mk, mv, p, status));
+    PE_TRY(pe_launch(attention_prefill_tcgen05_kernel<HALF_KEYS, SHARED>, dim3(nh, n_tiles, splits), AT_THREADS, smem, (cudaStream_t)stream, mq, mk, mv, p, status));
+    if (splits > 1) PE_TRY(pe_launch(attention_prefill_join_kernel, dim3(nh, n_tiles, 4), 256, 0, (cudaStream_t)stream, p));
     return 0;
+}
+
+// Into how many shares the steps of a run and head are cut, where all runs and heads together are fewer than the SMs: the number whose last wave ends first, a step taken for
+// 1 and the rest of a CTA for 5 (0.93 us and 4.3).  500 tokens on 15,937 positions, 14 heads of 64: 56 CTAs of 128 steps, 130 us in one share, AT_MEASURED in five.
+static int at_splits(long long ctas, int table_stride) {
+    const int steps = (table_stride + 1) / 2, sms = pe_sm_count();
+    int best = 1;
+    double least = 1e30;
+    for (int s = 1; s <= 8 && (s == 1 || s * AT_LEAST_STEPS * 4 <= steps); ++s) {
+        const double t = (double)((ctas * s + sms - 1) / sms) * ((double)steps / s + 5.0) + (s > 1 ? 5.0 : 0.0);
+        if (t < 0.9 * least) { least = t; best = s; }
+    }
+    return ctas < sms ? best : 1;
 }
 
 extern "C" int pe_attention_prefill_tcgen05(const void* q, int q_stride, void* out, const void* k_pool, const void* v_pool,
                                             long long pool_pages, const int* block_table, int table_stride, const void* tiles,
                                             int n_tiles, int n_tokens, int nh, int nkv, int hd, int window, float scale,
                                             int keep_first, const float* slopes, int* status, void* stream, const float* sinks) {
-    return at_launch<false>(q, q_stride, out, k_pool, v_pool, pool_pages, block_table, table_stride, tiles, n_tiles, n_tokens, nh, nkv, hd, window, scale, keep_first, slopes, status,
-                            stream, sinks, nullptr);
+    return at_launch<false, false>(q, q_stride, out, k_pool, v_pool, pool_pages, block_table, table_stride, tiles, n_tiles, n_tokens, nh, nkv, hd, window, scale, keep_first, slopes, status,
+                            stream, sinks, nullptr, 1, nullptr, 0);
+}
+
+// Bytes of scratch that the next one needs (0: none).
+extern "C" long long pe_attention_prefill_half_keys_scratch(int n_tiles, int nh, int table_stride) {
+    const long long ctas = (long long)n_tiles * nh;
+    const int s = ctas > 0 ? at_splits(ctas, table_stride) : 1;
+    return s > 1 ? ctas * s * AT_QTILE * AT_PARTIAL_ROW * 4 : 0;
 }
 
 // The same over float16 keys, the scores of a page's keys times factors[page][kv head].
 extern "C" int pe_attention_prefill_half_keys(const void* q, int q_stride, void* out, const void* k_pool, const void* v_pool, const float* factors, long long pool_pages,
-                                              const int* block_table, int table_stride, const void* tiles, int n_tiles, int n_tokens, int nh, int nkv, int hd, int window,
-                                              float scale, int* status, void* stream) {
-    if (!factors) return PE_ERR_UNSUPPORTED;
-    return at_launch<true>(q, q_stride, out, k_pool, v_pool, pool_pages, block_table, table_stride, tiles, n_tiles, n_tokens, nh, nkv, hd, window, scale, 0, nullptr, status, stream,
-                           nullptr, factors);
+                                              const int* block_table, int table_stride, int n_rows, const void* tiles, int n_tiles, int n_tokens, int nh, int nkv, int hd, int window,
+                                              float scale, void* scratch, int* status, void* stream) {
+    if (!factors || ((uintptr_t)scratch & 15)) return PE_ERR_UNSUPPORTED;
+    const int splits = scratch ? at_splits((long long)n_tiles * nh, table_stride) : 1;
+    return (splits > 1 ? at_launch<true, true> : at_launch<true, false>)(q, q_stride, out, k_pool, v_pool, pool_pages, block_table, table_stride, tiles, n_tiles, n_tokens, nh, nkv, hd, window,
+                                                                         scale, 0, nullptr, status, stream, nullptr, factors, splits, (float*)scratch, n_rows);
 }
 
 #else   // other head sizes: the mma.sync kernel of attention_prefill.cu takes them
@@ -491,8 +581,9 @@ extern "C" int pe_attention_prefill_tcgen05(const void*, int, void*, const void*
                                             int, int, int, int, int, int, float, int, const float*, int*, void*, const float*) {
     return PE_ERR_UNSUPPORTED;
 }
-extern "C" int pe_attention_prefill_half_keys(const void*, int, void*, const void*, const void*, const float*, long long, const int*, int, const void*, int, int, int, int, int, int,
-                                              float, int*, void*) {
+extern "C" long long pe_attention_prefill_half_keys_scratch(int, int, int) { return 0; }
+extern "C" int pe_attention_prefill_half_keys(const void*, int, void*, const void*, const void*, const float*, long long, const int*, int, int, const void*, int, int, int, int, int, int,
+                                              float, void*, int*, void*) {
     return PE_ERR_UNSUPPORTED;
 }
 

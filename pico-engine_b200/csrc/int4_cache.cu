@@ -343,7 +343,8 @@ extern "C" int pe_page_bounds(const void* pool, long long n_pages, int n_kv, int
 // ---------------------------------------------------------------------------- pages in 16 bits, for prompts
 // What the runs of a prompt read of a 4-bit cache, as operands of tcgen05.mma: values as bfloat16, keys as float16 times a power of two of their page and head (`factors` takes it
 // back), so that a key keeps 11 bits whatever its size: with keys of 8 bits the scores' errors are what the results are off by (0.0055 of their size; 0.0024 so).  Positions behind a
-// row's last run are zeros.  Expanded once a page and head, for all heads and runs that read it: 7.4 MB to 24 MB of a layer for prompts of 7,541 tokens.
+// row's last run are zeros.  A value with a group that is no number is zeros, and its key is none: a query that sees it has no result then, and one that does not keeps its own (a weight of zero
+// would not keep the value out of its sum).  Expanded once a page and head, for all heads and runs that read it: 7.4 MB to 24 MB of a layer for prompts of 7,541 tokens.
 // A block counts the pages of all rows from the runs, then takes every gridDim.x-th of them.
 
 #define XI_MAX_ROWS 1024
@@ -355,6 +356,7 @@ __global__ void __launch_bounds__(XI_THREADS) expand_int4_kernel(const unsigned 
     using B = Int4Block<D>;
     __shared__ int low[XI_MAX_ROWS], behind[XI_MAX_ROWS], before[XI_MAX_ROWS + 1];     // a row's first page, the position behind its last run, the pages of the rows before it
     __shared__ float largest[XI_THREADS / 32];
+    __shared__ bool none[PE_PAGE];                             // positions whose value has a group that is no number
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -396,7 +398,13 @@ __global__ void __launch_bounds__(XI_THREADS) expand_int4_kernel(const unsigned 
             most = fmaxf(most, fmaf(7.5f, fabsf(to_f(meta[0])), fabsf(to_f(meta[B::groups]))));
         }
         most = warp_max(most);
-        __syncthreads();                                       // (the last page's maxima have been read)
+        __syncthreads();                                       // (the last page's maxima and marks have been read)
+        if (threadIdx.x < PE_PAGE) {
+            bool any = false;
+#pragma unroll
+            for (int b = 0; b < B::groups; ++b) { const float m = to_f(*reinterpret_cast<const bf16*>(block + q4_value_step<D>(threadIdx.x, b))); any |= m != m; }
+            none[threadIdx.x] = any && threadIdx.x < there;
+        }
         if (lane == 0) largest[warp] = most;
         __syncthreads();
 #pragma unroll
@@ -419,6 +427,7 @@ __global__ void __launch_bounds__(XI_THREADS) expand_int4_kernel(const unsigned 
 #pragma unroll
                 for (int e = 0; e < 4; ++e) two[e] = __floats2half2_rn(fmaf(s, q4_level(word, e, 0), m), fmaf(s, q4_level(word, e, 1), m));
                 v = *reinterpret_cast<uint4*>(two);
+                if (none[p]) v = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
             }
             *reinterpret_cast<uint4*>(ko + p * D + 32 * b + 8 * t) = v;
         }
@@ -435,7 +444,7 @@ __global__ void __launch_bounds__(XI_THREADS) expand_int4_kernel(const unsigned 
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
                         uint2 v = make_uint2(0u, 0u);
-                        if (p < there) {
+                        if (p < there && !none[p]) {
                             const bf16* meta = reinterpret_cast<const bf16*>(block + q4_value_step<D>(p, 2 * h + b));
                             const float s = to_f(meta[0]), m = to_f(meta[B::groups * 16]);
                             __nv_bfloat162 two[2];

@@ -400,3 +400,51 @@ def test_refusals(K):
     none = torch.empty(0, dtype=torch.int32, device="cuda")
     assert K.attention_int4(q[:0], q.shape[1], 4, 2, 64, p.pool, p.table, p.width, none, none, None, 1.0, 1).shape == (0, 256)
     assert K.load_int4(p.pool, 2, 64, none, none, p.table, p.width)[0].shape == (0, 2, 64)
+
+
+def test_prompts_over_groups_that_are_none(K):
+    """A value or key that is no number reaches the tokens that see it, and no other."""
+    H, G, D, n = 4, 2, 64, 300
+    p = Paged(H, G, D, [n], 81)
+    q = randn(n, H * D, seed=7).bfloat16()
+    tiles = K.prefill_tiles([n], [0], "cuda", K.PREFILL_TILE_TCGEN05)
+    run = lambda: K.attention_int4_prompt(q, H * D, H, G, D, p.pool, p.table, p.width, tiles, n, None, p.scale)     # noqa: E731
+    clean = run()
+    keys, values = p.keys.clone(), p.values.clone()
+    keys[p.pages[0][1], 0, 36, 3], values[p.pages[0][3], 1, 8, 40] = float("nan"), float("inf")                       # positions 100 and 200
+    p.pool = plain.pack(keys.view(-1, 64, D), values.view(-1, 64, D)).view(p.n_pages, G, 80 * D)
+    out = run().view(n, H, D)
+    first, second = out[:, :2], out[:, 2:]
+    assert torch.equal(first[:100], clean.view(n, H, D)[:100, :2]) and torch.isnan(first[100:]).all()
+    assert torch.equal(second[:200], clean.view(n, H, D)[:200, 2:]) and torch.isnan(second[200:]).all()
+
+
+def test_runs_and_pages_that_are_none_of_the_call(K):
+    """Runs of rows, tokens or positions that the call does not have, and pages beyond the pool, read and write nothing."""
+    H, G, D = 4, 2, 64
+    p = Paged(H, G, D, [200], 91)
+    q = randn(200, H * D, seed=8).bfloat16()
+    out = torch.full((200, H * D), 7.0, dtype=torch.bfloat16, device="cuda")
+    table = p.table.clone()
+    table[0, 1] = p.n_pages + 5
+    runs = [[0, 0, 40, 130], [1, 50, 10, 0], [-1, 50, 10, 0], [0, 190, 20, 0], [0, 60, 0, 0], [0, 70, 10, -5], [0, -3, 10, 0], [0, 90, 5, 64 * p.width + 1000]]
+    K.attention_int4_prompt(q, H * D, H, G, D, p.pool, table, p.width, ints(runs), 200, None, p.scale, out=out)
+    assert (out[40:90] == 7).all() and (out[95:] == 7).all()
+    there = table.clone()
+    there[0, 1] = -1
+    p.check(out[:40], list(range(130, 170)), [0] * 40, q=q[:40], table=there, halves=True)
+    got = p.attention(K, [180], [0], q=q, table=table)
+    p.check(got, [180], [0], q=q, table=there)
+
+
+@pytest.mark.parametrize("H,G,D", [(14, 2, 64), (4, 1, 128)])
+@pytest.mark.parametrize("start,n,window", [(4000, 200, None), (5000, 1, None), (3000, 130, 2500), (300, 100, None)])
+def test_a_prompt_behind_a_long_context(K, H, G, D, start, n, window):
+    """Few runs on many pages: their steps are shared by several CTAs."""
+    p = Paged(H, G, D, [start + n, 70], 101)
+    q = randn(n + 70, H * D, seed=9, scale=1.5).bfloat16()
+    tiles = K.prefill_tiles([n, 70], [start, 0], "cuda", K.PREFILL_TILE_TCGEN05)
+    got = K.attention_int4_prompt(q, H * D, H, G, D, p.pool, p.table, p.width, tiles, n + 70, window, p.scale)
+    some = sorted({0, n // 2, n - 1, n, n + 33, n + 69})
+    pos = [start + i if i < n else i - n for i in some]
+    p.check(got[some], pos, [0 if i < n else 1 for i in some], q=q[some], window=window, halves=True)
