@@ -781,9 +781,12 @@ struct AiStreamLaunch {
 
 // Whether a call's blocks are dealt to the warps in equal runs: from 35,000 blocks on, the longest sequence's for every row (one CTA or cluster a pair / equal runs, us; 14 heads of 64 on 2: 64 rows of 20,000
 // to 32,700 72 / 65, 200 of up to 6,000 37 / 35, 32 of 4,000 to 8,192 16.6 / 22.7; 28 heads of 128 on 4: 200 of up to 6,000 94 / 86, 64 of 6,000 to 8,000 63.7 / 64.5, 16 of 8,000 to 16,000 37 / 40).
+// Selected pages are as many a row as the call says: one CTA a pair takes (16 + pages) units for each wave of as many pairs as SMs, equal runs 50 + 1.25 a block and SM (a unit is 0.23 us of 128
+// channels, 0.14 of 64).  28 heads of 128 on 4, us: 38 rows of 128 pages 65 / 48, 48 of 64 37.5 / 37.1, 64 of 64 39 / 44, 48 of 32 21 / 23.
 static bool ai_streams(int T, int n_heads, int n_kv, int hd, int max_context, int selected) {
-    const long long places = selected ? (long long)T * n_kv : T, pairs = (long long)T * n_kv * ((n_heads / n_kv + 7) / 8), pages = (max_context - 1) / PE_PAGE + 1;
-    return places <= AI_MAX_PLACES && pairs * pages >= 35000 && pairs * pages <= 0x7fffffffll;
+    const long long places = selected ? (long long)T * n_kv : T, pairs = (long long)T * n_kv * ((n_heads / n_kv + 7) / 8), pages = (max_context - 1) / PE_PAGE + 1, sms = pe_sm_count();
+    if (places > AI_MAX_PLACES || pairs * pages > 0x7fffffffll) return false;
+    return selected ? pairs > sms && 4 * ((pairs + sms - 1) / sms) * (16 + pages) * sms >= 200 * sms + 5 * pairs * pages : pairs * pages >= 35000;
 }
 
 extern "C" void pe_set_pdl(int on) { pe_pdl_enabled() = on ? 1 : 0; }
