@@ -28,9 +28,13 @@ __device__ __forceinline__ float ps_max(float a, float b) { float r; asm("max.Na
 struct PsArgs {
     const bf16* q; const bf16* bounds; const int* block_table; const int* tok_pos; const int* tok_row;
     int q_stride, n_heads, n_kv, n_pages, table_stride, n_rows, keep, most;
-    // pages of a token (its own the last), and its row of the page table
-    __device__ __forceinline__ int pages(int pos) const { return min(min(pos / PE_PAGE + 1, table_stride), most); }
-    __device__ __forceinline__ const int* table(int tok) const { return block_table + (size_t)min(max(tok_row[tok], 0), n_rows - 1) * table_stride; }
+    // a token's position (-1: it sees nothing), its pages, its own the last, and its row of the page table
+    __device__ __forceinline__ int position(int tok) const {
+        const int row = tok_row[tok];
+        return row >= 0 && row < n_rows ? max(-1, min(tok_pos[tok], most * PE_PAGE - 1)) : -1;
+    }
+    __device__ __forceinline__ int pages(int pos) const { return pos < 0 ? 0 : pos / PE_PAGE + 1; }
+    __device__ __forceinline__ const int* table(int tok) const { return block_table + (size_t)tok_row[tok] * table_stride; }
 };
 
 template <int D>
@@ -46,7 +50,7 @@ __global__ void __launch_bounds__(PS_THREADS) score_pages_kernel(const PsArgs p,
     pdl_launch_dependents();
     pdl_wait();
     const int kvh = blockIdx.y, tok = blockIdx.z, G = p.n_heads / p.n_kv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % S::lanes;
-    const int pages = p.pages(max(p.tok_pos[tok], 0)), first = 1 + (int)blockIdx.x * S::pages;
+    const int pages = p.pages(p.position(tok)), first = 1 + (int)blockIdx.x * S::pages;
     if (pages <= p.keep || first >= pages - 1) return;         // (the first and the last page are kept whatever they score)
     const int* table = p.table(tok);
     uint4 v[S::ahead][2];
@@ -184,10 +188,10 @@ __global__ void __launch_bounds__(PS_THREADS) select_pages_kernel(const PsArgs p
     pdl_launch_dependents();
     pdl_wait();
     const int kvh = blockIdx.x, tok = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_kv = p.n_kv, keep = p.keep;
-    const int pos = max(p.tok_pos[tok], 0), pages = p.pages(pos);
+    const int pos = p.position(tok), pages = p.pages(pos);
     const bool choose = pages > keep && keep > 2;
     const int wanted = keep - 2;                               // besides the first and the last page
-    {
+    if (pages) {
         const int* table = p.table(tok);
         const float2* scores = all_scores + ((size_t)tok * n_kv + kvh) * p.most;
         float error = 0.f;
@@ -310,7 +314,7 @@ __global__ void __launch_bounds__(PS_THREADS) select_pages_kernel(const PsArgs p
         if (kept) mine[at] = entries[j] >= 0 ? entries[j] * n_kv + kvh : -1;
     }
     for (int i = done + threadIdx.x; i < keep; i += PS_THREADS) mine[i] = -1;
-    if (threadIdx.x == 0) out_pos[tok * n_kv + kvh] = (done - 1) * PE_PAGE + pos % PE_PAGE;
+    if (threadIdx.x == 0) out_pos[tok * n_kv + kvh] = done ? (done - 1) * PE_PAGE + pos % PE_PAGE : -1;
 }
 
 static int ps_most(int max_context, int table_stride) { const int pages = (max_context - 1) / PE_PAGE + 1; return pages < table_stride ? pages : table_stride; }

@@ -2339,7 +2339,7 @@ def select_pages(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int, 
                  tok_pos: torch.Tensor, tok_row: torch.Tensor, keep: int, max_context: int) -> SelectedPages:
     """For every token and key/value head the ``keep`` pages to attend to: its own, the sequence's first (where ``keep`` is 2 or more), and those whose keys can score highest by
     their ``bounds`` (``page_bounds``): the sum over the head's queries and over the channels of max(q * least, q * greatest), in float64; of equal ones the earlier page.  All pages, where a token sees
-    no more than ``keep``.  ``max_context`` bounds every token's position + 1."""
+    no more than ``keep``; none (and place -1) for a token in front of position 0 or of no row of the table.  ``max_context`` bounds every token's position + 1."""
     T = tok_pos.shape[0]
     _int4_heads(n_heads, n_kv_heads, head_dim)
     device = _device_here(q, "q")

@@ -316,6 +316,28 @@ def test_selected_pages(K, H, G, D, keep):
         assert ((got[t].double().view(H, D) - w).abs() <= bound + 1e-30).all()
 
 
+@pytest.mark.parametrize("H,G,D,rows,keep", [(28, 4, 128, 38, 12), (14, 2, 64, 96, 40), (20, 1, 128, 150, 30)])
+def test_selected_pages_of_many_rows(K, H, G, D, rows, keep):
+    lengths = [1 + (b * 677) % (64 * 60) for b in range(rows)]
+    p = Paged(H, G, D, lengths, 43, rubbish=float("nan"))
+    bounds = bounds_of(p)
+    pos, row = [n - 1 for n in lengths], list(range(rows))
+    pages = K.select_pages(p.q, p.q.shape[1], H, G, D, bounds, p.table, p.width, ints(pos), ints(row), keep, max(lengths))
+    got = K.attention_int4_selected(p.q, p.q.shape[1], H, G, D, p.pool, pages, p.scale)
+    wide = K.SelectedPages(torch.cat([pages.table, torch.full((rows * G, 300 - keep), -1, dtype=torch.int32, device="cuda")], 1), pages.pos)      # a launch for more
+    for out in (got, K.attention_int4_selected(p.q, p.q.shape[1], H, G, D, p.pool, wide, p.scale)):
+        for t in range(0, rows, 7):
+            seen = torch.zeros(G, p.width * PAGE, dtype=torch.bool, device="cuda")
+            for g in range(G):
+                for page in pages.table[t * G + g].tolist():
+                    if page >= 0:
+                        j = p.pages[t].index(page // G)
+                        seen[g, j * PAGE: (j + 1) * PAGE] = True
+            seen[:, pos[t] + 1:] = False
+            w, bound = plain.attend(p.q[t, :H * D].view(H, D), p.pool[p.table[t].clamp(min=0).long()], seen, p.scale)
+            assert ((out[t].double().view(H, D) - w).abs() <= bound + 1e-30).all()
+
+
 def test_pages_that_score_alike_and_bounds_that_are_none(K):
     H, G, D = 4, 2, 64
     p = Paged(H, G, D, [64 * 30], 51)
@@ -328,6 +350,22 @@ def test_pages_that_score_alike_and_bounds_that_are_none(K):
     bounds[p.pages[0][20], :, 1] = float("inf")
     pages = K.select_pages(*args)
     assert pages.table.tolist() == [ids([0, 1, 2, 20, 29], 0), ids([0, 1, 17, 20, 29], 1)]
+
+
+def test_tokens_that_see_nothing_and_positions_behind_the_table(K):
+    H, G, D = 14, 2, 64
+    p = Paged(H, G, D, [64 * 9, 64 * 9, 64 * 9, 700], 52)
+    bounds = bounds_of(p)
+    pos, row = [-1, 300, 300, 64 * p.width + 5, 575], [0, -1, 4, 3, 1]
+    q = randn(5, H * D, seed=5).bfloat16()
+    for keep in (2, 5, 40):
+        pages = K.select_pages(q, H * D, H, G, D, bounds, p.table, p.width, ints(pos), ints(row), keep, 64 * p.width + 10)
+        assert (pages.table[:3 * G] == -1).all() and (pages.pos[:3 * G] == -1).all()
+        got = K.attention_int4_selected(q, H * D, H, G, D, p.pool, pages, p.scale)
+        assert (got[:3] == 0).all()
+        assert pages.pos[4 * G:].tolist() == [(min(keep, 9) - 1) * 64 + 63] * G
+    assert torch.equal(pages.pos[3 * G: 4 * G], ints([64 * p.width - 1] * G))
+    p.check(got[3:], [64 * p.width - 1, 575], [3, 1], q=q[3:])
 
 
 def test_a_context_of_many_pages(K):
