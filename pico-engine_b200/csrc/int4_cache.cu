@@ -168,7 +168,12 @@ __global__ void __launch_bounds__(SI_THREADS, 4) store_int4_kernel(const bf16* q
         const int n = threadIdx.x, r = n < SI_TOKENS ? at_pos[n] & 15 : 0;
         bool leads = n < SI_TOKENS && at_page[n] >= 0;
         unsigned own = 0, from = ~0u;
-        bool mine = true;
+        // where positions of a tile follow one another with a gap, tokens that lead parts of one word stand where nobody looks for them
+        bool gap = false;
+#pragma unroll
+        for (int k = n + 1; k < 3 * SI_TOKENS; k += 32)
+            gap |= near_row[k] == near_row[k - 1] && near_pos[k] >> 4 == near_pos[k - 1] >> 4 && near_pos[k] != near_pos[k - 1] + 1;
+        bool mine = !__any_sync(0xffffffffu, gap);
         if (leads)
 #pragma unroll
             for (int f = 0; f < 2; ++f)
@@ -379,6 +384,7 @@ __global__ void __launch_bounds__(XI_THREADS) expand_int4_kernel(const unsigned 
     using B = Int4Block<D>;
     __shared__ int low[XI_MAX_ROWS], behind[XI_MAX_ROWS], before[XI_MAX_ROWS + 1];     // a row's first page, the position behind its last run, the pages of the rows before it
     __shared__ float largest[XI_THREADS / 32];
+    __shared__ int further[XI_THREADS / 32];
     __shared__ bool none[PE_PAGE];                             // positions whose value has a group that is no number
     pdl_launch_dependents();
     pdl_wait();
@@ -410,8 +416,20 @@ __global__ void __launch_bounds__(XI_THREADS) expand_int4_kernel(const unsigned 
         const int kvh = (int)(item % n_kv), x = (int)(item / n_kv);
         int row = 0, top = n_rows;
         while (top - row > 1) { const int mid = (row + top) >> 1; if (before[mid] <= x) row = mid; else top = mid; }
-        const int j = low[row] + x - before[row], there = min(PE_PAGE, behind[row] - j * PE_PAGE), page = block_table[(size_t)row * table_stride + j];
+        const int j = low[row] + x - before[row], page = block_table[(size_t)row * table_stride + j];
         if (page < 0 || page >= n_pages) continue;             // (the same for the whole block)
+        int there = min(PE_PAGE, behind[row] - j * PE_PAGE);
+        if (there < PE_PAGE) {
+            // another row that has the page may see further into it: its block writes the same
+            for (int r = threadIdx.x; r < n_rows; r += XI_THREADS)
+                if (low[r] <= j && behind[r] > j * PE_PAGE + there && block_table[(size_t)r * table_stride + j] == page) there = min(PE_PAGE, behind[r] - j * PE_PAGE);
+            there = -__reduce_min_sync(0xffffffffu, -there);
+            __syncthreads();                                   // (the last page's have been read)
+            if (lane == 0) further[warp] = there;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < XI_THREADS / 32; ++w) there = max(there, further[w]);
+        }
         const size_t at = (size_t)page * n_kv + kvh;
         const unsigned char* block = pool + at * B::bytes;
         // the largest key that the page's steps and middles allow

@@ -2200,7 +2200,8 @@ def store_int4(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, cos: Optio
     within its bounds, and stands for mid + step * (c - 7.5): at most half a step from x, but for the roundings of step and middle.  A group whose numbers are equal is held as it is; one with an
     infinity or NaN is NaN as a whole.  Keys are turned in float64 and rounded to bfloat16 before they are coded.
 
-    Tokens of a sequence stand behind one another in the call, in the order of their positions, and no position twice; tokens whose page is not there (-1) are not stored."""
+    Tokens of a sequence stand behind one another in the call, in the order of their positions (which may leave some out), and no position twice; tokens whose page is not there (-1) are not
+    stored."""
     T, n_bytes, device = tok_pos.shape[0], _int4_heads(n_q, n_kv, head_dim), _device_here(qkv, "qkv")
     row, width = (T,), n_q * head_dim
     _here(device, (qkv, "qkv", torch.bfloat16, (T, width + 2 * n_kv * head_dim)), (tok_pos, "tok_pos", torch.int32, row), (tok_row, "tok_row", torch.int32, row),
@@ -2281,7 +2282,8 @@ def attention_int4_prompt(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_hea
                           tiles: torch.Tensor, n_tokens: int, window: Optional[int], scale: float, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The same for runs of at most 128 tokens of a sequence, ``tiles`` int32 [n, 4] (``prefill_tiles`` with ``PREFILL_TILE_TCGEN05``), whose own keys and values the cache holds already;
     ``q`` has ``n_tokens`` rows.  The pages that the runs see are expanded to 16 bits first, once a page and key head (scratch of the call, as large as one layer of a 16-bit cache: float16 keys, which
-    the queries' products need all eleven bits of, and bfloat16 values), and the products run on the tensor cores.  A page table has at most 1,024 rows.  A token that sees a key or value with a
+    the queries' products need all eleven bits of, and bfloat16 values), and the products run on the tensor cores.  A page table has at most 1,024 rows; a page that several of them
+    have stands at the same place of each.  A token that sees a key or value with a
     group that is no number has no number in the head's results."""
     n_bytes, device, width = _int4_heads(n_heads, n_kv_heads, head_dim), _device_here(q, "q"), n_heads * head_dim
     _here(device, (q, "q", torch.bfloat16, None), (tiles, "tiles", torch.int32, (tiles.shape[0], 4)), (pool, "pool", torch.uint8, (pool.shape[0], n_kv_heads, n_bytes)),

@@ -133,6 +133,22 @@ def test_pieces_leave_the_same_bytes(K, H, G, D):
     assert at == n and torch.equal(whole, pieces) and torch.equal(q, torch.cat(rows))
 
 
+@pytest.mark.parametrize("H,G,D", [(14, 2, 64), (4, 4, 128)])
+def test_positions_with_gaps(K, H, G, D):
+    """Tokens of a sequence whose positions leave some out: those of one word (positions two or one and eight apart of sixteen) stand anywhere in the call."""
+    rows = [[4, 13], [4, 5, 12, 13, 20], [0, 1, 9], [3, 10, 11, 64, 66, 73, 75], list(range(0, 60, 3)), [5], [16, 18, 25, 27, 30]] * 6
+    p = Paged(H, G, D, [80] * len(rows), 35)
+    pos, row = [x for r in rows for x in r], [b for b, r in enumerate(rows) for _ in r]
+    qkv = randn(len(pos), (H + 2 * G) * D, seed=36).bfloat16()
+    want, got = p.pool.clone(), p.pool.clone()
+    for i, (a, b) in enumerate(zip(pos, row)):
+        K.store_int4(qkv[i:i + 1], H, G, D, None, None, ints([a]), ints([b]), want, p.table, p.width)
+    for _ in range(3):
+        K.store_int4(qkv, H, G, D, None, None, ints(pos), ints(row), got, p.table, p.width)
+        assert torch.equal(got, want)
+        got.copy_(p.pool)
+
+
 def test_numbers_that_are_none_and_pages_that_are_not_there(K):
     H, G, D = 2, 2, 64
     p = Paged(H, G, D, [70, 70], 4)
@@ -473,6 +489,22 @@ def test_runs_and_pages_that_are_none_of_the_call(K):
     p.check(out[:40], list(range(130, 170)), [0] * 40, q=q[:40], table=there, halves=True)
     got = p.attention(K, [180], [0], q=q, table=table)
     p.check(got, [180], [0], q=q, table=there)
+
+
+@pytest.mark.parametrize("H,G,D", [(14, 2, 64), (28, 4, 128)])
+def test_rows_that_share_a_page_see_it_as_far_as_they_go(K, H, G, D):
+    """One sequence on the pages of several rows, each with a part of the tokens, the last page's among them: as one row has it."""
+    n, cuts = 64 * 20 + 50, [64 * 20, 64 * 20 + 1, 64 * 20 + 10, 64 * 20 + 33, 64 * 20 + 50]
+    p = Paged(H, G, D, [n], 93)
+    q = randn(n, H * D, seed=94).bfloat16()
+    whole = K.attention_int4_prompt(q, H * D, H, G, D, p.pool, p.table, p.width, K.prefill_tiles([n], [0], "cuda", K.PREFILL_TILE_TCGEN05), n, None, p.scale)
+    lens = [b - a for a, b in zip([0] + cuts, cuts)]
+    table = p.table.expand(len(lens), -1).contiguous()
+    for _ in range(5):
+        got = K.attention_int4_prompt(q, H * D, H, G, D, p.pool, table, p.width, K.prefill_tiles(lens, [0] + cuts[:-1], "cuda", K.PREFILL_TILE_TCGEN05), n, None, p.scale)
+        some = [c - 1 for c in cuts]
+        p.check(got[some], some, [0] * len(some), q=q[some], halves=True)
+        assert torch.equal(got[:64 * 20], whole[:64 * 20])
 
 
 @pytest.mark.parametrize("H,G,D", [(14, 2, 64), (4, 1, 128)])
