@@ -375,14 +375,17 @@ extern "C" int pe_page_bounds(const void* pool, long long n_pages, int n_kv, int
 // would not keep the value out of its sum).  Expanded once a page and head, for all heads and runs that read it: 7.4 MB to 24 MB of a layer for prompts of 7,541 tokens.
 // A block counts the pages of all rows from the runs, then takes every gridDim.x-th of them.
 
-#define XI_MAX_ROWS 1024
+#define XI_MAX_ROWS 16384                                     // twelve bytes each of shared memory
 #define XI_THREADS 256
 
 template <int D>
 __global__ void __launch_bounds__(XI_THREADS) expand_int4_kernel(const unsigned char* pool, int n_pages, int n_kv, const int4* tiles, int n_tiles, const int* block_table, int table_stride,
                                                                  int n_rows, int window, __half* keys, bf16* values, float* factors) {
     using B = Int4Block<D>;
-    __shared__ int low[XI_MAX_ROWS], behind[XI_MAX_ROWS], before[XI_MAX_ROWS + 1];     // a row's first page, the position behind its last run, the pages of the rows before it
+    extern __shared__ int xi_rows[];                           // a row's first page, the position behind its last run, the pages of the rows before it
+    int* const low = xi_rows;
+    int* const behind = low + n_rows;
+    int* const before = behind + n_rows;
     __shared__ float largest[XI_THREADS / 32];
     __shared__ int further[XI_THREADS / 32];
     __shared__ bool none[PE_PAGE];                             // positions whose value has a group that is no number
@@ -507,7 +510,9 @@ extern "C" int pe_expand_int4(const void* pool, long long n_pages, int n_kv, int
     if ((hd != 64 && hd != 128) || n_kv <= 0 || n_rows < 1 || n_rows > XI_MAX_ROWS || n_pages * n_kv > 0x7fffffffll) return PE_ERR_UNSUPPORTED;
     if (((uintptr_t)pool | (uintptr_t)keys | (uintptr_t)values | (uintptr_t)tiles) & 15) return PE_ERR_UNSUPPORTED;
     auto kernel = hd == 64 ? expand_int4_kernel<64> : expand_int4_kernel<128>;
-    PE_TRY(pe_launch(kernel, dim3(pe_sm_count() * 6), dim3(XI_THREADS), 0, (cudaStream_t)stream, (const unsigned char*)pool, (int)n_pages, n_kv, (const int4*)tiles, n_tiles,
+    const size_t smem = (size_t)(3 * n_rows + 1) * 4;
+    if (smem > 40 * 1024) PE_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    PE_TRY(pe_launch(kernel, dim3(pe_sm_count() * 6), dim3(XI_THREADS), smem, (cudaStream_t)stream, (const unsigned char*)pool, (int)n_pages, n_kv, (const int4*)tiles, n_tiles,
                      block_table, table_stride, n_rows, window, (__half*)keys, (bf16*)values, factors));
     PE_LAUNCH_CHECK();
     return 0;

@@ -96,6 +96,8 @@ class Engine:
         """Make the cache hold ``max_tokens`` tokens (in pages) and sequences of ``max_context``."""
         max_tokens = max(max_tokens, self._want_tokens or 0, PAGE)
         max_context = min(max(max_context, self._want_context or 0, 1), self.model.plan.max_positions)
+        if self.attend_pages is not None and max_context > 10000 * PAGE:
+            raise ValueError(f"pages are selected of contexts of at most {10000 * PAGE:,} positions, not {max_context:,}")
         max_seqs = max_seqs or max(self.max_batch, 1)
         c = self.cache
         if c is not None and c.n_pages * PAGE >= max_tokens and self.stepper.max_context >= max_context \

@@ -2260,7 +2260,8 @@ def attention_int4(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int
     stream may still run: they must have written, of the cache, no page but each token's own, and neither positions nor page tables.
 
     Scores are sums of exact products of the queries with codes, in float32; steps and middles join in float32.  Weights are rounded to bfloat16 for the product with
-    the values, and once more behind their multiplication by a value's step.  A row that sees nothing is zeros; one that sees a group that is no number is none where that reaches."""
+    the values, and once more behind their multiplication by a value's step.  Queries, keys and values of sizes between 2^-40 and 2^60 keep that: the products with codes are taken in units
+    of 2^-65.  A row that sees nothing is zeros; one that sees a group that is no number is none where that reaches."""
     T, n_bytes, device, width = tok_pos.shape[0], _int4_heads(n_heads, n_kv_heads, head_dim), _device_here(q, "q"), n_heads * head_dim
     _here(device, (q, "q", torch.bfloat16, None), (tok_pos, "tok_pos", torch.int32, (T,)), (tok_row, "tok_row", torch.int32, (T,)),
           (pool, "pool", torch.uint8, (pool.shape[0], n_kv_heads, n_bytes)), (block_table, "block_table", torch.int32, None))
@@ -2282,7 +2283,7 @@ def attention_int4_prompt(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_hea
                           tiles: torch.Tensor, n_tokens: int, window: Optional[int], scale: float, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The same for runs of at most 128 tokens of a sequence, ``tiles`` int32 [n, 4] (``prefill_tiles`` with ``PREFILL_TILE_TCGEN05``), whose own keys and values the cache holds already;
     ``q`` has ``n_tokens`` rows.  The pages that the runs see are expanded to 16 bits first, once a page and key head (scratch of the call, as large as one layer of a 16-bit cache: float16 keys, which
-    the queries' products need all eleven bits of, and bfloat16 values), and the products run on the tensor cores.  A page table has at most 1,024 rows; a page that several of them
+    the queries' products need all eleven bits of, and bfloat16 values), and the products run on the tensor cores.  A page table has at most 16,384 rows; a page that several of them
     have stands at the same place of each.  A token that sees a key or value with a
     group that is no number has no number in the head's results."""
     n_bytes, device, width = _int4_heads(n_heads, n_kv_heads, head_dim), _device_here(q, "q"), n_heads * head_dim
@@ -2292,8 +2293,8 @@ def attention_int4_prompt(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_hea
     rows = _page_rows(block_table, table_stride)
     if (window is not None and window < 0) or not scale > 0:
         raise KernelError("scale must be positive, and a window not negative")
-    if rows > 1024:
-        raise KernelError(f"prompts over a 4-bit cache take page tables of at most 1,024 rows, not {rows}")
+    if rows > 16384:
+        raise KernelError(f"prompts over a 4-bit cache take page tables of at most 16,384 rows, not {rows}")
     if out is None:
         out = q.new_empty((n_tokens, width))
     else:

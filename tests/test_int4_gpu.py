@@ -242,6 +242,19 @@ def test_scores_and_values_of_any_size(K, size):
     p.check(p.attention(K, [699], [0]), [699], [0])
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("q_up,k_up,v_up", [(-40, 40, 60), (40, -40, -40), (60, -60, 0), (0, 0, -40)])
+def test_sizes_near_the_ends(K, D, q_up, k_up, v_up):
+    """Powers of two change no code and no weight: results are the plain ones' times the values' power, bit for bit."""
+    p = Paged(4, 2, D, [700, 90], 12)
+    pos, row = [699, 89], [0, 1]
+    want = p.attention(K, pos, row)
+    p.pool = plain.pack((p.keys.double() * 2.0 ** k_up).bfloat16().view(-1, 64, D), (p.values.double() * 2.0 ** v_up).bfloat16().view(-1, 64, D)).view(p.n_pages, 2, -1)
+    p.scale *= 2.0 ** -(q_up + k_up)
+    got = p.attention(K, pos, row, q=(p.q.double() * 2.0 ** q_up).bfloat16())
+    assert torch.equal(got.double(), want.double() * 2.0 ** v_up)
+
+
 # ---------------------------------------------------------------------------- prompts
 
 @pytest.mark.parametrize("H,G,D", [(14, 2, 64), (28, 4, 128), (2, 2, 64), (20, 1, 128)])
@@ -491,6 +504,18 @@ def test_runs_and_pages_that_are_none_of_the_call(K):
     p.check(got, [180], [0], q=q, table=there)
 
 
+@pytest.mark.parametrize("H,G,D", [(4, 2, 64)])
+def test_prompts_of_many_rows(K, H, G, D):
+    lens = [1 + b % 3 for b in range(5000)]
+    p = Paged(H, G, D, [1 + b % 3 for b in range(5000)], 96)
+    n = sum(lens)
+    q = randn(n, H * D, seed=97).bfloat16()
+    got = K.attention_int4_prompt(q, H * D, H, G, D, p.pool, p.table, p.width, K.prefill_tiles(lens, [0] * 5000, "cuda", K.PREFILL_TILE_TCGEN05), n, None, p.scale)
+    pos, row = [i for c in lens for i in range(c)], [b for b, c in enumerate(lens) for _ in range(c)]
+    some = list(range(0, n, 997))
+    p.check(got[some], [pos[i] for i in some], [row[i] for i in some], q=q[some], halves=True)
+
+
 @pytest.mark.parametrize("H,G,D", [(14, 2, 64), (28, 4, 128)])
 def test_rows_that_share_a_page_see_it_as_far_as_they_go(K, H, G, D):
     """One sequence on the pages of several rows, each with a part of the tokens, the last page's among them: as one row has it."""
@@ -518,3 +543,77 @@ def test_a_prompt_behind_a_long_context(K, H, G, D, start, n, window):
     some = sorted({0, n // 2, n - 1, n, n + 33, n + 69})
     pos = [start + i if i < n else i - n for i in some]
     p.check(got[some], pos, [0 if i < n else 1 for i in some], q=q[some], window=window, halves=True)
+
+
+# ---------------------------------------------------------------------------- large caches, streams, captured calls
+
+def test_a_cache_beyond_four_gigabytes(K):
+    """Pages behind the four billionth byte (and 16-bit pages behind it, in a prompt's scratch): the same as on a small pool."""
+    H, G, D, n = 16, 8, 128, 1500
+    p = Paged(H, G, D, [n], 101)
+    far = 53000
+    pool = K.int4_pool(far + p.n_pages, G, D, "cuda")
+    assert pool.numel() > 1 << 32
+    table = torch.where(p.table >= 0, p.table + far, p.table)
+    x = randn(n, (H + 2 * G) * D, seed=102).bfloat16()
+    bounds, near = [torch.zeros(m.shape[0], G, 2, D, dtype=torch.bfloat16, device="cuda") for m in (pool, p.pool)]
+    outs = []
+    for where, places, ends in ((pool, table, bounds), (p.pool.zero_(), p.table, near)):
+        q, pos, row = append(K, p, x, [0], [n], pool=where, table=places)
+        K.page_bounds(where, G, D, ints(pos), ints(row), places, p.width, ends)
+        out = [q, *K.load_int4(where, G, D, ints(pos), ints(row), places, p.width)]
+        tiles = K.prefill_tiles([n], [0], "cuda", K.PREFILL_TILE_TCGEN05)
+        out.append(K.attention_int4_prompt(q, H * D, H, G, D, where, places, p.width, tiles, n, None, p.scale))
+        for most in (n, 1 << 21):
+            out.append(K.attention_int4(q[-40:], H * D, H, G, D, where, places, p.width, ints(pos[-40:]), ints(row[-40:]), None, p.scale, most))
+        pages = K.select_pages(q[-40:], H * D, H, G, D, ends, places, p.width, ints(pos[-40:]), ints(row[-40:]), 6, n)
+        out.append(K.attention_int4_selected(q[-40:], H * D, H, G, D, where, pages, p.scale))
+        outs.append(out)
+    assert torch.equal(pool[far:far + p.n_pages], p.pool) and torch.equal(bounds[far:far + p.n_pages], near) and not pool[:far].any()
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+
+
+def test_calls_on_two_streams_and_captured(K):
+    """Two graphs, of calls with scratch of their own, replayed at the same time, many times over: every result as the eager call's."""
+    cases = []
+    for seed, (H, G, D) in ((111, (28, 4, 128)), (112, (14, 2, 64))):
+        lengths = [3000 + 37 * b for b in range(48)]
+        p = Paged(H, G, D, lengths, seed)
+        bounds = bounds_of(p)
+        pos, row, lens = ints([n - 1 for n in lengths]), ints(list(range(48))), [150, 1, 33]
+        tiles = K.prefill_tiles(lens, [2000, 500, 2900], "cuda", K.PREFILL_TILE_TCGEN05)
+        long = randn(184, H * D, seed=seed).bfloat16()
+
+        def run(p=p, bounds=bounds, pos=pos, row=row, tiles=tiles, long=long, H=H, G=G, D=D):
+            a = K.attention_int4(p.q, p.q.shape[1], H, G, D, p.pool, p.table, p.width, pos, row, None, p.scale, 1 << 21)
+            pages = K.select_pages(p.q, p.q.shape[1], H, G, D, bounds, p.table, p.width, pos, row, 40, 5000)
+            return [a, pages.table, pages.pos, K.attention_int4_selected(p.q, p.q.shape[1], H, G, D, p.pool, pages, p.scale),
+                    K.attention_int4(p.q, p.q.shape[1], H, G, D, p.pool, p.table, p.width, pos, row, 500, p.scale, 5000),
+                    K.attention_int4_prompt(long, H * D, H, G, D, p.pool, p.table, p.width, tiles, 184, None, p.scale)]
+        cases.append((run, [x.clone() for x in run()]))
+    torch.cuda.synchronize()
+    graphs, streams = [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for run, _ in cases:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = run()
+        graphs.append((g, out))
+    for _ in range(20):
+        for out in (o for _, outs in graphs for o in outs):
+            out.zero_()
+        torch.cuda.synchronize()
+        for (g, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for (_, outs), (_, want) in zip(graphs, cases):
+            assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    for _ in range(20):
+        got = []
+        for (run, _), s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                got.append(run())
+        torch.cuda.synchronize()
+        for outs, (_, want) in zip(got, cases):
+            assert all(torch.equal(a, b) for a, b in zip(outs, want))
