@@ -5,14 +5,18 @@
 // parts and one of the negative parts against the page's two rows, 2 D multiply-adds a page whatever the number of heads.  Which pages are
 // kept is defined by the sums in float64; a bound that is no number counts as the largest.
 //
-// One kernel scores in float32, a run of pages of a token and key head a block, and leaves every page's score with a bound of its error.  A second one has a block a token and
-// head: it finds the last score that is kept by histograms of eight bits, from the first bit in which the scores differ.  Pages whose scores lie further from that one than
-// twice the largest error are decided; the others (as a rule the one page of that score) are scored in float64 and chosen by those, of equal ones the earlier page.
-// In float64 throughout, the first kernel took 28 us of 44 (48 tokens of 4 heads of 128 on 410 pages): conversions run at an eighth of the rate of multiply-adds.
+// A block a token and head scores its pages in float32, with a bound of the errors: eight or sixteen lanes a page, two batches of pages in flight.  It finds the last score that is kept by a
+// histogram of eight bits, from the first bit in which the scores differ, and a list of what that leaves.  Pages whose scores lie further from that one than twice the largest error are
+// decided; the others (as a rule the one page of that score) are scored in float64 and chosen by those, of equal ones the earlier page.
+//
+// Bound by what one SM takes in: 48 tokens of 4 heads of 128 on 410 pages (40 MB) 16.0 us, with two blocks on some SMs; one token of 2 heads of 64 on 510 pages 8.5 us, a chain of a dozen
+// waits.  With a kernel of its own that scores, a run of pages a block, 22.1 and 8.5; beyond 1,024 pages that one is used (one token on 2,046 pages 15.7 us, in one kernel 18.5).
+// A ring filled by asynchronous copies instead of registers: 20.2.  In float64 throughout: 44, since conversions run at an eighth of the rate of multiply-adds.
 #include "common.cuh"
 
 #define PS_THREADS 256
 #define PS_WARPS (PS_THREADS / 32)
+#define PS_ONE_PAGES 1024                                      // up to so many pages a block scores those that it selects from
 
 // a float64 as 64 bits that compare like it; NaN above all
 __device__ __forceinline__ unsigned long long ps_key(double v) {
@@ -43,82 +47,126 @@ struct PsScore {
     static constexpr int lanes = D / 8, at_once = 32 / lanes, ahead = 4, pages = PS_WARPS * at_once * ahead;     // lanes a page, pages a warp at a time, and how often; pages a block
 };
 
-template <int D>
-__global__ void __launch_bounds__(PS_THREADS) score_pages_kernel(const PsArgs p, float2* scores) {
-    using S = PsScore<D>;
-    __shared__ __align__(16) float sums[2][D];
-    pdl_launch_dependents();
-    pdl_wait();
-    const int kvh = blockIdx.y, tok = blockIdx.z, G = p.n_heads / p.n_kv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % S::lanes;
-    const int pages = p.pages(p.position(tok)), first = 1 + (int)blockIdx.x * S::pages;
-    if (pages <= p.keep || first >= pages - 1) return;         // (the first and the last page are kept whatever they score)
-    const int* table = p.table(tok);
-    uint4 v[S::ahead][2];
-    int place[S::ahead];                                       // of the page's score, -1: none of this warp's
-#pragma unroll
-    for (int u = 0; u < S::ahead; ++u) {
-        const int j = first + (u * PS_WARPS + warp) * S::at_once + lane / S::lanes, page = j < pages - 1 ? table[j] : -1;
-        place[u] = page >= 0 && page < p.n_pages ? j : -1;
-        const uint4* row = reinterpret_cast<const uint4*>(p.bounds + ((size_t)max(place[u] >= 0 ? page : 0, 0) * p.n_kv + kvh) * 2 * D) + l;
-        v[u][0] = row[D / 8]; v[u][1] = row[0];
-    }
-    if (threadIdx.x < D) {
-        float up = 0.f, down = 0.f;
-        const bf16* q = p.q + (size_t)tok * p.q_stride + (size_t)kvh * G * D + threadIdx.x;
+// the sums of the positive and of the negative parts of a head's queries, into shared memory (T: float or double)
+template <int D, typename T>
+__device__ __forceinline__ void ps_queries(const PsArgs& p, int tok, int kvh, T (*sums)[D]) {
+    if (threadIdx.x >= D) return;
+    const int G = p.n_heads / p.n_kv;
+    const bf16* q = p.q + (size_t)tok * p.q_stride + (size_t)kvh * G * D + threadIdx.x;
+    T up = 0, down = 0;
 #pragma unroll 8
-        for (int h = 0; h < G; ++h) {
-            const float x = __bfloat162float(q[h * D]);
-            up += x > 0.f || x != x ? x : 0.f;
-            down += x < 0.f ? x : 0.f;
-        }
-        sums[0][threadIdx.x] = up; sums[1][threadIdx.x] = down;
+    for (int h = 0; h < G; ++h) {
+        const float x = __bfloat162float(q[h * D]);
+        up += x > 0.f || x != x ? x : 0.f;
+        down += x < 0.f ? x : 0.f;
     }
-    __syncthreads();
-    float by[2][8];
+    sums[0][threadIdx.x] = up; sums[1][threadIdx.x] = down;
+}
+
+// a lane's sixteen factors, in pairs: those of eight channels of the greatest keys, then of the least
+template <int D>
+__device__ __forceinline__ void ps_factors(const float (*sums)[D], int l, unsigned long long (&by)[2][4]) {
 #pragma unroll
     for (int side = 0; side < 2; ++side)
 #pragma unroll
-        for (int e = 0; e < 8; e += 4) {
-            const float4 four = *reinterpret_cast<const float4*>(&sums[side][8 * l + e]);
-            by[side][e] = four.x; by[side][e + 1] = four.y; by[side][e + 2] = four.z; by[side][e + 3] = four.w;
+        for (int e = 0; e < 4; e += 2) {
+            const ulonglong2 four = *reinterpret_cast<const ulonglong2*>(&sums[side][8 * l + 2 * e]);
+            by[side][e] = four.x; by[side][e + 1] = four.y;
         }
-    // roundings: a head's sum, a product, the chain of a lane's sixteen and the lanes' tree: less than 24 + heads of 2^-24 of the terms' sizes; twice that
-    const float unit = (float)(32 + G) * 1.1920929e-7f;
-    float r[2 * S::ahead];                                     // scores, then their terms' sizes
+}
+
+// a lane's part of the rows of `ahead` pages
+template <int D>
+__device__ __forceinline__ void ps_load(const PsArgs& p, int kvh, int l, const int (&page)[PsScore<D>::ahead], uint4 (&v)[PsScore<D>::ahead][2]) {
+#pragma unroll
+    for (int u = 0; u < PsScore<D>::ahead; ++u) {
+        const uint4* row = reinterpret_cast<const uint4*>(p.bounds + ((size_t)max(page[u], 0) * p.n_kv + kvh) * 2 * D) + l;
+        v[u][0] = v[u][1] = make_uint4(0u, 0u, 0u, 0u);
+        if (page[u] >= 0) { v[u][0] = row[D / 8]; v[u][1] = row[0]; }
+    }
+}
+
+// The pages' scores, one a lane (l < 4): of page ps_mine(l).  `sizes` gathers the largest size of each number that the lane has met.
+__device__ __forceinline__ int ps_mine(int l) { return (l & 1) * 2 + ((l >> 1) & 1); }
+template <int D>
+__device__ __forceinline__ float ps_scores(const uint4 (&v)[PsScore<D>::ahead][2], const unsigned long long (&by)[2][4], int l, __nv_bfloat162 (&sizes)[2][4]) {
+    using S = PsScore<D>;
+    float r[S::ahead];
 #pragma unroll
     for (int u = 0; u < S::ahead; ++u) {
-        float s = 0.f, size = 0.f;
+        unsigned long long s = 0ull;                           // two float32 sums
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
             const unsigned w[4] = {v[u][side].x, v[u][side].y, v[u][side].z, v[u][side].w};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float term = by[side][e] * __uint_as_float((e & 1) ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
-                s += term;
-                size += fabsf(term);
+            for (int e = 0; e < 4; ++e) {
+                const unsigned long long x = (unsigned long long)(w[e] & 0xffff0000u) << 32 | (w[e] << 16);
+                asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(s) : "l"(x), "l"(by[side][e]));
+                sizes[side][e] = __hmax2_nan(sizes[side][e], __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[e])));
             }
         }
-        r[u] = s; r[S::ahead + u] = size;
+        r[u] = __uint_as_float((unsigned)s) + __uint_as_float((unsigned)(s >> 32));
     }
-    // eight sums over the page's lanes: each exchange halves what a lane has, until it has one
+    // four sums over the page's lanes: each exchange halves what a lane has, until it has one
 #pragma unroll
-    for (int n = S::ahead, o = 1; n; n >>= 1, o <<= 1)
+    for (int n = S::ahead / 2, o = 1; n; n >>= 1, o <<= 1)
 #pragma unroll
         for (int i = 0; i < n; ++i) {
             const float give = l & o ? r[i] : r[n + i], have = l & o ? r[n + i] : r[i];
             r[i] = have + __shfl_xor_sync(0xffffffffu, give, o);
         }
 #pragma unroll
-    for (int o = 8; o < S::lanes; o <<= 1) r[0] += __shfl_xor_sync(0xffffffffu, r[0], o);
-    // lane bits 0, 1, 2 have chosen size or score, then bits 1 and 0 of u
-    const int mine = ((l >> 1) & 1) * 2 + ((l >> 2) & 1);
+    for (int o = 4; o < S::lanes; o <<= 1) r[0] += __shfl_xor_sync(0xffffffffu, r[0], o);
+    return r[0];
+}
+
+// A bound of the scores' errors, of all pages whose numbers `sizes` has: roundings of a head's sum, a lane's chain of eight twice and the lanes' tree are less than 24 + heads of 2^-24 of
+// the terms' sizes, which are less than their sum with every number at its largest; twice that.
+template <int D>
+__device__ __forceinline__ float ps_error(const PsArgs& p, const unsigned long long (&by)[2][4], const __nv_bfloat162 (&sizes)[2][4]) {
+    float size = 0.f;
+#pragma unroll
+    for (int side = 0; side < 2; ++side)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float2 x = __bfloat1622float2(sizes[side][e]);
+            size += fabsf(__uint_as_float((unsigned)by[side][e])) * x.x + fabsf(__uint_as_float((unsigned)(by[side][e] >> 32))) * x.y;
+        }
+#pragma unroll
+    for (int o = 1; o < PsScore<D>::lanes; o <<= 1) size += __shfl_xor_sync(0xffffffffu, size, o);
+    return size * ((float)(32 + p.n_heads / p.n_kv) * 1.1920929e-7f);
+}
+
+template <int D>
+__global__ void __launch_bounds__(PS_THREADS) score_pages_kernel(const PsArgs p, float2* scores) {
+    using S = PsScore<D>;
+    __shared__ __align__(16) float sums[2][D];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int kvh = blockIdx.y, tok = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % S::lanes;
+    const int pages = p.pages(p.position(tok)), first = 1 + (int)blockIdx.x * S::pages;
+    if (pages <= p.keep || first >= pages - 1) return;         // (the first and the last page are kept whatever they score)
+    const int* table = p.table(tok);
+    uint4 v[S::ahead][2];
+    int place[S::ahead], page[S::ahead];                       // of the page's score, -1: none of this warp's
+#pragma unroll
+    for (int u = 0; u < S::ahead; ++u) {
+        const int j = first + (u * PS_WARPS + warp) * S::at_once + lane / S::lanes;
+        page[u] = j < pages - 1 ? table[j] : -1;
+        if (page[u] >= p.n_pages) page[u] = -1;
+        place[u] = page[u] >= 0 ? j : -1;
+    }
+    ps_load<D>(p, kvh, l, page, v);
+    ps_queries<D>(p, tok, kvh, sums);
+    __syncthreads();
+    unsigned long long by[2][4];
+    __nv_bfloat162 sizes[2][4] = {};
+    ps_factors<D>(sums, l, by);
+    const float r = ps_scores<D>(v, by, l, sizes), error = ps_error<D>(p, by, sizes);
     int to = place[0];
 #pragma unroll
-    for (int u = 1; u < S::ahead; ++u) to = mine == u ? place[u] : to;
-    if (l < 8 && to >= 0) {
-        float* at = reinterpret_cast<float*>(scores + ((size_t)tok * p.n_kv + kvh) * p.most + to);
-        if (l & 1) at[1] = r[0] * unit; else at[0] = r[0];
-    }
+    for (int u = 1; u < S::ahead; ++u) to = ps_mine(l) == u ? place[u] : to;
+    if (l < 4 && to >= 0) scores[((size_t)tok * p.n_kv + kvh) * p.most + to] = make_float2(r, error);
 }
 
 // The `wanted`-th largest of the keys first .. last - 1 of shared memory (a key an element, `step` words apart): keys from `least` on are kept, of those equal to it the first `equal`
@@ -169,12 +217,33 @@ __device__ __forceinline__ void ps_cut(const Key* keys, int first, int last, int
         least = prefix;
         if (told[2] == wanted) { equal = -1; return; }         // all of the bin
         if (shift == 0) { equal = wanted; return; }
+        if constexpr (bits == 32) {
+            // few are left, as a rule after the first histogram: in a list, of which each thread counts those above its own
+            const int n = told[2];
+            if (n <= PS_THREADS) {
+                __syncthreads();                               // (told has been read)
+                if (threadIdx.x == 0) told[1] = 0;
+                __syncthreads();
+                for (int j = first + threadIdx.x; j < last; j += PS_THREADS) if ((keys[j] ^ prefix) >> shift == 0) hist[atomicAdd(&told[1], 1)] = keys[j];
+                __syncthreads();
+                if (threadIdx.x < n) {
+                    const Key k = hist[threadIdx.x];
+                    int above = 0, same = 0;
+                    for (int i = 0; i < n; ++i) { above += hist[i] > k; same += hist[i] == k; }
+                    if (above < wanted && wanted <= above + same) { told[0] = (int)k; told[2] = wanted == above + same ? -1 : wanted - above; }
+                }
+                __syncthreads();
+                least = (Key)told[0]; equal = told[2];
+                return;
+            }
+        }
         top = shift;
         __syncthreads();                                       // (told and the histogram have been read)
     }
 }
 
-template <int D>
+// SCORES: the block scores its pages itself (all_scores: none)
+template <int D, bool SCORES>
 __global__ void __launch_bounds__(PS_THREADS) select_pages_kernel(const PsArgs p, const float2* all_scores, int* out_table, int* out_pos) {
     extern __shared__ unsigned long long ps_exact[];           // [most] keys of float64 scores, where some are needed; [most] keys of the scores; [most] entries of the page table; [most] pages to score again
     unsigned* keys = reinterpret_cast<unsigned*>(ps_exact + p.most);
@@ -184,6 +253,7 @@ __global__ void __launch_bounds__(PS_THREADS) select_pages_kernel(const PsArgs p
     __shared__ unsigned long long ends64[2][PS_WARPS];
     __shared__ float errors[PS_WARPS];
     __shared__ double sums[2][D];
+    __shared__ __align__(16) float sums32[2][D];
     __shared__ int n_listed;
     pdl_launch_dependents();
     pdl_wait();
@@ -191,18 +261,53 @@ __global__ void __launch_bounds__(PS_THREADS) select_pages_kernel(const PsArgs p
     const int pos = p.position(tok), pages = p.pages(pos);
     const bool choose = pages > keep && keep > 2;
     const int wanted = keep - 2;                               // besides the first and the last page
+    float error = 0.f;
     if (pages) {
         const int* table = p.table(tok);
         const float2* scores = all_scores + ((size_t)tok * n_kv + kvh) * p.most;
-        float error = 0.f;
+        if constexpr (SCORES) { if (choose) ps_queries<D>(p, tok, kvh, sums32); }
         for (int j = threadIdx.x; j < pages; j += PS_THREADS) {
             const int page = table[j];
-            entries[j] = page < p.n_pages ? page : -1;
+            const bool there = page >= 0 && page < p.n_pages;
+            entries[j] = there ? page : -1;
             if (choose && j > 0 && j < pages - 1) {
-                const bool there = page >= 0 && page < p.n_pages;
-                const float2 s = there ? scores[j] : make_float2(-INFINITY, 0.f);
-                keys[j] = there ? (s.x != s.x ? ~0u : ps_key(s.x)) : 0u;
+                if (SCORES || !there) { keys[j] = 0u; continue; }
+                const float2 s = scores[j];
+                keys[j] = s.x != s.x ? ~0u : ps_key(s.x);
                 error = ps_max(error, s.y);
+            }
+        }
+        if constexpr (SCORES) {
+            using S = PsScore<D>;
+            __syncthreads();
+            if (choose) {
+                const int l = lane % S::lanes, run = S::ahead * S::at_once;
+                unsigned long long by[2][4];
+                __nv_bfloat162 sizes[2][4] = {};
+                ps_factors<D>(sums32, l, by);
+                uint4 v[2][S::ahead][2];
+                const auto fetch = [&](int base, uint4 (&to)[S::ahead][2]) {
+                    int page[S::ahead];
+#pragma unroll
+                    for (int u = 0; u < S::ahead; ++u) { const int j = base + u * S::at_once + lane / S::lanes; page[u] = j < pages - 1 ? entries[j] : -1; }
+                    ps_load<D>(p, kvh, l, page, to);
+                };
+                const auto score = [&](int base, const uint4 (&from)[S::ahead][2]) {
+                    const float r = ps_scores<D>(from, by, l, sizes);
+                    const int j = base + ps_mine(l) * S::at_once + lane / S::lanes;
+                    if (l < 4 && j < pages - 1 && entries[j] >= 0) keys[j] = r != r ? ~0u : ps_key(r);
+                };
+                const int step = PS_WARPS * run;
+                int base = 1 + warp * run;
+                if (base < pages - 1) fetch(base, v[0]);
+                for (; base < pages - 1; base += 2 * step) {
+                    if (base + step < pages - 1) fetch(base + step, v[1]);
+                    score(base, v[0]);
+                    if (base + step >= pages - 1) break;
+                    if (base + 2 * step < pages - 1) fetch(base + 2 * step, v[0]);
+                    score(base + step, v[1]);
+                }
+                error = ps_error<D>(p, by, sizes);
             }
         }
 #pragma unroll
@@ -219,7 +324,7 @@ __global__ void __launch_bounds__(PS_THREADS) select_pages_kernel(const PsArgs p
         unsigned cut;
         int same;
         ps_cut<unsigned>(keys, 1, pages - 1, wanted, cut, same, hist, ends, told);
-        float error = 0.f;
+        error = 0.f;
 #pragma unroll
         for (int w = 0; w < PS_WARPS; ++w) error = ps_max(error, errors[w]);
         // the score of the last one kept (the least key from `cut` on)
@@ -244,30 +349,20 @@ __global__ void __launch_bounds__(PS_THREADS) select_pages_kernel(const PsArgs p
         n_over = n_near = 0;
 #pragma unroll
         for (int w = 0; w < PS_WARPS; ++w) { n_over += parts[0][w]; n_near += parts[1][w]; }
-        refine = n_over + n_near != wanted;
-        if (refine) {
-            // the pages that are near, and the queries' sums
+        if (n_over + n_near != wanted) {
+            // the pages that are near, their scores in float64
             unsigned* list = reinterpret_cast<unsigned*>(entries + p.most);
+            refine = none || n_near > PS_THREADS;
             if (threadIdx.x == 0) n_listed = 0;
-            if (threadIdx.x < D) {
-                const int G = p.n_heads / n_kv;
-                const bf16* q = p.q + (size_t)tok * p.q_stride + (size_t)kvh * G * D + threadIdx.x;
-                double up = 0.0, down = 0.0;
-#pragma unroll 8
-                for (int h = 0; h < G; ++h) {
-                    const float x = __bfloat162float(q[h * D]);
-                    up += x > 0.f || x != x ? x : 0.f;
-                    down += x < 0.f ? x : 0.f;
-                }
-                sums[0][threadIdx.x] = up; sums[1][threadIdx.x] = down;
-            }
+            ps_queries<D>(p, tok, kvh, sums);
             __syncthreads();
             for (int j = 1 + threadIdx.x; j < pages - 1; j += PS_THREADS) {
-                ps_exact[j] = keys[j] > over ? ~0ull : 0ull;   // (decided ones beside the others)
+                if (refine) ps_exact[j] = keys[j] > over ? ~0ull : 0ull;                  // (decided ones beside the others)
                 if (keys[j] >= under && keys[j] <= over && entries[j] >= 0) list[atomicAdd(&n_listed, 1)] = j;
             }
             __syncthreads();
-            for (int x = warp; x < n_listed; x += PS_WARPS) {
+            const int listed = n_listed;
+            for (int x = warp; x < listed; x += PS_WARPS) {
                 const int j = list[x];
                 const bf16* lo = p.bounds + ((size_t)entries[j] * n_kv + kvh) * 2 * D;
                 double s = 0.0;
@@ -278,10 +373,22 @@ __global__ void __launch_bounds__(PS_THREADS) select_pages_kernel(const PsArgs p
                 }
                 s = warp_sum_d(s);
                 // (below the decided ones and above the pages that are not there)
-                if (lane == 0) ps_exact[j] = min(max(ps_key(s), 1ull), ~0ull - 1);
+                if (lane == 0) ps_exact[refine ? j : x] = min(max(ps_key(s), 1ull), ~0ull - 1);
             }
             __syncthreads();
-            ps_cut<unsigned long long>(ps_exact, 1, pages - 1, wanted, least, equal, hist, ends64, told);
+            if (refine) {
+                ps_cut<unsigned long long>(ps_exact, 1, pages - 1, wanted, least, equal, hist, ends64, told);
+            } else {
+                // few: each thread counts those in front of its page
+                if (threadIdx.x < listed) {
+                    const unsigned j = list[threadIdx.x];
+                    const unsigned long long key = ps_exact[threadIdx.x];
+                    int before = n_over;
+                    for (int x = 0; x < listed; ++x) before += ps_exact[x] > key || (ps_exact[x] == key && list[x] < j);
+                    keys[j] = before < wanted ? ~0u : 0u;
+                }
+                __syncthreads();
+            }
         }
     }
     // the kept pages in the order of the positions
@@ -319,9 +426,7 @@ __global__ void __launch_bounds__(PS_THREADS) select_pages_kernel(const PsArgs p
 
 static int ps_most(int max_context, int table_stride) { const int pages = (max_context - 1) / PE_PAGE + 1; return pages < table_stride ? pages : table_stride; }
 
-// Bytes of scratch: a score and its error a page of every token and head.
-extern "C" long long pe_select_pages_scratch(int T, int n_kv, int table_stride, int max_context) { return (long long)T * n_kv * ps_most(max_context, table_stride) * 8; }
-
+// scratch: 8 bytes a page of every token and head, a score and its error, where there are more than PS_ONE_PAGES
 extern "C" int pe_select_pages(const void* q, int q_stride, int T, int n_heads, int n_kv, int hd, const void* bounds, long long n_pages, const int* block_table,
                                int table_stride, int n_rows, const int* tok_pos, const int* tok_row, int keep, int max_context, int* out_table, int* out_pos, void* scratch, void* stream) {
     if (T <= 0) return 0;
@@ -330,12 +435,13 @@ extern "C" int pe_select_pages(const void* q, int q_stride, int T, int n_heads, 
     if (((uintptr_t)bounds) & 15) return PE_ERR_UNSUPPORTED;
     const int most = ps_most(max_context, table_stride);
     const size_t smem = (size_t)most * 20;
-    if (smem > 200 * 1024 || ((uintptr_t)scratch & 7) || !scratch) return PE_ERR_UNSUPPORTED;
+    const bool one = most <= PS_ONE_PAGES;
+    if (smem > 200 * 1024 || (!one && (((uintptr_t)scratch & 7) || !scratch))) return PE_ERR_UNSUPPORTED;
     const PsArgs p = {(const bf16*)q, (const bf16*)bounds, block_table, tok_pos, tok_row, q_stride, n_heads, n_kv, (int)n_pages, table_stride, n_rows, keep, most};
     float2* scores = (float2*)scratch;
-    auto kernel = hd == 64 ? select_pages_kernel<64> : select_pages_kernel<128>;
+    auto kernel = one ? (hd == 64 ? select_pages_kernel<64, true> : select_pages_kernel<128, true>) : hd == 64 ? select_pages_kernel<64, false> : select_pages_kernel<128, false>;
     const int per = hd == 64 ? PsScore<64>::pages : PsScore<128>::pages;
-    if (most > keep && keep > 2) {                                                                    // (else every token has all of its pages)
+    if (!one && most > keep && keep > 2) {                     // (else every token has all of its pages)
         PE_TRY(pe_launch(hd == 64 ? score_pages_kernel<64> : score_pages_kernel<128>, dim3((unsigned)((most + per - 1) / per), (unsigned)n_kv, (unsigned)T),
                          dim3(PS_THREADS), 0, (cudaStream_t)stream, p, scores));
         PE_LAUNCH_CHECK();

@@ -2130,6 +2130,7 @@ def step_tables(slots: torch.Tensor, starts: torch.Tensor, lens: torch.Tensor, h
 
 INT4_HEAD_DIMS = (64, 128)
 INT4_GROUP = 32               # channels that share a step and a middle
+SELECT_ONE_PAGES = 1024       # PS_ONE_PAGES of csrc/page_select.cu
 
 
 def int4_takes(dtype: torch.dtype, n_heads: int, n_kv_heads: int, head_dim: int) -> bool:
@@ -2356,10 +2357,11 @@ def select_pages(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int, 
     n = T * n_kv_heads
     table, pos = tok_pos.new_empty((n, keep)), tok_pos.new_empty(n)
     if T:
-        scores = tok_pos.new_empty(2 * n * most)      # (the call's own: calls on two streams and captured graphs share none)
+        apart = most > SELECT_ONE_PAGES
+        scores = tok_pos.new_empty(2 * n * most) if apart else None           # (the call's own: calls on two streams and captured graphs share none)
         check(long_context().pe_select_pages(q.data_ptr(), q_stride, T, n_heads, n_kv_heads, head_dim, bounds.data_ptr(), bounds.shape[0], block_table.data_ptr(), table_stride, rows,
-                                             tok_pos.data_ptr(), tok_row.data_ptr(), keep, max_context, table.data_ptr(), pos.data_ptr(), scores.data_ptr(),
-                                             torch._C._cuda_getCurrentRawStream(device)), "select_pages", 2 if most > keep > 2 else 1)
+                                             tok_pos.data_ptr(), tok_row.data_ptr(), keep, max_context, table.data_ptr(), pos.data_ptr(), _ptr(scores),
+                                             torch._C._cuda_getCurrentRawStream(device)), "select_pages", 2 if apart and most > keep > 2 else 1)
     return SelectedPages(table, pos)
 
 

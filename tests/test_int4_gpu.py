@@ -381,6 +381,32 @@ def test_pages_that_score_alike_and_bounds_that_are_none(K):
     assert pages.table.tolist() == [ids([0, 1, 2, 20, 29], 0), ids([0, 1, 17, 20, 29], 1)]
 
 
+@pytest.mark.parametrize("n_pages", [700, 1024, 1025, 1400])
+@pytest.mark.parametrize("kind", ["close", "equal", "none"])
+def test_scores_that_differ_by_little(K, n_pages, kind):
+    """Scores closer to one another than their errors in float32, many and few of them; runs of equal ones; bounds that are no number, here and there and nearly everywhere."""
+    H, G, D = 14, 2, 64
+    p = Paged(H, G, D, [64 * n_pages - 5, 64 * 60], 53)
+    g = gen(54)
+    bounds = torch.zeros(p.n_pages, G, 2, D, dtype=torch.bfloat16, device="cuda")
+    base = torch.randn(G, 1, D, generator=g, device="cuda") * 100
+    bounds[:] = base.bfloat16()
+    if kind == "close":                                                      # one channel of one row tells them apart, by less than the others' roundings
+        bounds[:, :, :, 3] = (torch.randn(p.n_pages, G, 1, generator=g, device="cuda") * 1e-5).bfloat16()
+    elif kind == "equal":
+        bounds[:, :, 1, 9] += torch.randint(0, 3, (p.n_pages, G), generator=g, device="cuda") * 64.0
+    else:
+        few = torch.rand(p.n_pages, G, generator=g, device="cuda")
+        bounds[:, 0, 0, 5] = torch.where(few[:, 0] < 0.02, float("nan"), bounds[:, 0, 0, 5].float()).bfloat16()
+        bounds[:, 1, 1, 60] = torch.where(few[:, 1] < 0.97, float("nan"), bounds[:, 1, 1, 60].float()).bfloat16()
+    pos = [64 * n_pages - 6, 64 * 60 - 1]
+    for keep in (3, 30, 200, 650):
+        pages = K.select_pages(p.q, p.q.shape[1], H, G, D, bounds, p.table, p.width, ints(pos), ints([0, 1]), keep, 64 * n_pages)
+        for t in range(2):
+            for h, js in enumerate(chosen(p, bounds, t, pos[t], t, keep)):
+                assert pages.table[t * G + h].tolist() == [p.pages[t][j] * G + h for j in js] + [-1] * (keep - len(js)), (t, h, keep)
+
+
 def test_tokens_that_see_nothing_and_positions_behind_the_table(K):
     H, G, D = 14, 2, 64
     p = Paged(H, G, D, [64 * 9, 64 * 9, 64 * 9, 700], 52)
