@@ -779,21 +779,24 @@ struct AiStreamLaunch {
 };
 }  // namespace
 
-// Whether a call's blocks are dealt to the warps in equal runs: from 35,000 blocks on, the longest sequence's for every row (one CTA or cluster a pair / equal runs, us; 14 heads of 64 on 2: 64 rows of 20,000
-// to 32,700 72 / 65, 200 of up to 6,000 37 / 35, 32 of 4,000 to 8,192 16.6 / 22.7; 28 heads of 128 on 4: 200 of up to 6,000 94 / 86, 64 of 6,000 to 8,000 63.7 / 64.5, 16 of 8,000 to 16,000 37 / 40).
-// Selected pages are as many a row as the call says: one CTA a pair takes (16 + pages) units for each wave of as many pairs as SMs, equal runs 50 + 1.25 a block and SM (a unit is 0.23 us of 128
-// channels, 0.14 of 64).  28 heads of 128 on 4, us: 38 rows of 128 pages 65 / 48, 48 of 64 37.5 / 37.1, 64 of 64 39 / 44, 48 of 32 21 / 23.
-static bool ai_streams(int T, int n_heads, int n_kv, int hd, int max_context, int selected) {
+// Whether a call's blocks are dealt to the warps in equal runs.
+// Rows of any lengths: from 35,000 blocks on, the longest sequence's for every row (one CTA or cluster a pair / equal runs, us; 14 heads of 64 on 2: 64 rows of 20,000 to 32,700 72 / 65, 200 of
+// up to 6,000 37 / 35, 32 of 4,000 to 8,192 16.6 / 22.7; 28 heads of 128 on 4: 200 of up to 6,000 94 / 86, 64 of 6,000 to 8,000 63.7 / 64.5, 16 of 8,000 to 16,000 37 / 40).
+// Selected pages and windows are as many a row as the call says: one CTA a pair takes (16 + pages) units for each wave of as many pairs as SMs, equal runs 50 + 1.25 a block and SM (a unit is
+// 0.23 us of 128 channels, 0.14 of 64).  28 heads of 128 on 4, us: 38 rows of 128 pages 65 / 48, 48 of 64 37.5 / 37.1, 64 of 64 39 / 44, 48 of 32 21 / 23; 256 rows of 14 heads of 64 on 2 with a
+// window of 1,000 21.1 / 19.7.
+static bool ai_streams(int T, int n_heads, int n_kv, int hd, int max_context, int selected, int window) {
     const long long places = selected ? (long long)T * n_kv : T, pairs = (long long)T * n_kv * ((n_heads / n_kv + 7) / 8), pages = (max_context - 1) / PE_PAGE + 1, sms = pe_sm_count();
     if (places > AI_MAX_PLACES || pairs * pages > 0x7fffffffll) return false;
-    return selected ? pairs > sms && 4 * ((pairs + sms - 1) / sms) * (16 + pages) * sms >= 200 * sms + 5 * pairs * pages : pairs * pages >= 35000;
+    if (!selected && pairs * pages >= 35000) return true;
+    return (selected || window > 0) && pairs > sms && 4 * ((pairs + sms - 1) / sms) * (16 + pages) * sms >= 200 * sms + 5 * pairs * pages;
 }
 
 extern "C" void pe_set_pdl(int on) { pe_pdl_enabled() = on ? 1 : 0; }
 
 // Bytes of scratch that a call needs (0: none).
-extern "C" long long pe_attention_int4_scratch(int T, int n_heads, int n_kv, int hd, int max_context, int selected) {
-    if (T <= 0 || n_kv <= 0 || n_heads % n_kv || (hd != 64 && hd != 128) || !ai_streams(T, n_heads, n_kv, hd, max_context, selected)) return 0;
+extern "C" long long pe_attention_int4_scratch(int T, int n_heads, int n_kv, int hd, int max_context, int selected, int window) {
+    if (T <= 0 || n_kv <= 0 || n_heads % n_kv || (hd != 64 && hd != 128) || !ai_streams(T, n_heads, n_kv, hd, max_context, selected, window)) return 0;
     const int places = selected ? T * n_kv : T;
     return hd == 64 ? AiStreamLaunch<64>::scratch(places) : AiStreamLaunch<128>::scratch(places);
 }
@@ -811,7 +814,7 @@ extern "C" int pe_attention_int4(const void* q, int q_stride, void* out, const v
     early = early && !selected;
     const AiPlaces p = {tok_pos, tok_row, block_table, selected ? T * n_kv : T, table_stride, n_rows, (int)(selected ? n_blocks : n_blocks / n_kv), n_kv, n_heads, head_tiles, window, selected};
     const float scale_log2e = scale * 1.4426950408889634f;
-    if (scratch && ai_streams(T, n_heads, n_kv, hd, max_context, selected) && (long long)T * n_kv * head_tiles * table_stride <= 0x7fffffffll) {
+    if (scratch && ai_streams(T, n_heads, n_kv, hd, max_context, selected, window) && (long long)T * n_kv * head_tiles * table_stride <= 0x7fffffffll) {
         const auto go = [&](auto v) {
             return decltype(v)::go(p, (const bf16*)q, q_stride, (const unsigned char*)pool, scale_log2e, early, scratch, status, (bf16*)out, (cudaStream_t)stream);
         };

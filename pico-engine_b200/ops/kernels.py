@@ -2240,12 +2240,12 @@ def load_int4(pool: torch.Tensor, n_kv: int, head_dim: int, tok_pos: torch.Tenso
 
 
 @lru_cache(maxsize=4096)
-def _int4_scratch_bytes(T: int, n_heads: int, n_kv_heads: int, head_dim: int, max_context: int, selected: int) -> int:
-    return long_context().pe_attention_int4_scratch(T, n_heads, n_kv_heads, head_dim, max_context, selected)
+def _int4_scratch_bytes(T: int, n_heads: int, n_kv_heads: int, head_dim: int, max_context: int, selected: int, window: int) -> int:
+    return long_context().pe_attention_int4_scratch(T, n_heads, n_kv_heads, head_dim, max_context, selected, window)
 
 
 def _attend_int4(q, q_stride, out, pool, table, table_stride, rows, tok_pos, tok_row, T, n_heads, n_kv_heads, head_dim, window, scale, max_context, selected, early, device, name) -> None:
-    n = _int4_scratch_bytes(T, n_heads, n_kv_heads, head_dim, max_context, selected)
+    n = _int4_scratch_bytes(T, n_heads, n_kv_heads, head_dim, max_context, selected, window)
     # (what a call leaves for its second kernel to join is the call's own: calls on two streams and captured graphs share none)
     scratch = pool.new_empty(n) if n else None
     check(long_context().pe_attention_int4(q.data_ptr(), q_stride, out.data_ptr(), pool.data_ptr(), pool.shape[0] * n_kv_heads, table.data_ptr(), table_stride, rows, tok_pos.data_ptr(),
@@ -2274,6 +2274,8 @@ def attention_int4(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int
         out = q.new_empty((T, width))
     else:
         _here(device, (out, "out", torch.bfloat16, (T, width)))
+    if window:
+        max_context = min(max_context, (window + PAGE - 2) // PAGE * PAGE + PAGE)         # (positions of as many pages as a window can lie on)
     if T:
         _attend_int4(q, q_stride, out, pool, block_table, table_stride, rows, tok_pos, tok_row, T, n_heads, n_kv_heads, head_dim, window or 0, scale, max_context, 0,
                      1 if early_pages else 0, device, "attention_int4")

@@ -205,6 +205,20 @@ def test_attention_under_a_window(K, H, G, D, window):
         p.check(p.attention(K, pos, row, window=window, table=table, bound=bound), pos, row, window=window, table=table)
 
 
+@pytest.mark.parametrize("H,G,D,rows,window", [(28, 4, 128, 48, 300), (14, 2, 64, 120, 1000), (20, 1, 128, 100, 130)])
+def test_many_rows_under_a_window(K, H, G, D, rows, window):
+    """Launches for as many pages as a window can lie on, short and long rows among them."""
+    lengths = [1 + (b * 997) % 2600 for b in range(rows)]
+    p = Paged(H, G, D, lengths, 13, rubbish=float("nan"))
+    table = p.table.clone()
+    for r, n in enumerate(lengths):
+        table[r, :max(0, n - window) // PAGE] = -1
+    pos, row, q = [n - 1 for n in lengths], list(range(rows)), p.q
+    got = p.attention(K, pos, row, window=window, table=table)
+    some = list(range(0, rows, 5))
+    p.check(got[some], [pos[i] for i in some], some, q=q[some], window=window, table=table)
+
+
 def test_several_tokens_of_a_row_and_rows_in_any_order(K):
     p = Paged(14, 2, 64, [300, 90, 700], 2)
     pos, row = [0, 299, 17, 89, 650, 5, 699], [2, 0, 1, 1, 2, 0, 2]
