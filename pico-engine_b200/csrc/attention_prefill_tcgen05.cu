@@ -68,15 +68,17 @@ struct AtArgs {
     const float* slopes; float inv_scale;          // [nh] or null: slopes[h] * (query position - key position) is taken off the scaled score
     int pool_rows;                                 // rows of the key (and value) pool seen as a matrix [rows][head size]
     const float* sinks;                            // [nh] or null: one more place of this (scaled) score joins a row's denominator and carries no value
-    const float* factors;                          // of float16 keys: [pages][nkv], what the scores of a page's keys are multiplied by
-    int n_rows, n_tokens, pool_pages;              // of float16 keys: what runs and page tables may name
-    int splits; float* partial;                    // of float16 keys: CTAs that may share a run and head's steps, and where each leaves its rows' sums
+    const float2* factors;                         // HALF: [pages][nkv], what the scores of a page's keys are multiplied by, and f: its values lie 2^(14 - f) higher
+    int n_rows, n_tokens, pool_pages;              // HALF: what runs and page tables may name
+    int splits; float* partial;                    // HALF: CTAs that may share a run and head's steps, and where each leaves its rows' sums
 };
 
 // How many CTAs share the steps of a run (a few steps each at least), and the first step of one of them.
 #define AT_LEAST_STEPS 4
 __device__ __forceinline__ int at_shares(int steps, int splits) { return min(splits, max(1, steps / AT_LEAST_STEPS)); }
 __device__ __forceinline__ int at_share(int z, int steps, int shares) { return z * steps / shares; }
+#define AT_HALF_UP 6                               // HALF: weights lie 2^6 higher
+#define AT_HALF_DOWN (1.f / (float)(1 << (AT_HALF_UP + 14)))   // what a row's sums are multiplied by at its end
 #define AT_PARTIAL_ROW (AT_HD + 4)                 // of a row: its columns' sums, reference point, sum of weights
 
 // 64 columns of a row of queries, in place: bfloat16 to float16, times `up`
@@ -95,11 +97,13 @@ __device__ __forceinline__ void at_to_half(unsigned row, int r, int groups, int 
 }
 
 // tiles[i] = (batch row, first packed token, number of tokens (<= AT_QTILE), position of the first token)
-// HALF_KEYS: the keys are float16, times a power of two of their page and head (expanded from a cache of fewer bits, whose products with queries bfloat16 keys would be off by more than
-// all else).  The softmax warps then take the queries to float16 before the first product, each row times a power of two of its own, and scores are multiplied back in
-// the exponent's multiply-add, which costs nothing.  SHARED (of those): several CTAs share a run and head's steps (blockIdx.z) and leave the rows' sums to a second kernel; a variant of
+// HALF: keys and values are float16, times powers of two of their page and head (expanded from a cache of fewer bits, of which bfloat16 would lose more than the cache's reader does: with bfloat16
+// keys results are off by 0.0055 of their size, with bfloat16 values and weights by 0.0029, the results' own rounding, 0.0017, among it).  The softmax warps then take the queries to float16 before the
+// first product, each row times a power of two of its own, and scores are multiplied back in the exponent's multiply-add.  A value's power 2^f joins its weights' exponents there, so that
+// the reference point is the largest of score + f; a page's sum of weights is taken back by 2^-f.  Weights are 2^6 higher, at most 2^14, so float16 keeps those down to 2^-20
+// of the reference point in full.  SHARED (of those): several CTAs share a run and head's steps (blockIdx.z) and leave the rows' sums to a second kernel; a variant of
 // its own, since what it keeps in registers is spilled in the loop (7,541 tokens, 28 heads of 128: 274 us without, 304 with it).
-template <bool HALF_KEYS, bool SHARED>
+template <bool HALF, bool SHARED>
 __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q,
                                                                                   const __grid_constant__ CUtensorMap map_k,
                                                                                   const __grid_constant__ CUtensorMap map_v,
@@ -134,13 +138,13 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
     const int first_key = (p.window > 0 && pos0 - p.window + 1 > 0) ? pos0 - p.window + 1 : 0;
     // (with kept first keys: their pages first, then the window's; where the two meet, all pages from the sequence's start)
     int page_lo = first_key / AT_KTILE, kept = 0;
-    const int page_hi = HALF_KEYS ? min((pos0 + n - 1) / AT_KTILE, p.table_stride - 1) : (pos0 + n - 1) / AT_KTILE;
+    const int page_hi = HALF ? min((pos0 + n - 1) / AT_KTILE, p.table_stride - 1) : (pos0 + n - 1) / AT_KTILE;
     if (p.window > 0 && p.keep_first > 0) {
         const int keep_pages = (p.keep_first + AT_KTILE - 1) / AT_KTILE;
         if (page_lo <= keep_pages) page_lo = 0; else kept = keep_pages;
     }
     int n_pages = kept + page_hi - page_lo + 1, n_steps = (n_pages + 1) / 2, shares = 1;
-    if constexpr (HALF_KEYS) {
+    if constexpr (HALF) {
         if (brow < 0 || brow >= p.n_rows || n <= 0 || n > AT_QTILE || pos0 < 0 || tok0 < 0 || tok0 + n > p.n_tokens || n_pages <= 0) return;      // (no run of this call)
         if constexpr (SHARED) {                                     // this CTA's share of the steps
             shares = at_shares(n_steps, p.splits);
@@ -216,12 +220,12 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
             const unsigned elected = pe_elect();
             // instruction descriptors: float32 accumulator, bfloat16 operands, M = 128;
             // S: A and B K-major, N = 128 keys;  O: B MN-major (bit 16), N = head size
-            const unsigned idesc_s = (1u << 4) | (HALF_KEYS ? 0u : (1u << 7) | (1u << 10)) | ((unsigned)((2 * AT_KTILE) >> 3) << 17) | ((unsigned)(AT_QTILE >> 4) << 24);
-            const unsigned idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((unsigned)(AT_HD >> 3) << 17) | ((unsigned)(AT_QTILE >> 4) << 24);
+            const unsigned idesc_s = (1u << 4) | (HALF ? 0u : (1u << 7) | (1u << 10)) | ((unsigned)((2 * AT_KTILE) >> 3) << 17) | ((unsigned)(AT_QTILE >> 4) << 24);
+            const unsigned idesc_o = (1u << 4) | (HALF ? 0u : (1u << 7) | (1u << 10)) | (1u << 16) | ((unsigned)(AT_HD >> 3) << 17) | ((unsigned)(AT_QTILE >> 4) << 24);
             // operand descriptors of stage 0; a stage further on adds its offset in 16-byte units
             const unsigned long long dq = at_desc(q_s, 0, 1024), dk = at_desc(kv_s, 0, 1024);
             const unsigned long long dv = at_desc(kv_s + AT_STAGE_BYTES / 2, 2 * AT_KTILE * 128, 1024);
-            bool ok = at_wait_warp(at_smem(HALF_KEYS ? q_half : &q_full), 0u);
+            bool ok = at_wait_warp(at_smem(HALF ? q_half : &q_full), 0u);
             auto issue_s = [&](int it) -> bool {                    // S = Q . K^T of step `it`, when P.V has read the P that lay in its buffer
                 const int s = it % AT_STAGES, b = it % AT_BUFFERS;
                 if (it >= AT_BUFFERS && !at_wait_warp(at_smem(&pv_done[b]), (unsigned)(it / AT_BUFFERS - 1) & 1u)) return false;
@@ -260,10 +264,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
         const int r = quarter * 32 + lane;                          // this thread's query row
         const int p_r = pos0 + r;
         const unsigned lane_addr = tmem + ((unsigned)(quarter * 32) << 16);
-        const float slope = p.slopes ? p.slopes[h] * p.inv_scale : 0.f;     // in units of the unscaled score
+        const float slope = !HALF && p.slopes ? p.slopes[h] * p.inv_scale : 0.f;     // in units of the unscaled score
         float row_scale = p.scale_log2e;
         bool ok = true;
-        if constexpr (HALF_KEYS) {
+        if constexpr (HALF) {
             // half a row of queries a thread: its largest, then the row's (through the other half's thread), then float16
             ok = at_wait_warp(at_smem(&q_full), 0u);
             constexpr int groups = AT_HD / 16;
@@ -296,16 +300,17 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
         for (int it = g; it < n_steps && ok; it += 2) {
             const int b = it % AT_BUFFERS;
             const unsigned s_addr = lane_addr + b * (2 * AT_KTILE);
-            const bool there[2] = {entry[0] >= 0 && (!HALF_KEYS || entry[0] < p.pool_pages), entry[1] >= 0 && (!HALF_KEYS || entry[1] < p.pool_pages)};   // (a page that is not there was read as zeros and is masked)
-            float page_scale[2] = {1.f, 1.f};                       // of float16 keys: what takes the page's scores to powers of two
-            if constexpr (HALF_KEYS) {
+            const bool there[2] = {entry[0] >= 0 && (!HALF || entry[0] < p.pool_pages), entry[1] >= 0 && (!HALF || entry[1] < p.pool_pages)};   // (a page that is not there was read as zeros and is masked)
+            float2 page_scale[2] = {make_float2(1.f, 0.f), make_float2(1.f, 0.f)};      // HALF: what takes the page's scores to powers of two, and f
+            if constexpr (HALF) {
 #pragma unroll
-                for (int x = 0; x < 2; ++x) page_scale[x] = there[x] ? row_scale * p.factors[entry[x] * p.nkv + kvh] : 1.f;
+                for (int x = 0; x < 2; ++x)
+                    if (there[x]) { page_scale[x] = p.factors[entry[x] * p.nkv + kvh]; page_scale[x].x *= row_scale; }
             }
 #pragma unroll
             for (int x = 0; x < 2; ++x) entry[x] = 2 * it + 4 + x < n_pages ? table[page_at(2 * it + 4 + x)] : -1;
             if (!at_wait_warp(at_smem(&s_full[b]), (unsigned)(it / AT_BUFFERS) & 1u)) { ok = false; break; }
-            if (!HALF_KEYS && it + 1 == n_steps && (pos0 + n) % AT_KTILE) {       // (expanded pages have zeros there) values behind the run's last token, in the second or the first of the step's pages
+            if (!HALF && it + 1 == n_steps && (pos0 + n) % AT_KTILE) {       // (expanded pages have zeros there) values behind the run's last token, in the second or the first of the step's pages
                 if (!at_wait_warp(at_smem(&v_full[it % AT_STAGES]), (unsigned)(it / AT_STAGES) & 1u)) { ok = false; break; }
                 at_clear_rows(kv_s + it % AT_STAGES * AT_STAGE_BYTES + AT_STAGE_BYTES / 2, AT_PANELS, 2 * AT_KTILE * 128,
                               (n_pages - 1 - 2 * it) * AT_KTILE + (pos0 + n) % AT_KTILE, (threadIdx.x - 64) & 127, 128);
@@ -336,7 +341,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
                 }
                 // the distance's share of the score, slope * (key - row): the part that grows along the page is added here, the
                 // page's own part (`base`, one number a page) joins the maximum and the exponent's offset
-                if (p.slopes) {
+                if (!HALF && p.slopes) {
                     base[x] = slope * (float)(key0 - p_r);
 #pragma unroll
                     for (int c = 0; c < AT_KTILE; ++c) sx[c] = fmaf(slope, (float)c, sx[c]);
@@ -362,7 +367,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
             // The reference point of the exponentials follows the row's maximum only when that has grown by more than
             // AT_LAZY (in powers of two): P then holds values up to 2^AT_LAZY, which bfloat16 and the float32 sums take
             // as well as values up to 1, and O is rescaled on few steps instead of on nearly all.
-            const float m_tile = HALF_KEYS ? fmaxf(m_first * page_scale[0], m_second * page_scale[1]) : fmaxf(m_first, m_second) * p.scale_log2e;
+            const float m_tile = HALF ? fmaxf(fmaf(m_first, page_scale[0].x, page_scale[0].y), fmaf(m_second, page_scale[1].x, page_scale[1].y)) : fmaxf(m_first, m_second) * p.scale_log2e;
             const float m_new = (m_run != -INFINITY && m_tile <= m_run + AT_LAZY) ? m_run : fmaxf(m_run, m_tile);
             refs[g * AT_QTILE + r] = m_new;
             __syncwarp();
@@ -375,13 +380,17 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 float packed[AT_KTILE / 2];
-                const unsigned long long scale_x = HALF_KEYS ? at_two(page_scale[x], page_scale[x]) : scale2;
-                const float off = fmaf(base[x], p.scale_log2e, -m_use);
+                const unsigned long long scale_x = HALF ? at_two(page_scale[x].x, page_scale[x].x) : scale2;
+                const float off = HALF ? page_scale[x].y - m_use + AT_HALF_UP : fmaf(base[x], p.scale_log2e, -m_use);
 #pragma unroll
-                for (int c = 0; c < AT_KTILE; c += 2) packed[c >> 1] = __uint_as_float(at_exp2_pair(s[x * AT_KTILE + c], s[x * AT_KTILE + c + 1], scale_x, at_two(off, off), sum[(c >> 1) & 1]));
+                for (int c = 0; c < AT_KTILE; c += 2) packed[c >> 1] = __uint_as_float(at_exp2_pair<HALF>(s[x * AT_KTILE + c], s[x * AT_KTILE + c + 1], scale_x, at_two(off, off), sum[(c >> 1) & 1]));
                 at_st32(s_addr + x * (AT_KTILE / 2), packed);       // P over the scores, two keys a column
+                if constexpr (HALF) {
+                    l_mine = fmaf(at_sum_four(sum[0], sum[1]), __uint_as_float((unsigned)(127 - AT_HALF_UP - (int)page_scale[x].y) << 23), l_mine);
+                    sum[0] = sum[1] = 0ull;
+                }
             }
-            l_mine += at_sum_four(sum[0], sum[1]);
+            if constexpr (!HALF) l_mine += at_sum_four(sum[0], sum[1]);
             if (it > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) { // a row's reference point moved: rescale the warp's rows of O
                 if (!at_wait_warp(at_smem(&pv_done[(it - 1) % AT_BUFFERS]), (unsigned)((it - 1) / AT_BUFFERS) & 1u)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -418,7 +427,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
                 const float m = refs[w * AT_QTILE + r];
                 if (m != -INFINITY) l = fmaf(sums[w * AT_QTILE + r], at_exp2(m - m_run), l);
             }
-            if (p.sinks) l += at_exp2(fmaf(p.sinks[h], 1.4426950408889634f, -m_run));   // (a row that saw no key: 2^inf, and 1 / l = 0)
+            if (!HALF && p.sinks) l += at_exp2(fmaf(p.sinks[h], 1.4426950408889634f, -m_run));   // (a row that saw no key: 2^inf, and 1 / l = 0)
             if constexpr (SHARED) {
                 if (shares > 1) {                                   // a share of the row's sums, for the kernel that joins them
                     float* to = p.partial + (((size_t)(blockIdx.y * p.nh + h) * p.splits + blockIdx.z) * AT_QTILE + r) * AT_PARTIAL_ROW;
@@ -433,7 +442,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
                     }
                 }
             }
-            const float inv = l > 0.f ? 1.0f / l : 0.f;
+            const float inv = l > 0.f ? (HALF ? AT_HALF_DOWN : 1.0f) / l : 0.f;
             if (!SHARED || shares == 1) {
                 // through the queries' place: the last products have read them
                 const unsigned o_addr = lane_addr + AT_O_COL + g * (AT_HD / 2);
@@ -484,7 +493,7 @@ __global__ void __launch_bounds__(256) attention_prefill_join_kernel(const AtArg
 #pragma unroll
             for (int c = 0; c < COLS; ++c) o[c] = fmaf(row[lane * COLS + c], w, o[c]);
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float inv = l == 0.f ? 0.f : AT_HALF_DOWN / l;
         bf16* to = p.out + ((size_t)(tok0 + r) * p.nh + h) * AT_HD + lane * COLS;
 #pragma unroll
         for (int c = 0; c < COLS; c += 2) *reinterpret_cast<unsigned*>(to + c) = at_pack(o[c] * inv, o[c + 1] * inv);
@@ -502,10 +511,10 @@ extern "C" int pe_attention_prefill_tcgen05_ctas_per_sm() {
 }
 
 // q: [n_tokens][q_stride] with head h at columns h * hd; pools: [pool_pages][nkv][64][hd]
-template <bool HALF_KEYS, bool SHARED>
+template <bool HALF, bool SHARED>
 static int at_launch(const void* q, int q_stride, void* out, const void* k_pool, const void* v_pool, long long pool_pages, const int* block_table, int table_stride, const void* tiles,
                      int n_tiles, int n_tokens, int nh, int nkv, int hd, int window, float scale, int keep_first, const float* slopes, int* status, void* stream, const float* sinks,
-                     const float* factors, int splits, float* partial, int n_rows) {
+                     const float2* factors, int splits, float* partial, int n_rows) {
     if (n_tiles <= 0) return 0;
     if (hd != AT_HD || nkv <= 0 || nh % nkv || n_tiles > 65535 || q_stride % 8 || !(scale > 0.f) || !status) return PE_ERR_UNSUPPORTED;
     if (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)out | (uintptr_t)tiles) & 15) return PE_ERR_UNSUPPORTED;
@@ -513,7 +522,7 @@ static int at_launch(const void* q, int q_stride, void* out, const void* k_pool,
     CUtensorMap mq, mk, mv;
     int rc = at_make_map(&mq, q, n_tokens, (long long)nh * hd, q_stride, AT_QTILE);
     if (rc) return rc;
-    rc = at_make_map(&mk, k_pool, pool_pages * nkv * AT_KTILE, hd, hd, AT_KTILE);     // (float16 keys are 16-bit numbers like any others to a copy)
+    rc = at_make_map(&mk, k_pool, pool_pages * nkv * AT_KTILE, hd, hd, AT_KTILE);     // (float16 numbers are 16-bit numbers like any others to a copy)
     if (rc) return rc;
     rc = at_make_map(&mv, v_pool, pool_pages * nkv * AT_KTILE, hd, hd, AT_KTILE);
     if (rc) return rc;
@@ -525,18 +534,20 @@ static int at_launch(const void* q, int q_stride, void* out, const void* k_pool,
     p.n_rows = n_rows; p.n_tokens = n_tokens; p.pool_pages = (int)pool_pages;
     p.sinks = sinks; p.factors = factors; p.splits = splits; p.partial = partial;
     const size_t smem = AT_SMEM_BYTES;
-    static bool attr_set = false;
-    if (!attr_set) {
-        PE_TRY(cudaFuncSetAttribute(attention_prefill_tcgen05_kernel<HALF_KEYS, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        attr_set = true;
+    static bool attr_set[64] = {};                                  // (per device)
+    int dev = 0;
+    PE_TRY(cudaGetDevice(&dev));
+    if (dev >= 64 || !attr_set[dev]) {
+        PE_TRY(cudaFuncSetAttribute(attention_prefill_tcgen05_kernel<HALF, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        if (dev < 64) attr_set[dev] = true;
     }
-    PE_TRY(pe_launch(attention_prefill_tcgen05_kernel<HALF_KEYS, SHARED>, dim3(nh, n_tiles, splits), AT_THREADS, smem, (cudaStream_t)stream, mq, mk, mv, p, status));
+    PE_TRY(pe_launch(attention_prefill_tcgen05_kernel<HALF, SHARED>, dim3(nh, n_tiles, splits), AT_THREADS, smem, (cudaStream_t)stream, mq, mk, mv, p, status));
     if (splits > 1) PE_TRY(pe_launch(attention_prefill_join_kernel, dim3(nh, n_tiles, 4), 256, 0, (cudaStream_t)stream, p));
     return 0;
 }
 
 // Into how many shares the steps of a run and head are cut, where all runs and heads together are fewer than the SMs: the number whose last wave ends first, a step taken for
-// 1 and the rest of a CTA for 5 (0.93 us and 4.3).  500 tokens on 15,937 positions, 14 heads of 64: 56 CTAs of 128 steps, 130 us in one share, AT_MEASURED in five.
+// 1 and the rest of a CTA for 5 (0.93 us and 4.3).  500 tokens on 15,937 positions, 14 heads of 64: 56 CTAs of 128 steps, 130 us in one share, 80 us in five.
 static int at_splits(long long ctas, int table_stride) {
     const int steps = (table_stride + 1) / 2, sms = pe_sm_count();
     int best = 1;
@@ -557,20 +568,20 @@ extern "C" int pe_attention_prefill_tcgen05(const void* q, int q_stride, void* o
 }
 
 // Bytes of scratch that the next one needs (0: none).
-extern "C" long long pe_attention_prefill_half_keys_scratch(int n_tiles, int nh, int table_stride) {
+extern "C" long long pe_attention_prefill_half_scratch(int n_tiles, int nh, int table_stride) {
     const long long ctas = (long long)n_tiles * nh;
     const int s = ctas > 0 ? at_splits(ctas, table_stride) : 1;
     return s > 1 ? ctas * s * AT_QTILE * AT_PARTIAL_ROW * 4 : 0;
 }
 
-// The same over float16 keys, the scores of a page's keys times factors[page][kv head].
-extern "C" int pe_attention_prefill_half_keys(const void* q, int q_stride, void* out, const void* k_pool, const void* v_pool, const float* factors, long long pool_pages,
+// The same over float16 keys and values with their pages' powers of two, factors[page][kv head].
+extern "C" int pe_attention_prefill_half(const void* q, int q_stride, void* out, const void* k_pool, const void* v_pool, const void* factors, long long pool_pages,
                                               const int* block_table, int table_stride, int n_rows, const void* tiles, int n_tiles, int n_tokens, int nh, int nkv, int hd, int window,
                                               float scale, void* scratch, int* status, void* stream) {
-    if (!factors || ((uintptr_t)scratch & 15)) return PE_ERR_UNSUPPORTED;
+    if (!factors || ((uintptr_t)factors & 7) || ((uintptr_t)scratch & 15)) return PE_ERR_UNSUPPORTED;
     const int splits = scratch ? at_splits((long long)n_tiles * nh, table_stride) : 1;
     return (splits > 1 ? at_launch<true, true> : at_launch<true, false>)(q, q_stride, out, k_pool, v_pool, pool_pages, block_table, table_stride, tiles, n_tiles, n_tokens, nh, nkv, hd, window,
-                                                                         scale, 0, nullptr, status, stream, nullptr, factors, splits, (float*)scratch, n_rows);
+                                                                         scale, 0, nullptr, status, stream, nullptr, (const float2*)factors, splits, (float*)scratch, n_rows);
 }
 
 #else   // other head sizes: the mma.sync kernel of attention_prefill.cu takes them
@@ -581,8 +592,8 @@ extern "C" int pe_attention_prefill_tcgen05(const void*, int, void*, const void*
                                             int, int, int, int, int, int, float, int, const float*, int*, void*, const float*) {
     return PE_ERR_UNSUPPORTED;
 }
-extern "C" long long pe_attention_prefill_half_keys_scratch(int, int, int) { return 0; }
-extern "C" int pe_attention_prefill_half_keys(const void*, int, void*, const void*, const void*, const float*, long long, const int*, int, int, const void*, int, int, int, int, int, int,
+extern "C" long long pe_attention_prefill_half_scratch(int, int, int) { return 0; }
+extern "C" int pe_attention_prefill_half(const void*, int, void*, const void*, const void*, const void*, long long, const int*, int, int, const void*, int, int, int, int, int, int,
                                               float, void*, int*, void*) {
     return PE_ERR_UNSUPPORTED;
 }

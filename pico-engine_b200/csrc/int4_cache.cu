@@ -369,10 +369,11 @@ extern "C" int pe_page_bounds(const void* pool, long long n_pages, int n_kv, int
 }
 
 // ---------------------------------------------------------------------------- pages in 16 bits, for prompts
-// What the runs of a prompt read of a 4-bit cache, as operands of tcgen05.mma: values as bfloat16, keys as float16 times a power of two of their page and head (`factors` takes it
-// back), so that a key keeps 11 bits whatever its size: with keys of 8 bits the scores' errors are what the results are off by (0.0055 of their size; 0.0024 so).  Positions behind a
-// row's last run are zeros.  A value with a group that is no number is zeros, and its key is none: a query that sees it has no result then, and one that does not keeps its own (a weight of zero
-// would not keep the value out of its sum).  Expanded once a page and head, for all heads and runs that read it: 7.4 MB to 24 MB of a layer for prompts of 7,541 tokens.
+// What the runs of a prompt read of a 4-bit cache, as operands of tcgen05.mma: keys and values as float16 times powers of two of their page and head (`factors`: what takes a key back, and the
+// exponent f of values 2^(14 - f) higher), so that a number keeps 11 bits whatever its size.  Positions behind a row's last run are zeros.  A value with a group that is no number is zeros, and
+// its key is none: a query that sees it has no result then, and one that does not keeps its own (a weight of zero
+// would not keep the value out of its sum).  Expanded once a page and head, for all heads and runs that read it.
+// Bound by its writes: 7,541 tokens of 4 heads of 128 (and the 4,071 in front of a run of theirs) 9 MB read and 24 MB written, 10 to 11 us.
 // A block counts the pages of all rows from the runs, then takes every gridDim.x-th of them.
 
 #define XI_MAX_ROWS 16384                                     // twelve bytes each of shared memory
@@ -380,13 +381,13 @@ extern "C" int pe_page_bounds(const void* pool, long long n_pages, int n_kv, int
 
 template <int D>
 __global__ void __launch_bounds__(XI_THREADS) expand_int4_kernel(const unsigned char* pool, int n_pages, int n_kv, const int4* tiles, int n_tiles, const int* block_table, int table_stride,
-                                                                 int n_rows, int window, __half* keys, bf16* values, float* factors) {
+                                                                 int n_rows, int window, __half* keys, __half* values, float2* factors) {
     using B = Int4Block<D>;
     extern __shared__ int xi_rows[];                           // a row's first page, the position behind its last run, the pages of the rows before it
     int* const low = xi_rows;
     int* const behind = low + n_rows;
     int* const before = behind + n_rows;
-    __shared__ float largest[XI_THREADS / 32];
+    __shared__ float2 largest[XI_THREADS / 32];
     __shared__ int further[XI_THREADS / 32];
     __shared__ bool none[PE_PAGE];                             // positions whose value has a group that is no number
     pdl_launch_dependents();
@@ -435,13 +436,17 @@ __global__ void __launch_bounds__(XI_THREADS) expand_int4_kernel(const unsigned 
         }
         const size_t at = (size_t)page * n_kv + kvh;
         const unsigned char* block = pool + at * B::bytes;
-        // the largest key that the page's steps and middles allow
-        float most = 0.f;
+        // the largest key and value that the page's steps and middles allow
+        float most = 0.f, most_v = 0.f;
         for (int i = threadIdx.x; i < there * B::groups; i += XI_THREADS) {
-            const bf16* meta = reinterpret_cast<const bf16*>(block + q4_key_step<D>(i / B::groups, i % B::groups));
+            const int q = i / B::groups, g = i % B::groups;
+            const bf16* meta = reinterpret_cast<const bf16*>(block + q4_key_step<D>(q, g));
+            const bf16* vmeta = reinterpret_cast<const bf16*>(block + q4_value_step<D>(q, g));
             most = fmaxf(most, fmaf(7.5f, fabsf(to_f(meta[0])), fabsf(to_f(meta[B::groups]))));
+            most_v = fmaxf(most_v, fmaf(7.5f, fabsf(to_f(vmeta[0])), fabsf(to_f(vmeta[B::groups * 16]))));
         }
         most = warp_max(most);
+        most_v = warp_max(most_v);
         __syncthreads();                                       // (the last page's maxima and marks have been read)
         if (threadIdx.x < PE_PAGE) {
             bool any = false;
@@ -449,16 +454,18 @@ __global__ void __launch_bounds__(XI_THREADS) expand_int4_kernel(const unsigned 
             for (int b = 0; b < B::groups; ++b) { const float m = to_f(*reinterpret_cast<const bf16*>(block + q4_value_step<D>(threadIdx.x, b))); any |= m != m; }
             none[threadIdx.x] = any && threadIdx.x < there;
         }
-        if (lane == 0) largest[warp] = most;
+        if (lane == 0) largest[warp] = make_float2(most, most_v);
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < XI_THREADS / 32; ++w) most = fmaxf(most, largest[w]);
-        int exponent = 0;
+        for (int w = 0; w < XI_THREADS / 32; ++w) { most = fmaxf(most, largest[w].x); most_v = fmaxf(most_v, largest[w].y); }
+        int exponent = 0, f = 0;
         if (most > 0.f) frexpf(fminf(most, 3.0e38f), &exponent);                          // most <= 2^exponent
-        const float up = ldexpf(1.f, 14 - max(exponent, -30));
-        if (threadIdx.x == 0) factors[at] = 1.f / up;
+        if (most_v > 0.f) frexpf(fminf(most_v, 3.0e38f), &f);
+        f = min(max(f, -30), 115);                             // (2^-f and 2^-f times the weights' power are normal numbers)
+        const float up = ldexpf(1.f, 14 - max(exponent, -30)), up_v = ldexpf(1.f, 14 - f);
+        if (threadIdx.x == 0) factors[at] = make_float2(1.f / up, (float)f);
         __half* ko = keys + at * PE_PAGE * D;
-        bf16* vo = values + at * PE_PAGE * D;
+        __half* vo = values + at * PE_PAGE * D;
 #pragma unroll
         for (int i = threadIdx.x; i < PE_PAGE * B::key_words; i += XI_THREADS) {
             const int p = i / B::key_words, rest = i % B::key_words, t = rest / B::groups, b = rest % B::groups;
@@ -490,11 +497,11 @@ __global__ void __launch_bounds__(XI_THREADS) expand_int4_kernel(const unsigned 
                         uint2 v = make_uint2(0u, 0u);
                         if (p < there && !none[p]) {
                             const bf16* meta = reinterpret_cast<const bf16*>(block + q4_value_step<D>(p, 2 * h + b));
-                            const float s = to_f(meta[0]), m = to_f(meta[B::groups * 16]);
-                            __nv_bfloat162 two[2];
+                            const float s = to_f(meta[0]) * up_v, m = to_f(meta[B::groups * 16]) * up_v;
+                            __half2 two[2];
 #pragma unroll
                             for (int w = 0; w < 2; ++w)
-                                two[w] = __floats2bfloat162_rn(fmaf(s, q4_level(words[2 * b + w], 2 * f, e), m), fmaf(s, q4_level(words[2 * b + w], 2 * f + 1, e), m));
+                                two[w] = __floats2half2_rn(fmaf(s, q4_level(words[2 * b + w], 2 * f, e), m), fmaf(s, q4_level(words[2 * b + w], 2 * f + 1, e), m));
                             v = *reinterpret_cast<uint2*>(two);
                         }
                         *reinterpret_cast<uint2*>(vo + p * D + 32 * (2 * h + b) + 4 * g) = v;
@@ -505,15 +512,15 @@ __global__ void __launch_bounds__(XI_THREADS) expand_int4_kernel(const unsigned 
 }
 
 extern "C" int pe_expand_int4(const void* pool, long long n_pages, int n_kv, int hd, const int* tiles, int n_tiles, const int* block_table, int table_stride, int n_rows, int window,
-                              void* keys, void* values, float* factors, void* stream) {
+                              void* keys, void* values, void* factors, void* stream) {
     if (n_tiles <= 0) return 0;
     if ((hd != 64 && hd != 128) || n_kv <= 0 || n_rows < 1 || n_rows > XI_MAX_ROWS || n_pages * n_kv > 0x7fffffffll) return PE_ERR_UNSUPPORTED;
-    if (((uintptr_t)pool | (uintptr_t)keys | (uintptr_t)values | (uintptr_t)tiles) & 15) return PE_ERR_UNSUPPORTED;
+    if (((uintptr_t)pool | (uintptr_t)keys | (uintptr_t)values | (uintptr_t)tiles) & 15 || ((uintptr_t)factors & 7)) return PE_ERR_UNSUPPORTED;
     auto kernel = hd == 64 ? expand_int4_kernel<64> : expand_int4_kernel<128>;
     const size_t smem = (size_t)(3 * n_rows + 1) * 4;
     if (smem > 40 * 1024) PE_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     PE_TRY(pe_launch(kernel, dim3(pe_sm_count() * 6), dim3(XI_THREADS), smem, (cudaStream_t)stream, (const unsigned char*)pool, (int)n_pages, n_kv, (const int4*)tiles, n_tiles,
-                     block_table, table_stride, n_rows, window, (__half*)keys, (bf16*)values, factors));
+                     block_table, table_stride, n_rows, window, (__half*)keys, (__half*)values, (float2*)factors));
     PE_LAUNCH_CHECK();
     return 0;
 }

@@ -136,13 +136,19 @@ __device__ __forceinline__ float2 at_both(unsigned long long v) {
     asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
     return r;
 }
-// 2^(a * scale + off) and 2^(b * scale + off) as two bfloat16 numbers, and both (unrounded) into `sum`
+// 2^(a * scale + off) and 2^(b * scale + off) as two bfloat16 (HALF: float16) numbers, and both (unrounded) into `sum`
+template <bool HALF = false>
 __device__ __forceinline__ unsigned at_exp2_pair(float a, float b, unsigned long long scale, unsigned long long off, unsigned long long& sum) {
     unsigned long long x = at_two(a, b);
     asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(x) : "l"(scale), "l"(off));
     const float2 v = at_both(x);
     const float e0 = at_exp2(v.x), e1 = at_exp2(v.y);
     asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum) : "l"(at_two(e0, e1)));
+    if constexpr (HALF) {
+        unsigned r;
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(e1), "f"(e0));
+        return r;
+    }
     return at_pack(e0, e1);
 }
 __device__ __forceinline__ float at_sum_four(unsigned long long a, unsigned long long b) {

@@ -2285,8 +2285,8 @@ def attention_int4(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int
 def attention_int4_prompt(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int, head_dim: int, pool: torch.Tensor, block_table: torch.Tensor, table_stride: int,
                           tiles: torch.Tensor, n_tokens: int, window: Optional[int], scale: float, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The same for runs of at most 128 tokens of a sequence, ``tiles`` int32 [n, 4] (``prefill_tiles`` with ``PREFILL_TILE_TCGEN05``), whose own keys and values the cache holds already;
-    ``q`` has ``n_tokens`` rows.  The pages that the runs see are expanded to 16 bits first, once a page and key head (scratch of the call, as large as one layer of a 16-bit cache: float16 keys, which
-    the queries' products need all eleven bits of, and bfloat16 values), and the products run on the tensor cores.  A page table has at most 16,384 rows; a page that several of them
+    ``q`` has ``n_tokens`` rows.  The pages that the runs see are expanded to 16 bits first, once a page and key head (scratch of the call, as large as one layer of a 16-bit cache: float16 numbers
+    with a power of two for each page's keys and values), and the products, with weights in float16, run on the tensor cores.  A page table has at most 16,384 rows; a page that several of them
     have stands at the same place of each.  A token that sees a key or value with a
     group that is no number has no number in the head's results."""
     n_bytes, device, width = _int4_heads(n_heads, n_kv_heads, head_dim), _device_here(q, "q"), n_heads * head_dim
@@ -2307,13 +2307,13 @@ def attention_int4_prompt(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_hea
         pages, lib = pool.shape[0], for_head_dim(head_dim)
         # (scratch of the call's own: calls on two streams and captured graphs share none)
         keys = q.new_empty((pages, n_kv_heads, PAGE, head_dim), dtype=torch.float16)
-        values = q.new_empty((pages, n_kv_heads, PAGE, head_dim))
-        factors = q.new_empty((pages, n_kv_heads), dtype=torch.float32)
-        nbytes = lib.pe_attention_prefill_half_keys_scratch(tiles.shape[0], n_heads, table_stride)
+        values = torch.empty_like(keys)
+        factors = q.new_empty((pages, n_kv_heads, 2), dtype=torch.float32)
+        nbytes = lib.pe_attention_prefill_half_scratch(tiles.shape[0], n_heads, table_stride)
         shares = pool.new_empty(nbytes) if nbytes else None
         check(long_context().pe_expand_int4(pool.data_ptr(), pages, n_kv_heads, head_dim, tiles.data_ptr(), tiles.shape[0], block_table.data_ptr(), table_stride, rows, window or 0,
                                             keys.data_ptr(), values.data_ptr(), factors.data_ptr(), stream), "attention_int4_prompt")
-        check(lib.pe_attention_prefill_half_keys(
+        check(lib.pe_attention_prefill_half(
             q.data_ptr(), q_stride, out.data_ptr(), keys.data_ptr(), values.data_ptr(), factors.data_ptr(), pages, block_table.data_ptr(), table_stride, rows, tiles.data_ptr(), tiles.shape[0],
             n_tokens, n_heads, n_kv_heads, head_dim, window or 0, scale, _ptr(shares), status_ptr(q.device), stream), "attention_int4_prompt", 2 if nbytes else 1)
     return out

@@ -156,7 +156,7 @@ _HEAD_DIM_SIGNATURES = {
     "pe_attention_decode": [P, I, P, P, P, P, I, P, P, I, I, I, I, I, F, I, I, P, P, I, P, P],
     "pe_attention_decode_splits": [I, I, I, I, P],
     "pe_attention_prefill": [P, I, P, P, P, P, I, P, P, P, I, I, I, I, I, F, P],
-    "pe_attention_prefill_half_keys": [P, I, P, P, P, P, LL, P, I, I, P, I, I, I, I, I, I, F, P, P, P],
+    "pe_attention_prefill_half": [P, I, P, P, P, P, LL, P, I, I, P, I, I, I, I, I, I, F, P, P, P],
     "pe_attention_prefill_tcgen05": [P, I, P, P, P, LL, P, I, P, I, I, I, I, I, I, F, I, P, P, P, P],
 }
 
@@ -342,8 +342,8 @@ def for_head_dim(head_dim: int) -> ctypes.CDLL:
         declare(lib, _HEAD_DIM_SIGNATURES)
         lib.pe_attention_shared_scratch.argtypes = [I, I, I]
         lib.pe_attention_shared_scratch.restype = c_longlong
-        lib.pe_attention_prefill_half_keys_scratch.argtypes = [I, I, I]
-        lib.pe_attention_prefill_half_keys_scratch.restype = c_longlong
+        lib.pe_attention_prefill_half_scratch.argtypes = [I, I, I]
+        lib.pe_attention_prefill_half_scratch.restype = c_longlong
         lib.pe_set_pdl(0 if os.environ.get("PICO_ENGINE_PDL", "1") == "0" else 1)
         _by_head_dim[head_dim] = lib
     return lib

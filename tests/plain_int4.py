@@ -76,7 +76,7 @@ def unpack(blocks):
 
 def attend(q, kept, seen, scale, halves=False):
     """q [H, D] over blocks of one row: ``kept`` [P, G, 80 D], ``seen`` bool [G, 64 P].  (result [H, D], its bound per number in halves of a bfloat16 step,
-    see the tests) in 64 bits.  ``halves``: for a kernel that takes keys as float16 and values as bfloat16."""
+    see the tests) in 64 bits.  ``halves``: for a kernel that takes keys, values and weights as float16."""
     H, D = q.shape
     P, G, _ = kept.shape
     keys, values, part, mids = (x.view(P, G, 64, D).transpose(0, 1).reshape(G, P * 64, D) for x in unpack(kept.flatten(0, 1)))
@@ -97,8 +97,16 @@ def attend(q, kept, seen, scale, halves=False):
         if halves:
             # half a step of float16, 2^-11, of every key; below 2^-14 of the page's largest times 2^14, a step of 2^-24 of that (page and query row are brought to 2^14 at most)
             err = scale * (2.0 ** -11 + (D + 16) * 2.0 ** -23) * (k.abs() @ q[h].abs()) + scale * 2.0 ** -37 * D * k.abs().max() * q[h].abs().max() + 2.0 ** -20
-            s = v                                        # values are rounded to bfloat16, and so are weights
         out.append(o)
-        # weights rounded (on v), once more behind a step (on the part that the codes carry), the result rounded; what scores are off moves weights by as much
-        bound.append(2.0 ** -8 * (w @ (v.abs() + s.abs()) + o.abs()) + 2 * (w * err) @ (v - o).abs() + 2 * (w @ err) * (w @ (v - o).abs()))
+        # what scores are off moves weights by as much; the result is rounded
+        moved = 2 * (w * err) @ (v - o).abs() + 2 * (w @ err) * (w @ (v - o).abs()) + 2.0 ** -8 * o.abs()
+        if halves:
+            # weights and values rounded to float16, 2^-11 each.  Of a page with values up to 2^f weights are held times 2^f, up to 2^14 for the largest of all pages (2^6 where the
+            # reference point lags behind it): below 2^-14 their steps are 2^-24, 2^-30 of the largest; values below 2^-28 of 2^f are off by 2^-39 of it.
+            most = values[g].nan_to_num(0.0).abs().view(P, -1).amax(1).repeat_interleave(64)[seen[g]] * 2
+            moved = moved + 2 * 2.0 ** -11 * (w @ v.abs()) + k.shape[0] * 2.0 ** -30 * (w * most).max() + 2.0 ** -38 * (w @ most)
+        else:
+            # weights rounded (on v), and once more behind a step (on the part that the codes carry)
+            moved = moved + 2.0 ** -8 * (w @ (v.abs() + s.abs()))
+        bound.append(moved)
     return torch.stack(out), torch.stack(bound)

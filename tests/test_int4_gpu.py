@@ -544,6 +544,21 @@ def test_runs_and_pages_that_are_none_of_the_call(K):
     p.check(got, [180], [0], q=q, table=there)
 
 
+@pytest.mark.parametrize("H,G,D", [(14, 2, 64), (4, 1, 128)])
+@pytest.mark.parametrize("start,n", [(0, 300), (4000, 130)])
+def test_prompts_over_pages_of_all_sizes(K, H, G, D, start, n):
+    """Pages whose values differ by many powers of two, and queries and keys far from one."""
+    total = start + n
+    p = Paged(H, G, D, [total], 98)
+    up = torch.randint(-25, 60, (p.n_pages, G, 1, 1), generator=gen(99), device="cuda")
+    p.pool = plain.pack((p.keys.double() * 2.0 ** -20).bfloat16().view(-1, 64, D), (p.values.double() * 2.0 ** up).bfloat16().view(-1, 64, D)).view(p.n_pages, G, 80 * D)
+    q = (randn(n, H * D, seed=100).double() * 2.0 ** 30).bfloat16()
+    p.scale *= 2.0 ** -10
+    got = K.attention_int4_prompt(q, H * D, H, G, D, p.pool, p.table, p.width, K.prefill_tiles([n], [start], "cuda", K.PREFILL_TILE_TCGEN05), n, None, p.scale)
+    some = [0, n // 2, n - 1]
+    p.check(got[some], [start + i for i in some], [0] * 3, q=q[some], halves=True)
+
+
 @pytest.mark.parametrize("H,G,D", [(4, 2, 64)])
 def test_prompts_of_many_rows(K, H, G, D):
     lens = [1 + b % 3 for b in range(5000)]
