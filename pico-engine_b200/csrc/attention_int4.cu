@@ -1,4 +1,20 @@
 // Attention of single tokens over the paged cache of 4-bit keys and values (int4_pages.cuh).
+//
+// A key is mid + step c per group of 32 channels, c = +-(k + 1/2), so a score is the sum over the groups of step (q . c) + mid (sum of q): products of the queries with codes as they stand, and one
+// more product of the groups' sums with their middles.  A value likewise: o = sum_j (w_j step_j) c_j + w_j mid_j.  The codes are bfloat16 numbers of 2^-129 units (subnormal, which mma.sync
+// keeps exactly), so queries and weights are taken 2^64 higher and sums 2^65 down; the bits of two codes cost two instructions, a rotation and one with a mask, and no conversion.
+// Scores, softmax statistics and results are float32 (running maximum and sum, one pass); a weight is rounded to bfloat16 for its product, and once more behind its
+// multiplication by a value's step: scaling the weights takes a multiplication a group and position, scaling the products would take one a channel and position.
+//
+// Keys (or channels) are the 16 rows of mma.sync m16n8k16 and a key head's queries its 8 columns: eight heads of a group are few for tcgen05.mma, whose operands would have to be written
+// to shared memory in 16 bits first.  A warp takes a page and key head at a time, a block of 80 D bytes that one bulk copy brings into its own ring of two, asked for by a warp
+// that does nothing else (with copies by each warp for itself 1.03 us a block and SM partition, 0.82 so; three places a warp leave room for fewer warps, which is slower; keys and values
+// in copies of their own wait 0.4 us a page longer).  The warps' sums are joined in shared memory, those of a cluster's CTAs through distributed shared memory.
+//
+// What bounds it: instructions.  A block of 64 channels takes 618, 319 of them on the logic units (two a pair of codes), 40 on the tensor cores (a quarter of their time).  The same kernel with the arithmetic
+// taken out copies its blocks in 46 us where the whole takes 65.5 (64 rows of 20,000 to 32,700, 14 heads of 64 on 2: 266 MB, 41 us at the copy rate of 6.5 TB/s); 63 of 86 (200 rows of up to 6,000,
+// 28 heads of 128 on 4: 385 MB, 59 us).  Fifteen warps (eleven of 128 channels, 168 registers) are what registers allow: the schedulers issue in 58 of 100 cycles, the logic units are
+// busy for 57 of them, DRAM for 53 to 62.  One row of 4,096 positions takes 4.5 us: a launch, and one chain of positions, table, block, join.
 #include "int4_pages.cuh"
 #include <map>
 #include <mutex>

@@ -11,8 +11,9 @@
 // values' codes holds four positions: a block takes the values of sixteen tokens of a head as they stand behind one another, and the first of a word's tokens gathers the others from shared
 // memory.  A word keeps the bits of positions that are not in the call; one of a tile that lies across two blocks is changed bit for bit by two atomic operations, so the other block may
 // change its own at the same time.
-// Bound by the memory for prompts: 7,541 tokens of 28 + 4 heads x 128 are 73 MB read and 59 MB written in 36.4 us (42.6 us with a block's keys and values in its two halves, which waited for
-// one another; 45 us with the queries' blocks in between).  A call for one token takes 3.9 us, which is a launch and one chain of loads.
+// Bound by the latency of a thread's chain of loads (position, angles) with as many threads as an SM holds: 7,541 tokens of 28 + 4 heads x 128 are 73 MB read and 59 MB written in 32.5 us
+// (36.9 us with 1,024 threads an SM, two query heads a thread; 42.6 us with a block's keys and values in its two halves, which waited for one another; 45 us with the queries' blocks in
+// between).  A call for one token takes 3.6 us, which is a launch and one chain of loads.
 template <int D>
 __device__ __forceinline__ void q4_load8(const bf16* p, float (&x)[8]) {
     const uint4 v = *reinterpret_cast<const uint4*>(p);
@@ -21,40 +22,30 @@ __device__ __forceinline__ void q4_load8(const bf16* p, float (&x)[8]) {
     for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
 }
 
-// HEADS query heads a thread, which share the angles it reads
-template <int D, int HEADS>
-__device__ __forceinline__ void store_queries(const bf16* qkv, int row_width, int n_q, const float* cos_t, const float* sin_t, int angles,
-                                              const int* tok_pos, bf16* q_out, long long item) {
+template <int D>
+__device__ __forceinline__ void store_queries(const bf16* qkv, int row_width, int n_q, const float* cos_t, const float* sin_t, int angles, const int* tok_pos, bf16* q_out, long long item) {
     constexpr int half = D / 2, parts = half / 8;
-    const int runs = (n_q + HEADS - 1) / HEADS, part = (int)(item % parts), run = (int)(item / parts % runs), t = (int)(item / parts / runs), j = part * 8;
-    const bf16* src = qkv + (size_t)t * row_width + run * HEADS * D + j;
-    bf16* dst = q_out + ((size_t)t * n_q + run * HEADS) * D + j;
-    const int heads = min(HEADS, n_q - run * HEADS);
-    uint4 lo[HEADS], hi[HEADS];
-#pragma unroll
-    for (int h = 0; h < HEADS; ++h)
-        if (h < heads) { lo[h] = *reinterpret_cast<const uint4*>(src + h * D); hi[h] = *reinterpret_cast<const uint4*>(src + h * D + half); }
+    const int j = (int)(item % parts) * 8, h = (int)(item / parts % n_q), t = (int)(item / parts / n_q);
+    const bf16* src = qkv + (size_t)t * row_width + h * D + j;
+    bf16* dst = q_out + ((size_t)t * n_q + h) * D + j;
+    uint4 lo = *reinterpret_cast<const uint4*>(src), hi = *reinterpret_cast<const uint4*>(src + half);
     if (cos_t) {
         const size_t at = (size_t)min(max(tok_pos[t], 0), angles - 1) * half + j;
         const float4* cp = reinterpret_cast<const float4*>(cos_t + at);
         const float4* sp = reinterpret_cast<const float4*>(sin_t + at);
         const float4 c0 = cp[0], c1 = cp[1], s0 = sp[0], s1 = sp[1];
         const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+        __nv_bfloat162* l2 = reinterpret_cast<__nv_bfloat162*>(&lo);
+        __nv_bfloat162* h2 = reinterpret_cast<__nv_bfloat162*>(&hi);
 #pragma unroll
-        for (int h = 0; h < HEADS; ++h) {
-            __nv_bfloat162* l2 = reinterpret_cast<__nv_bfloat162*>(&lo[h]);
-            __nv_bfloat162* h2 = reinterpret_cast<__nv_bfloat162*>(&hi[h]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 a = __bfloat1622float2(l2[e]), b = __bfloat1622float2(h2[e]);
-                l2[e] = __floats2bfloat162_rn(a.x * c[2 * e] - b.x * s[2 * e], a.y * c[2 * e + 1] - b.y * s[2 * e + 1]);
-                h2[e] = __floats2bfloat162_rn(a.x * s[2 * e] + b.x * c[2 * e], a.y * s[2 * e + 1] + b.y * c[2 * e + 1]);
-            }
+        for (int e = 0; e < 4; ++e) {
+            const float2 a = __bfloat1622float2(l2[e]), b = __bfloat1622float2(h2[e]);
+            l2[e] = __floats2bfloat162_rn(a.x * c[2 * e] - b.x * s[2 * e], a.y * c[2 * e + 1] - b.y * s[2 * e + 1]);
+            h2[e] = __floats2bfloat162_rn(a.x * s[2 * e] + b.x * c[2 * e], a.y * s[2 * e + 1] + b.y * c[2 * e + 1]);
         }
     }
-#pragma unroll
-    for (int h = 0; h < HEADS; ++h)
-        if (h < heads) { *reinterpret_cast<uint4*>(dst + h * D) = lo[h]; *reinterpret_cast<uint4*>(dst + h * D + half) = hi[h]; }
+    *reinterpret_cast<uint4*>(dst) = lo;
+    *reinterpret_cast<uint4*>(dst + half) = hi;
 }
 
 // step and mid of the group that four neighbouring lanes hold eight numbers each of, and the levels of the lane's own
@@ -89,8 +80,8 @@ __device__ __forceinline__ float q4_turned(float a, float c, float b, float s) {
 #define SI_THREADS 256
 #define SI_TOKENS 16
 
-template <int D, int HEADS>
-__global__ void __launch_bounds__(SI_THREADS, 4) store_int4_kernel(const bf16* qkv, int T, int n_q, int n_kv, const float* cos_t, const float* sin_t, int angles,
+template <int D>
+__global__ void __launch_bounds__(SI_THREADS, 8) store_int4_kernel(const bf16* qkv, int T, int n_q, int n_kv, const float* cos_t, const float* sin_t, int angles,
                                                                 const int* tok_pos, const int* tok_row, unsigned char* pool, long long n_pages,
                                                                 const int* block_table, int table_stride, int n_rows, bf16* q_out, int k_blocks, int v_blocks) {
     using B = Int4Block<D>;
@@ -108,7 +99,7 @@ __global__ void __launch_bounds__(SI_THREADS, 4) store_int4_kernel(const bf16* q
     const int w = threadIdx.x % lanes, b = w >> 2, t = w & 3, ch = w * 8;
     if ((int)blockIdx.x >= k_blocks + v_blocks) {
         const long long item = (long long)(blockIdx.x - k_blocks - v_blocks) * SI_THREADS + threadIdx.x;
-        if (item < (long long)T * ((n_q + HEADS - 1) / HEADS) * (D / 16)) store_queries<D, HEADS>(qkv, row_width, n_q, cos_t, sin_t, angles, tok_pos, q_out, item);
+        if (item < (long long)T * n_q * (D / 16)) store_queries<D>(qkv, row_width, n_q, cos_t, sin_t, angles, tok_pos, q_out, item);
         return;
     }
     if ((int)blockIdx.x < k_blocks) {
@@ -235,14 +226,11 @@ extern "C" int pe_store_int4(const void* qkv, int T, int n_q, int n_kv, int hd, 
     if (T <= 0) return 0;
     if ((hd != 64 && hd != 128) || n_q <= 0 || n_kv <= 0 || (((uintptr_t)qkv | (uintptr_t)pool | (uintptr_t)q_out) & 15)) return PE_ERR_UNSUPPORTED;
     if (cos_t && (angles <= 0 || (((uintptr_t)cos_t | (uintptr_t)sin_t) & 15))) return PE_ERR_UNSUPPORTED;
-    // one head a thread where the queries are few (its chain is what takes time), two where they fill the GPU (angles are read once for them)
-    const bool few = (long long)T * n_q * (hd / 16) <= pe_sm_count() * 2048ll;
-    const int runs = few ? n_q : (n_q + 1) / 2;
-    const long long items = (long long)T * runs * (hd / 16), q_blocks = (items + SI_THREADS - 1) / SI_THREADS;
+    const long long items = (long long)T * n_q * (hd / 16), q_blocks = (items + SI_THREADS - 1) / SI_THREADS;
     const long long per_k = SI_THREADS / (hd / 8), k_blocks = (T + per_k - 1) / per_k * n_kv, v_blocks = (long long)((T + SI_TOKENS - 1) / SI_TOKENS) * n_kv;
     const long long blocks = k_blocks + v_blocks + q_blocks, threads = SI_THREADS;
     if (blocks > 0x7fffffffll) return PE_ERR_UNSUPPORTED;
-    auto kernel = hd == 64 ? (few ? store_int4_kernel<64, 1> : store_int4_kernel<64, 2>) : few ? store_int4_kernel<128, 1> : store_int4_kernel<128, 2>;
+    auto kernel = hd == 64 ? store_int4_kernel<64> : store_int4_kernel<128>;
     PE_TRY(pe_launch(kernel, dim3((unsigned)blocks), dim3((unsigned)threads), 0, (cudaStream_t)stream, (const bf16*)qkv, T, n_q, n_kv, cos_t, sin_t, angles, tok_pos,
                      tok_row, (unsigned char*)pool, n_pages, block_table, table_stride, n_rows, (bf16*)q_out, (int)k_blocks, (int)v_blocks));
     PE_LAUNCH_CHECK();
