@@ -367,7 +367,7 @@ extern "C" int pe_page_bounds(const void* pool, long long n_pages, int n_kv, int
 // Bound by its writes: 7,541 tokens of 4 heads of 128 (and the 4,071 in front of a run of theirs) 7.5 MB read and 24 MB written, 10 to 11 us.
 // A block counts the pages of all rows from the runs, then takes every gridDim.x-th of them.
 
-#define XI_MAX_ROWS 16384                                     // twelve bytes each of shared memory
+#define XI_MAX_ROWS 18000                                     // twelve bytes each of shared memory
 #define XI_THREADS 256
 
 template <int D>

@@ -2286,7 +2286,7 @@ def attention_int4_prompt(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_hea
                           tiles: torch.Tensor, n_tokens: int, window: Optional[int], scale: float, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The same for runs of at most 128 tokens of a sequence, ``tiles`` int32 [n, 4] (``prefill_tiles`` with ``PREFILL_TILE_TCGEN05``), whose own keys and values the cache holds already;
     ``q`` has ``n_tokens`` rows.  The pages that the runs see are expanded to 16 bits first, once a page and key head (scratch of the call, as large as one layer of a 16-bit cache: float16 numbers
-    with a power of two for each page's keys and values), and the products, with weights in float16, run on the tensor cores.  A page table has at most 16,384 rows; a page that several of them
+    with a power of two for each page's keys and values), and the products, with weights in float16, run on the tensor cores.  A page table has at most 18,000 rows; a page that several of them
     have stands at the same place of each.  A token that sees a key or value with a
     group that is no number has no number in the head's results."""
     n_bytes, device, width = _int4_heads(n_heads, n_kv_heads, head_dim), _device_here(q, "q"), n_heads * head_dim
@@ -2296,8 +2296,8 @@ def attention_int4_prompt(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_hea
     rows = _page_rows(block_table, table_stride)
     if (window is not None and window < 0) or not scale > 0:
         raise KernelError("scale must be positive, and a window not negative")
-    if rows > 16384:
-        raise KernelError(f"prompts over a 4-bit cache take page tables of at most 16,384 rows, not {rows}")
+    if rows > 18000:
+        raise KernelError(f"prompts over a 4-bit cache take page tables of at most 18,000 rows, not {rows}")
     if out is None:
         out = q.new_empty((n_tokens, width))
     else:

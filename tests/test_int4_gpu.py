@@ -559,13 +559,13 @@ def test_prompts_over_pages_of_all_sizes(K, H, G, D, start, n):
     p.check(got[some], [start + i for i in some], [0] * 3, q=q[some], halves=True)
 
 
-@pytest.mark.parametrize("H,G,D", [(4, 2, 64)])
-def test_prompts_of_many_rows(K, H, G, D):
-    lens = [1 + b % 3 for b in range(5000)]
-    p = Paged(H, G, D, [1 + b % 3 for b in range(5000)], 96)
+@pytest.mark.parametrize("H,G,D,rows", [(4, 2, 64, 5000), (2, 1, 128, 17000)])
+def test_prompts_of_many_rows(K, H, G, D, rows):
+    lens = [1 + b % 3 for b in range(rows)]
+    p = Paged(H, G, D, lens, 96)
     n = sum(lens)
     q = randn(n, H * D, seed=97).bfloat16()
-    got = K.attention_int4_prompt(q, H * D, H, G, D, p.pool, p.table, p.width, K.prefill_tiles(lens, [0] * 5000, "cuda", K.PREFILL_TILE_TCGEN05), n, None, p.scale)
+    got = K.attention_int4_prompt(q, H * D, H, G, D, p.pool, p.table, p.width, K.prefill_tiles(lens, [0] * rows, "cuda", K.PREFILL_TILE_TCGEN05), n, None, p.scale)
     pos, row = [i for c in lens for i in range(c)], [b for b, c in enumerate(lens) for _ in range(c)]
     some = list(range(0, n, 997))
     p.check(got[some], [pos[i] for i in some], [row[i] for i in some], q=q[some], halves=True)
