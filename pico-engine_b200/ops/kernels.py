@@ -2168,15 +2168,18 @@ def _device_here(t: torch.Tensor, name: str) -> int:
     return device
 
 
-def _here(device: int, *tensors) -> None:
-    """(tensor, name, dtype, shape or None) of every argument of a call: contiguous, from a 16-byte boundary on, on the call's device."""
+def _here(device: int, *tensors) -> list:
+    """(tensor, name, dtype, shape or None) of every argument of a call: contiguous, from a 16-byte boundary on, on the call's device.  Their addresses."""
+    places = []
     for t, name, dtype, shape in tensors:
-        if t.dtype is dtype and t.get_device() == device and t.is_contiguous() and (shape is None or t.shape == shape) and t.data_ptr() % 16 == 0:
-            continue
-        _need(t, name, dtype, shape)
-        if t.get_device() != device:
-            raise KernelError(f"{name} lives on {t.device}, the current device is cuda:{device}")
-        raise KernelError(f"{name} must start on a 16-byte boundary")
+        at = t.data_ptr()
+        if t.dtype is not dtype or at & 15 or t.get_device() != device or not t.is_contiguous() or (shape is not None and t.shape != shape):
+            _need(t, name, dtype, shape)
+            if t.get_device() != device:
+                raise KernelError(f"{name} lives on {t.device}, the current device is cuda:{device}")
+            raise KernelError(f"{name} must start on a 16-byte boundary")
+        places.append(at)
+    return places
 
 
 def _page_rows(block_table: torch.Tensor, table_stride: int) -> int:
@@ -2199,21 +2202,22 @@ def store_int4(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, cos: Optio
 
     A group of 32 channels of a row is held as 32 codes c of 0 to 15, a step and a middle in bfloat16, mid = (max + min) / 2, step = (max - min) / 15: c = floor((x - mid) / step) + 8
     within its bounds, and stands for mid + step * (c - 7.5): at most half a step from x, but for the roundings of step and middle.  A group whose numbers are equal is held as it is; one with an
-    infinity or NaN is NaN as a whole.  Keys are turned in float64 and rounded to bfloat16 before they are coded.
+    infinity or NaN is NaN as a whole.  Keys are turned as in float64 and rounded to bfloat16 before they are coded.
 
     Tokens of a sequence stand behind one another in the call, in the order of their positions (which may leave some out), and no position twice; tokens whose page is not there (-1) are not
     stored."""
     T, n_bytes, device = tok_pos.shape[0], _int4_heads(n_q, n_kv, head_dim), _device_here(qkv, "qkv")
-    row, width = (T,), n_q * head_dim
-    _here(device, (qkv, "qkv", torch.bfloat16, (T, width + 2 * n_kv * head_dim)), (tok_pos, "tok_pos", torch.int32, row), (tok_row, "tok_row", torch.int32, row),
-          (pool, "pool", torch.uint8, (pool.shape[0], n_kv, n_bytes)), (block_table, "block_table", torch.int32, None))
+    row, width, pages = (T,), n_q * head_dim, pool.shape[0]
+    qkv_at, pos_at, row_at, pool_at, table_at = _here(device, (qkv, "qkv", torch.bfloat16, (T, width + 2 * n_kv * head_dim)), (tok_pos, "tok_pos", torch.int32, row),
+                                                      (tok_row, "tok_row", torch.int32, row), (pool, "pool", torch.uint8, (pages, n_kv, n_bytes)),
+                                                      (block_table, "block_table", torch.int32, None))
     rows = _page_rows(block_table, table_stride)
     if (cos is None) != (sin is None):
         raise KernelError("cos and sin go together")
-    angles = 0
+    angles, cos_at, sin_at = 0, None, None
     if cos is not None:
         angles = cos.shape[0]
-        _here(device, (cos, "cos", torch.float32, (angles, head_dim // 2)), (sin, "sin", torch.float32, (angles, head_dim // 2)))
+        cos_at, sin_at = _here(device, (cos, "cos", torch.float32, (angles, head_dim // 2)), (sin, "sin", torch.float32, (angles, head_dim // 2)))
         if angles < 1:
             raise KernelError("cos and sin must hold a position at least")
     if out is None:
@@ -2221,21 +2225,22 @@ def store_int4(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, cos: Optio
     else:
         _here(device, (out, "out", torch.bfloat16, (T, width)))
     if T:
-        check(long_context().pe_store_int4(qkv.data_ptr(), T, n_q, n_kv, head_dim, _ptr(cos), _ptr(sin), angles, tok_pos.data_ptr(), tok_row.data_ptr(), pool.data_ptr(), pool.shape[0],
-                                           block_table.data_ptr(), table_stride, rows, out.data_ptr(), torch._C._cuda_getCurrentRawStream(device)), "store_int4")
+        check(long_context().pe_store_int4(qkv_at, T, n_q, n_kv, head_dim, cos_at, sin_at, angles, pos_at, row_at, pool_at, pages, table_at, table_stride, rows, out.data_ptr(),
+                                           torch._C._cuda_getCurrentRawStream(device)), "store_int4")
     return out
 
 
 def load_int4(pool: torch.Tensor, n_kv: int, head_dim: int, tok_pos: torch.Tensor, tok_row: torch.Tensor, block_table: torch.Tensor, table_stride: int):
     """What a 4-bit cache holds at positions ``tok_pos`` of the sequences ``tok_row`` (int32 [T]): keys and values, float32 [T, n_kv, head_dim].  Zeros where no page is."""
     T, n_bytes, device = tok_pos.shape[0], _int4_heads(n_kv, n_kv, head_dim), _device_here(pool, "pool")
-    _here(device, (tok_pos, "tok_pos", torch.int32, (T,)), (tok_row, "tok_row", torch.int32, (T,)), (pool, "pool", torch.uint8, (pool.shape[0], n_kv, n_bytes)),
-          (block_table, "block_table", torch.int32, None))
+    pages = pool.shape[0]
+    pos_at, row_at, pool_at, table_at = _here(device, (tok_pos, "tok_pos", torch.int32, (T,)), (tok_row, "tok_row", torch.int32, (T,)), (pool, "pool", torch.uint8, (pages, n_kv, n_bytes)),
+                                              (block_table, "block_table", torch.int32, None))
     rows = _page_rows(block_table, table_stride)
     keys, values = pool.new_empty((2, T, n_kv, head_dim), dtype=torch.float32).unbind(0)
     if T:
-        check(long_context().pe_load_int4(pool.data_ptr(), pool.shape[0], n_kv, head_dim, tok_pos.data_ptr(), tok_row.data_ptr(), T, block_table.data_ptr(), table_stride, rows,
-                                          keys.data_ptr(), values.data_ptr(), torch._C._cuda_getCurrentRawStream(device)), "load_int4")
+        check(long_context().pe_load_int4(pool_at, pages, n_kv, head_dim, pos_at, row_at, T, table_at, table_stride, rows, keys.data_ptr(), values.data_ptr(),
+                                          torch._C._cuda_getCurrentRawStream(device)), "load_int4")
     return keys, values
 
 
@@ -2244,13 +2249,14 @@ def _int4_scratch_bytes(T: int, n_heads: int, n_kv_heads: int, head_dim: int, ma
     return long_context().pe_attention_int4_scratch(T, n_heads, n_kv_heads, head_dim, max_context, selected, window)
 
 
-def _attend_int4(q, q_stride, out, pool, table, table_stride, rows, tok_pos, tok_row, T, n_heads, n_kv_heads, head_dim, window, scale, max_context, selected, early, device, name) -> None:
+def _attend_int4(q_at, q_stride, out, pool, pool_at, pages, table_at, table_stride, rows, pos_at, row_at, T, n_heads, n_kv_heads, head_dim, window, scale, max_context, selected, early, device,
+                 name) -> None:
     n = _int4_scratch_bytes(T, n_heads, n_kv_heads, head_dim, max_context, selected, window)
     # (what a call leaves for its second kernel to join is the call's own: calls on two streams and captured graphs share none)
     scratch = pool.new_empty(n) if n else None
-    check(long_context().pe_attention_int4(q.data_ptr(), q_stride, out.data_ptr(), pool.data_ptr(), pool.shape[0] * n_kv_heads, table.data_ptr(), table_stride, rows, tok_pos.data_ptr(),
-                                           _ptr(tok_row), T, n_heads, n_kv_heads, head_dim, window, scale, max_context, selected, early, _ptr(scratch), status_ptr(q.device),
-                                           torch._C._cuda_getCurrentRawStream(device)), name, 1 if scratch is None else 2)
+    check(long_context().pe_attention_int4(q_at, q_stride, out.data_ptr(), pool_at, pages * n_kv_heads, table_at, table_stride, rows, pos_at, row_at, T, n_heads, n_kv_heads, head_dim, window,
+                                           scale, max_context, selected, early, _ptr(scratch), status_ptr(out.device), torch._C._cuda_getCurrentRawStream(device)),
+          name, 1 if scratch is None else 2)
 
 
 def attention_int4(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int, head_dim: int, pool: torch.Tensor, block_table: torch.Tensor, table_stride: int,
@@ -2264,8 +2270,9 @@ def attention_int4(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int
     the values, and once more behind their multiplication by a value's step.  Queries, keys and values of sizes between 2^-40 and 2^60 keep that: the products with codes are taken in units
     of 2^-65.  A row that sees nothing is zeros; one that sees a group that is no number is none where that reaches."""
     T, n_bytes, device, width = tok_pos.shape[0], _int4_heads(n_heads, n_kv_heads, head_dim), _device_here(q, "q"), n_heads * head_dim
-    _here(device, (q, "q", torch.bfloat16, None), (tok_pos, "tok_pos", torch.int32, (T,)), (tok_row, "tok_row", torch.int32, (T,)),
-          (pool, "pool", torch.uint8, (pool.shape[0], n_kv_heads, n_bytes)), (block_table, "block_table", torch.int32, None))
+    pages = pool.shape[0]
+    q_at, pos_at, row_at, pool_at, table_at = _here(device, (q, "q", torch.bfloat16, None), (tok_pos, "tok_pos", torch.int32, (T,)), (tok_row, "tok_row", torch.int32, (T,)),
+                                                    (pool, "pool", torch.uint8, (pages, n_kv_heads, n_bytes)), (block_table, "block_table", torch.int32, None))
     _query_rows(q, q_stride, T, width)
     rows = _page_rows(block_table, table_stride)
     if max_context < 1 or (window is not None and window < 0) or not scale > 0:
@@ -2277,7 +2284,7 @@ def attention_int4(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int
     if window:
         max_context = min(max_context, (window + PAGE - 2) // PAGE * PAGE + PAGE)         # (positions of as many pages as a window can lie on)
     if T:
-        _attend_int4(q, q_stride, out, pool, block_table, table_stride, rows, tok_pos, tok_row, T, n_heads, n_kv_heads, head_dim, window or 0, scale, max_context, 0,
+        _attend_int4(q_at, q_stride, out, pool, pool_at, pages, table_at, table_stride, rows, pos_at, row_at, T, n_heads, n_kv_heads, head_dim, window or 0, scale, max_context, 0,
                      1 if early_pages else 0, device, "attention_int4")
     return out
 
@@ -2324,12 +2331,13 @@ def page_bounds(pool: torch.Tensor, n_kv: int, head_dim: int, tok_pos: torch.Ten
     """The least and the greatest key of every channel of the pages that the tokens of a step have filled: where a token is the last of its page, ``bounds`` (bfloat16 [pages, n_kv, 2, head_dim])
     gets the page's rows, in place; the others stay as they are.  Of the keys that the 4-bit cache stands for, rounded to bfloat16."""
     T, n_bytes, device = tok_pos.shape[0], _int4_heads(n_kv, n_kv, head_dim), _device_here(pool, "pool")
-    _here(device, (tok_pos, "tok_pos", torch.int32, (T,)), (tok_row, "tok_row", torch.int32, (T,)), (pool, "pool", torch.uint8, (pool.shape[0], n_kv, n_bytes)),
-          (block_table, "block_table", torch.int32, None), (bounds, "bounds", torch.bfloat16, (pool.shape[0], n_kv, 2, head_dim)))
+    pages = pool.shape[0]
+    pos_at, row_at, pool_at, table_at, bounds_at = _here(device, (tok_pos, "tok_pos", torch.int32, (T,)), (tok_row, "tok_row", torch.int32, (T,)),
+                                                         (pool, "pool", torch.uint8, (pages, n_kv, n_bytes)), (block_table, "block_table", torch.int32, None),
+                                                         (bounds, "bounds", torch.bfloat16, (pages, n_kv, 2, head_dim)))
     rows = _page_rows(block_table, table_stride)
     if T:
-        check(long_context().pe_page_bounds(pool.data_ptr(), pool.shape[0], n_kv, head_dim, tok_pos.data_ptr(), tok_row.data_ptr(), T, block_table.data_ptr(), table_stride, rows,
-                                            bounds.data_ptr(), torch._C._cuda_getCurrentRawStream(device)), "page_bounds")
+        check(long_context().pe_page_bounds(pool_at, pages, n_kv, head_dim, pos_at, row_at, T, table_at, table_stride, rows, bounds_at, torch._C._cuda_getCurrentRawStream(device)), "page_bounds")
     return bounds
 
 
@@ -2348,9 +2356,9 @@ def select_pages(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int, 
     no more than ``keep``; none (and place -1) for a token in front of position 0 or of no row of the table.  ``max_context`` bounds every token's position + 1."""
     T = tok_pos.shape[0]
     _int4_heads(n_heads, n_kv_heads, head_dim)
-    device = _device_here(q, "q")
-    _here(device, (q, "q", torch.bfloat16, None), (tok_pos, "tok_pos", torch.int32, (T,)), (tok_row, "tok_row", torch.int32, (T,)),
-          (bounds, "bounds", torch.bfloat16, (bounds.shape[0], n_kv_heads, 2, head_dim)), (block_table, "block_table", torch.int32, None))
+    device, n_pages = _device_here(q, "q"), bounds.shape[0]
+    q_at, pos_at, row_at, bounds_at, table_at = _here(device, (q, "q", torch.bfloat16, None), (tok_pos, "tok_pos", torch.int32, (T,)), (tok_row, "tok_row", torch.int32, (T,)),
+                                                      (bounds, "bounds", torch.bfloat16, (n_pages, n_kv_heads, 2, head_dim)), (block_table, "block_table", torch.int32, None))
     _query_rows(q, q_stride, T, n_heads * head_dim)
     rows = _page_rows(block_table, table_stride)
     most = min((max_context - 1) // PAGE + 1, table_stride)
@@ -2361,9 +2369,8 @@ def select_pages(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int, 
     if T:
         apart = most > SELECT_ONE_PAGES
         scores = tok_pos.new_empty(2 * n * most) if apart else None           # (the call's own: calls on two streams and captured graphs share none)
-        check(long_context().pe_select_pages(q.data_ptr(), q_stride, T, n_heads, n_kv_heads, head_dim, bounds.data_ptr(), bounds.shape[0], block_table.data_ptr(), table_stride, rows,
-                                             tok_pos.data_ptr(), tok_row.data_ptr(), keep, max_context, table.data_ptr(), pos.data_ptr(), _ptr(scores),
-                                             torch._C._cuda_getCurrentRawStream(device)), "select_pages", 2 if apart and most > keep > 2 else 1)
+        check(long_context().pe_select_pages(q_at, q_stride, T, n_heads, n_kv_heads, head_dim, bounds_at, n_pages, table_at, table_stride, rows, pos_at, row_at, keep, max_context,
+                                             table.data_ptr(), pos.data_ptr(), _ptr(scores), torch._C._cuda_getCurrentRawStream(device)), "select_pages", 2 if apart and most > keep > 2 else 1)
     return SelectedPages(table, pos)
 
 
@@ -2372,8 +2379,9 @@ def attention_int4_selected(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_h
     """``attention_int4`` over the pages that ``select_pages`` has found."""
     n_bytes, device, width, places = _int4_heads(n_heads, n_kv_heads, head_dim), _device_here(q, "q"), n_heads * head_dim, pages.pos.shape[0]
     T, keep = places // n_kv_heads, pages.table.shape[1]
-    _here(device, (q, "q", torch.bfloat16, None), (pool, "pool", torch.uint8, (pool.shape[0], n_kv_heads, n_bytes)), (pages.pos, "pages.pos", torch.int32, (T * n_kv_heads,)),
-          (pages.table, "pages.table", torch.int32, (places, keep)))
+    n_pages = pool.shape[0]
+    q_at, pool_at, pos_at, table_at = _here(device, (q, "q", torch.bfloat16, None), (pool, "pool", torch.uint8, (n_pages, n_kv_heads, n_bytes)),
+                                            (pages.pos, "pages.pos", torch.int32, (T * n_kv_heads,)), (pages.table, "pages.table", torch.int32, (places, keep)))
     _query_rows(q, q_stride, T, width)
     if not scale > 0:
         raise KernelError("scale must be positive")
@@ -2382,5 +2390,6 @@ def attention_int4_selected(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_h
     else:
         _here(device, (out, "out", torch.bfloat16, (T, width)))
     if T:
-        _attend_int4(q, q_stride, out, pool, pages.table, keep, places, pages.pos, None, T, n_heads, n_kv_heads, head_dim, 0, scale, keep * PAGE, 1, 0, device, "attention_int4_selected")
+        _attend_int4(q_at, q_stride, out, pool, pool_at, n_pages, table_at, keep, places, pos_at, None, T, n_heads, n_kv_heads, head_dim, 0, scale, keep * PAGE, 1, 0, device,
+                     "attention_int4_selected")
     return out
