@@ -2,6 +2,7 @@
 and the head that gives logits at the wanted rows."""
 from __future__ import annotations
 
+from dataclasses import replace
 from typing import Dict, List, Optional
 
 import torch
@@ -70,6 +71,11 @@ class DecoderModel:
         """Per schedule entry; None for an entry that reads another entry's cache.  Behind the schedule's entries comes what
         the model itself keeps per sequence: the token before the next one (int32), where the embedding reads pairs."""
         needs = [None if e.cache_of is not None else self.layers[e.layer].cache_needs() for e in self.plan.schedule]
+        for e in self.plan.schedule:                        # pages of codes only where all their readers take them
+            if e.cache_of is not None and needs[e.cache_of] is not None and needs[e.cache_of].kv is not None and needs[e.cache_of].kv.may_be_int4:
+                reader = self.layers[e.layer].cache_needs()
+                if reader is None or reader.kv is None or not reader.kv.may_be_int4:
+                    needs[e.cache_of] = replace(needs[e.cache_of], kv=replace(needs[e.cache_of].kv, may_be_int4=False))
         if self.plan.embedding_pairs is not None:
             needs.append(CacheNeeds(state_elems=1, state_dtype="int32"))
         return needs

@@ -51,3 +51,15 @@ def test_heads_are_checked_before_tensors():
                 call(*heads)
         with pytest.raises(KernelError, match="must live on a CUDA device"):
             call(4, 2, 64)
+
+
+def test_pages_of_codes_only_where_all_their_readers_take_them():
+    from types import SimpleNamespace as N
+    from pico_engine.cache import CacheNeeds
+    from pico_engine.cache.needs import KVNeed
+    from pico_engine.parts.model import DecoderModel
+    takes, other = CacheNeeds(kv=KVNeed(2, 64, may_be_int4=True)), CacheNeeds(kv=KVNeed(2, 64))
+    model = object.__new__(DecoderModel)
+    model.layers = [N(cache_needs=lambda n=n: n) for n in (takes, takes, other, takes)]
+    model.plan = N(embedding_pairs=None, schedule=[N(layer=0, cache_of=None), N(layer=1, cache_of=None), N(layer=2, cache_of=0), N(layer=3, cache_of=1), N(layer=3, cache_of=None)])
+    assert model.cache_needs() == [other, takes, None, None, takes]
