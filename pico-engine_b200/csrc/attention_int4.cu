@@ -16,9 +16,7 @@
 // 28 heads of 128 on 4: 385 MB, 59 us).  Fifteen warps (eleven of 128 channels, 168 registers) are what registers allow: the schedulers issue in 58 of 100 cycles, the logic units are
 // busy for 57 of them, DRAM for 53 to 62.  One row of 4,096 positions takes 4.5 us: a launch, and one chain of positions, table, block, join.
 #include "int4_pages.cuh"
-#include <map>
-#include <mutex>
-#include <utility>
+#include <atomic>
 
 #define AI_MAX_SPLITS 16
 #define AI_WAIT_CYCLES 2000000000ll                            // about a second of SM clock
@@ -729,15 +727,13 @@ struct AiLaunch {
         static bool done[64] = {};
         return ai_allow((const void*)attention_int4_kernel<D, WARPS>, S::smem, done, true);
     }
-    // clusters of so many CTAs that the GPU holds at once
+    // clusters of so many CTAs (a power of two) that the GPU holds at once; asked once a device
     static int at_once(int splits) {
-        static std::mutex lock;
-        static std::map<std::pair<int, int>, int> known;
-        std::lock_guard<std::mutex> hold(lock);
-        int dev = 0;
+        static std::atomic<int> known[64][8];                  // one more than the number, 0: not asked yet
+        int dev = 0, power = 0;
         if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-        auto it = known.find({dev, splits});
-        if (it != known.end()) return it->second;
+        while ((1 << power) < splits) ++power;
+        if (dev < 64) { const int k = known[dev][power].load(std::memory_order_relaxed); if (k) return k - 1; }
         int n = 0;
         if (allow() == 0) {
             cudaLaunchConfig_t cfg = {};
@@ -751,7 +747,7 @@ struct AiLaunch {
             cfg.numAttrs = 1;
             if (cudaOccupancyMaxActiveClusters(&n, attention_int4_kernel<D, WARPS>, &cfg) != cudaSuccess) { cudaGetLastError(); n = 0; }
         }
-        known[{dev, splits}] = n;
+        if (dev < 64) known[dev][power].store(n + 1, std::memory_order_relaxed);
         return n;
     }
     // CTAs of a (token, key head, tile of heads): as many as run at once, each warp with a page at least.  (Large clusters find room for fewer than the occupancy says while
