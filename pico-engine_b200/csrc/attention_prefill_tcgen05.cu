@@ -283,6 +283,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) attention_prefill_tcgen05_kerne
             sums[g * AT_QTILE + r] = most;
             asm volatile("bar.sync 1, 256;" ::: "memory");          // the softmax warps
             most = fmaxf(most, sums[(g ^ 1) * AT_QTILE + r]);
+            asm volatile("bar.sync 1, 256;" ::: "memory");          // (a group without a step writes its sums at once: not before the other one has read)
             int exponent = 0;
             if (most > 0.f) frexpf(fminf(most, 3.0e38f), &exponent);
             const float up = ldexpf(1.f, 14 - max(exponent, -30));
