@@ -174,7 +174,7 @@ def open_sequences(engine, batch: int, length: int, seed: int = 0) -> List[int]:
         s = engine.cache.open()
         ids = torch.randint(0, engine.model.plan.vocab_size, (length,), generator=g).tolist()
         for at in range(0, length, 4096):
-            engine.stepper.step([s], [ids[at:at + 4096]], [[]])
+            engine.stepper.step([s], [ids[at:at + 4096]], [[]], prompts=True)
         slots.append(s)
     return slots
 
@@ -248,7 +248,7 @@ def prefill_device(engine, tokens: int, repetitions: int = 5, warmup: int = 3, s
         e0.record()
         if i == warmup + repetitions - 1:                 # one step, the last, is marked for a profiler's launch list
             torch.cuda.nvtx.range_push("pico_prefill")
-        engine.stepper.step([s], [ids], use_graph=use_graph)
+        engine.stepper.step([s], [ids], use_graph=use_graph, prompts=True)
         if i == warmup + repetitions - 1:
             torch.cuda.nvtx.range_pop()
         e1.record()
@@ -325,7 +325,7 @@ def last_logits(engine, prompts: Sequence[Sequence[int]], batch: int = 8) -> tor
     for at in range(0, len(prompts), batch):
         group = prompts[at:at + batch]
         slots = [engine.cache.open() for _ in group]
-        rows.append(engine.stepper.step(slots, group).cpu())
+        rows.append(engine.stepper.step(slots, group, prompts=True).cpu())
         for s in slots:
             engine.cache.close(s)
     return torch.cat(rows)

@@ -231,7 +231,7 @@ class EngineBackend:
             for pieces in cut_prompts([len(p) for p in prompts], budget):
                 ends = [at + n == len(prompts[r]) for r, at, n in pieces]
                 out = self.e.stepper.step([slots[r] for r, _, _ in pieces], [prompts[r][at:at + n] for r, at, n in pieces],
-                                          [[n - 1] if end else [] for (_, _, n), end in zip(pieces, ends)])
+                                          [[n - 1] if end else [] for (_, _, n), end in zip(pieces, ends)], prompts=True)
                 for k, r in enumerate(r for (r, _, _), end in zip(pieces, ends) if end):
                     rows[r] = out[k]
             return torch.stack(rows)

@@ -143,7 +143,7 @@ class GraphedPrompt:
         all_slots = list(slots) + [cache.idle_slot] * len(pad)
         _, host, starts = st.describe(all_slots, lens + pad, None, list(token_ids) + [[0] * n for n in pad], self.widths, self.n_tiles)
         st.upload(host, self.dev)
-        ctx = st.context(lay, self.dev, lens + pad, starts, all_slots)
+        ctx = st.context(lay, self.dev, lens + pad, starts, all_slots, prompts=True)
         ctx.max_context = st.max_context                  # what the captured launches were shaped for
         self.launches += 1
         if self.graph is None and not self.failed and self.launches >= 2:

@@ -255,7 +255,7 @@ class Stepper:
         return starts
 
     def context(self, lay: StepLayout, dev: torch.Tensor, lens: List[int], starts: List[int],
-                slot_ids: Sequence[int] = ()) -> StepContext:
+                slot_ids: Sequence[int] = (), prompts: bool = False) -> StepContext:
         tables = {g: dev[off: off + lay.B * lay.widths[g]].view(lay.B, lay.widths[g])
                   for g, off in enumerate(lay.tables)}
         scratch = {name: dev[off: off + 4 * n].view(n, 4)
@@ -268,7 +268,7 @@ class Stepper:
             slots=dev[lay.slots: lay.slots + lay.B], row_first=dev[lay.first: lay.first + lay.B + 1],
             row_lens=dev[lay.lens: lay.lens + lay.B], slot_ids=list(slot_ids), lens=list(lens), starts=list(starts),
             one_token_each=all(n == 1 for n in lens), cache=self.cache, tables=tables,
-            max_context=max(s + n for s, n in zip(starts, lens)), attend_pages=self.attend_pages)
+            max_context=max(s + n for s, n in zip(starts, lens)), attend_pages=None if prompts or any(n != 1 for n in lens) else self.attend_pages)
 
     def upload(self, host: np.ndarray, dev: Optional[torch.Tensor] = None) -> torch.Tensor:
         slot, staged = self._stage(host)
@@ -307,12 +307,14 @@ class Stepper:
     @torch.inference_mode()
     def step(self, slots: Sequence[int], token_ids: Sequence[Sequence[int]],
              want: Optional[Sequence[Sequence[int]]] = None,
-             device_tokens: Optional[torch.Tensor] = None, use_graph: bool = False) -> torch.Tensor:
+             device_tokens: Optional[torch.Tensor] = None, use_graph: bool = False, prompts: bool = False) -> torch.Tensor:
         """Run one step; returns float32 logits [wanted places, vocab] on the device, in the
         order of the rows and of ``want``.  With ``device_tokens`` (int32 [B], one token per row,
         already on the device) ``token_ids`` only gives the rows' lengths (all 1).  ``use_graph``: a step
         that brings prompts and wants each row's last logits runs at padded sizes (``engine.graph.GraphedPrompt``:
-        rows and tokens filled up with idle rows), from the second time on as a captured graph."""
+        rows and tokens filled up with idle rows), from the second time on as a captured graph.  ``prompts``: the
+        tokens are prompts or pieces of them, which attend to everything, also where each row brings one token; a step
+        of one token a row is one of decoded tokens otherwise, one in which a row brings several is one of prompts."""
         if use_graph and want is None and device_tokens is None and any(len(t) != 1 for t in token_ids):
             g = self._prompt_graph(len(slots), sum(len(t) for t in token_ids))
             if g is not None:
@@ -324,7 +326,7 @@ class Stepper:
             lens = [len(t) for t in token_ids]
             lay, host, starts = self.describe(slots, lens, want, token_ids, shared=all(n == 1 for n in lens) and self.sharing_pays(slots))
         dev = self.upload(host)
-        ctx = self.context(lay, dev, lens, starts, slots)
+        ctx = self.context(lay, dev, lens, starts, slots, prompts)
         ids = device_tokens if device_tokens is not None else dev[lay.ids: lay.ids + lay.T]
         x = self.model.hidden(ids, ctx)
         for s, n in zip(slots, lens):

@@ -85,7 +85,7 @@ class StepContext:
     pending_norm: Optional["Norm"] = None   # the norm that product passes on its way into the stream (None: it is added as it is)
     pending_streams: Optional["Part"] = None  # how it enters a residual of several streams (a StreamMix)
     pending_rows: Optional[tuple] = None    # (rows [T, hidden], weights [T]): rows times a number a token that are added with the pending product
-    attend_pages: Optional[int] = None    # pages that single tokens attend to in groups with bounds (None: all)
+    attend_pages: Optional[int] = None    # pages that the step's decoded tokens attend to in groups with bounds (None: all; so in a step of prompts)
     stream_source: Optional[torch.Tensor] = None  # the one matrix [T, hidden] that all streams still equal, before the first sum into them
 
     # A part whose product comes out of the library may leave the sum into the residual stream pending, so

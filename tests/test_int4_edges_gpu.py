@@ -35,3 +35,33 @@ def test_short_prompts_again_and_again(K, H, G, D):
     p.check(first[some], [pos[i] for i in some], [row[i] for i in some], q=q[some], halves=True)
     for _ in range(100):
         assert torch.equal(run(), first)
+
+
+# ---------------------------------------------------------------------------- the part and the engine
+
+@pytest.fixture(scope="module")
+def folder(tmp_path_factory):
+    from conftest import make_weights, write_model
+    from test_int4_engine_gpu import LONG
+    return write_model(tmp_path_factory.mktemp("int4_edges") / "long", LONG, make_weights(LONG, 8, sharp=True)), LONG
+
+
+def test_a_prompts_last_piece_of_one_token_attends_to_everything(folder):
+    """However a prompt is cut, its tokens see all of it; decoded tokens see the pages that are selected."""
+    from pico_engine import Engine
+    from pico_engine.engine.engine import EngineBackend
+    from pico_engine.sampling import Sampler, SamplingParams
+    from test_int4_engine_gpu import prompts
+    path, cfg = folder
+    texts, logits = prompts(cfg, [6 * 64 + 1, 65, 700]), {}
+    for attend in (None, 4):
+        eng = Engine(path, cache="int4", attend_pages=attend, max_context=1500, max_tokens_in_cache=64 * 60)
+        eng.ensure_cache(64 * 60, 1500)
+        eng.prefill_tokens_per_step = 64
+        slots = [eng.cache.open() for _ in texts]
+        back = EngineBackend(eng, Sampler(SamplingParams(0.0, 0, 1.0, 0)), False)
+        logits[attend] = [back._prompts(slots[:1], texts[:1])[0], *back._prompts(slots[1:], texts[1:])]
+        logits[attend].append(eng.stepper.step(slots, [[3], [4], [5]]))
+    for a, b in zip(logits[None][:3], logits[4][:3]):
+        assert torch.equal(a, b)
+    assert not torch.equal(logits[None][3], logits[4][3])
