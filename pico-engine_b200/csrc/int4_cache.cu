@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(XI_THREADS) expand_int4_kernel(const unsigned 
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < XI_THREADS / 32; ++w) { most = fmaxf(most, largest[w].x); most_v = fmaxf(most_v, largest[w].y); }
-        int exponent = 0, f = 0;
+        int exponent = 0, f = -30;                             // (a page of zero values asks for no more of the weights' range than one of the smallest)
         if (most > 0.f) frexpf(fminf(most, 3.0e38f), &exponent);                          // most <= 2^exponent
         if (most_v > 0.f) frexpf(fminf(most_v, 3.0e38f), &f);
         f = min(max(f, -30), 115);                             // (2^-f and 2^-f times the weights' power are normal numbers)

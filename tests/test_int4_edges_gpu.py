@@ -37,6 +37,21 @@ def test_short_prompts_again_and_again(K, H, G, D):
         assert torch.equal(run(), first)
 
 
+@pytest.mark.parametrize("H,G,D", [(14, 2, 64), (8, 2, 128)])
+def test_prompts_over_pages_without_a_value(K, H, G, D):
+    """Pages whose values are all zero beside pages of small ones: they weigh in the softmax and carry nothing, and the others keep their bits."""
+    n = 500
+    p = Paged(H, G, D, [n], 131)
+    up = torch.full((p.n_pages, 1, 1, 1), 2.0 ** -30, device="cuda", dtype=torch.float64)
+    up[p.pages[0][2]] = 0.0
+    up[p.pages[0][5]] = 0.0
+    p.pool = plain.pack(p.keys.view(-1, 64, D), (p.values.double() * up).bfloat16().view(-1, 64, D)).view(p.n_pages, G, 80 * D)
+    q = randn(n, H * D, seed=132).bfloat16()
+    got = K.attention_int4_prompt(q, H * D, H, G, D, p.pool, p.table, p.width, K.prefill_tiles([n], [0], "cuda", K.PREFILL_TILE_TCGEN05), n, None, p.scale)
+    some = [0, 100, 200, 383, n - 1]
+    p.check(got[some], some, [0] * len(some), q=q[some], halves=True)
+
+
 # ---------------------------------------------------------------------------- the part and the engine
 
 @pytest.fixture(scope="module")
