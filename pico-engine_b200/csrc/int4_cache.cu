@@ -59,9 +59,9 @@ __device__ __forceinline__ void q4_group(const float (&x)[8], int (&level)[8], b
         hi = q4_max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
     q4_scale(lo, hi, step, mid);
-    const float s = __bfloat162float(step), m = __bfloat162float(mid), by = s == 0.f ? 0.f : 1.f / s;
+    const float up = q4_up(__bfloat162float(step)), s = __bfloat162float(step) * up, m = __bfloat162float(mid) * up, by = s == 0.f ? 0.f : 1.f / s;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) level[i] = q4_quantise(x[i], s, m, by);
+    for (int i = 0; i < 8; ++i) level[i] = q4_quantise(x[i] * up, s, m, by);
 }
 
 // a c + b s rounded to bfloat16 by way of a float32 that is as if from twice as many bits: products with their errors, and the error of their sum.  Two products, one with its error, are off by

@@ -59,6 +59,9 @@ __device__ __forceinline__ void q4_scale(float lo, float hi, bf16& step, bf16& m
     mid = none ? __ushort_as_bfloat16(0x7fffu) : __float2bfloat16_rn(m);
     step = none ? __ushort_as_bfloat16(0x7fffu) : __float2bfloat16_rn(s);
 }
+// What numbers, middle and step of a group are multiplied by before they meet: a power of two with which the step has a reciprocal in float32 (subnormal ones do not), or 0 for a step of 0,
+// whose levels are 0 then.  (A number is less than 2^12 steps in size, where the step is none of the smallest of all: numbers have 8 bits.)
+__device__ __forceinline__ float q4_up(float step) { return step == 0.f ? 0.f : step < 5.421010862427522e-20f ? 18446744073709551616.f : 1.f; }
 // floor((x - mid) / step) within the levels; `by`: 1 / step (0 for a step of 0).  The quotient is rounded to the nearest integer through its last bits; the rest, exact in sign,
 // says whether that lies above it.
 __device__ __forceinline__ int q4_quantise(float x, float step, float mid, float by) {

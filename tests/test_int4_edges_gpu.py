@@ -52,6 +52,22 @@ def test_prompts_over_pages_without_a_value(K, H, G, D):
     p.check(got[some], some, [0] * len(some), q=q[some], halves=True)
 
 
+# ---------------------------------------------------------------------------- appending
+
+@pytest.mark.parametrize("G,D", [(2, 64), (2, 128)])
+def test_rows_whose_steps_are_subnormal(K, G, D):
+    """Groups of numbers down to the smallest that bfloat16 has, whose steps are subnormal."""
+    H, n = 2, 130
+    p = Paged(H, G, D, [n], 141)
+    x = torch.zeros(n, H + 2 * G, D, dtype=torch.float64, device="cuda")
+    for i in range(n):
+        x[i] = torch.randint(-200, 200, (H + 2 * G, D), generator=gen(i), device="cuda").double() * 2.0 ** (-133 + i % 13)
+    x = x.bfloat16()
+    append(K, p, x.view(n, -1), [0], [n])
+    k, v = K.load_int4(p.pool, G, D, ints(list(range(n))), ints([0] * n), p.table, p.width)
+    assert torch.equal(k.double(), plain.stands_for(x[:, H:H + G]).float().double()) and torch.equal(v.double(), plain.stands_for(x[:, H + G:]).float().double())
+
+
 # ---------------------------------------------------------------------------- the part and the engine
 
 @pytest.fixture(scope="module")
