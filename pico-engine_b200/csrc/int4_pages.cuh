@@ -62,11 +62,12 @@ __device__ __forceinline__ void q4_scale(float lo, float hi, bf16& step, bf16& m
 // What numbers, middle and step of a group are multiplied by before they meet: a power of two with which the step has a reciprocal in float32 (subnormal ones do not), or 0 for a step of 0,
 // whose levels are 0 then.  (A number is less than 2^12 steps in size, where the step is none of the smallest of all: numbers have 8 bits.)
 __device__ __forceinline__ float q4_up(float step) { return step == 0.f ? 0.f : step < 5.421010862427522e-20f ? 18446744073709551616.f : 1.f; }
-// floor((x - mid) / step) within the levels; `by`: 1 / step (0 for a step of 0).  The quotient is rounded to the nearest integer through its last bits; the rest, exact in sign,
-// says whether that lies above it.
+// floor((x - mid) / step) within the levels; `by`: 1 / step (0 for a step of 0).  The quotient is rounded to the nearest integer n through its last bits, and is one less where x lies below
+// mid + n step.  That is a float32 without rounding: where they are not 0, 2^-12 < step / mid < 2^7, since numbers have 8 bits, and n has 4.  (x - mid, which float32 rounds where x is far
+// smaller than mid, would not tell the side.)
 __device__ __forceinline__ int q4_quantise(float x, float step, float mid, float by) {
-    const float d = x - mid, r = __fmaf_rn(d, by, 12582912.f), n = r - 12582912.f;
-    const int l = __float_as_int(r) - 0x4b400000 - (__fmaf_rn(-n, step, d) < 0.f ? 1 : 0);
+    const float r = __fmaf_rn(x - mid, by, 12582912.f), n = r - 12582912.f;
+    const int l = __float_as_int(r) - 0x4b400000 - (x < __fmaf_rn(n, step, mid) ? 1 : 0);
     return min(max(l, -8), 7);
 }
 

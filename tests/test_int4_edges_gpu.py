@@ -68,6 +68,22 @@ def test_rows_whose_steps_are_subnormal(K, G, D):
     assert torch.equal(k.double(), plain.stands_for(x[:, H:H + G]).float().double()) and torch.equal(v.double(), plain.stands_for(x[:, H + G:]).float().double())
 
 
+@pytest.mark.parametrize("G,D", [(2, 64), (2, 128)])
+def test_numbers_next_to_a_border_of_two_codes(K, G, D):
+    """Groups of a middle of one and steps of a quarter, and numbers so much smaller than the middle that their difference in float32 lies on a border, whichever side of it they are on."""
+    H, n = 2, 64
+    p = Paged(H, G, D, [n], 145)
+    x = torch.randint(-4, 5, (n, H + 2 * G, D), generator=gen(146), device="cuda").double() * 0.25
+    tiny = torch.rand(x.shape, generator=gen(147), device="cuda") < 0.5
+    sign = torch.randint(0, 2, x.shape, generator=gen(148), device="cuda") * 2 - 1
+    x = torch.where(tiny, sign * 2.0 ** -30, x)
+    x[..., ::32], x[..., 1::32] = 2.875, -0.875
+    x = (x * 2.0 ** torch.randint(-60, 60, (n, 1, 1), generator=gen(149), device="cuda")).bfloat16()
+    append(K, p, x.view(n, -1), [0], [n])
+    k, v = K.load_int4(p.pool, G, D, ints(list(range(n))), ints([0] * n), p.table, p.width)
+    assert torch.equal(k.double(), plain.stands_for(x[:, H:H + G]).float().double()) and torch.equal(v.double(), plain.stands_for(x[:, H + G:]).float().double())
+
+
 # ---------------------------------------------------------------------------- the part and the engine
 
 @pytest.fixture(scope="module")
