@@ -2131,6 +2131,7 @@ def step_tables(slots: torch.Tensor, starts: torch.Tensor, lens: torch.Tensor, h
 INT4_HEAD_DIMS = (64, 128)
 INT4_GROUP = 32               # channels that share a step and a middle
 SELECT_ONE_PAGES = 1024       # PS_ONE_PAGES of csrc/page_select.cu
+_MOST_POSITIONS = 2 ** 31 - 1 # what the kernels hold a position in
 
 
 def int4_takes(dtype: torch.dtype, n_heads: int, n_kv_heads: int, head_dim: int) -> bool:
@@ -2187,7 +2188,13 @@ def _page_rows(block_table: torch.Tensor, table_stride: int) -> int:
     n = block_table.numel()
     if table_stride < 1 or n == 0 or n % table_stride:
         raise KernelError(f"block_table must have rows of {table_stride} pages, not {tuple(block_table.shape)}")
+    _row_pages(table_stride)
     return n // table_stride
+
+
+def _row_pages(pages: int) -> None:
+    if pages > _MOST_POSITIONS // PAGE:
+        raise KernelError(f"a row has at most {_MOST_POSITIONS // PAGE:,} pages, not {pages:,}")
 
 
 def _query_rows(q: torch.Tensor, q_stride: int, T: int, width: int) -> None:
@@ -2281,10 +2288,12 @@ def attention_int4(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int
         out = q.new_empty((T, width))
     else:
         _here(device, (out, "out", torch.bfloat16, (T, width)))
+    window = min(window or 0, _MOST_POSITIONS)
     if window:
         max_context = min(max_context, (window + PAGE - 2) // PAGE * PAGE + PAGE)         # (positions of as many pages as a window can lie on)
+    max_context = min(max_context, _MOST_POSITIONS)
     if T:
-        _attend_int4(q_at, q_stride, out, pool, pool_at, pages, table_at, table_stride, rows, pos_at, row_at, T, n_heads, n_kv_heads, head_dim, window or 0, scale, max_context, 0,
+        _attend_int4(q_at, q_stride, out, pool, pool_at, pages, table_at, table_stride, rows, pos_at, row_at, T, n_heads, n_kv_heads, head_dim, window, scale, max_context, 0,
                      1 if early_pages else 0, device, "attention_int4")
     return out
 
@@ -2309,7 +2318,7 @@ def attention_int4_prompt(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_hea
         out = q.new_empty((n_tokens, width))
     else:
         _here(device, (out, "out", torch.bfloat16, (n_tokens, width)))
-    stream = torch._C._cuda_getCurrentRawStream(device)
+    stream, window = torch._C._cuda_getCurrentRawStream(device), min(window or 0, _MOST_POSITIONS)
     if n_tokens and tiles.shape[0]:
         pages, lib = pool.shape[0], for_head_dim(head_dim)
         # (scratch of the call's own: calls on two streams and captured graphs share none)
@@ -2318,11 +2327,11 @@ def attention_int4_prompt(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_hea
         factors = q.new_empty((pages, n_kv_heads, 2), dtype=torch.float32)
         nbytes = lib.pe_attention_prefill_half_scratch(tiles.shape[0], n_heads, table_stride)
         shares = pool.new_empty(nbytes) if nbytes else None
-        check(long_context().pe_expand_int4(pool.data_ptr(), pages, n_kv_heads, head_dim, tiles.data_ptr(), tiles.shape[0], block_table.data_ptr(), table_stride, rows, window or 0,
+        check(long_context().pe_expand_int4(pool.data_ptr(), pages, n_kv_heads, head_dim, tiles.data_ptr(), tiles.shape[0], block_table.data_ptr(), table_stride, rows, window,
                                             keys.data_ptr(), values.data_ptr(), factors.data_ptr(), stream), "attention_int4_prompt")
         check(lib.pe_attention_prefill_half(
             q.data_ptr(), q_stride, out.data_ptr(), keys.data_ptr(), values.data_ptr(), factors.data_ptr(), pages, block_table.data_ptr(), table_stride, rows, tiles.data_ptr(), tiles.shape[0],
-            n_tokens, n_heads, n_kv_heads, head_dim, window or 0, scale, _ptr(shares), status_ptr(q.device), stream), "attention_int4_prompt", 2 if nbytes else 1)
+            n_tokens, n_heads, n_kv_heads, head_dim, window, scale, _ptr(shares), status_ptr(q.device), stream), "attention_int4_prompt", 2 if nbytes else 1)
     return out
 
 
@@ -2364,6 +2373,8 @@ def select_pages(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int, 
     most = min((max_context - 1) // PAGE + 1, table_stride)
     if keep < 1 or max_context < 1 or most > 10000:
         raise KernelError("keep and max_context must be positive, and a token's pages at most 10,000")
+    _row_pages(keep)
+    max_context = min(max_context, _MOST_POSITIONS)
     n = T * n_kv_heads
     table, pos = tok_pos.new_empty((n, keep)), tok_pos.new_empty(n)
     if T:
@@ -2383,6 +2394,7 @@ def attention_int4_selected(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_h
     q_at, pool_at, pos_at, table_at = _here(device, (q, "q", torch.bfloat16, None), (pool, "pool", torch.uint8, (n_pages, n_kv_heads, n_bytes)),
                                             (pages.pos, "pages.pos", torch.int32, (T * n_kv_heads,)), (pages.table, "pages.table", torch.int32, (places, keep)))
     _query_rows(q, q_stride, T, width)
+    _row_pages(keep)
     if not scale > 0:
         raise KernelError("scale must be positive")
     if out is None:

@@ -84,6 +84,41 @@ def test_numbers_next_to_a_border_of_two_codes(K, G, D):
     assert torch.equal(k.double(), plain.stands_for(x[:, H:H + G]).float().double()) and torch.equal(v.double(), plain.stands_for(x[:, H + G:]).float().double())
 
 
+# ---------------------------------------------------------------------------- arguments
+
+def test_windows_and_contexts_beyond_32_bits(K):
+    """A window or a bound of positions that a 32-bit integer does not hold is one that leaves nothing out."""
+    H, G, D = 14, 2, 64
+    p = Paged(H, G, D, [1500, 300], 151)
+    pos, row = [1499, 299], [0, 1]
+    want = p.attention(K, pos, row)
+    for window in (2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5, 2 ** 40):
+        assert torch.equal(p.attention(K, pos, row, window=window), want)
+    q = randn(1800, H * D, seed=152).bfloat16()
+    tiles = K.prefill_tiles([1500, 300], [0, 0], "cuda", K.PREFILL_TILE_TCGEN05)
+    runs = [K.attention_int4_prompt(q, H * D, H, G, D, p.pool, p.table, p.width, tiles, 1800, w, p.scale) for w in (None, 2 ** 31 - 1, 2 ** 32 + 5, 2 ** 40)]
+    assert all(torch.equal(runs[0], r) for r in runs[1:])
+    for bound in (2 ** 31, 2 ** 32 + 100, 2 ** 40):
+        p.check(p.attention(K, pos, row, bound=bound), pos, row)
+    bounds = bounds_of(p)
+    one, other = (K.select_pages(p.q, p.q.shape[1], H, G, D, bounds, p.table, p.width, ints(pos), ints(row), 5, most) for most in (1500, 2 ** 32 + 100))
+    assert torch.equal(one.table, other.table) and torch.equal(one.pos, other.pos)
+
+
+def test_rows_of_more_positions_than_an_integer_counts(K):
+    from pico_engine.ops import KernelError
+    p = Paged(2, 1, 64, [100], 155)
+    wide = torch.full((1, 1 << 25), -1, dtype=torch.int32, device="cuda")
+    wide[0, :2] = p.table[0, :2]
+    for call in (lambda: K.attention_int4(p.q, p.q.shape[1], 2, 1, 64, p.pool, wide, 1 << 25, ints([99]), ints([0]), None, 1.0, 100),
+                 lambda: K.attention_int4_selected(p.q, p.q.shape[1], 2, 1, 64, p.pool, K.SelectedPages(wide, ints([99])), 1.0)):
+        with pytest.raises(KernelError, match="a row has at most"):
+            call()
+    narrow = wide[:, :(1 << 25) - 1].contiguous()
+    got = K.attention_int4(p.q, p.q.shape[1], 2, 1, 64, p.pool, narrow, narrow.shape[1], ints([99]), ints([0]), None, p.scale, 100)
+    assert torch.equal(got, p.attention(K, [99], [0]))
+
+
 # ---------------------------------------------------------------------------- the part and the engine
 
 @pytest.fixture(scope="module")
