@@ -71,8 +71,11 @@ class Engine:
             store = torch.bfloat16
             load_into(self.model, lambda n: random_tensor(n, expected[n], _seed, store, _draw_on),
                       {n: s.shape for n, s in expected.items()}, "the random weights")
-        if self.int4 and not any(n is not None and n.kv is not None and n.kv.may_be_int4 for n in self.model.cache_needs()):
+        coded = [n.kv for n in self.model.cache_needs() if n is not None and n.kv is not None and n.kv.may_be_int4] if self.int4 else []
+        if self.int4 and not coded:
             raise ValueError("no layer of this model holds its keys and values in 4 bits: grouped attention in bfloat16 with heads of 64 or 128 does")
+        if attend_pages is not None and all(kv.window is not None for kv in coded):
+            raise ValueError("attend_pages has no layer to act on: every layer of this model with a 4-bit cache attends to a window")
         self.max_batch = max_batch
         self.prefill_tokens_per_step = 16384      # prompts of a batch beyond this many tokens are run in several steps
         self._want_tokens = max_tokens_in_cache

@@ -147,3 +147,13 @@ def test_a_prompts_last_piece_of_one_token_attends_to_everything(folder):
     for a, b in zip(logits[None][:3], logits[4][:3]):
         assert torch.equal(a, b)
     assert not torch.equal(logits[None][3], logits[4][3])
+
+
+def test_selection_without_a_layer_that_selects_is_refused(tmp_path):
+    from conftest import TINY_C, make_weights, write_model
+    from pico_engine import Engine
+    cfg = {**TINY_C, "max_position_embeddings": 512, "use_sliding_window": True, "sliding_window": 100, "max_window_layers": 0}
+    path = write_model(tmp_path / "windows", cfg, make_weights(cfg, 5))
+    Engine(path, cache="int4")
+    with pytest.raises(ValueError, match="attend_pages"):
+        Engine(path, cache="int4", attend_pages=4)
