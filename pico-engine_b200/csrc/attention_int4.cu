@@ -713,11 +713,8 @@ namespace {
 inline int ai_allow(const void* kernel, int smem, bool (&done)[64], bool wide) {
     int dev = 0;
     PE_TRY(cudaGetDevice(&dev));
-    if (dev < 64 && done[dev]) return 0;
-    PE_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    if (wide && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) cudaGetLastError();
-    if (dev < 64) done[dev] = true;
-    return 0;
+    if (wide && (dev >= 64 || !done[dev]) && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) cudaGetLastError();
+    return pe_allow_smem(kernel, smem, done);
 }
 
 template <int D, int WARPS>

@@ -48,6 +48,17 @@ inline int pe_sm_count() {
     return n;
 }
 
+// Lets a kernel's launches ask for up to `most` bytes of dynamic shared memory, once a device.  The limit is the kernel's, not a launch's: `most` is what any launch of it may need, so that a
+// call of another thread never lowers it between this one's and its launch.
+inline int pe_allow_smem(const void* kernel, int most, bool (&done)[64]) {
+    int dev = 0;
+    PE_TRY(cudaGetDevice(&dev));
+    if (dev < 64 && done[dev]) return 0;
+    PE_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    if (dev < 64) done[dev] = true;
+    return 0;
+}
+
 inline int& pe_pdl_enabled() { static int on = 1; return on; }
 
 template <typename... KArgs, typename... Args>

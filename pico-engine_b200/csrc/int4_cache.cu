@@ -509,7 +509,8 @@ extern "C" int pe_expand_int4(const void* pool, long long n_pages, int n_kv, int
     if (((uintptr_t)pool | (uintptr_t)keys | (uintptr_t)values | (uintptr_t)tiles) & 15 || ((uintptr_t)factors & 7)) return PE_ERR_UNSUPPORTED;
     auto kernel = hd == 64 ? expand_int4_kernel<64> : expand_int4_kernel<128>;
     const size_t smem = (size_t)(3 * n_rows + 1) * 4;
-    if (smem > 40 * 1024) PE_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    static bool allowed[2][64] = {};
+    { const int e = pe_allow_smem((const void*)kernel, (3 * XI_MAX_ROWS + 1) * 4, allowed[hd == 128]); if (e) return e; }
     PE_TRY(pe_launch(kernel, dim3(pe_sm_count() * 6), dim3(XI_THREADS), smem, (cudaStream_t)stream, (const unsigned char*)pool, (int)n_pages, n_kv, (const int4*)tiles, n_tiles,
                      block_table, table_stride, n_rows, window, (__half*)keys, (__half*)values, (float2*)factors));
     PE_LAUNCH_CHECK();

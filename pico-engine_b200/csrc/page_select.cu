@@ -16,6 +16,7 @@
 
 #define PS_THREADS 256
 #define PS_WARPS (PS_THREADS / 32)
+#define PS_MOST_SMEM (200 * 1024)                              // of a block that selects: twenty bytes a page
 #define PS_ONE_PAGES 1024                                      // up to so many pages a block scores those that it selects from
 
 // a float64 as 64 bits that compare like it; NaN above all
@@ -436,7 +437,7 @@ extern "C" int pe_select_pages(const void* q, int q_stride, int T, int n_heads, 
     const int most = ps_most(max_context, table_stride);
     const size_t smem = (size_t)most * 20;
     const bool one = most <= PS_ONE_PAGES;
-    if (smem > 200 * 1024 || (!one && (((uintptr_t)scratch & 7) || !scratch))) return PE_ERR_UNSUPPORTED;
+    if (smem > PS_MOST_SMEM || (!one && (((uintptr_t)scratch & 7) || !scratch))) return PE_ERR_UNSUPPORTED;
     const PsArgs p = {(const bf16*)q, (const bf16*)bounds, block_table, tok_pos, tok_row, q_stride, n_heads, n_kv, (int)n_pages, table_stride, n_rows, keep, most};
     float2* scores = (float2*)scratch;
     auto kernel = one ? (hd == 64 ? select_pages_kernel<64, true> : select_pages_kernel<128, true>) : hd == 64 ? select_pages_kernel<64, false> : select_pages_kernel<128, false>;
@@ -446,7 +447,8 @@ extern "C" int pe_select_pages(const void* q, int q_stride, int T, int n_heads, 
                          dim3(PS_THREADS), 0, (cudaStream_t)stream, p, scores));
         PE_LAUNCH_CHECK();
     }
-    if (smem > 40 * 1024) PE_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    static bool allowed[4][64] = {};
+    { const int e = pe_allow_smem((const void*)kernel, PS_MOST_SMEM, allowed[2 * (hd == 128) + one]); if (e) return e; }
     PE_TRY(pe_launch(kernel, dim3((unsigned)n_kv, (unsigned)T), dim3(PS_THREADS), smem, (cudaStream_t)stream, p, (const float2*)scores, out_table, out_pos));
     PE_LAUNCH_CHECK();
     return 0;

@@ -119,6 +119,41 @@ def test_rows_of_more_positions_than_an_integer_counts(K):
     assert torch.equal(got, p.attention(K, [99], [0]))
 
 
+def test_calls_of_two_threads(K):
+    """Calls that need little and much shared memory, from two threads at once: neither takes away what the other's launch needs."""
+    from threading import Thread
+    failed = []
+
+    def select(pages, times):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                q, bounds = torch.zeros(1, 128, dtype=torch.bfloat16, device="cuda"), torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16, device="cuda")
+                table = torch.full((1, pages), -1, dtype=torch.int32, device="cuda")
+                for _ in range(times):
+                    K.select_pages(q, 128, 2, 1, 64, bounds, table, pages, ints([64 * pages - 1]), ints([0]), 4, 64 * pages)
+        except Exception as e:                              # noqa: BLE001
+            failed.append(e)
+
+    def prompts(rows, times):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                q, pool = torch.zeros(1, 128, dtype=torch.bfloat16, device="cuda"), K.int4_pool(1, 1, 64, "cuda")
+                table = torch.zeros(rows, 1, dtype=torch.int32, device="cuda")
+                for _ in range(times):
+                    K.attention_int4_prompt(q, 128, 2, 1, 64, pool, table, 1, ints([[rows - 1, 0, 1, 0]]), 1, None, 1.0)
+        except Exception as e:                              # noqa: BLE001
+            failed.append(e)
+
+    for call, small, large in ((select, 2200, 9900), (prompts, 4000, 17900)):
+        threads = [Thread(target=call, args=(n, 1500)) for n in (small, large, small)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+    assert not failed, failed[0]
+
+
 # ---------------------------------------------------------------------------- the part and the engine
 
 @pytest.fixture(scope="module")
