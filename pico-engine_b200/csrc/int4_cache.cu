@@ -9,8 +9,8 @@
 // a 16-bit cache would hold it: what is coded next to the border of two codes then does not depend on the order of two roundings in float32.
 // Keys, values and queries have blocks of their own; a thread takes eight channels.  A word of the keys' codes is one token's, so keys need their group's four threads only.  A word of the
 // values' codes holds four positions: a block takes the values of sixteen tokens of a head as they stand behind one another, and the first of a word's tokens gathers the others from shared
-// memory.  A word keeps the bits of positions that are not in the call; one of a tile that lies across two blocks is changed bit for bit by two atomic operations, so the other block may
-// change its own at the same time.
+// memory.  A word of which it has all positions is stored; of another two atomic operations change the bits of those that it has, so whoever has the rest (another block, or tokens behind a gap
+// of the same one) changes them at the same time.  (Reading and writing the word where nobody else has a part of it: 6.3 us for 64 single tokens appended and read back, so 5.6.)
 // Bound by the latency of a thread's chain of loads (position, angles) with as many threads as an SM holds: 7,541 tokens of 28 + 4 heads x 128 are 73 MB read and 59 MB written in 32.5 us
 // (36.9 us with 1,024 threads an SM, two query heads a thread; 42.6 us with a block's keys and values in its two halves, which waited for one another; 45 us with the queries' blocks in
 // between).  A call for one token takes 3.6 us, which is a launch and one chain of loads.
@@ -86,12 +86,9 @@ __global__ void __launch_bounds__(SI_THREADS, 8) store_int4_kernel(const bf16* q
                                                                 const int* block_table, int table_stride, int n_rows, bf16* q_out, int k_blocks, int v_blocks) {
     using B = Int4Block<D>;
     __shared__ __align__(16) unsigned char fields[SI_TOKENS][D];       // the values' codes: sign << 3 | magnitude
-    __shared__ int near_pos[3 * SI_TOKENS], near_row[3 * SI_TOKENS], at_page[SI_TOKENS];    // of the tokens before the block's, its own and those behind; page -1: not stored
-    const int* const at_pos = near_pos + SI_TOKENS;
-    const int* const at_row = near_row + SI_TOKENS;
+    __shared__ int at_pos[SI_TOKENS], at_row[SI_TOKENS], at_page[SI_TOKENS];                // page -1: not stored
     __shared__ int leaders[SI_TOKENS], n_leaders, parts[SI_TOKENS];     // first tokens of words; the tokens of a leader's four positions (2 f + e), a byte each, 255: not here
     __shared__ unsigned owns[SI_TOKENS];                                // the bits of those
-    __shared__ bool alone[SI_TOKENS];                                   // nobody else has a part of them
     pdl_launch_dependents();
     pdl_wait();
     const int row_width = (n_q + 2 * n_kv) * D;
@@ -142,14 +139,11 @@ __global__ void __launch_bounds__(SI_THREADS, 8) store_int4_kernel(const bf16* q
     }
     // ---- values of sixteen tokens
     const int kvh = (blockIdx.x - k_blocks) % n_kv, first = (int)((blockIdx.x - k_blocks) / n_kv) * SI_TOKENS, i = threadIdx.x / lanes;
-    if (threadIdx.x < 3 * SI_TOKENS) {
-        const int n = threadIdx.x - SI_TOKENS, i = first + n, pos = i >= 0 && i < T ? tok_pos[i] : -1, row = i >= 0 && i < T ? tok_row[i] : -1;
-        near_pos[threadIdx.x] = pos; near_row[threadIdx.x] = row;
-        if (n >= 0 && n < SI_TOKENS) {
-            int page = -1;
-            if (pos >= 0 && row >= 0 && row < n_rows && pos / PE_PAGE < table_stride) page = block_table[(size_t)row * table_stride + pos / PE_PAGE];
-            at_page[n] = page < n_pages ? page : -1;
-        }
+    if (threadIdx.x < SI_TOKENS) {
+        const int n = threadIdx.x, pos = first + n < T ? tok_pos[first + n] : -1, row = first + n < T ? tok_row[first + n] : -1;
+        int page = -1;
+        if (pos >= 0 && row >= 0 && row < n_rows && pos / PE_PAGE < table_stride) page = block_table[(size_t)row * table_stride + pos / PE_PAGE];
+        at_pos[n] = pos; at_row[n] = row; at_page[n] = page < n_pages ? page : -1;
     }
     float x[8];
     const bool mine = i < SI_TOKENS && first + i < T;                  // (of 64 channels half the threads have none: whole warps)
@@ -159,27 +153,19 @@ __global__ void __launch_bounds__(SI_THREADS, 8) store_int4_kernel(const bf16* q
         const int n = threadIdx.x, r = n < SI_TOKENS ? at_pos[n] & 15 : 0;
         bool leads = n < SI_TOKENS && at_page[n] >= 0;
         unsigned own = 0, from = ~0u;
-        // where positions of a tile follow one another with a gap, tokens that lead parts of one word stand where nobody looks for them
-        bool gap = false;
-#pragma unroll
-        for (int k = n + 1; k < 3 * SI_TOKENS; k += 32)
-            gap |= near_row[k] == near_row[k - 1] && near_pos[k] >> 4 == near_pos[k - 1] >> 4 && near_pos[k] != near_pos[k - 1] + 1;
-        bool mine = !__any_sync(0xffffffffu, gap);
         if (leads)
 #pragma unroll
             for (int f = 0; f < 2; ++f)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int to = 8 * f + (r & 6) + e, o = n + to - r;                             // the token of position `to` of the tile
-                    if (at_row[o] != at_row[n] || at_pos[o] != at_pos[n] + to - r) continue;
-                    if (o < 0 || o >= SI_TOKENS) { mine = false; continue; }                        // another block's
-                    if (at_page[o] < 0) continue;
+                    if (o < 0 || o >= SI_TOKENS || at_row[o] != at_row[n] || at_pos[o] != at_pos[n] + to - r || at_page[o] < 0) continue;
                     leads &= to >= r;
                     own |= q4_position_bits(f, e);
                     from &= ~(255u << (8 * (2 * f + e))) | (unsigned)o << (8 * (2 * f + e));
                 }
         const unsigned set = __ballot_sync(0xffffffffu, leads);
-        if (leads) { leaders[__popc(set & ((1u << n) - 1u))] = n; owns[n] = own; parts[n] = (int)from; alone[n] = mine; }
+        if (leads) { leaders[__popc(set & ((1u << n) - 1u))] = n; owns[n] = own; parts[n] = (int)from; }
         if (n == 0) n_leaders = __popc(set);
     }
     if (i < SI_TOKENS) {                                               // (a warp as one: the groups' shuffles)
@@ -216,7 +202,6 @@ __global__ void __launch_bounds__(SI_THREADS, 8) store_int4_kernel(const bf16* q
         unsigned* dst = reinterpret_cast<unsigned*>(pool + ((size_t)at_page[n] * n_kv + kvh) * B::bytes + q4_value_words<D>(p >> 4, m >> 2, g, (p & 7) >> 1)) + (m & 3);
         const unsigned own = owns[n];
         if (own == ~0u) *dst = word;
-        else if (alone[n]) *dst = (*dst & ~own) | word;
         else { atomicAnd(dst, ~own); atomicOr(dst, word); }
     }
 }
