@@ -3,8 +3,10 @@
 // A key is mid + step c per group of 32 channels, c = +-(k + 1/2), so a score is the sum over the groups of step (q . c) + mid (sum of q): products of the queries with codes as they stand, and one
 // more product of the groups' sums with their middles.  A value likewise: o = sum_j (w_j step_j) c_j + w_j mid_j.  The codes are bfloat16 numbers of 2^-129 units (subnormal, which mma.sync
 // keeps exactly), so queries and weights are taken 2^64 higher and sums 2^65 down; the bits of two codes cost two instructions, a rotation and one with a mask, and no conversion.
-// Scores, softmax statistics and results are float32 (running maximum and sum, one pass); a weight is rounded to bfloat16 for its product, and once more behind its
-// multiplication by a value's step: scaling the weights takes a multiplication a group and position, scaling the products would take one a channel and position.
+// Scores, softmax statistics and results are float32 (running maximum and sum, one pass).  The groups' sums of queries keep float32's 24 bits, in three bfloat16 parts, which the product has
+// room for.  A weight is rounded to bfloat16 for its product, and once more behind its multiplication by a value's step: scaling the weights takes a multiplication a group and position, scaling
+// the products would take one a channel and position.  Results are off by 0.0021 of their size for it, of which their own rounding is 0.0017; a second product with what the second rounding
+// leaves brings 0.0019, one with what both leave 0.0017, and the two long cases below then take 70 and 94 us, or 75 and 97, for 65 and 87: the 16 bits a weight of the first form are kept.
 //
 // Keys (or channels) are the 16 rows of mma.sync m16n8k16 and a key head's queries its 8 columns: eight heads of a group are few for tcgen05.mma, whose operands would have to be written
 // to shared memory in 16 bits first.  A warp takes a page and key head at a time, a block of 80 D bytes that one bulk copy brings into its own ring of two, asked for by a warp
@@ -51,7 +53,7 @@ __host__ __device__ constexpr float ai_pow2(int n) { return n >= 0 ? (n == 0 ? 1
 template <int D>
 struct AiQuery {
     unsigned q[D / 16][2];                                     // fragments of 2^64 q, the channels of a group in the order of the keys' words
-    unsigned sums;                                             // of the groups: 2^-65 (sum of q) in two parts, for the product with the middles
+    unsigned sums[D / 64];                                     // of the groups: 2^-65 (sum of q) in three parts, 24 bits, for the product with the middles
 };
 
 template <int D>
@@ -90,12 +92,15 @@ __device__ __forceinline__ void ai_query(AiQuery<D>& f, const bf16* q, bool ther
         sum[b] += __shfl_xor_sync(0xffffffffu, sum[b], 2);
         sum[b] *= ai_pow2(AI_DOWN);
     }
-    // as the product's operand: rows 2 t and 2 t + 1, first the high parts of the groups, then the low ones
-    const int pair = D == 128 ? (t & 1) : 0;
-    const bool low = D == 128 ? t >= 2 : t == 1, none = D == 64 && t >= 2;
-    float a = pair ? sum[NB > 2 ? 2 : 0] : sum[0], b = pair ? sum[NB > 2 ? 3 : 1] : sum[1];
-    if (low) { a -= __bfloat162float(__float2bfloat16_rn(a)); b -= __bfloat162float(__float2bfloat16_rn(b)); }
-    f.sums = none ? 0u : ai_pack(a, b);
+    // as the product's operand, a pair of groups a register: the high parts, behind them what those leave, then what these leave (of 64 channels rows 2 t and 2 t + 1, t the part; of 128
+    // t & 1 the pair, t / 2 the part, and the third parts in the second half of the rows)
+    const int pair = D == 128 ? (t & 1) : 0, part = D == 128 ? t >> 1 : t;
+    float a[3], b[3];
+    a[0] = pair ? sum[NB > 2 ? 2 : 0] : sum[0]; b[0] = pair ? sum[NB > 2 ? 3 : 1] : sum[1];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) { a[i + 1] = a[i] - __bfloat162float(__float2bfloat16_rn(a[i])); b[i + 1] = b[i] - __bfloat162float(__float2bfloat16_rn(b[i])); }
+    f.sums[0] = part == 0 ? ai_pack(a[0], b[0]) : part == 1 ? ai_pack(a[1], b[1]) : part == 2 ? ai_pack(a[2], b[2]) : 0u;
+    if constexpr (D == 128) f.sums[1] = part == 0 ? ai_pack(a[2], b[2]) : 0u;
 }
 
 // Positions of a block that are not seen (below lo, above hi) may hold anything: their values' steps and middles become zero, in the warp's own copy.
@@ -135,7 +140,8 @@ __device__ __forceinline__ void ai_scores(float (&sc)[4][4], const AiQuery<D>& f
                 words[r][0] = v.x; words[r][1] = v.y; steps[r][0] = st.x; mid[r] = st.y;
             }
         }
-        ai_mma8(sc[j], mid[0], mid[1], f.sums);
+        if constexpr (D == 128) ai_mma0(sc[j], mid[0], mid[1], mid[0], mid[1], f.sums[0], f.sums[1]);
+        else ai_mma8(sc[j], mid[0], mid[1], f.sums[0]);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             float c[4];

@@ -2273,7 +2273,7 @@ def attention_int4(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int
     ``window`` of them).  ``max_context`` bounds every token's position + 1 and fixes the launch shape.  With ``early_pages`` the kernel copies pages while the two kernels before it on the
     stream may still run: they must have written, of the cache, no page but each token's own, and neither positions nor page tables.
 
-    Scores are sums of exact products of the queries with codes, in float32; steps and middles join in float32.  Weights are rounded to bfloat16 for the product with
+    Scores are sums of exact products of the queries with codes, in float32; steps and middles join in float32 (sums of queries in 24 bits).  Weights are rounded to bfloat16 for the product with
     the values, and once more behind their multiplication by a value's step.  Queries, keys and values of sizes between 2^-40 and 2^60 keep that: the products with codes are taken in units
     of 2^-65.  A row that sees nothing is zeros; one that sees a group that is no number is none where that reaches."""
     T, n_bytes, device, width = tok_pos.shape[0], _int4_heads(n_heads, n_kv_heads, head_dim), _device_here(q, "q"), n_heads * head_dim

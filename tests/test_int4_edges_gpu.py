@@ -154,6 +154,36 @@ def test_calls_of_two_threads(K):
     assert not failed, failed[0]
 
 
+# ---------------------------------------------------------------------------- tokens
+
+@pytest.mark.parametrize("H,G,D", [(6, 2, 64), (14, 1, 128)])
+@pytest.mark.parametrize("bound", [200, 1 << 21])
+def test_sums_of_queries_keep_the_bits_of_float32(K, H, G, D, bound):
+    """Scores that are the small difference of large products of middles with sums of queries: 128.25 and a few 2^-12 times 8,192, less 128.25 times 8,192."""
+    p = Paged(H, G, D, [150, 70], 171)
+    keys = torch.zeros_like(p.keys)
+    keys[:, :, ::2, :32], keys[:, :, ::2, 32:64] = 8192.0, -8192.0
+    if D == 128:
+        keys[:, :, 1::2, 64:96], keys[:, :, 1::2, 96:] = -8192.0, 8192.0
+    p.pool = plain.pack(keys.view(-1, 64, D), p.values.view(-1, 64, D)).view(p.n_pages, G, 80 * D)
+    q = torch.zeros(2, H, D, device="cuda")
+    for b in range(0, D, 32):
+        q[..., b], q[..., b + 9] = 128.0, 0.25
+    extra = torch.tensor([(1 + h % 3) * 2.0 ** -12 for h in range(H)], device="cuda")
+    q[..., 17], q[1, :, D - 5] = extra, 2 * extra                             # in the first group, and in the last one's too
+    q = q.bfloat16().view(2, H * D)
+    got = K.attention_int4(q, H * D, H, G, D, p.pool, p.table, p.width, ints([149, 69]), ints([0, 1]), None, 0.5, bound).double().view(2, H, D)
+    for t, n in enumerate((150, 70)):
+        blocks = p.pool[p.table[t, :n // 64 + 1].long()]
+        k, v, part, _ = (x.view(-1, G, 64, D).transpose(0, 1).reshape(G, -1, D)[:, :n] for x in plain.unpack(blocks.flatten(0, 1)))
+        for h in range(H):
+            g = h * G // H
+            w = torch.softmax(k[g] @ q[t].double().view(H, D)[h] * 0.5, 0)
+            # sums and scores have no rounding here; weights are rounded (on v), once more behind a step, and the result
+            bound_of = 2.0 ** -8 * (w @ (v[g].abs() + part[g].abs()) + (w @ v[g]).abs()) + 2.0 ** -18
+            assert ((got[t, h] - w @ v[g]).abs() <= bound_of).all(), (t, h)
+
+
 # ---------------------------------------------------------------------------- the part and the engine
 
 @pytest.fixture(scope="module")
