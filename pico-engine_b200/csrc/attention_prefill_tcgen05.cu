@@ -548,9 +548,9 @@ static int at_launch(const void* q, int q_stride, void* out, const void* k_pool,
 }
 
 // Into how many shares the steps of a run and head are cut, where all runs and heads together are fewer than the SMs: the number whose last wave ends first, a step taken for
-// 1 and the rest of a CTA for 5 (0.93 us and 4.3).  500 tokens on 15,937 positions, 14 heads of 64: 56 CTAs of 128 steps, 130 us in one share, 80 us in five.
-static int at_splits(long long ctas, int table_stride) {
-    const int steps = (table_stride + 1) / 2, sms = pe_sm_count();
+// 1 and the rest of a CTA for 5 (0.93 us and 4.3).  `pages`: what a run sees at most.  500 tokens on 15,937 positions, 14 heads of 64: 56 CTAs of 128 steps, 130 us in one share, 80 us in five.
+static int at_splits(long long ctas, int pages) {
+    const int steps = (pages + 1) / 2, sms = pe_sm_count();
     int best = 1;
     double least = 1e30;
     for (int s = 1; s <= 8 && (s == 1 || s * AT_LEAST_STEPS * 4 <= steps); ++s) {
@@ -569,18 +569,18 @@ extern "C" int pe_attention_prefill_tcgen05(const void* q, int q_stride, void* o
 }
 
 // Bytes of scratch that the next one needs (0: none).
-extern "C" long long pe_attention_prefill_half_scratch(int n_tiles, int nh, int table_stride) {
+extern "C" long long pe_attention_prefill_half_scratch(int n_tiles, int nh, int row_pages) {
     const long long ctas = (long long)n_tiles * nh;
-    const int s = ctas > 0 ? at_splits(ctas, table_stride) : 1;
+    const int s = ctas > 0 ? at_splits(ctas, row_pages) : 1;
     return s > 1 ? ctas * s * AT_QTILE * AT_PARTIAL_ROW * 4 : 0;
 }
 
 // The same over float16 keys and values with their pages' powers of two, factors[page][kv head].
 extern "C" int pe_attention_prefill_half(const void* q, int q_stride, void* out, const void* k_pool, const void* v_pool, const void* factors, long long pool_pages,
-                                              const int* block_table, int table_stride, int n_rows, const void* tiles, int n_tiles, int n_tokens, int nh, int nkv, int hd, int window,
+                                              const int* block_table, int table_stride, int row_pages, int n_rows, const void* tiles, int n_tiles, int n_tokens, int nh, int nkv, int hd, int window,
                                               float scale, void* scratch, int* status, void* stream) {
     if (!factors || ((uintptr_t)factors & 7) || ((uintptr_t)scratch & 15)) return PE_ERR_UNSUPPORTED;
-    const int splits = scratch ? at_splits((long long)n_tiles * nh, table_stride) : 1;
+    const int splits = scratch ? at_splits((long long)n_tiles * nh, row_pages) : 1;
     return (splits > 1 ? at_launch<true, true> : at_launch<true, false>)(q, q_stride, out, k_pool, v_pool, pool_pages, block_table, table_stride, tiles, n_tiles, n_tokens, nh, nkv, hd, window,
                                                                          scale, 0, nullptr, status, stream, nullptr, (const float2*)factors, splits, (float*)scratch, n_rows);
 }
@@ -594,7 +594,7 @@ extern "C" int pe_attention_prefill_tcgen05(const void*, int, void*, const void*
     return PE_ERR_UNSUPPORTED;
 }
 extern "C" long long pe_attention_prefill_half_scratch(int, int, int) { return 0; }
-extern "C" int pe_attention_prefill_half(const void*, int, void*, const void*, const void*, const void*, long long, const int*, int, int, const void*, int, int, int, int, int, int,
+extern "C" int pe_attention_prefill_half(const void*, int, void*, const void*, const void*, const void*, long long, const int*, int, int, int, const void*, int, int, int, int, int, int,
                                               float, void*, int*, void*) {
     return PE_ERR_UNSUPPORTED;
 }

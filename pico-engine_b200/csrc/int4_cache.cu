@@ -351,13 +351,15 @@ extern "C" int pe_page_bounds(const void* pool, long long n_pages, int n_kv, int
 // would not keep the value out of its sum).  Expanded once a page and head, for all heads and runs that read it.
 // Bound by its writes: 7,541 tokens of 4 heads of 128 (and the 4,071 in front of a run of theirs) 7.5 MB read and 24 MB written, 10 to 11 us.
 // A block counts the pages of all rows from the runs, then takes every gridDim.x-th of them.
+// A page's numbers lie at its own place of a scratch as large as the pool, or, where rows times `row_pages` are fewer, at place row * row_pages + j of one of so many, which `places` says
+// instead of the page table: a prompt on a large cache asks for no more than its rows can see.
 
 #define XI_MAX_ROWS 18000                                     // twelve bytes each of shared memory
 #define XI_THREADS 256
 
 template <int D>
 __global__ void __launch_bounds__(XI_THREADS) expand_int4_kernel(const unsigned char* pool, int n_pages, int n_kv, const int4* tiles, int n_tiles, const int* block_table, int table_stride,
-                                                                 int n_rows, int window, __half* keys, __half* values, float2* factors) {
+                                                                 int n_rows, int window, int row_pages, int* places, __half* keys, __half* values, float2* factors) {
     using B = Int4Block<D>;
     extern __shared__ int xi_rows[];                           // a row's first page, the position behind its last run, the pages of the rows before it
     int* const low = xi_rows;
@@ -375,7 +377,7 @@ __global__ void __launch_bounds__(XI_THREADS) expand_int4_kernel(const unsigned 
         const int4 run = tiles[i];                             // row, first token, tokens, position
         if (run.x < 0 || run.x >= n_rows || run.z <= 0 || run.w < 0) continue;
         atomicMin(&low[run.x], (window > 0 ? max(0, run.w - window + 1) : 0) / PE_PAGE);
-        atomicMax(&behind[run.x], min(run.w + run.z, table_stride * PE_PAGE));
+        atomicMax(&behind[run.x], min(run.w + run.z, row_pages * PE_PAGE));
     }
     __syncthreads();
     if (warp == 0) {
@@ -397,9 +399,12 @@ __global__ void __launch_bounds__(XI_THREADS) expand_int4_kernel(const unsigned 
         int row = 0, top = n_rows;
         while (top - row > 1) { const int mid = (row + top) >> 1; if (before[mid] <= x) row = mid; else top = mid; }
         const int j = low[row] + x - before[row], page = block_table[(size_t)row * table_stride + j];
-        if (page < 0 || page >= n_pages) continue;             // (the same for the whole block)
+        const bool held = page >= 0 && page < n_pages;
+        const int place = places ? row * row_pages + j : page;
+        if (places && kvh == 0 && threadIdx.x == 0) places[place] = held ? place : -1;
+        if (!held) continue;                                   // (the same for the whole block)
         int there = min(PE_PAGE, behind[row] - j * PE_PAGE);
-        if (there < PE_PAGE) {
+        if (there < PE_PAGE && !places) {
             // another row that has the page may see further into it: its block writes the same
             for (int r = threadIdx.x; r < n_rows; r += XI_THREADS)
                 if (low[r] <= j && behind[r] > j * PE_PAGE + there && block_table[(size_t)r * table_stride + j] == page) there = min(PE_PAGE, behind[r] - j * PE_PAGE);
@@ -410,8 +415,8 @@ __global__ void __launch_bounds__(XI_THREADS) expand_int4_kernel(const unsigned 
 #pragma unroll
             for (int w = 0; w < XI_THREADS / 32; ++w) there = max(there, further[w]);
         }
-        const size_t at = (size_t)page * n_kv + kvh;
-        const unsigned char* block = pool + at * B::bytes;
+        const size_t at = (size_t)place * n_kv + kvh;
+        const unsigned char* block = pool + ((size_t)page * n_kv + kvh) * B::bytes;
         // the largest key and value that the page's steps and middles allow
         float most = 0.f, most_v = 0.f;
         for (int i = threadIdx.x; i < there * B::groups; i += XI_THREADS) {
@@ -488,16 +493,18 @@ __global__ void __launch_bounds__(XI_THREADS) expand_int4_kernel(const unsigned 
 }
 
 extern "C" int pe_expand_int4(const void* pool, long long n_pages, int n_kv, int hd, const int* tiles, int n_tiles, const int* block_table, int table_stride, int n_rows, int window,
-                              void* keys, void* values, void* factors, void* stream) {
+                              int row_pages, int* places, void* keys, void* values, void* factors, void* stream) {
     if (n_tiles <= 0) return 0;
-    if ((hd != 64 && hd != 128) || n_kv <= 0 || n_rows < 1 || n_rows > XI_MAX_ROWS || n_pages * n_kv > 0x7fffffffll) return PE_ERR_UNSUPPORTED;
+    if ((hd != 64 && hd != 128) || n_kv <= 0 || n_rows < 1 || n_rows > XI_MAX_ROWS || n_pages * n_kv > 0x7fffffffll || row_pages < 1 || row_pages > table_stride ||
+        (long long)n_rows * row_pages > 0x7fffffffll)
+        return PE_ERR_UNSUPPORTED;
     if (((uintptr_t)pool | (uintptr_t)keys | (uintptr_t)values | (uintptr_t)tiles) & 15 || ((uintptr_t)factors & 7)) return PE_ERR_UNSUPPORTED;
     auto kernel = hd == 64 ? expand_int4_kernel<64> : expand_int4_kernel<128>;
     const size_t smem = (size_t)(3 * n_rows + 1) * 4;
     static bool allowed[2][64] = {};
     { const int e = pe_allow_smem((const void*)kernel, (3 * XI_MAX_ROWS + 1) * 4, allowed[hd == 128]); if (e) return e; }
     PE_TRY(pe_launch(kernel, dim3(pe_sm_count() * 6), dim3(XI_THREADS), smem, (cudaStream_t)stream, (const unsigned char*)pool, (int)n_pages, n_kv, (const int4*)tiles, n_tiles,
-                     block_table, table_stride, n_rows, window, (__half*)keys, (__half*)values, (float2*)factors));
+                     block_table, table_stride, n_rows, window, row_pages, places, (__half*)keys, (__half*)values, (float2*)factors));
     PE_LAUNCH_CHECK();
     return 0;
 }

@@ -2299,11 +2299,13 @@ def attention_int4(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int
 
 
 def attention_int4_prompt(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int, head_dim: int, pool: torch.Tensor, block_table: torch.Tensor, table_stride: int,
-                          tiles: torch.Tensor, n_tokens: int, window: Optional[int], scale: float, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                          tiles: torch.Tensor, n_tokens: int, window: Optional[int], scale: float, out: Optional[torch.Tensor] = None,
+                          max_context: Optional[int] = None) -> torch.Tensor:
     """The same for runs of at most 128 tokens of a sequence, ``tiles`` int32 [n, 4] (``prefill_tiles`` with ``PREFILL_TILE_TCGEN05``), whose own keys and values the cache holds already;
-    ``q`` has ``n_tokens`` rows.  The pages that the runs see are expanded to 16 bits first, once a page and key head (scratch of the call, as large as one layer of a 16-bit cache: float16 numbers
-    with a power of two for each page's keys and values), and the products, with weights in float16, run on the tensor cores.  A page table has at most 18,000 rows; a page that several of them
-    have stands at the same place of each.  A token that sees a key or value with a
+    ``q`` has ``n_tokens`` rows.  ``max_context`` bounds every token's position + 1 (None: the page table does) and fixes the launch shape.  The pages that the runs see are expanded to 16 bits
+    first (float16 numbers with a power of two for each page's keys and values), and the products, with weights in float16, run on the tensor cores.  The expanded pages are scratch of the call,
+    as large as in a 16-bit cache: a page for each of ``max_context`` and row of the table, or for each of the pool's where these are fewer.  A page table has at most 18,000 rows; a page that
+    several of them have stands at the same place of each.  A token that sees a key or value with a
     group that is no number has no number in the head's results."""
     n_bytes, device, width = _int4_heads(n_heads, n_kv_heads, head_dim), _device_here(q, "q"), n_heads * head_dim
     _here(device, (q, "q", torch.bfloat16, None), (tiles, "tiles", torch.int32, (tiles.shape[0], 4)), (pool, "pool", torch.uint8, (pool.shape[0], n_kv_heads, n_bytes)),
@@ -2312,6 +2314,8 @@ def attention_int4_prompt(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_hea
     rows = _page_rows(block_table, table_stride)
     if (window is not None and window < 0) or not scale > 0:
         raise KernelError("scale must be positive, and a window not negative")
+    if max_context is not None and max_context < 1:
+        raise KernelError("max_context must be positive")
     if rows > 18000:
         raise KernelError(f"prompts over a 4-bit cache take page tables of at most 18,000 rows, not {rows}")
     if out is None:
@@ -2321,17 +2325,22 @@ def attention_int4_prompt(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_hea
     stream, window = torch._C._cuda_getCurrentRawStream(device), min(window or 0, _MOST_POSITIONS)
     if n_tokens and tiles.shape[0]:
         pages, lib = pool.shape[0], for_head_dim(head_dim)
+        row_pages = table_stride if max_context is None else min(table_stride, (max_context - 1) // PAGE + 1)
+        by_row = rows * row_pages < pages                    # the expanded pages lie row by row, and a table of the call's own says where
+        expanded = rows * row_pages if by_row else pages
         # (scratch of the call's own: calls on two streams and captured graphs share none)
-        keys = q.new_empty((pages, n_kv_heads, PAGE, head_dim), dtype=torch.float16)
+        places = block_table.new_empty(expanded) if by_row else None
+        keys = q.new_empty((expanded, n_kv_heads, PAGE, head_dim), dtype=torch.float16)
         values = torch.empty_like(keys)
-        factors = q.new_empty((pages, n_kv_heads, 2), dtype=torch.float32)
-        nbytes = lib.pe_attention_prefill_half_scratch(tiles.shape[0], n_heads, table_stride)
+        factors = q.new_empty((expanded, n_kv_heads, 2), dtype=torch.float32)
+        nbytes = lib.pe_attention_prefill_half_scratch(tiles.shape[0], n_heads, row_pages)
         shares = pool.new_empty(nbytes) if nbytes else None
         check(long_context().pe_expand_int4(pool.data_ptr(), pages, n_kv_heads, head_dim, tiles.data_ptr(), tiles.shape[0], block_table.data_ptr(), table_stride, rows, window,
-                                            keys.data_ptr(), values.data_ptr(), factors.data_ptr(), stream), "attention_int4_prompt")
+                                            row_pages, _ptr(places), keys.data_ptr(), values.data_ptr(), factors.data_ptr(), stream), "attention_int4_prompt")
         check(lib.pe_attention_prefill_half(
-            q.data_ptr(), q_stride, out.data_ptr(), keys.data_ptr(), values.data_ptr(), factors.data_ptr(), pages, block_table.data_ptr(), table_stride, rows, tiles.data_ptr(), tiles.shape[0],
-            n_tokens, n_heads, n_kv_heads, head_dim, window, scale, _ptr(shares), status_ptr(q.device), stream), "attention_int4_prompt", 2 if nbytes else 1)
+            q.data_ptr(), q_stride, out.data_ptr(), keys.data_ptr(), values.data_ptr(), factors.data_ptr(), expanded, (places if by_row else block_table).data_ptr(),
+            row_pages if by_row else table_stride, row_pages, rows, tiles.data_ptr(), tiles.shape[0], n_tokens, n_heads, n_kv_heads, head_dim, window, scale,
+            _ptr(shares), status_ptr(q.device), stream), "attention_int4_prompt", 2 if nbytes else 1)
     return out
 
 

@@ -148,7 +148,7 @@ _LONG_SIGNATURES = {
     "pe_page_bounds": [P, LL, I, I, P, P, I, P, I, I, P, P],
     "pe_select_pages": [P, I, I, I, I, I, P, LL, P, I, I, P, P, I, I, P, P, P, P],
     "pe_attention_int4": [P, I, P, P, LL, P, I, I, P, P, I, I, I, I, I, F, I, I, I, P, P, P],
-    "pe_expand_int4": [P, LL, I, I, P, I, P, I, I, I, P, P, P, P],
+    "pe_expand_int4": [P, LL, I, I, P, I, P, I, I, I, I, P, P, P, P, P],
 }
 
 _HEAD_DIM_SIGNATURES = {
@@ -156,7 +156,7 @@ _HEAD_DIM_SIGNATURES = {
     "pe_attention_decode": [P, I, P, P, P, P, I, P, P, I, I, I, I, I, F, I, I, P, P, I, P, P],
     "pe_attention_decode_splits": [I, I, I, I, P],
     "pe_attention_prefill": [P, I, P, P, P, P, I, P, P, P, I, I, I, I, I, F, P],
-    "pe_attention_prefill_half": [P, I, P, P, P, P, LL, P, I, I, P, I, I, I, I, I, I, F, P, P, P],
+    "pe_attention_prefill_half": [P, I, P, P, P, P, LL, P, I, I, I, P, I, I, I, I, I, I, F, P, P, P],
     "pe_attention_prefill_tcgen05": [P, I, P, P, P, LL, P, I, P, I, I, I, I, I, I, F, I, P, P, P, P],
 }
 

@@ -86,7 +86,7 @@ class GQAAttention(Mixer):
             tiles = ctx.scratch.get("prefill_tiles_128")
             if tiles is None:
                 tiles = ctx.scratch["prefill_tiles_128"] = kernels.prefill_tiles(ctx.lens, ctx.starts, q.device, kernels.PREFILL_TILE_TCGEN05)
-            return kernels.attention_int4_prompt(*heads, kv.k, *place, tiles, ctx.T, s.window, s.scale)
+            return kernels.attention_int4_prompt(*heads, kv.k, *place, tiles, ctx.T, s.window, s.scale, max_context=ctx.max_context)
         if kv.bounds is not None and ctx.attend_pages is not None and ctx.max_context > ctx.attend_pages * kernels.PAGE:
             pages = kernels.select_pages(*heads, kv.bounds, *place, ctx.tok_pos, ctx.tok_row, ctx.attend_pages, ctx.max_context)
             return kernels.attention_int4_selected(*heads, kv.k, pages, s.scale)

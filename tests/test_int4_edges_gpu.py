@@ -52,6 +52,60 @@ def test_prompts_over_pages_without_a_value(K, H, G, D):
     p.check(got[some], some, [0] * len(some), q=q[some], halves=True)
 
 
+@pytest.mark.parametrize("H,G,D", [(14, 2, 64), (28, 4, 128)])
+@pytest.mark.parametrize("window", [None, 100])
+def test_expanded_pages_lie_by_row_or_by_page(K, H, G, D, window):
+    """A prompt on a pool of many pages expands what its rows can see, one on a wide table the pool's: results are the same, with a bound of the positions too."""
+    starts, lens = [0, 700, 130], [300, 129, 1]
+    p = Paged(H, G, D, [s + n for s, n in zip(starts, lens)], 181, rubbish=float("nan"))
+    T, tiles = sum(lens), K.prefill_tiles(lens, starts, "cuda", K.PREFILL_TILE_TCGEN05)
+    q = randn(T, H * D, seed=182).bfloat16()
+    many = torch.cat([p.pool, torch.full((1500, G, 80 * D), 255, dtype=torch.uint8, device="cuda")])
+    wide = torch.full((3, 900), -1, dtype=torch.int32, device="cuda")
+    wide[:, :p.width] = p.table
+    run = lambda pool, table, most=None: K.attention_int4_prompt(q, H * D, H, G, D, pool, table, table.shape[1], tiles, T, window, p.scale, max_context=most)     # noqa: E731
+    by_page, by_row = run(p.pool, p.table), run(many, p.table)
+    pos, row = [s + i for s, n in zip(starts, lens) for i in range(n)], [b for b, n in enumerate(lens) for _ in range(n)]
+    some = sorted(set(range(0, T, 37)) | {T - 1, T - 2, 299, 300})
+    for got in (by_page, by_row, run(p.pool, wide), run(many, wide), run(many, wide, 829), run(many, wide, 1 << 40)):
+        p.check(got[some], [pos[i] for i in some], [row[i] for i in some], q=q[some], window=window, halves=True)
+    assert torch.equal(run(many, wide, 829), by_row)
+
+
+def test_a_short_prompt_on_a_large_cache_asks_for_little_memory(K):
+    H, G, D = 4, 2, 64
+    pool = K.int4_pool(20000, G, D, "cuda")
+    q, table = randn(33, H * D, seed=1).bfloat16(), torch.full((1, 512), -1, dtype=torch.int32, device="cuda")
+    table[0, 0] = 19999
+    tiles = K.prefill_tiles([33], [0], "cuda", K.PREFILL_TILE_TCGEN05)
+    K.attention_int4_prompt(q, H * D, H, G, D, pool, table, 512, tiles, 33, None, 1.0)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = K.attention_int4_prompt(q, H * D, H, G, D, pool, table, 512, tiles, 33, None, 1.0, max_context=64)
+    page = G * 64 * D * 4                                                    # of keys and values in 16 bits
+    assert torch.cuda.max_memory_allocated() - before <= page + out.numel() * 2 + 16384
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    K.attention_int4_prompt(q, H * D, H, G, D, pool, table, 512, tiles, 33, None, 1.0)
+    assert torch.cuda.max_memory_allocated() - before <= 600 * page
+
+
+def test_expanded_pages_beyond_four_gigabytes(K):
+    """A table of more places than the pool has pages: every page of the pool has its place in the scratch, those behind the four billionth byte too."""
+    H, G, D, n = 16, 8, 128, 1500
+    p = Paged(H, G, D, [n], 191)
+    far = 40000
+    pool = torch.cat([torch.zeros(far, G, 80 * D, dtype=torch.uint8, device="cuda"), p.pool])
+    table = torch.full((2000, p.width), -1, dtype=torch.int32, device="cuda")
+    table[1999] = torch.where(p.table[0] >= 0, p.table[0] + far, p.table[0])
+    assert table.numel() > pool.shape[0] and pool.shape[0] * G * 64 * D * 2 > 1 << 32
+    q, tiles = randn(n, H * D, seed=192).bfloat16(), K.prefill_tiles([n], [0], "cuda", K.PREFILL_TILE_TCGEN05)
+    want = K.attention_int4_prompt(q, H * D, H, G, D, p.pool, p.table, p.width, tiles, n, None, p.scale)
+    tiles[:, 0] = 1999
+    assert torch.equal(K.attention_int4_prompt(q, H * D, H, G, D, pool, table, p.width, tiles, n, None, p.scale), want)
+
+
 # ---------------------------------------------------------------------------- appending
 
 @pytest.mark.parametrize("G,D", [(2, 64), (2, 128)])
