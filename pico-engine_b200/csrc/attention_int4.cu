@@ -807,11 +807,26 @@ static bool ai_streams(int T, int n_heads, int n_kv, int hd, int max_context, in
     return (selected || window > 0) && pairs > sms && 4 * ((pairs + sms - 1) / sms) * (16 + pages) * sms >= 200 * sms + 5 * pairs * pages;
 }
 
+// How a call's blocks are dealt out: 2 equal runs for all warps, 1 and 0 one CTA or cluster a pair.
+// Form 1, seven warps, of which two CTAs share an SM, where pairs are few and each is cut over many CTAs (one row of 14 heads on 4,096 positions 4.5 us, with fifteen 5.6), but not where one
+// CTA's warps have a page each (500 positions 3.6, with seven 3.9); else as many as the registers allow (64 rows of 1,000 to 2,000 7.3, with seven 8.9).
+// The form goes by the bound of the positions that the call states: stated far too high it costs up to twice the time (64 rows of 1,000, 14 heads of 64 on 2, us: stated as 1,000 to 16,384
+// 5.4, as 32,768 12.9).
+static int ai_form(int T, int n_heads, int n_kv, int hd, int max_context, int selected, int window) {
+    if (ai_streams(T, n_heads, n_kv, hd, max_context, selected, window)) return 2;
+    return (long long)T * n_kv * ((n_heads / n_kv + 7) / 8) <= 8 && (max_context - 1) / PE_PAGE + 1 > (hd == 64 ? 15 : 11);
+}
+
 extern "C" void pe_set_pdl(int on) { pe_pdl_enabled() = on ? 1 : 0; }
+
+// The form of a call; -1: sizes that no call takes.
+extern "C" int pe_attention_int4_form(int T, int n_heads, int n_kv, int hd, int max_context, int selected, int window) {
+    return T <= 0 || n_kv <= 0 || n_heads % n_kv || (hd != 64 && hd != 128) ? -1 : ai_form(T, n_heads, n_kv, hd, max_context, selected, window);
+}
 
 // Bytes of scratch that a call needs (0: none).
 extern "C" long long pe_attention_int4_scratch(int T, int n_heads, int n_kv, int hd, int max_context, int selected, int window) {
-    if (T <= 0 || n_kv <= 0 || n_heads % n_kv || (hd != 64 && hd != 128) || !ai_streams(T, n_heads, n_kv, hd, max_context, selected, window)) return 0;
+    if (pe_attention_int4_form(T, n_heads, n_kv, hd, max_context, selected, window) != 2) return 0;
     const int places = selected ? T * n_kv : T;
     return hd == 64 ? AiStreamLaunch<64>::scratch(places) : AiStreamLaunch<128>::scratch(places);
 }
@@ -829,7 +844,8 @@ extern "C" int pe_attention_int4(const void* q, int q_stride, void* out, const v
     early = early && !selected;
     const AiPlaces p = {tok_pos, tok_row, block_table, selected ? T * n_kv : T, table_stride, n_rows, (int)(selected ? n_blocks : n_blocks / n_kv), n_kv, n_heads, head_tiles, window, selected};
     const float scale_log2e = scale * 1.4426950408889634f;
-    if (scratch && ai_streams(T, n_heads, n_kv, hd, max_context, selected, window) && (long long)T * n_kv * head_tiles * table_stride <= 0x7fffffffll) {
+    const int form = ai_form(T, n_heads, n_kv, hd, max_context, selected, window);
+    if (scratch && form == 2 && (long long)T * n_kv * head_tiles * table_stride <= 0x7fffffffll) {
         const auto go = [&](auto v) {
             return decltype(v)::go(p, (const bf16*)q, q_stride, (const unsigned char*)pool, scale_log2e, early, scratch, status, (bf16*)out, (cudaStream_t)stream);
         };
@@ -838,9 +854,6 @@ extern "C" int pe_attention_int4(const void* q, int q_stride, void* out, const v
     const auto go = [&](auto v) {
         return decltype(v)::go(p, T, pages, (const bf16*)q, q_stride, (const unsigned char*)pool, scale_log2e, early, status, (bf16*)out, (cudaStream_t)stream);
     };
-    // Seven warps, of which two CTAs share an SM, where pairs are few and each is cut over many CTAs (one row of 14 heads on 4,096 positions 4.5 us, with fifteen 5.6), but not where one
-    // CTA's warps have a page each (500 positions 3.6, with seven 3.9); else as many as the registers allow (64 rows of 1,000 to 2,000 7.3, with seven 8.9).
-    const bool few = (long long)T * n_kv * head_tiles <= 8;
-    if (hd == 64) return few && pages > 15 ? go(AiLaunch<64, 7>()) : go(AiLaunch<64, 15>());
-    return few && pages > 11 ? go(AiLaunch<128, 7>()) : go(AiLaunch<128, 11>());
+    if (hd == 64) return form == 1 ? go(AiLaunch<64, 7>()) : go(AiLaunch<64, 15>());
+    return form == 1 ? go(AiLaunch<128, 7>()) : go(AiLaunch<128, 11>());
 }

@@ -242,17 +242,19 @@ class EngineBackend:
     MAX_GRAPHS = 24      # captured decode steps an engine keeps (each holds its buffers); the least recently used goes
 
     def _graph(self, slots) -> GraphedDecode:
-        """The captured step for so many rows: one per bucket of rows, kind of sampling and of rules, and whether shared pages are read once.
+        """The captured step for so many rows: one per bucket of rows, kind of sampling and of rules, whether shared pages are read once, and, over 4-bit pages, what suits the longest row.
         Temperature, top-k, top-p, seed, penalties and biases are numbers the graph reads at run time, so calls that vary them share it."""
         shared = self.e.stepper.sharing_pays(slots)
-        key = (bucket_rows(len(slots)), self.sampler.kind(self.e.model.plan.vocab_size), self.sampler.rule_kind(), shared)
+        rows = bucket_rows(len(slots))
+        context = self.e.stepper.launch_context(rows, slots)
+        key = (rows, self.sampler.kind(self.e.model.plan.vocab_size), self.sampler.rule_kind(), shared, context)
         graphs = self.e._graphs
         g = graphs.pop(key, None)
         if g is None:
             if self.e._token_loop is None:
                 self.e._token_loop = TokenLoop(self.e.device)
             g = GraphedDecode(self.e.stepper, self.sampler, key[0], self.e._token_loop, shared,
-                              self.e.rule_memory() if self.sampler.params.ruled else None)
+                              self.e.rule_memory() if self.sampler.params.ruled else None, context)
             while len(graphs) >= self.MAX_GRAPHS:
                 graphs.pop(next(iter(graphs)))
         graphs[key] = g                                  # most recently used last

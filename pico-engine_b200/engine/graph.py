@@ -107,8 +107,9 @@ class GraphedPrompt:
     runs kernel by kernel at the same padded sizes, the second is captured: the kernels and their results are the same
     either way, so a call's tokens do not depend on whether its sizes have been seen before."""
 
-    def __init__(self, stepper: Stepper, B: int, T: int, pool=None):
+    def __init__(self, stepper: Stepper, B: int, T: int, pool=None, max_context: Optional[int] = None):
         self.stepper, self.B, self.T, self.pool = stepper, B, T, pool
+        self.max_context = max_context or stepper.max_context      # bounds every row's positions and fixes the launch shapes
         self.widths = [pages_for(stepper.max_context)] * len(stepper.cache.groups)
         self.n_tiles = (T // kernels.PREFILL_TILE + B, T // kernels.PREFILL_TILE_TCGEN05 + B)
         self.layout = StepLayout(T, B, B, self.widths, self.n_tiles)
@@ -141,10 +142,12 @@ class GraphedPrompt:
         lens = [len(t) for t in token_ids]
         pad = self.padding(len(slots), sum(lens), self.B, self.T)
         all_slots = list(slots) + [cache.idle_slot] * len(pad)
+        if self.max_context < st.max_context and max(cache.length(s) + n for s, n in zip(slots, lens)) > self.max_context:
+            raise ValueError(f"a captured step for up to {self.max_context} positions got a row that reaches further")
         _, host, starts = st.describe(all_slots, lens + pad, None, list(token_ids) + [[0] * n for n in pad], self.widths, self.n_tiles)
         st.upload(host, self.dev)
         ctx = st.context(lay, self.dev, lens + pad, starts, all_slots, prompts=True)
-        ctx.max_context = st.max_context                  # what the captured launches were shaped for
+        ctx.max_context = self.max_context                # what the captured launches were shaped for
         self.launches += 1
         if self.graph is None and not self.failed and self.launches >= 2:
             stream = torch.cuda.current_stream()
@@ -195,10 +198,11 @@ class GraphedDecode:
     are chosen (greedy, or which cuts a draw makes: that fixes the kernels of the graph); its temperature,
     top-k, top-p and seed are read from the device buffer at run time, so one graph serves every setting
     of the same kind (``launch(..., sampler=)``).  ``shared``: rows of a family of forked sequences read its pages once for
-    all.  A sampler with rules needs ``memory`` (``RuleMemory``), what its sequences have seen; their numbers are read from the buffer too."""
+    all.  ``max_context`` bounds the rows' positions (None: the longest context) and fixes the launch shapes.  A sampler with rules needs ``memory`` (``RuleMemory``), what its sequences have seen; their numbers are read from the buffer too."""
 
-    def __init__(self, stepper: Stepper, sampler, B: int, loop: Optional[TokenLoop] = None, shared: bool = False, memory=None):
+    def __init__(self, stepper: Stepper, sampler, B: int, loop: Optional[TokenLoop] = None, shared: bool = False, memory=None, max_context: Optional[int] = None):
         self.stepper, self.sampler, self.B, self.shared = stepper, sampler, B, shared
+        self.max_context = max_context or stepper.max_context
         cache = stepper.cache
         self.loop = loop or TokenLoop(stepper.device)
         if B > TokenLoop.ROWS:
@@ -253,6 +257,8 @@ class GraphedDecode:
         if (sampler or self.sampler).kind(self.stepper.vocab) != self.sampler.kind(self.stepper.vocab) or \
                 (sampler or self.sampler).rule_kind() != self.sampler.rule_kind():
             raise ValueError("this graph was captured for another kind of sampling")
+        if self.max_context < self.stepper.max_context and max(self.stepper.cache.length(s) for s in slots) >= self.max_context:
+            raise ValueError(f"a graph for up to {self.max_context} positions got a row that reaches further")
         idle = [self.stepper.cache.idle_slot] * (B - n)
         st, every = self.stepper, list(slots) + idle
         if self.tables is None:
@@ -308,8 +314,8 @@ class GraphedDecode:
     def _forward(self) -> None:
         lay, B, pad = self.layout, self.B, self.pad
         ctx = self.stepper.context(lay, self.dev, [1] * B, [0] * B, self._slots)
-        ctx.max_context = self.stepper.max_context       # launch shapes must not depend on the step
-        ctx.starts = [self.stepper.max_context - 1] * B
+        ctx.max_context = self.max_context               # launch shapes must not depend on the step
+        ctx.starts = [self.max_context - 1] * B
         ids = self.dev[lay.ids: lay.ids + B]
         if self.tables is not None:
             for g in range(len(self.widths)):

@@ -86,9 +86,10 @@ class Stepper:
         self._ring: List[list] = [[None, None] for _ in range(4)]     # pinned staging buffers and their copy events
         self._ring_at = 0
         self.h2d_bytes = 0                        # bytes of step descriptions copied to the device so far
-        self._prompt_graphs: dict = {}            # (rows, tokens) -> GraphedPrompt, the most recently used last
+        self._prompt_graphs: dict = {}            # (rows, tokens and, over 4-bit pages, bound of positions) -> GraphedPrompt, the most recently used last
         self._prompt_pool = None
         self._resident = None
+        self._launch_contexts: dict = {}          # (rows, positions) -> the bound of positions that a captured step of such rows states
 
     # ------------------------------------------------------------------ rows that share pages
     def families(self, slots: Sequence[int]):
@@ -121,6 +122,35 @@ class Stepper:
             a_position = 2 * (g.need.n_kv_heads * g.need.head_dim + heads * dim)
             most = max(most, sum((n - 1) * min(shared, g.need.window or shared) * a_position for n, shared, _ in members))
         return kernels.sharing_pays(most)
+
+    # ------------------------------------------------------------------ captured steps
+    def launch_context(self, rows: int, slots: Sequence[int]) -> int:
+        """The bound of positions that a captured step of ``rows`` rows states for one token more of each of these sequences.  Kernels over 4-bit pages go by it: the
+        largest power of two with which they are the same as with the next one to the longest sequence, so that a graph serves all contexts that its kernels suit.
+        (Without such pages: the longest context.)"""
+        if not any(g.int4 for g in self.cache.groups):
+            return self.max_context
+        positions, bound = max(self.cache.length(s) for s in slots) + 1, PAGE
+        while bound < positions:
+            bound *= 2
+        most = self._launch_contexts.get((rows, bound))
+        if most is None:
+            most = min(bound, self.max_context)
+            shapes = self.model.int4_shapes(rows, most, self.attend_pages)
+            while most < self.max_context and self.model.int4_shapes(rows, min(2 * most, self.max_context), self.attend_pages) == shapes:
+                most = min(2 * most, self.max_context)
+            self._launch_contexts[rows, bound] = most
+        return most
+
+    def prompt_context(self, n_tokens: int, slots: Sequence[int], lens: Sequence[int]) -> int:
+        """The same for a captured step of ``n_tokens`` tokens, idle ones among them, that brings these sequences ``lens`` tokens; it bounds their expanded pages too.  As many
+        positions as tokens, which prompts from their beginnings have at most, or a power of two times that."""
+        if not any(g.int4 for g in self.cache.groups):
+            return self.max_context
+        positions, bound = max(self.cache.length(s) + n for s, n in zip(slots, lens)), n_tokens
+        while bound < positions:
+            bound *= 2
+        return min(bound, self.max_context)
 
     # ------------------------------------------------------------------ building a step
     def _stage(self, host: np.ndarray):
@@ -285,20 +315,23 @@ class Stepper:
     MAX_PROMPT_GRAPHS = 8             # padded prompt steps a stepper keeps (captured ones share one memory pool)
     MAX_GRAPHED_PROMPT_TOKENS = 16384
 
-    def _prompt_graph(self, n_rows: int, n_tokens: int):
-        """The padded step that takes ``n_rows`` prompts of ``n_tokens`` tokens.  It is captured as a graph once
+    def _prompt_graph(self, slots: Sequence[int], lens: Sequence[int]):
+        """The padded step that takes prompts of ``lens`` tokens for these sequences.  It is captured as a graph once
         steps of its sizes have come twice (a capture costs two more runs of the step; sizes that never come back
         are not worth one); until then it runs kernel by kernel, at the same padded sizes and so with the same
         kernels and results as the replays that follow."""
         from .graph import GraphedPrompt, prompt_sizes
-        key = prompt_sizes(n_rows, n_tokens)
+        key = prompt_sizes(len(slots), sum(lens))
+        context = self.prompt_context(key[1], slots, lens)
+        if context != self.max_context:
+            key += (context,)
         if key[1] > self.MAX_GRAPHED_PROMPT_TOKENS or self.device.type != "cuda":
             return None
         g = self._prompt_graphs.pop(key, None)
         if g is None:
             if self._prompt_pool is None:
                 self._prompt_pool = torch.cuda.graph_pool_handle()
-            g = GraphedPrompt(self, key[0], key[1], self._prompt_pool)
+            g = GraphedPrompt(self, key[0], key[1], self._prompt_pool, context)
             while len(self._prompt_graphs) >= self.MAX_PROMPT_GRAPHS:
                 self._prompt_graphs.pop(next(iter(self._prompt_graphs)))
         self._prompt_graphs[key] = g
@@ -316,7 +349,7 @@ class Stepper:
         tokens are prompts or pieces of them, which attend to everything, also where each row brings one token; a step
         of one token a row is one of decoded tokens otherwise, one in which a row brings several is one of prompts."""
         if use_graph and want is None and device_tokens is None and any(len(t) != 1 for t in token_ids):
-            g = self._prompt_graph(len(slots), sum(len(t) for t in token_ids))
+            g = self._prompt_graph(slots, [len(t) for t in token_ids])
             if g is not None:
                 return g.launch(slots, token_ids)
         if device_tokens is not None:

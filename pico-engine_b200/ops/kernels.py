@@ -2251,6 +2251,18 @@ def load_int4(pool: torch.Tensor, n_kv: int, head_dim: int, tok_pos: torch.Tenso
     return keys, values
 
 
+def _int4_positions(max_context: int, window: int) -> int:
+    """What bounds the positions that a call of single tokens reads: those of as many pages as a window can lie on."""
+    return min(max_context, (window + PAGE - 2) // PAGE * PAGE + PAGE if window else max_context, _MOST_POSITIONS)
+
+
+@lru_cache(maxsize=4096)
+def int4_form(T: int, n_heads: int, n_kv_heads: int, head_dim: int, max_context: int, window: Optional[int]) -> int:
+    """Which of its forms ``attention_int4`` takes for T tokens of positions up to ``max_context``."""
+    window = min(window or 0, _MOST_POSITIONS)
+    return long_context().pe_attention_int4_form(T, n_heads, n_kv_heads, head_dim, _int4_positions(max_context, window), 0, window)
+
+
 @lru_cache(maxsize=4096)
 def _int4_scratch_bytes(T: int, n_heads: int, n_kv_heads: int, head_dim: int, max_context: int, selected: int, window: int) -> int:
     return long_context().pe_attention_int4_scratch(T, n_heads, n_kv_heads, head_dim, max_context, selected, window)
@@ -2289,12 +2301,9 @@ def attention_int4(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int
     else:
         _here(device, (out, "out", torch.bfloat16, (T, width)))
     window = min(window or 0, _MOST_POSITIONS)
-    if window:
-        max_context = min(max_context, (window + PAGE - 2) // PAGE * PAGE + PAGE)         # (positions of as many pages as a window can lie on)
-    max_context = min(max_context, _MOST_POSITIONS)
     if T:
-        _attend_int4(q_at, q_stride, out, pool, pool_at, pages, table_at, table_stride, rows, pos_at, row_at, T, n_heads, n_kv_heads, head_dim, window, scale, max_context, 0,
-                     1 if early_pages else 0, device, "attention_int4")
+        _attend_int4(q_at, q_stride, out, pool, pool_at, pages, table_at, table_stride, rows, pos_at, row_at, T, n_heads, n_kv_heads, head_dim, window, scale,
+                     _int4_positions(max_context, window), 0, 1 if early_pages else 0, device, "attention_int4")
     return out
 
 

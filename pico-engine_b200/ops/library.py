@@ -305,7 +305,7 @@ def long_context() -> ctypes.CDLL:
         lib = build.load("long", LONG_SOURCES)
         declare(lib, _LONG_SIGNATURES)
         lib.pe_set_pdl(0 if os.environ.get("PICO_ENGINE_PDL", "1") == "0" else 1)
-        lib.pe_attention_int4_scratch.argtypes = [I, I, I, I, I, I, I]
+        lib.pe_attention_int4_scratch.argtypes = lib.pe_attention_int4_form.argtypes = [I, I, I, I, I, I, I]
         lib.pe_attention_int4_scratch.restype = c_longlong
         _long = lib
     return _long

@@ -69,6 +69,17 @@ class GQAAttention(Mixer):
         return CacheNeeds(kv=KVNeed(s.n_kv_heads, s.head_dim, s.window, may_be_int4=type(self.position) in (RotaryHalf, NoPosition) and s.scale > 0 and
                                     kernels.int4_takes(self.dtype, s.n_heads, s.n_kv_heads, s.head_dim)))
 
+    def _selects(self, max_context, attend_pages) -> bool:
+        return attend_pages is not None and self.spec.window is None and max_context > attend_pages * kernels.PAGE
+
+    def int4_shape(self, rows, max_context, attend_pages):
+        s = self.spec
+        if not self.cache_needs().kv.may_be_int4:
+            return None
+        if self._selects(max_context, attend_pages):
+            return "selected", max_context > kernels.SELECT_ONE_PAGES * kernels.PAGE
+        return kernels.int4_form(rows, s.n_heads, s.n_kv_heads, s.head_dim, max_context, s.window)
+
     def _attend_int4(self, qkv, ctx, kv, owns_cache):
         """The same from the products' rows on, over a cache of 4 bits."""
         s = self.spec
@@ -87,7 +98,7 @@ class GQAAttention(Mixer):
             if tiles is None:
                 tiles = ctx.scratch["prefill_tiles_128"] = kernels.prefill_tiles(ctx.lens, ctx.starts, q.device, kernels.PREFILL_TILE_TCGEN05)
             return kernels.attention_int4_prompt(*heads, kv.k, *place, tiles, ctx.T, s.window, s.scale, max_context=ctx.max_context)
-        if kv.bounds is not None and ctx.attend_pages is not None and ctx.max_context > ctx.attend_pages * kernels.PAGE:
+        if kv.bounds is not None and self._selects(ctx.max_context, ctx.attend_pages):
             pages = kernels.select_pages(*heads, kv.bounds, *place, ctx.tok_pos, ctx.tok_row, ctx.attend_pages, ctx.max_context)
             return kernels.attention_int4_selected(*heads, kv.k, pages, s.scale)
         return kernels.attention_int4(*heads, kv.k, *place, ctx.tok_pos, ctx.tok_row, s.window, s.scale, ctx.max_context, early_pages=owns_cache)

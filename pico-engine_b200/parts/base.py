@@ -248,6 +248,10 @@ class Mixer(Part):
     def cache_needs(self) -> CacheNeeds:
         return CacheNeeds()
 
+    def int4_shape(self, rows: int, max_context: int, attend_pages: Optional[int]):
+        """What decides the kernels of a step of one token for each of so many rows on a 4-bit cache, beside its sizes; None where nothing does."""
+        return None
+
     def apply(self, h: torch.Tensor, ctx: StepContext, entry: int, cache_entry: int, owns_cache: bool) -> torch.Tensor:
         raise NotImplementedError
 

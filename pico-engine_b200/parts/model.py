@@ -80,6 +80,10 @@ class DecoderModel:
             needs.append(CacheNeeds(state_elems=1, state_dtype="int32"))
         return needs
 
+    def int4_shapes(self, rows: int, max_context: int, attend_pages: Optional[int]) -> tuple:
+        """``Mixer.int4_shape`` of every layer."""
+        return tuple(layer.mixer.int4_shape(rows, max_context, attend_pages) for layer in self.layers if layer.mixer is not None)
+
     # ------------------------------------------------------------------ a step
     def hidden(self, token_ids: torch.Tensor, ctx: StepContext) -> torch.Tensor:
         """The residual stream (the sum of the streams, where there are several) [T, hidden] float32 after the last layer."""

@@ -276,3 +276,52 @@ def test_selection_without_a_layer_that_selects_is_refused(tmp_path):
     Engine(path, cache="int4")
     with pytest.raises(ValueError, match="attend_pages"):
         Engine(path, cache="int4", attend_pages=4)
+
+
+@pytest.mark.parametrize("attend", [None, 4])
+def test_captured_steps_go_by_the_rows_they_have(folder, attend):
+    """An engine set up for long contexts launches for the ones it has: no selection before a row has more pages than are kept, prompts with scratch for their own positions; and the
+    results are those of steps that are not captured, across the borders."""
+    from pico_engine import Engine
+    from test_int4_engine_gpu import prompts
+    path, cfg = folder
+    eng = Engine(path, cache="int4", attend_pages=attend, max_context=2000)
+    texts = prompts(cfg, [230, 30, 100])
+    got = [eng.generate(texts, max_tokens=60, temperature=0.0, stop_token_ids=()) for _ in range(3)]
+    contexts = {key[4] for key in eng._graphs}
+    # (four rows of two key heads are few pairs, whose kernel changes at 15 pages: 512 positions have it as they do, 1,024 do not)
+    assert contexts == ({512} if attend is None else {256, 2000}) and all(g.graph is not None for g in eng._graphs.values())
+    assert {(key[1], key[2]) for key in eng.stepper._prompt_graphs} == {(384, 384)} and all(g.graph is not None for g in eng.stepper._prompt_graphs.values())
+    plainly = eng.generate(texts, max_tokens=60, temperature=0.0, stop_token_ids=(), use_graph=False)
+    assert got[0] == got[1] == got[2] == plainly
+    short = next(iter(eng._graphs.values()))
+    if attend is not None and short.max_context == 256:
+        slot = eng.cache.open()
+        eng.stepper.step([slot], [[1] * 256])
+        with pytest.raises(ValueError, match="reaches further"):
+            short.launch([slot], [1], [0], [1])
+        eng.cache.close(slot)
+    eng.cache.check()
+
+
+def test_the_bound_of_a_captured_steps_positions(K):
+    """The largest power of two whose kernels are those of the rows at hand."""
+    from types import SimpleNamespace
+    from pico_engine.cache import Cache
+    from pico_engine.engine.step import Stepper
+    from test_int4_engine_gpu import part_of
+    part = part_of(14, 2, 64, None, True)
+    cache = Cache([part.cache_needs()], 64 * 1200, 4, torch.bfloat16, "cuda", int4=True, bounds=True)
+    model = SimpleNamespace(plan=SimpleNamespace(vocab_size=1 << 20), dtype=torch.bfloat16, int4_shapes=lambda *a: (part.int4_shape(*a),))
+    slot = cache.open()
+    for attend, rows, length, want in ((None, 64, 999, 16384), (None, 64, 16384, 32768), (None, 1, 500, 512), (None, 1, 3000, 32768), (None, 32, 1000, 32768), (64, 64, 1000, 4096),
+                                       (64, 64, 4096, 32768), (64, 64, 4095, 4096)):
+        stepper = Stepper(model, cache, 32768, attend)
+        cache.lengths[slot] = length
+        assert stepper.launch_context(rows, [slot]) == want, (attend, rows, length)
+    cache.lengths[slot] = 0
+    stepper = Stepper(model, cache, 32768, None)
+    for tokens, start, n, want in ((128, 0, 100, 128), (2048, 0, 2000, 2048), (512, 9000, 400, 16384), (512, 0, 33, 512)):
+        cache.lengths[slot] = start
+        assert stepper.prompt_context(tokens, [slot], [n]) == want
+    cache.lengths[slot] = 0
