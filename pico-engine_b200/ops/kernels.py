@@ -2132,6 +2132,7 @@ INT4_HEAD_DIMS = (64, 128)
 INT4_GROUP = 32               # channels that share a step and a middle
 SELECT_ONE_PAGES = 1024       # PS_ONE_PAGES of csrc/page_select.cu
 _MOST_POSITIONS = 2 ** 31 - 1 # what the kernels hold a position in
+_MOST_SCALE = 2.0 ** 60       # (queries and codes are multiplied in units of 2^-65, which the scale makes up for)
 
 
 def int4_takes(dtype: torch.dtype, n_heads: int, n_kv_heads: int, head_dim: int) -> bool:
@@ -2195,6 +2196,11 @@ def _page_rows(block_table: torch.Tensor, table_stride: int) -> int:
 def _row_pages(pages: int) -> None:
     if pages > _MOST_POSITIONS // PAGE:
         raise KernelError(f"a row has at most {_MOST_POSITIONS // PAGE:,} pages, not {pages:,}")
+
+
+def _scaled(scale: float) -> None:
+    if not 0 < scale < _MOST_SCALE:
+        raise KernelError(f"scale must be positive and less than 2^60, not {scale}")
 
 
 def _query_rows(q: torch.Tensor, q_stride: int, T: int, width: int) -> None:
@@ -2286,16 +2292,17 @@ def attention_int4(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int
     stream may still run: they must have written, of the cache, no page but each token's own, and neither positions nor page tables.
 
     Scores are sums of exact products of the queries with codes, in float32; steps and middles join in float32 (sums of queries in 24 bits).  Weights are rounded to bfloat16 for the product with
-    the values, and once more behind their multiplication by a value's step.  Queries, keys and values of sizes between 2^-40 and 2^60 keep that: the products with codes are taken in units
-    of 2^-65.  A row that sees nothing is zeros; one that sees a group that is no number is none where that reaches."""
+    the values, and once more behind their multiplication by a value's step.  Queries, keys and values of sizes between 2^-40 and 2^60 keep that, where a query and a key
+    together have 2^-60 at least: the products with codes are taken in units of 2^-65.  ``scale`` is less than 2^60.  A row that sees nothing is zeros; one that sees a group that is no number is none where that reaches."""
     T, n_bytes, device, width = tok_pos.shape[0], _int4_heads(n_heads, n_kv_heads, head_dim), _device_here(q, "q"), n_heads * head_dim
     pages = pool.shape[0]
     q_at, pos_at, row_at, pool_at, table_at = _here(device, (q, "q", torch.bfloat16, None), (tok_pos, "tok_pos", torch.int32, (T,)), (tok_row, "tok_row", torch.int32, (T,)),
                                                     (pool, "pool", torch.uint8, (pages, n_kv_heads, n_bytes)), (block_table, "block_table", torch.int32, None))
     _query_rows(q, q_stride, T, width)
     rows = _page_rows(block_table, table_stride)
-    if max_context < 1 or (window is not None and window < 0) or not scale > 0:
-        raise KernelError("max_context and scale must be positive, and a window not negative")
+    _scaled(scale)
+    if max_context < 1 or (window is not None and window < 0):
+        raise KernelError("max_context must be positive, and a window not negative")
     if out is None:
         out = q.new_empty((T, width))
     else:
@@ -2321,8 +2328,9 @@ def attention_int4_prompt(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_hea
           (block_table, "block_table", torch.int32, None))
     _query_rows(q, q_stride, n_tokens, width)
     rows = _page_rows(block_table, table_stride)
-    if (window is not None and window < 0) or not scale > 0:
-        raise KernelError("scale must be positive, and a window not negative")
+    _scaled(scale)
+    if window is not None and window < 0:
+        raise KernelError("a window must not be negative")
     if max_context is not None and max_context < 1:
         raise KernelError("max_context must be positive")
     if rows > 18000:
@@ -2413,8 +2421,7 @@ def attention_int4_selected(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_h
                                             (pages.pos, "pages.pos", torch.int32, (T * n_kv_heads,)), (pages.table, "pages.table", torch.int32, (places, keep)))
     _query_rows(q, q_stride, T, width)
     _row_pages(keep)
-    if not scale > 0:
-        raise KernelError("scale must be positive")
+    _scaled(scale)
     if out is None:
         out = q.new_empty((T, width))
     else:

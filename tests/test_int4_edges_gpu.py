@@ -208,6 +208,30 @@ def test_calls_of_two_threads(K):
     assert not failed, failed[0]
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_scales_and_products_at_the_ends(K, D):
+    """Small queries against small keys under the largest scales, one token and prompts; scales that the kernels do not have are refused."""
+    from pico_engine.ops import KernelError
+    p = Paged(4, 2, D, [700, 90], 201)
+    pos, row = [699, 89], [0, 1]
+    p.pool = plain.pack((p.keys.double() * 2.0 ** -30).bfloat16().view(-1, 64, D), p.values.view(-1, 64, D)).view(p.n_pages, 2, -1)
+    p.scale *= 2.0 ** 60
+    q = (p.q.double() * 2.0 ** -30).bfloat16()
+    for bound in (700, 1 << 21):
+        p.check(p.attention(K, pos, row, q=q, bound=bound), pos, row, q=q)
+    long = (randn(90, 4 * D, seed=202).double() * 2.0 ** -30).bfloat16()
+    got = K.attention_int4_prompt(long, 4 * D, 4, 2, D, p.pool, p.table, p.width, K.prefill_tiles([0, 90], [0, 0], "cuda", K.PREFILL_TILE_TCGEN05), 90, None, p.scale)
+    some = [0, 40, 89]
+    p.check(got[some], some, [1] * 3, q=long[some], halves=True)
+    args = (q, q.shape[1], 4, 2, D, p.pool)
+    one = ints([3])
+    for scale in (0.0, -1.0, 2.0 ** 60, float("inf"), float("nan")):
+        for call in (lambda: K.attention_int4(*args, p.table, p.width, one, ints([0]), None, scale, 100), lambda: K.attention_int4_prompt(*args, p.table, p.width, ints([[0, 0, 1, 3]]), 1, None, scale),
+                     lambda: K.attention_int4_selected(*args, K.SelectedPages(ints([[0], [1]]), ints([3, 3])), scale)):
+            with pytest.raises(KernelError, match="scale must be positive and less than"):
+                call()
+
+
 # ---------------------------------------------------------------------------- tokens
 
 @pytest.mark.parametrize("H,G,D", [(6, 2, 64), (14, 1, 128)])
