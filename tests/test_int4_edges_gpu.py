@@ -262,6 +262,29 @@ def test_sums_of_queries_keep_the_bits_of_float32(K, H, G, D, bound):
             assert ((got[t, h] - w @ v[g]).abs() <= bound_of).all(), (t, h)
 
 
+@pytest.mark.parametrize("H,G,D", [(14, 2, 64), (28, 4, 128)])
+@pytest.mark.parametrize("window", [None, 300])
+@pytest.mark.parametrize("bound", [3100, 1 << 21])
+def test_pages_read_early_or_late_are_the_same(K, H, G, D, window, bound):
+    """``early_pages`` moves a wait, no result: behind an append of the tokens' own rows, one that ends a page and one that begins one among them."""
+    lengths = [64 * 40 + 1, 64 * 7, 1, 3000, 65] * (1 if bound == 3100 else 30)
+    p = Paged(H, G, D, lengths, 161)
+    T = len(lengths)
+    pos, row = ints([n - 1 for n in lengths]), ints(list(range(T)))
+    cos, sin = (randn(4000, D // 2, seed=s) for s in (1, 2))
+    for seed in range(6):
+        x, outs, pools = randn(T, (H + 2 * G) * D, seed=163 + seed).bfloat16(), [], []
+        for early in (True, False):
+            pool = p.pool.clone()
+            torch.cuda.synchronize()
+            q = K.store_int4(x, H, G, D, cos, sin, pos, row, pool, p.table, p.width)
+            outs.append(K.attention_int4(q, H * D, H, G, D, pool, p.table, p.width, pos, row, window, p.scale, bound, early_pages=early))
+            pools.append(pool)
+        assert torch.equal(*outs) and torch.equal(*pools)
+    p.pool, some = pools[0], list(range(0, T, 7))
+    p.check(outs[0][some], [lengths[i] - 1 for i in some], some, q=q[some], window=window)
+
+
 # ---------------------------------------------------------------------------- the part and the engine
 
 @pytest.fixture(scope="module")
@@ -349,3 +372,43 @@ def test_the_bound_of_a_captured_steps_positions(K):
         cache.lengths[slot] = start
         assert stepper.prompt_context(tokens, [slot], [n]) == want
     cache.lengths[slot] = 0
+
+
+@pytest.mark.parametrize("nh,nkv,hd,keep", [(14, 2, 64, None), (8, 2, 128, 3)])
+def test_a_part_that_reads_another_ones_cache(nh, nkv, hd, keep):
+    """Keys and values are the owner's; the reader turns its own queries and stores nothing."""
+    from types import SimpleNamespace
+    from pico_engine.cache import Cache
+    from pico_engine.engine.step import Stepper
+    from pico_engine.ops import linear
+    from test_int4_engine_gpu import part_of, rows_of
+    owner, reader = part_of(nh, nkv, hd, None, True), part_of(nh, nkv, hd, None, True)
+    reader.w_qkv.copy_(reader.w_qkv.flip(1))
+    cache = Cache([owner.cache_needs()], 64 * 20, 2, torch.bfloat16, "cuda", int4=True, bounds=keep is not None)
+    stepper = Stepper(SimpleNamespace(plan=SimpleNamespace(vocab_size=1 << 20), dtype=torch.bfloat16), cache, 1024, keep)
+    slots = [cache.open() for _ in range(2)]
+    keys, values = ([torch.zeros(0, nkv, hd, dtype=torch.float64, device="cuda") for _ in slots] for _ in range(2))
+    for step, lens in enumerate([[300, 70], [1, 1], [1, 1]]):
+        lay, host, starts = stepper.describe(slots, lens, None, None)
+        ctx = stepper.context(lay, stepper.upload(host), lens, starts, slots)
+        h = torch.randn(sum(lens), 96, generator=gen(step), device="cuda").bfloat16()
+        owner._attend(h, ctx, 0, True)
+        held, ends = cache.groups[0].k.clone(), None if keep is None else cache.groups[0].bounds.clone()
+        got = reader._attend(h, ctx, 0, False).double().view(-1, nh, hd)
+        assert torch.equal(held, cache.groups[0].k) and (keep is None or torch.equal(ends, cache.groups[0].bounds))
+        for s, n in zip(slots, lens):
+            cache.advance(s, n)
+        rows = [linear(h, part.w_qkv, part.b_qkv, out_dtype=torch.bfloat16).view(-1, nh + 2 * nkv, hd).double() for part in (owner, reader)]
+        at = 0
+        for b, (start, n) in enumerate(zip(starts, lens)):
+            c, s = (t.cuda().double()[start:start + n, None] for t in owner._tables(ctx))
+            turned = []
+            for x in rows:
+                lo, hi = x[at:at + n, :nh + nkv, :hd // 2], x[at:at + n, :nh + nkv, hd // 2:]
+                turned.append(torch.cat([lo * c - hi * s, lo * s + hi * c], -1).float().bfloat16())
+            keys[b] = torch.cat([keys[b], plain.stands_for(turned[0][:, nh:])])
+            values[b] = torch.cat([values[b], plain.stands_for(rows[0][at:at + n, nh + nkv:])])
+            for i in sorted({0, n // 2, n - 1}):
+                w, unit = rows_of(turned[1][i, :nh], keys[b][:start + i + 1], values[b][:start + i + 1], hd ** -0.5, None, keep if all(m == 1 for m in lens) else None)
+                assert (got[at + i] - w).abs().max() <= unit, (step, b, i)
+            at += n
