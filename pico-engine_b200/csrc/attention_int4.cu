@@ -13,10 +13,10 @@
 // that does nothing else (with copies by each warp for itself 1.03 us a block and SM partition, 0.82 so; three places a warp leave room for fewer warps, which is slower; keys and values
 // in copies of their own wait 0.4 us a page longer).  The warps' sums are joined in shared memory, those of a cluster's CTAs through distributed shared memory.
 //
-// What bounds it: instructions.  A block of 64 channels takes 618, 319 of them on the logic units (two a pair of codes), 40 on the tensor cores (a quarter of their time).  The same kernel with the arithmetic
+// What bounds it: a block's chain of instructions in few warps.  A block of 64 channels takes 618, 319 of them on the logic units (two a pair of codes), 40 on the tensor cores (a quarter of their time).  The same kernel with the arithmetic
 // taken out copies its blocks in 46 us where the whole takes 65.5 (64 rows of 20,000 to 32,700, 14 heads of 64 on 2: 266 MB, 41 us at the copy rate of 6.5 TB/s); 63 of 86 (200 rows of up to 6,000,
-// 28 heads of 128 on 4: 385 MB, 59 us).  Fifteen warps (eleven of 128 channels, 168 registers) are what registers allow: the schedulers issue in 58 of 100 cycles, the logic units are
-// busy for 57 of them, DRAM for 53 to 62.  One row of 4,096 positions takes 4.5 us: a launch, and one chain of positions, table, block, join.
+// 28 heads of 128 on 4: 385 MB, 59 us).  Fifteen warps (eleven of 128 channels, 168 registers) are what registers allow, and do not hide one another's waits: the schedulers issue in 58 of 100 cycles,
+// the logic units are busy for 57 of them, DRAM for 53 to 62.  One row of 4,096 positions takes 4.5 us: a launch, and one chain of positions, table, block, join.
 #include "int4_pages.cuh"
 #include <atomic>
 

@@ -3,7 +3,7 @@
 // A head's row of D channels (64 or 128) is cut into groups of 32 channels.  Of a group with largest and smallest number max and min (bfloat16)
 //   mid = (max + min) / 2, step = (max - min) / 15, both rounded to bfloat16;  level L = floor((x - mid) / step), between -8 and 7 (0 where step is 0)
 // and x is held as the 4 bits of L: it stands for mid + step * (L + 1/2).  5 bits a channel with step and mid.  A group with a number that is none
-// (an infinity, NaN, or a spread that bfloat16 does not hold) has step = mid = NaN.
+// (an infinity, NaN, or a sum or spread that float32 or bfloat16 does not hold) has step = mid = NaN.
 //
 // A block holds the 64 positions of one page and one head, 80 D bytes:
 //   [0, 32 D)     codes of the keys: position p, part t (4), group b: one word of the channels 32 b + 8 t + 2 i + e (i of 4, e of 2)

@@ -1,6 +1,7 @@
 // The pages of a long context that a token's heads can score highest.
 //
-// A page j holds keys between lo_j and hi_j, channel by channel (page_bounds).  No key of it scores more against a query q than sum_d max(q_d lo_jd, q_d hi_jd), which is
+// A page j holds keys between lo_j and hi_j, channel by channel (page_bounds).  But for their rounding to bfloat16 (2^-9 of them), no key of it scores more against a query q than
+// sum_d max(q_d lo_jd, q_d hi_jd), which is
 // sum_d max(q_d, 0) hi_jd + min(q_d, 0) lo_jd.  The heads that share a key head read the same pages, so their bounds are added up: one vector of the sums of the positive
 // parts and one of the negative parts against the page's two rows, 2 D multiply-adds a page whatever the number of heads.  Which pages are
 // kept is defined by the sums in float64; a bound that is no number counts as the largest.

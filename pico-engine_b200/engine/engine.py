@@ -43,8 +43,10 @@ class Engine:
     The cache is allocated on first use and grows when a call needs more.
 
     ``cache`` "int4" holds the keys and values of layers whose attention takes it (bfloat16, head sizes 64 and 128) in 4 bits, 5 with the steps and middles of
-    32 channels each, for 16: three times the context in the same memory, read three times as fast.  ``attend_pages``: with it, a decoded token attends, in layers without a window, to so
-    many pages of 64 positions at most: its own, the sequence's first, and those whose keys can score highest by their bounds; prompts attend to everything.
+    32 channels each, for 16: three times the context in the same memory, a third of the bytes to read.  (Steps of many rows on long contexts have 1.4 to 1.6 times the tokens a second for
+    it; one conversation of a small model has 7 % fewer, its step being a chain of small kernels of which there are more.)  ``attend_pages``: with it, a decoded token attends, in layers
+    without a window, to so many pages of 64 positions at most: its own, the sequence's first, and those whose keys can score highest by their bounds; prompts attend to everything, however
+    they are cut into steps.
     """
 
     def __init__(self, model_path: Union[str, os.PathLike, None], device: str = "cuda", dtype="bfloat16",

@@ -2215,7 +2215,7 @@ def store_int4(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, cos: Optio
 
     A group of 32 channels of a row is held as 32 codes c of 0 to 15, a step and a middle in bfloat16, mid = (max + min) / 2, step = (max - min) / 15: c = floor((x - mid) / step) + 8
     within its bounds, and stands for mid + step * (c - 7.5): at most half a step from x, but for the roundings of step and middle.  A group whose numbers are equal is held as it is; one with an
-    infinity or NaN is NaN as a whole.  Keys are turned as in float64 and rounded to bfloat16 before they are coded.
+    infinity or NaN, or whose max + min or max - min float32 does not hold, is NaN as a whole.  Keys are turned as in float64 and rounded to bfloat16 before they are coded.
 
     Tokens of a sequence stand behind one another in the call, in the order of their positions (which may leave some out), and no position twice; tokens whose page is not there (-1) are not
     stored."""
@@ -2288,8 +2288,9 @@ def attention_int4(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int
                    tok_pos: torch.Tensor, tok_row: torch.Tensor, window: Optional[int], scale: float, max_context: int, out: Optional[torch.Tensor] = None,
                    early_pages: bool = False) -> torch.Tensor:
     """``attention_decode`` over a 4-bit cache: T tokens (bfloat16), each at position ``tok_pos`` of row ``tok_row`` of the page table, see the positions up to their own (the last
-    ``window`` of them).  ``max_context`` bounds every token's position + 1 and fixes the launch shape.  With ``early_pages`` the kernel copies pages while the two kernels before it on the
-    stream may still run: they must have written, of the cache, no page but each token's own, and neither positions nor page tables.
+    ``window`` of them).  ``max_context`` bounds every token's position + 1 and fixes the launch shape.  With ``early_pages`` the kernel copies pages while kernels before it on the
+    stream may still run, back to the last one that did not let its successor start early: they must have written, of the cache, no page but each token's own, and neither positions nor page
+    tables.
 
     Scores are sums of exact products of the queries with codes, in float32; steps and middles join in float32 (sums of queries in 24 bits).  Weights are rounded to bfloat16 for the product with
     the values, and once more behind their multiplication by a value's step.  Queries, keys and values of sizes between 2^-40 and 2^60 keep that, where a query and a key
@@ -2387,7 +2388,7 @@ class SelectedPages:
 def select_pages(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_heads: int, head_dim: int, bounds: torch.Tensor, block_table: torch.Tensor, table_stride: int,
                  tok_pos: torch.Tensor, tok_row: torch.Tensor, keep: int, max_context: int) -> SelectedPages:
     """For every token and key/value head the ``keep`` pages to attend to: its own, the sequence's first (where ``keep`` is 2 or more), and those whose keys can score highest by
-    their ``bounds`` (``page_bounds``): the sum over the head's queries and over the channels of max(q * least, q * greatest), in float64; of equal ones the earlier page.  All pages, where a token sees
+    their ``bounds`` (``page_bounds``): the sum over the head's queries and over the channels of max(q * least, q * greatest), in float64; of equal ones the earlier page, and a bound that is NaN counts as the largest (bounds are finite or NaN).  All pages, where a token sees
     no more than ``keep``; none (and place -1) for a token in front of position 0 or of no row of the table.  ``max_context`` bounds every token's position + 1."""
     T = tok_pos.shape[0]
     _int4_heads(n_heads, n_kv_heads, head_dim)
