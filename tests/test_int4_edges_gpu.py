@@ -412,3 +412,74 @@ def test_a_part_that_reads_another_ones_cache(nh, nkv, hd, keep):
                 w, unit = rows_of(turned[1][i, :nh], keys[b][:start + i + 1], values[b][:start + i + 1], hd ** -0.5, None, keep if all(m == 1 for m in lens) else None)
                 assert (got[at + i] - w).abs().max() <= unit, (step, b, i)
             at += n
+
+
+@pytest.mark.parametrize("window,attend", [(False, None), (False, 3), (True, None)])
+def test_every_call_that_a_generation_makes(tmp_path, monkeypatch, K, window, attend):
+    """Prompts, tokens and selected pages of an engine, call by call: what is appended is what the codes of the call's own rows stand for, bit by bit, and attention is within its bounds of the plain
+    form over the pool's bytes.  (Logits of a whole model allow for more: a bfloat16 rounding in front of a code moves the code.)"""
+    from conftest import TINY_C, make_weights, write_model
+    from pico_engine import Engine
+    from test_int4_engine_gpu import LONG, prompts
+    cfg = TINY_C if window else LONG
+    eng = Engine(write_model(tmp_path / "model", cfg, make_weights(cfg, 9, sharp=True)), cache="int4", attend_pages=attend, max_context=512)
+    calls = {"store": 0, "prompt": 0, "token": 0, "selected": 0}
+    store, token, prompt, selected = K.store_int4, K.attention_int4, K.attention_int4_prompt, K.attention_int4_selected
+
+    def blocks_of(pool, table, row, n):
+        return pool[table[row, :n].clamp(min=0).long()]
+
+    def rows_checked(got, q, H, G, D, pool, table, pos, row, window, scale, halves):
+        for i in sorted({0, len(pos) // 3, len(pos) - 1}):
+            n, j = pos[i] // PAGE + 1, torch.arange((pos[i] // PAGE + 1) * PAGE, device="cuda")
+            seen = (j <= pos[i]) & ((j > pos[i] - window) if window else (j >= 0)) & (table[row[i], :n] >= 0).repeat_interleave(PAGE)
+            want, bound = plain.attend(q[i].view(H, D), blocks_of(pool, table, row[i], n), seen[None].expand(G, -1), scale, halves)
+            assert ((got[i].double().view(H, D) - want).abs() <= bound + 1e-30).all(), (pos[i], window)
+
+    def stored(qkv, H, G, D, cos, sin, pos, row, pool, table, width, out=None):
+        q = store(qkv, H, G, D, cos, sin, pos, row, pool, table, width, out)
+        x = qkv.view(-1, H + 2 * G, D).double()
+        c, s = (t.double()[pos.long()][:, None] for t in (cos, sin))
+        a, b = x[:, :H + G, :D // 2], x[:, :H + G, D // 2:]
+        turned = torch.cat([a * c - b * s, a * s + b * c], -1)
+        k, v = K.load_int4(pool, G, D, pos, row, table, width)
+        assert torch.equal(k.double(), plain.stands_for(turned[:, H:].float().bfloat16()).float().double()) and torch.equal(v.double(), plain.stands_for(x[:, H + G:]).float().double())
+        size = torch.cat([(a * c).abs() + (b * s).abs(), (a * s).abs() + (b * c).abs()], -1)[:, :H]
+        assert ((q.double().view(-1, H, D) - turned[:, :H]).abs() <= 2.0 ** -8 * turned[:, :H].abs() + 2.0 ** -22 * size + 1e-30).all()
+        calls["store"] += 1
+        return q
+
+    def tokens(q, stride, H, G, D, pool, table, width, pos, row, window, scale, most, out=None, early_pages=False):
+        got = token(q, stride, H, G, D, pool, table, width, pos, row, window, scale, most, out, early_pages)
+        rows_checked(got, q, H, G, D, pool, table, pos.tolist(), row.tolist(), window, scale, False)
+        calls["token"] += 1
+        return got
+
+    def prompted(q, stride, H, G, D, pool, table, width, tiles, n, window, scale, out=None, max_context=None):
+        got = prompt(q, stride, H, G, D, pool, table, width, tiles, n, window, scale, out, max_context)
+        where = {r[1] + i: (r[3] + i, r[0]) for r in tiles.tolist() for i in range(r[2])}
+        assert sorted(where) == list(range(n))
+        rows_checked(got, q, H, G, D, pool, table, [where[i][0] for i in range(n)], [where[i][1] for i in range(n)], window, scale, True)
+        calls["prompt"] += 1
+        return got
+
+    def chosen_pages(q, stride, H, G, D, pool, pages, scale, out=None):
+        got = selected(q, stride, H, G, D, pool, pages, scale, out)
+        for i in range(q.shape[0]):
+            for g in range(G):
+                ids, at = pages.table[i * G + g].tolist(), int(pages.pos[i * G + g])
+                ids = [x for x in ids if x >= 0]
+                assert len(ids) <= attend and at < len(ids) * PAGE
+                seen = torch.arange(len(ids) * PAGE, device="cuda") <= at
+                part = q[i].view(G, -1, D)[g]
+                want, bound = plain.attend(part, pool.flatten(0, 1)[ids][:, None], seen[None], scale)
+                assert ((got[i].double().view(G, -1, D)[g] - want).abs() <= bound + 1e-30).all()
+        calls["selected"] += 1
+        return got
+
+    for name, f in (("store_int4", stored), ("attention_int4", tokens), ("attention_int4_prompt", prompted), ("attention_int4_selected", chosen_pages)):
+        monkeypatch.setattr(K, name, f)
+    texts = prompts(cfg, [240, 30, 64, 129] if not window else [200, 30, 64, 129])
+    eng.prefill_tokens_per_step = 150
+    eng.generate(texts, max_tokens=20, temperature=0.0, stop_token_ids=(), use_graph=False)
+    assert calls["store"] > 20 and calls["prompt"] >= 3 and (calls["selected"] if attend else calls["token"]) >= 19
