@@ -133,6 +133,8 @@ class Stepper:
         positions, bound = max(self.cache.length(s) for s in slots) + 1, PAGE
         while bound < positions:
             bound *= 2
+        if self.attend_pages is not None and positions <= self.attend_pages * PAGE:
+            bound = min(bound, self.attend_pages * PAGE)      # (nothing to select from)
         most = self._launch_contexts.get((rows, bound))
         if most is None:
             most = min(bound, self.max_context)

@@ -362,7 +362,8 @@ def test_the_bound_of_a_captured_steps_positions(K):
     model = SimpleNamespace(plan=SimpleNamespace(vocab_size=1 << 20), dtype=torch.bfloat16, int4_shapes=lambda *a: (part.int4_shape(*a),))
     slot = cache.open()
     for attend, rows, length, want in ((None, 64, 999, 16384), (None, 64, 16384, 32768), (None, 1, 500, 512), (None, 1, 3000, 32768), (None, 32, 1000, 32768), (64, 64, 1000, 4096),
-                                       (64, 64, 4096, 32768), (64, 64, 4095, 4096)):
+                                       (64, 64, 4096, 32768), (64, 64, 4095, 4096), (100, 64, 5000, 6400), (100, 64, 6399, 6400),
+                                       (100, 64, 6400, 32768)):
         stepper = Stepper(model, cache, 32768, attend)
         cache.lengths[slot] = length
         assert stepper.launch_context(rows, [slot]) == want, (attend, rows, length)
