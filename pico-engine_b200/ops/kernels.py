@@ -2321,7 +2321,8 @@ def attention_int4_prompt(q: torch.Tensor, q_stride: int, n_heads: int, n_kv_hea
     """The same for runs of at most 128 tokens of a sequence, ``tiles`` int32 [n, 4] (``prefill_tiles`` with ``PREFILL_TILE_TCGEN05``), whose own keys and values the cache holds already;
     ``q`` has ``n_tokens`` rows.  ``max_context`` bounds every token's position + 1 (None: the page table does) and fixes the launch shape.  The pages that the runs see are expanded to 16 bits
     first (float16 numbers with a power of two for each page's keys and values), and the products, with weights in float16, run on the tensor cores.  The expanded pages are scratch of the call,
-    as large as in a 16-bit cache: a page for each of ``max_context`` and row of the table, or for each of the pool's where these are fewer.  A page table has at most 18,000 rows; a page that
+    as large as in a 16-bit cache: a page for each of ``max_context`` and row of the table, or for each of the pool's where these are fewer.  Of a page, numbers down to 2^-28 of its
+    largest keep 11 bits.  A page table has at most 18,000 rows; a page that
     several of them have stands at the same place of each.  A token that sees a key or value with a
     group that is no number has no number in the head's results."""
     n_bytes, device, width = _int4_heads(n_heads, n_kv_heads, head_dim), _device_here(q, "q"), n_heads * head_dim
